@@ -199,6 +199,10 @@ _SIGNATURES = {
                                _c_int, _c_int, _c_int, _c_int, _c_void_p],
     "bg_gemm_f32_nt_batched": [_c_void_p, _c_int, _c_ll, _c_void_p, _c_int, _c_ll, _c_void_p, _c_int, _c_ll, _c_int, _c_int,
                                _c_int, _c_int, _c_void_p, _c_void_p, _c_void_p],
+    "bg_adjust_logits": [_c_void_p, _c_ll, _c_void_p, _c_ll, _c_int, _c_int, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
+                         _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_int, _c_void_p, _c_void_p],
+    "bg_copy_pages_most": [],
+    "bg_copy_pages": [_c_void_p, _c_int, _c_ll, _c_int, _c_ll, _c_int, _c_int, _c_ll, _c_int, _c_void_p, _c_void_p, _c_int, _c_void_p],
     "bg_sample": [_c_void_p, _c_int, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p],
     "bg_sample_feed": [_c_void_p, _c_int, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
                        _c_void_p],
@@ -374,6 +378,21 @@ def _stream():
     if _raw_stream is not None:
         return _raw_stream(torch.cuda.current_device())
     return torch.cuda.current_stream().cuda_stream
+
+
+def _here(what: str, *tensors) -> None:
+    """All on the current device: a launch goes to the current device's stream."""
+    _cuda(*tensors)
+    now = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.device.index != now:
+            raise KernelError(f"{what}: a tensor on {t.device}, the current device is cuda:{now}")
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the memory from a's first element to its last meets that of b's."""
+    end = lambda t: t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+    return a.numel() > 0 and b.numel() > 0 and a.data_ptr() < end(b) and b.data_ptr() < end(a)
 
 
 def _i32(t: torch.Tensor, what: str) -> None:
@@ -1176,6 +1195,105 @@ def sample(logits: torch.Tensor, temperature: Optional[torch.Tensor], uniform: O
                                     _p(feed_positions), _p(advance), _stream()), "sample")
     global _launches
     _launches += 1            # two kernels
+
+
+def adjust_logits(logits: torch.Tensor, out: torch.Tensor, *, history: Optional[torch.Tensor] = None, lengths: Optional[torch.Tensor] = None,
+                  prompts: Optional[torch.Tensor] = None, newest: Optional[torch.Tensor] = None, repetition: Optional[torch.Tensor] = None,
+                  frequency: Optional[torch.Tensor] = None, presence: Optional[torch.Tensor] = None,
+                  bias: Optional[Tuple[torch.Tensor, torch.Tensor, torch.Tensor]] = None, allowed: Optional[torch.Tensor] = None,
+                  allowed_row: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None) -> None:
+    """out = what a token is chosen from: float32 logits [n, V] (rows may lie apart) under penalties, biases and masks; `out` may be `logits`.
+
+    `history` int32 [n, room] holds each request's tokens in order, `lengths` [n] of them, of which the first `prompts` [n] are the
+    prompt's (None: none are); `newest` [n] is one token more, which is also stored behind the others.  A token that occurs among them,
+    c times behind the prompt, has its logit x divided by `repetition` [n] where x > 0 and multiplied by it elsewhere, and then lowered by
+    `frequency` [n] times c and, where c > 0, by `presence` [n] (float32; None: 1, 0, 0).  `bias` = (tokens int32, values float32,
+    begins int32 [n + 1]): row r's biased tokens are tokens[begins[r] : begins[r + 1]], ascending (a token's values add up).  `allowed`
+    int32 [masks, words]: bit v % 32 of word v / 32 says whether token v may be chosen; the others become -inf.  Row r takes mask
+    `allowed_row`[r], -1: none (None: mask r).  Tokens outside [0, V), biased tokens out of order, a full history and masks that are
+    not there are passed over and recorded in `status`."""
+    if logits.dim() != 2 or logits.dtype != torch.float32 or out.dtype != torch.float32 or logits.shape != out.shape:
+        raise KernelError(f"adjust_logits: logits and out are float32 [n, V], got {logits.dtype} {tuple(logits.shape)} and {out.dtype} {tuple(out.shape)}")
+    n, V = logits.shape
+    if n == 0:
+        return
+    if V == 0 or any(V > 1 and t.stride(1) != 1 or n > 1 and t.stride(0) < V for t in (logits, out)):
+        raise KernelError("adjust_logits: rows of at least one logit, side by side and apart from one another")
+    same = out.data_ptr() == logits.data_ptr() and (n == 1 or out.stride(0) == logits.stride(0))
+    if not same and _overlap(logits, out):
+        raise KernelError("adjust_logits: out is logits itself, or memory apart from it")
+    if (history is None) != (lengths is None) or history is None and (newest is not None or prompts is not None):
+        raise KernelError("adjust_logits: a history goes with its lengths; prompts and newest go with a history")
+    if history is not None:
+        _i32(history, "adjust_logits: history")
+        if history.dim() != 2 or history.shape[0] != n or history.shape[1] == 0:
+            raise KernelError(f"adjust_logits: history is {tuple(history.shape)}, expected [{n}, room]")
+    for t, what in ((lengths, "lengths"), (prompts, "prompts"), (newest, "newest"), (allowed_row, "allowed_row")):
+        if t is not None:
+            _i32(t, f"adjust_logits: {what}")
+            if tuple(t.shape) != (n,):
+                raise KernelError(f"adjust_logits: {what} has one number per row, got {tuple(t.shape)} for {n} rows")
+    for t, what in ((repetition, "repetition"), (frequency, "frequency"), (presence, "presence")):
+        if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != (n,) or not t.is_contiguous()):
+            raise KernelError(f"adjust_logits: {what} is contiguous float32, one number per row")
+    if bias is not None:
+        ids, values, begins = bias
+        _i32(ids, "adjust_logits: biased tokens"); _i32(begins, "adjust_logits: begins of the biased tokens")
+        if values.dtype != torch.float32 or not values.is_contiguous() or values.shape != ids.shape or ids.dim() != 1 or tuple(begins.shape) != (n + 1,):
+            raise KernelError("adjust_logits: bias is (tokens int32 [k], values float32 [k], begins int32 [n + 1])")
+        if ids.numel() == 0:
+            bias = None
+    words = masks = 0
+    if allowed is not None:
+        _i32(allowed, "adjust_logits: allowed")
+        if allowed.dim() != 2 or allowed.shape[1] < -(-V // 32) or allowed.shape[0] < (1 if allowed_row is not None else n):
+            raise KernelError(f"adjust_logits: allowed is {tuple(allowed.shape)}, expected [masks, {-(-V // 32)}]" +
+                              ("" if allowed_row is not None else f" with a mask for each of {n} rows"))
+        masks, words = allowed.shape
+    elif allowed_row is not None:
+        raise KernelError("adjust_logits: allowed_row goes with masks")
+    ids, values, begins = bias or (None, None, None)
+    _here("adjust_logits", logits, out, history, lengths, prompts, newest, repetition, frequency, presence, ids, values, begins, allowed, allowed_row, status)
+    with phase("sample"):
+        _check(lib().bg_adjust_logits(_p(logits), logits.stride(0) if n > 1 else max(V, logits.stride(0)), _p(out), out.stride(0) if n > 1 else max(V, out.stride(0)),
+                                      n, V, _p(history), 0 if history is None else history.shape[1], _p(lengths), _p(prompts), _p(newest), _p(repetition),
+                                      _p(frequency), _p(presence), _p(ids), _p(values), _p(begins), _p(allowed), words, _p(allowed_row), masks, _p(status),
+                                      _stream()), "adjust_logits")
+
+
+def copy_pages(pool: torch.Tensor, src, dst, positions: int) -> None:
+    """pool[:, dst[i], ..., :positions, :] = pool[:, src[i], ..., :positions, :] for every i.  `pool` [stages, pages, ..., positions of a page, features]: a
+    page's numbers lie side by side, stages and pages may lie apart.  `src` and `dst` are sequences of page numbers on the host; a page is written once,
+    and none that is read."""
+    src, dst = [int(v) for v in src], [int(v) for v in dst]
+    if pool.dim() < 4 or any(n == 0 for n in pool.shape):
+        raise KernelError(f"copy_pages: pool is {tuple(pool.shape)}, expected [stages, pages, ..., positions, features]")
+    if not pool[0, 0].is_contiguous():
+        raise KernelError("copy_pages: the numbers of a page lie side by side")
+    stages, pages, rows = pool.shape[0], pool.shape[1], pool.shape[-2]
+    size, page = pool.element_size(), pool[0, 0].numel()
+    if stages > 1 and pool.stride(0) < page or pages > 1 and pool.stride(1) < page:
+        raise KernelError("copy_pages: pages that overlap")
+    if not 0 <= positions <= rows:
+        raise KernelError(f"copy_pages: {positions} positions of pages of {rows}")
+    if len(src) != len(dst):
+        raise KernelError(f"copy_pages: {len(src)} pages to read and {len(dst)} to write")
+    bad = [p for p in src + dst if not 0 <= p < pages]
+    if bad:
+        raise KernelError(f"copy_pages: page {bad[0]} outside the {pages} of the pool")
+    if len(set(dst)) != len(dst) or set(dst) & set(src):
+        raise KernelError("copy_pages: a page that is written twice, or read and written")
+    pairs = sorted(zip(src, dst))
+    _here("copy_pages", pool)
+    L = lib()
+    most = L.bg_copy_pages_most()
+    with phase("copy_pages"):
+        for i in range(0, len(pairs) if positions else 0, most):
+            part = pairs[i:i + most]
+            array = _c_int * len(part)
+            _check(L.bg_copy_pages(_p(pool), stages, pool.stride(0) * size if stages > 1 else page * size, pages, pool.stride(1) * size if pages > 1 else page * size,
+                                   page // (rows * pool.shape[-1]), rows, pool.shape[-1] * size, int(positions), array(*(s for s, _ in part)),
+                                   array(*(d for _, d in part)), len(part), _stream()), "copy_pages")
 
 
 # ------------------------------------------------------------------------------------------------
