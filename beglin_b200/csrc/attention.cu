@@ -23,6 +23,8 @@
 // With `slopes` [nh] the score of the key at position j falls by slopes[h] for every position that it lies behind the
 // query.  With `keep` k > 0 a window never loses the sequence's first k positions: a query at `pos` sees t <= pos with
 // t >= first_visible(pos, window) or t < k, the tiles and splits between the two ranges being passed over.
+#include <string.h>
+
 #include "common.cuh"
 #include "attention_f32.cuh"
 #include "attention_f32_tc.cuh"
@@ -59,9 +61,34 @@ struct AttnParams {
     unsigned* status;
 };
 
-template <typename TQ, typename TC>
+// Single tokens whose requests share their first positions: a block is either rows that share them, over splits of those, or one row over the
+// splits behind them (blocks and splits are thus those of every other call, and so is a row's result, bit for bit).
+struct AttnSharedParams : AttnParams {
+    // qblk is [n_qblk][8] = (request whose pages, first entry of `rows`, entries, first split, end of the splits, last position seen, 0, 0)
+    const int* rows;        // rows of the batch
+};
+
+// What a CTA takes: its block's request and rows, its split (nq 0: nothing), and the last position that the block's rows see.
+struct AttBlock { int req, row0, nq, sp, last; };
+__device__ __forceinline__ AttBlock att_block(const AttnParams& p, int qb) {
+    return {p.qblk[qb * 3 + 0], p.qblk[qb * 3 + 1], p.qblk[qb * 3 + 2], (int)blockIdx.z, 0x7fffffff};
+}
+__device__ __forceinline__ AttBlock att_block(const AttnSharedParams& p, int qb) {
+    const int4 a = *reinterpret_cast<const int4*>(p.qblk + qb * 8), b = *reinterpret_cast<const int4*>(p.qblk + qb * 8 + 4);
+    const int sp = a.w + (int)blockIdx.z;
+    return {a.x, a.y, sp < b.x ? a.z : 0, sp, b.y};
+}
+__device__ __forceinline__ int att_row(const AttnParams&, int i) { return i; }
+__device__ __forceinline__ int att_row(const AttnSharedParams& p, int i) { return p.rows[i]; }
+// the last position that any row of the block sees
+__device__ __forceinline__ int att_end(const AttnParams& p, const AttBlock& b) { return p.positions[b.row0 + b.nq - 1]; }
+__device__ __forceinline__ int att_end(const AttnSharedParams& p, const AttBlock& b) {
+    return b.nq > 1 ? b.last : min(p.positions[p.rows[b.row0]], b.last);
+}
+
+template <typename P, typename TQ, typename TC>
 __global__ void __launch_bounds__(ATT_THREADS)
-attention_partial_kernel(AttnParams p) {
+attention_partial_kernel(P p) {
     extern __shared__ float smem[];
     const int hd = p.hd, vd = p.vd, group = p.group;
     const int qhd = hd / p.maps;                         // features of a query
@@ -79,11 +106,12 @@ attention_partial_kernel(AttnParams p) {
 
     pdl_launch();
     pdl_wait();
-    const int qb = blockIdx.x, kvh = blockIdx.y, sp = blockIdx.z;
-    const int req = p.qblk[qb * 3 + 0], row0 = p.qblk[qb * 3 + 1], nq = p.qblk[qb * 3 + 2];
+    const int kvh = blockIdx.y;
+    const AttBlock blk = att_block(p, blockIdx.x);
+    const int req = blk.req, row0 = blk.row0, nq = blk.nq, sp = blk.sp;
     if (nq <= 0) return;
-    const int pos_first = p.positions[row0];
-    const int pos_last = p.positions[row0 + nq - 1];
+    const int pos_first = p.positions[att_row(p, row0)];
+    const int pos_last = att_end(p, blk);
     const int lo_first = first_visible(pos_first, p.window);
     const int k_first = sp * p.split;
     const int k_end = min((sp + 1) * p.split, pos_last + 1);       // exclusive
@@ -95,7 +123,7 @@ attention_partial_kernel(AttnParams p) {
     for (int idx = tid; idx < n_rows * qhd; idx += ATT_THREADS) {
         int r = idx / qhd, d = idx - r * qhd;
         int qi = r / group, g = r - qi * group;
-        q_s[idx] = to_float(q[(size_t)(row0 + qi) * p.q_stride + (size_t)(kvh * group + g) * qhd + d]);
+        q_s[idx] = to_float(q[(size_t)att_row(p, row0 + qi) * p.q_stride + (size_t)(kvh * group + g) * qhd + d]);
     }
     for (int idx = tid; idx < n_rows * vd; idx += ATT_THREADS) acc_s[idx] = 0.0f;
     for (int r = tid; r < n_rows; r += ATT_THREADS) { m_s[r] = -INFINITY; l_s[r] = 0.0f; }
@@ -139,7 +167,7 @@ attention_partial_kernel(AttnParams p) {
 
         for (int r = warp; r < n_rows; r += ATT_WARPS) {
             const int qi = r / group;
-            const int pos = p.positions[row0 + qi];
+            const int pos = min(p.positions[att_row(p, row0 + qi)], blk.last);
             const int lo = first_visible(pos, p.window);
             const float* qr = q_s + (size_t)r * qhd;
             const int map_off = (r % group) % p.maps * qhd;
@@ -208,10 +236,10 @@ attention_partial_kernel(AttnParams p) {
     // partial results, only for rows that see at least one key of this split
     for (int r = warp; r < n_rows; r += ATT_WARPS) {
         const int qi = r / group, g = r - qi * group;
-        const int pos = p.positions[row0 + qi];
+        const int pos = min(p.positions[att_row(p, row0 + qi)], blk.last);
         const int lo = first_visible(pos, p.window);
         if (pos < sp * p.split || (lo >= (sp + 1) * p.split && sp * p.split >= p.keep)) continue;
-        const size_t prow = ((size_t)(row0 + qi) * p.nh + (size_t)kvh * group + g) * p.max_splits + sp;
+        const size_t prow = ((size_t)att_row(p, row0 + qi) * p.nh + (size_t)kvh * group + g) * p.max_splits + sp;
         for (int d = lane; d < vd; d += 32) p.part_o[prow * vd + d] = acc_s[(size_t)r * vd + d];
         if (lane == 0) { p.part_ml[prow * 2 + 0] = m_s[r]; p.part_ml[prow * 2 + 1] = l_s[r]; }
     }
@@ -327,9 +355,10 @@ static bool attention_f32_takes(int rows, int hd, int vd, int maps) {
 
 // Whether the compiler gave attention_f32_tc_kernel the registers at launch that its split among the warpgroups counts on (else its calls go on
 // to the kernels of other sizes).
+template <typename P>
 static bool ax_fits() {
     static const bool fits = [] {
-        for (auto k : {attention_f32_tc_kernel<AttnParams, 64>, attention_f32_tc_kernel<AttnParams, 32>, attention_f32_tc_kernel<AttnParams, 0>}) {
+        for (auto k : {attention_f32_tc_kernel<P, 64>, attention_f32_tc_kernel<P, 32>, attention_f32_tc_kernel<P, 0>}) {
             cudaFuncAttributes a;
             if (cudaFuncGetAttributes(&a, k) != cudaSuccess || a.numRegs < AX_REGS) return false;
         }
@@ -354,27 +383,16 @@ extern "C" int bg_attention_plan(int group, int hd, int vd, int maps, int f32, i
     return BG_ERR_UNSUPPORTED;
 }
 
-extern "C" int bg_attention_partial(const void* q, int q_dtype, int q_stride, const void* kv_pool, int cache_dtype,
-                                    int num_pages, int page_size, const int* block_table, int max_pages,
-                                    const int* positions, const int* qblk, int n_qblk, float* part_o, float* part_ml,
-                                    int max_splits, int n_splits_launch, int nh, int nkv, int hd, int vd, int window, int split,
-                                    int tile, int bq, float scale, float softcap, int keep, const float* slopes, int maps,
-                                    unsigned* status, cudaStream_t stream) {
-    if (n_qblk <= 0 || n_splits_launch <= 0) return BG_OK;
-    if (maps < 1 || hd % maps || (nh / nkv) % maps) return BG_ERR_SHAPE;
-    if (nh % nkv != 0 || hd > 32 * ATT_MAX_DPL * maps || vd <= 0 || vd > 32 * ATT_MAX_DPL || (tile != 32 && tile != 64) || split % tile != 0) return BG_ERR_SHAPE;
-    if (n_splits_launch > max_splits || n_splits_launch > 65535 || nkv > 65535 || keep < 0) return BG_ERR_SHAPE;
-    AttnParams p;
-    p.q = q; p.q_stride = q_stride; p.kv_pool = kv_pool; p.num_pages = num_pages; p.page_size = page_size;
-    p.block_table = block_table; p.max_pages = max_pages; p.positions = positions; p.qblk = qblk;
-    p.part_o = part_o; p.part_ml = part_ml; p.max_splits = max_splits; p.nh = nh; p.nkv = nkv; p.hd = hd; p.vd = vd;
-    p.group = nh / nkv; p.window = window; p.split = split; p.tile = tile; p.bq = bq; p.scale = scale; p.softcap = softcap; p.status = status;
-    p.keep = keep; p.slopes = slopes; p.maps = maps;
-    dim3 grid(n_qblk, nkv, n_splits_launch);
-    const bool pieces = q_stride % 4 == 0 && (uintptr_t)q % 16 == 0 && (uintptr_t)kv_pool % 16 == 0 && (uintptr_t)part_o % 16 == 0;
-    if (q_dtype == BG_DTYPE_F32 && cache_dtype == BG_DTYPE_F32 && ax_takes(bq * p.group, hd, vd, maps) && split % AX_KEYS == 0 && pieces && ax_fits()) {
+// The partial results of n_qblk blocks over n_splits_launch splits, by the kernel that takes the sizes and types.
+template <typename P>
+static int attention_launch(P p, int q_dtype, int cache_dtype, int n_qblk, int n_splits_launch, cudaStream_t stream) {
+    const dim3 grid(n_qblk, p.nkv, n_splits_launch);
+    const int hd = p.hd, vd = p.vd, maps = p.maps, split = p.split, bq = p.bq;
+    int tile = p.tile;
+    const bool pieces = p.q_stride % 4 == 0 && (uintptr_t)p.q % 16 == 0 && (uintptr_t)p.kv_pool % 16 == 0 && (uintptr_t)p.part_o % 16 == 0;
+    if (q_dtype == BG_DTYPE_F32 && cache_dtype == BG_DTYPE_F32 && ax_takes(bq * p.group, hd, vd, maps) && split % AX_KEYS == 0 && pieces && ax_fits<P>()) {
         constexpr int need = 4 * AX_TILE + 1024;
-        auto kern = vd == 128 ? attention_f32_tc_kernel<AttnParams, 64> : vd == 64 ? attention_f32_tc_kernel<AttnParams, 32> : attention_f32_tc_kernel<AttnParams, 0>;
+        auto kern = vd == 128 ? attention_f32_tc_kernel<P, 64> : vd == 64 ? attention_f32_tc_kernel<P, 32> : attention_f32_tc_kernel<P, 0>;
         cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, need);
         if (e != cudaSuccess) return (int)e;
         launch(kern, grid, dim3(AX_THREADS), need, stream, p);
@@ -386,7 +404,7 @@ extern "C" int bg_attention_partial(const void* q, int q_dtype, int q_stride, co
         const size_t need = af_smem(hd / maps, hd, vd);
 #define BG_AF_LAUNCH(NC)                                                                                                    \
         do {                                                                                                                \
-            auto kern = maps == 1 && hd <= AF_NARROW ? attention_f32_kernel<AttnParams, NC, true> : attention_f32_kernel<AttnParams, NC, false>; \
+            auto kern = maps == 1 && hd <= AF_NARROW ? attention_f32_kernel<P, NC, true> : attention_f32_kernel<P, NC, false>; \
             cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)need);             \
             if (e != cudaSuccess) return (int)e;                                                                            \
             launch(kern, grid, dim3(AF_THREADS), need, stream, p);                                                          \
@@ -405,7 +423,7 @@ extern "C" int bg_attention_partial(const void* q, int q_dtype, int q_stride, co
     if (smem > 227 * 1024) return BG_ERR_UNSUPPORTED;
 #define BG_ATT_LAUNCH(TQ, TC)                                                                              \
     do {                                                                                                   \
-        auto kern = attention_partial_kernel<TQ, TC>;                                                      \
+        auto kern = attention_partial_kernel<P, TQ, TC>;                                                      \
         cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem); \
         if (e != cudaSuccess) return (int)e;                                                               \
         launch(kern, grid, dim3(ATT_THREADS), smem, stream, p);                                                      \
@@ -418,6 +436,43 @@ extern "C" int bg_attention_partial(const void* q, int q_dtype, int q_stride, co
 #undef BG_ATT_LAUNCH
     BG_LAUNCH_CHECK();
     return BG_OK;
+}
+
+extern "C" int bg_attention_partial(const void* q, int q_dtype, int q_stride, const void* kv_pool, int cache_dtype,
+                                    int num_pages, int page_size, const int* block_table, int max_pages,
+                                    const int* positions, const int* qblk, int n_qblk, float* part_o, float* part_ml,
+                                    int max_splits, int n_splits_launch, int nh, int nkv, int hd, int vd, int window, int split,
+                                    int tile, int bq, float scale, float softcap, int keep, const float* slopes, int maps,
+                                    unsigned* status, cudaStream_t stream) {
+    if (n_qblk <= 0 || n_splits_launch <= 0) return BG_OK;
+    if (maps < 1 || hd % maps || (nh / nkv) % maps) return BG_ERR_SHAPE;
+    if (nh % nkv != 0 || hd > 32 * ATT_MAX_DPL * maps || vd <= 0 || vd > 32 * ATT_MAX_DPL || (tile != 32 && tile != 64) || split % tile != 0) return BG_ERR_SHAPE;
+    if (n_splits_launch > max_splits || n_splits_launch > 65535 || nkv > 65535 || keep < 0) return BG_ERR_SHAPE;
+    AttnParams p;
+    p.q = q; p.q_stride = q_stride; p.kv_pool = kv_pool; p.num_pages = num_pages; p.page_size = page_size;
+    p.block_table = block_table; p.max_pages = max_pages; p.positions = positions; p.qblk = qblk;
+    p.part_o = part_o; p.part_ml = part_ml; p.max_splits = max_splits; p.nh = nh; p.nkv = nkv; p.hd = hd; p.vd = vd;
+    p.group = nh / nkv; p.window = window; p.split = split; p.tile = tile; p.bq = bq; p.scale = scale; p.softcap = softcap; p.status = status;
+    p.keep = keep; p.slopes = slopes; p.maps = maps;
+    return attention_launch(p, q_dtype, cache_dtype, n_qblk, n_splits_launch, stream);
+}
+
+// The same for single tokens whose requests share their first positions: qblk [n_qblk][8] and rows as AttnSharedParams says; a block of several rows
+// ends at its last position.  Partial results of split s at [row][head][s], as above.
+extern "C" int bg_attention_shared_partial(const void* q, int q_dtype, int q_stride, const void* kv_pool, int cache_dtype, int num_pages, int page_size,
+                                           const int* block_table, int max_pages, const int* positions, const int* qblk, int n_qblk, const int* rows,
+                                           float* part_o, float* part_ml, int max_splits, int n_splits_launch, int nh, int nkv, int hd, int vd, int split,
+                                           int tile, int bq, float scale, float softcap, unsigned* status, cudaStream_t stream) {
+    if (n_qblk <= 0 || n_splits_launch <= 0) return BG_OK;
+    if (nkv <= 0 || nh % nkv != 0 || hd <= 0 || hd > 32 * ATT_MAX_DPL || vd <= 0 || vd > 32 * ATT_MAX_DPL || (tile != 32 && tile != 64) || split <= 0 || split % tile != 0) return BG_ERR_SHAPE;
+    if (n_splits_launch > max_splits || n_splits_launch > 65535 || nkv > 65535 || bq <= 0 || (uintptr_t)qblk % 16) return BG_ERR_SHAPE;
+    AttnSharedParams p;
+    memset(&p, 0, sizeof(p));
+    p.q = q; p.q_stride = q_stride; p.kv_pool = kv_pool; p.num_pages = num_pages; p.page_size = page_size;
+    p.block_table = block_table; p.max_pages = max_pages; p.positions = positions; p.qblk = qblk;
+    p.part_o = part_o; p.part_ml = part_ml; p.max_splits = max_splits; p.nh = nh; p.nkv = nkv; p.hd = hd; p.vd = vd;
+    p.group = nh / nkv; p.split = split; p.tile = tile; p.bq = bq; p.scale = scale; p.softcap = softcap; p.status = status; p.maps = 1; p.rows = rows;
+    return attention_launch(p, q_dtype, cache_dtype, n_qblk, n_splits_launch, stream);
 }
 
 // The same for at most NS (8 or 16) splits and head_dim <= 128 (decoding): the maxima and sums and the partial outputs

@@ -51,7 +51,7 @@ template <bool V> struct AfAsk { static constexpr bool value = V; };
 
 template <typename P, int RI, int NC, bool NARROW>
 __device__ __forceinline__ void af_walk(const P& p, const AfShared& s, int req, int row0, int kvh, int sp, int n_rows,
-                                        int k_first, int k_end, int lo_first) {
+                                        int k_first, int k_end, int lo_first, int last) {
     const int tid = threadIdx.x, lane = tid & 31, ty = (tid >> 5) * 2 + (lane >> 4), tx = lane & 15;
     const int hd = p.hd, vd = p.vd, group = p.group, qhd = hd / p.maps;
     const float* pool = (const float*)p.kv_pool;
@@ -64,7 +64,7 @@ __device__ __forceinline__ void af_walk(const P& p, const AfShared& s, int req, 
 #pragma unroll
     for (int i = 0; i < RI; ++i) {
         const int r = ty + 16 * i, rr = r < n_rows ? r : 0;
-        pos[i] = r < n_rows ? p.positions[row0 + rr / group] : -1;       // (a row that is not there sees no key)
+        pos[i] = r < n_rows ? min(p.positions[att_row(p, row0 + rr / group)], last) : -1;       // (a row that is not there sees no key)
         lo[i] = first_visible(pos[i] < 0 ? 0 : pos[i], p.window);
         qc[i] = (rr % group) % p.maps * qhd / 4;
         slope[i] = p.slopes ? p.slopes[kvh * group + rr % group] : 0.0f;
@@ -265,7 +265,7 @@ __device__ __forceinline__ void af_walk(const P& p, const AfShared& s, int req, 
     for (int i = 0; i < RI; ++i) {
         const int r = ty + 16 * i;
         if (r >= n_rows || pos[i] < sp * p.split || (lo[i] >= (sp + 1) * p.split && sp * p.split >= p.keep)) continue;
-        const size_t prow = ((size_t)(row0 + r / group) * p.nh + (size_t)kvh * group + r % group) * p.max_splits + sp;
+        const size_t prow = ((size_t)att_row(p, row0 + r / group) * p.nh + (size_t)kvh * group + r % group) * p.max_splits + sp;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             const int d = tx * 4 + c * 64;
@@ -281,11 +281,12 @@ __global__ void __launch_bounds__(AF_THREADS, NC <= 2 ? 2 : 1) attention_f32_ker
     extern __shared__ __align__(16) float af_s[];
     pdl_launch();
     pdl_wait();
-    const int qb = blockIdx.x, kvh = blockIdx.y, sp = blockIdx.z;
-    const int req = p.qblk[qb * 3 + 0], row0 = p.qblk[qb * 3 + 1], nq = p.qblk[qb * 3 + 2];
+    const int kvh = blockIdx.y;
+    const auto blk = att_block(p, blockIdx.x);
+    const int req = blk.req, row0 = blk.row0, nq = blk.nq, sp = blk.sp;
     if (nq <= 0) return;
-    const int lo_first = first_visible(p.positions[row0], p.window);
-    const int k_first = sp * p.split, k_end = min((sp + 1) * p.split, p.positions[row0 + nq - 1] + 1);       // exclusive
+    const int lo_first = first_visible(p.positions[att_row(p, row0)], p.window);
+    const int k_first = sp * p.split, k_end = min((sp + 1) * p.split, att_end(p, blk) + 1);       // exclusive
     if (k_first >= k_end || (lo_first >= k_end && k_first >= p.keep)) return;      // no key of the split is seen
     const int qhd = p.hd / p.maps, n_rows = nq * p.group;
     AfShared s;
@@ -297,16 +298,16 @@ __global__ void __launch_bounds__(AF_THREADS, NC <= 2 ? 2 : 1) attention_f32_ker
     for (int idx = threadIdx.x; idx < rows16 * n4; idx += AF_THREADS) {
         const int r = idx / n4, c = idx - r * n4, qi = r / p.group, g = r - qi * p.group;
         const bool in = r < n_rows;
-        const float* src = (const float*)p.q + (in ? (size_t)(row0 + qi) * p.q_stride + (size_t)(kvh * p.group + g) * qhd + c * 4 : 0);
+        const float* src = (const float*)p.q + (in ? (size_t)att_row(p, row0 + qi) * p.q_stride + (size_t)(kvh * p.group + g) * qhd + c * 4 : 0);
         async_copy<16>(s.q + r * s.qld + c * 4, src, in);
     }
     async_commit();                           // (complete when the first keys are)
     if (s.vld > p.vd)
         for (int idx = threadIdx.x; idx < AF_KEYS * (s.vld - p.vd); idx += AF_THREADS)
             s.v[idx / (s.vld - p.vd) * s.vld + p.vd + idx % (s.vld - p.vd)] = 0.0f;
-    if (n_rows <= 16) af_walk<P, 1, NC, NARROW>(p, s, req, row0, kvh, sp, n_rows, k_first, k_end, lo_first);
-    else if (n_rows <= 32) af_walk<P, 2, NC, NARROW>(p, s, req, row0, kvh, sp, n_rows, k_first, k_end, lo_first);
-    else af_walk<P, 4, NC, NARROW>(p, s, req, row0, kvh, sp, n_rows, k_first, k_end, lo_first);
+    if (n_rows <= 16) af_walk<P, 1, NC, NARROW>(p, s, req, row0, kvh, sp, n_rows, k_first, k_end, lo_first, blk.last);
+    else if (n_rows <= 32) af_walk<P, 2, NC, NARROW>(p, s, req, row0, kvh, sp, n_rows, k_first, k_end, lo_first, blk.last);
+    else af_walk<P, 4, NC, NARROW>(p, s, req, row0, kvh, sp, n_rows, k_first, k_end, lo_first, blk.last);
 }
 
 }  // namespace bg

@@ -62,7 +62,7 @@ __global__ void __launch_bounds__(AX_THREADS, 1) attention_f32_tc_kernel(P p) {
     __shared__ int row_at[AX_ROWS];                    // a row's place among the partial results, -1: none
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int qb = blockIdx.x, kvh = blockIdx.y, sp = blockIdx.z;
+    const int kvh = blockIdx.y;
     if (tid == 0) {
         mbar_init(&q_full, 8);
         for (int b = 0; b < 2; ++b) { mbar_init(&k_full[b], 8); mbar_init(&k_empty[b], 1); mbar_init(&v_full[b], 8); mbar_init(&v_empty[b], 1); }
@@ -80,9 +80,10 @@ __global__ void __launch_bounds__(AX_THREADS, 1) attention_f32_tc_kernel(P p) {
     pdl_launch();                                      // (the columns are held)
     const unsigned tmem = tmem_sh;
     pdl_wait();
-    const int req = p.qblk[qb * 3 + 0], row0 = p.qblk[qb * 3 + 1], nq = p.qblk[qb * 3 + 2];
-    const int lo_first = nq > 0 ? first_visible(p.positions[row0], p.window) : 0;
-    const int k_first = sp * p.split, k_end = nq > 0 ? min((sp + 1) * p.split, p.positions[row0 + nq - 1] + 1) : 0;       // exclusive
+    const auto blk = att_block(p, blockIdx.x);
+    const int req = blk.req, row0 = blk.row0, nq = blk.nq, sp = blk.sp;
+    const int lo_first = nq > 0 ? first_visible(p.positions[att_row(p, row0)], p.window) : 0;
+    const int k_first = sp * p.split, k_end = nq > 0 ? min((sp + 1) * p.split, att_end(p, blk) + 1) : 0;       // exclusive
     const bool seen = nq > 0 && k_first < k_end && !(lo_first >= k_end && k_first >= p.keep);       // (else no key of the split is seen)
     const int hd = p.hd, vd = p.vd, group = p.group, n_rows = nq * group;
     const float* pool = (const float*)p.kv_pool;
@@ -245,8 +246,9 @@ __global__ void __launch_bounds__(AX_THREADS, 1) attention_f32_tc_kernel(P p) {
         const unsigned lanes = tmem + ((unsigned)(quarter * 32) << 16);
         const bool in = row < n_rows;
         const int qi = in ? row / group : 0, head = kvh * group + (in ? row - qi * group : 0);
-        const int pos = in ? p.positions[row0 + qi] : -1, lo = first_visible(pos < 0 ? 0 : pos, p.window);
-        const float* q = (const float*)p.q + (size_t)(row0 + qi) * p.q_stride + (size_t)head * hd;
+        const int at_row = in ? att_row(p, row0 + qi) : 0;
+        const int pos = in ? min(p.positions[at_row], blk.last) : -1, lo = first_visible(pos < 0 ? 0 : pos, p.window);
+        const float* q = (const float*)p.q + (size_t)at_row * p.q_stride + (size_t)head * hd;
         const float slope = p.slopes && in ? p.slopes[head] : 0.0f, scale_down = p.scale / AX_Q_UP;
         const int od = OD ? OD : vd / 2;               // output features of a thread, a multiple of 8
         constexpr int MOST = OD ? OD : 64;
@@ -425,7 +427,7 @@ __global__ void __launch_bounds__(AX_THREADS, 1) attention_f32_tc_kernel(P p) {
             add_values(i - 1, t_before, corr_before);
             // partial results of the rows that see at least one key of this split, through the tiles' room (their products are complete)
             row_max[half][row] = sum;
-            if (half == 0) row_at[row] = in && !(pos < sp * p.split || (lo >= (sp + 1) * p.split && sp * p.split >= p.keep)) ? (row0 + qi) * p.nh + head : -1;
+            if (half == 0) row_at[row] = in && !(pos < sp * p.split || (lo >= (sp + 1) * p.split && sp * p.split >= p.keep)) ? at_row * p.nh + head : -1;
             float* stage = (float*)kt;
             const int ld = vd + 4;
 #pragma unroll

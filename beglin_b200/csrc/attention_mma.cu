@@ -72,8 +72,15 @@ struct AttnMmaExtParams : AttnMmaParams {
     int keep;               // positions 0 .. keep - 1 stay visible behind a window
     const float* slopes;    // [nh] or null
 };
-template <bool EXT> struct AmParams { using type = AttnMmaParams; };
-template <> struct AmParams<true> { using type = AttnMmaExtParams; };
+// What the SHARED instances take besides: a row's first position that is its request's own (the ones before are attention_tcgen05.cu's).
+struct AttnMmaSharedParams : AttnMmaParams {
+    const int* own_first;   // [T]
+};
+template <bool EXT, bool SHARED> struct AmParams { using type = AttnMmaParams; };
+template <> struct AmParams<true, false> { using type = AttnMmaExtParams; };
+template <> struct AmParams<false, true> { using type = AttnMmaSharedParams; };
+__device__ __forceinline__ int am_own_first(const AttnMmaParams&, int) { return 0; }
+__device__ __forceinline__ int am_own_first(const AttnMmaSharedParams& p, int row) { return p.own_first[row]; }
 __device__ __forceinline__ int am_keep(const AttnMmaParams&) { return 0; }
 __device__ __forceinline__ int am_keep(const AttnMmaExtParams& p) { return p.keep; }
 __device__ __forceinline__ const float* am_slopes(const AttnMmaParams&) { return nullptr; }
@@ -130,10 +137,10 @@ __device__ __forceinline__ int swz_kv(int row, int c) {
     return (c >> 3) * (AM_STAGE_KEYS * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4);
 }
 
-template <int HD, bool BY_KEYS, int AM_STAGES, bool SWAP, bool EXT>
+template <int HD, bool BY_KEYS, int AM_STAGES, bool SWAP, bool EXT, bool SHARED = false>
 __global__ void __launch_bounds__(AM_ALL)
 attention_mma_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_constant__ CUtensorMap map_page,
-                     typename AmParams<EXT>::type p) {
+                     typename AmParams<EXT, SHARED>::type p) {
     constexpr int CH = HD / 8;                 // 16-byte columns per row
     constexpr int KSTEPS = HD / 16;            // k-steps of q.k
     constexpr int NT_O = HD / 8;               // 8-wide column tiles of the output
@@ -190,8 +197,10 @@ attention_mma_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_co
         mbar_init_fence();
     }
     const bool direct = !BY_KEYS && p.out != nullptr;
-    const int split = keys_per_split(p.split, pos_last + 1, (int)gridDim.z);
-    const int pre_key = direct ? 0 : sp * split;
+    // SHARED: the ranges cut what lies from the row's own first position on
+    const int own = SHARED ? am_own_first(p, row0) : 0;
+    const int split = keys_per_split(p.split, pos_last + 1 - own, (int)gridDim.z);
+    const int pre_key = direct ? 0 : own + sp * split;
     const int pre_group = (p.page_shift >= 0 ? pre_key >> p.page_shift : pre_key / p.page_size) / AM_TABLE;
     for (int i = tid; i < AM_TABLE; i += AM_ALL) {
         const int pi = pre_group * AM_TABLE + i;
@@ -199,13 +208,16 @@ attention_mma_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_co
     }
 
     const int lo_first = first_visible(pos_first, p.window);
-    const int k_first = direct ? 0 : sp * split;                  // this CTA's range of positions: [k_first, k_end)
+    const int k_first = direct ? 0 : own + sp * split;                  // this CTA's range of positions: [k_first, k_end)
     const int k_begin = direct ? lo_first : max(k_first, lo_first);   // of which the window's keys are [k_begin, k_end)
-    const int k_end = direct ? pos_last + 1 : min((sp + 1) * split, pos_last + 1);
+    const int k_end = direct ? pos_last + 1 : min(own + (sp + 1) * split, pos_last + 1);
     const int keep = am_keep(p);
     const int kept_end = min(keep, k_end);                        // and the kept ones [k_first, kept_end), possibly none
     const bool has_kept = EXT && k_first < kept_end;
-    if (k_begin >= k_end && !has_kept) return;
+    if (k_begin >= k_end && !has_kept) {
+        if (SHARED) pdl_wait();                // (no row may have positions of its own: what comes behind still waits for the shared ones' kernel)
+        return;
+    }
     auto in_range = [&](int key) { return key < k_end && (key >= k_begin || (EXT && key >= k_first && key < kept_end)); };
 
     // ---- stage loader: thread t copies 16-byte pieces of key rows of K and of V
@@ -708,7 +720,7 @@ attention_mma_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_co
         compute_sync();
         const int pos = pos_first;
         const int lo = first_visible(pos, p.window);
-        if (!(pos < sp * split || (lo >= (sp + 1) * split && !(EXT && sp * split < keep)))) {
+        if (SHARED ? pos >= k_first : !(pos < sp * split || (lo >= (sp + 1) * split && !(EXT && sp * split < keep)))) {
             // every thread takes one feature of all rows and works out the weights of the four warps' parts itself
             // (four exponentials a row: cheaper than a third barrier and a round through shared memory)
             if (tid < HD) {
@@ -751,9 +763,20 @@ static int am_launch_stages(const CUtensorMap& map, const CUtensorMap& map5, con
     if (e != cudaSuccess) return (int)e;
     dim3 grid(n_qblk, p.nkv, n_splits);
     e = launch(kern, grid, dim3(AM_ALL), smem, stream, map, map5,
-               static_cast<const typename AmParams<EXT>::type&>(p));
+               static_cast<const typename AmParams<EXT, false>::type&>(p));
     if (e != cudaSuccess) return (int)e;
     return BG_OK;
+}
+
+// The decoding arrangement over what lies behind positions that requests share.
+template <int HD, bool SWAP>
+static int am_launch_own(const CUtensorMap& map, const CUtensorMap& map5, const AttnMmaSharedParams& p, int T, int n_splits, cudaStream_t stream) {
+    auto kern = attention_mma_kernel<HD, true, AM_THREADS / 32, SWAP, false, true>;
+    const size_t smem = am_smem_bytes<HD, true, AM_THREADS / 32>();
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return (int)e;
+    e = launch(kern, dim3(T, p.nkv, n_splits), dim3(AM_ALL), smem, stream, map, map5, p);
+    return e == cudaSuccess ? BG_OK : (int)e;
 }
 
 template <int HD, bool BY_KEYS, bool EXT>
@@ -822,4 +845,33 @@ extern "C" int bg_attention_mma_partial(const void* q, int q_stride, const void*
     if (hd == 64) return by_keys ? am_launch<64, true>(map, map5, p, n_qblk, n_splits_launch, stream)
                                  : am_launch<64, false>(map, map5, p, n_qblk, n_splits_launch, stream);
     return BG_ERR_UNSUPPORTED;
+}
+
+// The partial results of T single tokens (row r of request r) over the positions from own_first[r] to their own, spread over n_splits ranges a row
+// (those of keys_per_split over the row's own positions): at slot first_slot + range of part_o [T][nh][slots][hd] and part_ml [T][nh][slots][2].  A row
+// without positions of its own writes nothing.
+extern "C" int bg_attention_mma_own(const void* q, int q_stride, const void* kv_pool, int num_pages, int page_size, const int* block_table, int max_pages,
+                                    const int* positions, const int* own_first, int T, float* part_o, float* part_ml, int slots, int first_slot, int n_splits,
+                                    int nh, int nkv, int hd, float scale, float softcap, unsigned* status, cudaStream_t stream) {
+    if (T <= 0 || n_splits <= 0) return BG_OK;
+    if (nkv <= 0 || nh % nkv != 0 || page_size <= 0 || first_slot < 0 || first_slot + n_splits > slots || n_splits > 65535 || nkv > 65535) return BG_ERR_SHAPE;
+    if ((q_stride % 8) != 0 || ((uintptr_t)q % 16) != 0 || ((uintptr_t)kv_pool % 16) != 0) return BG_ERR_ALIGN;
+    if ((hd != 64 && hd != 128) || nh / nkv > 16) return BG_ERR_UNSUPPORTED;
+    AttnMmaSharedParams p;
+    memset(&p, 0, sizeof(p));
+    p.q = (const __nv_bfloat16*)q; p.q_stride = q_stride; p.kv_pool = (const __nv_bfloat16*)kv_pool;
+    p.num_pages = num_pages; p.page_size = page_size; p.block_table = block_table; p.max_pages = max_pages;
+    p.page_shift = -1;
+    for (int sh = 0; sh < 30; ++sh) if ((1 << sh) == page_size) p.page_shift = sh;
+    p.positions = positions; p.max_splits = slots; p.nh = nh; p.nkv = nkv; p.group = nh / nkv; p.scale_log2 = scale * AM_LOG2E; p.status = status;
+    p.part_o = part_o + (size_t)first_slot * hd; p.part_ml = part_ml + (size_t)first_slot * 2;
+    p.cap_log2 = softcap > 0.0f ? softcap * AM_LOG2E : 0.0f; p.scale_over_cap = softcap > 0.0f ? scale / softcap : 0.0f;
+    p.own_first = own_first;
+    CUtensorMap map, map5;
+    memset(&map, 0, sizeof(map));
+    memset(&map5, 0, sizeof(map5));
+    p.use_tma = pt_page_size_ok(page_size) && p.page_shift >= 0 && pt_pool_map(&map, kv_pool, num_pages, nkv, page_size, hd) == BG_OK;
+    p.whole_pages = p.use_tma && page_size == AM_STAGE_KEYS && pt_page_map(&map5, kv_pool, num_pages, nkv, page_size, hd) == BG_OK;
+    if (hd == 128) return p.group <= 8 ? am_launch_own<128, true>(map, map5, p, T, n_splits, stream) : am_launch_own<128, false>(map, map5, p, T, n_splits, stream);
+    return p.group <= 8 ? am_launch_own<64, true>(map, map5, p, T, n_splits, stream) : am_launch_own<64, false>(map, map5, p, T, n_splits, stream);
 }

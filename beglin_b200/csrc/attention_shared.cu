@@ -1,0 +1,83 @@
+// Attention of single tokens whose requests share their first positions, in three parts: the shared positions, read once for all rows of a group
+// (attention_tcgen05.cu, SHARED), each request's own positions behind them (attention_mma.cu, SHARED), and here the joining of a row's partial results:
+//   m = max_i m_i,   out = sum_i o_i e^(m_i - m) / sum_i l_i e^(m_i - m),
+// over the slots 0 .. n - 1 of the row's group and those of the ranges that its own positions are cut into.
+#include "common.cuh"
+
+namespace bg {
+
+// A warp takes one (row, head); a lane takes four neighbouring features, HD / 4 lanes a slot, so that a warp reads 128 / HD slots at once.  Sums go in
+// the order of the slots.
+constexpr int SM_WARPS = 4;
+template <int HD>
+__global__ void __launch_bounds__(32 * SM_WARPS)
+attention_shared_merge_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml, const int* __restrict__ positions,
+                              const int* __restrict__ own_first, const int* __restrict__ shared_slots, int T, int nh, int slots, int first_slot,
+                              int n_own, const float* __restrict__ sink_w, int sink, __nv_bfloat16* __restrict__ out, int out_stride) {
+    constexpr int AT_ONCE = 8;
+    pdl_launch();
+    const int w = blockIdx.x * SM_WARPS + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const bool idle = w >= T * nh;
+    const int t = idle ? 0 : w / nh, h = w - t * nh;
+    const int n_shared = shared_slots[t];
+    const int own = positions[t] + 1 - own_first[t];
+    const int ranges = own > 0 ? (own + keys_per_split(0, own, n_own) - 1) / keys_per_split(0, own, n_own) : 0;
+    const int n = n_shared + ranges;
+    pdl_wait();
+    if (idle) return;
+    const size_t base = (size_t)w * slots;
+    auto slot_of = [&](int i) { return base + (i < n_shared ? i : first_slot + i - n_shared); };
+    const int d = lane * 4;
+    float m = -INFINITY, l = 0.0f;
+    if (sink) { m = sink_w ? sink_w[h] : 0.0f; l = 1.0f; }
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int i0 = 0; i0 < n; i0 += AT_ONCE) {
+        float2 ml[AT_ONCE];
+        float4 v[AT_ONCE];
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; ++j) {
+            const bool have = i0 + j < n;
+            ml[j] = have ? *reinterpret_cast<const float2*>(part_ml + slot_of(i0 + j) * 2) : make_float2(-INFINITY, 0.0f);
+            v[j] = have && d < HD ? *reinterpret_cast<const float4*>(part_o + slot_of(i0 + j) * HD + d) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+        float top = m;
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; ++j) top = fmaxf(top, ml[j].x);
+        if (top == -INFINITY) continue;                // no position seen so far
+        const float keep = expf(m - top);
+        l *= keep; acc.x *= keep; acc.y *= keep; acc.z *= keep; acc.w *= keep;
+        m = top;
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; ++j) {
+            const float f = ml[j].x == -INFINITY ? 0.0f : expf(ml[j].x - m);
+            l = fmaf(ml[j].y, f, l);
+            acc.x = fmaf(v[j].x, f, acc.x); acc.y = fmaf(v[j].y, f, acc.y); acc.z = fmaf(v[j].z, f, acc.z); acc.w = fmaf(v[j].w, f, acc.w);
+        }
+    }
+    if (d >= HD) return;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;      // (a row that sees nothing is nought)
+    const __nv_bfloat162 x = __floats2bfloat162_rn(acc.x * inv, acc.y * inv), y = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
+    *reinterpret_cast<uint2*>(out + (size_t)t * out_stride + (size_t)h * HD + d) =
+        make_uint2(*reinterpret_cast<const unsigned*>(&x), *reinterpret_cast<const unsigned*>(&y));
+}
+
+}  // namespace bg
+
+using namespace bg;
+
+// Joins the partial results of bg_attention_tc_shared (slots 0 .. shared_slots[t] - 1 of row t) and bg_attention_mma_own (n_own ranges from first_slot on).
+extern "C" int bg_attention_shared_merge(const float* part_o, const float* part_ml, const int* positions, const int* own_first, const int* shared_slots,
+                                         int T, int nh, int hd, int slots, int first_slot, int n_own, int sink, const float* sink_w, void* out, int out_stride,
+                                         cudaStream_t stream) {
+    if (T <= 0) return BG_OK;
+    if (nh <= 0 || slots <= 0 || n_own <= 0 || first_slot < 0 || first_slot + n_own > slots || (long long)T * nh > 0x7fffffff - 64) return BG_ERR_SHAPE;
+    if (out_stride % 4 || (uintptr_t)out % 8 || (uintptr_t)part_o % 16 || (uintptr_t)part_ml % 8) return BG_ERR_ALIGN;
+    const dim3 grid((unsigned)(((long long)T * nh + SM_WARPS - 1) / SM_WARPS)), block(32 * SM_WARPS);
+    cudaError_t e;
+    if (hd == 128) e = launch(attention_shared_merge_kernel<128>, grid, block, 0, stream, part_o, part_ml, positions, own_first, shared_slots, T, nh, slots,
+                              first_slot, n_own, sink_w, sink, (__nv_bfloat16*)out, out_stride);
+    else if (hd == 64) e = launch(attention_shared_merge_kernel<64>, grid, block, 0, stream, part_o, part_ml, positions, own_first, shared_slots, T, nh, slots,
+                                  first_slot, n_own, sink_w, sink, (__nv_bfloat16*)out, out_stride);
+    else return BG_ERR_UNSUPPORTED;
+    return e == cudaSuccess ? BG_OK : (int)e;
+}

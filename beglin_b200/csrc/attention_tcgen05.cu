@@ -71,8 +71,17 @@ struct AttnTcDiffParams : AttnTcParams {
     int vd;                     // a head's own features of the HD that its values are stored in
     float lambda, out_scale, eps;
 };
-template <bool DIFF> struct AtParams { using type = AttnTcParams; };
-template <> struct AtParams<true> { using type = AttnTcDiffParams; };
+// What the SHARED instances take besides, in place of query blocks and an output.
+struct AttnTcSharedParams : AttnTcParams {
+    const int* items;           // [n][8] = (request whose pages, first entry of `rows`, entries, first position, end, slot of the result, 0, 0)
+    const int* rows;            // rows of the batch, those of a block side by side
+    float* part_o;              // [rows][nh][slots][HD] unnormalised outputs
+    float* part_ml;             // [rows][nh][slots][2] maximum (of scores as they are), sum
+    int slots;
+};
+template <bool DIFF, bool SHARED> struct AtParams { using type = AttnTcParams; };
+template <> struct AtParams<true, false> { using type = AttnTcDiffParams; };
+template <> struct AtParams<false, true> { using type = AttnTcSharedParams; };
 
 __device__ __forceinline__ float at_ex2(float x) {
     float y;
@@ -99,10 +108,14 @@ __device__ __forceinline__ float at_squash(float x, float cap_log2, float cap_k)
 // keys and values is fetched once for both.  At the end the maps are not joined but subtracted, and the difference is normed:
 // out = o / sqrt(mean(o^2) + eps) * out_scale with o = O_0 / l_0 - lambda O_1 / l_1, the first `vd` of the HD features stored.
 // A stage of the rings serves two turns, so its release has barriers of its own (k_free, v_free).
-template <int HD, int AT_BK, bool SINK = false, bool EXT = false, bool DIFF = false>
+// SHARED: the rows are single tokens of several requests whose first positions lie in the same pages: a block is up to 128 rows (requests x query
+// heads of a kv head) over one range of those positions, and its result is partial: unnormalised sums with the rows' maxima and sums, which
+// attention_shared.cu joins with those of the other ranges and of each request's own positions.  A row sees the positions up to its own.
+template <int HD, int AT_BK, bool SINK = false, bool EXT = false, bool DIFF = false, bool SHARED = false>
 __global__ void __launch_bounds__(AT_THREADS)
-attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename AtParams<DIFF>::type p) {
+attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename AtParams<DIFF, SHARED>::type p) {
     static_assert(!DIFF || (AT_BK == 64 && !SINK && !EXT), "the two maps take tiles of 64 keys in turns");
+    static_assert(!SHARED || (AT_BK == 64 && !SINK && !EXT && !DIFF), "partial results of tiles of 64 keys");
     constexpr int AT_HALF = AT_BK / 2, AT_STAGES = 256 / AT_BK;
     constexpr int NSB = AT_STAGES;                       // score buffers in tensor memory: tiles whose scores may be under way
     // How the two groups of softmax warps share the keys.  Tiles of 128 keys: every tile is cut in two halves, one for
@@ -135,6 +148,8 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
     __shared__ __align__(8) unsigned long long s_full[NSB], p_full[2 * NSB], pv_done[NSB], o_ready;    // p_full: [2 buffer + group]
     __shared__ __align__(8) unsigned long long k_free[DIFF ? AT_STAGES : 1], v_free[DIFF ? AT_STAGES : 1];
     __shared__ float2 ml_other[AT_BM];                   // the second group's running maximum and sum of every row, for the join
+    __shared__ float2 ml_first[SHARED ? AT_BM : 1];      // and the first one's, where both groups write
+    __shared__ int row_of[SHARED ? AT_BM : 1];
     __shared__ unsigned tmem_sh;
     __shared__ int failed;
 
@@ -142,6 +157,11 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
     // the blocks with the most keys (the last ones of a prompt) are handed out first, for every kv head, so that
     // the short ones fill the machine's last wave
     const int kvh = blockIdx.x, qb = (int)gridDim.y - 1 - (int)blockIdx.y;
+    // (the list is older than the step: a CTA without work leaves before it holds anything, but not before the kernel ahead: this grid may have no work
+    // at all, and the one behind counts on that kernel being done)
+    if constexpr (SHARED) {
+        if (p.items[qb * 8 + 2] <= 0) { pdl_wait(); return; }
+    }
     if (tid == 0) {
         for (int s = 0; s < AT_STAGES; ++s) {
             mbar_init(&k_full[s], 1); mbar_init(&v_full[s], 1); mbar_init(&kv_landed[s], 1);
@@ -160,13 +180,22 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
     }
     pdl_wait();
-    const int req = p.qblk[qb * 3 + 0], row0 = p.qblk[qb * 3 + 1], nq = p.qblk[qb * 3 + 2];
+    int req, row0, nq;
+    if constexpr (SHARED) { req = p.items[qb * 8 + 0]; row0 = p.items[qb * 8 + 1]; nq = p.items[qb * 8 + 2]; }
+    else { req = p.qblk[qb * 3 + 0]; row0 = p.qblk[qb * 3 + 1]; nq = p.qblk[qb * 3 + 2]; }
     const int group = p.group;
     const int n_rows = nq * group;                       // <= 128
-    const int pos_first = p.positions[row0];
-    const int pos_last = pos_first + nq - 1;
-    const int k_begin = first_visible(pos_first, p.window);
-    const int k_end = pos_last + 1;
+    int pos_first, k_begin, k_end;
+    if constexpr (SHARED) {
+        pos_first = 0; k_begin = p.items[qb * 8 + 3]; k_end = p.items[qb * 8 + 4];
+    } else {
+        pos_first = p.positions[row0];
+        const int pos_last = pos_first + nq - 1;
+        k_begin = first_visible(pos_first, p.window);
+        k_end = pos_last + 1;
+    }
+    // the batch's row of the block's entry qi
+    auto batch_row = [&](int qi) { if constexpr (SHARED) return p.rows[row0 + qi]; else return row0 + qi; };
     const int keep = EXT ? p.keep : 0;
     const int n_kept = EXT ? (min(keep, k_end) + AT_BK - 1) / AT_BK : 0;         // tiles with kept positions
     const int tile0 = EXT ? max(k_begin / AT_BK, n_kept) : k_begin / AT_BK;      // the window's first tile behind those
@@ -180,7 +209,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
         uint4 v = make_uint4(0, 0, 0, 0);
         if (r < n_rows) {
             const int qi = r / group, g = r - qi * group;
-            v = *reinterpret_cast<const uint4*>(p.q + (size_t)(row0 + qi) * p.q_stride + (size_t)(kvh * group + g) * HD + c * 8);
+            v = *reinterpret_cast<const uint4*>(p.q + (size_t)batch_row(qi) * p.q_stride + (size_t)(kvh * group + g) * HD + c * 8);
         }
         const int cb = c >> 3, cc = c & 7;
         *reinterpret_cast<uint4*>(q_s + cb * (AT_BM * 128) + r * 128 + ((cc ^ (r & 7)) << 4)) = v;
@@ -302,8 +331,9 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
         const int r = quarter * 32 + lane;
         const unsigned lane_addr = (unsigned)(quarter * 32) << 16;
         const bool real = r < n_rows;
-        const int pos = real ? pos_first + r / group : -1;
-        const int lo = real ? first_visible(pos, p.window) : 0;
+        const int own_row = real ? batch_row(r / group) : 0;
+        const int pos = !real ? -1 : SHARED ? min(p.positions[own_row], k_end - 1) : pos_first + r / group;
+        const int lo = real && !SHARED ? first_visible(pos, p.window) : 0;
         const int warp_pos_min = __reduce_min_sync(0xffffffffu, real ? pos : 0x7fffffff);
         const int warp_lo_max = __reduce_max_sync(0xffffffffu, lo);
         float m = -INFINITY, l = 0.0f;
@@ -391,6 +421,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
         // the join of the two groups: the second hands its maximum and sum over, the first group's thread of the
         // same row (the same lanes of tensor memory) reads both accumulators
         if (grp == 1) ml_other[r] = make_float2(m, l);
+        if constexpr (SHARED) { if (grp == 0) ml_first[r] = make_float2(m, l); }
         asm volatile("bar.sync 1, 256;\n" ::: "memory");
         if constexpr (DIFF) {
             if (grp == 0 && ok && n_tiles > 0) {
@@ -432,6 +463,42 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
                         }
                     }
                 }
+            }
+        } else if constexpr (SHARED) {
+            // both accumulators through the keys' ring (its products are complete) into whole rows of the partial results; a group takes
+            // half of the features
+            constexpr int LD = HD + 4;
+            float* stage = reinterpret_cast<float*>(k_s);
+            const float2 first = ml_first[r], other = ml_other[r];
+            const float m_all = fmaxf(first.x, other.x), m_ref = (m_all == -INFINITY) ? 0.0f : m_all;
+            const float a0 = at_ex2(first.x - m_ref), a1 = at_ex2(other.x - m_ref);
+            const bool has1 = n_tiles > 1;               // with one tile the second group's accumulator was never written
+            tc_fence_after();
+#pragma unroll
+            for (int c0 = 0; c0 < HD / 2; c0 += 32) {
+                const int c = grp * (HD / 2) + c0;
+                float t[32], u[32];
+                tc_ld32(tmem + lane_addr + O_COL + c, t);
+                tc_ld32(tmem + lane_addr + O_COL + 128u + c, u);
+#pragma unroll
+                for (int q = 0; q < 32; q += 4)
+                    *reinterpret_cast<float4*>(stage + r * LD + c + q) =
+                        make_float4(t[q] * a0 + (has1 ? u[q] * a1 : 0.0f), t[q + 1] * a0 + (has1 ? u[q + 1] * a1 : 0.0f),
+                                    t[q + 2] * a0 + (has1 ? u[q + 2] * a1 : 0.0f), t[q + 3] * a0 + (has1 ? u[q + 3] * a1 : 0.0f));
+            }
+            if (grp == 0) {
+                row_of[r] = real ? (own_row * p.nh + kvh * group + r % group) : 0;
+                if (real) {
+                    const size_t at = ((size_t)row_of[r] * p.slots + p.items[qb * 8 + 5]) * 2;
+                    // (a wait that ran out: the row shows it)
+                    *reinterpret_cast<float2*>(p.part_ml + at) = make_float2(m_all * 0.6931471805599453f, ok ? first.y * a0 + other.y * a1 : NAN);
+                }
+            }
+            asm volatile("bar.sync 1, 256;\n" ::: "memory");
+            const int slot = p.items[qb * 8 + 5], w = grp * 4 + quarter;
+            for (int i = w * (128 / HD) + (lane * 4) / HD; i < n_rows; i += 8 * (128 / HD)) {
+                const int d = (lane * 4) % HD;
+                *reinterpret_cast<float4*>(p.part_o + ((size_t)row_of[i] * p.slots + slot) * HD + d) = *reinterpret_cast<const float4*>(stage + i * LD + d);
             }
         } else if (grp == 0 && ok && n_tiles > 0) {
             tc_fence_after();
@@ -576,6 +643,19 @@ static int at_launch(const CUtensorMap& map, const AttnTcParams& p, int n_qblk, 
     return BG_OK;
 }
 
+// The same for positions that requests share (tiles of 64 keys).
+template <int HD>
+static int at_launch_shared(const CUtensorMap& map, const AttnTcSharedParams& p, int n_items, cudaStream_t stream) {
+    auto kern = attention_tcgen05_kernel<HD, 64, false, false, false, true>;
+    const size_t smem = (size_t)(HD / 64) * AT_BM * 128 + (size_t)2 * 256 * (HD / 64) * 128 + 1024;
+    static_assert(AT_BM * (HD + 4) * 4 <= 2 * 256 * (HD / 64) * 128, "the rows' sums fit the rings");
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return (int)e;
+    e = launch(kern, dim3(p.nkv, n_items), dim3(AT_THREADS), smem, stream, map, p);
+    if (e != cudaSuccess) return (int)e;
+    return BG_OK;
+}
+
 // The same for differential attention (tiles of 64 keys).
 template <int HD>
 static int at_launch_difference(const CUtensorMap& map, const AttnTcDiffParams& p, int n_qblk, cudaStream_t stream) {
@@ -705,4 +785,30 @@ extern "C" int bg_attention_tc_difference(const void* q, int q_stride, const voi
     if (rc != BG_OK) return rc;
     if (hd == 128) return at_launch_difference<128>(map, p, n_qblk, stream);
     return at_launch_difference<64>(map, p, n_qblk, stream);
+}
+
+// The partial results of single tokens over positions that their requests share: items [n_items][8] and rows as AttnTcSharedParams says (an item of no
+// entries is passed over; an item's first position is a multiple of 64), part_o [rows][nh][slots][hd] and part_ml [rows][nh][slots][2].
+extern "C" int bg_attention_tc_shared(const void* q, int q_stride, const void* kv_pool, int num_pages, int page_size,
+                                      const int* block_table, int max_pages, const int* positions, const int* items, int n_items,
+                                      const int* rows, float* part_o, float* part_ml, int slots, int nh, int nkv, int hd, float scale,
+                                      float softcap, unsigned* status, cudaStream_t stream) {
+    if (n_items <= 0) return BG_OK;
+    if (nkv <= 0 || nh % nkv != 0 || (hd != 64 && hd != 128) || nh / nkv > 128 || !(scale > 0.0f) || softcap < 0.0f) return BG_ERR_UNSUPPORTED;
+    if (page_size < 1 || page_size > 64 || 64 % page_size != 0) return BG_ERR_UNSUPPORTED;
+    if (n_items > 65535 || slots <= 0) return BG_ERR_SHAPE;
+    if ((q_stride % 8) || ((uintptr_t)q % 16) || ((uintptr_t)kv_pool % 16) || ((uintptr_t)part_o % 16) || ((uintptr_t)part_ml % 8)) return BG_ERR_ALIGN;
+    AttnTcSharedParams p;
+    memset(&p, 0, sizeof(p));
+    p.q = (const __nv_bfloat16*)q; p.q_stride = q_stride; p.kv_pool = (const __nv_bfloat16*)kv_pool;
+    p.num_pages = num_pages; p.page_size = page_size; p.page_shift = -1;
+    for (int sh = 0; sh < 30; ++sh) if ((1 << sh) == page_size) p.page_shift = sh;
+    p.block_table = block_table; p.max_pages = max_pages; p.positions = positions;
+    p.nh = nh; p.nkv = nkv; p.group = nh / nkv; p.scale_log2 = scale * AT_LOG2E; p.status = status;
+    p.cap_log2 = softcap > 0.0f ? softcap * AT_LOG2E : 0.0f; p.cap_k = softcap > 0.0f ? 2.0f * AT_LOG2E * scale / softcap : 0.0f;
+    p.items = items; p.rows = rows; p.part_o = part_o; p.part_ml = part_ml; p.slots = slots;
+    CUtensorMap map;
+    int rc = pt_pool_map(&map, kv_pool, num_pages, nkv, page_size, hd);
+    if (rc != BG_OK) return rc;
+    return hd == 128 ? at_launch_shared<128>(map, p, n_items, stream) : at_launch_shared<64>(map, p, n_items, stream);
 }

@@ -10,9 +10,11 @@ import ctypes
 import functools
 from typing import Optional, Tuple
 
+import numpy as np
 import torch
 
 from . import build as _build
+from . import shared_plan as _shared
 
 F32, BF16 = 0, 1
 STATUS_BAD_TOKEN, STATUS_BAD_PAGE, STATUS_TIMEOUT, STATUS_BAD_POSITION = 1, 2, 4, 8
@@ -199,6 +201,15 @@ _SIGNATURES = {
                                _c_int, _c_int, _c_int, _c_int, _c_void_p],
     "bg_gemm_f32_nt_batched": [_c_void_p, _c_int, _c_ll, _c_void_p, _c_int, _c_ll, _c_void_p, _c_int, _c_ll, _c_int, _c_int,
                                _c_int, _c_int, _c_void_p, _c_void_p, _c_void_p],
+    "bg_attention_shared_partial": [_c_void_p, _c_int, _c_int, _c_void_p, _c_int, _c_int, _c_int, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_int, _c_void_p,
+                                    _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_float, _c_void_p,
+                                    _c_void_p],
+    "bg_attention_tc_shared": [_c_void_p, _c_int, _c_void_p, _c_int, _c_int, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p,
+                               _c_int, _c_int, _c_int, _c_int, _c_float, _c_float, _c_void_p, _c_void_p],
+    "bg_attention_mma_own": [_c_void_p, _c_int, _c_void_p, _c_int, _c_int, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_int,
+                             _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_float, _c_void_p, _c_void_p],
+    "bg_attention_shared_merge": [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_void_p,
+                                  _c_void_p, _c_int, _c_void_p],
     "bg_adjust_logits": [_c_void_p, _c_ll, _c_void_p, _c_ll, _c_int, _c_int, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
                          _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_int, _c_void_p, _c_void_p],
     "bg_copy_pages_most": [],
@@ -832,6 +843,164 @@ def _attention(q: torch.Tensor, q_stride: int, kv_pool: torch.Tensor, block_tabl
         raise KernelError(f"unknown attention kernel '{kernel}'")
     _check(L.bg_attention_merge(_p(part_o), _p(part_ml), _p(positions), _p(out), _dt(out), out.stride(0), n_rows, nh,
                                 vd, n_splits, split, window, 1 if sink else 0, _p(sink_weight), int(keep), _stream()), "attention_merge")
+
+
+# ------------------------------------------------------------------------------------------------
+# Attention of single tokens whose requests share their first positions
+class SharedPlan:
+    """How a layer's attention goes over shared positions: made by `shared_plan` for one `SharedPrefix`, and renewed in place by `update`, so that a
+    captured graph reads the groups of the step that it is replayed for."""
+
+    def __init__(self, n_rows, nh, nkv, hd, vd, dtype, query_dtype, page_size, kernel, bq, tile, split, device):
+        self.n_rows, self.nh, self.nkv, self.hd, self.vd, self.dtype, self.query_dtype, self.page_size = n_rows, nh, nkv, hd, vd, dtype, query_dtype, page_size
+        self.kernel, self.bq, self.tile, self.split, self.device = kernel, bq, tile, split, torch.device(device)
+        if self.device.type == "cuda" and self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
+        self.sms = sm_count(self.device) if self.device.type == "cuda" else 148
+        self.shared = None
+        if kernel == "tc":
+            self.room, sizes = _shared.items_room(n_rows, bq, nkv, self.sms), (n_rows, n_rows, n_rows)
+        else:
+            self.room, sizes = _shared.blocks_room(n_rows), (2 * n_rows,)
+        # one buffer, so that a renewal is one copy: the list, then the rows' numbers
+        total = self.room * 8 + sum(sizes)
+        self.buffer = torch.zeros(total, dtype=torch.int32, device=self.device)
+        self.items, at = self.buffer[:self.room * 8].view(self.room, 8), self.room * 8
+        self.arrays = []
+        for n in sizes:
+            self.arrays.append(self.buffer[at:at + n])
+            at += n
+        self.rows = self.arrays[0]
+        if kernel == "tc":
+            self.own_first, self.parts = self.arrays[1:]
+        self.slots = 0         # results of a row over what it shares, at most
+
+    MOST_RANGES = 64
+
+    def pack(self, shared) -> "np.ndarray":
+        """What the device holds for these groups, as one array on the host."""
+        if shared.n_rows != self.n_rows:
+            raise KernelError(f"shared_plan: groups of {shared.n_rows} rows for a plan of {self.n_rows}")
+        if self.kernel == "tc":
+            arrays = _shared.shared_items(shared, self.bq, self.nkv, self.sms, self.room, self.MOST_RANGES)
+        else:
+            arrays = _shared.shared_blocks(shared, self.bq, self.split, self.room)
+        return np.concatenate([a.reshape(-1) for a in arrays])
+
+    def update(self, shared, fixed: bool = False) -> None:
+        """Take the groups of `shared`.  `fixed`: the launches keep the shape that serves any groups of these rows (for a captured graph)."""
+        host = torch.from_numpy(self.pack(shared))
+        if self.device.type == "cuda":
+            host = host.pin_memory()
+        self.buffer.copy_(host, non_blocking=True)
+        self._staged = host            # (kept until the next renewal: the copy may be under way)
+        self._shape(shared, host, fixed)
+
+    def _shape(self, shared, host, fixed: bool) -> None:
+        self.shared = shared
+        items = host[:self.room * 8].view(self.room, 8).numpy()
+        used = int((items[:, 2] > 0).sum())
+        if self.kernel == "tc":
+            self.n_items = self.room if fixed else used
+            self.slots = self.MOST_RANGES if fixed else int(host[self.room * 8 + 2 * self.n_rows:].max()) if self.n_rows else 0
+            self.least_own = 0 if fixed or not self.n_rows else int(host[self.room * 8 + self.n_rows:self.room * 8 + 2 * self.n_rows].min())
+        else:
+            self.n_items = self.room if fixed else used
+            own = items[:used][items[:used, 4] == _shared.MOST]
+            self.slots = int(items[:used][items[:used, 4] != _shared.MOST][:, 4].max(initial=0))
+            self.least_own = 0 if fixed else int(own[:, 3].min(initial=0)) if len(own) else 0
+
+
+def shared_plan(shared, nh: int, nkv: int, hd: int, dtype: torch.dtype, page_size: int = 64, vd: Optional[int] = None, split: int = 256, prefer: str = "auto",
+                query_dtype: Optional[torch.dtype] = None, device="cuda", fixed: bool = False) -> SharedPlan:
+    """The plan of `shared_attention` for the groups of `shared` (a `cache.shared.SharedPrefix`), heads of `hd` features (values of `vd`), a cache of `dtype` and
+    queries of `query_dtype`.  Kernels: "tc" (bfloat16, heads of 64 or 128: the shared positions on tcgen05) or "generic" (every size and type, splits at
+    multiples of `split` positions, whole splits shared: a row's result is bit for bit that of `attention`).  `fixed`: launches of one shape for any groups,
+    for a captured graph, whose groups `SharedPlan.update` then renews."""
+    vd, query_dtype = hd if vd is None else int(vd), query_dtype or dtype
+    if nkv <= 0 or nh % nkv:
+        raise KernelError(f"shared_plan: {nh} query heads are not a multiple of {nkv} kv heads")
+    if prefer not in ("auto", "generic", "tc"):
+        raise KernelError(f"shared_plan: unknown kernel choice '{prefer}'")
+    L, bq, tile = lib(), _c_int(0), _c_int(0)
+    group = nh // nkv
+    takes = dtype == query_dtype == torch.bfloat16 and vd == hd and L.bg_attention_tc_plan(group, hd, page_size, ctypes.byref(bq)) == 0 \
+        and L.bg_attention_mma_plan(group, hd, 1, ctypes.byref(tile)) == 0
+    if prefer == "tc" and not takes:
+        raise KernelError(f"shared_plan: the tensor-core kernels do not take {dtype} heads of {hd} with {group} query heads per kv head and pages of {page_size}")
+    if takes and prefer != "generic":
+        plan = SharedPlan(shared.n_rows, nh, nkv, hd, vd, dtype, query_dtype, page_size, "tc", bq.value, 64, 0, device)
+    else:
+        if L.bg_attention_plan(group, hd, vd, 1, 1 if dtype == query_dtype == torch.float32 else 0, ctypes.byref(bq), ctypes.byref(tile)) != 0:
+            raise KernelError(f"shared_plan: heads of {hd} (values of {vd}) with {group} query heads per kv head are not supported")
+        if split <= 0 or split % tile.value:
+            raise KernelError(f"shared_plan: splits of {split} positions are not whole tiles of {tile.value}")
+        plan = SharedPlan(shared.n_rows, nh, nkv, hd, vd, dtype, query_dtype, page_size, "generic", bq.value, tile.value, split, device)
+    plan.update(shared, fixed)
+    return plan
+
+
+def shared_attention(*args, **kwargs) -> None:
+    """`_shared_attention` under the phase timer of its kernel class (all its kernels together)."""
+    with phase("attn"):
+        _shared_attention(*args, **kwargs)
+
+
+def _shared_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_table: torch.Tensor, positions: torch.Tensor, plan: SharedPlan, max_position: int,
+                      scale: float, out: torch.Tensor, status: Optional[torch.Tensor], sink: bool = False, sink_weight: Optional[torch.Tensor] = None,
+                      softcap: float = 0.0) -> None:
+    """Paged grouped-query attention of a step of single tokens, row r that of request r, over every position up to its own: what a group of `plan` shares is
+    read once for all of its rows, through the pages of the group's first row, and what lies behind through each row's own.  q [T, nh * hd] (rows may lie
+    apart), kv_pool and block_table as `attention` takes them, `max_position` a bound on the positions, out [T, nh * vd].  `sink`, `sink_weight` and
+    `softcap` as in `attention`.  A row whose position lies inside what its group shares sees that far; values behind it that are not finite reach it, which
+    those behind the shared positions never do."""
+    T, nh, nkv, hd, vd = plan.n_rows, plan.nh, plan.nkv, plan.hd, plan.vd
+    _i32(positions, "positions"); _i32(block_table, "block_table")
+    if q.dim() != 2 or q.shape[0] != T or q.shape[1] != nh * hd or q.stride(1) != 1 or q.dtype != plan.query_dtype:
+        raise KernelError(f"shared_attention: q is {q.dtype} {tuple(q.shape)}, expected {plan.query_dtype} [{T}, {nh * hd}]")
+    if out.dim() != 2 or out.shape[0] != T or out.shape[1] != nh * vd or out.stride(1) != 1 or T > 1 and out.stride(0) < nh * vd:
+        raise KernelError(f"shared_attention: out is {tuple(out.shape)}, expected [{T}, {nh * vd}]")
+    if positions.numel() != T or block_table.dim() != 2 or block_table.shape[0] != T:
+        raise KernelError("shared_attention: a position and a row of the block table for every row")
+    page = (2, nkv, plan.page_size, hd) if vd == hd else (nkv * plan.page_size * (hd + vd),)
+    if kv_pool.dtype != plan.dtype or tuple(kv_pool.shape[1:]) != page or not kv_pool.is_contiguous():
+        raise KernelError(f"shared_attention: kv_pool is {kv_pool.dtype} {tuple(kv_pool.shape)}, expected {plan.dtype} [pages, {', '.join(map(str, page))}]")
+    if sink_weight is not None and (sink_weight.dtype != torch.float32 or sink_weight.numel() != nh or not sink_weight.is_contiguous()):
+        raise KernelError("shared_attention: the sink's scores are contiguous float32, one per query head")
+    if max_position < 0 or softcap < 0.0:
+        raise KernelError("shared_attention: max_position and softcap are not negative")
+    if T == 0:
+        return
+    _here("shared_attention", q, kv_pool, block_table, positions, plan.buffer, out, sink_weight, status)
+    sink, L, num_pages = 1 if sink or sink_weight is not None else 0, lib(), kv_pool.shape[0]
+    if plan.kernel == "generic":
+        n_splits = max_position // plan.split + 1
+        at_once = max(plan.slots, n_splits - plan.least_own, 1)
+        at_once = min(at_once, n_splits)
+        part = torch.empty(T * nh * n_splits * (vd + 2), dtype=torch.float32, device=q.device)
+        part_o, part_ml = part[:T * nh * n_splits * vd], part[T * nh * n_splits * vd:]
+        _check(L.bg_attention_shared_partial(
+            _p(q), _dt(q), q.stride(0), _p(kv_pool), _dt(kv_pool), num_pages, plan.page_size, _p(block_table), block_table.shape[1], _p(positions),
+            _p(plan.items), plan.n_items, _p(plan.rows), _p(part_o), _p(part_ml), n_splits, at_once, nh, nkv, hd, vd, plan.split, plan.tile, plan.bq,
+            float(scale), float(softcap), _p(status), _stream()), "attention_shared_partial")
+        _check(L.bg_attention_merge(_p(part_o), _p(part_ml), _p(positions), _p(out), _dt(out), out.stride(0), T, nh, vd, n_splits, plan.split, 0, sink,
+                                    _p(sink_weight), 0, _stream()), "attention_merge")
+        return
+    if status is None or out.dtype != torch.bfloat16:
+        raise KernelError("shared_attention: the tensor-core kernels want a status word and write bfloat16")
+    n_own = decode_splits(T * nkv, max(1, max_position + 1 - plan.least_own))
+    slots = plan.slots + n_own
+    part = torch.empty(T * nh * slots * (hd + 2), dtype=torch.float32, device=q.device)
+    part_o, part_ml = part.data_ptr(), part.data_ptr() + T * nh * slots * hd * 4
+    if plan.n_items:
+        _check(L.bg_attention_tc_shared(_p(q), q.stride(0), _p(kv_pool), num_pages, plan.page_size, _p(block_table), block_table.shape[1], _p(positions),
+                                        _p(plan.items), plan.n_items, _p(plan.rows), part_o, part_ml, slots, nh, nkv, hd, float(scale), float(softcap),
+                                        _p(status), _stream()), "attention_tcgen05_shared")
+    _check(L.bg_attention_mma_own(_p(q), q.stride(0), _p(kv_pool), num_pages, plan.page_size, _p(block_table), block_table.shape[1], _p(positions),
+                                  _p(plan.own_first), T, part_o, part_ml, slots, plan.slots, n_own, nh, nkv, hd, float(scale), float(softcap), _p(status),
+                                  _stream()), "attention_mma_own")
+    _check(L.bg_attention_shared_merge(part_o, part_ml, _p(positions), _p(plan.own_first), _p(plan.parts), T, nh, hd, slots, plan.slots, n_own, sink,
+                                       _p(sink_weight), _p(out), out.stride(0), _stream()), "attention_shared_merge")
 
 
 # ------------------------------------------------------------------------------------------------
