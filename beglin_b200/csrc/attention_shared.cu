@@ -4,6 +4,26 @@
 // over the slots 0 .. n - 1 of the row's group and those of the ranges that its own positions are cut into.
 #include "common.cuh"
 
+// How a layer's attention goes over shared positions, and what a step brings to it.  The host side fills the fields by name.
+struct SharedAttnArgs {
+    const int* items;           // [n_items][8], as the kernel of the shared positions takes them
+    const int* rows;
+    const int* own_first;       // [T] tensor cores: a row's first position of its own
+    const int* parts;           // [T] tensor cores: results of a row over what it shares
+    int tensor_cores, T, nh, nkv, hd, vd, page_size, q_dtype, cache_dtype, n_items;
+    int slots;                  // the most results of a row over what it shares
+    int split, tile, bq;        // float units: keys of a split and a tile, rows of a block
+};
+struct SharedAttnStep {
+    const void* q; const void* pool; const int* table; const int* positions; void* out; const float* sink_w; unsigned* status; float* scratch;
+    long long scratch_floats;
+    int q_stride, out_stride, max_pages, num_pages;
+    int ranges;                 // tensor cores: ranges that a row's own positions are cut into; float units: splits of the longest row
+    int at_once;                // float units: the most splits of a block
+    int sink, out_dtype;
+    float scale, softcap;
+};
+
 namespace bg {
 
 // A warp takes one (row, head); a lane takes four neighbouring features, HD / 4 lanes a slot, so that a warp reads 128 / HD slots at once.  Sums go in
@@ -65,19 +85,47 @@ attention_shared_merge_kernel(const float* __restrict__ part_o, const float* __r
 
 using namespace bg;
 
-// Joins the partial results of bg_attention_tc_shared (slots 0 .. shared_slots[t] - 1 of row t) and bg_attention_mma_own (n_own ranges from first_slot on).
-extern "C" int bg_attention_shared_merge(const float* part_o, const float* part_ml, const int* positions, const int* own_first, const int* shared_slots,
-                                         int T, int nh, int hd, int slots, int first_slot, int n_own, int sink, const float* sink_w, void* out, int out_stride,
-                                         cudaStream_t stream) {
-    if (T <= 0) return BG_OK;
-    if (nh <= 0 || slots <= 0 || n_own <= 0 || first_slot < 0 || first_slot + n_own > slots || (long long)T * nh > 0x7fffffff - 64) return BG_ERR_SHAPE;
-    if (out_stride % 4 || (uintptr_t)out % 8 || (uintptr_t)part_o % 16 || (uintptr_t)part_ml % 8) return BG_ERR_ALIGN;
+// Joins the partial results of bg_attention_tc_shared (slots 0 .. parts[t] - 1 of row t) and bg_attention_mma_own (n_own ranges from first_slot on).
+static int shared_merge(const float* part_o, const float* part_ml, const int* positions, const int* own_first, const int* parts, int T, int nh, int hd, int slots,
+                        int first_slot, int n_own, int sink, const float* sink_w, void* out, int out_stride, cudaStream_t stream) {
+    if (first_slot + n_own > slots || (long long)T * nh > 0x7fffffff - 64) return BG_ERR_SHAPE;
+    if (out_stride % 4 || (uintptr_t)out % 8) return BG_ERR_ALIGN;
     const dim3 grid((unsigned)(((long long)T * nh + SM_WARPS - 1) / SM_WARPS)), block(32 * SM_WARPS);
-    cudaError_t e;
-    if (hd == 128) e = launch(attention_shared_merge_kernel<128>, grid, block, 0, stream, part_o, part_ml, positions, own_first, shared_slots, T, nh, slots,
-                              first_slot, n_own, sink_w, sink, (__nv_bfloat16*)out, out_stride);
-    else if (hd == 64) e = launch(attention_shared_merge_kernel<64>, grid, block, 0, stream, part_o, part_ml, positions, own_first, shared_slots, T, nh, slots,
-                                  first_slot, n_own, sink_w, sink, (__nv_bfloat16*)out, out_stride);
-    else return BG_ERR_UNSUPPORTED;
+    auto kern = hd == 128 ? attention_shared_merge_kernel<128> : attention_shared_merge_kernel<64>;
+    cudaError_t e = launch(kern, grid, block, 0, stream, part_o, part_ml, positions, own_first, parts, T, nh, slots, first_slot, n_own, sink_w, sink,
+                           (__nv_bfloat16*)out, out_stride);
     return e == cudaSuccess ? BG_OK : (int)e;
+}
+
+// Bytes of what the host side mirrors field by field; it compares them when it loads the library.
+extern "C" int bg_shared_attention_bytes(int step) { return (int)(step ? sizeof(SharedAttnStep) : sizeof(SharedAttnArgs)); }
+
+// The whole attention of a step of single tokens over shared and own positions, as one call.  scratch: T * nh * n * (vd + 2) floats, n the float units' `ranges`
+// or the tensor cores' slots + ranges.
+extern "C" int bg_shared_attention(const SharedAttnArgs* args, const SharedAttnStep* step, cudaStream_t stream) {
+    const SharedAttnArgs& a = *args;
+    const SharedAttnStep& s = *step;
+    if (a.T <= 0) return BG_OK;
+    if (a.nh <= 0 || a.nkv <= 0 || a.nh % a.nkv || a.hd <= 0 || a.vd <= 0 || s.ranges <= 0 || a.slots < 0 || (uintptr_t)s.scratch % 16) return BG_ERR_SHAPE;
+    const long long results = (long long)a.T * a.nh * (a.tensor_cores ? a.slots + s.ranges : s.ranges);
+    if (s.scratch_floats < results * (a.vd + 2)) return BG_ERR_SHAPE;
+    float *part_o = s.scratch, *part_ml = s.scratch + results * a.vd;
+    if (!a.tensor_cores) {
+        int rc = bg_attention_shared_partial(s.q, a.q_dtype, s.q_stride, s.pool, a.cache_dtype, s.num_pages, a.page_size, s.table, s.max_pages, s.positions, a.items,
+                                             a.n_items, a.rows, part_o, part_ml, s.ranges, s.at_once, a.nh, a.nkv, a.hd, a.vd, a.split, a.tile, a.bq, s.scale,
+                                             s.softcap, s.status, stream);
+        if (rc != BG_OK) return rc;
+        return bg_attention_merge(part_o, part_ml, s.positions, s.out, s.out_dtype, s.out_stride, a.T, a.nh, a.vd, s.ranges, a.split, 0, s.sink, s.sink_w, 0, stream);
+    }
+    if (a.q_dtype != BG_DTYPE_BF16 || a.cache_dtype != BG_DTYPE_BF16 || s.out_dtype != BG_DTYPE_BF16) return BG_ERR_DTYPE;
+    const int slots = a.slots + s.ranges;
+    int rc = bg_attention_tc_shared(s.q, s.q_stride, s.pool, s.num_pages, a.page_size, s.table, s.max_pages, s.positions, a.items, a.n_items, a.rows, part_o,
+                                    part_ml, slots, a.nh, a.nkv, a.hd, s.scale, s.softcap, s.status, stream);
+    if (rc == BG_OK)
+        rc = bg_attention_mma_own(s.q, s.q_stride, s.pool, s.num_pages, a.page_size, s.table, s.max_pages, s.positions, a.own_first, a.T, part_o, part_ml, slots,
+                                  a.slots, s.ranges, a.nh, a.nkv, a.hd, s.scale, s.softcap, s.status, stream);
+    if (rc == BG_OK)
+        rc = shared_merge(part_o, part_ml, s.positions, a.own_first, a.parts, a.T, a.nh, a.hd, slots, a.slots, s.ranges, s.sink, s.sink_w, s.out, s.out_stride,
+                          stream);
+    return rc;
 }

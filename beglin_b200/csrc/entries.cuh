@@ -10,6 +10,17 @@ int bg_attention_partial(const void* q, int q_dtype, int q_stride, const void* k
     stream);
 int bg_attention_merge(const float* part_o, const float* part_ml, const int* positions, void* out, int out_dtype, int out_stride, int T, int nh, int hd, int
     max_splits, int split, int window, int sink, const float* sink_w, int keep, cudaStream_t stream);
+int bg_attention_shared_partial(const void* q, int q_dtype, int q_stride, const void* kv_pool, int cache_dtype, int num_pages, int page_size, const int*
+    block_table, int max_pages, const int* positions, const int* qblk, int n_qblk, const int* rows, float* part_o, float* part_ml, int max_splits, int
+    n_splits_launch, int nh, int nkv, int hd, int vd, int split, int tile, int bq, float scale, float softcap, unsigned* status, cudaStream_t stream);
+// attention_mma.cu
+int bg_attention_mma_own(const void* q, int q_stride, const void* kv_pool, int num_pages, int page_size, const int* block_table, int max_pages, const int*
+    positions, const int* own_first, int T, float* part_o, float* part_ml, int slots, int first_slot, int n_splits, int nh, int nkv, int hd, float scale,
+    float softcap, unsigned* status, cudaStream_t stream);
+// attention_tcgen05.cu
+int bg_attention_tc_shared(const void* q, int q_stride, const void* kv_pool, int num_pages, int page_size, const int* block_table, int max_pages, const int*
+    positions, const int* items, int n_items, const int* rows, float* part_o, float* part_ml, int slots, int nh, int nkv, int hd, float scale, float softcap,
+    unsigned* status, cudaStream_t stream);
 // elementwise.cu
 int bg_swiglu(const void* gu, int in_dtype, int parts, long long part_stride, void* out, int out_dtype, int rows, int im, int block, int act, float limit,
     cudaStream_t stream);

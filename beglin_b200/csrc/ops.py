@@ -201,15 +201,8 @@ _SIGNATURES = {
                                _c_int, _c_int, _c_int, _c_int, _c_void_p],
     "bg_gemm_f32_nt_batched": [_c_void_p, _c_int, _c_ll, _c_void_p, _c_int, _c_ll, _c_void_p, _c_int, _c_ll, _c_int, _c_int,
                                _c_int, _c_int, _c_void_p, _c_void_p, _c_void_p],
-    "bg_attention_shared_partial": [_c_void_p, _c_int, _c_int, _c_void_p, _c_int, _c_int, _c_int, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_int, _c_void_p,
-                                    _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_float, _c_void_p,
-                                    _c_void_p],
-    "bg_attention_tc_shared": [_c_void_p, _c_int, _c_void_p, _c_int, _c_int, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p,
-                               _c_int, _c_int, _c_int, _c_int, _c_float, _c_float, _c_void_p, _c_void_p],
-    "bg_attention_mma_own": [_c_void_p, _c_int, _c_void_p, _c_int, _c_int, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_int,
-                             _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_float, _c_void_p, _c_void_p],
-    "bg_attention_shared_merge": [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_void_p,
-                                  _c_void_p, _c_int, _c_void_p],
+    "bg_shared_attention_bytes": [_c_int],
+    "bg_shared_attention": [_c_void_p, _c_void_p, _c_void_p],
     "bg_adjust_logits": [_c_void_p, _c_ll, _c_void_p, _c_ll, _c_int, _c_int, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
                          _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_int, _c_void_p, _c_void_p],
     "bg_copy_pages_most": [],
@@ -242,7 +235,8 @@ def lib():
             fn.restype = _RESULTS.get(name, _c_int)
         for cls, name, which in ((AttnF32Args, "bg_attention_f32_bytes", (0,)), (AttnF32Step, "bg_attention_f32_bytes", (1,)), (LatentArgs, "bg_latent_bytes", (0,)),
                                  (LatentStep, "bg_latent_bytes", (1,)), (Mamba2Args, "bg_mamba2_bytes", (0,)), (Mamba2Step, "bg_mamba2_bytes", (1,)),
-                                 (ExpertsArgs, "bg_experts_bytes", ()), (_GlaArgs, "bg_gla_bytes", ())):
+                                 (ExpertsArgs, "bg_experts_bytes", ()), (_GlaArgs, "bg_gla_bytes", ()), (SharedAttnArgs, "bg_shared_attention_bytes", (0,)),
+                                 (SharedAttnStep, "bg_shared_attention_bytes", (1,))):
             if getattr(handle, name)(*which) != ctypes.sizeof(cls):
                 raise KernelError(f"the kernel library's {cls.__name__} has another size than its mirror here")
         _lib = handle
@@ -393,10 +387,12 @@ def _stream():
 
 def _here(what: str, *tensors) -> None:
     """All on the current device: a launch goes to the current device's stream."""
-    _cuda(*tensors)
+    for t in tensors:
+        if t is not None and t.get_device() < 0:           # (an attribute less than t.is_cuda and t.device.index together)
+            _cuda(t)
     now = torch.cuda.current_device()
     for t in tensors:
-        if t is not None and t.device.index != now:
+        if t is not None and t.get_device() != now:
             raise KernelError(f"{what}: a tensor on {t.device}, the current device is cuda:{now}")
 
 
@@ -847,6 +843,19 @@ def _attention(q: torch.Tensor, q_stride: int, kv_pool: torch.Tensor, block_tabl
 
 # ------------------------------------------------------------------------------------------------
 # Attention of single tokens whose requests share their first positions
+class SharedAttnArgs(ctypes.Structure):
+    """What `shared_attention` needs of its plan (csrc/attention_shared.cu says what the fields are)."""
+    _fields_ = [(n, _c_void_p) for n in ("items", "rows", "own_first", "parts")] \
+        + [(n, _c_int) for n in ("tensor_cores", "T", "nh", "nkv", "hd", "vd", "page_size", "q_dtype", "cache_dtype", "n_items", "slots", "split", "tile", "bq")]
+
+
+class SharedAttnStep(ctypes.Structure):
+    """What a step brings to `shared_attention`."""
+    _fields_ = [(n, _c_void_p) for n in ("q", "pool", "table", "positions", "out", "sink_w", "status", "scratch")] + [("scratch_floats", _c_ll)] \
+        + [(n, _c_int) for n in ("q_stride", "out_stride", "max_pages", "num_pages", "ranges", "at_once", "sink", "out_dtype")] \
+        + [("scale", _c_float), ("softcap", _c_float)]
+
+
 class SharedPlan:
     """How a layer's attention goes over shared positions: made by `shared_plan` for one `SharedPrefix`, and renewed in place by `update`, so that a
     captured graph reads the groups of the step that it is replayed for."""
@@ -908,7 +917,16 @@ class SharedPlan:
             self.n_items = self.room if fixed else used
             own = items[:used][items[:used, 4] == _shared.MOST]
             self.slots = int(items[:used][items[:used, 4] != _shared.MOST][:, 4].max(initial=0))
-            self.least_own = 0 if fixed else int(own[:, 3].min(initial=0)) if len(own) else 0
+            self.least_own = 0 if fixed or not len(own) else int(own[:, 3].min())
+        ptr = lambda t: t.data_ptr()
+        tc = self.kernel == "tc"
+        self.args = SharedAttnArgs(ptr(self.items), ptr(self.rows), ptr(self.own_first) if tc else None, ptr(self.parts) if tc else None, int(tc), self.n_rows,
+                                   self.nh, self.nkv, self.hd, self.vd, self.page_size, F32 if self.query_dtype == torch.float32 else BF16,
+                                   F32 if self.dtype == torch.float32 else BF16, self.n_items, self.slots, self.split, self.tile, self.bq)
+        self._args = ctypes.byref(self.args)
+        # what `shared_attention` compares its tensors with
+        self.q_shape, self.out_shape = (self.n_rows, self.nh * self.hd), (self.n_rows, self.nh * self.vd)
+        self.page_shape = (2, self.nkv, self.page_size, self.hd) if self.vd == self.hd else (self.nkv * self.page_size * (self.hd + self.vd),)
 
 
 def shared_plan(shared, nh: int, nkv: int, hd: int, dtype: torch.dtype, page_size: int = 64, vd: Optional[int] = None, split: int = 256, prefer: str = "auto",
@@ -954,17 +972,16 @@ def _shared_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_table: torch
     apart), kv_pool and block_table as `attention` takes them, `max_position` a bound on the positions, out [T, nh * vd].  `sink`, `sink_weight` and
     `softcap` as in `attention`.  A row whose position lies inside what its group shares sees that far; values behind it that are not finite reach it, which
     those behind the shared positions never do."""
-    T, nh, nkv, hd, vd = plan.n_rows, plan.nh, plan.nkv, plan.hd, plan.vd
+    T, nh, vd = plan.n_rows, plan.nh, plan.vd
     _i32(positions, "positions"); _i32(block_table, "block_table")
-    if q.dim() != 2 or q.shape[0] != T or q.shape[1] != nh * hd or q.stride(1) != 1 or q.dtype != plan.query_dtype:
-        raise KernelError(f"shared_attention: q is {q.dtype} {tuple(q.shape)}, expected {plan.query_dtype} [{T}, {nh * hd}]")
-    if out.dim() != 2 or out.shape[0] != T or out.shape[1] != nh * vd or out.stride(1) != 1 or T > 1 and out.stride(0) < nh * vd:
-        raise KernelError(f"shared_attention: out is {tuple(out.shape)}, expected [{T}, {nh * vd}]")
+    if q.shape != plan.q_shape or q.stride(1) != 1 or q.dtype != plan.query_dtype:
+        raise KernelError(f"shared_attention: q is {q.dtype} {tuple(q.shape)}, expected {plan.query_dtype} {list(plan.q_shape)}")
+    if out.shape != plan.out_shape or out.stride(1) != 1 or T > 1 and out.stride(0) < nh * vd:
+        raise KernelError(f"shared_attention: out is {tuple(out.shape)}, expected {list(plan.out_shape)}")
     if positions.numel() != T or block_table.dim() != 2 or block_table.shape[0] != T:
         raise KernelError("shared_attention: a position and a row of the block table for every row")
-    page = (2, nkv, plan.page_size, hd) if vd == hd else (nkv * plan.page_size * (hd + vd),)
-    if kv_pool.dtype != plan.dtype or tuple(kv_pool.shape[1:]) != page or not kv_pool.is_contiguous():
-        raise KernelError(f"shared_attention: kv_pool is {kv_pool.dtype} {tuple(kv_pool.shape)}, expected {plan.dtype} [pages, {', '.join(map(str, page))}]")
+    if kv_pool.dtype != plan.dtype or kv_pool.shape[1:] != plan.page_shape or not kv_pool.is_contiguous():
+        raise KernelError(f"shared_attention: kv_pool is {kv_pool.dtype} {tuple(kv_pool.shape)}, expected {plan.dtype} [pages, {', '.join(map(str, plan.page_shape))}]")
     if sink_weight is not None and (sink_weight.dtype != torch.float32 or sink_weight.numel() != nh or not sink_weight.is_contiguous()):
         raise KernelError("shared_attention: the sink's scores are contiguous float32, one per query head")
     if max_position < 0 or softcap < 0.0:
@@ -972,35 +989,21 @@ def _shared_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_table: torch
     if T == 0:
         return
     _here("shared_attention", q, kv_pool, block_table, positions, plan.buffer, out, sink_weight, status)
-    sink, L, num_pages = 1 if sink or sink_weight is not None else 0, lib(), kv_pool.shape[0]
-    if plan.kernel == "generic":
-        n_splits = max_position // plan.split + 1
-        at_once = max(plan.slots, n_splits - plan.least_own, 1)
-        at_once = min(at_once, n_splits)
-        part = torch.empty(T * nh * n_splits * (vd + 2), dtype=torch.float32, device=q.device)
-        part_o, part_ml = part[:T * nh * n_splits * vd], part[T * nh * n_splits * vd:]
-        _check(L.bg_attention_shared_partial(
-            _p(q), _dt(q), q.stride(0), _p(kv_pool), _dt(kv_pool), num_pages, plan.page_size, _p(block_table), block_table.shape[1], _p(positions),
-            _p(plan.items), plan.n_items, _p(plan.rows), _p(part_o), _p(part_ml), n_splits, at_once, nh, nkv, hd, vd, plan.split, plan.tile, plan.bq,
-            float(scale), float(softcap), _p(status), _stream()), "attention_shared_partial")
-        _check(L.bg_attention_merge(_p(part_o), _p(part_ml), _p(positions), _p(out), _dt(out), out.stride(0), T, nh, vd, n_splits, plan.split, 0, sink,
-                                    _p(sink_weight), 0, _stream()), "attention_merge")
-        return
-    if status is None or out.dtype != torch.bfloat16:
-        raise KernelError("shared_attention: the tensor-core kernels want a status word and write bfloat16")
-    n_own = decode_splits(T * nkv, max(1, max_position + 1 - plan.least_own))
-    slots = plan.slots + n_own
-    part = torch.empty(T * nh * slots * (hd + 2), dtype=torch.float32, device=q.device)
-    part_o, part_ml = part.data_ptr(), part.data_ptr() + T * nh * slots * hd * 4
-    if plan.n_items:
-        _check(L.bg_attention_tc_shared(_p(q), q.stride(0), _p(kv_pool), num_pages, plan.page_size, _p(block_table), block_table.shape[1], _p(positions),
-                                        _p(plan.items), plan.n_items, _p(plan.rows), part_o, part_ml, slots, nh, nkv, hd, float(scale), float(softcap),
-                                        _p(status), _stream()), "attention_tcgen05_shared")
-    _check(L.bg_attention_mma_own(_p(q), q.stride(0), _p(kv_pool), num_pages, plan.page_size, _p(block_table), block_table.shape[1], _p(positions),
-                                  _p(plan.own_first), T, part_o, part_ml, slots, plan.slots, n_own, nh, nkv, hd, float(scale), float(softcap), _p(status),
-                                  _stream()), "attention_mma_own")
-    _check(L.bg_attention_shared_merge(part_o, part_ml, _p(positions), _p(plan.own_first), _p(plan.parts), T, nh, hd, slots, plan.slots, n_own, sink,
-                                       _p(sink_weight), _p(out), out.stride(0), _stream()), "attention_shared_merge")
+    if plan.kernel == "tc":
+        if status is None or out.dtype != torch.bfloat16:
+            raise KernelError("shared_attention: the tensor-core kernels want a status word and write bfloat16")
+        ranges, at_once = decode_splits(T * plan.nkv, max(1, max_position + 1 - plan.least_own), plan.sms), 0
+        floats, kernels = T * nh * (plan.slots + ranges) * (vd + 2), 3
+    else:
+        ranges, kernels = max_position // plan.split + 1, 2
+        at_once = min(ranges, max(plan.slots, ranges - plan.least_own, 1))
+        floats = T * nh * ranges * (vd + 2)
+    scratch = torch.empty(floats, dtype=torch.float32, device=q.device)
+    step = SharedAttnStep(q.data_ptr(), kv_pool.data_ptr(), block_table.data_ptr(), positions.data_ptr(), out.data_ptr(), _p(sink_weight), _p(status),
+                          scratch.data_ptr(), floats, q.stride(0), out.stride(0), block_table.shape[1], kv_pool.shape[0], ranges, at_once,
+                          1 if sink or sink_weight is not None else 0, _dt(out), scale, softcap)
+    _check(lib().bg_shared_attention(plan._args, ctypes.byref(step), _stream()), "shared_attention")
+    count_launches(kernels - 1)
 
 
 # ------------------------------------------------------------------------------------------------
