@@ -75,12 +75,17 @@ struct AttnMmaExtParams : AttnMmaParams {
 // What the SHARED instances take besides: a row's first position that is its request's own (the ones before are attention_tcgen05.cu's).
 struct AttnMmaSharedParams : AttnMmaParams {
     const int* own_first;   // [T]
+    int ahead_done;         // the kernel ahead is the shared positions': the queries are there when this one begins
 };
 template <bool EXT, bool SHARED> struct AmParams { using type = AttnMmaParams; };
 template <> struct AmParams<true, false> { using type = AttnMmaExtParams; };
 template <> struct AmParams<false, true> { using type = AttnMmaSharedParams; };
 __device__ __forceinline__ int am_own_first(const AttnMmaParams&, int) { return 0; }
 __device__ __forceinline__ int am_own_first(const AttnMmaSharedParams& p, int row) { return p.own_first[row]; }
+// The wait for the kernel that made the queries.  The shared positions' kernel lets this one begin only when it has waited for that itself (its results are
+// another's to wait for: this kernel waits for it at the end).
+__device__ __forceinline__ void am_wait(const AttnMmaParams&) { pdl_wait(); }
+__device__ __forceinline__ void am_wait(const AttnMmaSharedParams& p) { if (!p.ahead_done) pdl_wait(); }
 __device__ __forceinline__ int am_keep(const AttnMmaParams&) { return 0; }
 __device__ __forceinline__ int am_keep(const AttnMmaExtParams& p) { return p.keep; }
 __device__ __forceinline__ const float* am_slopes(const AttnMmaParams&) { return nullptr; }
@@ -235,7 +240,7 @@ attention_mma_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_co
     __syncthreads();                           // table_s and the barriers are ready (and q_s, rows arrangement)
     auto compute_sync = [] { asm volatile("bar.sync 1, %0;\n" ::"n"(AM_THREADS) : "memory"); };   // the four computing warps
     if (BY_KEYS && warp < AM_THREADS / 32) {
-        pdl_wait();                            // the queries come from the kernel before this one
+        am_wait(p);                            // the queries come from the kernel before this one
         load_queries(tid, AM_THREADS);
         compute_sync();
     }
@@ -261,7 +266,7 @@ attention_mma_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_co
         const int n_early = BY_KEYS ? min(AM_STAGES, k_end == pos_last + 1 ? n_stage - 1 : n_stage) : 0;
         int next_page = page_of(0, p.whole_pages ? lane * PER_PAGE : lane);
         for (int s = 0; s < n_stage; ++s) {
-            if (BY_KEYS && s == n_early) pdl_wait();
+            if (BY_KEYS && s == n_early) am_wait(p);
             const int buf = s % AM_STAGES;
             int page = next_page;
             next_page = page_of(s + 1, p.whole_pages ? lane * PER_PAGE : lane);   // fetched while this stage's copies go out
@@ -659,6 +664,7 @@ attention_mma_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_co
     if (!p.use_tma && !BY_KEYS) cp_async_wait<0>();
 
     // ---- write the partial results
+    if constexpr (SHARED) pdl_wait();      // (what comes behind waits for this kernel, and with it for the shared positions')
     if (direct) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -773,7 +779,7 @@ template <int HD, bool SWAP>
 static int am_launch_own(const CUtensorMap& map, const CUtensorMap& map5, const AttnMmaSharedParams& p, int T, int n_splits, cudaStream_t stream) {
     auto kern = attention_mma_kernel<HD, true, AM_THREADS / 32, SWAP, false, true>;
     const size_t smem = am_smem_bytes<HD, true, AM_THREADS / 32>();
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    cudaError_t e = smem_limit(kern, smem);
     if (e != cudaSuccess) return (int)e;
     e = launch(kern, dim3(T, p.nkv, n_splits), dim3(AM_ALL), smem, stream, map, map5, p);
     return e == cudaSuccess ? BG_OK : (int)e;
@@ -849,10 +855,10 @@ extern "C" int bg_attention_mma_partial(const void* q, int q_stride, const void*
 
 // The partial results of T single tokens (row r of request r) over the positions from own_first[r] to their own, spread over n_splits ranges a row
 // (those of keys_per_split over the row's own positions): at slot first_slot + range of part_o [T][nh][slots][hd] and part_ml [T][nh][slots][2].  A row
-// without positions of its own writes nothing.
+// without positions of its own writes nothing.  ahead_done: the launch ahead on the stream is bg_attention_tc_shared's.
 extern "C" int bg_attention_mma_own(const void* q, int q_stride, const void* kv_pool, int num_pages, int page_size, const int* block_table, int max_pages,
                                     const int* positions, const int* own_first, int T, float* part_o, float* part_ml, int slots, int first_slot, int n_splits,
-                                    int nh, int nkv, int hd, float scale, float softcap, unsigned* status, cudaStream_t stream) {
+                                    int nh, int nkv, int hd, float scale, float softcap, int ahead_done, unsigned* status, cudaStream_t stream) {
     if (T <= 0 || n_splits <= 0) return BG_OK;
     if (nkv <= 0 || nh % nkv != 0 || page_size <= 0 || first_slot < 0 || first_slot + n_splits > slots || n_splits > 65535 || nkv > 65535) return BG_ERR_SHAPE;
     if ((q_stride % 8) != 0 || ((uintptr_t)q % 16) != 0 || ((uintptr_t)kv_pool % 16) != 0) return BG_ERR_ALIGN;
@@ -866,7 +872,7 @@ extern "C" int bg_attention_mma_own(const void* q, int q_stride, const void* kv_
     p.positions = positions; p.max_splits = slots; p.nh = nh; p.nkv = nkv; p.group = nh / nkv; p.scale_log2 = scale * AM_LOG2E; p.status = status;
     p.part_o = part_o + (size_t)first_slot * hd; p.part_ml = part_ml + (size_t)first_slot * 2;
     p.cap_log2 = softcap > 0.0f ? softcap * AM_LOG2E : 0.0f; p.scale_over_cap = softcap > 0.0f ? scale / softcap : 0.0f;
-    p.own_first = own_first;
+    p.own_first = own_first; p.ahead_done = ahead_done;
     CUtensorMap map, map5;
     memset(&map, 0, sizeof(map));
     memset(&map5, 0, sizeof(map5));

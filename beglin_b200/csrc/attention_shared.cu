@@ -26,39 +26,41 @@ struct SharedAttnStep {
 
 namespace bg {
 
-// A warp takes one (row, head); a lane takes four neighbouring features, HD / 4 lanes a slot, so that a warp reads 128 / HD slots at once.  Sums go in
-// the order of the slots.
-constexpr int SM_WARPS = 4;
-template <int HD>
-__global__ void __launch_bounds__(32 * SM_WARPS)
+// WARPS warps take one (row, head), a lane four neighbouring features; warp w joins the slots w, w + WARPS, ...
+// eight at a time, all on their way together, and the warps' results are joined in their order.  Which slots a warp takes hangs on the slots' numbers alone.
+constexpr int SM_THREADS = 256;
+template <int HD, int WARPS>
+__global__ void __launch_bounds__(SM_THREADS)
 attention_shared_merge_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml, const int* __restrict__ positions,
                               const int* __restrict__ own_first, const int* __restrict__ shared_slots, int T, int nh, int slots, int first_slot,
                               int n_own, const float* __restrict__ sink_w, int sink, __nv_bfloat16* __restrict__ out, int out_stride) {
-    constexpr int AT_ONCE = 8;
+    constexpr int AT_ONCE = 8, GROUPS = SM_THREADS / 32 / WARPS;       // (row, head) pairs of a CTA
+    __shared__ float4 acc_s[WARPS > 1 ? SM_THREADS / 32 : 1][32];
+    __shared__ float2 ml_s[WARPS > 1 ? SM_THREADS / 32 : 1];
     pdl_launch();
-    const int w = blockIdx.x * SM_WARPS + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp % WARPS;
+    const int w = blockIdx.x * GROUPS + warp / WARPS;
     const bool idle = w >= T * nh;
     const int t = idle ? 0 : w / nh, h = w - t * nh;
     const int n_shared = shared_slots[t];
     const int own = positions[t] + 1 - own_first[t];
-    const int ranges = own > 0 ? (own + keys_per_split(0, own, n_own) - 1) / keys_per_split(0, own, n_own) : 0;
-    const int n = n_shared + ranges;
+    const int range = keys_per_split(0, own, n_own);
+    const int n = idle ? 0 : n_shared + (own > 0 ? (own + range - 1) / range : 0);
     pdl_wait();
-    if (idle) return;
     const size_t base = (size_t)w * slots;
-    auto slot_of = [&](int i) { return base + (i < n_shared ? i : first_slot + i - n_shared); };
     const int d = lane * 4;
     float m = -INFINITY, l = 0.0f;
-    if (sink) { m = sink_w ? sink_w[h] : 0.0f; l = 1.0f; }
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int i0 = 0; i0 < n; i0 += AT_ONCE) {
+    for (int i0 = part; i0 < n; i0 += AT_ONCE * WARPS) {
         float2 ml[AT_ONCE];
         float4 v[AT_ONCE];
 #pragma unroll
         for (int j = 0; j < AT_ONCE; ++j) {
-            const bool have = i0 + j < n;
-            ml[j] = have ? *reinterpret_cast<const float2*>(part_ml + slot_of(i0 + j) * 2) : make_float2(-INFINITY, 0.0f);
-            v[j] = have && d < HD ? *reinterpret_cast<const float4*>(part_o + slot_of(i0 + j) * HD + d) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            const int i = i0 + j * WARPS;
+            const bool have = i < n;
+            const size_t slot = base + (i < n_shared ? i : first_slot + i - n_shared);
+            ml[j] = have ? *reinterpret_cast<const float2*>(part_ml + slot * 2) : make_float2(-INFINITY, 0.0f);
+            v[j] = have && d < HD ? *reinterpret_cast<const float4*>(part_o + slot * HD + d) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         }
         float top = m;
 #pragma unroll
@@ -74,9 +76,34 @@ attention_shared_merge_kernel(const float* __restrict__ part_o, const float* __r
             acc.x = fmaf(v[j].x, f, acc.x); acc.y = fmaf(v[j].y, f, acc.y); acc.z = fmaf(v[j].z, f, acc.z); acc.w = fmaf(v[j].w, f, acc.w);
         }
     }
-    if (d >= HD) return;
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;      // (a row that sees nothing is nought)
-    const __nv_bfloat162 x = __floats2bfloat162_rn(acc.x * inv, acc.y * inv), y = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
+    if constexpr (WARPS > 1) {
+        acc_s[warp][lane] = acc;
+        if (lane == 0) ml_s[warp] = make_float2(m, l);
+        __syncthreads();
+        if (part) return;
+    }
+    if (idle || d >= HD) return;
+    const float sv = sink && sink_w ? sink_w[h] : 0.0f;
+    float top = sink ? fmaxf(m, sv) : m;
+    if constexpr (WARPS > 1) {
+#pragma unroll
+        for (int j = 1; j < WARPS; ++j) top = fmaxf(top, ml_s[warp + j].x);
+    }
+    const float f0 = m == -INFINITY ? 0.0f : expf(m - top);
+    float sum = fmaf(l, f0, sink ? expf(sv - top) : 0.0f);
+    float4 o = make_float4(acc.x * f0, acc.y * f0, acc.z * f0, acc.w * f0);
+    if constexpr (WARPS > 1) {
+#pragma unroll
+        for (int j = 1; j < WARPS; ++j) {
+            const float2 ml = ml_s[warp + j];
+            const float4 v = acc_s[warp + j][lane];
+            const float f = ml.x == -INFINITY ? 0.0f : expf(ml.x - top);
+            sum = fmaf(ml.y, f, sum);
+            o.x = fmaf(v.x, f, o.x); o.y = fmaf(v.y, f, o.y); o.z = fmaf(v.z, f, o.z); o.w = fmaf(v.w, f, o.w);
+        }
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;          // (a row that sees nothing is nought)
+    const __nv_bfloat162 x = __floats2bfloat162_rn(o.x * inv, o.y * inv), y = __floats2bfloat162_rn(o.z * inv, o.w * inv);
     *reinterpret_cast<uint2*>(out + (size_t)t * out_stride + (size_t)h * HD + d) =
         make_uint2(*reinterpret_cast<const unsigned*>(&x), *reinterpret_cast<const unsigned*>(&y));
 }
@@ -90,10 +117,12 @@ static int shared_merge(const float* part_o, const float* part_ml, const int* po
                         int first_slot, int n_own, int sink, const float* sink_w, void* out, int out_stride, cudaStream_t stream) {
     if (first_slot + n_own > slots || (long long)T * nh > 0x7fffffff - 64) return BG_ERR_SHAPE;
     if (out_stride % 4 || (uintptr_t)out % 8) return BG_ERR_ALIGN;
-    const dim3 grid((unsigned)(((long long)T * nh + SM_WARPS - 1) / SM_WARPS)), block(32 * SM_WARPS);
-    auto kern = hd == 128 ? attention_shared_merge_kernel<128> : attention_shared_merge_kernel<64>;
-    cudaError_t e = launch(kern, grid, block, 0, stream, part_o, part_ml, positions, own_first, parts, T, nh, slots, first_slot, n_own, sink_w, sink,
-                           (__nv_bfloat16*)out, out_stride);
+    // more warps to a (row, head) where slots are many and rows few
+    const int warps = slots > 8 ? 4 : 1, groups = SM_THREADS / 32 / warps;
+    auto kern = hd == 128 ? (warps > 1 ? attention_shared_merge_kernel<128, 4> : attention_shared_merge_kernel<128, 1>)
+                          : (warps > 1 ? attention_shared_merge_kernel<64, 4> : attention_shared_merge_kernel<64, 1>);
+    cudaError_t e = launch(kern, dim3((unsigned)(((long long)T * nh + groups - 1) / groups)), dim3(SM_THREADS), 0, stream, part_o, part_ml, positions, own_first,
+                           parts, T, nh, slots, first_slot, n_own, sink_w, sink, (__nv_bfloat16*)out, out_stride);
     return e == cudaSuccess ? BG_OK : (int)e;
 }
 
@@ -123,7 +152,7 @@ extern "C" int bg_shared_attention(const SharedAttnArgs* args, const SharedAttnS
                                     part_ml, slots, a.nh, a.nkv, a.hd, s.scale, s.softcap, s.status, stream);
     if (rc == BG_OK)
         rc = bg_attention_mma_own(s.q, s.q_stride, s.pool, s.num_pages, a.page_size, s.table, s.max_pages, s.positions, a.own_first, a.T, part_o, part_ml, slots,
-                                  a.slots, s.ranges, a.nh, a.nkv, a.hd, s.scale, s.softcap, s.status, stream);
+                                  a.slots, s.ranges, a.nh, a.nkv, a.hd, s.scale, s.softcap, a.n_items > 0, s.status, stream);
     if (rc == BG_OK)
         rc = shared_merge(part_o, part_ml, s.positions, a.own_first, a.parts, a.T, a.nh, a.hd, slots, a.slots, s.ranges, s.sink, s.sink_w, s.out, s.out_stride,
                           stream);

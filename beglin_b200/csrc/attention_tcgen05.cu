@@ -73,8 +73,8 @@ struct AttnTcDiffParams : AttnTcParams {
 };
 // What the SHARED instances take besides, in place of query blocks and an output.
 struct AttnTcSharedParams : AttnTcParams {
-    const int* items;           // [n][8] = (request whose pages, first entry of `rows`, entries, first position, end, slot of the result, 0, 0)
-    const int* rows;            // rows of the batch, those of a block side by side
+    const int* items;           // [n][8] = (request whose pages, first row, rows, first position, end, slot of the result, 0, 0)
+    const int* rows;            // rows of the batch, those of a group side by side; an item's row i is head i % group of rows[i / group]
     float* part_o;              // [rows][nh][slots][HD] unnormalised outputs
     float* part_ml;             // [rows][nh][slots][2] maximum (of scores as they are), sum
     int slots;
@@ -108,14 +108,17 @@ __device__ __forceinline__ float at_squash(float x, float cap_log2, float cap_k)
 // keys and values is fetched once for both.  At the end the maps are not joined but subtracted, and the difference is normed:
 // out = o / sqrt(mean(o^2) + eps) * out_scale with o = O_0 / l_0 - lambda O_1 / l_1, the first `vd` of the HD features stored.
 // A stage of the rings serves two turns, so its release has barriers of its own (k_free, v_free).
-// SHARED: the rows are single tokens of several requests whose first positions lie in the same pages: a block is up to 128 rows (requests x query
+// SHARED: the rows are single tokens of several requests whose first positions lie in the same pages: a block is up to 256 rows (requests x query
 // heads of a kv head) over one range of those positions, and its result is partial: unnormalised sums with the rows' maxima and sums, which
-// attention_shared.cu joins with those of the other ranges and of each request's own positions.  A row sees the positions up to its own.
+// attention_shared.cu joins with those of the other ranges and of each request's own positions.  A row sees the positions up to its own.  More than 128
+// rows are two tiles of rows, and the two groups of softmax warps take one each, as the maps of DIFF: a tile of keys and values is fetched once for
+// both (256 rows of 28 heads over 32,768 positions are bound by what the L2 delivers with 128 rows a CTA: 7.1 TB/s).
 template <int HD, int AT_BK, bool SINK = false, bool EXT = false, bool DIFF = false, bool SHARED = false>
 __global__ void __launch_bounds__(AT_THREADS)
 attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename AtParams<DIFF, SHARED>::type p) {
     static_assert(!DIFF || (AT_BK == 64 && !SINK && !EXT), "the two maps take tiles of 64 keys in turns");
     static_assert(!SHARED || (AT_BK == 64 && !SINK && !EXT && !DIFF), "partial results of tiles of 64 keys");
+    constexpr bool MAY_TWICE = DIFF || SHARED;           // a tile of keys may be taken twice, by one softmax group and then by the other
     constexpr int AT_HALF = AT_BK / 2, AT_STAGES = 256 / AT_BK;
     constexpr int NSB = AT_STAGES;                       // score buffers in tensor memory: tiles whose scores may be under way
     // How the two groups of softmax warps share the keys.  Tiles of 128 keys: every tile is cut in two halves, one for
@@ -125,7 +128,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
     constexpr bool ALT = AT_BK == 64;
     constexpr int GK = ALT ? AT_BK : AT_HALF;            // keys of a tile that one group takes
     constexpr int CB = HD / 64;                          // 64-feature column blocks of a row
-    constexpr int Q_BYTES = CB * AT_BM * 128;
+    constexpr int QT_BYTES = CB * AT_BM * 128, Q_BYTES = (SHARED ? 2 : 1) * QT_BYTES;
     constexpr int KV_BLOCK = AT_BK * 128;                // one column block of a key or value tile
     constexpr int KV_BYTES = CB * KV_BLOCK;
     // tensor memory: S in NSB buffers of AT_BK columns, 256 in all (the first half of a buffer's columns are the first
@@ -146,10 +149,10 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
     // overwritten, the softmax warps that O may be rescaled, and the value loader that the stage is free.
     __shared__ __align__(8) unsigned long long k_full[AT_STAGES], v_full[AT_STAGES], kv_landed[AT_STAGES];
     __shared__ __align__(8) unsigned long long s_full[NSB], p_full[2 * NSB], pv_done[NSB], o_ready;    // p_full: [2 buffer + group]
-    __shared__ __align__(8) unsigned long long k_free[DIFF ? AT_STAGES : 1], v_free[DIFF ? AT_STAGES : 1];
+    __shared__ __align__(8) unsigned long long k_free[MAY_TWICE ? AT_STAGES : 1], v_free[MAY_TWICE ? AT_STAGES : 1];
     __shared__ float2 ml_other[AT_BM];                   // the second group's running maximum and sum of every row, for the join
     __shared__ float2 ml_first[SHARED ? AT_BM : 1];      // and the first one's, where both groups write
-    __shared__ int row_of[SHARED ? AT_BM : 1];
+    __shared__ int row_of[SHARED ? 2 * AT_BM : 1];
     __shared__ unsigned tmem_sh;
     __shared__ int failed;
 
@@ -169,7 +172,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
         for (int b = 0; b < NSB; ++b) { mbar_init(&s_full[b], 1); mbar_init(&pv_done[b], 1); }
         for (int b = 0; b < 2 * NSB; ++b) mbar_init(&p_full[b], 4);       // one arrival per softmax warp of a group
         mbar_init(&o_ready, 1);
-        if constexpr (DIFF) {
+        if constexpr (MAY_TWICE) {
             for (int s = 0; s < AT_STAGES; ++s) { mbar_init(&k_free[s], 1); mbar_init(&v_free[s], 1); }
         }
         failed = 0;
@@ -184,7 +187,8 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
     if constexpr (SHARED) { req = p.items[qb * 8 + 0]; row0 = p.items[qb * 8 + 1]; nq = p.items[qb * 8 + 2]; }
     else { req = p.qblk[qb * 3 + 0]; row0 = p.qblk[qb * 3 + 1]; nq = p.qblk[qb * 3 + 2]; }
     const int group = p.group;
-    const int n_rows = nq * group;                       // <= 128
+    const int n_rows = SHARED ? nq : nq * group;         // <= 128 (SHARED: 256)
+    const bool twice = DIFF || (SHARED && n_rows > AT_BM);
     int pos_first, k_begin, k_end;
     if constexpr (SHARED) {
         pos_first = 0; k_begin = p.items[qb * 8 + 3]; k_end = p.items[qb * 8 + 4];
@@ -194,25 +198,25 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
         k_begin = first_visible(pos_first, p.window);
         k_end = pos_last + 1;
     }
-    // the batch's row of the block's entry qi
-    auto batch_row = [&](int qi) { if constexpr (SHARED) return p.rows[row0 + qi]; else return row0 + qi; };
+    // the batch's row of the block's row r, and its head within the group
+    auto batch_row = [&](int r) { if constexpr (SHARED) return p.rows[(row0 + r) / group]; else return row0 + r / group; };
+    auto head_of = [&](int r) { if constexpr (SHARED) return (row0 + r) % group; else return r % group; };
     const int keep = EXT ? p.keep : 0;
     const int n_kept = EXT ? (min(keep, k_end) + AT_BK - 1) / AT_BK : 0;         // tiles with kept positions
     const int tile0 = EXT ? max(k_begin / AT_BK, n_kept) : k_begin / AT_BK;      // the window's first tile behind those
     const int n_tiles = EXT ? n_kept + max((k_end + AT_BK - 1) / AT_BK - tile0, 0) : (k_end + AT_BK - 1) / AT_BK - tile0;
-    const int n_turns = DIFF ? 2 * n_tiles : n_tiles;            // a turn: one score product and one softmax group's share of a tile
+    const int n_turns = twice ? 2 * n_tiles : n_tiles;            // a turn: one score product and one softmax group's share of a tile
     auto tile_key = [&](int i) { return (EXT && i < n_kept ? i : tile0 + i - n_kept) * AT_BK; };
 
     // ---- Q into shared memory: row r, column block cb, 16-byte piece c at r*128 + ((c ^ (r & 7)) * 16)
-    for (int idx = tid; idx < AT_BM * (HD / 8); idx += AT_THREADS) {
+    for (int idx = tid; idx < (SHARED && twice ? 2 : 1) * AT_BM * (HD / 8); idx += AT_THREADS) {
         const int r = idx / (HD / 8), c = idx - r * (HD / 8);
         uint4 v = make_uint4(0, 0, 0, 0);
-        if (r < n_rows) {
-            const int qi = r / group, g = r - qi * group;
-            v = *reinterpret_cast<const uint4*>(p.q + (size_t)batch_row(qi) * p.q_stride + (size_t)(kvh * group + g) * HD + c * 8);
-        }
+        if (r < n_rows)
+            v = *reinterpret_cast<const uint4*>(p.q + (size_t)batch_row(r) * p.q_stride + (size_t)(kvh * group + head_of(r)) * HD + c * 8);
         const int cb = c >> 3, cc = c & 7;
-        *reinterpret_cast<uint4*>(q_s + cb * (AT_BM * 128) + r * 128 + ((cc ^ (r & 7)) << 4)) = v;
+        const int rr = SHARED ? r & (AT_BM - 1) : r;
+        *reinterpret_cast<uint4*>(q_s + (SHARED ? (r / AT_BM) * QT_BYTES : 0) + cb * (AT_BM * 128) + rr * 128 + ((cc ^ (rr & 7)) << 4)) = v;
     }
     fence_proxy_async();
     tc_fence_before();
@@ -241,7 +245,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
             // scores: S[b] = Q K(i)^T as soon as the keys have landed and both groups' P of the buffer's last tile
             // have been used up
             for (int i = 0; i < n_turns && ok; ++i) {
-                const int tile = DIFF ? i >> 1 : i, map = DIFF ? i & 1 : 0;
+                const int tile = twice ? i >> 1 : i, map = twice ? i & 1 : 0;
                 const int st = tile % AT_STAGES, b = i % NSB;
                 // (which of the two waits comes first is measured: with four score buffers the older event, the
                 // buffer's release, first: 234 -> 227 us at 8,192 tokens; with two buffers the keys first: 812
@@ -272,10 +276,11 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
 #pragma unroll
                         for (int ks = 0; ks < HD / 16; ++ks) {
                             const unsigned off = (ks & 3) * 32;
-                            tc_mma(tmem + (unsigned)b * AT_BK, smem_desc_sw128(q_addr + (ks >> 2) * (AT_BM * 128) + off),
+                            tc_mma(tmem + (unsigned)b * AT_BK, smem_desc_sw128(q_addr + (SHARED ? map * QT_BYTES : 0) + (ks >> 2) * (AT_BM * 128) + off),
                                    smem_desc_sw128(k_addr + (ks >> 2) * KV_BLOCK + off), idesc_qk, ks > 0 ? 1u : 0u);
                         }
                         tc_commit(&s_full[b]);
+                        if (SHARED && map == 1) tc_commit(&k_free[st]);
                     }
                 }
                 __syncwarp();
@@ -283,9 +288,9 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
         } else {
             // values: O[g] += P(i, g) V(i, g) once group g's softmax warps have written their half of P
             for (int i = 0; i < n_turns && ok; ++i) {
-                const int tile = DIFF ? i >> 1 : i;
+                const int tile = twice ? i >> 1 : i;
                 const int st = tile % AT_STAGES, b = i % NSB;
-                if (!DIFF || (i & 1) == 0) ok = wait_all(&v_full[st], (tile / AT_STAGES) & 1);
+                if (!twice || (i & 1) == 0) ok = wait_all(&v_full[st], (tile / AT_STAGES) & 1);
                 const unsigned v_addr = smem_u32(v_s + st * KV_BYTES);
                 if constexpr (ALT) {
                     const int g = i & 1;
@@ -298,7 +303,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
                             tc_mma_ts(tmem + O_COL + 128u * (unsigned)g, tmem + (unsigned)b * AT_BK + (unsigned)ks * 8,
                                       smem_desc_sw128_nmajor(v_addr + ks * 2048, KV_BLOCK, 1024), idesc_pv, (i >= 2 || ks > 0) ? 1u : 0u);
                         tc_commit(&pv_done[b]);
-                        if (DIFF && g == 1) tc_commit(&v_free[st]);
+                        if (MAY_TWICE && twice && g == 1) tc_commit(&v_free[st]);
                     }
                     __syncwarp();
                 } else {
@@ -330,8 +335,9 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
         const int quarter = warp & 3;                    // the tensor-memory lanes this warp may touch
         const int r = quarter * 32 + lane;
         const unsigned lane_addr = (unsigned)(quarter * 32) << 16;
-        const bool real = r < n_rows;
-        const int own_row = real ? batch_row(r / group) : 0;
+        const int block_row = SHARED && twice ? grp * AT_BM + r : r;
+        const bool real = block_row < n_rows;
+        const int own_row = SHARED && real ? batch_row(block_row) : 0;
         const int pos = !real ? -1 : SHARED ? min(p.positions[own_row], k_end - 1) : pos_first + r / group;
         const int lo = real && !SHARED ? first_visible(pos, p.window) : 0;
         const int warp_pos_min = __reduce_min_sync(0xffffffffu, real ? pos : 0x7fffffff);
@@ -345,7 +351,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
         for (int i = i_first; i < n_turns && ok; i += (ALT ? 2 : 1)) {
             const int b = i % NSB;
             const unsigned s_col = (unsigned)b * AT_BK + (ALT ? 0u : (unsigned)grp * AT_HALF);    // this group's scores of the tile, and its P
-            const int key0 = tile_key(DIFF ? i >> 1 : i) + (ALT ? 0 : grp * AT_HALF);
+            const int key0 = tile_key(twice ? i >> 1 : i) + (ALT ? 0 : grp * AT_HALF);
             ok = mbar_wait(&s_full[b], (i / NSB) & 1);
             if (!ok) break;
             tc_fence_after();
@@ -465,40 +471,48 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
                 }
             }
         } else if constexpr (SHARED) {
-            // both accumulators through the keys' ring (its products are complete) into whole rows of the partial results; a group takes
-            // half of the features
+            // the accumulators through the room of the queries and keys (all products are complete) into whole rows of the partial results
             constexpr int LD = HD + 4;
-            float* stage = reinterpret_cast<float*>(k_s);
-            const float2 first = ml_first[r], other = ml_other[r];
-            const float m_all = fmaxf(first.x, other.x), m_ref = (m_all == -INFINITY) ? 0.0f : m_all;
-            const float a0 = at_ex2(first.x - m_ref), a1 = at_ex2(other.x - m_ref);
-            const bool has1 = n_tiles > 1;               // with one tile the second group's accumulator was never written
+            const int slot = p.items[qb * 8 + 5];
+            float* stage = reinterpret_cast<float*>(q_s) + (twice ? grp * AT_BM * LD : 0);
+            int* place = row_of + (twice ? grp * AT_BM : 0);
             tc_fence_after();
+            if (twice || grp == 0) place[r] = real ? own_row * p.nh + kvh * group + head_of(block_row) : 0;
+            float2 ml = make_float2(m, l);
+            if (twice) {
 #pragma unroll
-            for (int c0 = 0; c0 < HD / 2; c0 += 32) {
-                const int c = grp * (HD / 2) + c0;
-                float t[32], u[32];
-                tc_ld32(tmem + lane_addr + O_COL + c, t);
-                tc_ld32(tmem + lane_addr + O_COL + 128u + c, u);
+                for (int c = 0; c < HD; c += 32) {
+                    float t[32];
+                    tc_ld32(tmem + lane_addr + o_col + c, t);
 #pragma unroll
-                for (int q = 0; q < 32; q += 4)
-                    *reinterpret_cast<float4*>(stage + r * LD + c + q) =
-                        make_float4(t[q] * a0 + (has1 ? u[q] * a1 : 0.0f), t[q + 1] * a0 + (has1 ? u[q + 1] * a1 : 0.0f),
-                                    t[q + 2] * a0 + (has1 ? u[q + 2] * a1 : 0.0f), t[q + 3] * a0 + (has1 ? u[q + 3] * a1 : 0.0f));
-            }
-            if (grp == 0) {
-                row_of[r] = real ? (own_row * p.nh + kvh * group + r % group) : 0;
-                if (real) {
-                    const size_t at = ((size_t)row_of[r] * p.slots + p.items[qb * 8 + 5]) * 2;
-                    // (a wait that ran out: the row shows it)
-                    *reinterpret_cast<float2*>(p.part_ml + at) = make_float2(m_all * 0.6931471805599453f, ok ? first.y * a0 + other.y * a1 : NAN);
+                    for (int q = 0; q < 32; q += 4) *reinterpret_cast<float4*>(stage + r * LD + c + q) = make_float4(t[q], t[q + 1], t[q + 2], t[q + 3]);
                 }
+            } else {                                     // both groups' accumulators together, a group half of the features
+                const float2 first = ml_first[r], other = ml_other[r];
+                const float m_all = fmaxf(first.x, other.x), m_ref = (m_all == -INFINITY) ? 0.0f : m_all;
+                const float a0 = at_ex2(first.x - m_ref), a1 = at_ex2(other.x - m_ref);
+                const bool has1 = n_tiles > 1;           // with one tile the second group's accumulator was never written
+#pragma unroll
+                for (int c0 = 0; c0 < HD / 2; c0 += 32) {
+                    const int c = grp * (HD / 2) + c0;
+                    float t[32], u[32];
+                    tc_ld32(tmem + lane_addr + O_COL + c, t);
+                    tc_ld32(tmem + lane_addr + O_COL + 128u + c, u);
+#pragma unroll
+                    for (int q = 0; q < 32; q += 4)
+                        *reinterpret_cast<float4*>(stage + r * LD + c + q) =
+                            make_float4(t[q] * a0 + (has1 ? u[q] * a1 : 0.0f), t[q + 1] * a0 + (has1 ? u[q + 1] * a1 : 0.0f),
+                                        t[q + 2] * a0 + (has1 ? u[q + 2] * a1 : 0.0f), t[q + 3] * a0 + (has1 ? u[q + 3] * a1 : 0.0f));
+                }
+                ml = make_float2(m_all, first.y * a0 + other.y * a1);
             }
+            if (real && (twice || grp == 0))             // (a wait that ran out: the row shows it)
+                *reinterpret_cast<float2*>(p.part_ml + ((size_t)place[r] * p.slots + slot) * 2) = make_float2(ml.x * 0.6931471805599453f, ok ? ml.y : NAN);
             asm volatile("bar.sync 1, 256;\n" ::: "memory");
-            const int slot = p.items[qb * 8 + 5], w = grp * 4 + quarter;
-            for (int i = w * (128 / HD) + (lane * 4) / HD; i < n_rows; i += 8 * (128 / HD)) {
+            const int w = twice ? quarter : grp * 4 + quarter, n_warps = twice ? 4 : 8, count = twice ? min(n_rows - grp * AT_BM, AT_BM) : n_rows;
+            for (int i = w * (128 / HD) + (lane * 4) / HD; i < count; i += n_warps * (128 / HD)) {
                 const int d = (lane * 4) % HD;
-                *reinterpret_cast<float4*>(p.part_o + ((size_t)row_of[i] * p.slots + slot) * HD + d) = *reinterpret_cast<const float4*>(stage + i * LD + d);
+                *reinterpret_cast<float4*>(p.part_o + ((size_t)place[i] * p.slots + slot) * HD + d) = *reinterpret_cast<const float4*>(stage + i * LD + d);
             }
         } else if (grp == 0 && ok && n_tiles > 0) {
             tc_fence_after();
@@ -540,7 +554,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
         const int lsub = warp >= 12;
         unsigned char* ring = which ? v_s : k_s;
         unsigned long long* full = which ? v_full : k_full;
-        unsigned long long* empty = DIFF ? (which ? v_free : k_free) : (which ? pv_done : s_full);      // AT_STAGES == NSB: stage st is buffer st
+        unsigned long long* empty = twice ? (which ? v_free : k_free) : (which ? pv_done : s_full);      // AT_STAGES == NSB: stage st is buffer st
         const int ps = p.page_size, sh = p.page_shift;   // the page size is a power of two
         const int n_pg = AT_BK >> sh;                    // pages per tile (page_size divides 64)
         bool ok = true;
@@ -643,13 +657,14 @@ static int at_launch(const CUtensorMap& map, const AttnTcParams& p, int n_qblk, 
     return BG_OK;
 }
 
-// The same for positions that requests share (tiles of 64 keys).
+// The same for positions that requests share (tiles of 64 keys, two tiles of rows).
 template <int HD>
 static int at_launch_shared(const CUtensorMap& map, const AttnTcSharedParams& p, int n_items, cudaStream_t stream) {
     auto kern = attention_tcgen05_kernel<HD, 64, false, false, false, true>;
-    const size_t smem = (size_t)(HD / 64) * AT_BM * 128 + (size_t)2 * 256 * (HD / 64) * 128 + 1024;
-    static_assert(AT_BM * (HD + 4) * 4 <= 2 * 256 * (HD / 64) * 128, "the rows' sums fit the rings");
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    constexpr int queries = 2 * (HD / 64) * AT_BM * 128, rings = 2 * 256 * (HD / 64) * 128;
+    static_assert(2 * AT_BM * (HD + 4) * 4 <= queries + rings, "the rows' sums fit the room of queries, keys and values");
+    const size_t smem = (size_t)queries + rings + 1024;
+    cudaError_t e = smem_limit(kern, smem);
     if (e != cudaSuccess) return (int)e;
     e = launch(kern, dim3(p.nkv, n_items), dim3(AT_THREADS), smem, stream, map, p);
     if (e != cudaSuccess) return (int)e;
@@ -788,7 +803,7 @@ extern "C" int bg_attention_tc_difference(const void* q, int q_stride, const voi
 }
 
 // The partial results of single tokens over positions that their requests share: items [n_items][8] and rows as AttnTcSharedParams says (an item of no
-// entries is passed over; an item's first position is a multiple of 64), part_o [rows][nh][slots][hd] and part_ml [rows][nh][slots][2].
+// rows is passed over; an item's first position is a multiple of 64), part_o [rows][nh][slots][hd] and part_ml [rows][nh][slots][2].
 extern "C" int bg_attention_tc_shared(const void* q, int q_stride, const void* kv_pool, int num_pages, int page_size,
                                       const int* block_table, int max_pages, const int* positions, const int* items, int n_items,
                                       const int* rows, float* part_o, float* part_ml, int slots, int nh, int nkv, int hd, float scale,

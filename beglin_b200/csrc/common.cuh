@@ -8,6 +8,10 @@
 #include <stdint.h>
 #include <stdlib.h>
 
+#include <map>
+#include <mutex>
+#include <utility>
+
 #define BG_DTYPE_F32 0
 #define BG_DTYPE_BF16 1
 
@@ -63,6 +67,22 @@ inline int sm_count() {
         cached[dev] = n;
     }
     return cached[dev];
+}
+
+// Lets a kernel ask for `bytes` of dynamic shared memory (a kernel always asks for the same): once per kernel and device.
+template <typename... KArgs>
+inline cudaError_t smem_limit(void (*kern)(KArgs...), size_t bytes) {
+    static std::mutex mu;
+    static std::map<std::pair<const void*, int>, size_t> known;
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    std::lock_guard<std::mutex> g(mu);
+    size_t& have = known[{(const void*)kern, dev}];
+    if (have >= bytes) return cudaSuccess;
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess) have = bytes;
+    return e;
 }
 
 template <typename... KArgs, typename... Args>

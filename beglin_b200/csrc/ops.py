@@ -868,7 +868,7 @@ class SharedPlan:
         self.sms = sm_count(self.device) if self.device.type == "cuda" else 148
         self.shared = None
         if kernel == "tc":
-            self.room, sizes = _shared.items_room(n_rows, bq, nkv, self.sms), (n_rows, n_rows, n_rows)
+            self.room, sizes = _shared.items_room(n_rows, nh // nkv, nkv, self.sms), (n_rows, n_rows, n_rows)
         else:
             self.room, sizes = _shared.blocks_room(n_rows), (2 * n_rows,)
         # one buffer, so that a renewal is one copy: the list, then the rows' numbers
@@ -891,7 +891,7 @@ class SharedPlan:
         if shared.n_rows != self.n_rows:
             raise KernelError(f"shared_plan: groups of {shared.n_rows} rows for a plan of {self.n_rows}")
         if self.kernel == "tc":
-            arrays = _shared.shared_items(shared, self.bq, self.nkv, self.sms, self.room, self.MOST_RANGES)
+            arrays = _shared.shared_items(shared, self.nh // self.nkv, self.nkv, self.sms, self.room, self.MOST_RANGES)
         else:
             arrays = _shared.shared_blocks(shared, self.bq, self.split, self.room)
         return np.concatenate([a.reshape(-1) for a in arrays])

@@ -38,51 +38,69 @@ def blocks_room(n_rows: int) -> int:
     return n_rows + n_rows // 2 + 1 if n_rows > 1 else 1
 
 
-# What a range costs beside its positions, in positions: measured as the time of a CTA that takes one tile.
-RANGE_COST = 320
+# Time of a CTA of the tensor-core kernel in units of a tile of positions for up to 128 rows: what it takes before and behind its tiles, and what a tile
+# takes for up to 256 rows (measured at heads of 128: 0.6 us a tile, some 4 us beside, 0.85 us a tile for 256 rows).
+CTA_COST, PAIR_COST = 6.0, 1.4
 
 
-def range_length(tiles: Sequence[Tuple[int, int]], nkv: int, sms: int, most: int) -> int:
-    """Positions of a range, a multiple of TILE, for blocks of rows `tiles` = [(blocks, positions of their group)]: the length for which the CTAs, `sms` of
-    them at once, are done first, each taking its positions and RANGE_COST.  No more than `most` ranges a group."""
-    longest = max(p for _, p in tiles)
-    best, best_cost = None, None
-    floor = -(-longest // most)
-    for n in range(1, most + 1):
-        length = -(-max(-(-longest // n), TILE) // TILE) * TILE
-        if length < floor:
-            break
-        ctas = nkv * sum(b * -(-p // length) for b, p in tiles)
-        cost = -(-ctas // sms) * (length + RANGE_COST)
-        if best is None or cost < best_cost:
-            best, best_cost = length, cost
-    return best
+def _done(ctas: int, longest: float, total: float, sms: int) -> float:
+    """About when CTAs are through, the longest first."""
+    return longest if ctas <= sms else max(longest, total / sms + longest / 2)
 
 
-def shared_items(shared, bq: int, nkv: int, sms: int, room: int, most: int):
+def cut_ranges(groups: Sequence[Tuple[int, int]], nkv: int, sms: int, room: int, most: int) -> Tuple[int, int]:
+    """(rows of a block, positions of a range) for groups = [(rows of a kv head, positions)]: blocks of 128 or of 256 rows, and ranges, a multiple of TILE and
+    of one length for all groups, at most `most` a group, that are through first.  No more than `room` items."""
+    longest = max(p for _, p in groups)
+    best, choice = None, (256, -(-longest // TILE) * TILE)
+    for block in (128, 256):
+        blocks = sum(-(-r // block) for r, _ in groups)
+        for n in range(1, most + 1):
+            length = -(-max(-(-longest // n), TILE) // TILE) * TILE
+            if -(-longest // length) < n and n > 1:
+                continue
+            if sum(-(-r // block) * -(-p // length) for r, p in groups) > room:
+                break
+            ctas, total, slowest = 0, 0.0, 0.0
+            for r, p in groups:
+                ranges, tiles = -(-p // length), min(length, p) / TILE
+                for rows, count in ((block, r // block), (r % block, 1)):
+                    if rows and count:
+                        one = CTA_COST + tiles * (PAIR_COST if rows > 128 else 1.0)
+                        ctas += nkv * ranges * count
+                        total += nkv * ranges * count * one
+                        slowest = max(slowest, one)
+            done = _done(ctas, slowest, total, sms)
+            if best is None or done < best:
+                best, choice = done, (block, length)
+    return choice
+
+
+def shared_items(shared, group_heads: int, nkv: int, sms: int, room: int, most: int):
     """For the tensor-core kernel: (items int32 [room, 8], rows int32 [n], first position of its own of every row int32 [n], results of every row over what it
-    shares int32 [n]).  A group's rows are cut into blocks of `bq`, its positions into ranges of one length for all groups."""
+    shares int32 [n]).  A group's rows (requests x query heads of a kv head) are cut into blocks, its positions into ranges."""
     n = shared.n_rows
     rows, first, parts = np.zeros(n, dtype=np.int32), np.zeros(n, dtype=np.int32), np.zeros(n, dtype=np.int32)
     items, at = [], 0
     if shared.groups:
-        tiles = [(-(-len(g) // bq), p) for g, p in shared.groups]
-        length = range_length(tiles, nkv, sms, min(most, max(1, room // sum(b for b, _ in tiles))))
+        block, length = cut_ranges([(len(g) * group_heads, p) for g, p in shared.groups], nkv, sms, room, most)
         for group, positions in shared.groups:
             rows[at:at + len(group)] = group
             first[list(group)] = positions
-            ranges = -(-positions // length)
+            ranges, count = -(-positions // length), len(group) * group_heads
             parts[list(group)] = ranges
-            for b in range(0, len(group), bq):
-                items += [(group[0], at + b, min(bq, len(group) - b), s * length, min(positions, (s + 1) * length), s, 0, 0) for s in range(ranges)]
+            for b in range(0, count, block):
+                items += [(group[0], at * group_heads + b, min(block, count - b), s * length, min(positions, (s + 1) * length), s, 0, 0) for s in range(ranges)]
             at += len(group)
     if len(items) > room:
         raise ValueError(f"{len(items)} items, room for {room}")
+    # those that take longest come first (they are begun in this order)
+    items.sort(key=lambda i: -(i[4] - i[3]) * (PAIR_COST if i[2] > 128 else 1.0))
     out = np.zeros((room, 8), dtype=np.int32)
     out[:len(items)] = np.asarray(items, dtype=np.int32).reshape(-1, 8)
     return out, rows, first, parts
 
 
-def items_room(n_rows: int, bq: int, nkv: int, sms: int) -> int:
-    """Room for the items of any groups of n rows: two waves of CTAs, or a range for every block."""
-    return max(-(-2 * sms // nkv), n_rows // 2 + 1)
+def items_room(n_rows: int, group_heads: int, nkv: int, sms: int) -> int:
+    """Room for the items of any groups of n rows: three waves of CTAs, or a range for every block of every group (a group has two rows at least)."""
+    return max(-(-3 * sms // nkv), n_rows // 2 + -(-n_rows * group_heads // 256) + 1)

@@ -133,6 +133,21 @@ def test_shared_attention_on_tensor_cores(name, nh, nkv, hd, page):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("block,length", [(128, 192), (256, 192), (256, 64), (256, 6400)])
+@pytest.mark.parametrize("name", ["many", "long", "mixed"])
+@pytest.mark.parametrize("nh,nkv,hd", [(12, 2, 128), (32, 2, 64), (16, 1, 128)])
+def test_shared_attention_in_blocks_of_one_and_of_two_tiles_of_rows(name, nh, nkv, hd, block, length, monkeypatch):
+    monkeypatch.setattr(shared_plan, "cut_ranges", lambda *a: (block, length))
+    monkeypatch.setattr(shared_plan, "items_room", lambda *a: 3000)
+    monkeypatch.setattr(ops.SharedPlan, "MOST_RANGES", 100)
+    c = Case(*SETS[name], nh, nkv, hd, 64, torch.bfloat16, seed=nh)
+    got, plan = c.run()
+    assert int(plan.items[:plan.n_items, 2].max()) == min(block, nh // nkv * max(len(g) for g, _ in c.groups))
+    want, size = c.plain()
+    assert bool(((got.double() - want).abs() <= bound(size, want, torch.bfloat16)).all())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("name", ["odd", "mixed", "many"])
 @pytest.mark.parametrize("options", [dict(sink=True), dict(cap=20.0), dict(sink=True, cap=5.0)], ids=["sink", "cap", "both"])
 def test_shared_attention_options(name, options):
@@ -276,22 +291,25 @@ def test_every_position_of_a_row_is_taken_once(seed):
     for r, spans in taken.items():
         whole = of_row.get(r, (0, 0))[1] // split
         assert sorted(spans) == ([(0, whole)] if whole else []) + [(whole, shared_plan.MOST)]
-    room = shared_plan.items_room(n, bq, nkv, 148)
-    items, rows, first, parts = shared_plan.shared_items(shared, bq, nkv, 148, room, 64)
-    spans = {r: {} for r in range(n)}
+    heads = int(rng.choice([1, 6, 7, 16]))
+    room = shared_plan.items_room(n, heads, nkv, 148)
+    items, rows, first, parts = shared_plan.shared_items(shared, heads, nkv, 148, room, 64)
+    spans = {(r, h): {} for r in range(n) for h in range(heads)}
     for req, at, k, lo, hi, slot, _, _ in items.tolist():
-        assert k <= bq and lo % shared_plan.TILE == 0
-        for r in rows[at:at + k].tolist():
-            assert req == of_row[r][0] and lo < hi and slot not in spans[r]
-            spans[r][slot] = (lo, hi)
+        assert k <= 256 and lo % shared_plan.TILE == 0
+        for i in range(at, at + k):
+            r, h = int(rows[i // heads]), i % heads
+            assert req == of_row[r][0] and lo < hi and slot not in spans[r, h]
+            spans[r, h][slot] = (lo, hi)
     for r in range(n):
         p = of_row.get(r, (0, 0))[1]
-        assert first[r] == p and parts[r] == len(spans[r]) <= 64
-        at = 0
-        for slot in range(len(spans[r])):
-            assert spans[r][slot][0] == at
-            at = spans[r][slot][1]
-        assert at == p
+        for h in range(heads):
+            assert first[r] == p and parts[r] == len(spans[r, h]) <= 64
+            at = 0
+            for slot in range(len(spans[r, h])):
+                assert spans[r, h][slot][0] == at
+                at = spans[r, h][slot][1]
+            assert at == p
 
 
 def test_shared_attention_refuses_what_does_not_fit():
