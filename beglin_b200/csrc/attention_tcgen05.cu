@@ -43,6 +43,7 @@ inline int& at_wide_from() {
 }
 // Stages of the key and value rings: 256 keys each.
 constexpr int AT_THREADS = 448;            // warps 0 and 6: MMA issue; warps 1-4 and 8-11: softmax; warps 5, 7, 12, 13: loaders
+constexpr int AT_SHARED_THREADS = 512;     // warps 14 and 15: a second issuer of either product
 constexpr float AT_LOG2E = 1.4426950408889634f;
 
 struct AttnTcParams {
@@ -113,8 +114,10 @@ __device__ __forceinline__ float at_squash(float x, float cap_log2, float cap_k)
 // attention_shared.cu joins with those of the other ranges and of each request's own positions.  A row sees the positions up to its own.  More than 128
 // rows are two tiles of rows, and the two groups of softmax warps take one each, as the maps of DIFF: a tile of keys and values is fetched once for
 // both (256 rows of 28 heads over 32,768 positions are bound by what the L2 delivers with 128 rows a CTA: 7.1 TB/s).
+// SHARED also has two warps to issue the scores' products and two for the values', each pair taking the turns in turns (warps 14 and 15 beside 0 and 6):
+// a turn's waits, eight MMAs and commits take one warp some 1,200 cycles, more than the tensor cores need for it.
 template <int HD, int AT_BK, bool SINK = false, bool EXT = false, bool DIFF = false, bool SHARED = false>
-__global__ void __launch_bounds__(AT_THREADS)
+__global__ void __launch_bounds__(SHARED ? AT_SHARED_THREADS : AT_THREADS)
 attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename AtParams<DIFF, SHARED>::type p) {
     static_assert(!DIFF || (AT_BK == 64 && !SINK && !EXT), "the two maps take tiles of 64 keys in turns");
     static_assert(!SHARED || (AT_BK == 64 && !SINK && !EXT && !DIFF), "partial results of tiles of 64 keys");
@@ -171,9 +174,9 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
         }
         for (int b = 0; b < NSB; ++b) { mbar_init(&s_full[b], 1); mbar_init(&pv_done[b], 1); }
         for (int b = 0; b < 2 * NSB; ++b) mbar_init(&p_full[b], 4);       // one arrival per softmax warp of a group
-        mbar_init(&o_ready, 1);
+        mbar_init(&o_ready, SHARED ? 2 : 1);             // (an arrival of every issuer whose products are waited for)
         if constexpr (MAY_TWICE) {
-            for (int s = 0; s < AT_STAGES; ++s) { mbar_init(&k_free[s], 1); mbar_init(&v_free[s], 1); }
+            for (int s = 0; s < AT_STAGES; ++s) { mbar_init(&k_free[s], SHARED ? 2 : 1); mbar_init(&v_free[s], SHARED ? 2 : 1); }
         }
         failed = 0;
         mbar_init_fence();
@@ -209,7 +212,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
     auto tile_key = [&](int i) { return (EXT && i < n_kept ? i : tile0 + i - n_kept) * AT_BK; };
 
     // ---- Q into shared memory: row r, column block cb, 16-byte piece c at r*128 + ((c ^ (r & 7)) * 16)
-    for (int idx = tid; idx < (SHARED && twice ? 2 : 1) * AT_BM * (HD / 8); idx += AT_THREADS) {
+    for (int idx = tid; idx < (SHARED && twice ? 2 : 1) * AT_BM * (HD / 8); idx += (SHARED ? AT_SHARED_THREADS : AT_THREADS)) {
         const int r = idx / (HD / 8), c = idx - r * (HD / 8);
         uint4 v = make_uint4(0, 0, 0, 0);
         if (r < n_rows)
@@ -228,7 +231,9 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
     // this kernel to end while this CTA waits for its columns.
     pdl_launch();
 
-    if (warp == 0 || warp == 6) {
+    if (warp == 0 || warp == 6 || (SHARED && warp >= 14)) {
+        const int i_first = warp >= 14 ? 1 : 0;          // this issuer's first turn
+        constexpr int i_step = SHARED ? 2 : 1;
         // ------------------------------------------------------------------ MMA issuers: warp 0 the scores, warp 6 the values
         // The whole warp runs the loop and one elected lane issues: addresses and descriptors then stay in
         // uniform registers, which keeps the issue of one small MMA to a few cycles.  P, the left operand of the
@@ -241,10 +246,10 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
         auto wait_all = [&](unsigned long long* bar, unsigned parity) {
             return __all_sync(0xffffffffu, mbar_wait(bar, parity)) != 0;
         };
-        if (warp == 0) {
+        if (warp == 0 || warp == 14) {
             // scores: S[b] = Q K(i)^T as soon as the keys have landed and both groups' P of the buffer's last tile
             // have been used up
-            for (int i = 0; i < n_turns && ok; ++i) {
+            for (int i = i_first; i < n_turns && ok; i += i_step) {
                 const int tile = twice ? i >> 1 : i, map = twice ? i & 1 : 0;
                 const int st = tile % AT_STAGES, b = i % NSB;
                 // (which of the two waits comes first is measured: with four score buffers the older event, the
@@ -252,7 +257,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
                 // against 864 us at 16,384 tokens)
                 if (ALT) {
                     if (i >= NSB) ok = wait_all(&pv_done[b], ((i / NSB) - 1) & 1);
-                    if (ok && map == 0) ok = wait_all(&k_full[st], (tile / AT_STAGES) & 1);
+                    if (ok && (SHARED || map == 0)) ok = wait_all(&k_full[st], (tile / AT_STAGES) & 1);
                 } else {
                     ok = wait_all(&k_full[st], (i / AT_STAGES) & 1);
                     if (ok && i >= NSB) ok = wait_all(&pv_done[b], ((i / NSB) - 1) & 1);
@@ -280,17 +285,17 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
                                    smem_desc_sw128(k_addr + (ks >> 2) * KV_BLOCK + off), idesc_qk, ks > 0 ? 1u : 0u);
                         }
                         tc_commit(&s_full[b]);
-                        if (SHARED && map == 1) tc_commit(&k_free[st]);
+                        if (SHARED && twice) tc_commit(&k_free[st]);
                     }
                 }
                 __syncwarp();
             }
         } else {
             // values: O[g] += P(i, g) V(i, g) once group g's softmax warps have written their half of P
-            for (int i = 0; i < n_turns && ok; ++i) {
+            for (int i = i_first; i < n_turns && ok; i += i_step) {
                 const int tile = twice ? i >> 1 : i;
                 const int st = tile % AT_STAGES, b = i % NSB;
-                if (!twice || (i & 1) == 0) ok = wait_all(&v_full[st], (tile / AT_STAGES) & 1);
+                if (SHARED || !twice || (i & 1) == 0) ok = wait_all(&v_full[st], (tile / AT_STAGES) & 1);
                 const unsigned v_addr = smem_u32(v_s + st * KV_BYTES);
                 if constexpr (ALT) {
                     const int g = i & 1;
@@ -303,7 +308,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
                             tc_mma_ts(tmem + O_COL + 128u * (unsigned)g, tmem + (unsigned)b * AT_BK + (unsigned)ks * 8,
                                       smem_desc_sw128_nmajor(v_addr + ks * 2048, KV_BLOCK, 1024), idesc_pv, (i >= 2 || ks > 0) ? 1u : 0u);
                         tc_commit(&pv_done[b]);
-                        if (MAY_TWICE && twice && g == 1) tc_commit(&v_free[st]);
+                        if (MAY_TWICE && twice && (SHARED || g == 1)) tc_commit(&v_free[st]);
                     }
                     __syncwarp();
                 } else {
@@ -544,7 +549,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
                 }
             }
         }
-    } else {
+    } else if (warp == 5 || warp == 7 || warp == 12 || warp == 13) {
         // ------------------------------------------------------------------ loaders: TMA, a tile of keys at a time;
         // warps 5 and 12 bring the keys, warps 7 and 13 the values, each pair through a ring of stages of its own.
         // A loader's turn for one tile (page numbers, the barrier's byte count, the copies: each an operation of a
@@ -666,7 +671,7 @@ static int at_launch_shared(const CUtensorMap& map, const AttnTcSharedParams& p,
     const size_t smem = (size_t)queries + rings + 1024;
     cudaError_t e = smem_limit(kern, smem);
     if (e != cudaSuccess) return (int)e;
-    e = launch(kern, dim3(p.nkv, n_items), dim3(AT_THREADS), smem, stream, map, p);
+    e = launch(kern, dim3(p.nkv, n_items), dim3(AT_SHARED_THREADS), smem, stream, map, p);
     if (e != cudaSuccess) return (int)e;
     return BG_OK;
 }
