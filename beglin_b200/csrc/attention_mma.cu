@@ -26,6 +26,11 @@
 //          the MMAs of a stage (the heads fill 6 of 8 columns instead of 6 of 16 rows); P^T reaches its
 //          operand layout through movmatrix.
 //
+// SHARED instances take what lies behind positions that requests share.  Where that is more CTAs than SMs (many rows with a few hundred keys each, so that a
+// CTA's beginning and end count), QUARTER instances: every warp takes a quarter of every stage, three buffers are enough and two CTAs fit an SM.  1,024 streams
+// of 100 to 800 keys of 128 features: 66 us with a stage a warp, 52 with quarters (floor 37); 140 of up to 900 in pages of 16: 15.9 and 11.9; 16 of 300: 5.0
+// and 6.5, where the chain of a stage's steps is what counts.
+//
 // EXT instances: a score falls by slopes[head] per position that its key lies back, and a window never loses the sequence's
 // first `keep` positions.  The stages of a CTA are then those of its kept keys followed by those of its window's, the
 // stages between the two passed over.
@@ -142,7 +147,7 @@ __device__ __forceinline__ int swz_kv(int row, int c) {
     return (c >> 3) * (AM_STAGE_KEYS * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4);
 }
 
-template <int HD, bool BY_KEYS, int AM_STAGES, bool SWAP, bool EXT, bool SHARED = false>
+template <int HD, bool BY_KEYS, int AM_STAGES, bool SWAP, bool EXT, bool SHARED = false, bool QUARTER = false>
 __global__ void __launch_bounds__(AM_ALL)
 attention_mma_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_constant__ CUtensorMap map_page,
                      typename AmParams<EXT, SHARED>::type p) {
@@ -197,7 +202,7 @@ attention_mma_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_co
     // The group fetched here is the one the first keys of this CTA's range lie in when there is no window.
     __shared__ int table_s[AM_TABLE];
     if (tid == 0) {
-        for (int s = 0; s < AM_STAGES; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], BY_KEYS ? 1 : AM_THREADS / 32); }
+        for (int s = 0; s < AM_STAGES; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], BY_KEYS && !QUARTER ? 1 : AM_THREADS / 32); }
         gave_up = 0;
         mbar_init_fence();
     }
@@ -426,14 +431,16 @@ attention_mma_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_co
         for (int db = 0; db < HD / 16; ++db) voff_a[db] = swz_kv((lane & 7) + ((lane >> 4) << 3), db * 2 + ((lane >> 3) & 1));
     }
 
-    constexpr int KB = 4;                               // 16-key blocks of a stage
+    constexpr int KB = QUARTER ? 1 : 4;                 // 16-key blocks of a stage that a warp takes
     constexpr int BLOCK_BYTES = 16 * 128;               // 16 keys further down, in every block of 64 features
-    for (int s = BY_KEYS ? warp : 0; s < n_stage; s += (BY_KEYS ? AM_THREADS / 32 : 1)) {
+    for (int s = BY_KEYS && !QUARTER ? warp : 0; s < n_stage; s += (BY_KEYS && !QUARTER ? AM_THREADS / 32 : 1)) {
         if (!BY_KEYS) load_stage(s + AM_STAGES - 1);
         const int buf = s % AM_STAGES;
-        unsigned char* kt = k_s + buf * BUF_BYTES;
-        unsigned char* vt = v_s + buf * BUF_BYTES;
-        const int stage_key0 = stage_key(s);
+        // (QUARTER: the warp's 16 keys of the stage are all that it sees of it)
+        unsigned char* kt = k_s + buf * BUF_BYTES + (QUARTER ? warp * BLOCK_BYTES : 0);
+        unsigned char* vt = v_s + buf * BUF_BYTES + (QUARTER ? warp * BLOCK_BYTES : 0);
+        constexpr int OWN_KEYS = QUARTER ? 16 : AM_STAGE_KEYS;
+        const int stage_key0 = stage_key(s) + (QUARTER ? warp * 16 : 0);
         // who reads this stage: the warp alone (keys arrangement) or the four warps together
         const int t0 = BY_KEYS ? lane : tid, nt = BY_KEYS ? 32 : AM_THREADS;
         if (p.use_tma) {
@@ -441,10 +448,10 @@ attention_mma_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_co
             // the status): every thread then still reaches the barriers below.
             if (!mbar_wait<4000>(&full_bar[buf], (s / AM_STAGES) & 1, &gave_up) && p.status) atomicOr(p.status, BG_STATUS_TIMEOUT);
             const bool kept_stage = EXT && has_kept && stage_key0 >= k_first && stage_key0 + AM_STAGE_KEYS <= kept_end;
-            if ((stage_key0 < k_begin && !kept_stage) || stage_key0 + AM_STAGE_KEYS > k_end) {     // uniform over the readers
+            if ((stage_key0 < k_begin && !kept_stage) || stage_key0 + OWN_KEYS > k_end) {     // uniform over the readers
                 // whole pages were copied: rows outside the range of keys become zeros (a value row that no
                 // query sees must not hold garbage, since 0 * NaN is NaN)
-                for (int idx = t0; idx < AM_STAGE_KEYS * CH; idx += nt) {
+                for (int idx = t0; idx < OWN_KEYS * CH; idx += nt) {
                     const int j = idx / CH, c = idx - j * CH;
                     if (EXT ? !in_range(stage_key0 + j) : (stage_key0 + j < k_begin || stage_key0 + j >= k_end)) {
                         *reinterpret_cast<uint4*>(kt + swz_kv(j, c)) = make_uint4(0, 0, 0, 0);
@@ -456,7 +463,7 @@ attention_mma_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_co
             }
         } else if (BY_KEYS) {
             // pages of a size that does not divide 64: the warp copies its stage itself, 16 bytes at a time
-            for (int idx = lane; idx < AM_STAGE_KEYS * CH; idx += 32) {
+            for (int idx = lane; idx < OWN_KEYS * CH; idx += 32) {
                 const int j = idx / CH, c = idx - j * CH, key = stage_key0 + j;
                 const __nv_bfloat16* src = nullptr;
                 if (EXT ? in_range(key) : (key >= k_begin && key < k_end)) {
@@ -775,14 +782,20 @@ static int am_launch_stages(const CUtensorMap& map, const CUtensorMap& map5, con
 }
 
 // The decoding arrangement over what lies behind positions that requests share.
-template <int HD, bool SWAP>
-static int am_launch_own(const CUtensorMap& map, const CUtensorMap& map5, const AttnMmaSharedParams& p, int T, int n_splits, cudaStream_t stream) {
-    auto kern = attention_mma_kernel<HD, true, AM_THREADS / 32, SWAP, false, true>;
-    const size_t smem = am_smem_bytes<HD, true, AM_THREADS / 32>();
+template <int HD, bool SWAP, bool QUARTER>
+static int am_launch_own_as(const CUtensorMap& map, const CUtensorMap& map5, const AttnMmaSharedParams& p, int T, int n_splits, cudaStream_t stream) {
+    constexpr int stages = QUARTER ? 3 : AM_THREADS / 32;
+    auto kern = attention_mma_kernel<HD, true, stages, SWAP, false, true, QUARTER>;
+    const size_t smem = am_smem_bytes<HD, true, stages>();
     cudaError_t e = smem_limit(kern, smem);
     if (e != cudaSuccess) return (int)e;
     e = launch(kern, dim3(T, p.nkv, n_splits), dim3(AM_ALL), smem, stream, map, map5, p);
     return e == cudaSuccess ? BG_OK : (int)e;
+}
+template <int HD, bool SWAP>
+static int am_launch_own(const CUtensorMap& map, const CUtensorMap& map5, const AttnMmaSharedParams& p, int T, int n_splits, cudaStream_t stream) {
+    if ((long long)T * p.nkv * n_splits > sm_count()) return am_launch_own_as<HD, SWAP, true>(map, map5, p, T, n_splits, stream);
+    return am_launch_own_as<HD, SWAP, false>(map, map5, p, T, n_splits, stream);
 }
 
 template <int HD, bool BY_KEYS, bool EXT>

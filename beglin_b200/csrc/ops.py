@@ -679,6 +679,12 @@ def decode_splits(n_streams: int, context: int, sms: Optional[int] = None) -> in
     return -(-context // per)                             # no CTA without keys
 
 
+def own_ranges(n_streams: int, positions: int, sms: int) -> int:
+    """How many CTAs share the positions of one (request, kv head) stream behind those that requests share: those of `decode_splits` where a wave of CTAs
+    holds two of a stream; else the kernel has two CTAs an SM, and a stream is cut for three waves of SMs (as many as have work: lengths differ)."""
+    return decode_splits(n_streams, positions, sms if 2 * n_streams <= sms else 3 * sms)
+
+
 class AttnF32Args(ctypes.Structure):
     """What `attention_f32_step` needs of a layer (csrc/attention_f32_step.cu says what the fields are)."""
     _fields_ = [(n, _c_void_p) for n in ("qkv", "qkv_bias", "out", "out_bias", "sink_w", "status")] \
@@ -992,7 +998,7 @@ def _shared_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_table: torch
     if plan.kernel == "tc":
         if status is None or out.dtype != torch.bfloat16:
             raise KernelError("shared_attention: the tensor-core kernels want a status word and write bfloat16")
-        ranges, at_once = decode_splits(T * plan.nkv, max(1, max_position + 1 - plan.least_own), plan.sms), 0
+        ranges, at_once = own_ranges(T * plan.nkv, max(1, max_position + 1 - plan.least_own), plan.sms), 0
         floats, kernels = T * nh * (plan.slots + ranges) * (vd + 2), 3
     else:
         ranges, kernels = max_position // plan.split + 1, 2
