@@ -31,6 +31,7 @@
 // Every wait on an mbarrier is bounded in time and records BG_STATUS_TIMEOUT.
 //
 // The result is the finished row, out[t, h, :] = O / l, as in attention_mma.cu's rows arrangement.
+#include "float_pairs.cuh"
 #include "page_tma.cuh"
 
 namespace bg {
@@ -43,7 +44,7 @@ inline int& at_wide_from() {
 }
 // Stages of the key and value rings: 256 keys each.
 constexpr int AT_THREADS = 448;            // warps 0 and 6: MMA issue; warps 1-4 and 8-11: softmax; warps 5, 7, 12, 13: loaders
-constexpr int AT_SHARED_THREADS = 512;     // warps 14 and 15: a second issuer of either product
+constexpr int AT_SHARED_THREADS = 512;     // two issuers of either product
 constexpr float AT_LOG2E = 1.4426950408889634f;
 
 struct AttnTcParams {
@@ -80,6 +81,10 @@ struct AttnTcSharedParams : AttnTcParams {
     float* part_ml;             // [rows][nh][slots][2] maximum (of scores as they are), sum
     int slots;
 };
+template <bool V> struct AtSplit { static constexpr bool value = V; };
+// SHARED: of the pairs of exponentials every eighth is the float units' (256 rows of 28 heads over 32,768 positions, 280 CTAs: 113.5 us; none of them
+// 120.6, every fourth 125.7: the special function units and the instructions' issue are both near their limits).
+constexpr int AT_FLOAT_EVERY = 7;
 template <bool DIFF, bool SHARED> struct AtParams { using type = AttnTcParams; };
 template <> struct AtParams<true, false> { using type = AttnTcDiffParams; };
 template <> struct AtParams<false, true> { using type = AttnTcSharedParams; };
@@ -88,6 +93,23 @@ __device__ __forceinline__ float at_ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
     return y;
+}
+
+// 2^x of two numbers up to 2^8 by the float units: 2^n from the bits of n = x rounded, times a polynomial of degree four in x - n.  Its coefficients make the
+// largest relative error on [-1/2, 1/2] as small as can be (Remez' exchange algorithm): 2.6e-6.  Below -126 it is 2^-126; what is not a number stays so.
+__device__ __forceinline__ unsigned long long at_ex2_float2(unsigned long long x) {
+    float a = low2(x), b = high2(x);
+    asm("max.NaN.f32 %0, %0, %1;\n" : "+f"(a) : "f"(-126.0f));
+    asm("max.NaN.f32 %0, %0, %1;\n" : "+f"(b) : "f"(-126.0f));
+    const unsigned long long one = pair2(1.0f, 1.0f), y = pair2(a, b);
+    const unsigned long long t = fma2(y, one, pair2(12582912.0f, 12582912.0f));          // 1.5 2^23: the integer lies in the low bits
+    const unsigned long long n = fma2(t, one, pair2(-12582912.0f, -12582912.0f)), f = fma2(n, pair2(-1.0f, -1.0f), y);
+    unsigned long long r = fma2(f, pair2(0.009570101908084362f, 0.009570101908084362f), pair2(0.05591786031930516f, 0.05591786031930516f));
+    r = fma2(r, f, pair2(0.2402474482794395f, 0.2402474482794395f));
+    r = fma2(r, f, pair2(0.6931218147367705f, 0.6931218147367705f));
+    r = fma2(r, f, pair2(0.9999992614457144f, 0.9999992614457144f));
+    const unsigned long long two_n = pair2(__uint_as_float(((unsigned)t << 23) + 0x3f800000u), __uint_as_float(((unsigned)(t >> 32) << 23) + 0x3f800000u));
+    return fma2(r, two_n, 0ull);
 }
 
 // c log2(e) tanh(scale * x / c) as 1 - 2 / (1 + 2^(2 log2(e) scale x / c)): two special-function operations, exact at both
@@ -114,8 +136,8 @@ __device__ __forceinline__ float at_squash(float x, float cap_log2, float cap_k)
 // attention_shared.cu joins with those of the other ranges and of each request's own positions.  A row sees the positions up to its own.  More than 128
 // rows are two tiles of rows, and the two groups of softmax warps take one each, as the maps of DIFF: a tile of keys and values is fetched once for
 // both (256 rows of 28 heads over 32,768 positions are bound by what the L2 delivers with 128 rows a CTA: 7.1 TB/s).
-// SHARED also has two warps to issue the scores' products and two for the values', each pair taking the turns in turns (warps 14 and 15 beside 0 and 6):
-// a turn's waits, eight MMAs and commits take one warp some 1,200 cycles, more than the tensor cores need for it.
+// SHARED also has two warps to issue the scores' products (0 and 13) and two for the values' (6 and 15), each pair taking the turns in turns: a turn's
+// waits, eight MMAs and commits take one warp some 1,200 cycles, more than the tensor cores need for it.
 template <int HD, int AT_BK, bool SINK = false, bool EXT = false, bool DIFF = false, bool SHARED = false>
 __global__ void __launch_bounds__(SHARED ? AT_SHARED_THREADS : AT_THREADS)
 attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename AtParams<DIFF, SHARED>::type p) {
@@ -231,8 +253,9 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
     // this kernel to end while this CTA waits for its columns.
     pdl_launch();
 
-    if (warp == 0 || warp == 6 || (SHARED && warp >= 14)) {
-        const int i_first = warp >= 14 ? 1 : 0;          // this issuer's first turn
+    // (SHARED: an issuer on each of the four sub-partitions, with a loader and a softmax warp of either group)
+    if (warp == 0 || warp == 6 || (SHARED && (warp == 13 || warp == 15))) {
+        const int i_first = warp >= 13 ? 1 : 0;          // this issuer's first turn
         constexpr int i_step = SHARED ? 2 : 1;
         // ------------------------------------------------------------------ MMA issuers: warp 0 the scores, warp 6 the values
         // The whole warp runs the loop and one elected lane issues: addresses and descriptors then stay in
@@ -246,7 +269,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
         auto wait_all = [&](unsigned long long* bar, unsigned parity) {
             return __all_sync(0xffffffffu, mbar_wait(bar, parity)) != 0;
         };
-        if (warp == 0 || warp == 14) {
+        if (warp == 0 || warp == 13) {
             // scores: S[b] = Q K(i)^T as soon as the keys have landed and both groups' P of the buffer's last tile
             // have been used up
             for (int i = i_first; i < n_turns && ok; i += i_step) {
@@ -374,7 +397,8 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
             }
             // only a half that some row of the warp sees in part is masked element by element
             float tm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-            if (key0 + GK - 1 > warp_pos_min || (key0 < warp_lo_max && !(EXT && key0 + GK <= keep))) {
+            const bool masked = key0 + GK - 1 > warp_pos_min || (key0 < warp_lo_max && !(EXT && key0 + GK <= keep));
+            if (masked) {
 #pragma unroll
                 for (int q = 0; q < GK; ++q) {
                     const int key = key0 + q;
@@ -395,6 +419,24 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
             const float corr = grow ? at_ex2(m - m_use) : 1.0f;
             float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
             float pk[GK / 2];                            // P: two keys a column
+            if constexpr (SHARED) {
+                const unsigned long long unit2 = pair2(sl2, sl2), less2 = pair2(-m_use, -m_use), one = pair2(1.0f, 1.0f);
+                unsigned long long sums2[2] = {0ull, 0ull};
+                auto weights = [&](auto split) {
+#pragma unroll
+                    for (int c = 0; c < GK / 2; ++c) {
+                        unsigned long long e = fma2(pair2(s[2 * c], s[2 * c + 1]), unit2, less2);
+                        if (decltype(split)::value && (c & AT_FLOAT_EVERY) == AT_FLOAT_EVERY) e = at_ex2_float2(e);
+                        else e = pair2(at_ex2(low2(e)), at_ex2(high2(e)));
+                        sums2[c & 1] = fma2(e, one, sums2[c & 1]);
+                        const __nv_bfloat162 h2 = __floats2bfloat162_rn(low2(e), high2(e));
+                        pk[c] = __uint_as_float(*reinterpret_cast<const unsigned*>(&h2));
+                    }
+                };
+                if (masked) weights(AtSplit<false>{});   // (a weight that is nought has to be)
+                else weights(AtSplit<true>{});
+                sums[0] = low2(sums2[0]); sums[1] = high2(sums2[0]); sums[2] = low2(sums2[1]); sums[3] = high2(sums2[1]);
+            } else
 #pragma unroll
             for (int c = 0; c < GK / 2; ++c) {
                 const float e0 = at_ex2(fmaf(s[2 * c], sl2, -m_use)), e1 = at_ex2(fmaf(s[2 * c + 1], sl2, -m_use));
@@ -549,13 +591,13 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
                 }
             }
         }
-    } else if (warp == 5 || warp == 7 || warp == 12 || warp == 13) {
+    } else {
         // ------------------------------------------------------------------ loaders: TMA, a tile of keys at a time;
         // warps 5 and 12 bring the keys, warps 7 and 13 the values, each pair through a ring of stages of its own.
         // A loader's turn for one tile (page numbers, the barrier's byte count, the copies: each an operation of a
         // few hundred cycles, one after the other) takes longer than the tensor cores need for the tile, so two
         // warps share a ring: one takes the even tiles, the other the odd ones.
-        const int which = (warp == 7 || warp == 13);
+        const int which = (warp == 7 || warp == (SHARED ? 14 : 13));
         const int lsub = warp >= 12;
         unsigned char* ring = which ? v_s : k_s;
         unsigned long long* full = which ? v_full : k_full;

@@ -866,13 +866,13 @@ class SharedPlan:
     """How a layer's attention goes over shared positions: made by `shared_plan` for one `SharedPrefix`, and renewed in place by `update`, so that a
     captured graph reads the groups of the step that it is replayed for."""
 
-    def __init__(self, n_rows, nh, nkv, hd, vd, dtype, query_dtype, page_size, kernel, bq, tile, split, device):
+    def __init__(self, n_rows, nh, nkv, hd, vd, dtype, query_dtype, page_size, kernel, bq, tile, split, device, fixed, all_groups):
+        self.fixed, self.all_groups = fixed, all_groups
         self.n_rows, self.nh, self.nkv, self.hd, self.vd, self.dtype, self.query_dtype, self.page_size = n_rows, nh, nkv, hd, vd, dtype, query_dtype, page_size
         self.kernel, self.bq, self.tile, self.split, self.device = kernel, bq, tile, split, torch.device(device)
         if self.device.type == "cuda" and self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
         self.sms = sm_count(self.device) if self.device.type == "cuda" else 148
-        self.shared = None
         if kernel == "tc":
             self.room, sizes = _shared.items_room(n_rows, nh // nkv, nkv, self.sms), (n_rows, n_rows, n_rows)
         else:
@@ -897,29 +897,35 @@ class SharedPlan:
         if shared.n_rows != self.n_rows:
             raise KernelError(f"shared_plan: groups of {shared.n_rows} rows for a plan of {self.n_rows}")
         if self.kernel == "tc":
+            if not self.all_groups:
+                kept = _shared.worth_sharing(shared, self.nh // self.nkv, self.nkv, self.sms, self.room, self.MOST_RANGES,
+                                             lambda streams, positions: own_ranges(streams, positions, self.sms), 4 * self.hd)
+                shared = type(shared)(self.n_rows, kept)
             arrays = _shared.shared_items(shared, self.nh // self.nkv, self.nkv, self.sms, self.room, self.MOST_RANGES)
         else:
             arrays = _shared.shared_blocks(shared, self.bq, self.split, self.room)
         return np.concatenate([a.reshape(-1) for a in arrays])
 
-    def update(self, shared, fixed: bool = False) -> None:
-        """Take the groups of `shared`.  `fixed`: the launches keep the shape that serves any groups of these rows (for a captured graph)."""
+    def update(self, shared) -> None:
+        """Take the groups of `shared`, for the calls that are queued from now on."""
         host = torch.from_numpy(self.pack(shared))
         if self.device.type == "cuda":
             host = host.pin_memory()
         self.buffer.copy_(host, non_blocking=True)
         self._staged = host            # (kept until the next renewal: the copy may be under way)
-        self._shape(shared, host, fixed)
+        self._shape(host)
 
-    def _shape(self, shared, host, fixed: bool) -> None:
-        self.shared = shared
+    def _shape(self, host) -> None:
+        fixed = self.fixed
         items = host[:self.room * 8].view(self.room, 8).numpy()
         used = int((items[:, 2] > 0).sum())
         if self.kernel == "tc":
+            self.shares = used > 0             # whether anything is read for several rows at once
             self.n_items = self.room if fixed else used
             self.slots = self.MOST_RANGES if fixed else int(host[self.room * 8 + 2 * self.n_rows:].max()) if self.n_rows else 0
             self.least_own = 0 if fixed or not self.n_rows else int(host[self.room * 8 + self.n_rows:self.room * 8 + 2 * self.n_rows].min())
         else:
+            self.shares = used > self.n_rows
             self.n_items = self.room if fixed else used
             own = items[:used][items[:used, 4] == _shared.MOST]
             self.slots = int(items[:used][items[:used, 4] != _shared.MOST][:, 4].max(initial=0))
@@ -939,7 +945,8 @@ def shared_plan(shared, nh: int, nkv: int, hd: int, dtype: torch.dtype, page_siz
                 query_dtype: Optional[torch.dtype] = None, device="cuda", fixed: bool = False) -> SharedPlan:
     """The plan of `shared_attention` for the groups of `shared` (a `cache.shared.SharedPrefix`), heads of `hd` features (values of `vd`), a cache of `dtype` and
     queries of `query_dtype`.  Kernels: "tc" (bfloat16, heads of 64 or 128: the shared positions on tcgen05) or "generic" (every size and type, splits at
-    multiples of `split` positions, whole splits shared: a row's result is bit for bit that of `attention`).  `fixed`: launches of one shape for any groups,
+    multiples of `split` positions, whole splits shared: a row's result is bit for bit that of `attention`).  "auto" takes "tc" where it can, for the groups
+    whose sharing is expected to pay; "tc" shares whatever is shared.  `fixed`: launches of one shape for any groups,
     for a captured graph, whose groups `SharedPlan.update` then renews."""
     vd, query_dtype = hd if vd is None else int(vd), query_dtype or dtype
     if nkv <= 0 or nh % nkv:
@@ -953,14 +960,14 @@ def shared_plan(shared, nh: int, nkv: int, hd: int, dtype: torch.dtype, page_siz
     if prefer == "tc" and not takes:
         raise KernelError(f"shared_plan: the tensor-core kernels do not take {dtype} heads of {hd} with {group} query heads per kv head and pages of {page_size}")
     if takes and prefer != "generic":
-        plan = SharedPlan(shared.n_rows, nh, nkv, hd, vd, dtype, query_dtype, page_size, "tc", bq.value, 64, 0, device)
+        plan = SharedPlan(shared.n_rows, nh, nkv, hd, vd, dtype, query_dtype, page_size, "tc", bq.value, 64, 0, device, fixed, prefer == "tc")
     else:
         if L.bg_attention_plan(group, hd, vd, 1, 1 if dtype == query_dtype == torch.float32 else 0, ctypes.byref(bq), ctypes.byref(tile)) != 0:
             raise KernelError(f"shared_plan: heads of {hd} (values of {vd}) with {group} query heads per kv head are not supported")
         if split <= 0 or split % tile.value:
             raise KernelError(f"shared_plan: splits of {split} positions are not whole tiles of {tile.value}")
-        plan = SharedPlan(shared.n_rows, nh, nkv, hd, vd, dtype, query_dtype, page_size, "generic", bq.value, tile.value, split, device)
-    plan.update(shared, fixed)
+        plan = SharedPlan(shared.n_rows, nh, nkv, hd, vd, dtype, query_dtype, page_size, "generic", bq.value, tile.value, split, device, fixed, True)
+    plan.update(shared)
     return plan
 
 

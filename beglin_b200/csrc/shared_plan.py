@@ -38,9 +38,12 @@ def blocks_room(n_rows: int) -> int:
     return n_rows + n_rows // 2 + 1 if n_rows > 1 else 1
 
 
-# Time of a CTA of the tensor-core kernel in units of a tile of positions for up to 128 rows: what it takes before and behind its tiles, and what a tile
-# takes for up to 256 rows (measured at heads of 128: 0.6 us a tile, some 4 us beside, 0.85 us a tile for 256 rows).
-CTA_COST, PAIR_COST = 6.0, 1.4
+# What the tensor-core kernels take, in microseconds, measured on B200 with heads of 128 features: a CTA beside its tiles, a tile of 64 positions for up to 128
+# rows and for up to 256.
+CTA_US, TILE_US, PAIR_US = 6.0, 0.52, 1.03
+# A stream's own positions: the launch, and a position in a CTA; where more CTAs than SMs run, bytes a microsecond.  The kernel that joins results.
+OWN_US, POSITION_US, OWN_RATE, JOIN_US = 4.0, 0.0085, 4.5e6, 3.5
+OWN_GUESS = 256            # positions that a request is taken to hold behind those that it shares
 
 
 def _done(ctas: int, longest: float, total: float, sms: int) -> float:
@@ -48,32 +51,63 @@ def _done(ctas: int, longest: float, total: float, sms: int) -> float:
     return longest if ctas <= sms else max(longest, total / sms + longest / 2)
 
 
-def cut_ranges(groups: Sequence[Tuple[int, int]], nkv: int, sms: int, room: int, most: int) -> Tuple[int, int]:
-    """(rows of a block, positions of a range) for groups = [(rows of a kv head, positions)]: blocks of 128 or of 256 rows, and ranges, a multiple of TILE and
-    of one length for all groups, at most `most` a group, that are through first.  No more than `room` items."""
+def cut_ranges(groups: Sequence[Tuple[int, int]], nkv: int, sms: int, room: int, most: int) -> Tuple[int, int, float]:
+    """(rows of a block, positions of a range, microseconds) for groups = [(rows of a kv head, positions)]: blocks of 128 or of 256 rows, and ranges, a multiple
+    of TILE and of one length for all groups, at most `most` a group, that are through first.  No more than `room` items."""
     longest = max(p for _, p in groups)
-    best, choice = None, (256, -(-longest // TILE) * TILE)
+    best = None
     for block in (128, 256):
-        blocks = sum(-(-r // block) for r, _ in groups)
-        for n in range(1, most + 1):
+        if block > 128 and all(r <= 128 for r, _ in groups):
+            break
+        n, last = 1, 0
+        while n <= most:
             length = -(-max(-(-longest // n), TILE) // TILE) * TILE
-            if -(-longest // length) < n and n > 1:
-                continue
-            if sum(-(-r // block) * -(-p // length) for r, p in groups) > room:
-                break
-            ctas, total, slowest = 0, 0.0, 0.0
-            for r, p in groups:
-                ranges, tiles = -(-p // length), min(length, p) / TILE
-                for rows, count in ((block, r // block), (r % block, 1)):
-                    if rows and count:
-                        one = CTA_COST + tiles * (PAIR_COST if rows > 128 else 1.0)
-                        ctas += nkv * ranges * count
-                        total += nkv * ranges * count * one
-                        slowest = max(slowest, one)
-            done = _done(ctas, slowest, total, sms)
-            if best is None or done < best:
-                best, choice = done, (block, length)
-    return choice
+            if length != last:
+                ctas, total, slowest, items = 0, 0.0, 0.0, 0
+                for r, p in groups:
+                    ranges, tiles = -(-p // length), min(length, p) / TILE
+                    for rows, count in ((block, r // block), (r % block, 1)):
+                        if rows and count:
+                            one = CTA_US + tiles * (PAIR_US if rows > 128 else TILE_US)
+                            items += ranges * count
+                            total += nkv * ranges * count * one
+                            slowest = max(slowest, one)
+                ctas = nkv * items
+                if items > room:
+                    break
+                done = _done(ctas, slowest, total, sms) + 0.05 * -(-longest // length)       # (every range is one more result to join)
+                if best is None or done < best[2]:
+                    best = block, length, done
+            last = length
+            n += 1 if n < 16 else 4
+    return best or (256, -(-longest // TILE) * TILE, 0.0)
+
+
+def own_us(lengths: Sequence[int], nkv: int, ranges, sms: int, row_bytes: int) -> float:
+    """About what the kernel of the rows' own positions takes; `ranges`(streams, positions) is how a stream is cut."""
+    n, longest = len(lengths), max(max(lengths), 1)
+    cut = ranges(n * nkv, longest)
+    if n * nkv * cut <= sms:
+        return OWN_US + -(-longest // cut) * POSITION_US * row_bytes / 512
+    return OWN_US + max(sum(lengths) * nkv * row_bytes / OWN_RATE, -(-longest // cut) * POSITION_US * row_bytes / 512)
+
+
+def worth_sharing(shared, group_heads: int, nkv: int, sms: int, room: int, most: int, ranges, row_bytes: int):
+    """The groups of `shared` whose sharing is expected to pay, those that save most first: few rows of few positions are read from the L2 again sooner than they
+    are split off and joined.  `row_bytes`: of a key and a value of one kv head."""
+    order = sorted(shared.groups, key=lambda g: -(len(g[0]) - 1) * g[1])
+    best, kept = None, 0
+    for k in sorted({0, 1, 2, len(order) // 2, len(order)} & set(range(len(order) + 1))):
+        lengths = [OWN_GUESS] * shared.n_rows
+        for g, p in order[k:]:
+            for r in g:
+                lengths[r] += p
+        us = own_us(lengths, nkv, ranges, sms, row_bytes) + JOIN_US
+        if k:
+            us += cut_ranges([(len(g) * group_heads, p) for g, p in order[:k]], nkv, sms, room, most)[2]
+        if best is None or us < best:
+            best, kept = us, k
+    return order[:kept]
 
 
 def shared_items(shared, group_heads: int, nkv: int, sms: int, room: int, most: int):
@@ -83,7 +117,7 @@ def shared_items(shared, group_heads: int, nkv: int, sms: int, room: int, most: 
     rows, first, parts = np.zeros(n, dtype=np.int32), np.zeros(n, dtype=np.int32), np.zeros(n, dtype=np.int32)
     items, at = [], 0
     if shared.groups:
-        block, length = cut_ranges([(len(g) * group_heads, p) for g, p in shared.groups], nkv, sms, room, most)
+        block, length, _ = cut_ranges([(len(g) * group_heads, p) for g, p in shared.groups], nkv, sms, room, most)
         for group, positions in shared.groups:
             rows[at:at + len(group)] = group
             first[list(group)] = positions
@@ -95,7 +129,7 @@ def shared_items(shared, group_heads: int, nkv: int, sms: int, room: int, most: 
     if len(items) > room:
         raise ValueError(f"{len(items)} items, room for {room}")
     # those that take longest come first (they are begun in this order)
-    items.sort(key=lambda i: -(i[4] - i[3]) * (PAIR_COST if i[2] > 128 else 1.0))
+    items.sort(key=lambda i: -(i[4] - i[3]) * (2 if i[2] > 128 else 1))
     out = np.zeros((room, 8), dtype=np.int32)
     out[:len(items)] = np.asarray(items, dtype=np.int32).reshape(-1, 8)
     return out, rows, first, parts

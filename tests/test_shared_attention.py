@@ -70,11 +70,12 @@ class Case:
             size.append(torch.einsum("hn,nhd->hd", w, v.abs()).reshape(-1))
         return torch.stack(out), torch.stack(size)
 
-    def run(self, prefer="auto", sink=None, cap=0.0, fixed=False, max_position=None, plan=None, split=256):
+    def run(self, prefer=None, sink=None, cap=0.0, fixed=False, max_position=None, plan=None, split=256):
         to = lambda t: t.to(DEV)
         buf = torch.full((self.q.shape[0], self.q.stride(0)), 3.0, dtype=self.q.dtype, device=DEV)
         q = buf[:, :self.q.shape[1]]
         q.copy_(self.q)
+        prefer = prefer or ("tc" if self.pool.dtype == torch.bfloat16 else "auto")
         plan = plan or ops.shared_plan(self.shared, self.nh, self.nkv, self.hd, self.pool.dtype, page_size=self.page, vd=self.vd, split=split, prefer=prefer,
                                        device=DEV, fixed=fixed)
         wide = torch.full((len(self.lengths), self.nh * self.vd + 8), 7.0, dtype=self.q.dtype, device=DEV)
@@ -137,7 +138,7 @@ def test_shared_attention_on_tensor_cores(name, nh, nkv, hd, page):
 @pytest.mark.parametrize("name", ["many", "long", "mixed"])
 @pytest.mark.parametrize("nh,nkv,hd", [(12, 2, 128), (32, 2, 64), (16, 1, 128)])
 def test_shared_attention_in_blocks_of_one_and_of_two_tiles_of_rows(name, nh, nkv, hd, block, length, monkeypatch):
-    monkeypatch.setattr(shared_plan, "cut_ranges", lambda *a: (block, length))
+    monkeypatch.setattr(shared_plan, "cut_ranges", lambda *a: (block, length, 0.0))
     monkeypatch.setattr(shared_plan, "items_room", lambda *a: 3000)
     monkeypatch.setattr(ops.SharedPlan, "MOST_RANGES", 100)
     c = Case(*SETS[name], nh, nkv, hd, 64, torch.bfloat16, seed=nh)
@@ -193,7 +194,7 @@ def test_shared_attention_of_fixed_shape_follows_its_groups(dtype):
     pages = max(c.pool.shape[0] for c in cases.values())
     width = max(c.table.shape[1] for c in cases.values())
     c = cases["many"]
-    plan = ops.shared_plan(c.shared, 12, 2, 128, dtype, device=DEV, fixed=True)
+    plan = ops.shared_plan(c.shared, 12, 2, 128, dtype, prefer="tc" if dtype == torch.bfloat16 else "auto", device=DEV, fixed=True)
     q = torch.zeros(48, 12 * 128, dtype=dtype, device=DEV)
     pool = torch.zeros((pages,) + tuple(c.pool.shape[1:]), dtype=dtype, device=DEV)
     table = torch.full((48, width), -1, dtype=torch.int32, device=DEV)
@@ -207,7 +208,7 @@ def test_shared_attention_of_fixed_shape_follows_its_groups(dtype):
         table.fill_(-1)
         table[:, :c.table.shape[1]].copy_(c.table)
         positions.copy_(c.positions)
-        plan.update(c.shared, fixed=True)
+        plan.update(c.shared)
 
     load(c)
     side = torch.cuda.Stream()
@@ -229,6 +230,18 @@ def test_shared_attention_of_fixed_shape_follows_its_groups(dtype):
             assert torch.equal(out.cpu(), cases[name].alone())
         else:
             assert bool(((got - want).abs() <= bound(size, want, dtype)).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kept", [0, 1, 2])
+def test_shared_attention_of_groups_that_pay(kept, monkeypatch):
+    """Groups that are left to their rows' own pages beside groups that are read once."""
+    monkeypatch.setattr(shared_plan, "worth_sharing", lambda shared, *a: shared.groups[:kept])
+    c = Case(*SETS["mixed"], 12, 2, 128, 64, torch.bfloat16, seed=5)
+    got, plan = c.run(prefer="auto")
+    assert plan.shares == (kept > 0)
+    want, size = c.plain()
+    assert bool(((got.double() - want).abs() <= bound(size, want, torch.bfloat16)).all())
 
 
 @pytest.mark.gpu
@@ -310,6 +323,18 @@ def test_every_position_of_a_row_is_taken_once(seed):
                 assert spans[r, h][slot][0] == at
                 at = spans[r, h][slot][1]
             assert at == p
+
+
+def test_groups_that_pay_are_kept():
+    """Few rows of few positions are left alone; many rows of many positions are not."""
+    ranges = lambda streams, positions: ops.own_ranges(streams, positions, 148)
+    args = (6, 2, 148, 444, 64, ranges, 512)
+    keep = lambda n, groups: shared_plan.worth_sharing(SharedPrefix(n, groups), *args)
+    assert keep(2, [([0, 1], 512)]) == []
+    assert keep(64, [(range(64), 8192)]) == [(tuple(range(64)), 8192)]
+    big, small = (tuple(range(40)), 20000), ((40, 41), 64)
+    assert big in keep(42, [small, big])
+    assert keep(3, []) == []
 
 
 def test_shared_attention_refuses_what_does_not_fit():
