@@ -101,6 +101,15 @@ __device__ __forceinline__ float am_score(float c, const AttnMmaParams& p) {
     return p.cap_log2 > 0.0f ? p.cap_log2 * tanhf(c * p.scale_over_cap) : c * p.scale_log2;
 }
 
+// The same by two special-function operations in place of tanhf: 1 - 2 / (1 + 2^(2 log2(e) x)), exact at both ends and a few units in the last place elsewhere.
+__device__ __forceinline__ float am_score(float c, const AttnMmaSharedParams& p) {
+    if (!(p.cap_log2 > 0.0f)) return c * p.scale_log2;
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(e) : "f"(c * p.scale_over_cap * (2.0f * AM_LOG2E)));
+    asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(1.0f + e));
+    return p.cap_log2 * fmaf(-2.0f, r, 1.0f);
+}
+
 __device__ __forceinline__ void cp_async16(void* smem_dst, const void* gmem_src) {
     unsigned d = (unsigned)__cvta_generic_to_shared(smem_dst);
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(d), "l"(gmem_src) : "memory");

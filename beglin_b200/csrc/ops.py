@@ -375,25 +375,30 @@ def _cuda(*tensors) -> None:
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+# (a tensor on a CUDA device has initialised CUDA: torch.cuda.current_device's check of that is left out)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def _stream():
     """The raw handle of torch's current stream on the current device (a cheap call; the public
     torch.cuda.current_stream() costs several microseconds, which counts at hundreds of launches a step)."""
     if _raw_stream is not None:
-        return _raw_stream(torch.cuda.current_device())
+        return _raw_stream(_current_device())
     return torch.cuda.current_stream().cuda_stream
 
 
 def _here(what: str, *tensors) -> None:
     """All on the current device: a launch goes to the current device's stream."""
+    now = None
     for t in tensors:
-        if t is not None and t.get_device() < 0:           # (an attribute less than t.is_cuda and t.device.index together)
-            _cuda(t)
-    now = torch.cuda.current_device()
-    for t in tensors:
-        if t is not None and t.get_device() != now:
-            raise KernelError(f"{what}: a tensor on {t.device}, the current device is cuda:{now}")
+        if t is not None:
+            at = t.get_device()                # (costs less than t.is_cuda and t.device.index; -1: not on a CUDA device)
+            if at < 0:
+                _cuda(t)
+            if now is None:
+                now = _current_device()
+            if at != now:
+                raise KernelError(f"{what}: a tensor on {t.device}, the current device is cuda:{now}")
 
 
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
@@ -971,13 +976,7 @@ def shared_plan(shared, nh: int, nkv: int, hd: int, dtype: torch.dtype, page_siz
     return plan
 
 
-def shared_attention(*args, **kwargs) -> None:
-    """`_shared_attention` under the phase timer of its kernel class (all its kernels together)."""
-    with phase("attn"):
-        _shared_attention(*args, **kwargs)
-
-
-def _shared_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_table: torch.Tensor, positions: torch.Tensor, plan: SharedPlan, max_position: int,
+def shared_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_table: torch.Tensor, positions: torch.Tensor, plan: SharedPlan, max_position: int,
                       scale: float, out: torch.Tensor, status: Optional[torch.Tensor], sink: bool = False, sink_weight: Optional[torch.Tensor] = None,
                       softcap: float = 0.0) -> None:
     """Paged grouped-query attention of a step of single tokens, row r that of request r, over every position up to its own: what a group of `plan` shares is
@@ -986,7 +985,8 @@ def _shared_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_table: torch
     `softcap` as in `attention`.  A row whose position lies inside what its group shares sees that far; values behind it that are not finite reach it, which
     those behind the shared positions never do."""
     T, nh, vd = plan.n_rows, plan.nh, plan.vd
-    _i32(positions, "positions"); _i32(block_table, "block_table")
+    if positions.dtype != torch.int32 or block_table.dtype != torch.int32 or not positions.is_contiguous() or not block_table.is_contiguous():
+        raise KernelError("shared_attention: positions and the block table are contiguous int32")
     if q.shape != plan.q_shape or q.stride(1) != 1 or q.dtype != plan.query_dtype:
         raise KernelError(f"shared_attention: q is {q.dtype} {tuple(q.shape)}, expected {plan.query_dtype} {list(plan.q_shape)}")
     if out.shape != plan.out_shape or out.stride(1) != 1 or T > 1 and out.stride(0) < nh * vd:
@@ -1006,7 +1006,7 @@ def _shared_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_table: torch
         if status is None or out.dtype != torch.bfloat16:
             raise KernelError("shared_attention: the tensor-core kernels want a status word and write bfloat16")
         ranges, at_once = own_ranges(T * plan.nkv, max(1, max_position + 1 - plan.least_own), plan.sms), 0
-        floats, kernels = T * nh * (plan.slots + ranges) * (vd + 2), 3
+        floats, kernels = T * nh * (plan.slots + ranges) * (vd + 2), 3 if plan.n_items else 2
     else:
         ranges, kernels = max_position // plan.split + 1, 2
         at_once = min(ranges, max(plan.slots, ranges - plan.least_own, 1))
@@ -1015,7 +1015,8 @@ def _shared_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_table: torch
     step = SharedAttnStep(q.data_ptr(), kv_pool.data_ptr(), block_table.data_ptr(), positions.data_ptr(), out.data_ptr(), _p(sink_weight), _p(status),
                           scratch.data_ptr(), floats, q.stride(0), out.stride(0), block_table.shape[1], kv_pool.shape[0], ranges, at_once,
                           1 if sink or sink_weight is not None else 0, _dt(out), scale, softcap)
-    _check(lib().bg_shared_attention(plan._args, ctypes.byref(step), _stream()), "shared_attention")
+    with phase("attn"):                        # (all its kernels together)
+        _check(lib().bg_shared_attention(plan._args, ctypes.byref(step), _stream()), "shared_attention")
     count_launches(kernels - 1)
 
 

@@ -41,8 +41,9 @@ def blocks_room(n_rows: int) -> int:
 # What the tensor-core kernels take, in microseconds, measured on B200 with heads of 128 features: a CTA beside its tiles, a tile of 64 positions for up to 128
 # rows and for up to 256.
 CTA_US, TILE_US, PAIR_US = 6.0, 0.52, 1.03
-# A stream's own positions: the launch, and a position in a CTA; where more CTAs than SMs run, bytes a microsecond.  The kernel that joins results.
-OWN_US, POSITION_US, OWN_RATE, JOIN_US = 4.0, 0.0085, 4.5e6, 3.5
+# The rows' own positions and the joining of results: what the two kernels take by themselves beside a CTA's positions, and behind the shared positions' kernel
+# (they begin while it runs); a position in a CTA; where more CTAs than SMs run, bytes a microsecond.
+ALONE_US, BEHIND_US, POSITION_US, OWN_RATE = 2.9, 0.4, 0.0135, 4.5e6
 OWN_GUESS = 256            # positions that a request is taken to hold behind those that it shares
 
 
@@ -84,12 +85,11 @@ def cut_ranges(groups: Sequence[Tuple[int, int]], nkv: int, sms: int, room: int,
 
 
 def own_us(lengths: Sequence[int], nkv: int, ranges, sms: int, row_bytes: int) -> float:
-    """About what the kernel of the rows' own positions takes; `ranges`(streams, positions) is how a stream is cut."""
+    """About what the kernel of the rows' own positions takes; `ranges`(streams, positions) is how a stream is cut (in whole multiples of 256 positions)."""
     n, longest = len(lengths), max(max(lengths), 1)
     cut = ranges(n * nkv, longest)
-    if n * nkv * cut <= sms:
-        return OWN_US + -(-longest // cut) * POSITION_US * row_bytes / 512
-    return OWN_US + max(sum(lengths) * nkv * row_bytes / OWN_RATE, -(-longest // cut) * POSITION_US * row_bytes / 512)
+    one = -(-(-(-longest // cut)) // 256) * 256 * POSITION_US
+    return one if n * nkv * cut <= sms else max(sum(lengths) * nkv * row_bytes / OWN_RATE, one)
 
 
 def worth_sharing(shared, group_heads: int, nkv: int, sms: int, room: int, most: int, ranges, row_bytes: int):
@@ -102,9 +102,8 @@ def worth_sharing(shared, group_heads: int, nkv: int, sms: int, room: int, most:
         for g, p in order[k:]:
             for r in g:
                 lengths[r] += p
-        us = own_us(lengths, nkv, ranges, sms, row_bytes) + JOIN_US
-        if k:
-            us += cut_ranges([(len(g) * group_heads, p) for g, p in order[:k]], nkv, sms, room, most)[2]
+        us = own_us(lengths, nkv, ranges, sms, row_bytes)
+        us += BEHIND_US + cut_ranges([(len(g) * group_heads, p) for g, p in order[:k]], nkv, sms, room, most)[2] if k else ALONE_US
         if best is None or us < best:
             best, kept = us, k
     return order[:kept]
