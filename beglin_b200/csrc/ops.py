@@ -941,7 +941,8 @@ class SharedPlan:
                                    self.nh, self.nkv, self.hd, self.vd, self.page_size, F32 if self.query_dtype == torch.float32 else BF16,
                                    F32 if self.dtype == torch.float32 else BF16, self.n_items, self.slots, self.split, self.tile, self.bq)
         self._args = ctypes.byref(self.args)
-        # what `shared_attention` compares its tensors with
+        # what `shared_attention` compares its tensors with, and floats of a result of every row
+        self.row_floats = self.n_rows * self.nh * (self.vd + 2)
         self.q_shape, self.out_shape = (self.n_rows, self.nh * self.hd), (self.n_rows, self.nh * self.vd)
         self.page_shape = (2, self.nkv, self.page_size, self.hd) if self.vd == self.hd else (self.nkv * self.page_size * (self.hd + self.vd),)
 
@@ -984,19 +985,22 @@ def shared_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_table: torch.
     apart), kv_pool and block_table as `attention` takes them, `max_position` a bound on the positions, out [T, nh * vd].  `sink`, `sink_weight` and
     `softcap` as in `attention`.  A row whose position lies inside what its group shares sees that far; values behind it that are not finite reach it, which
     those behind the shared positions never do."""
-    T, nh, vd = plan.n_rows, plan.nh, plan.vd
+    # (every look at a tensor costs the host a tenth of a microsecond or two, as much as a small step's kernels in all: contiguous tensors are asked for little)
+    T, pool_shape, table_shape = plan.n_rows, kv_pool.shape, block_table.shape
     if positions.dtype != torch.int32 or block_table.dtype != torch.int32 or not positions.is_contiguous() or not block_table.is_contiguous():
         raise KernelError("shared_attention: positions and the block table are contiguous int32")
-    if q.shape != plan.q_shape or q.stride(1) != 1 or q.dtype != plan.query_dtype:
+    if q.shape != plan.q_shape or q.dtype != plan.query_dtype or not q.is_contiguous() and q.stride(1) != 1:
         raise KernelError(f"shared_attention: q is {q.dtype} {tuple(q.shape)}, expected {plan.query_dtype} {list(plan.q_shape)}")
-    if out.shape != plan.out_shape or out.stride(1) != 1 or T > 1 and out.stride(0) < nh * vd:
+    if out.shape != plan.out_shape or not out.is_contiguous() and (out.stride(1) != 1 or T > 1 and out.stride(0) < plan.out_shape[1]):
         raise KernelError(f"shared_attention: out is {tuple(out.shape)}, expected {list(plan.out_shape)}")
-    if positions.numel() != T or block_table.dim() != 2 or block_table.shape[0] != T:
+    if positions.numel() != T or len(table_shape) != 2 or table_shape[0] != T:
         raise KernelError("shared_attention: a position and a row of the block table for every row")
-    if kv_pool.dtype != plan.dtype or kv_pool.shape[1:] != plan.page_shape or not kv_pool.is_contiguous():
-        raise KernelError(f"shared_attention: kv_pool is {kv_pool.dtype} {tuple(kv_pool.shape)}, expected {plan.dtype} [pages, {', '.join(map(str, plan.page_shape))}]")
-    if sink_weight is not None and (sink_weight.dtype != torch.float32 or sink_weight.numel() != nh or not sink_weight.is_contiguous()):
-        raise KernelError("shared_attention: the sink's scores are contiguous float32, one per query head")
+    if kv_pool.dtype != plan.dtype or pool_shape[1:] != plan.page_shape or not kv_pool.is_contiguous():
+        raise KernelError(f"shared_attention: kv_pool is {kv_pool.dtype} {tuple(pool_shape)}, expected {plan.dtype} [pages, {', '.join(map(str, plan.page_shape))}]")
+    if sink_weight is not None:
+        sink = True
+        if sink_weight.dtype != torch.float32 or sink_weight.numel() != plan.nh or not sink_weight.is_contiguous():
+            raise KernelError("shared_attention: the sink's scores are contiguous float32, one per query head")
     if max_position < 0 or softcap < 0.0:
         raise KernelError("shared_attention: max_position and softcap are not negative")
     if T == 0:
@@ -1005,16 +1009,16 @@ def shared_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_table: torch.
     if plan.kernel == "tc":
         if status is None or out.dtype != torch.bfloat16:
             raise KernelError("shared_attention: the tensor-core kernels want a status word and write bfloat16")
-        ranges, at_once = own_ranges(T * plan.nkv, max(1, max_position + 1 - plan.least_own), plan.sms), 0
-        floats, kernels = T * nh * (plan.slots + ranges) * (vd + 2), 3 if plan.n_items else 2
+        ranges, at_once, kernels = own_ranges(T * plan.nkv, max(1, max_position + 1 - plan.least_own), plan.sms), 0, 3 if plan.n_items else 2
+        floats = plan.row_floats * (plan.slots + ranges)
     else:
         ranges, kernels = max_position // plan.split + 1, 2
         at_once = min(ranges, max(plan.slots, ranges - plan.least_own, 1))
-        floats = T * nh * ranges * (vd + 2)
-    scratch = torch.empty(floats, dtype=torch.float32, device=q.device)
-    step = SharedAttnStep(q.data_ptr(), kv_pool.data_ptr(), block_table.data_ptr(), positions.data_ptr(), out.data_ptr(), _p(sink_weight), _p(status),
-                          scratch.data_ptr(), floats, q.stride(0), out.stride(0), block_table.shape[1], kv_pool.shape[0], ranges, at_once,
-                          1 if sink or sink_weight is not None else 0, _dt(out), scale, softcap)
+        floats = plan.row_floats * ranges
+    scratch = torch.empty(floats, dtype=torch.float32, device=plan.device)
+    step = SharedAttnStep(q.data_ptr(), kv_pool.data_ptr(), block_table.data_ptr(), positions.data_ptr(), out.data_ptr(),
+                          None if sink_weight is None else sink_weight.data_ptr(), None if status is None else status.data_ptr(), scratch.data_ptr(), floats,
+                          q.stride(0), out.stride(0), table_shape[1], pool_shape[0], ranges, at_once, sink, _dt(out), scale, softcap)
     with phase("attn"):                        # (all its kernels together)
         _check(lib().bg_shared_attention(plan._args, ctypes.byref(step), _stream()), "shared_attention")
     count_launches(kernels - 1)
