@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+from array import array
 from typing import Optional, Tuple
 
 import numpy as np
@@ -203,8 +204,8 @@ _SIGNATURES = {
                                _c_int, _c_int, _c_void_p, _c_void_p, _c_void_p],
     "bg_shared_attention_bytes": [_c_int],
     "bg_shared_attention": [_c_void_p, _c_void_p, _c_void_p],
-    "bg_adjust_logits": [_c_void_p, _c_ll, _c_void_p, _c_ll, _c_int, _c_int, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
-                         _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_int, _c_void_p, _c_void_p],
+    "bg_logits_bytes": [],
+    "bg_adjust_logits": [_c_void_p, ctypes.POINTER(_c_int), _c_void_p],
     "bg_copy_pages_most": [],
     "bg_copy_pages": [_c_void_p, _c_int, _c_ll, _c_int, _c_ll, _c_int, _c_int, _c_ll, _c_int, _c_void_p, _c_void_p, _c_int, _c_void_p],
     "bg_sample": [_c_void_p, _c_int, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p],
@@ -236,7 +237,7 @@ def lib():
         for cls, name, which in ((AttnF32Args, "bg_attention_f32_bytes", (0,)), (AttnF32Step, "bg_attention_f32_bytes", (1,)), (LatentArgs, "bg_latent_bytes", (0,)),
                                  (LatentStep, "bg_latent_bytes", (1,)), (Mamba2Args, "bg_mamba2_bytes", (0,)), (Mamba2Step, "bg_mamba2_bytes", (1,)),
                                  (ExpertsArgs, "bg_experts_bytes", ()), (_GlaArgs, "bg_gla_bytes", ()), (SharedAttnArgs, "bg_shared_attention_bytes", (0,)),
-                                 (SharedAttnStep, "bg_shared_attention_bytes", (1,))):
+                                 (SharedAttnStep, "bg_shared_attention_bytes", (1,)), (LogitsArgs, "bg_logits_bytes", ())):
             if getattr(handle, name)(*which) != ctypes.sizeof(cls):
                 raise KernelError(f"the kernel library's {cls.__name__} has another size than its mirror here")
         _lib = handle
@@ -399,12 +400,6 @@ def _here(what: str, *tensors) -> None:
                 now = _current_device()
             if at != now:
                 raise KernelError(f"{what}: a tensor on {t.device}, the current device is cuda:{now}")
-
-
-def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether the memory from a's first element to its last meets that of b's."""
-    end = lambda t: t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
-    return a.numel() > 0 and b.numel() > 0 and a.data_ptr() < end(b) and b.data_ptr() < end(a)
 
 
 def _i32(t: torch.Tensor, what: str) -> None:
@@ -1387,6 +1382,13 @@ def sample(logits: torch.Tensor, temperature: Optional[torch.Tensor], uniform: O
     _launches += 1            # two kernels
 
 
+class LogitsArgs(ctypes.Structure):
+    """What `adjust_logits` hands over (csrc/logits.cu says what the fields are)."""
+    _fields_ = [(n, _c_void_p) for n in ("x", "out", "history", "lengths", "prompts", "newest", "repetition", "frequency", "presence", "bias_id", "bias", "bias_row",
+                                         "allowed", "allowed_row", "status")] \
+        + [(n, _c_ll) for n in ("ldx", "ldo")] + [(n, _c_int) for n in ("n", "V", "cap", "n_bias", "words", "masks")]
+
+
 def adjust_logits(logits: torch.Tensor, out: torch.Tensor, *, history: Optional[torch.Tensor] = None, lengths: Optional[torch.Tensor] = None,
                   prompts: Optional[torch.Tensor] = None, newest: Optional[torch.Tensor] = None, repetition: Optional[torch.Tensor] = None,
                   frequency: Optional[torch.Tensor] = None, presence: Optional[torch.Tensor] = None,
@@ -1402,38 +1404,44 @@ def adjust_logits(logits: torch.Tensor, out: torch.Tensor, *, history: Optional[
     int32 [masks, words]: bit v % 32 of word v / 32 says whether token v may be chosen; the others become -inf.  Row r takes mask
     `allowed_row`[r], -1: none (None: mask r).  Tokens outside [0, V), biased tokens out of order, a full history and masks that are
     not there are passed over and recorded in `status`."""
-    if logits.dim() != 2 or logits.dtype != torch.float32 or out.dtype != torch.float32 or logits.shape != out.shape:
-        raise KernelError(f"adjust_logits: logits and out are float32 [n, V], got {logits.dtype} {tuple(logits.shape)} and {out.dtype} {tuple(out.shape)}")
-    n, V = logits.shape
+    shape, f32, i32 = logits.shape, torch.float32, torch.int32
+    if len(shape) != 2 or logits.dtype != f32 or out.dtype != f32 or shape != out.shape:
+        raise KernelError(f"adjust_logits: logits and out are float32 [n, V], got {logits.dtype} {tuple(shape)} and {out.dtype} {tuple(out.shape)}")
+    n, V = shape
     if n == 0:
         return
-    if V == 0 or any(V > 1 and t.stride(1) != 1 or n > 1 and t.stride(0) < V for t in (logits, out)):
+    ldx, ldo = (V if t.is_contiguous() else max(t.stride(0), V) if n == 1 else t.stride(0) if V == 1 or t.stride(1) == 1 else 0 for t in (logits, out))
+    if V == 0 or ldx < V or ldo < V:
         raise KernelError("adjust_logits: rows of at least one logit, side by side and apart from one another")
-    same = out.data_ptr() == logits.data_ptr() and (n == 1 or out.stride(0) == logits.stride(0))
-    if not same and _overlap(logits, out):
-        raise KernelError("adjust_logits: out is logits itself, or memory apart from it")
-    if (history is None) != (lengths is None) or history is None and (newest is not None or prompts is not None):
-        raise KernelError("adjust_logits: a history goes with its lengths; prompts and newest go with a history")
-    if history is not None:
+    x, y = logits.data_ptr(), out.data_ptr()
+    if x != y or n > 1 and ldx != ldo:
+        if x < y + 4 * ((n - 1) * ldo + V) and y < x + 4 * ((n - 1) * ldx + V):
+            raise KernelError("adjust_logits: out is logits itself, or memory apart from it")
+    if history is None:
+        if lengths is not None or newest is not None or prompts is not None:
+            raise KernelError("adjust_logits: a history goes with its lengths; prompts and newest go with a history")
+        room = 0
+    else:
+        if lengths is None:
+            raise KernelError("adjust_logits: a history goes with its lengths; prompts and newest go with a history")
         _i32(history, "adjust_logits: history")
         if history.dim() != 2 or history.shape[0] != n or history.shape[1] == 0:
             raise KernelError(f"adjust_logits: history is {tuple(history.shape)}, expected [{n}, room]")
-    for t, what in ((lengths, "lengths"), (prompts, "prompts"), (newest, "newest"), (allowed_row, "allowed_row")):
-        if t is not None:
-            _i32(t, f"adjust_logits: {what}")
-            if tuple(t.shape) != (n,):
-                raise KernelError(f"adjust_logits: {what} has one number per row, got {tuple(t.shape)} for {n} rows")
-    for t, what in ((repetition, "repetition"), (frequency, "frequency"), (presence, "presence")):
-        if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != (n,) or not t.is_contiguous()):
-            raise KernelError(f"adjust_logits: {what} is contiguous float32, one number per row")
+        room = history.shape[1]
+    for t in (lengths, prompts, newest, allowed_row):
+        if t is not None and (t.dtype != i32 or t.shape != (n,) or not t.is_contiguous()):
+            raise KernelError(f"adjust_logits: lengths, prompts, newest and allowed_row are contiguous int32, one number per row, got {t.dtype} {tuple(t.shape)} for {n} rows")
+    for t in (repetition, frequency, presence):
+        if t is not None and (t.dtype != f32 or t.shape != (n,) or not t.is_contiguous()):
+            raise KernelError(f"adjust_logits: repetition, frequency and presence are contiguous float32, one number per row, got {t.dtype} {tuple(t.shape)} for {n} rows")
+    ids = values = begins = None
+    n_bias = words = masks = 0
     if bias is not None:
         ids, values, begins = bias
         _i32(ids, "adjust_logits: biased tokens"); _i32(begins, "adjust_logits: begins of the biased tokens")
-        if values.dtype != torch.float32 or not values.is_contiguous() or values.shape != ids.shape or ids.dim() != 1 or tuple(begins.shape) != (n + 1,):
+        if values.dtype != f32 or not values.is_contiguous() or values.shape != ids.shape or ids.dim() != 1 or begins.shape != (n + 1,):
             raise KernelError("adjust_logits: bias is (tokens int32 [k], values float32 [k], begins int32 [n + 1])")
-        if ids.numel() == 0:
-            bias = None
-    words = masks = 0
+        n_bias = ids.numel()
     if allowed is not None:
         _i32(allowed, "adjust_logits: allowed")
         if allowed.dim() != 2 or allowed.shape[1] < -(-V // 32) or allowed.shape[0] < (1 if allowed_row is not None else n):
@@ -1442,48 +1450,54 @@ def adjust_logits(logits: torch.Tensor, out: torch.Tensor, *, history: Optional[
         masks, words = allowed.shape
     elif allowed_row is not None:
         raise KernelError("adjust_logits: allowed_row goes with masks")
-    ids, values, begins = bias or (None, None, None)
     _here("adjust_logits", logits, out, history, lengths, prompts, newest, repetition, frequency, presence, ids, values, begins, allowed, allowed_row, status)
+    args = LogitsArgs(x, y, _p(history), _p(lengths), _p(prompts), _p(newest), _p(repetition), _p(frequency), _p(presence), _p(ids) if n_bias else None, _p(values),
+                      _p(begins), _p(allowed), _p(allowed_row), _p(status), ldx, ldo, n, V, room, n_bias, words, masks)
+    launched = _c_int(0)
     with phase("sample"):
-        _check(lib().bg_adjust_logits(_p(logits), logits.stride(0) if n > 1 else max(V, logits.stride(0)), _p(out), out.stride(0) if n > 1 else max(V, out.stride(0)),
-                                      n, V, _p(history), 0 if history is None else history.shape[1], _p(lengths), _p(prompts), _p(newest), _p(repetition),
-                                      _p(frequency), _p(presence), _p(ids), _p(values), _p(begins), _p(allowed), words, _p(allowed_row), masks, _p(status),
-                                      _stream()), "adjust_logits")
+        _check(lib().bg_adjust_logits(ctypes.byref(args), ctypes.byref(launched), _stream()), "adjust_logits")
+    count_launches(launched.value - 1)
 
 
 def copy_pages(pool: torch.Tensor, src, dst, positions: int) -> None:
     """pool[:, dst[i], ..., :positions, :] = pool[:, src[i], ..., :positions, :] for every i.  `pool` [stages, pages, ..., positions of a page, features]: a
     page's numbers lie side by side, stages and pages may lie apart.  `src` and `dst` are sequences of page numbers on the host; a page is written once,
     and none that is read."""
-    src, dst = [int(v) for v in src], [int(v) for v in dst]
-    if pool.dim() < 4 or any(n == 0 for n in pool.shape):
-        raise KernelError(f"copy_pages: pool is {tuple(pool.shape)}, expected [stages, pages, ..., positions, features]")
-    if not pool[0, 0].is_contiguous():
-        raise KernelError("copy_pages: the numbers of a page lie side by side")
-    stages, pages, rows = pool.shape[0], pool.shape[1], pool.shape[-2]
-    size, page = pool.element_size(), pool[0, 0].numel()
-    if stages > 1 and pool.stride(0) < page or pages > 1 and pool.stride(1) < page:
+    src, dst = list(map(int, src)), list(map(int, dst))
+    shape, strides, size = pool.shape, pool.stride(), pool.element_size()
+    if len(shape) < 4 or 0 in shape:
+        raise KernelError(f"copy_pages: pool is {tuple(shape)}, expected [stages, pages, ..., positions, features]")
+    page = 1
+    for n, stride in zip(reversed(shape[2:]), reversed(strides[2:])):
+        if n > 1 and stride != page:
+            raise KernelError("copy_pages: the numbers of a page lie side by side")
+        page *= n
+    stages, pages, rows, features = shape[0], shape[1], shape[-2], shape[-1]
+    stage_step, page_step = strides[0] if stages > 1 else page, strides[1] if pages > 1 else page
+    if stage_step < page or page_step < page:
         raise KernelError("copy_pages: pages that overlap")
     if not 0 <= positions <= rows:
         raise KernelError(f"copy_pages: {positions} positions of pages of {rows}")
     if len(src) != len(dst):
         raise KernelError(f"copy_pages: {len(src)} pages to read and {len(dst)} to write")
-    bad = [p for p in src + dst if not 0 <= p < pages]
-    if bad:
-        raise KernelError(f"copy_pages: page {bad[0]} outside the {pages} of the pool")
-    if len(set(dst)) != len(dst) or set(dst) & set(src):
+    if not src:
+        return
+    if min(src) < 0 or min(dst) < 0 or max(src) >= pages or max(dst) >= pages:
+        raise KernelError(f"copy_pages: page {[p for p in src + dst if not 0 <= p < pages][0]} outside the {pages} of the pool")
+    written = set(dst)
+    if len(written) != len(dst) or not written.isdisjoint(src):
         raise KernelError("copy_pages: a page that is written twice, or read and written")
-    pairs = sorted(zip(src, dst))
+    if len(set(src)) > 1:                      # equal sources side by side
+        pairs = sorted(zip(src, dst))
+        src, dst = [s for s, _ in pairs], [d for _, d in pairs]
     _here("copy_pages", pool)
     L = lib()
     most = L.bg_copy_pages_most()
     with phase("copy_pages"):
-        for i in range(0, len(pairs) if positions else 0, most):
-            part = pairs[i:i + most]
-            array = _c_int * len(part)
-            _check(L.bg_copy_pages(_p(pool), stages, pool.stride(0) * size if stages > 1 else page * size, pages, pool.stride(1) * size if pages > 1 else page * size,
-                                   page // (rows * pool.shape[-1]), rows, pool.shape[-1] * size, int(positions), array(*(s for s, _ in part)),
-                                   array(*(d for _, d in part)), len(part), _stream()), "copy_pages")
+        for i in range(0, len(src) if positions else 0, most):
+            s, d = array("i", src[i:i + most]), array("i", dst[i:i + most])
+            _check(L.bg_copy_pages(pool.data_ptr(), stages, stage_step * size, pages, page_step * size, page // (rows * features), rows, features * size,
+                                   int(positions), s.buffer_info()[0], d.buffer_info()[0], len(s), _stream()), "copy_pages")
 
 
 # ------------------------------------------------------------------------------------------------

@@ -1,5 +1,6 @@
 """Penalties, biases and masks of logits against a plain restatement in 64 bits, token by token from the lists."""
 import math
+from collections import Counter
 
 import pytest
 import torch
@@ -25,8 +26,7 @@ def _plain(x, history, lengths, prompts, newest, rep, freq, pres, bias, allowed,
             v = float(x[r, t])
             x[r, t] = v / k if v > 0 else v * k
         size[r] = x[r].abs()
-        for t in set(made):
-            c = made.count(t)
+        for t, c in Counter(made).items():
             x[r, t] -= f * c + p
             size[r, t] += abs(f * c) + abs(p)
         if bias is not None:
@@ -36,9 +36,8 @@ def _plain(x, history, lengths, prompts, newest, rep, freq, pres, bias, allowed,
                 size[r, int(ids[j])] += abs(float(values[j]))
         row = -1 if allowed is None else r if allowed_row is None else int(allowed_row[r])
         if row >= 0:
-            for t in range(V):
-                if not (int(allowed[row, t >> 5]) >> (t & 31)) & 1:
-                    x[r, t] = -math.inf
+            t = torch.arange(V)
+            x[r, (allowed[row].long()[t >> 5] >> (t & 31)) & 1 == 0] = -math.inf
     return x, size
 
 
@@ -111,7 +110,10 @@ CASES = [dict(n=1, V=1, held=1), dict(n=2, V=31, held=0, masks="own"), dict(n=3,
          dict(n=5, V=16387, held=1000, masks="some", bias=300, pad=1), dict(n=2, V=5000, held=2000, pad=3, offset=1),
          dict(n=3, V=9000, held=50, newest=False), dict(n=3, V=9000, held=50, prompts=False, masks="own"),
          dict(n=70, V=3001, held=37, masks="some", bias=4), dict(n=2, V=40000, held=77, penalties=False, masks="some", bias=9),
-         dict(n=1, V=151936, held=513, bias=3)]
+         dict(n=1, V=151936, held=513, bias=3),
+         # many rows: a copy and a mending kernel; texts in a table of their tokens, longer ones and more biases than a thread holds, texts without a table
+         dict(n=70, V=20011, held=300, masks="some", bias=4, pad=1), dict(n=140, V=10000, held=40, bias=3), dict(n=40, V=33000, held=9000, bias=1500, masks="some"),
+         dict(n=40, V=33001, held=13000, bias=300, pad=3), dict(n=75, V=16390, held=900, penalties=False, bias=50), dict(n=64, V=20000, held=70, newest=False, masks="own")]
 
 
 @pytest.mark.gpu
@@ -201,7 +203,7 @@ def test_adjusted_logits_refuse_what_does_not_fit():
     refused("side by side", out=torch.zeros(1, 40).expand(2, 40))
     both = torch.zeros(3, 40)
     refused("memory apart", logits=both[:2], out=both[1:])
-    refused("lengths", history=history)
+    refused("goes with its lengths", history=history)
     refused("history", newest=lengths)
     refused("history is", history=history[:1].contiguous(), lengths=lengths)
     refused("int32", history=history.long(), lengths=lengths)
