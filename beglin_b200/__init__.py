@@ -7,7 +7,7 @@ above it (`engine`), sampling (`sampling`) and hand-written CUDA kernels (`csrc`
 """
 __version__ = "0.1.0"
 
-__all__ = ["Engine", "Entry", "load_config", "write_random_model"]
+__all__ = ["Engine", "Entry", "LogitRules", "load_config", "write_random_model"]
 
 
 def __getattr__(name):
@@ -17,6 +17,9 @@ def __getattr__(name):
     if name == "Entry":
         from .engine.batch import Entry
         return Entry
+    if name == "LogitRules":
+        from .sampling import LogitRules
+        return LogitRules
     if name == "load_config":
         from .config import load_config
         return load_config

@@ -17,17 +17,29 @@ slab [stages, slots, ...]; a request's slot is zeroed when the request starts.  
 branches (attention beside a recurrence) hands in a composite need: each of its needs joins the group of its kind,
 and the stage's view is the tuple of the branches' views.
 
+Requests may go on from another's text (`fork`): they hold its whole pages together with it, a page counting its holders and free
+again when the last has given it back; the positions at the text's end that do not fill a page, and state of fixed size, are
+copied.  Shared pages are never written: a request writes at its own length and behind.
+
 All accounting is host code on plain Python and numpy and is tested without a GPU; only `allocate`
-makes device tensors.
+makes device tensors, and only `fork` touches them.
 """
 from __future__ import annotations
 
+from collections import Counter
 from typing import Dict, Hashable, List, Optional, Sequence
 
 import numpy as np
 import torch
 
+from .shared import SharedPrefix
 from ..parts.cache_need import PAGED_NEEDS, CompositeNeed, FixedStateNeed, FixedStateView, PagedKVNeed, PagedKVView
+
+
+def ops():
+    """The kernels' faces (imported when a copy on the device is made: the accounting does without)."""
+    from ..csrc import ops as faces
+    return faces
 
 
 class OutOfPages(RuntimeError):
@@ -39,14 +51,15 @@ class CacheError(RuntimeError):
 
 
 class PagePool:
-    """Free list of page numbers.  Last freed, first reused, so reuse shows up early."""
+    """Free list of page numbers, and how many requests hold each.  Last freed, first reused, so reuse shows up early."""
 
     def __init__(self, num_pages: int):
         if num_pages <= 0:
             raise ValueError("a page pool needs at least one page")
         self.num_pages = num_pages
         self._free: List[int] = list(range(num_pages - 1, -1, -1))
-        self._held = bytearray(num_pages)
+        self._held = [0] * num_pages           # holders of every page
+        self.shared = 0                        # holdings beyond a page's first
 
     @property
     def num_free(self) -> int:
@@ -60,19 +73,36 @@ class PagePool:
             self._held[p] = 1
         return out
 
+    def share(self, pages: Sequence[int]) -> None:
+        """One more request holds these pages."""
+        for p in pages:
+            if not 0 <= p < self.num_pages or not self._held[p]:
+                raise CacheError(f"page {p} shared but not held")
+            self._held[p] += 1
+        self.shared += len(pages)
+
+    def holders(self, page: int) -> int:
+        return self._held[page]
+
     def free(self, pages: Sequence[int]) -> None:
+        """One request gives these pages back."""
         for p in pages:
             if not 0 <= p < self.num_pages or not self._held[p]:
                 raise CacheError(f"page {p} freed but not held")
-            self._held[p] = 0
-            self._free.append(p)
+            self._held[p] -= 1
+            if self._held[p]:
+                self.shared -= 1
+            else:
+                self._free.append(p)
 
     def check(self) -> None:
         """No page lost or listed twice."""
         if len(set(self._free)) != len(self._free):
             raise CacheError("a page is on the free list twice")
-        if len(self._free) + sum(self._held) != self.num_pages:
+        if len(self._free) + sum(1 for h in self._held if h) != self.num_pages:
             raise CacheError("pages lost: free + held != total")
+        if self.shared != sum(h - 1 for h in self._held if h):
+            raise CacheError("shared pages miscounted")
         for p in self._free:
             if self._held[p]:
                 raise CacheError(f"page {p} is both free and held")
@@ -234,6 +264,62 @@ class CacheManager:
         del self.lengths[rid]
         del self.births[rid]
 
+    def fork(self, rid: Hashable, new_rids: Sequence[Hashable]) -> None:
+        """Start requests that go on from what `rid` holds now: its whole pages together with it, the positions behind them and its state of fixed size as
+        copies of their own.  Raises and changes nothing where names are taken or slots or pages run out."""
+        new_rids = list(new_rids)
+        if rid not in self.lengths:
+            raise CacheError(f"request {rid!r} is not live")
+        for i, new in enumerate(new_rids):
+            if new in self.lengths or new in new_rids[:i]:
+                raise CacheError(f"request {new!r} is already live")
+        if len(new_rids) > len(self._free_slots):
+            raise CacheError(f"{len(new_rids)} request slots wanted, {len(self._free_slots)} of {self.max_requests} free")
+        length = self.lengths[rid]
+        whole, rest = divmod(length, self.page_size)
+        for g in self.kv_groups:
+            if rest and len(new_rids) > g.pool.num_free:
+                raise OutOfPages(f"{len(new_rids)} pages wanted, {g.pool.num_free} of {g.pool.num_pages} free")
+        for new in new_rids:
+            slot = self._free_slots.pop()
+            self.lengths[new] = length
+            self.slots[new] = slot
+            self._born += 1
+            self.births[new] = self._born
+        for g in self.kv_groups:
+            table = g.tables[rid]
+            for new in new_rids:
+                g.pool.share([p for p in table[:whole] if p >= 0])
+                g.tables[new] = table[:whole] + (g.pool.alloc(1) if rest else [])
+            if rest and new_rids and g.device_pool is not None and table[whole] >= 0:
+                for part in g.need.page_parts(g.device_pool, self.page_size):
+                    ops().copy_pages(part, [table[whole]] * len(new_rids), [g.tables[new][whole] for new in new_rids], rest)
+        for g in self.state_groups:
+            if g.slab is not None and new_rids:
+                flat = g.slab.view(g.slab.shape[0], g.slab.shape[1], 1, -1)
+                ops().copy_pages(flat, [self.slots[rid]] * len(new_rids), [self.slots[new] for new in new_rids], 1)
+
+    def shared_prefix(self, rids: Sequence[Hashable]) -> Optional[SharedPrefix]:
+        """Which of these requests hold their first positions in the same pages, for attention over all positions: rows of one first page are a group, and
+        what it shares is the pages that all of its tables begin with.  None where nothing is shared."""
+        g = next((g for g in self.kv_groups if not g.gives_back and g.pool.shared), None)
+        if g is None:
+            return None
+        by_first: Dict[int, List[int]] = {}
+        for row, rid in enumerate(rids):
+            table = g.tables[rid]
+            if table and g.pool.holders(table[0]) > 1:
+                by_first.setdefault(table[0], []).append(row)
+        groups = []
+        for rows in by_first.values():
+            if len(rows) < 2:
+                continue
+            n = min(self.lengths[rids[r]] for r in rows) // self.page_size
+            tables = np.asarray([g.tables[rids[r]][:n] for r in rows], dtype=np.int64)
+            differ = np.nonzero((tables != tables[0]).any(axis=0))[0]
+            groups.append((rows, (int(differ[0]) if differ.size else n) * self.page_size))
+        return SharedPrefix(len(rids), groups) if groups else None
+
     def identity(self, rids: Sequence[Hashable]) -> tuple:
         """(request, number of its start) for each: equal only for the same live requests."""
         return tuple((r, self.births[r]) for r in rids)
@@ -273,17 +359,24 @@ class CacheManager:
         return out
 
     @staticmethod
-    def _short(groups, plans) -> int:
+    def _freed(g: _KVGroup, plan: Sequence[tuple], per_request) -> int:
+        """How many pages are free once everything that the plan gives back is: all of it, but for pages that other requests still hold."""
+        if not g.pool.shared:
+            return sum(len(drop) for drop, _ in per_request)
+        given = Counter(g.tables[rid][i] for (rid, _), (drop, _) in zip(plan, per_request) for i in drop)
+        return sum(1 for page, n in given.items() if n == g.pool.holders(page))
+
+    def _short(self, plan: Sequence[tuple], plans) -> int:
         short = 0
-        for g, per_request in zip(groups, plans):
-            need = sum(add - len(drop) for drop, add in per_request)
+        for g, per_request in zip(self.kv_groups, plans):
+            need = sum(add for _, add in per_request) - self._freed(g, plan, per_request)
             short = max(short, need - g.pool.num_free)
         return max(0, short)
 
     def pages_short(self, plan: Sequence[tuple]) -> int:
         """How many pages the fullest pool lacks for `plan` = [(request, new length), ...], counting
         what the plan itself gives back.  0 means the plan fits."""
-        return self._short(self.kv_groups, self._plans(plan))
+        return self._short(plan, self._plans(plan))
 
     def reserve(self, plan: Sequence[tuple]) -> None:
         """Make room for every (request, new length) of a step, or raise OutOfPages and change
@@ -298,7 +391,7 @@ class CacheManager:
             if new_len < self.lengths[rid]:
                 raise CacheError(f"request {rid!r} cannot shrink from {self.lengths[rid]} to {new_len}")
         plans = self._plans(plan)
-        short = self._short(self.kv_groups, plans)
+        short = self._short(plan, plans)
         if short:
             raise OutOfPages(f"the step needs {short} more pages than are free")
         for g, per_request in zip(self.kv_groups, plans):
@@ -324,17 +417,18 @@ class CacheManager:
         return min((g.pool.num_free for g in self.kv_groups), default=self.num_pages)
 
     def check(self) -> None:
-        """Invariants: no page lost, held by two requests, or free while held."""
+        """Invariants: no page lost, held by other requests than it counts, or free while held."""
         for g in self.kv_groups:
             g.pool.check()
-            seen = set()
+            seen = Counter()
             for rid, table in g.tables.items():
-                for p in table:
-                    if p < 0:
-                        continue
-                    if p in seen:
-                        raise CacheError(f"page {p} is held twice")
-                    seen.add(p)
+                held = [p for p in table if p >= 0]
+                if len(set(held)) != len(held):
+                    raise CacheError(f"request {rid!r} holds a page twice")
+                seen.update(held)
+            for p, n in seen.items():
+                if g.pool.holders(p) != n:
+                    raise CacheError(f"page {p} is held by {n} requests and counts {g.pool.holders(p)}")
             if len(seen) + g.pool.num_free != g.pool.num_pages:
                 raise CacheError("pages held by requests + free != total")
         if len(set(self.slots.values())) != len(self.slots):

@@ -63,6 +63,7 @@ __global__ void __launch_bounds__(AX_THREADS, 1) attention_f32_tc_kernel(P p) {
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int kvh = blockIdx.y;
+    if (att_leaves(p)) { pdl_wait(); return; }
     if (tid == 0) {
         mbar_init(&q_full, 8);
         for (int b = 0; b < 2; ++b) { mbar_init(&k_full[b], 8); mbar_init(&k_empty[b], 1); mbar_init(&v_full[b], 8); mbar_init(&v_empty[b], 1); }

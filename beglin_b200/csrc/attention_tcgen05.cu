@@ -184,7 +184,8 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
     // the blocks with the most keys (the last ones of a prompt) are handed out first, for every kv head, so that
     // the short ones fill the machine's last wave
-    const int kvh = blockIdx.x, qb = (int)gridDim.y - 1 - (int)blockIdx.y;
+    // (SHARED: its list is in that order, those without work at its end)
+    const int kvh = blockIdx.x, qb = SHARED ? (int)blockIdx.y : (int)gridDim.y - 1 - (int)blockIdx.y;
     // (the list is older than the step: a CTA without work leaves before it holds anything, but not before the kernel ahead: this grid may have no work
     // at all, and the one behind counts on that kernel being done)
     if constexpr (SHARED) {

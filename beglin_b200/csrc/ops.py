@@ -874,7 +874,7 @@ class SharedPlan:
             self.device = torch.device("cuda", torch.cuda.current_device())
         self.sms = sm_count(self.device) if self.device.type == "cuda" else 148
         if kernel == "tc":
-            self.room, sizes = _shared.items_room(n_rows, nh // nkv, nkv, self.sms), (n_rows, n_rows, n_rows)
+            self.room, sizes = _shared.items_room(n_rows, nh // nkv, nkv, self.sms, fixed), (n_rows, n_rows, n_rows)
         else:
             self.room, sizes = _shared.blocks_room(n_rows), (2 * n_rows,)
         # one buffer, so that a renewal is one copy: the list, then the rows' numbers

@@ -134,6 +134,7 @@ def shared_items(shared, group_heads: int, nkv: int, sms: int, room: int, most: 
     return out, rows, first, parts
 
 
-def items_room(n_rows: int, group_heads: int, nkv: int, sms: int) -> int:
-    """Room for the items of any groups of n rows: three waves of CTAs, or a range for every block of every group (a group has two rows at least)."""
-    return max(-(-3 * sms // nkv), n_rows // 2 + -(-n_rows * group_heads // 256) + 1)
+def items_room(n_rows: int, group_heads: int, nkv: int, sms: int, fixed: bool = False) -> int:
+    """Room for the items of any groups of n rows: three waves of CTAs (one, where the launch always has as many), or a range for every block of every group
+    (a group has two rows at least)."""
+    return max(-(-(1 if fixed else 3) * sms // nkv), n_rows // 2 + -(-n_rows * group_heads // 256) + 1)

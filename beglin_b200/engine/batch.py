@@ -12,6 +12,8 @@ from typing import Dict, Hashable, List, Optional, Sequence, Tuple
 import numpy as np
 import torch
 
+from ..csrc import ops
+
 
 @dataclass
 class Entry:
@@ -92,6 +94,19 @@ class StepBatch:
         self.slots: Optional[torch.Tensor] = dev.get("slots")
         self.scratch: Dict[object, object] = {}       # per-step tables made by parts (rotary tables)
         self._qblk: Dict[int, Tuple[torch.Tensor, int]] = {}
+        # which rows hold their first positions in the same pages (single tokens only: portions take their pages alone)
+        self.shared = cache.shared_prefix([e.rid for e in self.entries]) if cache is not None and self.decode_only and self.n_req > 1 else None
+
+    def shared_plan(self, *sizes, **options):
+        """The plan of `ops.shared_attention` for heads of these sizes (`ops.shared_plan`'s arguments behind the groups), or None where nothing is read for
+        several rows at once."""
+        if self.shared is None:
+            return None
+        key = ("shared", sizes, tuple(sorted(options.items())))
+        if key not in self.scratch:
+            plan = ops.shared_plan(self.shared, *sizes, device=self.device, **options)
+            self.scratch[key] = plan if plan.shares else None
+        return self.scratch[key]
 
     def long_blocks(self, bq: int, min_rows: int):
         """`cut_long_requests` of this step on the device: (short, n, blocks, n, longs, n), one upload."""

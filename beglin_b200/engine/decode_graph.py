@@ -17,6 +17,10 @@ float32 kernel cuts the keys at fixed positions, so a replayed float32 step comp
 bitwise as the uncaptured step function does; the bfloat16 decoding kernel spreads a request's keys
 over a number of CTAs that depends on the batch's size and the context limit, so there a replayed
 step agrees with the uncaptured one up to rounding only.
+
+A step comes in variants, each captured when it first comes: requests that share their first positions (the layers read those
+once for all of them; the groups are data that change with the requests) or not, tokens chosen under rules (penalties, biases;
+and masks) or from the logits as they are.
 """
 from __future__ import annotations
 
@@ -26,7 +30,9 @@ import numpy as np
 import torch
 
 from ..cache.manager import CacheError, OutOfPages
+from ..cache.shared import SharedPrefix
 from ..csrc import ops
+from ..sampling.rules import RuleTables
 from .capture import no_collection
 
 
@@ -65,8 +71,23 @@ class _StaticBatch:
         self.slots = torch.zeros(n, **i32)
         self.block_tables = {gi: torch.full((n, cache.max_pages), -1, **i32) for gi in range(len(cache.kv_groups))}
         self.scratch: Dict[object, object] = {}
+        self.shared: Optional[SharedPrefix] = None     # the groups of the step, where its variant reads them
+        self.plans: Dict[object, object] = {}          # one per head size, of fixed shape
         self._qblk = torch.stack([torch.arange(n), torch.arange(n), torch.ones(n, dtype=torch.long)], dim=1) \
             .to(torch.int32).to(device).contiguous()
+
+    def shared_plan(self, *sizes, **options):
+        """As `StepBatch.shared_plan`; the plans stay, and `renew` brings them up to date."""
+        if self.shared is None:
+            return None
+        key = (sizes, tuple(sorted(options.items())))
+        if key not in self.plans:
+            self.plans[key] = ops.shared_plan(self.shared, *sizes, device=self.device, fixed=True, **options)
+        return self.plans[key]
+
+    def renew(self, shared: SharedPrefix) -> None:
+        for plan in self.plans.values():
+            plan.update(shared)
 
     def query_blocks(self, bq: int) -> Tuple[Optional[torch.Tensor], int]:
         """Block i is row i of request i.  The decoding kernel knows that without a list (bq == 1 and
@@ -105,11 +126,14 @@ class DecodeGraph:
         self.h_out = torch.zeros(n, dtype=torch.int32).pin_memory()
         self.h_in = torch.zeros(n, dtype=torch.int32).pin_memory()
         self.h_in_np = self.h_in.numpy()
-        self.graph: Optional[torch.cuda.CUDAGraph] = None
-        # the same step with the host's tokens copied in at its head and the sampled ones copied out at its
-        # tail, for a caller that feeds every step from the host and reads every result: one launch per step
-        self.graph_fed: Optional[torch.cuda.CUDAGraph] = None
-        self.launches = 0
+        # (graph, its kernels, its logits) of every variant (fed, shared, rules).  fed: with the host's tokens copied in at its head and the
+        # sampled ones copied out at its tail, for a caller that feeds every step from the host and reads every result: one launch
+        # per step
+        self.graphs: Dict[tuple, tuple] = {}
+        self._groups: Optional[SharedPrefix] = None    # what the requests share, for the variants that read it
+        self._shares = False
+        self.rules: Optional[RuleTables] = None
+        self._rules_of = None                  # (rids, positions) whose texts and rules the tables hold
         self.h2d_bytes = 0                     # bytes uploaded by the last step
         self._rids: Optional[tuple] = None     # what the device buffers describe
         self._positions: Optional[List[int]] = None
@@ -118,23 +142,26 @@ class DecodeGraph:
         self._ahead = None                     # ((rids), positions) whose pages and tables are in place already
         self._ahead_bytes = 0
 
-    def _body(self) -> None:
+    def _body(self, rules: str) -> None:
         b = self.batch
         b.scratch.clear()
         logits = self.engine.model.forward(b, self.engine.cache)
+        if rules:                              # (positions[r] tokens lie in front of a row's input token)
+            self.rules.apply(logits, b.positions, b.token_ids, self.engine.ctx.status, rules == "masks")
         # the sampled tokens become the next step's input and the positions move on inside the sampling kernel, so
         # the next step of the same requests needs no upload and the graph holds no kernel but the package's own
         ops.sample(logits, self.temperature, self.uniform, self.out_tokens, feed_tokens=b.token_ids,
                    feed_positions=b.positions, advance=self.advance)
         self.logits = logits
 
-    def _body_fed(self) -> None:
+    def _body_fed(self, rules: str) -> None:
         self.batch.token_ids.copy_(self.h_in, non_blocking=True)
-        self._body()
+        self._body(rules)
         self.h_out.copy_(self.out_tokens, non_blocking=True)
 
-    def _capture(self, fed: bool = False) -> None:
+    def _capture(self, fed: bool, shared: bool, rules: str) -> None:
         body = self._body_fed if fed else self._body
+        self.batch.shared = self._groups if shared else None
         side = torch.cuda.Stream(device=self.engine.device)
         side.wait_stream(torch.cuda.current_stream())
         saved_tokens, saved_pos = self.batch.token_ids.clone(), self.batch.positions.clone()
@@ -143,7 +170,7 @@ class DecodeGraph:
             # same step again: keys and values are written twice with the same contents, and state of fixed
             # size, which a mixer reads, changes and writes, is put back as it was.
             saved_state = self.engine.cache.snapshot_state()
-            self._body()
+            self._body(rules)
             self.engine.cache.restore_state(saved_state)
             self.batch.token_ids.copy_(saved_tokens)
             self.batch.positions.copy_(saved_pos)
@@ -152,12 +179,22 @@ class DecodeGraph:
         before = ops.launch_count()
         g = torch.cuda.CUDAGraph()
         with no_collection(), torch.cuda.graph(g):
-            body()
-        self.launches = ops.launch_count() - before
-        if fed:
-            self.graph_fed = g
-        else:
-            self.graph = g
+            body(rules)
+        self.graphs[fed, shared, rules] = (g, ops.launch_count() - before, self.logits)
+        self.batch.shared = None
+
+    def _regroup(self, rids) -> None:
+        """What the step's requests share: kept for the plans of the variant that reads it, and whether that variant pays."""
+        found = self.engine.cache.shared_prefix(rids) if len(rids) > 1 else None
+        if found is None:
+            self._groups, self._shares = None, False
+            return
+        groups = SharedPrefix(self.n, found.groups)
+        if groups != self._groups:
+            self._groups = groups
+            self.batch.renew(groups)
+            # (before the first such step there is no plan to ask: it is captured, and its plans answer from then on)
+            self._shares = not self.batch.plans or any(plan.shares for plan in self.batch.plans.values())
 
     def _upload_tables(self, rids, st) -> int:
         """Upload the block tables that differ from what the device holds; returns the bytes sent.  The
@@ -205,13 +242,28 @@ class DecodeGraph:
             return False
         return all(cache.length(r) == p for r, p in zip(rids, self._ahead[1]))
 
+    def _load_rules(self, key, positions, rows) -> Tuple[str, int]:
+        """Bring the tables of the rows' rules up to date: (variant, bytes sent)."""
+        if rows is None or all(r is None or r.plain for r, _, _ in rows):
+            return "", 0
+        sent = 0
+        if self.rules is None:
+            self.rules = RuleTables(self.n, self.engine.vocab, self.engine.cache.max_context, self.engine.device)
+        if self._rules_of != (key, positions):
+            sent += self.rules.load(rows)
+        # (the step adds its input token to every text)
+        self._rules_of = (key, [p + 1 for p in positions])
+        sent += self.rules.load_masks(rows)
+        return ("masks" if self.rules.masked else "rules"), sent
+
     def step(self, rids: Sequence[Hashable], tokens: Optional[Sequence[int]], temperatures: Optional[Sequence[float]] = None,
-             uniforms: Optional[Sequence[float]] = None, read_back: bool = True):
+             uniforms: Optional[Sequence[float]] = None, read_back: bool = True, rules: Optional[Sequence] = None):
         """One decoding step for `rids` (all live, pages reserved by the caller for one more position
         each).  `tokens` None means: feed what the previous replay sampled (kept on the device).
         Returns the sampled tokens as a list (read_back) or the device tensor.  Only what changed since
         the last step is uploaded: positions advance on the device, block tables change when a request
-        gets a new page."""
+        gets a new page.  `rules`: (LogitRules or None, prompt, generated tokens) of every request; the tokens are those that the host
+        knows, the step's input last."""
         cache, n, b = self.engine.cache, self.n, self.batch
         m = len(rids)
         assert 1 <= m <= n
@@ -231,6 +283,8 @@ class DecodeGraph:
             b.slots.copy_(st.meta[1], non_blocking=True)
             self.advance.copy_(st.meta[2], non_blocking=True)
             sent += 12 * n
+            if key != self._rids:
+                self._regroup(rids)
             self._rids = key
         fed = tokens is not None and read_back     # the copies in and out are part of the replayed graph
         if fed:
@@ -253,21 +307,22 @@ class DecodeGraph:
         elif self._sampling:
             self.temperature.zero_()
             self._sampling = False
+        variant, loaded = self._load_rules(key, positions, rules)
+        sent += loaded
         if self._ahead != (key, positions):    # else the last step has brought the tables up to date already
             sent += self._upload_tables(rids, st)
         if sent > (4 * n if fed else 0):
             st.event = torch.cuda.Event()
             st.event.record()
         self.h2d_bytes = sent + self._ahead_bytes
-        if fed:
-            if self.graph_fed is None:
-                self._capture(fed=True)
-            self.graph_fed.replay()
-        else:
-            if self.graph is None:
-                self._capture()
-            self.graph.replay()
-        ops.count_launches(self.launches)
+        which = (fed, self._shares, variant)
+        if which not in self.graphs:
+            self._capture(*which)
+        graph, launches, self.logits = self.graphs[which]
+        graph.replay()
+        ops.count_launches(launches)
+        if self._shares and which[1]:          # (the first such step has made the plans)
+            self._shares = any(plan.shares for plan in self.batch.plans.values())
         cache.commit([(r, p + 1) for r, p in zip(rids, positions)])
         self._positions = [p + 1 for p in positions]
         self._look_ahead(key, rids)

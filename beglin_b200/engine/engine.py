@@ -18,6 +18,7 @@ from ..cache.manager import CacheManager
 from ..config import load_config
 from ..csrc import ops
 from ..parts.context import BuildContext
+from ..sampling.rules import LogitRules
 from ..sampling.sampler import Sampler, uniform
 from ..weights import Checkpoint, TensorDict, bind, random_tensors
 from .batch import Entry, StepBatch
@@ -183,6 +184,12 @@ class Engine:
     def release(self, rid: Hashable) -> None:
         self.cache.release(rid)
 
+    def fork(self, rid: Hashable, new_rids: Sequence[Hashable]) -> None:
+        """Start requests that go on from what `rid` holds: several completions of one text.  Its whole pages are shared (a step of single tokens reads those
+        once for all requests), the positions behind them and state of fixed size copied."""
+        with torch.cuda.device(self.device):
+            self.cache.fork(rid, new_rids)
+
     # ------------------------------------------------------------------ decoding as a CUDA graph
     def decode_graph(self, n: int):
         """The graph that serves decoding steps of n requests: one per bucket of batch sizes (1, 2, 4, ...),
@@ -197,26 +204,42 @@ class Engine:
 
     def decode(self, rids: Sequence[Hashable], tokens: Optional[Sequence[int]] = None,
                temperatures: Optional[Sequence[float]] = None, uniforms: Optional[Sequence[float]] = None,
-               read_back: bool = True):
+               read_back: bool = True, rules: Optional[Sequence] = None):
         """One decoding step for live requests, one token each, run as a replayed CUDA graph:
         `tokens` (host ids; None feeds what the last step sampled, kept on the device) in, the
-        sampled tokens out (greedy unless temperatures and uniform numbers are given)."""
+        sampled tokens out (greedy unless temperatures and uniform numbers are given).  `rules`: (LogitRules or None, prompt, generated
+        tokens, the step's input last) of every request."""
         g = self.decode_graph(len(rids))
         if not g.prepared(rids):               # else the last step made room while the device was busy
             self.cache.reserve([(r, self.cache.length(r) + 1) for r in rids])
         with torch.cuda.device(self.device):
-            return g.step(rids, tokens, temperatures, uniforms, read_back)
+            return g.step(rids, tokens, temperatures, uniforms, read_back, rules)
 
     # ------------------------------------------------------------------ generation
     def generate(self, prompts: Sequence[Sequence[int]], max_new_tokens: Union[int, Sequence[int]] = 32,
                  temperature: float = 0.0, seed: int = 0, stop_ids: Optional[Sequence[int]] = None,
                  max_batch: Optional[int] = None, max_step_tokens: int = 2048,
-                 prefill_budget: Optional[int] = None, return_requests: bool = False, mixed: bool = True):
+                 prefill_budget: Optional[int] = None, return_requests: bool = False, mixed: bool = True, completions: int = 1,
+                 rules: Union[None, LogitRules, Sequence[Optional[LogitRules]]] = None):
         """Generate for every prompt (lists of token ids on the host) and return the new token ids
         per prompt (the stop token included, as the reference records it, qwen_infer.c:2032-2039).
         `stop_ids` defaults to the configuration's eos ids; pass () to run to the token limit, as
         the reference's `greedy` mode does.  `mixed` False runs every prompt in steps of its own while the
-        decoding requests wait (the reference's QWEN_CB_MIXED=0); the tokens are the same."""
+        decoding requests wait (the reference's QWEN_CB_MIXED=0); the tokens are the same.
+
+        `completions` k > 1: k completions of every prompt, which goes through the model once; the result is then a list of k lists per
+        prompt.  `rules`: what the choice of tokens obeys (`sampling.LogitRules`: penalties, biases, a mask of the tokens that may come
+        next), one for all prompts or one for each."""
+        if completions < 1:
+            raise ValueError(f"completions={completions}, at least one")
+        if rules is None or isinstance(rules, LogitRules):
+            rules = [rules] * len(prompts)
+        if len(rules) != len(prompts):
+            raise ValueError(f"rules for {len(rules)} of {len(prompts)} prompts")
+        for r in rules:
+            if r is not None:
+                r.check(self.vocab)
+        ruled = any(r is not None and not r.plain for r in rules)
         if stop_ids is None:
             stop_ids = tuple(self.spec.eos_ids)
         if isinstance(max_new_tokens, int):
@@ -228,30 +251,48 @@ class Engine:
             bad = [t for t in p if not 0 <= int(t) < self.vocab]
             if bad:
                 raise ValueError(f"prompt {i}: token id {bad[0]} is outside the vocabulary [0, {self.vocab})")
-            r = Request(rid=("gen", i), prompt=[int(t) for t in p], max_new_tokens=int(n),
-                        temperature=float(temperature), seed=int(seed), stop_ids=tuple(stop_ids))
-            reqs.append(r)
+            family = [Request(rid=("gen", i) if j == 0 else ("gen", i, j), prompt=[int(t) for t in p], max_new_tokens=int(n),
+                              temperature=float(temperature), seed=int(seed), stop_ids=tuple(stop_ids), rules=rules[i]) for j in range(completions)]
+            reqs += family
             if n <= 0:
-                r.phase, r.finish_reason = "done", "length"
+                for r in family:
+                    r.phase, r.finish_reason = "done", "length"
             else:
-                sched.add(r)
+                family[0].siblings = family[1:]
+                sched.add(family[0])
+
+        def draws(rs):
+            # (a prompt's first completion draws as it would alone)
+            key = lambda r: r.rid[1] if len(r.rid) == 2 else r.rid[1:]
+            return [r.temperature for r in rs], [uniform(r.seed, key(r), len(r.output)) if r.temperature > 0 else 0.0 for r in rs]
+
+        told = lambda rs: [(r.rules, r.prompt, r.output) for r in rs] if ruled else None
         try:
             while True:
                 plan = sched.plan()
                 if plan is None:
                     break
                 wanted = sched.wanted(plan)
-                temps = [r.temperature for r in wanted]
-                us = [uniform(r.seed, r.rid[1], len(r.output)) if r.temperature > 0 else 0.0 for r in wanted]
+                temps, us = draws(wanted)
                 tokens: List[int] = []
                 if self.use_graphs and not plan.prefill:
                     with torch.cuda.device(self.device):
                         tokens = self.decode_graph(len(wanted)).step(
-                            [r.rid for r in wanted], [r.output[-1] for r in wanted], temps, us)
+                            [r.rid for r in wanted], [r.output[-1] for r in wanted], temps, us, rules=told(wanted))
                 else:
                     logits = self.run(plan.entries, plan.lengths)
-                    if wanted:
-                        tokens = self.sampler.sample(logits, temps, us)
+                    with torch.cuda.device(self.device):
+                        # the other completions of a prompt that is complete now begin with its last row's logits
+                        started = [(lead, sched.adopt(lead)) for lead in sched.leads(plan)]
+                        place = {r.rid: i for i, r in enumerate(wanted)}
+                        rows = [logits[place[lead.rid]].expand(len(more), -1) for lead, more in started if more]
+                        more = [r for _, rs in started for r in rs]
+                        first: List[int] = []
+                        if more:
+                            first = self.sampler.sample(torch.cat(rows), *draws(more), rules=told(more))
+                        if wanted:
+                            tokens = self.sampler.sample(logits, temps, us, rules=told(wanted))
+                    sched.first_tokens(more, first)
                 sched.update(plan, tokens, committed=True)      # the step functions above have recorded the lengths
             ops.raise_on_status(self.ctx.status)
         finally:
@@ -261,4 +302,5 @@ class Engine:
         self.last_counters = sched.counters
         if return_requests:
             return reqs
-        return [list(r.output) for r in reqs]
+        out = [list(r.output) for r in reqs]
+        return out if completions == 1 else [out[i:i + completions] for i in range(0, len(out), completions)]

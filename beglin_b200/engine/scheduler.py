@@ -14,6 +14,9 @@ has generated appended to its prompt, to be recomputed when admitted again.  Pro
 shortened to what the free pages hold, down to nothing.  A request that does not fit even when it is
 the only one ends with the reason "out_of_pages".
 
+Several completions of one prompt are a family: the lead is a request like others, and when its prompt is in the cache the others go on from there
+(`adopt`), as far as there are slots and pages for them; the rest wait in the queue as requests with a prompt of their own.
+
 Pure host code: it talks to the cache manager's accounting and is tested without a GPU.
 """
 from __future__ import annotations
@@ -35,6 +38,8 @@ class Request:
     temperature: float = 0.0
     seed: int = 0
     stop_ids: Tuple[int, ...] = ()
+    rules: Optional[object] = None    # of choosing its tokens (sampling.LogitRules); the scheduler hands them on
+    siblings: List["Request"] = field(default_factory=list)       # further completions of its prompt, not in the queue
     # filled by the scheduler
     output: List[int] = field(default_factory=list)
     phase: str = "waiting"            # waiting, prefill, decode, done
@@ -120,11 +125,19 @@ class Scheduler:
 
     def _finish(self, req: Request, reason: str) -> None:
         req.phase, req.finish_reason = "done", reason
+        self._end_family(req, reason)
         if self.cache.has(req.rid):
             self.cache.release(req.rid)
         if req in self.running:
             self.running.remove(req)
         self.finished.append(req)
+
+    def _end_family(self, lead: Request, reason: str) -> None:
+        """Siblings that still wait for a lead whose prompt will not be complete end with it."""
+        for r in lead.siblings:
+            r.phase, r.finish_reason = "done", reason
+            self.finished.append(r)
+        lead.siblings = []
 
     def _preempt(self, req: Request) -> None:
         """Give back what `req` holds and queue it again, first in line, to be recomputed."""
@@ -145,6 +158,7 @@ class Scheduler:
                 self.waiting.popleft()
                 self.finished.append(req)
                 req.phase, req.finish_reason = "done", "context_limit"
+                self._end_family(req, "context_limit")
                 continue
             if self.running and self.cache.free_pages() < 1:
                 break                               # no room to make progress on another request
@@ -256,18 +270,52 @@ class Scheduler:
                 c.gaps += 1
                 c.gap_sum_s += gap
                 c.gap_max_s = max(c.gap_max_s, gap)
-            r.last_token_at = now
-            r.output.append(int(tok))
-            r.phase = "decode"
-            length = self.cache.length(r.rid)
-            if int(tok) in r.stop_ids:
-                reason = "stop"
-            elif len(r.output) >= r.max_new_tokens:
-                reason = "length"
-            elif length + 1 > self.max_context:
-                reason = "context_limit"
-            else:
-                continue
-            self._finish(r, reason)
-            ended.append(r)
+            if self._record(r, int(tok), now):
+                ended.append(r)
         return ended
+
+    def _record(self, r: Request, tok: int, now: float) -> bool:
+        """A request's new token; whether the request ended with it."""
+        r.last_token_at = now
+        r.output.append(tok)
+        r.phase = "decode"
+        if tok in r.stop_ids:
+            reason = "stop"
+        elif len(r.output) >= r.max_new_tokens:
+            reason = "length"
+        elif self.cache.length(r.rid) + 1 > self.max_context:
+            reason = "context_limit"
+        else:
+            return False
+        self._finish(r, reason)
+        return True
+
+    # ------------------------------------------------------------------ families
+    def leads(self, plan: StepPlan) -> List[Request]:
+        """The requests of the step whose prompt it completes and whose siblings wait for that."""
+        return [r for r, _, last in plan.prefill if last and r.siblings]
+
+    def adopt(self, lead: Request) -> List[Request]:
+        """Start siblings of `lead`, whose prompt's last step has run, from what it holds (before `update`, which may end it).  Those that there is no slot or
+        page for go to the head of the queue.  Returns those that have started: each takes its first token from the lead's logits (`first_tokens`)."""
+        family, lead.siblings = lead.siblings, []
+        free = min(self.max_batch - len(self.running), self.cache.max_requests - len(self.cache.live()))
+        if self.cache.length(lead.rid) % self.cache.page_size:
+            free = min(free, self.cache.free_pages())
+        now, later = family[:max(free, 0)], family[max(free, 0):]
+        if now:
+            self.cache.fork(lead.rid, [r.rid for r in now])
+        for r in now:
+            r.tokens_in, r.done_prompt = list(r.prompt), len(r.prompt)
+            r.admitted_at = self._clock
+            self._clock += 1
+            self.running.append(r)
+        for r in reversed(later):
+            r.tokens_in, r.phase = list(r.prompt), "waiting"
+            self.waiting.appendleft(r)
+        return now
+
+    def first_tokens(self, started: Sequence[Request], tokens: Sequence[int]) -> None:
+        now = self._now()
+        for r, tok in zip(started, tokens):
+            self._record(r, int(tok), now)

@@ -15,6 +15,9 @@ positions; a gate, sigmoid of a further
 product of the mixer's input, on the joined heads before the output product, feature by feature or one number per head.  The gate's matrix is
 one more block of rows of the one q/k/v product.  With any of the first two the kernel that norms, rotates and appends
 is `qk_norm_rope_append`.
+
+A step of single tokens whose requests hold their first positions in the same pages (requests that go on from one text) reads those once for all of
+them (`shared_attention`), where a query sees every position.
 """
 from __future__ import annotations
 
@@ -150,6 +153,8 @@ class GQAAttention:
         self.slopes = None if spec.slopes is None else torch.tensor(spec.slopes, dtype=torch.float64).to(torch.float32).to(ctx.device)
         # what the kernels are told: a positive number is a sliding window, a negative one the size of the blocks
         self.window = int(spec.window) if spec.window else (-int(spec.block) if spec.block else 0)
+        # positions that requests share are read once where a query sees them all, whatever their distance
+        self.sees_all = spec.window is None and spec.block is None and spec.slopes is None
         # the fused q/k/v product can rotate and append itself: whole heads rotated in halves, a cache of its own
         # in bfloat16
         self.rope_in_product = (spec.own_kv and self.position.rotary_dim == self.hd and not self.position.interleaved
@@ -171,13 +176,21 @@ class GQAAttention:
                                    split=ctx.kv_split, bq=bq, tile=tile, sink=int(bool(s.sink)), scale=self.scale, softcap=self.score_cap)
                 for d, (_, bq, tile) in self.plans.items()}
 
+    def _shared_plan(self, batch):
+        if not self.sees_all or getattr(batch, "shared", None) is None:
+            return None
+        khd, kvd_ = (self.hd, self.vd) if self.stored is None else (self.stored, self.stored)
+        return batch.shared_plan(self.nh, self.nkv, khd, self.ctx.cache_dtype, page_size=self.ctx.page_size, vd=kvd_, split=self.ctx.kv_split,
+                                 prefer="generic" if self.ctx.attention == "generic" else "auto", query_dtype=self.ctx.compute_dtype)
+
     takes_stream = True        # forward takes a NormedInput and may add its result to the stream itself
 
     def forward(self, h, batch, cache: PagedKVView, stream: Optional[ResidualStream] = None) -> Optional[torch.Tensor]:
         """h: the normed rows, or a NormedInput.  With `stream` the result is added to it (or left owed to
         it) and None is returned; without, the addend is returned."""
         T = batch.n_rows
-        if self._args is not None and not ops.profiling():
+        shared = self._shared_plan(batch)
+        if self._args is not None and shared is None and not ops.profiling():
             rows = h if isinstance(h, torch.Tensor) else h.tensor()
             args = self._args[bool(getattr(batch, "decode_only", False))]
             qblk, n_qblk = batch.query_blocks(args.bq)
@@ -213,16 +226,20 @@ class GQAAttention:
             ops.rope_kv_append(qkv, q, T, self.nh, self.nkv, self.hd, self.position.rotary_dim, self.position.interleaved,
                                self.position.table(batch), batch.positions, batch.row_req, cache.block_table,
                                cache.pool if self.spec.own_kv else None, cache.page_size, self.ctx.status)
-        kernel, bq, tile = self.plans[bool(getattr(batch, "decode_only", False))]
-        qblk, n_qblk = batch.query_blocks(bq)
-        if qblk is None and kernel != "mma_keys":
-            batch.implicit_blocks = False              # this kernel wants the list
-            qblk, n_qblk = batch.query_blocks(bq)
         out = torch.empty((T, self.nh * kvd_), dtype=self.ctx.compute_dtype, device=q.device)
-        ops.attention(q, q.stride(0), cache.pool, cache.block_table, batch.positions, qblk, n_qblk,
-                      batch.max_position, T, self.nh, self.nkv, khd, self.window, self.ctx.kv_split, tile, bq,
-                      self.scale, out, self.ctx.status, kernel, vd=kvd_, sink=bool(self.spec.sink),
-                      sink_weight=self.sink_weight, softcap=self.score_cap, keep=self.spec.keep_first, slopes=self.slopes)
+        if shared is not None:
+            ops.shared_attention(q, cache.pool, cache.block_table, batch.positions, shared, batch.max_position, self.scale, out, self.ctx.status,
+                                 sink=bool(self.spec.sink), sink_weight=self.sink_weight, softcap=self.score_cap)
+        else:
+            kernel, bq, tile = self.plans[bool(getattr(batch, "decode_only", False))]
+            qblk, n_qblk = batch.query_blocks(bq)
+            if qblk is None and kernel != "mma_keys":
+                batch.implicit_blocks = False          # this kernel wants the list
+                qblk, n_qblk = batch.query_blocks(bq)
+            ops.attention(q, q.stride(0), cache.pool, cache.block_table, batch.positions, qblk, n_qblk,
+                          batch.max_position, T, self.nh, self.nkv, khd, self.window, self.ctx.kv_split, tile, bq,
+                          self.scale, out, self.ctx.status, kernel, vd=kvd_, sink=bool(self.spec.sink),
+                          sink_weight=self.sink_weight, softcap=self.score_cap, keep=self.spec.keep_first, slopes=self.slopes)
         gate_per = self.vd if self.spec.gate == "head" else 1      # one gate per head, or one per feature
         if self.spec.gate is not None and self.stored is None:
             ops.sigmoid_gate(out, qkv, self.gate_col, self.od, gate_per=gate_per)

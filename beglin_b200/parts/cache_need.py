@@ -7,7 +7,7 @@ for paged keys and values, one slab of slots for per-request state of fixed size
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import Optional, Tuple
+from typing import List, Optional, Tuple
 
 import torch
 
@@ -33,6 +33,16 @@ class PagedKVNeed:
             return (2, self.n_kv_heads, page_size, self.head_dim)
         return (self.n_kv_heads * page_size * (self.head_dim + self.v_head_dim),)
 
+    def page_parts(self, pool: torch.Tensor, page_size: int) -> List[torch.Tensor]:
+        """The pool [stages, pages, *page_shape] as views [stages, pages, ..., positions, features]."""
+        if self.v_head_dim is None or self.v_head_dim == self.head_dim:
+            return [pool]
+        n, at, parts = self.n_kv_heads, pool.storage_offset(), []
+        for width in (self.head_dim, self.v_head_dim):
+            parts.append(pool.as_strided((pool.shape[0], pool.shape[1], n, page_size, width), (pool.stride(0), pool.stride(1), page_size * width, width, 1), at))
+            at += n * page_size * width
+        return parts
+
 
 @dataclass(frozen=True)
 class PagedLatentNeed:
@@ -44,6 +54,9 @@ class PagedLatentNeed:
 
     def page_shape(self, page_size: int) -> Tuple[int, ...]:
         return (page_size, self.width)
+
+    def page_parts(self, pool: torch.Tensor, page_size: int) -> List[torch.Tensor]:
+        return [pool]
 
 
 PAGED_NEEDS = (PagedKVNeed, PagedLatentNeed)

@@ -10,12 +10,13 @@ from __future__ import annotations
 
 import zlib
 from dataclasses import dataclass
-from typing import Hashable, List, Sequence
+from typing import Hashable, List, Optional, Sequence
 
 import numpy as np
 import torch
 
 from ..csrc import ops
+from .rules import RuleTables
 
 _MASK = (1 << 64) - 1
 
@@ -52,9 +53,16 @@ class Sampler:
     def __init__(self, device):
         self.device = torch.device(device)
 
-    def sample(self, logits: torch.Tensor, temperatures: Sequence[float], uniforms: Sequence[float]) -> List[int]:
-        """One token per row of float logits [n, V]; rows with temperature <= 0 are greedy."""
+    def sample(self, logits: torch.Tensor, temperatures: Sequence[float], uniforms: Sequence[float], rules: Optional[Sequence] = None) -> List[int]:
+        """One token per row of float logits [n, V]; rows with temperature <= 0 are greedy.  `rules`: (LogitRules or None, prompt, generated tokens) of every row;
+        the logits are changed by them."""
         n = logits.shape[0]
+        if rules is not None and any(r is not None and not r.plain for r, _, _ in rules):
+            lengths = [len(prompt) + len(made) for _, prompt, made in rules]
+            tables = RuleTables(n, logits.shape[1], max(lengths), logits.device)
+            tables.load(rules)
+            tables.load_masks(rules)
+            tables.apply(logits, torch.tensor(lengths, dtype=torch.int32).to(logits.device), None, None, tables.masked)
         out = torch.empty(n, dtype=torch.int32, device=logits.device)
         if any(t > 0.0 for t in temperatures):
             t = torch.from_numpy(np.asarray(temperatures, dtype=np.float32)).to(logits.device)
