@@ -78,9 +78,14 @@ __device__ __forceinline__ AttBlock att_block(const AttnSharedParams& p, int qb)
     const int sp = a.w + (int)blockIdx.z;
     return {a.x, a.y, sp < b.x ? a.z : 0, sp, b.y};
 }
-// whether CTAs without a block leave before they set anything up (in a list of fixed length many have none)
+// whether CTAs without a block leave before they set anything up (in a list of fixed length many have none) ..
 __device__ __forceinline__ bool att_leaves(const AttnParams&) { return false; }
-__device__ __forceinline__ bool att_leaves(const AttnSharedParams& p) { return att_block(p, blockIdx.x).nq <= 0; }
+// .. and those whose splits lie behind their row's position (which no kernel of the step writes)
+__device__ __forceinline__ int att_end(const AttnSharedParams& p, const AttBlock& b);
+__device__ __forceinline__ bool att_leaves(const AttnSharedParams& p) {
+    const AttBlock b = att_block(p, blockIdx.x);
+    return b.nq <= 0 || b.sp * p.split > att_end(p, b);
+}
 __device__ __forceinline__ int att_row(const AttnParams&, int i) { return i; }
 __device__ __forceinline__ int att_row(const AttnSharedParams& p, int i) { return p.rows[i]; }
 // the last position that any row of the block sees

@@ -273,7 +273,9 @@ attention_mma_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_co
             if (!EXT && (s >= n_stage || o >= n_box || key_lo >= k_end || key_lo + ps <= k_begin || (key_lo >> shift) >= p.max_pages)) return -1;
             if (EXT && (s >= n_stage || o >= n_box || key_lo >= k_end || (key_lo >> shift) >= p.max_pages ||
                         (key_lo + ps <= k_begin && !(has_kept && key_lo < kept_end && key_lo + ps > k_first)))) return -1;
-            return table[key_lo >> shift];
+            const int held = table[key_lo >> shift];
+            if (SHARED && held < 0 && p.status) atomicOr(p.status, BG_STATUS_BAD_PAGE);
+            return held;
         };
         // stages of old keys only may be asked for before the kernel ahead has finished: all but the one that
         // holds the newest position

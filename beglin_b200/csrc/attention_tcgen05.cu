@@ -208,7 +208,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&tmem_sh)), "r"(TMEM_COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
     }
-    pdl_wait();
+    if constexpr (!SHARED) pdl_wait();
     int req, row0, nq;
     if constexpr (SHARED) { req = p.items[qb * 8 + 0]; row0 = p.items[qb * 8 + 1]; nq = p.items[qb * 8 + 2]; }
     else { req = p.qblk[qb * 3 + 0]; row0 = p.qblk[qb * 3 + 1]; nq = p.qblk[qb * 3 + 2]; }
@@ -235,19 +235,35 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
     auto tile_key = [&](int i) { return (EXT && i < n_kept ? i : tile0 + i - n_kept) * AT_BK; };
 
     // ---- Q into shared memory: row r, column block cb, 16-byte piece c at r*128 + ((c ^ (r & 7)) * 16)
-    for (int idx = tid; idx < (SHARED && twice ? 2 : 1) * AT_BM * (HD / 8); idx += (SHARED ? AT_SHARED_THREADS : AT_THREADS)) {
-        const int r = idx / (HD / 8), c = idx - r * (HD / 8);
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (r < n_rows)
-            v = *reinterpret_cast<const uint4*>(p.q + (size_t)batch_row(r) * p.q_stride + (size_t)(kvh * group + head_of(r)) * HD + c * 8);
-        const int cb = c >> 3, cc = c & 7;
-        const int rr = SHARED ? r & (AT_BM - 1) : r;
-        *reinterpret_cast<uint4*>(q_s + (SHARED ? (r / AT_BM) * QT_BYTES : 0) + cb * (AT_BM * 128) + rr * 128 + ((cc ^ (rr & 7)) << 4)) = v;
+    auto load_queries = [&](int first, int step) {
+        for (int idx = first; idx < (SHARED && twice ? 2 : 1) * AT_BM * (HD / 8); idx += step) {
+            const int r = idx / (HD / 8), c = idx - r * (HD / 8);
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (r < n_rows)
+                v = *reinterpret_cast<const uint4*>(p.q + (size_t)(SHARED ? row_of[r] : batch_row(r)) * p.q_stride + (size_t)(kvh * group + head_of(r)) * HD + c * 8);
+            const int cb = c >> 3, cc = c & 7;
+            const int rr = SHARED ? r & (AT_BM - 1) : r;
+            *reinterpret_cast<uint4*>(q_s + (SHARED ? (r / AT_BM) * QT_BYTES : 0) + cb * (AT_BM * 128) + rr * 128 + ((cc ^ (rr & 7)) << 4)) = v;
+        }
+        fence_proxy_async();
+    };
+    if constexpr (SHARED) {
+        // what the lists say is there before the kernel ahead is done; behind it, the keys are asked for while the others fetch the queries
+        if (tid < 2 * AT_BM) row_of[tid] = tid < n_rows ? batch_row(tid) : 0;
+        tc_fence_before();
+        __syncthreads();
+        tc_fence_after();
+        pdl_wait();
+        if (warp != 5 && warp != 7 && warp != 12 && warp != 14) {
+            load_queries((warp - (warp > 5) - (warp > 7) - (warp > 12) - (warp > 14)) * 32 + lane, AT_SHARED_THREADS - 128);
+            asm volatile("bar.sync 2, %0;\n" ::"n"(AT_SHARED_THREADS - 128) : "memory");
+        }
+    } else {
+        load_queries(tid, AT_THREADS);
+        tc_fence_before();
+        __syncthreads();
+        tc_fence_after();
     }
-    fence_proxy_async();
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
     const unsigned tmem = tmem_sh;
     // The kernel behind this one may be scheduled only now that this CTA holds its tensor memory: it takes all 512
     // columns, and a CTA of the successor that came to the same SM first and allocated a few would then wait for
@@ -617,6 +633,8 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
                 pg[h] = -1;
                 if (i < n_tiles && k < n_pg && pi < p.max_pages && key0 + k * ps < k_end && (key0 + (k + 1) * ps > k_begin || (EXT && key0 + k * ps < keep)))
                     pg[h] = p.block_table[(size_t)req * p.max_pages + pi];
+                // (what a group shares is held: where a page is not, there are no keys to read)
+                if (SHARED && pg[h] < 0 && i < n_tiles && k < n_pg && key0 + k * ps < k_end && p.status) atomicOr(p.status, BG_STATUS_BAD_PAGE);
             }
         };
         int pg_next[ROUNDS];

@@ -20,7 +20,7 @@ struct PageCopies {
 template <typename T>
 __global__ void __launch_bounds__(PAGES_THREADS) copy_pages_kernel(unsigned char* pool, long long stage_bytes, long long page_bytes, long long block_bytes,
                                                                    int per_block, long long pieces, const __grid_constant__ PageCopies c) {
-    pdl_launch();
+    // (no early start for what comes behind: the attention kernels ask for older positions before they wait for the kernel ahead of them, and these are older)
     pdl_wait();
     const long long at = (long long)blockIdx.x * PAGES_THREADS + threadIdx.x;
     if (at >= pieces) return;

@@ -180,8 +180,10 @@ class GQAAttention:
         if not self.sees_all or getattr(batch, "shared", None) is None:
             return None
         khd, kvd_ = (self.hd, self.vd) if self.stored is None else (self.stored, self.stored)
-        return batch.shared_plan(self.nh, self.nkv, khd, self.ctx.cache_dtype, page_size=self.ctx.page_size, vd=kvd_, split=self.ctx.kv_split,
+        plan = batch.shared_plan(self.nh, self.nkv, khd, self.ctx.cache_dtype, page_size=self.ctx.page_size, vd=kvd_, split=self.ctx.kv_split,
                                  prefer="generic" if self.ctx.attention == "generic" else "auto", query_dtype=self.ctx.compute_dtype)
+        # (where only the decoding kernel takes the sizes on the tensor cores, it is ahead of the float units' sharing)
+        return None if plan is None or plan.kernel == "generic" and self.plans[True][0] != "generic" else plan
 
     takes_stream = True        # forward takes a NormedInput and may add its result to the stream itself
 

@@ -16,6 +16,9 @@ import torch
 from ..csrc import ops
 
 
+MOST_BIASES = 512          # biased tokens of a request
+
+
 @dataclass(frozen=True)
 class LogitRules:
     """`allowed` is called before every token with the tokens that the request has generated so far and returns which may come next: token ids, or truth
@@ -31,6 +34,8 @@ class LogitRules:
             raise ValueError(f"repetition={self.repetition} must be positive and finite (1: none)")
         if not (math.isfinite(self.frequency) and math.isfinite(self.presence)):
             raise ValueError(f"frequency={self.frequency} and presence={self.presence} must be finite")
+        if len(self.bias) > MOST_BIASES:
+            raise ValueError(f"{len(self.bias)} biased tokens, at most {MOST_BIASES}")
         for token, value in self.bias.items():
             if not 0 <= int(token) < vocab:
                 raise ValueError(f"biased token {token} is outside the vocabulary [0, {vocab})")
@@ -75,15 +80,13 @@ class RuleTables:
     """The rules of a step's rows on the device, as `ops.adjust_logits` reads them.  Of a fixed number of rows and with room for `room` tokens of text each, so
     that a captured step reads them too; the newest token of every row is the step's input, which the kernel adds to the text."""
 
-    BIASES = 512               # biased tokens of a row that a table has room for
-
     def __init__(self, n: int, vocab: int, room: int, device):
         i32, f32 = dict(dtype=torch.int32, device=device), dict(dtype=torch.float32, device=device)
         self.n, self.vocab, self.room = n, vocab, room
         self.history = torch.zeros((n, max(room, 1)), **i32)
         self.prompts = torch.zeros(n, **i32)
         self.penalties = torch.zeros((3, n), **f32)
-        self.bias_ids, self.bias_values, self.begins = torch.zeros(n * self.BIASES, **i32), torch.zeros(n * self.BIASES, **f32), torch.zeros(n + 1, **i32)
+        self.bias_ids, self.bias_values, self.begins = torch.zeros(n * MOST_BIASES, **i32), torch.zeros(n * MOST_BIASES, **f32), torch.zeros(n + 1, **i32)
         self.allowed, self.allowed_row = torch.zeros((n, -(-vocab // 32)), **i32), torch.full((n,), -1, **i32)
         self._masked = False
         self._staged: List[torch.Tensor] = []
@@ -112,8 +115,6 @@ class RuleTables:
             history[r, :len(text)] = text
             if rules is not None:
                 pen[:, r] = rules.repetition, rules.frequency, rules.presence
-                if len(rules.bias) > self.BIASES:
-                    raise ValueError(f"{len(rules.bias)} biased tokens, at most {self.BIASES}")
                 for token in sorted(rules.bias):
                     ids.append(int(token)); values.append(float(rules.bias[token]))
             begins.append(len(ids))

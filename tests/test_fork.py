@@ -202,7 +202,7 @@ def test_a_prompt_goes_through_once():
 def test_rules_are_checked():
     from beglin_b200.sampling import LogitRules
     for bad, match in ((dict(repetition=0.0), "repetition"), (dict(repetition=float("inf")), "repetition"), (dict(frequency=float("nan")), "frequency"),
-                       (dict(bias={10: 1.0}), "outside"), (dict(bias={-1: 1.0}), "outside"), (dict(bias={1: float("nan")}), "not a number")):
+                       (dict(bias={10: 1.0}), "outside"), (dict(bias={-1: 1.0}), "outside"), (dict(bias={1: float("nan")}), "not a number"), (dict(bias={i: 1.0 for i in range(513)}), "at most")):
         with pytest.raises(ValueError, match=match):
             LogitRules(**bad).check(10)
     assert LogitRules().plain and not LogitRules(presence=0.1).plain

@@ -257,13 +257,14 @@ def test_shared_attention_twice_is_the_same(dtype):
 @pytest.mark.parametrize("prefer", ["tc", "generic"])
 @pytest.mark.parametrize("row,entry", [(0, 1), (4, 6)])
 def test_shared_attention_records_bad_pages(prefer, row, entry):
-    """A page beyond the pool in what the group shares (the first row's table counts) or among a row's own."""
+    """A page beyond the pool, or none, in what the group shares (the first row's table counts) or among a row's own."""
     c = Case(*SETS["odd"], 4, 2, 128, 64, torch.bfloat16, seed=1)
     c.lengths = [n if i != 4 else 450 for i, n in enumerate(c.lengths)]
     c.positions = torch.tensor(c.lengths, dtype=torch.int32) - 1
-    c.table[row, entry] = c.pool.shape[0]
-    with pytest.raises(ops.KernelError, match="page pool"):
-        c.run(prefer=prefer)
+    for page in (c.pool.shape[0], -1):
+        c.table[row, entry] = page
+        with pytest.raises(ops.KernelError, match="page pool"):
+            c.run(prefer=prefer)
 
 
 # ------------------------------------------------------------------------------------------------ without a GPU
