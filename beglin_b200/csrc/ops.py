@@ -899,7 +899,8 @@ class SharedPlan:
         if self.kernel == "tc":
             if not self.all_groups:
                 kept = _shared.worth_sharing(shared, self.nh // self.nkv, self.nkv, self.sms, self.room, self.MOST_RANGES,
-                                             lambda streams, positions: own_ranges(streams, positions, self.sms), 4 * self.hd)
+                                             lambda streams, positions: own_ranges(streams, positions, self.sms),
+                                             lambda streams, positions: decode_splits(streams, positions, self.sms), 4 * self.hd)
                 shared = type(shared)(self.n_rows, kept)
             arrays = _shared.shared_items(shared, self.nh // self.nkv, self.nkv, self.sms, self.room, self.MOST_RANGES)
         else:
@@ -1004,7 +1005,9 @@ def shared_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_table: torch.
     if plan.kernel == "tc":
         if status is None or out.dtype != torch.bfloat16:
             raise KernelError("shared_attention: the tensor-core kernels want a status word and write bfloat16")
-        ranges, at_once, kernels = own_ranges(T * plan.nkv, max(1, max_position + 1 - plan.least_own), plan.sms), 0, 3 if plan.n_items else 2
+        own = max(1, max_position + 1 - plan.least_own)
+        at_once, kernels = 0, 3 if plan.n_items else 2
+        ranges = own_ranges(T * plan.nkv, own, plan.sms) if plan.n_items else decode_splits(T * plan.nkv, own, plan.sms)
         floats = plan.row_floats * (plan.slots + ranges)
     else:
         ranges, kernels = max_position // plan.split + 1, 2

@@ -38,13 +38,19 @@ def blocks_room(n_rows: int) -> int:
     return n_rows + n_rows // 2 + 1 if n_rows > 1 else 1
 
 
-# What the tensor-core kernels take, in microseconds, measured on B200 with heads of 128 features: a CTA beside its tiles, a tile of 64 positions for up to 128
-# rows and for up to 256.
-CTA_US, TILE_US, PAIR_US = 6.0, 0.52, 1.03
-# The rows' own positions and the joining of results: what the two kernels take by themselves beside a CTA's positions, and behind the shared positions' kernel
-# (they begin while it runs); a position in a CTA; where more CTAs than SMs run, bytes a microsecond.
-ALONE_US, BEHIND_US, POSITION_US, OWN_RATE = 2.9, 0.4, 0.0135, 4.5e6
+# What the tensor-core kernels take, in microseconds, measured on B200 with heads of 128 features (64 do not differ much: these are latencies).  The shared
+# positions' kernel: a CTA beside its tiles, a tile of 64 positions for up to 128 rows and for up to 256; one more range is one more result to join.
+CTA_US, TILE_US, PAIR_US, RANGE_US = 6.0, 0.52, 1.03, 0.05
+# The rows' own positions and the joining of results behind it: the two kernels, a position in a CTA, bytes a microsecond of many CTAs, and what more it is
+# where the shared positions' kernel leaves them no SMs to begin on.
+BEHIND_US, OWN_POSITION_US, OWN_RATE, CROWDED_US = 0.4, 0.0135, 4.5e6, 3.6
 OWN_GUESS = 256            # positions that a request is taken to hold behind those that it shares
+# Every row by itself over all of its positions: beside a CTA's positions, and a position (pages that several rows hold come from the L2).
+ALONE_US, ALONE_POSITION_US = 6.0, 0.0058
+
+
+def _up(n: int, unit: int) -> int:
+    return -(-n // unit) * unit
 
 
 def _done(ctas: int, longest: float, total: float, sms: int) -> float:
@@ -52,19 +58,21 @@ def _done(ctas: int, longest: float, total: float, sms: int) -> float:
     return longest if ctas <= sms else max(longest, total / sms + longest / 2)
 
 
-def cut_ranges(groups: Sequence[Tuple[int, int]], nkv: int, sms: int, room: int, most: int) -> Tuple[int, int, float]:
+def cut_ranges(groups: Sequence[Tuple[int, int]], nkv: int, sms: int, room: int, most: int, streams: int = 0) -> Tuple[int, int, float]:
     """(rows of a block, positions of a range, microseconds) for groups = [(rows of a kv head, positions)]: blocks of 128 or of 256 rows, and ranges, a multiple
-    of TILE and of one length for all groups, at most `most` a group, that are through first.  No more than `room` items."""
+    of TILE and of one length for all groups, at most `most` a group, that are through first.  No more than `room` items.  Of the SMs those that the step's
+    `streams` (rows x kv heads) have use for by themselves are left to them, where they are few (two streams an SM)."""
     longest = max(p for _, p in groups)
+    left = sms - -(-streams // 2) if -(-streams // 2) <= sms // 4 else 0
     best = None
     for block in (128, 256):
         if block > 128 and all(r <= 128 for r, _ in groups):
             break
         n, last = 1, 0
         while n <= most:
-            length = -(-max(-(-longest // n), TILE) // TILE) * TILE
+            length = _up(max(-(-longest // n), TILE), TILE)
             if length != last:
-                ctas, total, slowest, items = 0, 0.0, 0.0, 0
+                total, slowest, items = 0.0, 0.0, 0
                 for r, p in groups:
                     ranges, tiles = -(-p // length), min(length, p) / TILE
                     for rows, count in ((block, r // block), (r % block, 1)):
@@ -73,38 +81,42 @@ def cut_ranges(groups: Sequence[Tuple[int, int]], nkv: int, sms: int, room: int,
                             items += ranges * count
                             total += nkv * ranges * count * one
                             slowest = max(slowest, one)
-                ctas = nkv * items
                 if items > room:
                     break
-                done = _done(ctas, slowest, total, sms) + 0.05 * -(-longest // length)       # (every range is one more result to join)
+                done = _done(nkv * items, slowest, total, sms) + RANGE_US * -(-longest // length) + (CROWDED_US if nkv * items > left else 0.0)
                 if best is None or done < best[2]:
                     best = block, length, done
             last = length
             n += 1 if n < 16 else 4
-    return best or (256, -(-longest // TILE) * TILE, 0.0)
+    return best or (256, _up(longest, TILE), 0.0)
 
 
-def own_us(lengths: Sequence[int], nkv: int, ranges, sms: int, row_bytes: int) -> float:
-    """About what the kernel of the rows' own positions takes; `ranges`(streams, positions) is how a stream is cut (in whole multiples of 256 positions)."""
-    n, longest = len(lengths), max(max(lengths), 1)
-    cut = ranges(n * nkv, longest)
-    one = -(-(-(-longest // cut)) // 256) * 256 * POSITION_US
-    return one if n * nkv * cut <= sms else max(sum(lengths) * nkv * row_bytes / OWN_RATE, one)
+def own_us(longest: int, total: int, n_rows: int, nkv: int, ranges, row_bytes: int) -> float:
+    """About what the rows' own positions take behind the shared ones, `total` in all; `ranges`(streams, positions) is how a stream is cut (in whole multiples of
+    256 positions)."""
+    one = _up(-(-longest // ranges(n_rows * nkv, longest)), 256) * OWN_POSITION_US
+    return BEHIND_US + max(total * nkv * row_bytes / OWN_RATE, one)
 
 
-def worth_sharing(shared, group_heads: int, nkv: int, sms: int, room: int, most: int, ranges, row_bytes: int):
+def alone_us(longest: int, streams: int, ranges, sms: int) -> float:
+    """About what a step takes whose rows are read by themselves, the longest of `longest` positions."""
+    cut = ranges(streams, longest)
+    return ALONE_US + _up(-(-longest // cut), 256) * ALONE_POSITION_US * -(-streams * cut // sms)
+
+
+def worth_sharing(shared, group_heads: int, nkv: int, sms: int, room: int, most: int, own_ranges, alone_ranges, row_bytes: int):
     """The groups of `shared` whose sharing is expected to pay, those that save most first: few rows of few positions are read from the L2 again sooner than they
-    are split off and joined.  `row_bytes`: of a key and a value of one kv head."""
+    are split off and joined.  own_ranges, alone_ranges(streams, positions): how a stream is cut with sharing and without; `row_bytes`: of a key and a value of
+    one kv head."""
     order = sorted(shared.groups, key=lambda g: -(len(g[0]) - 1) * g[1])
-    best, kept = None, 0
-    for k in sorted({0, 1, 2, len(order) // 2, len(order)} & set(range(len(order) + 1))):
-        lengths = [OWN_GUESS] * shared.n_rows
-        for g, p in order[k:]:
-            for r in g:
-                lengths[r] += p
-        us = own_us(lengths, nkv, ranges, sms, row_bytes)
-        us += BEHIND_US + cut_ranges([(len(g) * group_heads, p) for g, p in order[:k]], nkv, sms, room, most)[2] if k else ALONE_US
-        if best is None or us < best:
+    streams = shared.n_rows * nkv
+    best, kept = alone_us(max((p for _, p in order), default=0) + OWN_GUESS, streams, alone_ranges, sms), 0
+    for k in sorted({1, 2, len(order) // 2, len(order)} & set(range(1, len(order) + 1))):
+        left = order[k:]                       # groups that are left alone are walked by their rows
+        us = own_us(OWN_GUESS + max((p for _, p in left), default=0), OWN_GUESS * shared.n_rows + sum(len(g) * p for g, p in left), shared.n_rows, nkv, own_ranges,
+                    row_bytes)
+        us += cut_ranges([(len(g) * group_heads, p) for g, p in order[:k]], nkv, sms, room, most, streams)[2]
+        if us < best:
             best, kept = us, k
     return order[:kept]
 
@@ -116,7 +128,7 @@ def shared_items(shared, group_heads: int, nkv: int, sms: int, room: int, most: 
     rows, first, parts = np.zeros(n, dtype=np.int32), np.zeros(n, dtype=np.int32), np.zeros(n, dtype=np.int32)
     items, at = [], 0
     if shared.groups:
-        block, length, _ = cut_ranges([(len(g) * group_heads, p) for g, p in shared.groups], nkv, sms, room, most)
+        block, length, _ = cut_ranges([(len(g) * group_heads, p) for g, p in shared.groups], nkv, sms, room, most, n * nkv)
         for group, positions in shared.groups:
             rows[at:at + len(group)] = group
             first[list(group)] = positions

@@ -328,8 +328,8 @@ def test_every_position_of_a_row_is_taken_once(seed):
 
 def test_groups_that_pay_are_kept():
     """Few rows of few positions are left alone; many rows of many positions are not."""
-    ranges = lambda streams, positions: ops.own_ranges(streams, positions, 148)
-    args = (6, 2, 148, 444, 64, ranges, 512)
+    own, alone = (lambda streams, positions: ops.own_ranges(streams, positions, 148)), (lambda streams, positions: ops.decode_splits(streams, positions, 148))
+    args = (6, 2, 148, 444, 64, own, alone, 512)
     keep = lambda n, groups: shared_plan.worth_sharing(SharedPrefix(n, groups), *args)
     assert keep(2, [([0, 1], 512)]) == []
     assert keep(64, [(range(64), 8192)]) == [(tuple(range(64)), 8192)]
