@@ -82,7 +82,7 @@ struct AttnTcSharedParams : AttnTcParams {
     int slots;
 };
 template <bool V> struct AtSplit { static constexpr bool value = V; };
-// SHARED: of the pairs of exponentials every eighth is the float units' (256 rows of 28 heads over 32,768 positions, 280 CTAs: 113.5 us; none of them
+// SHARED: of the pairs of exponentials every eighth is the float units' (256 rows of 28 heads over 32,768 positions, 140 CTAs: 113.5 us; none of them
 // 120.6, every fourth 125.7: the special function units and the instructions' issue are both near their limits).
 constexpr int AT_FLOAT_EVERY = 7;
 template <bool DIFF, bool SHARED> struct AtParams { using type = AttnTcParams; };
@@ -204,11 +204,14 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
         failed = 0;
         mbar_init_fence();
     }
-    if (warp == 0) {
+    auto allocate = [&]() {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&tmem_sh)), "r"(TMEM_COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+    };
+    if constexpr (!SHARED) {
+        if (warp == 0) allocate();
+        pdl_wait();
     }
-    if constexpr (!SHARED) pdl_wait();
     int req, row0, nq;
     if constexpr (SHARED) { req = p.items[qb * 8 + 0]; row0 = p.items[qb * 8 + 1]; nq = p.items[qb * 8 + 2]; }
     else { req = p.qblk[qb * 3 + 0]; row0 = p.qblk[qb * 3 + 1]; nq = p.qblk[qb * 3 + 2]; }
@@ -248,15 +251,21 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
         fence_proxy_async();
     };
     if constexpr (SHARED) {
-        // what the lists say is there before the kernel ahead is done; behind it, the keys are asked for while the others fetch the queries
+        // What the lists say is there before the kernel ahead is done; behind it, the keys are asked for while the others fetch the queries.  Tensor memory is
+        // taken behind it too: the kernel ahead is a product that lets its successor start before it has taken its own columns, and a CTA of this
+        // kernel that came to the same SM first (with heads of 64 there is room beside the product's CTA) would hold all of them and wait for the product.
         if (tid < 2 * AT_BM) row_of[tid] = tid < n_rows ? batch_row(tid) : 0;
-        tc_fence_before();
         __syncthreads();
-        tc_fence_after();
         pdl_wait();
+        if (warp == 0) {
+            allocate();
+            pdl_launch();                                // (as below: only now that the columns are held)
+            tc_fence_before();
+        }
         if (warp != 5 && warp != 7 && warp != 12 && warp != 14) {
             load_queries((warp - (warp > 5) - (warp > 7) - (warp > 12) - (warp > 14)) * 32 + lane, AT_SHARED_THREADS - 128);
             asm volatile("bar.sync 2, %0;\n" ::"n"(AT_SHARED_THREADS - 128) : "memory");
+            tc_fence_after();
         }
     } else {
         load_queries(tid, AT_THREADS);
@@ -268,7 +277,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
     // The kernel behind this one may be scheduled only now that this CTA holds its tensor memory: it takes all 512
     // columns, and a CTA of the successor that came to the same SM first and allocated a few would then wait for
     // this kernel to end while this CTA waits for its columns.
-    pdl_launch();
+    if constexpr (!SHARED) pdl_launch();
 
     // (SHARED: an issuer on each of the four sub-partitions, with a loader and a softmax warp of either group)
     if (warp == 0 || warp == 6 || (SHARED && (warp == 13 || warp == 15))) {
