@@ -263,7 +263,10 @@ attention_mma_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_co
         // box o of the stage is lane o's, so that one instruction of the warp asks for up to 32 boxes (what
         // costs is the instruction, not the box).  Pages that lie wholly outside the range of keys are left
         // out; rows outside it are zeroed by the computing warps once the stage has landed.
-        if (!p.use_tma) return;
+        if (!p.use_tma) {
+            if constexpr (SHARED) pdl_wait();
+            return;
+        }
         constexpr int PER_PAGE = 2 * (HD / 64);
         const int ps = p.page_size, shift = p.page_shift;
         const int n_box = (AM_STAGE_KEYS >> shift) * PER_PAGE;
@@ -288,6 +291,7 @@ attention_mma_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_co
             next_page = page_of(s + 1, p.whole_pages ? lane * PER_PAGE : lane);   // fetched while this stage's copies go out
             if (s >= AM_STAGES && !mbar_wait<4000>(&empty_bar[buf], ((s / AM_STAGES) - 1) & 1, &gave_up)) {
                 if (p.status) atomicOr(p.status, BG_STATUS_TIMEOUT);
+                if constexpr (SHARED) pdl_wait();
                 return;
             }
             unsigned char* kd = k_s + buf * BUF_BYTES;
@@ -319,6 +323,7 @@ attention_mma_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_co
             __syncwarp();
             if (lane == 0) mbar_arrive(&full_bar[buf]);   // the one arrival the phase waits for, after every expect_tx
         }
+        if constexpr (SHARED) pdl_wait();                 // (no warp leaves before the wait that the others make at their end)
         return;
     }
     const size_t page_elems = (size_t)2 * p.nkv * p.page_size * HD;
