@@ -133,7 +133,7 @@ class DecodeGraph:
         self._groups: Optional[SharedPrefix] = None    # what the requests share, for the variants that read it
         self._shares = False
         self.rules: Optional[RuleTables] = None
-        self._rules_of = None                  # (rids, positions) whose texts and rules the tables hold
+        self._rules_of = self._rules_next = None       # (rids, positions, rules) that the tables hold, and will once the step has run
         self.h2d_bytes = 0                     # bytes uploaded by the last step
         self._rids: Optional[tuple] = None     # what the device buffers describe
         self._positions: Optional[List[int]] = None
@@ -243,17 +243,28 @@ class DecodeGraph:
         return all(cache.length(r) == p for r, p in zip(rids, self._ahead[1]))
 
     def _load_rules(self, key, positions, rows) -> Tuple[str, int]:
-        """Bring the tables of the rows' rules up to date: (variant, bytes sent)."""
-        if rows is None or all(r is None or r.plain for r, _, _ in rows):
+        """Bring the tables of the rows' rules up to date: (variant, bytes sent).  `step` notes what they hold once it has run: a step adds its input token to
+        every text, and one without rules does not."""
+        known, self._rules_of, self._rules_next = self._rules_of, None, None
+        if rows is None:
             return "", 0
+        if len(rows) != len(key):
+            raise ValueError(f"rules for {len(rows)} of {len(key)} requests")
+        if all(r is None or r.plain for r, _, _ in rows):
+            return "", 0
+        asked = [(rules, len(prompt)) for rules, prompt, _ in rows]
+        fresh = known != (key, positions, asked)
+        for (rules, prompt, made), p in zip(rows, positions):
+            have = len(prompt) + len(made)
+            if fresh and have not in (p, p + 1) or rules is not None and rules.allowed is not None and have != p + 1:
+                raise ValueError(f"rules with a text of {have} tokens for a request at position {p}")
         sent = 0
         if self.rules is None:
             self.rules = RuleTables(self.n, self.engine.vocab, self.engine.cache.max_context, self.engine.device)
-        if self._rules_of != (key, positions):
+        if fresh:
             sent += self.rules.load(rows)
-        # (the step adds its input token to every text)
-        self._rules_of = (key, [p + 1 for p in positions])
         sent += self.rules.load_masks(rows)
+        self._rules_next = (key, [p + 1 for p in positions], asked)
         return ("masks" if self.rules.masked else "rules"), sent
 
     def step(self, rids: Sequence[Hashable], tokens: Optional[Sequence[int]], temperatures: Optional[Sequence[float]] = None,
@@ -263,7 +274,7 @@ class DecodeGraph:
         Returns the sampled tokens as a list (read_back) or the device tensor.  Only what changed since
         the last step is uploaded: positions advance on the device, block tables change when a request
         gets a new page.  `rules`: (LogitRules or None, prompt, generated tokens) of every request; the tokens are those that the host
-        knows, the step's input last."""
+        knows, the step's input last (a mask needs them all; without one the device keeps count where the host lags behind)."""
         cache, n, b = self.engine.cache, self.n, self.batch
         m = len(rids)
         assert 1 <= m <= n
@@ -321,6 +332,7 @@ class DecodeGraph:
         graph, launches, self.logits = self.graphs[which]
         graph.replay()
         ops.count_launches(launches)
+        self._rules_of = self._rules_next
         if self._shares and which[1]:          # (the first such step has made the plans)
             self._shares = any(plan.shares for plan in self.batch.plans.values())
         cache.commit([(r, p + 1) for r, p in zip(rids, positions)])

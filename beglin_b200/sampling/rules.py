@@ -29,6 +29,9 @@ class LogitRules:
     bias: Mapping[int, float] = field(default_factory=dict)
     allowed: Optional[Callable[[Sequence[int]], Optional[Sequence[int]]]] = None
 
+    def __post_init__(self):
+        object.__setattr__(self, "bias", dict(self.bias))      # (the caller's own may change)
+
     def check(self, vocab: int) -> None:
         if not (self.repetition > 0.0 and math.isfinite(self.repetition)):
             raise ValueError(f"repetition={self.repetition} must be positive and finite (1: none)")
@@ -114,6 +117,7 @@ class RuleTables:
             prompts[r] = len(prompt)
             history[r, :len(text)] = text
             if rules is not None:
+                rules.check(self.vocab)
                 pen[:, r] = rules.repetition, rules.frequency, rules.presence
                 for token in sorted(rules.bias):
                     ids.append(int(token)); values.append(float(rules.bias[token]))

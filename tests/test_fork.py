@@ -218,6 +218,47 @@ def test_rules_are_checked():
             mask(bad)
 
 
+def test_tables_of_a_replayed_step_follow_the_rules():
+    """What a replayed step's tables hold is loaded again when the rules change, when a step in between ran without them and when one was given up."""
+    from types import SimpleNamespace
+    from beglin_b200.engine.decode_graph import DecodeGraph
+    from beglin_b200.sampling import LogitRules
+    from beglin_b200.sampling.rules import RuleTables
+    g = DecodeGraph.__new__(DecodeGraph)
+    g.n, g._rules_of, g._rules_next, g.rules = 2, None, None, RuleTables(2, 50, 16, "cpu")
+    g.engine, loads = SimpleNamespace(vocab=50), []
+    load = g.rules.load
+    g.rules.load = lambda rows: loads.append(1) or load(rows)
+
+    def step(rules, made, at, runs=True):
+        variant = g._load_rules(("a",), [at], None if rules is None else [(rules, [1, 2], made)])[0]
+        if runs:
+            g._rules_of = g._rules_next
+        return variant, len(loads)
+
+    first, second = LogitRules(bias={3: 1.0}), LogitRules(bias={3: -1.0})
+    assert step(first, [4], 2) == ("rules", 1)
+    assert step(first, [4, 5], 3) == ("rules", 1)                      # nothing new
+    assert step(LogitRules(bias={3: 1.0}), [4, 5, 6], 4) == ("rules", 1)
+    assert step(second, [4, 5, 6, 7], 5) == ("rules", 2) and float(g.rules.bias_values[0]) == -1.0
+    assert step(None, [], 6) == ("", 2) and step(second, [4, 5, 6, 7, 8, 9], 7) == ("rules", 3)
+    assert step(second, [4, 5, 6, 7, 8, 9, 9], 8, runs=False) == ("rules", 3) and step(second, [4, 5, 6, 7, 8, 9, 9], 8) == ("rules", 4)
+    assert step(second, [4], 9) == ("rules", 4)                        # the device keeps count
+    never = LogitRules(allowed=lambda made: [])
+    with pytest.raises(ValueError, match="no token"):
+        step(never, [4, 5, 6, 7, 8, 9, 9, 9, 9], 10)
+    assert g._rules_of is None
+    for rules, made, at in ((first, [4], 10), (LogitRules(allowed=lambda made: [1]), [4], 3), (LogitRules(bias={50: 1.0}), [4], 2)):
+        with pytest.raises(ValueError, match="position|outside"):
+            step(rules, made, at)
+    with pytest.raises(ValueError, match="rules for"):
+        g._load_rules(("a", "b"), [2, 2], [(first, [1, 2], [4])])
+    given = {3: 1.0}
+    kept = LogitRules(bias=given)
+    given[3] = 2.0
+    assert kept.bias == {3: 1.0}
+
+
 # ------------------------------------------------------------------------------------------------ the engine
 DESIGNS = {"qwen2": ("helpers", "D"), "qwen2 window": ("helpers", "C"), "sukisun": ("sukisun_helpers", None), "nadilorn": ("nadilorn_helpers", None),
            "sofudra": ("sofudra_helpers", None), "tuzupel": ("tuzupel_helpers", None), "dinatar": ("dinatar_helpers", None), "fanitar": ("fanitar_helpers", None)}
