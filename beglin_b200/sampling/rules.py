@@ -21,8 +21,8 @@ MOST_BIASES = 512          # biased tokens of a request
 
 @dataclass(frozen=True)
 class LogitRules:
-    """`allowed` is called before every token with the tokens that the request has generated so far and returns which may come next: token ids, or truth
-    values [vocab] (a bool array), or None for all."""
+    """`allowed` is called before every token with the tokens that the request has generated so far and returns which may come next: token ids, truth
+    values [vocab] (a bool array), those packed as bits already (a uint32 array: bit v % 32 of word v / 32 is token v's), or None for all."""
     repetition: float = 1.0
     frequency: float = 0.0
     presence: float = 0.0
@@ -58,6 +58,13 @@ class LogitRules:
         if given is None:
             return None
         given = np.asarray(given)
+        if given.dtype == np.uint32:
+            if given.shape != (-(-vocab // 32),):
+                raise ValueError(f"allowed: packed bits of {given.shape}, expected ({-(-vocab // 32)},)")
+            words = np.ascontiguousarray(given)
+            if not (words[:-1].any() or int(words[-1]) & ((1 << (vocab - 1) % 32 + 1) - 1)):
+                raise ValueError("allowed: no token may come next")
+            return words.view(np.int32)
         if given.dtype == np.bool_:
             if given.shape != (vocab,):
                 raise ValueError(f"allowed: truth values of {given.shape}, expected ({vocab},)")

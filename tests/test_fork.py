@@ -213,7 +213,11 @@ def test_rules_are_checked():
     truth = np.zeros(70, dtype=bool)
     truth[[0, 31, 32, 69]] = True
     assert mask(truth).tolist() == words.tolist()
-    for bad, match in (([70], "outside"), ([-1], "outside"), ([], "no token"), (np.zeros(70, dtype=bool), "no token"), (np.ones(5, dtype=bool), "truth values")):
+    packed = words.view(np.uint32).copy()
+    assert mask(packed).tolist() == words.tolist() and mask(np.stack([packed, packed], axis=1)[:, 0]).tolist() == words.tolist()
+    assert mask(np.asarray([5], dtype=np.uint32), vocab=3).tolist() == [5] and mask(np.asarray([1 << 31], dtype=np.uint32), vocab=32) is not None
+    for bad, match in (([70], "outside"), ([-1], "outside"), ([], "no token"), (np.zeros(70, dtype=bool), "no token"), (np.ones(5, dtype=bool), "truth values"),
+                       (np.zeros(3, dtype=np.uint32), "no token"), (np.asarray([0, 0, 1 << 6], dtype=np.uint32), "no token"), (np.ones(2, dtype=np.uint32), "packed bits")):
         with pytest.raises(ValueError, match=match):
             mask(bad)
 
