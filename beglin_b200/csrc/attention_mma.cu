@@ -26,10 +26,11 @@
 //          the MMAs of a stage (the heads fill 6 of 8 columns instead of 6 of 16 rows); P^T reaches its
 //          operand layout through movmatrix.
 //
-// SHARED instances take what lies behind positions that requests share.  Where that is more CTAs than SMs (many rows with a few hundred keys each, so that a
-// CTA's beginning and end count), QUARTER instances: every warp takes a quarter of every stage, three buffers are enough and two CTAs fit an SM.  1,024 streams
-// of 100 to 800 keys of 128 features: 66 us with a stage a warp, 52 with quarters (floor 37); 140 of up to 900 in pages of 16: 15.9 and 11.9; 16 of 300: 5.0
-// and 6.5, where the chain of a stage's steps is what counts.
+// SHARED instances take what lies behind positions that requests share.  Where that is more CTAs of 128 features than SMs (many rows with a few
+// hundred keys each, so that a CTA's beginning and end count), QUARTER instances: every warp takes a quarter of every stage, three buffers are enough and
+// two CTAs fit an SM in place of one (with 64 features three fit as it is: 856 streams of 450 to 1,500 keys take 31 us, 39 with quarters).  1,024 streams of 100 to 800 keys of 128 features: 66 us with a stage a warp, 52
+// with quarters (floor 37); 140 of up to 900 in pages of 16, cut in ranges: 15.9 and 11.9; 16 of 300: 5.0 and 6.5, where the chain of a stage's steps is what
+// counts.  Where nothing is shared and a row is one range, the finished rows are written: 11 rows of 180 to 230 keys take 5.3 us, 7.1 with the joining.
 //
 // EXT instances: a score falls by slopes[head] per position that its key lies back, and a window never loses the sequence's
 // first `keep` positions.  The stages of a CTA are then those of its kept keys followed by those of its window's, the
@@ -81,6 +82,8 @@ struct AttnMmaExtParams : AttnMmaParams {
 struct AttnMmaSharedParams : AttnMmaParams {
     const int* own_first;   // [T]
     int ahead_done;         // the kernel ahead is the shared positions': the queries are there when this one begins
+    int sink;               // `out`: the denominator is enlarged, by a score head by head (null: 0)
+    const float* sink_w;
 };
 template <bool EXT, bool SHARED> struct AmParams { using type = AttnMmaParams; };
 template <> struct AmParams<true, false> { using type = AttnMmaExtParams; };
@@ -91,6 +94,11 @@ __device__ __forceinline__ int am_own_first(const AttnMmaSharedParams& p, int ro
 // another's to wait for: this kernel waits for it at the end).
 __device__ __forceinline__ void am_wait(const AttnMmaParams&) { pdl_wait(); }
 __device__ __forceinline__ void am_wait(const AttnMmaSharedParams& p) { if (!p.ahead_done) pdl_wait(); }
+// The sink's share of a denominator whose weights are 2^(score - m) (infinite where the sink is far above all keys, and the row then nought).
+__device__ __forceinline__ float am_sink(const AttnMmaParams&, int, float) { return 0.0f; }
+__device__ __forceinline__ float am_sink(const AttnMmaSharedParams& p, int head, float m) {
+    return p.sink ? exp2f((p.sink_w ? p.sink_w[head] : 0.0f) * AM_LOG2E - m) : 0.0f;
+}
 __device__ __forceinline__ int am_keep(const AttnMmaParams&) { return 0; }
 __device__ __forceinline__ int am_keep(const AttnMmaExtParams& p) { return p.keep; }
 __device__ __forceinline__ const float* am_slopes(const AttnMmaParams&) { return nullptr; }
@@ -234,7 +242,11 @@ attention_mma_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_co
     const int kept_end = min(keep, k_end);                        // and the kept ones [k_first, kept_end), possibly none
     const bool has_kept = EXT && k_first < kept_end;
     if (k_begin >= k_end && !has_kept) {
-        if (SHARED) pdl_wait();                // (no row may have positions of its own: what comes behind still waits for the shared ones' kernel)
+        if constexpr (SHARED) {
+            pdl_wait();                        // (no row may have positions of its own: what comes behind still waits for the shared ones' kernel)
+            if (p.out)                         // a row that sees nothing is nought
+                for (int i = tid; i < group * HD; i += AM_ALL) p.out[(size_t)row0 * p.out_stride + (size_t)kvh * group * HD + i] = __float2bfloat16_rn(0.0f);
+        }
         return;
     }
     auto in_range = [&](int key) { return key < k_end && (key >= k_begin || (EXT && key >= k_first && key < kept_end)); };
@@ -766,7 +778,10 @@ attention_mma_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_co
                         acc = fmaf(o_sh[((size_t)w * 16 + r) * HP + d], f, acc);
                         l = fmaf(ml_sh[(w * 16 + r) * 2 + 1], f, l);
                     }
-                    if (p.out) {                               // the only range of its request: the finished row
+                    if (SHARED && p.out) {                     // (likewise, with a sink; what all its keys' weights leave out is nought, as the joining makes it)
+                        l += am_sink(p, kvh * group + r, m);
+                        p.out[(size_t)row0 * p.out_stride + (size_t)(kvh * group + r) * HD + d] = __float2bfloat16_rn(l == 0.0f ? 0.0f : acc / l);
+                    } else if (p.out) {                        // the only range of its request: the finished row
                         p.out[(size_t)row0 * p.out_stride + (size_t)(kvh * group + r) * HD + d] = __float2bfloat16_rn(acc / l);
                     } else {
                         const size_t prow = ((size_t)row0 * p.nh + (size_t)kvh * group + r) * p.max_splits + sp;
@@ -810,7 +825,9 @@ static int am_launch_own_as(const CUtensorMap& map, const CUtensorMap& map5, con
 }
 template <int HD, bool SWAP>
 static int am_launch_own(const CUtensorMap& map, const CUtensorMap& map5, const AttnMmaSharedParams& p, int T, int n_splits, cudaStream_t stream) {
-    if ((long long)T * p.nkv * n_splits > sm_count()) return am_launch_own_as<HD, SWAP, true>(map, map5, p, T, n_splits, stream);
+    if constexpr (HD == 128) {
+        if ((long long)T * p.nkv * n_splits > sm_count()) return am_launch_own_as<HD, SWAP, true>(map, map5, p, T, n_splits, stream);
+    }
     return am_launch_own_as<HD, SWAP, false>(map, map5, p, T, n_splits, stream);
 }
 
@@ -884,11 +901,14 @@ extern "C" int bg_attention_mma_partial(const void* q, int q_stride, const void*
 
 // The partial results of T single tokens (row r of request r) over the positions from own_first[r] to their own, spread over n_splits ranges a row
 // (those of keys_per_split over the row's own positions): at slot first_slot + range of part_o [T][nh][slots][hd] and part_ml [T][nh][slots][2].  A row
-// without positions of its own writes nothing.  ahead_done: the launch ahead on the stream is bg_attention_tc_shared's.
+// without positions of its own writes nothing.  ahead_done: the launch ahead on the stream is bg_attention_tc_shared's.  With `out` (nothing is shared, one
+// range) the finished rows instead.
 extern "C" int bg_attention_mma_own(const void* q, int q_stride, const void* kv_pool, int num_pages, int page_size, const int* block_table, int max_pages,
                                     const int* positions, const int* own_first, int T, float* part_o, float* part_ml, int slots, int first_slot, int n_splits,
-                                    int nh, int nkv, int hd, float scale, float softcap, int ahead_done, unsigned* status, cudaStream_t stream) {
+                                    int nh, int nkv, int hd, float scale, float softcap, int ahead_done, void* out, int out_stride, int sink,
+                                    const float* sink_w, unsigned* status, cudaStream_t stream) {
     if (T <= 0 || n_splits <= 0) return BG_OK;
+    if (out && (n_splits != 1 || ahead_done)) return BG_ERR_SHAPE;
     if (nkv <= 0 || nh % nkv != 0 || page_size <= 0 || first_slot < 0 || first_slot + n_splits > slots || n_splits > 65535 || nkv > 65535) return BG_ERR_SHAPE;
     if ((q_stride % 8) != 0 || ((uintptr_t)q % 16) != 0 || ((uintptr_t)kv_pool % 16) != 0) return BG_ERR_ALIGN;
     if ((hd != 64 && hd != 128) || nh / nkv > 16) return BG_ERR_UNSUPPORTED;
@@ -901,7 +921,7 @@ extern "C" int bg_attention_mma_own(const void* q, int q_stride, const void* kv_
     p.positions = positions; p.max_splits = slots; p.nh = nh; p.nkv = nkv; p.group = nh / nkv; p.scale_log2 = scale * AM_LOG2E; p.status = status;
     p.part_o = part_o + (size_t)first_slot * hd; p.part_ml = part_ml + (size_t)first_slot * 2;
     p.cap_log2 = softcap > 0.0f ? softcap * AM_LOG2E : 0.0f; p.scale_over_cap = softcap > 0.0f ? scale / softcap : 0.0f;
-    p.own_first = own_first; p.ahead_done = ahead_done;
+    p.own_first = own_first; p.ahead_done = ahead_done; p.out = (__nv_bfloat16*)out; p.out_stride = out_stride; p.sink = sink; p.sink_w = sink_w;
     CUtensorMap map, map5;
     memset(&map, 0, sizeof(map));
     memset(&map5, 0, sizeof(map5));

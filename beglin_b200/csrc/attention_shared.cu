@@ -130,13 +130,13 @@ static int shared_merge(const float* part_o, const float* part_ml, const int* po
 extern "C" int bg_shared_attention_bytes(int step) { return (int)(step ? sizeof(SharedAttnStep) : sizeof(SharedAttnArgs)); }
 
 // The whole attention of a step of single tokens over shared and own positions, as one call.  scratch: T * nh * n * (vd + 2) floats, n the float units' `ranges`
-// or the tensor cores' slots + ranges.
+// or the tensor cores' slots + ranges (none where nothing is shared and there is one range).
 extern "C" int bg_shared_attention(const SharedAttnArgs* args, const SharedAttnStep* step, cudaStream_t stream) {
     const SharedAttnArgs& a = *args;
     const SharedAttnStep& s = *step;
     if (a.T <= 0) return BG_OK;
     if (a.nh <= 0 || a.nkv <= 0 || a.nh % a.nkv || a.hd <= 0 || a.vd <= 0 || s.ranges <= 0 || a.slots < 0 || (uintptr_t)s.scratch % 16) return BG_ERR_SHAPE;
-    const long long results = (long long)a.T * a.nh * (a.tensor_cores ? a.slots + s.ranges : s.ranges);
+    const long long results = a.tensor_cores && !a.n_items && s.ranges == 1 ? 0 : (long long)a.T * a.nh * (a.tensor_cores ? a.slots + s.ranges : s.ranges);
     if (s.scratch_floats < results * (a.vd + 2)) return BG_ERR_SHAPE;
     float *part_o = s.scratch, *part_ml = s.scratch + results * a.vd;
     if (!a.tensor_cores) {
@@ -147,12 +147,15 @@ extern "C" int bg_shared_attention(const SharedAttnArgs* args, const SharedAttnS
         return bg_attention_merge(part_o, part_ml, s.positions, s.out, s.out_dtype, s.out_stride, a.T, a.nh, a.vd, s.ranges, a.split, 0, s.sink, s.sink_w, 0, stream);
     }
     if (a.q_dtype != BG_DTYPE_BF16 || a.cache_dtype != BG_DTYPE_BF16 || s.out_dtype != BG_DTYPE_BF16) return BG_ERR_DTYPE;
+    if (!a.n_items && s.ranges == 1)                 // nothing is shared, and a CTA walks all of a row's positions: one kernel, which writes the rows
+        return bg_attention_mma_own(s.q, s.q_stride, s.pool, s.num_pages, a.page_size, s.table, s.max_pages, s.positions, a.own_first, a.T, nullptr, nullptr, 1, 0, 1,
+                                    a.nh, a.nkv, a.hd, s.scale, s.softcap, 0, s.out, s.out_stride, s.sink, s.sink_w, s.status, stream);
     const int slots = a.slots + s.ranges;
     int rc = bg_attention_tc_shared(s.q, s.q_stride, s.pool, s.num_pages, a.page_size, s.table, s.max_pages, s.positions, a.items, a.n_items, a.rows, part_o,
                                     part_ml, slots, a.nh, a.nkv, a.hd, s.scale, s.softcap, s.status, stream);
     if (rc == BG_OK)
         rc = bg_attention_mma_own(s.q, s.q_stride, s.pool, s.num_pages, a.page_size, s.table, s.max_pages, s.positions, a.own_first, a.T, part_o, part_ml, slots,
-                                  a.slots, s.ranges, a.nh, a.nkv, a.hd, s.scale, s.softcap, a.n_items > 0, s.status, stream);
+                                  a.slots, s.ranges, a.nh, a.nkv, a.hd, s.scale, s.softcap, a.n_items > 0, nullptr, 0, 0, nullptr, s.status, stream);
     if (rc == BG_OK)
         rc = shared_merge(part_o, part_ml, s.positions, a.own_first, a.parts, a.T, a.nh, a.hd, slots, a.slots, s.ranges, s.sink, s.sink_w, s.out, s.out_stride,
                           stream);

@@ -16,7 +16,7 @@ int bg_attention_shared_partial(const void* q, int q_dtype, int q_stride, const 
 // attention_mma.cu
 int bg_attention_mma_own(const void* q, int q_stride, const void* kv_pool, int num_pages, int page_size, const int* block_table, int max_pages, const int*
     positions, const int* own_first, int T, float* part_o, float* part_ml, int slots, int first_slot, int n_splits, int nh, int nkv, int hd, float scale,
-    float softcap, int ahead_done, unsigned* status, cudaStream_t stream);
+    float softcap, int ahead_done, void* out, int out_stride, int sink, const float* sink_w, unsigned* status, cudaStream_t stream);
 // attention_tcgen05.cu
 int bg_attention_tc_shared(const void* q, int q_stride, const void* kv_pool, int num_pages, int page_size, const int* block_table, int max_pages, const int*
     positions, const int* items, int n_items, const int* rows, float* part_o, float* part_ml, int slots, int nh, int nkv, int hd, float scale, float softcap,

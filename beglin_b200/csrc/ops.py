@@ -900,7 +900,7 @@ class SharedPlan:
             if not self.all_groups:
                 kept = _shared.worth_sharing(shared, self.nh // self.nkv, self.nkv, self.sms, self.room, self.MOST_RANGES,
                                              lambda streams, positions: own_ranges(streams, positions, self.sms),
-                                             lambda streams, positions: decode_splits(streams, positions, self.sms), 4 * self.hd)
+                                             lambda streams, positions: decode_splits(streams, positions, self.sms), 4 * self.hd, self.page_size)
                 shared = type(shared)(self.n_rows, kept)
             arrays = _shared.shared_items(shared, self.nh // self.nkv, self.nkv, self.sms, self.room, self.MOST_RANGES)
         else:
@@ -1006,9 +1006,12 @@ def shared_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_table: torch.
         if status is None or out.dtype != torch.bfloat16:
             raise KernelError("shared_attention: the tensor-core kernels want a status word and write bfloat16")
         own = max(1, max_position + 1 - plan.least_own)
-        at_once, kernels = 0, 3 if plan.n_items else 2
+        at_once = 0
         ranges = own_ranges(T * plan.nkv, own, plan.sms) if plan.n_items else decode_splits(T * plan.nkv, own, plan.sms)
-        floats = plan.row_floats * (plan.slots + ranges)
+        if not plan.n_items and ranges == 1:   # nothing is shared and a CTA walks all of a row's positions: it writes the row
+            kernels, floats = 1, 0
+        else:
+            kernels, floats = 3 if plan.n_items else 2, plan.row_floats * (plan.slots + ranges)
     else:
         ranges, kernels = max_position // plan.split + 1, 2
         at_once = min(ranges, max(plan.slots, ranges - plan.least_own, 1))

@@ -45,8 +45,10 @@ CTA_US, TILE_US, PAIR_US, RANGE_US = 6.0, 0.52, 1.03, 0.05
 # where the shared positions' kernel leaves them no SMs to begin on.
 BEHIND_US, OWN_POSITION_US, OWN_RATE, CROWDED_US = 0.4, 0.0135, 4.5e6, 3.6
 OWN_GUESS = 256            # positions that a request is taken to hold behind those that it shares
-# Every row by itself over all of its positions: beside a CTA's positions, and a position (pages that several rows hold come from the L2).
-ALONE_US, ALONE_POSITION_US = 6.0, 0.0058
+# Every row by itself over all of its positions: beside the CTAs, beside a CTA's positions, a position (pages that several rows hold come from the L2) and
+# what more it is for every page of 64 positions where pages are smaller; CTAs that come to an SM behind others begin under those.  (Against 220 steps of 2 to
+# 256 rows the choices that follow from these numbers take 0.6 % longer than the better of both ways would.)
+ALONE_US, ALONE_CTA_US, ALONE_POSITION_US, ALONE_PAGE_US, ALONE_BEHIND = 1.5, 4.5, 0.0058, 0.001, 0.7
 
 
 def _up(n: int, unit: int) -> int:
@@ -98,19 +100,26 @@ def own_us(longest: int, total: int, n_rows: int, nkv: int, ranges, row_bytes: i
     return BEHIND_US + max(total * nkv * row_bytes / OWN_RATE, one)
 
 
-def alone_us(longest: int, streams: int, ranges, sms: int) -> float:
-    """About what a step takes whose rows are read by themselves, the longest of `longest` positions."""
+def alone_us(longest: int, total: int, n_rows: int, nkv: int, ranges, sms: int, row_bytes: int, page_size: int) -> float:
+    """About what a step takes whose rows are read by themselves, the longest of `longest` positions, `total` in all."""
+    streams, at_once = n_rows * nkv, sms * (1 if row_bytes > 256 else 3)
     cut = ranges(streams, longest)
-    return ALONE_US + _up(-(-longest // cut), 256) * ALONE_POSITION_US * -(-streams * cut // sms)
+    ctas, each = streams * cut, ALONE_POSITION_US + (ALONE_PAGE_US * 64 / page_size if page_size < 64 else 0.0)
+    one = ALONE_CTA_US + _up(-(-longest // cut), 256) * each
+    if ctas <= at_once:
+        return ALONE_US + one
+    return ALONE_US + max(one, ALONE_BEHIND * ctas / at_once * (ALONE_CTA_US + total * nkv / ctas * each) + one / 2)
 
 
-def worth_sharing(shared, group_heads: int, nkv: int, sms: int, room: int, most: int, own_ranges, alone_ranges, row_bytes: int):
+def worth_sharing(shared, group_heads: int, nkv: int, sms: int, room: int, most: int, own_ranges, alone_ranges, row_bytes: int,
+                  page_size: int = 64):
     """The groups of `shared` whose sharing is expected to pay, those that save most first: few rows of few positions are read from the L2 again sooner than they
     are split off and joined.  own_ranges, alone_ranges(streams, positions): how a stream is cut with sharing and without; `row_bytes`: of a key and a value of
     one kv head."""
     order = sorted(shared.groups, key=lambda g: -(len(g[0]) - 1) * g[1])
     streams = shared.n_rows * nkv
-    best, kept = alone_us(max((p for _, p in order), default=0) + OWN_GUESS, streams, alone_ranges, sms), 0
+    best, kept = alone_us(max((p for _, p in order), default=0) + OWN_GUESS, sum(len(g) * p for g, p in order) + OWN_GUESS * shared.n_rows, shared.n_rows, nkv,
+                          alone_ranges, sms, row_bytes, page_size), 0
     for k in sorted({1, 2, len(order) // 2, len(order)} & set(range(1, len(order) + 1))):
         left = order[k:]                       # groups that are left alone are walked by their rows
         us = own_us(OWN_GUESS + max((p for _, p in left), default=0), OWN_GUESS * shared.n_rows + sum(len(g) * p for g, p in left), shared.n_rows, nkv, own_ranges,

@@ -245,6 +245,37 @@ def test_shared_attention_of_groups_that_pay(kept, monkeypatch):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("cap", [0.0, 4.0])
+@pytest.mark.parametrize("sink", [None, 0.0, 30.0])
+@pytest.mark.parametrize("lengths", [[1], [0, 65, 64, 1, 130], [(37 * i) % 190 + (i != 5) for i in range(90)]], ids=["one", "few", "many"])
+@pytest.mark.parametrize("nh,nkv,hd,page", [(12, 2, 128, 64), (32, 2, 128, 16), (14, 2, 64, 64), (9, 3, 64, 8)])
+def test_rows_that_share_nothing_are_finished_by_one_kernel(nh, nkv, hd, page, lengths, sink, cap):
+    """Rows that share nothing and are short, a row that sees nothing among them; few rows the same with the joining (a bound on the positions that cuts them into
+    ranges)."""
+    c = Case([], lengths, nh, nkv, hd, page, torch.bfloat16, seed=len(lengths))
+    weight = None if sink is None else torch.linspace(-2.0, 2.0, nh) + sink
+    want, size = c.plain(weight, cap)
+    before = ops.launch_count()
+    got, plan = c.run(sink=weight, cap=cap)
+    assert plan.n_items == 0 and ops.launch_count() - before == 1
+    assert bool(((got.double() - want).abs() <= bound(size, want, torch.bfloat16)).all())
+    before = ops.launch_count()
+    joined, _ = c.run(sink=weight, cap=cap, plan=plan, max_position=20000)
+    assert ops.launch_count() - before == (2 if len(lengths) < 10 else 1)
+    assert bool(((joined.double() - want).abs() <= bound(size, want, torch.bfloat16)).all())
+    assert bool((got[[n == 0 for n in lengths]] == 0).all()) and bool((joined[[n == 0 for n in lengths]] == 0).all())
+
+
+@pytest.mark.gpu
+def test_a_page_that_is_not_there_is_recorded_where_nothing_is_shared():
+    for page in (9999, -1):
+        c = Case([], [200, 100, 130], 4, 2, 128, 64, torch.bfloat16)
+        c.table[1, 1] = page
+        with pytest.raises(ops.KernelError, match="page pool"):
+            c.run()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_shared_attention_twice_is_the_same(dtype):
     c = Case(*SETS["many"], 12, 2, 128, 64, dtype, seed=9)
