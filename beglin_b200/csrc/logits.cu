@@ -26,7 +26,7 @@ struct LogitsParams {
     int* history;               // [n][cap] the tokens that a request holds, in order, or null
     int cap;
     const int* lengths;         // [n] how many, without `newest`
-    const int* prompts;         // [n] how many of them are the prompt's, or null: all are generated
+    const int* prompts;         // [n] how many of them, `newest` among them, are the prompt's, or null: all are generated
     const int* newest;          // [n] one more token, stored at history[r][lengths[r]] for the steps to come, or null
     const float *repetition, *frequency, *presence;      // [n], or null: 1, 0, 0
     const int* bias_id;         // the rows' biased tokens, ascending in each row, or null
@@ -209,7 +209,7 @@ struct LogitsMend {
                     if (i < w.len) hold(held[j], i < w.prompt);
                 }
             }
-            if (tid == 0 && p.newest) hold(w.newest, false);
+            if (tid == 0 && p.newest) hold(w.newest, w.len < w.prompt);
         }
         for (int i = b_at; i < w.b1; i += THREADS) {
             const int id = i == b_at ? b_id : p.bias_id[i], before = i == b_at ? b_before : p.bias_id[i - 1];

@@ -1402,8 +1402,8 @@ def adjust_logits(logits: torch.Tensor, out: torch.Tensor, *, history: Optional[
                   allowed_row: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None) -> None:
     """out = what a token is chosen from: float32 logits [n, V] (rows may lie apart) under penalties, biases and masks; `out` may be `logits`.
 
-    `history` int32 [n, room] holds each request's tokens in order, `lengths` [n] of them, of which the first `prompts` [n] are the
-    prompt's (None: none are); `newest` [n] is one token more, which is also stored behind the others.  A token that occurs among them,
+    `history` int32 [n, room] holds each request's tokens in order, `lengths` [n] of them; `newest` [n] is one token more, which is also
+    stored behind the others.  The first `prompts` [n] of all of them are the prompt's (None: none are).  A token that occurs among them,
     c times behind the prompt, has its logit x divided by `repetition` [n] where x > 0 and multiplied by it elsewhere, and then lowered by
     `frequency` [n] times c and, where c > 0, by `presence` [n] (float32; None: 1, 0, 0).  `bias` = (tokens int32, values float32,
     begins int32 [n + 1]): row r's biased tokens are tokens[begins[r] : begins[r + 1]], ascending (a token's values add up).  `allowed`

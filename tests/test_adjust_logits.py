@@ -215,3 +215,24 @@ def test_adjusted_logits_refuse_what_does_not_fit():
     refused("expected", allowed=words[:, :1].contiguous())
     refused("mask for each", allowed=words[:1].contiguous())
     refused("goes with masks", allowed_row=i32(0, 0))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("n,V,held,bias", [(3, 300, 5, 0), (70, 20011, 40, 3), (40, 33001, 13000, 2)])
+def test_the_newest_token_is_the_prompts_where_its_place_is(n, V, held, bias, in_place):
+    """A token in front of the prompt's end counts as the prompt's whether it is the newest or lies in the history: one kernel, a table of the text's tokens and
+    ranges of the vocabulary."""
+    x, a = _case(n, V, held, seed=n + V, bias=bias)
+    rows = torch.arange(n)
+    a["prompts"] = (a["lengths"] + torch.tensor([1, 7, 0])[rows % 3]).int()
+    whole = dict(a, history=a["history"].clone(), lengths=a["lengths"] + 1, newest=None)
+    whole["history"][rows, a["lengths"].long()] = a["newest"]
+    got, history = _run(x, a, in_place)
+    want, size = _plain(x, **whole)
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    fine = torch.isfinite(want)
+    # (the roundings of test_adjusted_logits, and at most four biases of one token)
+    assert bool(((got.double() - want).abs()[fine] <= 2.0 ** -24 * (5 + 4) * size[fine]).all())
+    assert torch.equal(got.nan_to_num(9.0), _run(x, whole, in_place)[0].nan_to_num(9.0))
+    assert torch.equal(history, whole["history"])

@@ -467,3 +467,21 @@ def test_generation_under_rules(model_root, graphs):
         eng.generate(prompts, rules=[small])
     with pytest.raises(ValueError, match="outside"):
         eng.generate(prompts, rules=LogitRules(bias={200: 1.0}))
+
+
+@pytest.mark.gpu
+def test_a_prompts_last_token_fed_by_a_decoding_step_is_the_prompts(model_root):
+    """A request whose prompt is in the cache but for its last token, which the first decoding step under rules brings: that token is no generated one."""
+    from beglin_b200 import LogitRules
+    folder, page = _folder(model_root, "qwen2", torch.float32)
+    eng = _engine(folder, "float32", page)
+    prompt, rules = _ids(20, 200, 1), LogitRules(frequency=3.0, presence=2.0, repetition=1.2)
+    for rid in "ab":
+        eng.step([(rid, prompt[:-1], [])])
+    made, row = [], eng.step([("a", prompt[-1:], [0])])[0]
+    for _ in range(3):
+        made += eng.decode(["b"], prompt[-1:] if not made else made[-1:], rules=[(rules, prompt, list(made))])
+        got, want = eng.decode_graph(1).logits[0].double().cpu(), _ruled(row, rules, prompt, made[:-1])
+        # the two step functions' rows agree in float32 to rounding, and three roundings more come with the rules
+        assert float((got - want).abs().max()) <= 1e-5 * float(want.abs().max())
+        row = eng.step([("a", made[-1:], [0])])[0]
