@@ -1416,7 +1416,8 @@ def adjust_logits(logits: torch.Tensor, out: torch.Tensor, *, history: Optional[
     n, V = shape
     if n == 0:
         return
-    ldx, ldo = (V if t.is_contiguous() else max(t.stride(0), V) if n == 1 else t.stride(0) if V == 1 or t.stride(1) == 1 else 0 for t in (logits, out))
+    # (one row has no next one, whose distance counts; a row's logits lie side by side whether there are others or not)
+    ldx, ldo = (V if t.is_contiguous() else 0 if V > 1 and t.stride(1) != 1 else max(t.stride(0), V) if n == 1 else t.stride(0) for t in (logits, out))
     if V == 0 or ldx < V or ldo < V:
         raise KernelError("adjust_logits: rows of at least one logit, side by side and apart from one another")
     x, y = logits.data_ptr(), out.data_ptr()

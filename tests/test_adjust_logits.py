@@ -236,3 +236,17 @@ def test_the_newest_token_is_the_prompts_where_its_place_is(n, V, held, bias, in
     assert bool(((got.double() - want).abs()[fine] <= 2.0 ** -24 * (5 + 4) * size[fine]).all())
     assert torch.equal(got.nan_to_num(9.0), _run(x, whole, in_place)[0].nan_to_num(9.0))
     assert torch.equal(history, whole["history"])
+
+
+def test_one_row_of_logits_lies_side_by_side_too():
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32)
+    row, apart, same = torch.zeros(1, 40), torch.zeros(1, 80)[:, ::2], torch.zeros(1, 1).expand(1, 40)
+    column = torch.zeros(40, 3).t()[:1]
+    for bad in (apart, same, column):
+        for logits, out in ((bad, row), (row, bad), (bad, bad)):
+            with pytest.raises(ops.KernelError, match="side by side"):
+                ops.adjust_logits(logits, out, history=torch.zeros((1, 4), dtype=torch.int32), lengths=i32(1))
+    # (one logit a row has nothing beside it, and one row nothing behind it)
+    for fine in (torch.zeros(1, 80)[:, :40], torch.zeros(1, 8)[:, ::8], torch.zeros(3, 8)[:, ::8], torch.zeros(2, 40)[:1], torch.zeros(1, 40).as_strided((1, 40), (7, 1))):
+        with pytest.raises(ops.KernelError, match="CUDA device only"):
+            ops.adjust_logits(fine, torch.zeros(fine.shape))
