@@ -191,8 +191,8 @@ class DecodeGraph:
             return
         groups = SharedPrefix(self.n, found.groups)
         if groups != self._groups:
-            self._groups = groups
             self.batch.renew(groups)
+            self._groups = groups
             # (before the first such step there is no plan to ask: it is captured, and its plans answer from then on)
             self._shares = not self.batch.plans or any(plan.shares for plan in self.batch.plans.values())
 
@@ -282,10 +282,12 @@ class DecodeGraph:
         self.turn = (self.turn + 1) % self.RING
         if st.event is not None:
             st.event.synchronize()             # the device has read this set's last contents
-        sent = 0
         positions = [cache.length(r) for r in rids]
         key = cache.identity(rids)             # a request that ended and one that began under its name differ
-        if key != self._rids or positions != self._positions:
+        variant, sent = self._load_rules(key, positions, rules)
+        known, ahead = (self._rids, self._positions), self._ahead
+        self._positions = self._ahead = None   # (a step that is given up from here on may leave its own positions and tables)
+        if (key, positions) != known:
             meta = st.meta.numpy()
             meta[0, :m], meta[0, m:] = positions, 0
             meta[1, :m], meta[1, m:] = cache.slot_ids(rids), cache.dump_slot
@@ -294,7 +296,8 @@ class DecodeGraph:
             b.slots.copy_(st.meta[1], non_blocking=True)
             self.advance.copy_(st.meta[2], non_blocking=True)
             sent += 12 * n
-            if key != self._rids:
+            if key != known[0]:
+                self._rids = None
                 self._regroup(rids)
             self._rids = key
         fed = tokens is not None and read_back     # the copies in and out are part of the replayed graph
@@ -318,9 +321,7 @@ class DecodeGraph:
         elif self._sampling:
             self.temperature.zero_()
             self._sampling = False
-        variant, loaded = self._load_rules(key, positions, rules)
-        sent += loaded
-        if self._ahead != (key, positions):    # else the last step has brought the tables up to date already
+        if ahead != (key, positions):          # else the last step has brought the tables up to date already
             sent += self._upload_tables(rids, st)
         if sent > (4 * n if fed else 0):
             st.event = torch.cuda.Event()

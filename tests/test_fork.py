@@ -485,3 +485,49 @@ def test_a_prompts_last_token_fed_by_a_decoding_step_is_the_prompts(model_root):
         # the two step functions' rows agree in float32 to rounding, and three roundings more come with the rules
         assert float((got - want).abs().max()) <= 1e-5 * float(want.abs().max())
         row = eng.step([("a", made[-1:], [0])])[0]
+
+
+@pytest.mark.gpu
+def test_a_step_that_was_given_up_leaves_nothing_for_the_next(model_root):
+    """A decoding step that its rules end when its positions have gone to the device; later another step's positions are those that the last whole step
+    left, in a page that has become another request's too."""
+    from beglin_b200 import LogitRules
+    folder, page = _folder(model_root, "qwen2", torch.float32)
+    eng = _engine(folder, "float32", page)
+    text, never, at = _ids(4 * page, 200, 1), LogitRules(allowed=lambda made: []), 2 * page - 4
+    eng.step([("a", text[:at + 5], []), ("b", text[:at], []), ("c", text[:at], [])])
+    eng.decode(["a"], text[:1])                            # on to position at + 6
+    with pytest.raises(ValueError, match="no token"):
+        eng.decode(["b"], text[at:at + 1], rules=[(never, text[:at], text[at:at + 1])])
+    eng.step([("b", text[at:at + 6], []), ("c", text[at:at + 6], [])])
+    eng.fork("b", ["d"])
+    rows = {rid: [] for rid in "bcd"}
+    for rid in "bcd":
+        for t in text[at + 6:at + 9]:
+            eng.decode([rid], [t])
+            rows[rid].append(eng.decode_graph(1).logits[0].clone())
+    for rid in "bd":
+        assert all(torch.equal(x, y) for x, y in zip(rows[rid], rows["c"]))
+
+
+@pytest.mark.gpu
+def test_pages_that_were_made_ready_are_asked_for_again_after_a_step_that_was_given_up(model_root, monkeypatch):
+    """A step that ends between the upload of its block tables and its replay (a capture that fails): the tables of the step before are not the device's any more."""
+    from beglin_b200 import LogitRules
+    folder, page = _folder(model_root, "qwen2", torch.float32)
+    eng = _engine(folder, "float32", page)
+    text = _ids(40, 200, 1)
+    for rid in "ac":
+        eng.step([(rid, text[:page + 3], [])])
+    eng.step([("b", _ids(page + 3, 200, 2), [])])
+    eng.decode(["c"], text[page + 3:page + 4])
+    eng.decode(["c"], text[page + 4:page + 5])
+    want = eng.decode_graph(1).logits[0].clone()
+    eng.decode(["a"], text[page + 3:page + 4])
+    graph = eng.decode_graph(1)
+    with monkeypatch.context() as m:
+        m.setattr(graph, "_capture", lambda *which: (_ for _ in ()).throw(RuntimeError("no room")))
+        with pytest.raises(RuntimeError, match="no room"):
+            eng.decode(["b"], [1], rules=[(LogitRules(bias={1: 1.0}), [0] * (page + 3), [1])])
+    eng.decode(["a"], text[page + 4:page + 5])
+    assert torch.equal(graph.logits[0], want)
