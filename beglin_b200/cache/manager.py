@@ -189,6 +189,7 @@ class CacheManager:
         # of the same name.
         self.births: Dict[Hashable, int] = {}
         self._born = 0
+        self.trims = 0                         # how often pages have been given back that a reservation took: whoever counts on one looks
         # One page and one state slot more than are ever handed out: rows that pad a batch of fixed shape
         # write their keys, values and state there, where no request reads.
         self.dump_page = num_pages
@@ -334,6 +335,7 @@ class CacheManager:
             for g in self.kv_groups:
                 table = g.tables[rid]
                 if len(table) > keep:
+                    self.trims += 1
                     g.pool.free([p for p in table[keep:] if p >= 0])
                     del table[keep:]
 

@@ -139,7 +139,7 @@ class DecodeGraph:
         self._positions: Optional[List[int]] = None
         self._tables: Dict[int, np.ndarray] = {}
         self._sampling = False
-        self._ahead = None                     # ((rids), positions) whose pages and tables are in place already
+        self._ahead = None                     # (rids, positions, the cache's trims) whose pages and tables are in place already
         self._ahead_bytes = 0
 
     def _body(self, rules: str) -> None:
@@ -233,12 +233,12 @@ class DecodeGraph:
         if sent:
             st.event = torch.cuda.Event()
             st.event.record()
-        self._ahead, self._ahead_bytes = (key, list(self._positions)), sent
+        self._ahead, self._ahead_bytes = (key, list(self._positions), cache.trims), sent
 
     def prepared(self, rids: Sequence[Hashable]) -> bool:
         """Whether the last step has already made room for the next step of exactly these requests."""
         cache = self.engine.cache
-        if self._ahead is None or not all(cache.has(r) for r in rids) or self._ahead[0] != cache.identity(rids):
+        if self._ahead is None or not all(cache.has(r) for r in rids) or self._ahead[::2] != (cache.identity(rids), cache.trims):
             return False
         return all(cache.length(r) == p for r, p in zip(rids, self._ahead[1]))
 
@@ -321,7 +321,7 @@ class DecodeGraph:
         elif self._sampling:
             self.temperature.zero_()
             self._sampling = False
-        if ahead != (key, positions):          # else the last step has brought the tables up to date already
+        if ahead != (key, positions, cache.trims):      # else the last step has brought the tables up to date already
             sent += self._upload_tables(rids, st)
         if sent > (4 * n if fed else 0):
             st.event = torch.cuda.Event()

@@ -531,3 +531,29 @@ def test_pages_that_were_made_ready_are_asked_for_again_after_a_step_that_was_gi
             eng.decode(["b"], [1], rules=[(LogitRules(bias={1: 1.0}), [0] * (page + 3), [1])])
     eng.decode(["a"], text[page + 4:page + 5])
     assert torch.equal(graph.logits[0], want)
+
+
+@pytest.mark.gpu
+def test_a_page_made_ready_and_given_back_is_asked_for_again(model_root, monkeypatch):
+    """A decoding step makes room for its next one; a portion of the same request that fails gives that page back, and another request takes it."""
+    folder, page = _folder(model_root, "qwen2", torch.float32)
+    eng = _engine(folder, "float32", page)
+    text, other = _ids(4 * page, 200, 1), _ids(2 * page + 1, 200, 2)
+    eng.step([("a", text[:2 * page - 1], [])])
+    eng.decode(["a"], text[2 * page - 1:2 * page])         # the next position begins a page
+    with monkeypatch.context() as m:
+        m.setattr(eng.model, "forward", lambda *a: (_ for _ in ()).throw(RuntimeError("no room")))
+        with pytest.raises(RuntimeError, match="no room"):
+            eng.step([("a", text[2 * page:2 * page + 3], [])])
+    eng.step([("b", other[:-1], [])])
+    got = []
+    for t in text[2 * page:2 * page + 4]:
+        eng.decode(["a"], [t])
+        got.append(eng.decode_graph(1).logits[0].clone())
+    eng.cache.check()
+    eng.step([("c", text[:2 * page], []), ("d", other[:-1], [])])
+    for t, row in zip(text[2 * page:], got):
+        eng.decode(["c"], [t])
+        assert torch.equal(eng.decode_graph(1).logits[0], row)
+    rows = eng.step([("b", other[-1:], [0]), ("d", other[-1:], [0])])
+    assert torch.equal(rows[0], rows[1])
