@@ -876,7 +876,7 @@ class SharedPlan:
         if kernel == "tc":
             self.room, sizes = _shared.items_room(n_rows, nh // nkv, nkv, self.sms, fixed), (n_rows, n_rows, n_rows)
         else:
-            self.room, sizes = _shared.blocks_room(n_rows), (2 * n_rows,)
+            self.room, sizes = _shared.blocks_room(n_rows, bq), (2 * n_rows,)
         # one buffer, so that a renewal is one copy: the list, then the rows' numbers
         total = self.room * 8 + sum(sizes)
         self.buffer = torch.zeros(total, dtype=torch.int32, device=self.device)
@@ -926,7 +926,7 @@ class SharedPlan:
             self.slots = self.MOST_RANGES if fixed else int(host[self.room * 8 + 2 * self.n_rows:].max()) if self.n_rows else 0
             self.least_own = 0 if fixed or not self.n_rows else int(host[self.room * 8 + self.n_rows:self.room * 8 + 2 * self.n_rows].min())
         else:
-            self.shares = used > self.n_rows
+            self.shares = int(items[:, 2].max(initial=0)) > 1      # (blocks of one row read for themselves)
             self.n_items = self.room if fixed else used
             own = items[:used][items[:used, 4] == _shared.MOST]
             self.slots = int(items[:used][items[:used, 4] != _shared.MOST][:, 4].max(initial=0))

@@ -33,9 +33,10 @@ def shared_blocks(shared, bq: int, split: int, room: int):
     return out, rows
 
 
-def blocks_room(n_rows: int) -> int:
-    """The most blocks that `shared_blocks` makes of n rows (a group has two rows at least)."""
-    return n_rows + n_rows // 2 + 1 if n_rows > 1 else 1
+def blocks_room(n_rows: int, bq: int = 3) -> int:
+    """The most blocks that `shared_blocks` makes of n rows: one for each, and those of the groups, of two rows and more: k rows in blocks of `bq` are k blocks
+    where bq is 1, at most 2 k / 3 where it is 2 (three rows), and at most k / 2 else."""
+    return n_rows + (n_rows if bq == 1 else 2 * n_rows // 3 if bq == 2 else n_rows // 2) + 1 if n_rows > 1 else 1
 
 
 # What the tensor-core kernels take, in microseconds, measured on B200 with heads of 128 features (64 do not differ much: these are latencies).  The shared

@@ -405,3 +405,32 @@ def test_shared_attention_refuses_what_does_not_fit():
     refused("sink", sink_weight=torch.zeros(3))
     refused("not negative", most=-1)
     refused("not negative", softcap=-1.0)
+
+
+@pytest.mark.parametrize("heads,hd,dtype,bq", [(64, 128, torch.float32, 2), (48, 64, torch.float32, 2), (64, 256, torch.float32, 1), (32, 256, torch.bfloat16, 1),
+                                               (64, 80, torch.bfloat16, 2), (12, 256, torch.bfloat16, 2)])
+@pytest.mark.parametrize("sizes", [(2,), (3, 3, 3), (4,), (5, 2, 3, 7), (3,) * 20, (1, 41), (2,) * 9])
+def test_blocks_of_one_and_of_two_rows_have_room(heads, hd, dtype, bq, sizes):
+    """Many query heads to a kv head: a block of the float units' kernels holds two rows, or one, which then has nobody to share with."""
+    groups, at = [], 1
+    for k in sizes:
+        groups.append((range(at, at + k), 700))
+        at += k
+    for fixed in (False, True):
+        plan = ops.shared_plan(SharedPrefix(at, groups), heads, 1, hd, dtype, split=64, device="cpu", fixed=fixed)
+        assert (plan.kernel, plan.bq) == ("generic", bq) and plan.shares == (bq > 1)
+        blocks = plan.items[plan.items[:, 2] > 0].tolist()
+        assert sorted(r for b in blocks if b[4] == shared_plan.MOST for r in plan.rows[b[1]:b[1] + b[2]].tolist()) == list(range(at))
+        together = [r for b in blocks if b[4] != shared_plan.MOST for r in plan.rows[b[1]:b[1] + b[2]].tolist()]
+        assert sorted(together) == sorted(r for g, _ in groups if len(g) > 1 for r in g)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nh,hd,dtype", [(64, 128, torch.float32), (48, 64, torch.float32), (32, 256, torch.bfloat16)])
+def test_shared_attention_of_many_heads_to_a_kv_head(nh, hd, dtype):
+    groups = [([1, 2, 3], 200), ([4, 6, 8], 130), ([9, 7, 5], 500), ([10, 11, 12, 13], 64)]
+    lengths = [70, 210, 201, 260, 131, 501, 150, 600, 140, 505, 65, 70, 128, 129]
+    c = Case(groups, lengths, nh, 1, hd, 16, dtype, seed=nh)
+    got, plan = c.run(prefer="generic", split=64)
+    assert plan.shares == (dtype == torch.float32)
+    assert torch.equal(got, c.alone(64))
