@@ -319,7 +319,7 @@ class CacheManager:
             tables = np.asarray([g.tables[rids[r]][:n] for r in rows], dtype=np.int64)
             differ = np.nonzero((tables != tables[0]).any(axis=0))[0]
             groups.append((rows, (int(differ[0]) if differ.size else n) * self.page_size))
-        return SharedPrefix(len(rids), groups) if groups else None
+        return SharedPrefix(len(rids), groups, [self.lengths[r] for r in rids]) if groups else None
 
     def identity(self, rids: Sequence[Hashable]) -> tuple:
         """(request, number of its start) for each: equal only for the same live requests."""

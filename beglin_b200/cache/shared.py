@@ -2,15 +2,19 @@
 `CacheManager.fork`)."""
 from __future__ import annotations
 
-from typing import List, Sequence, Tuple
+from typing import List, Optional, Sequence, Tuple
 
 
 class SharedPrefix:
     """`groups` = [(rows, positions)]: the requests of these rows (row r is request r) hold their first `positions` positions in the same pages.
-    A row is in one group at most; a row in none shares nothing."""
+    A row is in one group at most; a row in none shares nothing.  `lengths`: about how many positions every row's request holds in all, which whether
+    sharing pays hangs on (None: not known); prefixes of the same groups are equal whatever their lengths."""
 
-    def __init__(self, n_rows: int, groups: Sequence[Tuple[Sequence[int], int]]):
+    def __init__(self, n_rows: int, groups: Sequence[Tuple[Sequence[int], int]], lengths: Optional[Sequence[int]] = None):
         self.n_rows = int(n_rows)
+        self.lengths = None if lengths is None else tuple(int(n) for n in lengths)
+        if self.lengths is not None and (len(self.lengths) != self.n_rows or min(self.lengths, default=0) < 0):
+            raise ValueError(f"{self.n_rows} rows have as many lengths, none of them negative")
         self.groups: List[Tuple[Tuple[int, ...], int]] = []
         seen = set()
         for rows, positions in groups:

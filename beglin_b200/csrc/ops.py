@@ -948,7 +948,8 @@ def shared_plan(shared, nh: int, nkv: int, hd: int, dtype: torch.dtype, page_siz
     """The plan of `shared_attention` for the groups of `shared` (a `cache.shared.SharedPrefix`), heads of `hd` features (values of `vd`), a cache of `dtype` and
     queries of `query_dtype`.  Kernels: "tc" (bfloat16, heads of 64 or 128: the shared positions on tcgen05) or "generic" (every size and type, splits at
     multiples of `split` positions, whole splits shared: a row's result is bit for bit that of `attention`).  "auto" takes "tc" where it can, for the groups
-    whose sharing is expected to pay; "tc" shares whatever is shared.  `fixed`: launches of one shape for any groups,
+    whose sharing is expected to pay (`lengths` in `shared` let long requests count; where none pays, the plan's `shares` is False and
+    `attention` is the call to make); "tc" shares whatever is shared.  `fixed`: launches of one shape for any groups,
     for a captured graph, whose groups `SharedPlan.update` then renews."""
     vd, query_dtype = hd if vd is None else int(vd), query_dtype or dtype
     if nkv <= 0 or nh % nkv:

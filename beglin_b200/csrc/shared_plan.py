@@ -115,16 +115,23 @@ def alone_us(longest: int, total: int, n_rows: int, nkv: int, ranges, sms: int, 
 def worth_sharing(shared, group_heads: int, nkv: int, sms: int, room: int, most: int, own_ranges, alone_ranges, row_bytes: int,
                   page_size: int = 64):
     """The groups of `shared` whose sharing is expected to pay, those that save most first: few rows of few positions are read from the L2 again sooner than they
-    are split off and joined.  own_ranges, alone_ranges(streams, positions): how a stream is cut with sharing and without; `row_bytes`: of a key and a value of
-    one kv head."""
+    are split off and joined, and a long request beside a family is walked by fewer CTAs where its rows' own positions are cut by themselves.  A row is taken to
+    hold OWN_GUESS positions behind what it shares, or what `shared.lengths` says where that is more (63 rows of 8,192 shared positions and one request of 16,384
+    alone, 4 kv heads: 181 us row by row, 249 with sharing; with 2 kv heads 103 and 95).  own_ranges, alone_ranges(streams, positions): how a stream is cut with
+    sharing and without; `row_bytes`: of a key and a value of one kv head."""
     order = sorted(shared.groups, key=lambda g: -(len(g[0]) - 1) * g[1])
-    streams = shared.n_rows * nkv
-    best, kept = alone_us(max((p for _, p in order), default=0) + OWN_GUESS, sum(len(g) * p for g, p in order) + OWN_GUESS * shared.n_rows, shared.n_rows, nkv,
-                          alone_ranges, sms, row_bytes, page_size), 0
+    n, streams = shared.n_rows, shared.n_rows * nkv
+    before = np.zeros(n, dtype=np.int64)
+    for rows, p in order:
+        before[list(rows)] = p
+    own = np.full(n, OWN_GUESS) if shared.lengths is None else np.maximum(np.asarray(shared.lengths, dtype=np.int64) - before, OWN_GUESS)
+    walked = before + own                      # by the rows themselves
+    best, kept = alone_us(int(walked.max(initial=OWN_GUESS)), int(walked.sum()), n, nkv, alone_ranges, sms, row_bytes, page_size), 0
     for k in sorted({1, 2, len(order) // 2, len(order)} & set(range(1, len(order) + 1))):
-        left = order[k:]                       # groups that are left alone are walked by their rows
-        us = own_us(OWN_GUESS + max((p for _, p in left), default=0), OWN_GUESS * shared.n_rows + sum(len(g) * p for g, p in left), shared.n_rows, nkv, own_ranges,
-                    row_bytes)
+        walked = before + own
+        for rows, p in order[:k]:              # (groups that are left alone are walked by their rows)
+            walked[list(rows)] -= p
+        us = own_us(int(walked.max()), int(walked.sum()), n, nkv, own_ranges, row_bytes)
         us += cut_ranges([(len(g) * group_heads, p) for g, p in order[:k]], nkv, sms, room, most, streams)[2]
         if us < best:
             best, kept = us, k

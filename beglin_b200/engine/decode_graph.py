@@ -110,6 +110,7 @@ class _Staging:
 
 class DecodeGraph:
     RING = 4          # the host may prepare this many steps ahead of the device
+    REGROUP = 1024    # steps of the same requests after which it is asked again whether sharing pays: their own positions grow
 
     def __init__(self, engine, n: int):
         self.engine, self.n = engine, n
@@ -132,6 +133,7 @@ class DecodeGraph:
         self.graphs: Dict[tuple, tuple] = {}
         self._groups: Optional[SharedPrefix] = None    # what the requests share, for the variants that read it
         self._shares = False
+        self._regroup_at = 0                           # the first request's length at which that is asked again
         self.rules: Optional[RuleTables] = None
         self._rules_of = self._rules_next = None       # (rids, positions, rules) that the tables hold, and will once the step has run
         self.h2d_bytes = 0                     # bytes uploaded by the last step
@@ -189,8 +191,9 @@ class DecodeGraph:
         if found is None:
             self._groups, self._shares = None, False
             return
-        groups = SharedPrefix(self.n, found.groups)
-        if groups != self._groups:
+        groups = SharedPrefix(self.n, found.groups, found.lengths + (0,) * (self.n - len(rids)))
+        self._regroup_at = self.engine.cache.length(rids[0]) + self.REGROUP
+        if groups != self._groups or groups.lengths != self._groups.lengths:
             self.batch.renew(groups)
             self._groups = groups
             # (before the first such step there is no plan to ask: it is captured, and its plans answer from then on)
@@ -300,6 +303,8 @@ class DecodeGraph:
                 self._rids = None
                 self._regroup(rids)
             self._rids = key
+        if self._groups is not None and positions[0] >= self._regroup_at:
+            self._regroup(rids)
         fed = tokens is not None and read_back     # the copies in and out are part of the replayed graph
         if fed:
             self.h_in_np[:m] = tokens              # safe: the last fed step was waited for before it returned

@@ -557,3 +557,62 @@ def test_a_page_made_ready_and_given_back_is_asked_for_again(model_root, monkeyp
         assert torch.equal(eng.decode_graph(1).logits[0], row)
     rows = eng.step([("b", other[-1:], [0]), ("d", other[-1:], [0])])
     assert torch.equal(rows[0], rows[1])
+
+
+def test_groups_know_their_requests_lengths():
+    m = CacheManager([PagedKVNeed(1, 8)], 4, 40, 8)
+    _hold(m, "a", 10); _hold(m, "z", 33)
+    m.fork("a", ["b"])
+    _hold(m, "b", 15)
+    assert m.shared_prefix(["b", "z", "a"]).lengths == (15, 33, 10)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("graph", [False, True])
+def test_a_long_request_beside_a_family_is_not_left_to_one_block(model_root, graph, monkeypatch):
+    """A family beside a request that is much longer goes row by row, and in a captured step by the same graph, until it ends; then its pages are read once."""
+    from helpers import make_model
+    from beglin_b200.csrc import ops
+    eng = _engine(make_model(model_root, "wide", config=WIDE), "bfloat16", 64, max_tokens=32768, max_requests=40)
+    for part in range(4):
+        eng.step([("family", _ids(2048, 500, part), [])])
+    eng.fork("family", list(range(30)))
+    for part in range(9):
+        eng.step([("long", _ids(2048, 500, part), [])])
+    real, calls = ops.shared_attention, []
+    monkeypatch.setattr(ops, "shared_attention", lambda *a, **kw: calls.append(1) or real(*a, **kw))
+
+    def step(rids):
+        calls.clear()
+        if graph:
+            g = eng.decode_graph(len(rids))
+            eng.decode(rids, [3] * len(rids))
+            return g._shares
+        eng.step([(r, [3], [0]) for r in rids])
+        return bool(calls)
+
+    family = list(range(30)) + ["family"]
+    if graph:
+        step(family + ["long"])                            # (the first step of forked requests makes the plans, which answer from then on)
+    assert not step(family + ["long"])
+    assert step(family)
+
+
+@pytest.mark.gpu
+def test_whether_sharing_pays_is_asked_again_as_requests_grow(model_root, monkeypatch):
+    from helpers import make_model
+    from beglin_b200.csrc import shared_plan
+    from beglin_b200.engine.decode_graph import DecodeGraph
+    eng = _engine(make_model(model_root, "wide", config=WIDE), "bfloat16", 64, max_tokens=8192, max_requests=8)
+    eng.step([("a", _ids(200, 500, 1), [])])
+    eng.fork("a", ["b", "c"])
+    asked = []
+    monkeypatch.setattr(shared_plan, "worth_sharing", lambda shared, *a: asked.append(shared.lengths) or (shared.groups if shared.lengths[0] < 205 else []))
+    monkeypatch.setattr(DecodeGraph, "REGROUP", 4)
+    eng.decode(["a", "b", "c"], [1, 2, 3])                 # positions 200 .. 202 with sharing, to be asked again at 204
+    g = eng.decode_graph(3)
+    assert asked == [(200, 200, 200, 0)] and g._shares
+    for i in range(12):
+        eng.decode(["a", "b", "c"], [1, 2, 3])
+        assert g._shares == (eng.cache.length("a") <= 208)
+    assert asked == [(n, n, n, 0) for n in (200, 204, 208, 212)]

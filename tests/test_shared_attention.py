@@ -434,3 +434,26 @@ def test_shared_attention_of_many_heads_to_a_kv_head(nh, hd, dtype):
     got, plan = c.run(prefer="generic", split=64)
     assert plan.shares == (dtype == torch.float32)
     assert torch.equal(got, c.alone(64))
+
+
+def test_long_requests_beside_a_family_count():
+    """Times measured with heads of 128 in pages of 64, microseconds with sharing and row by row: the choice is the faster one."""
+    own, alone = (lambda streams, positions: ops.own_ranges(streams, positions, 148)), (lambda streams, positions: ops.decode_splits(streams, positions, 148))
+    for rows, shared, own_each, lone, nkv, sharing, without in ((63, 8192, 200, [16384], 4, 249.4, 181.4), (63, 4096, 200, [32000], 4, 458.2, 272.8),
+                                                                (60, 2048, 300, [4000, 8000, 16000, 32000], 4, 468.8, 260.0), (16, 8192, 200, [16384], 2, 45.9, 30.6),
+                                                                (8, 4096, 200, [4000] * 8, 2, 21.4, 13.6), (32, 4096, 200, [4000] * 32, 4, 82.8, 73.5),
+                                                                (63, 32000, 200, [32000], 4, 485.4, 468.9), (63, 8192, 200, [16384], 2, 95.3, 102.8),
+                                                                (63, 4096, 200, [32000], 2, 164.2, 196.9), (63, 8192, 200, [200], 4, 29.4, 111.1),
+                                                                (63, 8192, 3000, [16384], 2, 115.7, 129.2)):
+        group = (tuple(range(rows)), shared)
+        for front in (0, 1):                               # (lone requests first or last)
+            n = rows + len(lone)
+            group = (tuple(range(front * len(lone), front * len(lone) + rows)), shared)
+            lengths = lone * front + [shared + own_each + 7 * i % 50 for i in range(rows)] + lone * (1 - front)
+            kept = shared_plan.worth_sharing(SharedPrefix(n, [group], lengths), 6, nkv, 148, shared_plan.items_room(n, 6, nkv, 148), 64, own, alone, 512)
+            assert kept == ([group] if sharing < without else []), (rows, shared, lone, nkv)
+    with pytest.raises(ValueError, match="lengths"):
+        SharedPrefix(3, [([0, 1], 64)], [1, 2])
+    with pytest.raises(ValueError, match="lengths"):
+        SharedPrefix(3, [([0, 1], 64)], [1, 2, -1])
+    assert SharedPrefix(2, [([0, 1], 64)], [70, 80]) == SharedPrefix(2, [([0, 1], 64)])
