@@ -943,14 +943,9 @@ class SharedPlan:
         self.page_shape = (2, self.nkv, self.page_size, self.hd) if self.vd == self.hd else (self.nkv * self.page_size * (self.hd + self.vd),)
 
 
-def shared_plan(shared, nh: int, nkv: int, hd: int, dtype: torch.dtype, page_size: int = 64, vd: Optional[int] = None, split: int = 256, prefer: str = "auto",
-                query_dtype: Optional[torch.dtype] = None, device="cuda", fixed: bool = False) -> SharedPlan:
-    """The plan of `shared_attention` for the groups of `shared` (a `cache.shared.SharedPrefix`), heads of `hd` features (values of `vd`), a cache of `dtype` and
-    queries of `query_dtype`.  Kernels: "tc" (bfloat16, heads of 64 or 128: the shared positions on tcgen05) or "generic" (every size and type, splits at
-    multiples of `split` positions, whole splits shared: a row's result is bit for bit that of `attention`).  "auto" takes "tc" where it can, for the groups
-    whose sharing is expected to pay (`lengths` in `shared` let long requests count; where none pays, the plan's `shares` is False and
-    `attention` is the call to make); "tc" shares whatever is shared.  `fixed`: launches of one shape for any groups,
-    for a captured graph, whose groups `SharedPlan.update` then renews."""
+def shared_kernel(nh: int, nkv: int, hd: int, dtype: torch.dtype, page_size: int = 64, vd: Optional[int] = None, prefer: str = "auto",
+                  query_dtype: Optional[torch.dtype] = None) -> Tuple[str, int, int]:
+    """(kernel, rows of a block, positions of a tile) that `shared_plan` takes for these sizes and types."""
     vd, query_dtype = hd if vd is None else int(vd), query_dtype or dtype
     if nkv <= 0 or nh % nkv:
         raise KernelError(f"shared_plan: {nh} query heads are not a multiple of {nkv} kv heads")
@@ -963,13 +958,26 @@ def shared_plan(shared, nh: int, nkv: int, hd: int, dtype: torch.dtype, page_siz
     if prefer == "tc" and not takes:
         raise KernelError(f"shared_plan: the tensor-core kernels do not take {dtype} heads of {hd} with {group} query heads per kv head and pages of {page_size}")
     if takes and prefer != "generic":
-        plan = SharedPlan(shared.n_rows, nh, nkv, hd, vd, dtype, query_dtype, page_size, "tc", bq.value, 64, 0, device, fixed, prefer == "tc")
-    else:
-        if L.bg_attention_plan(group, hd, vd, 1, 1 if dtype == query_dtype == torch.float32 else 0, ctypes.byref(bq), ctypes.byref(tile)) != 0:
-            raise KernelError(f"shared_plan: heads of {hd} (values of {vd}) with {group} query heads per kv head are not supported")
-        if split <= 0 or split % tile.value:
-            raise KernelError(f"shared_plan: splits of {split} positions are not whole tiles of {tile.value}")
-        plan = SharedPlan(shared.n_rows, nh, nkv, hd, vd, dtype, query_dtype, page_size, "generic", bq.value, tile.value, split, device, fixed, True)
+        return "tc", bq.value, 64
+    if L.bg_attention_plan(group, hd, vd, 1, 1 if dtype == query_dtype == torch.float32 else 0, ctypes.byref(bq), ctypes.byref(tile)) != 0:
+        raise KernelError(f"shared_plan: heads of {hd} (values of {vd}) with {group} query heads per kv head are not supported")
+    return "generic", bq.value, tile.value
+
+
+def shared_plan(shared, nh: int, nkv: int, hd: int, dtype: torch.dtype, page_size: int = 64, vd: Optional[int] = None, split: int = 256, prefer: str = "auto",
+                query_dtype: Optional[torch.dtype] = None, device="cuda", fixed: bool = False) -> SharedPlan:
+    """The plan of `shared_attention` for the groups of `shared` (a `cache.shared.SharedPrefix`), heads of `hd` features (values of `vd`), a cache of `dtype` and
+    queries of `query_dtype`.  Kernels: "tc" (bfloat16, heads of 64 or 128: the shared positions on tcgen05) or "generic" (every size and type, splits at
+    multiples of `split` positions, whole splits shared: a row's result is bit for bit that of `attention`).  "auto" takes "tc" where it can, for the groups
+    whose sharing is expected to pay (`lengths` in `shared` let long requests count; where none pays, the plan's `shares` is False and
+    `attention` is the call to make); "tc" shares whatever is shared.  `fixed`: launches of one shape for any groups,
+    for a captured graph, whose groups `SharedPlan.update` then renews."""
+    kernel, bq, tile = shared_kernel(nh, nkv, hd, dtype, page_size, vd, prefer, query_dtype)
+    vd, query_dtype = hd if vd is None else int(vd), query_dtype or dtype
+    if kernel == "generic" and (split <= 0 or split % tile):
+        raise KernelError(f"shared_plan: splits of {split} positions are not whole tiles of {tile}")
+    plan = SharedPlan(shared.n_rows, nh, nkv, hd, vd, dtype, query_dtype, page_size, kernel, bq, tile, 0 if kernel == "tc" else split, device, fixed,
+                      prefer == "tc" or kernel == "generic")
     plan.update(shared)
     return plan
 

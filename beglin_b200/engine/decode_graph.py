@@ -187,7 +187,7 @@ class DecodeGraph:
 
     def _regroup(self, rids) -> None:
         """What the step's requests share: kept for the plans of the variant that reads it, and whether that variant pays."""
-        found = self.engine.cache.shared_prefix(rids) if len(rids) > 1 else None
+        found = self.engine.cache.shared_prefix(rids) if len(rids) > 1 and self.engine.ctx.reads_shared else None
         if found is None:
             self._groups, self._shares = None, False
             return

@@ -153,8 +153,13 @@ class GQAAttention:
         self.slopes = None if spec.slopes is None else torch.tensor(spec.slopes, dtype=torch.float64).to(torch.float32).to(ctx.device)
         # what the kernels are told: a positive number is a sliding window, a negative one the size of the blocks
         self.window = int(spec.window) if spec.window else (-int(spec.block) if spec.block else 0)
-        # positions that requests share are read once where a query sees them all, whatever their distance
-        self.sees_all = spec.window is None and spec.block is None and spec.slopes is None
+        # positions that requests share are read once where a query sees them all, whatever their distance, and by kernels that are not behind the layer's own:
+        # where only the decoding kernel takes the sizes on the tensor cores, it is ahead of the float units' sharing, whose blocks of one row share nothing
+        self.shared_kernel = dict(page_size=ctx.page_size, vd=kvd_, prefer="generic" if ctx.attention == "generic" else "auto", query_dtype=ctx.compute_dtype)
+        kernel, rows, _ = ops.shared_kernel(self.nh, self.nkv, khd, ctx.cache_dtype, **self.shared_kernel)
+        self.reads_shared = spec.window is None and spec.block is None and spec.slopes is None \
+            and (kernel == "tc" or rows > 1 and self.plans[True][0] == "generic")
+        ctx.reads_shared |= self.reads_shared
         # the fused q/k/v product can rotate and append itself: whole heads rotated in halves, a cache of its own
         # in bfloat16
         self.rope_in_product = (spec.own_kv and self.position.rotary_dim == self.hd and not self.position.interleaved
@@ -177,13 +182,9 @@ class GQAAttention:
                 for d, (_, bq, tile) in self.plans.items()}
 
     def _shared_plan(self, batch):
-        if not self.sees_all or getattr(batch, "shared", None) is None:
+        if not self.reads_shared or getattr(batch, "shared", None) is None:
             return None
-        khd, kvd_ = (self.hd, self.vd) if self.stored is None else (self.stored, self.stored)
-        plan = batch.shared_plan(self.nh, self.nkv, khd, self.ctx.cache_dtype, page_size=self.ctx.page_size, vd=kvd_, split=self.ctx.kv_split,
-                                 prefer="generic" if self.ctx.attention == "generic" else "auto", query_dtype=self.ctx.compute_dtype)
-        # (where only the decoding kernel takes the sizes on the tensor cores, it is ahead of the float units' sharing)
-        return None if plan is None or plan.kernel == "generic" and self.plans[True][0] != "generic" else plan
+        return batch.shared_plan(self.nh, self.nkv, self.stored or self.hd, self.ctx.cache_dtype, split=self.ctx.kv_split, **self.shared_kernel)
 
     takes_stream = True        # forward takes a NormedInput and may add its result to the stream itself
 

@@ -24,6 +24,7 @@ class BuildContext:
     # measured to pay; "all": wherever the sizes allow it (tests of the fused kernels on tiny models); False: nowhere
     fuse: object = True
     status: Optional[torch.Tensor] = None   # device word in which kernels record bad ids and pages
+    reads_shared: bool = False              # whether a layer reads positions that requests share once for all of them
     shared: Dict[object, object] = field(default_factory=dict)   # parts shared between layers, by spec
 
     def __post_init__(self):

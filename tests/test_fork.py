@@ -616,3 +616,23 @@ def test_whether_sharing_pays_is_asked_again_as_requests_grow(model_root, monkey
         eng.decode(["a", "b", "c"], [1, 2, 3])
         assert g._shares == (eng.cache.length("a") <= 208)
     assert asked == [(n, n, n, 0) for n in (200, 204, 208, 212)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["latent", "pages of 48"])
+def test_models_that_do_not_read_shared_positions_keep_one_graph(model_root, kind):
+    """Where no layer reads shared positions, or only by a kernel that its own is ahead of, forked requests go through the graph that every step goes through."""
+    from helpers import make_model
+    if kind == "latent":
+        import sukisun_helpers
+        page, dtype, folder = 16, "float32", sukisun_helpers.make_model(model_root, "sharp", seed=5)
+    else:                                                  # (a size that the tensor-core kernel of shared positions does not take)
+        page, dtype, folder = 48, "bfloat16", make_model(model_root, "wide", config=WIDE)
+    eng = _engine(folder, dtype, page)
+    text = _ids(3 * page + 2, 150, 1)
+    eng.step([("a", text, []), ("x", text[:5], []), ("y", text[:9], [])])
+    eng.decode(["x", "y"], [1, 2])
+    eng.fork("a", ["b"])
+    for _ in range(2):
+        eng.decode(["a", "b"], [1, 2])
+    assert len(eng.decode_graph(2).graphs) == 1
