@@ -74,7 +74,7 @@ class Engine:
                 limit = min(limit, spec.max_positions)
             self.cache = CacheManager(self.model.cache_needs(), page_size, num_pages, max_requests, limit)
             self.cache.allocate(self.device, self.dtype)
-        self.sampler = Sampler(self.device)
+        self.sampler = Sampler(self.device, self.ctx.status)
         self.vocab = spec.vocab
         self.use_graphs = use_graphs
         self._graphs = {}

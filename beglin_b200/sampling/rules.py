@@ -122,7 +122,10 @@ class RuleTables:
         history, ids, values, begins = np.zeros((len(rows), width), dtype=np.int32), [], [], [0]
         for r, ((rules, prompt, _), text) in enumerate(zip(rows, texts)):
             prompts[r] = len(prompt)
-            history[r, :len(text)] = text
+            tokens = np.asarray(text, dtype=np.int64)
+            if len(text) and (tokens.min() < 0 or tokens.max() >= self.vocab):
+                raise ValueError(f"row {r}: token {int(tokens[(tokens < 0) | (tokens >= self.vocab)][0])} of its text is outside the vocabulary [0, {self.vocab})")
+            history[r, :len(text)] = tokens
             if rules is not None:
                 rules.check(self.vocab)
                 pen[:, r] = rules.repetition, rules.frequency, rules.presence

@@ -50,8 +50,9 @@ class SamplingParams:
 
 
 class Sampler:
-    def __init__(self, device):
-        self.device = torch.device(device)
+    def __init__(self, device, status: Optional[torch.Tensor] = None):
+        """`status`: the word in which kernels record what is wrong, for whoever looks at it (`ops.raise_on_status`); without one `sample` looks itself."""
+        self.device, self.status = torch.device(device), status
 
     def sample(self, logits: torch.Tensor, temperatures: Sequence[float], uniforms: Sequence[float], rules: Optional[Sequence] = None) -> List[int]:
         """One token per row of float logits [n, V]; rows with temperature <= 0 are greedy.  `rules`: (LogitRules or None, prompt, generated tokens) of every row;
@@ -62,7 +63,10 @@ class Sampler:
             tables = RuleTables(n, logits.shape[1], max(lengths), logits.device)
             tables.load(rules)
             tables.load_masks(rules)
-            tables.apply(logits, torch.tensor(lengths, dtype=torch.int32).to(logits.device), None, None, tables.masked)
+            status = self.status if self.status is not None else ops.new_status(logits.device)
+            tables.apply(logits, torch.tensor(lengths, dtype=torch.int32).to(logits.device), None, status, tables.masked)
+            if self.status is None:
+                ops.raise_on_status(status)
         out = torch.empty(n, dtype=torch.int32, device=logits.device)
         if any(t > 0.0 for t in temperatures):
             t = torch.from_numpy(np.asarray(temperatures, dtype=np.float32)).to(logits.device)

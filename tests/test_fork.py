@@ -636,3 +636,35 @@ def test_models_that_do_not_read_shared_positions_keep_one_graph(model_root, kin
     for _ in range(2):
         eng.decode(["a", "b"], [1, 2])
     assert len(eng.decode_graph(2).graphs) == 1
+
+
+@pytest.mark.parametrize("text", [([3, 50], []), ([3], [4, -1]), ([2 ** 33], [1])])
+def test_a_text_with_a_token_outside_the_vocabulary_is_refused(text):
+    """The host has the texts: what the kernel would pass over and record is refused before it goes to the device."""
+    from beglin_b200.sampling import LogitRules
+    from beglin_b200.sampling.rules import RuleTables
+    tables = RuleTables(2, 50, 8, "cpu")
+    before = tables.history.clone()
+    with pytest.raises(ValueError, match="outside the vocabulary"):
+        tables.load([(None, [1], []), (LogitRules(presence=1.0),) + text])
+    assert torch.equal(tables.history, before)
+    tables.load([(None, [1], []), (LogitRules(presence=1.0), [49], [0])])
+    assert tables.history[1, :2].tolist() == [49, 0]
+
+
+@pytest.mark.gpu
+def test_what_is_recorded_under_rules_reaches_the_caller(monkeypatch):
+    from beglin_b200.csrc import ops
+    from beglin_b200.sampling import LogitRules, Sampler
+    from beglin_b200.sampling.rules import RuleTables
+    status = ops.new_status("cuda:0")
+    sampler, rules = Sampler("cuda:0", status), LogitRules(presence=1.0)
+    logits = torch.arange(100, dtype=torch.float32, device="cuda:0").repeat(2, 1)
+    assert sampler.sample(logits.clone(), [0.0, 0.0], [0.0, 0.0], [(rules, [3], [99]), (None, [3], [99])]) == [98, 99]
+    ops.raise_on_status(status)
+    monkeypatch.setattr(RuleTables, "load", lambda self, rows: (self.history.fill_(100), self.penalties.fill_(2.0)))
+    sampler.sample(logits.clone(), [0.0, 0.0], [0.0, 0.0], [(rules, [3], [99]), (None, [3], [99])])
+    with pytest.raises(ops.KernelError, match="token id"):
+        ops.raise_on_status(status)
+    with pytest.raises(ops.KernelError, match="token id"):
+        Sampler("cuda:0").sample(logits.clone(), [0.0, 0.0], [0.0, 0.0], [(rules, [3], [99]), (None, [3], [99])])
