@@ -888,6 +888,8 @@ class SharedPlan:
         self.rows = self.arrays[0]
         if kernel == "tc":
             self.own_first, self.parts = self.arrays[1:]
+        # ranges of a group, at most: a captured call makes room for so many results of every row, and more than a wave of CTAs would be no faster
+        self.most = min(self.MOST_RANGES, -(-self.sms // nkv)) if fixed else self.MOST_RANGES
         self.slots = 0         # results of a row over what it shares, at most
 
     MOST_RANGES = 64
@@ -898,11 +900,11 @@ class SharedPlan:
             raise KernelError(f"shared_plan: groups of {shared.n_rows} rows for a plan of {self.n_rows}")
         if self.kernel == "tc":
             if not self.all_groups:
-                kept = _shared.worth_sharing(shared, self.nh // self.nkv, self.nkv, self.sms, self.room, self.MOST_RANGES,
+                kept = _shared.worth_sharing(shared, self.nh // self.nkv, self.nkv, self.sms, self.room, self.most,
                                              lambda streams, positions: own_ranges(streams, positions, self.sms),
                                              lambda streams, positions: decode_splits(streams, positions, self.sms), 4 * self.hd, self.page_size)
                 shared = type(shared)(self.n_rows, kept)
-            arrays = _shared.shared_items(shared, self.nh // self.nkv, self.nkv, self.sms, self.room, self.MOST_RANGES)
+            arrays = _shared.shared_items(shared, self.nh // self.nkv, self.nkv, self.sms, self.room, self.most)
         else:
             arrays = _shared.shared_blocks(shared, self.bq, self.split, self.room)
         return np.concatenate([a.reshape(-1) for a in arrays])
@@ -923,7 +925,7 @@ class SharedPlan:
         if self.kernel == "tc":
             self.shares = used > 0             # whether anything is read for several rows at once
             self.n_items = self.room if fixed else used
-            self.slots = self.MOST_RANGES if fixed else int(host[self.room * 8 + 2 * self.n_rows:].max()) if self.n_rows else 0
+            self.slots = self.most if fixed else int(host[self.room * 8 + 2 * self.n_rows:].max()) if self.n_rows else 0
             self.least_own = 0 if fixed or not self.n_rows else int(host[self.room * 8 + self.n_rows:self.room * 8 + 2 * self.n_rows].min())
         else:
             self.shares = int(items[:, 2].max(initial=0)) > 1      # (blocks of one row read for themselves)

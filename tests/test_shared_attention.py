@@ -457,3 +457,17 @@ def test_long_requests_beside_a_family_count():
     with pytest.raises(ValueError, match="lengths"):
         SharedPrefix(3, [([0, 1], 64)], [1, 2, -1])
     assert SharedPrefix(2, [([0, 1], 64)], [70, 80]) == SharedPrefix(2, [([0, 1], 64)])
+
+
+@pytest.mark.parametrize("nh,nkv", [(12, 2), (28, 4), (64, 8), (16, 16), (7, 1)])
+def test_a_captured_call_has_room_for_one_wave_of_ranges(nh, nkv):
+    rng = np.random.default_rng(nh)
+    sets = [_random_groups(rng) for _ in range(8)] + [SharedPrefix(90, [(range(90), 120000)]), SharedPrefix(90, [([0, 1], 60000), (range(2, 90), 64)])]
+    for shared in sets:
+        plan = ops.shared_plan(shared, nh, nkv, 128, torch.bfloat16, prefer="tc", device="cpu", fixed=True)
+        items = plan.items[plan.items[:, 2] > 0]
+        assert plan.slots <= min(64, -(-148 // nkv)) and (not len(items) or int(items[:, 5].max()) < plan.slots)
+        assert int(plan.parts.max()) <= plan.slots
+        for group, positions in shared.groups:
+            assert sorted((a, b) for req, _, _, a, b, _, _, _ in items.tolist() if req == group[0] and a == 0)
+            assert max(b for req, _, _, _, b, _, _, _ in items.tolist() if req == group[0]) == positions
