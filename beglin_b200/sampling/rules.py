@@ -19,6 +19,18 @@ from ..csrc import ops
 MOST_BIASES = 512          # biased tokens of a request
 
 
+class Biases(dict):
+    """Token -> bias, as given: replayed steps keep what they have loaded for as long as the rules are the same."""
+
+    def _stay(self, *args, **kw):
+        raise TypeError("the biases of rules stay as they are: make new rules")
+
+    __setitem__ = __delitem__ = __ior__ = update = pop = popitem = clear = setdefault = _stay
+
+    def __reduce__(self):
+        return Biases, (dict(self),)
+
+
 @dataclass(frozen=True)
 class LogitRules:
     """`allowed` is called before every token with the tokens that the request has generated so far and returns which may come next: token ids, truth
@@ -30,7 +42,7 @@ class LogitRules:
     allowed: Optional[Callable[[Sequence[int]], Optional[Sequence[int]]]] = None
 
     def __post_init__(self):
-        object.__setattr__(self, "bias", dict(self.bias))      # (the caller's own may change)
+        object.__setattr__(self, "bias", Biases(self.bias))    # (the caller's own may change)
 
     def check(self, vocab: int) -> None:
         if not (self.repetition > 0.0 and math.isfinite(self.repetition)):

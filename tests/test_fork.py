@@ -668,3 +668,18 @@ def test_what_is_recorded_under_rules_reaches_the_caller(monkeypatch):
         ops.raise_on_status(status)
     with pytest.raises(ops.KernelError, match="token id"):
         Sampler("cuda:0").sample(logits.clone(), [0.0, 0.0], [0.0, 0.0], [(rules, [3], [99]), (None, [3], [99])])
+
+
+def test_the_biases_of_rules_stay_as_they_are():
+    """Replayed steps keep the tables of rules that they know: rules do not change behind them."""
+    import copy
+    import pickle
+    from beglin_b200.sampling import LogitRules
+    rules = LogitRules(bias={3: 1.0})
+    for change in (lambda b: b.update({3: 2.0}), lambda b: b.__setitem__(4, 1.0), lambda b: b.pop(3), lambda b: b.clear(), lambda b: b.popitem(), lambda b: b.setdefault(5, 1.0),
+                   lambda b: b.__delitem__(3), lambda b: b.__ior__({5: 1.0})):
+        with pytest.raises(TypeError, match="stay"):
+            change(rules.bias)
+    for same in (copy.copy(rules), copy.deepcopy(rules), pickle.loads(pickle.dumps(rules))):
+        assert same == rules == LogitRules(bias={3: 1.0}) and same.bias == {3: 1.0}
+    assert {**rules.bias, 4: 1.0} == {3: 1.0, 4: 1.0} and LogitRules(bias=rules.bias) == rules
