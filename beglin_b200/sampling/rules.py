@@ -82,6 +82,8 @@ class LogitRules:
                 raise ValueError(f"allowed: truth values of {given.shape}, expected ({vocab},)")
             bits = given
         else:
+            if given.size and given.dtype.kind not in "iu":
+                raise ValueError(f"allowed: token ids are whole numbers, got {given.dtype}")
             ids = given.astype(np.int64).reshape(-1)
             if ids.size and (ids.min() < 0 or ids.max() >= vocab):
                 raise ValueError(f"allowed: token {int(ids[(ids < 0) | (ids >= vocab)][0])} is outside the vocabulary [0, {vocab})")

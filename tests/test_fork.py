@@ -683,3 +683,11 @@ def test_the_biases_of_rules_stay_as_they_are():
     for same in (copy.copy(rules), copy.deepcopy(rules), pickle.loads(pickle.dumps(rules))):
         assert same == rules == LogitRules(bias={3: 1.0}) and same.bias == {3: 1.0}
     assert {**rules.bias, 4: 1.0} == {3: 1.0, 4: 1.0} and LogitRules(bias=rules.bias) == rules
+
+
+def test_ids_of_a_mask_are_whole_numbers():
+    from beglin_b200.sampling import LogitRules
+    for bad in ([1.5], [3.0], ["5"], [2 ** 70], np.asarray([1.0, 2.0])):
+        with pytest.raises(ValueError, match="whole numbers"):
+            LogitRules(allowed=lambda made: bad).mask([], 70)
+    assert LogitRules(allowed=lambda made: np.asarray([5], dtype=np.int16)).mask([], 70).tolist() == [32, 0, 0]
