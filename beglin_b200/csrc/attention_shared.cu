@@ -65,7 +65,11 @@ attention_shared_merge_kernel(const float* __restrict__ part_o, const float* __r
         float top = m;
 #pragma unroll
         for (int j = 0; j < AT_ONCE; ++j) top = fmaxf(top, ml[j].x);
-        if (top == -INFINITY) continue;                // no position seen so far
+        if (top == -INFINITY) {                        // no position seen so far, or scores that are no numbers: those have no maximum, and show by their sum
+#pragma unroll
+            for (int j = 0; j < AT_ONCE; ++j) l += ml[j].y;
+            continue;
+        }
         const float keep = expf(m - top);
         l *= keep; acc.x *= keep; acc.y *= keep; acc.z *= keep; acc.w *= keep;
         m = top;

@@ -471,3 +471,47 @@ def test_a_captured_call_has_room_for_one_wave_of_ranges(nh, nkv):
         for group, positions in shared.groups:
             assert sorted((a, b) for req, _, _, a, b, _, _, _ in items.tolist() if req == group[0] and a == 0)
             assert max(b for req, _, _, _, b, _, _, _ in items.tolist() if req == group[0]) == positions
+
+
+def test_the_exponentials_of_the_float_units_are_as_near_as_is_said():
+    """The polynomial in place of 2^f, evaluated in 64 bits from the numbers that the kernel holds: 2.7e-6 of it on [-1/2, 1/2]."""
+    import os
+    import re
+    text = open(os.path.join(os.path.dirname(ops.__file__), "attention_tcgen05.cu")).read()
+    body = text[text.index("at_ex2_float2(unsigned long long x) {"):text.index("const unsigned long long two_n")]
+    numbers = [float(a) for a, b in re.findall(r"pair2\((0\.\d+)f, (0\.\d+)f\)", body) if a == b]
+    assert len(numbers) == 5
+    f = np.linspace(-0.5, 0.5, 200001)
+    worst = np.abs(np.polyval(np.asarray(numbers, dtype=np.float32).astype(np.float64), f) / np.exp2(f) - 1.0).max()
+    assert worst <= 2.7e-6
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["two", "many", "long", "none"])
+@pytest.mark.parametrize("what", [float("nan"), float("inf")])
+@pytest.mark.parametrize("sink", [False, True])
+def test_a_row_that_is_no_number_shows_it(name, what, sink):
+    """A query that is not a number, or infinite (its scores are then no numbers either): its row is no number, as without sharing, and the others are theirs."""
+    c = Case(*SETS[name], 12, 2, 128, 64, torch.bfloat16, seed=2)
+    c.q[1] = what
+    weight = torch.linspace(-1, 2, 12) if sink else None
+    rest = [r for r in range(len(c.lengths)) if r != 1]
+    want, size = c.plain(weight)
+    for most in (None, 20000):                             # (ranges of a row's own positions, and for rows that share nothing one kernel or two)
+        got, _ = c.run(sink=weight, max_position=most)
+        assert bool(torch.isnan(got[1].float()).all())
+        assert bool(((got.double() - want).abs() <= bound(size, want, torch.bfloat16))[rest].all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 128])
+def test_weights_of_nothing(hd):
+    """Scores so far apart that all weights but one are nothing (below 2^-126 of the largest), among the shared positions and among a row's own."""
+    c = Case(*SETS["many"], 12, 2, hd, 64, torch.bfloat16, seed=hd)
+    for row, at in ((1, 17), (7, 999), (20, 1000), (30, c.lengths[30] - 1)):
+        c.q[row] = (16.0 * c.keys[row][at].float().repeat_interleave(6, 0)).reshape(-1).to(torch.bfloat16)
+    got, plan = c.run()
+    want, size = c.plain()
+    # (with hd features the largest score leads by more than 16 sqrt(hd) less the rest's spread, some 100 in base two: what is left of the others is nothing
+    # beside the bound, and so is a score's own error)
+    assert plan.n_items > 0 and bool(((got.double() - want).abs() <= bound(size, want, torch.bfloat16)).all())
