@@ -96,7 +96,7 @@ __device__ __forceinline__ float at_ex2(float x) {
 }
 
 // 2^x of two numbers up to 2^8 by the float units: 2^n from the bits of n = x rounded, times a polynomial of degree four in x - n.  Its coefficients make the
-// largest relative error on [-1/2, 1/2] as small as can be (Remez' exchange algorithm): 2.6e-6.  Below -126 it is 2^-126; what is not a number stays so.
+// largest relative error on [-1/2, 1/2] as small as can be (Remez' exchange algorithm): 2.7e-6, their roundings to floats included.  Below -126 it is 2^-126; what is not a number stays so.
 __device__ __forceinline__ unsigned long long at_ex2_float2(unsigned long long x) {
     float a = low2(x), b = high2(x);
     asm("max.NaN.f32 %0, %0, %1;\n" : "+f"(a) : "f"(-126.0f));
