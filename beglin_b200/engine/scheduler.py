@@ -15,7 +15,7 @@ shortened to what the free pages hold, down to nothing.  A request that does not
 the only one ends with the reason "out_of_pages".
 
 Several completions of one prompt are a family: the lead is a request like others, and when its prompt is in the cache the others go on from there
-(`adopt`), as far as there are slots and pages for them; the rest wait in the queue as requests with a prompt of their own.
+(`adopt`), as far as there are slots and pages for them; the rest wait in the queue as a family of their own.
 
 Pure host code: it talks to the cache manager's accounting and is tested without a GPU.
 """
@@ -297,7 +297,8 @@ class Scheduler:
 
     def adopt(self, lead: Request) -> List[Request]:
         """Start siblings of `lead`, whose prompt's last step has run, from what it holds (before `update`, which may end it).  Those that there is no slot or
-        page for go to the head of the queue.  Returns those that have started: each takes its first token from the lead's logits (`first_tokens`)."""
+        page for go to the head of the queue as a family of their own, whose first brings the prompt again.  Returns those that have started: each takes its
+        first token from the lead's logits (`first_tokens`)."""
         family, lead.siblings = lead.siblings, []
         free = min(self.max_batch - len(self.running), self.cache.max_requests - len(self.cache.live()))
         if self.cache.length(lead.rid) % self.cache.page_size:
@@ -310,9 +311,10 @@ class Scheduler:
             r.admitted_at = self._clock
             self._clock += 1
             self.running.append(r)
-        for r in reversed(later):
-            r.tokens_in, r.phase = list(r.prompt), "waiting"
-            self.waiting.appendleft(r)
+        if later:
+            first = later[0]
+            first.siblings, first.tokens_in, first.phase = later[1:], list(first.prompt), "waiting"
+            self.waiting.appendleft(first)
         return now
 
     def first_tokens(self, started: Sequence[Request], tokens: Sequence[int]) -> None:

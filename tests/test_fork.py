@@ -691,3 +691,15 @@ def test_ids_of_a_mask_are_whole_numbers():
         with pytest.raises(ValueError, match="whole numbers"):
             LogitRules(allowed=lambda made: bad).mask([], 70)
     assert LogitRules(allowed=lambda made: np.asarray([5], dtype=np.int16)).mask([], 70).tolist() == [32, 0, 0]
+
+
+@pytest.mark.parametrize("slots,completions,runs", [(3, 9, 3), (8, 16, 2), (1, 4, 4), (4, 5, 2)])
+def test_what_is_left_of_a_family_is_one(slots, completions, runs):
+    """Completions that find no slot bring the prompt again for as many of them as find one then, not each for itself."""
+    m = CacheManager([PagedKVNeed(1, 8)], 4, 200, slots)
+    sched = Scheduler(m, max_batch=slots)
+    family = _family(0, 30, 5, completions)
+    sched.add(family[0])
+    _drive(sched)
+    assert sched.counters.prefill_rows == 30 * runs
+    assert [r.output for r in family] == [[100 + i for i in range(5)]] * completions and len(sched.finished) == completions
