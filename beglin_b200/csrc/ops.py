@@ -991,7 +991,8 @@ def shared_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_table: torch.
     read once for all of its rows, through the pages of the group's first row, and what lies behind through each row's own.  q [T, nh * hd] (rows may lie
     apart), kv_pool and block_table as `attention` takes them, `max_position` a bound on the positions, out [T, nh * vd].  `sink`, `sink_weight` and
     `softcap` as in `attention`.  A row whose position lies inside what its group shares sees that far; values behind it that are not finite reach it, which
-    those behind the shared positions never do."""
+    those behind the shared positions never do.  In the "tc" form a weight below 2^-126 of the largest in its range of shared positions may count as 2^-126 (which
+    only values near bfloat16's largest show)."""
     # (every look at a tensor costs the host a tenth of a microsecond or two, as much as a small step's kernels in all: contiguous tensors are asked for little)
     T, pool_shape, table_shape = plan.n_rows, kv_pool.shape, block_table.shape
     if positions.dtype != torch.int32 or block_table.dtype != torch.int32 or not positions.is_contiguous() or not block_table.is_contiguous():

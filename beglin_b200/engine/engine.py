@@ -227,8 +227,9 @@ class Engine:
         the reference's `greedy` mode does.  `mixed` False runs every prompt in steps of its own while the
         decoding requests wait (the reference's QWEN_CB_MIXED=0); the tokens are the same.
 
-        `completions` k > 1: k completions of every prompt, which goes through the model once; the result is then a list of k lists per
-        prompt.  `rules`: what the choice of tokens obeys (`sampling.LogitRules`: penalties, biases, a mask of the tokens that may come
+        `completions` k > 1: k completions of every prompt; the result is then a list of k lists per prompt.  Those for which a slot and a page are
+        free when a prompt's first completion has brought it go on from there; the others wait as a family of their own that brings it again (many
+        prompts at once take the slots for their first completions: fewer prompts a call, or more slots, share more).  `rules`: what the choice of tokens obeys (`sampling.LogitRules`: penalties, biases, a mask of the tokens that may come
         next), one for all prompts or one for each."""
         if completions < 1:
             raise ValueError(f"completions={completions}, at least one")
