@@ -267,7 +267,7 @@ class CacheManager:
 
     def fork(self, rid: Hashable, new_rids: Sequence[Hashable]) -> None:
         """Start requests that go on from what `rid` holds now: its whole pages together with it, the positions behind them and its state of fixed size as
-        copies of their own.  Raises and changes nothing where names are taken or slots or pages run out."""
+        copies of their own.  Raises and changes nothing where names are taken, slots or pages run out or a copy cannot be made."""
         new_rids = list(new_rids)
         if rid not in self.lengths:
             raise CacheError(f"request {rid!r} is not live")
@@ -292,6 +292,17 @@ class CacheManager:
             for new in new_rids:
                 g.pool.share([p for p in table[:whole] if p >= 0])
                 g.tables[new] = table[:whole] + (g.pool.alloc(1) if rest else [])
+        try:
+            self._copy_fork(rid, new_rids, whole, rest)
+        except Exception:                      # (nobody goes on from what was not copied)
+            for new in new_rids:
+                self.release(new)
+            raise
+
+    def _copy_fork(self, rid: Hashable, new_rids: Sequence[Hashable], whole: int, rest: int) -> None:
+        """What a fork does not share: `rest` positions behind the whole pages, and state of fixed size."""
+        for g in self.kv_groups:
+            table = g.tables[rid]
             if rest and new_rids and g.device_pool is not None and table[whole] >= 0:
                 for part in g.need.page_parts(g.device_pool, self.page_size):
                     ops().copy_pages(part, [table[whole]] * len(new_rids), [g.tables[new][whole] for new in new_rids], rest)

@@ -703,3 +703,16 @@ def test_what_is_left_of_a_family_is_one(slots, completions, runs):
     _drive(sched)
     assert sched.counters.prefill_rows == 30 * runs
     assert [r.output for r in family] == [[100 + i for i in range(5)]] * completions and len(sched.finished) == completions
+
+
+@pytest.mark.parametrize("needs", [[PagedKVNeed(1, 8)], [PagedKVNeed(1, 8), FixedStateNeed((3,))], [FixedStateNeed((3,))]])
+def test_a_fork_whose_copies_cannot_be_made_leaves_no_request(needs):
+    from beglin_b200.csrc import ops
+    m = CacheManager(needs, 4, 8, 4)
+    m.allocate("cpu", torch.float32)                       # (the kernel copies on a device only)
+    _hold(m, "a", 10)
+    before = (m.free_pages(), list(m._free_slots))
+    with pytest.raises(ops.KernelError, match="CUDA device only"):
+        m.fork("a", ["b", "c"])
+    assert m.live() == ["a"] and m.free_pages() == before[0] and sorted(m._free_slots) == sorted(before[1])
+    m.check()
