@@ -208,6 +208,22 @@ _SIGNATURES = {
     "bg_adjust_logits": [_c_void_p, ctypes.POINTER(_c_int), _c_void_p],
     "bg_copy_pages_most": [],
     "bg_copy_pages": [_c_void_p, _c_int, _c_ll, _c_int, _c_ll, _c_int, _c_int, _c_ll, _c_int, _c_void_p, _c_void_p, _c_int, _c_void_p],
+    "bg_packed_tile_bytes": [_c_int],
+    "bg_packed_append": [_c_void_p, _c_int, _c_ll, _c_int, _c_ll, _c_void_p, _c_int, _c_ll, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int,
+                         _c_void_p, _c_ll, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_void_p, _c_void_p],
+    "bg_packed_rows": [_c_void_p, _c_ll, _c_int, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_void_p, _c_int, _c_int, _c_int, _c_int,
+                       _c_void_p, _c_void_p],
+    "bg_packed_bounds": [_c_void_p, _c_ll, _c_int, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_void_p, _c_void_p],
+    "bg_packed_wide_page": [],
+    "bg_packed_unpack": [_c_void_p, _c_ll, _c_int, _c_int, _c_void_p, _c_void_p, _c_int, _c_int, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_int, _c_int,
+                         _c_int, _c_int, _c_void_p, _c_void_p],
+    "bg_packed_attention_columns": [_c_int, _c_int, _c_int, ctypes.POINTER(_c_int)],
+    "bg_packed_attention": [_c_void_p, _c_int, _c_ll, _c_void_p, _c_ll, _c_int, _c_int, _c_void_p, _c_int, _c_int, _c_void_p, _c_void_p, _c_int, _c_int,
+                            _c_void_p, _c_int, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_float, _c_void_p, _c_int, _c_void_p,
+                            _c_ll, _c_void_p, _c_void_p],
+    "bg_packed_select_most": [],
+    "bg_packed_select": [_c_void_p, _c_int, _c_ll, _c_void_p, _c_ll, _c_int, _c_int, _c_void_p, _c_int, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int,
+                         _c_int, _c_int, _c_int, _c_void_p, _c_void_p, _c_void_p],
     "bg_sample": [_c_void_p, _c_int, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p],
     "bg_sample_feed": [_c_void_p, _c_int, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
                        _c_void_p],
@@ -846,6 +862,257 @@ def _attention(q: torch.Tensor, q_stride: int, kv_pool: torch.Tensor, block_tabl
     _check(L.bg_attention_merge(_p(part_o), _p(part_ml), _p(positions), _p(out), _dt(out), out.stride(0), n_rows, nh,
                                 vd, n_splits, split, window, 1 if sink else 0, _p(sink_weight), int(keep), _stream()), "attention_merge")
 
+
+# ------------------------------------------------------------------------------------------------
+# A cache in 4 bits
+PACKED_TILE = 16           # positions of a tile: pages hold whole tiles
+
+
+def packed_page_bytes(hd: int, page_size: int, bounds: bool = False) -> int:
+    """Bytes that a page of `page_size` positions holds of one kv head in 4 bits: codes and, for every position and each group of 64 features of its key
+    and of its value, a (step, lowest) pair; with `bounds` the smallest and largest value of every feature of the page's keys behind them."""
+    if hd not in (64, 128):
+        raise KernelError(f"a cache in 4 bits holds heads of 64 or 128 features, not {hd}")
+    if page_size <= 0 or page_size % PACKED_TILE:
+        raise KernelError(f"pages in 4 bits hold a multiple of {PACKED_TILE} positions, not {page_size}")
+    return page_size * (hd + hd // 64 * 8) + (4 * hd if bounds else 0)
+
+
+def _packed_pool(what: str, pool: torch.Tensor, hd: int, page_size: int, nkv: Optional[int] = None, bounds: bool = False) -> int:
+    """The pool's bytes of a (page, kv head), checked: uint8 [pages, nkv, bytes], with room for bounds or without."""
+    if pool.dtype != torch.uint8 or pool.dim() != 3 or not pool.is_contiguous() or (nkv is not None and pool.shape[1] != nkv):
+        raise KernelError(f"{what}: the pool is {tuple(pool.shape)} of {pool.dtype}, expected contiguous uint8 [pages, {'kv heads' if nkv is None else nkv}, bytes]")
+    plain, more = packed_page_bytes(hd, page_size), packed_page_bytes(hd, page_size, True)
+    if pool.shape[2] != more and (bounds or pool.shape[2] != plain):
+        raise KernelError(f"{what}: a page of {page_size} positions holds {more if bounds else plain} bytes a kv head of {hd} features"
+                          + (" and their bounds" if bounds else f" ({more} with bounds)") + f", not {pool.shape[2]}")
+    return pool.shape[2]
+
+
+def _packed_rows_of(what: str, positions: torch.Tensor, row_req: Optional[torch.Tensor], block_table: torch.Tensor, n_rows: int) -> None:
+    _i32(positions, f"{what}: positions"); _i32(block_table, f"{what}: block_table")
+    if block_table.dim() != 2 or positions.dim() != 1 or positions.numel() < n_rows:
+        raise KernelError(f"{what}: a position for every row, block tables [requests, pages]")
+    if row_req is not None:
+        _i32(row_req, f"{what}: row_req")
+        if row_req.dim() != 1 or row_req.numel() < n_rows:
+            raise KernelError(f"{what}: a request for every row")
+
+
+def packed_append(src: torch.Tensor, q_out: torch.Tensor, nh: int, nkv: int, hd: int, rot: int, interleaved: bool, cos_sin: Optional[torch.Tensor],
+                  positions: torch.Tensor, row_req: torch.Tensor, block_table: torch.Tensor, pool: torch.Tensor, page_size: int,
+                  status: Optional[torch.Tensor]) -> None:
+    """Rows [q | k | v] of `src` ([T, W], or partial sums [parts, T, W]): rotate q into q_out [T, nh*hd], rotate k, and store k and v in 4 bits in the pages of
+    `pool` uint8 [pages, nkv, packed_page_bytes] through the block table [requests, max_pages].  A group of 64 features x is held as lowest = bf16(min x),
+    step = bf16((max x - lowest) / 15) and codes clamp(round((x - lowest) / step), 0, 15), as 64 bits give them; one that holds what is not finite is not a
+    number throughout.  A (request, position) comes once a call."""
+    _here("packed_append", src, q_out, cos_sin, positions, row_req, block_table, pool, status)
+    parts, stride = _parts(src, "packed_append: src")
+    T, width = src.shape[-2], src.shape[-1]
+    block = _packed_pool("packed_append", pool, hd, page_size, nkv)
+    _packed_rows_of("packed_append", positions, row_req, block_table, T)
+    if src.stride(-1) != 1 or width < (nh + 2 * nkv) * hd:
+        raise KernelError(f"packed_append: rows of {width} features cannot hold q, k, v ({(nh + 2 * nkv) * hd})")
+    if q_out.dim() != 2 or q_out.stride(1) != 1 or q_out.shape[1] < nh * hd or q_out.shape[0] < T or (T and q_out.data_ptr() == src.data_ptr()):
+        raise KernelError("packed_append: q_out must be a separate [T, nh*hd] tensor")
+    if not 0 <= rot <= hd or rot % 2:
+        raise KernelError(f"packed_append: {rot} rotated features of {hd}")
+    if rot > 0 and (cos_sin is None or cos_sin.shape[0] < T or tuple(cos_sin.shape[1:]) != (rot // 2, 2) or cos_sin.dtype != torch.float32
+                    or not cos_sin.is_contiguous()):
+        raise KernelError("packed_append: cos_sin must be contiguous float32 [T, rot/2, 2]")
+    if T == 0:
+        return
+    with phase("rope+kv_write"):
+        _check(lib().bg_packed_append(_p(src), _dt(src), src.stride(-2), parts, stride, _p(q_out), _dt(q_out), q_out.stride(0), _p(cos_sin), _p(positions),
+                                      _p(row_req), _p(block_table), block_table.shape[1], block_table.shape[0], _p(pool), block, pool.shape[0], page_size, T,
+                                      nh, nkv, hd, rot, 1 if interleaved else 0, _p(status), _stream()), "packed_append")
+
+
+def packed_bounds(pool: torch.Tensor, positions: torch.Tensor, row_req: torch.Tensor, block_table: torch.Tensor, hd: int, page_size: int,
+                  status: Optional[torch.Tensor]) -> None:
+    """For every row whose position is the last of its page: the smallest and largest value that the page holds of every feature of its keys, written behind
+    the page's codes.  Behind `packed_append` of the same rows; a page that is not full has no bounds."""
+    _here("packed_bounds", pool, positions, row_req, block_table, status)
+    block = _packed_pool("packed_bounds", pool, hd, page_size, bounds=True)
+    T = positions.numel()
+    _packed_rows_of("packed_bounds", positions, row_req, block_table, T)
+    if T == 0:
+        return
+    with phase("rope+kv_write"):
+        _check(lib().bg_packed_bounds(_p(pool), block, pool.shape[0], page_size, _p(positions), _p(row_req), _p(block_table), block_table.shape[1],
+                                      block_table.shape[0], T, pool.shape[1], hd, _p(status), _stream()), "packed_bounds")
+
+
+def packed_rows(pool: torch.Tensor, positions: torch.Tensor, row_req: torch.Tensor, block_table: torch.Tensor, hd: int, page_size: int, out: torch.Tensor,
+                status: Optional[torch.Tensor]) -> None:
+    """The keys and values that the pages hold of rows (request, position): out [T, 2, nkv, hd] float32 or bfloat16."""
+    _here("packed_rows", pool, positions, row_req, block_table, out, status)
+    block = _packed_pool("packed_rows", pool, hd, page_size)
+    T = positions.numel()
+    _packed_rows_of("packed_rows", positions, row_req, block_table, T)
+    if tuple(out.shape) != (T, 2, pool.shape[1], hd) or not out.is_contiguous():
+        raise KernelError(f"packed_rows: out is {tuple(out.shape)}, expected contiguous {(T, 2, pool.shape[1], hd)}")
+    if T == 0:
+        return
+    _check(lib().bg_packed_rows(_p(pool), block, pool.shape[0], page_size, _p(positions), _p(row_req), _p(block_table), block_table.shape[1],
+                                block_table.shape[0], _p(out), _dt(out), T, pool.shape[1], hd, _p(status), _stream()), "packed_rows")
+
+
+# Rows that a request brings from which its pages are written out in bfloat16 for the prompt attention.
+PACKED_LONG_ROWS = 64
+
+
+def _packed_columns(group: int, f32: bool, rows: int) -> Tuple[int, int]:
+    """(columns of a CTA's block, query heads of a block) of the packed attention kernel for blocks of `rows` rows."""
+    each = _c_int(0)
+    n = lib().bg_packed_attention_columns(group, 1 if f32 else 0, rows, ctypes.byref(each))
+    if n < 0:
+        raise KernelError(f"packed_attention: {rows} rows of {group} query heads per kv head")
+    return 8 * n, each.value
+
+
+class PackedPlan:
+    """How attention over pages in 4 bits goes over a step's rows: made by `packed_plan`."""
+
+    def __init__(self, lens, row_start, nh, nkv, hd, dtype, page_size, device, starts):
+        self.sizes, self.n_rows = (nh, nkv, hd, dtype, page_size), sum(lens)
+        group, f32 = nh // nkv, dtype == torch.float32
+        self.rows = max(1, (8 if f32 else 16) // group)        # rows of a block that the packed kernel takes
+        kernel, bq, tile = ("", 1, 0) if f32 else attention_plan(group, hd, torch.bfloat16, False, "auto", lib().bg_packed_wide_page())
+        self.kernel, self.tile, self.bq = kernel, tile, bq
+        long_from = PACKED_LONG_ROWS if kernel == "tc_rows" else 1 << 62
+        short, blocks, longs = [], [], []
+        for i, (r0, n) in enumerate(zip(row_start, lens)):
+            if n >= long_from:
+                blocks += [(len(longs), r0 + f, min(bq, n - f)) for f in range(0, n, bq)]
+                longs.append((i, r0, n))
+            else:
+                short += [(i, r0 + f, min(self.rows, n - f)) for f in range(0, n, self.rows)]
+        self.most = max((s[2] for s in short), default=1)
+        self.n_short, self.n_blocks, self.n_long = len(short), len(blocks), len(longs)
+        self.long_end = None if starts is None else max((starts[i] + n for i, _, n in longs), default=0)
+        flat = torch.tensor([v for rows in (short, blocks, longs) for r in rows for v in r] or [0], dtype=torch.int32)
+        device = torch.device(device)
+        flat = flat.pin_memory().to(device, non_blocking=True) if device.type == "cuda" else flat
+        a, b = 3 * len(short), 3 * (len(short) + len(blocks))
+        self.short, self.blocks, self.longs = flat[:a], flat[a:b], flat[b:b + 3 * len(longs)]
+
+
+def packed_plan(lens, nh: int, nkv: int, hd: int, dtype: torch.dtype, page_size: int, device, row_start=None, starts=None) -> PackedPlan:
+    """The plan of `packed_attention` for a step whose request i brings lens[i] rows, from row row_start[i] on (default: one behind the other).  `starts`: the
+    positions of their first rows, where the host knows them (less room is made then).  Requests of PACKED_LONG_ROWS rows and more (bfloat16) have their pages
+    written out in bfloat16 and run the prompt attention; the others' rows go in blocks of as many (row, query head) pairs as the kernel has columns."""
+    lens = [int(n) for n in lens]
+    if any(n < 0 for n in lens) or nh <= 0 or nkv <= 0 or nh % nkv:
+        raise KernelError(f"packed_plan: rows {lens}, {nh} query heads for {nkv} kv heads")
+    if dtype not in (torch.float32, torch.bfloat16):
+        raise KernelError(f"packed_plan: queries in float32 or bfloat16, got {dtype}")
+    packed_page_bytes(hd, page_size)
+    if row_start is None:
+        row_start = [sum(lens[:i]) for i in range(len(lens))] if len(lens) < 64 else np.concatenate([[0], np.cumsum(lens)[:-1]]).tolist()
+    if len(row_start) != len(lens) or (starts is not None and len(starts) != len(lens)):
+        raise KernelError("packed_plan: a first row and a first position for every request")
+    return PackedPlan(lens, [int(r) for r in row_start], nh, nkv, hd, dtype, page_size, device, starts)
+
+
+def packed_splits(n_streams: int, positions: int, at_once: int) -> int:
+    """How many CTAs share the positions of one (block of rows, kv head): those that make one wave of the `at_once` CTAs that run side by side, three waves where a
+    wave holds less than two of a stream (lengths differ), and none with fewer than 256 positions of the longest stream."""
+    most = -(-positions // 256)
+    want = at_once // n_streams if 2 * n_streams <= at_once else 3 * at_once // n_streams
+    return max(1, min(most, want))
+
+
+def packed_attention(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor, positions: torch.Tensor, nh: int, nkv: int, hd: int, page_size: int,
+                     max_position: int, scale: float, out: torch.Tensor, status: Optional[torch.Tensor], plan: Optional[PackedPlan] = None, window: int = 0,
+                     softcap: float = 0.0, sink: bool = False, sink_weight: Optional[torch.Tensor] = None, pages: Optional[torch.Tensor] = None) -> None:
+    """Grouped-query attention of rows q [T, nh*hd] over pages in 4 bits; out [T, nh*hd].  Without a plan row i is the one row of request i; with one
+    (`packed_plan`) the requests bring what it was made for.  `max_position` bounds the rows' positions.  `window` w > 0: a query sees itself and the w - 1
+    positions before it.  `softcap`, `sink` and `sink_weight` as `attention` has them.  `pages` int32 [T, nkv, n] (single tokens): the pages, by their index in
+    the row's block table, that a row reads for a kv head, each once, -1 behind them (`packed_select` makes such lists)."""
+    _here("packed_attention", q, pool, block_table, positions, out, status, sink_weight, pages, None if plan is None else plan.short)
+    block = _packed_pool("packed_attention", pool, hd, page_size, nkv)
+    T = q.shape[0]
+    _packed_rows_of("packed_attention", positions, None, block_table, T)
+    if q.dim() != 2 or q.stride(1) != 1 or q.shape[1] < nh * hd or out.dim() != 2 or out.stride(1) != 1 or out.shape[1] < nh * hd or out.shape[0] < T:
+        raise KernelError("packed_attention: q and out are [T, nh*hd] with unit inner stride")
+    if q.dtype != out.dtype or _dt(q) < 0:
+        raise KernelError(f"packed_attention: queries of {q.dtype} and results of {out.dtype}")
+    if nkv <= 0 or nh % nkv:
+        raise KernelError(f"packed_attention: {nh} query heads for {nkv} kv heads")
+    if window < 0 or softcap < 0.0:
+        raise KernelError("packed_attention: a sliding window or none, a positive bound of the scores or none")
+    if sink_weight is not None:
+        sink = True
+        if sink_weight.dtype != torch.float32 or sink_weight.numel() != nh or not sink_weight.is_contiguous():
+            raise KernelError("packed_attention: the sink's scores are contiguous float32, one per query head")
+    if plan is not None and (plan.sizes != (nh, nkv, hd, q.dtype, page_size) or plan.n_rows != T):
+        raise KernelError("packed_attention: the plan is for other sizes")
+    if plan is None and block_table.shape[0] < T:
+        raise KernelError(f"packed_attention: {T} rows without a plan need a block table each, there are {block_table.shape[0]}")
+    top = 0
+    if pages is not None:
+        _i32(pages, "packed_attention: pages")
+        if plan is not None or window or pages.dim() != 3 or tuple(pages.shape[:2]) != (T, nkv) or pages.shape[2] < 1:
+            raise KernelError(f"packed_attention: pages [{T}, {nkv}, n] for single tokens without a window")
+        top = pages.shape[2]
+    if T == 0:
+        return
+    L, f32 = lib(), q.dtype == torch.float32
+    with phase("attn"):
+        n, most = (T, 1) if plan is None else (plan.n_short, plan.most)
+        if n:
+            cols, each = _packed_columns(nh // nkv, f32, most)
+            streams = nkv * -(-(nh // nkv) // each)
+            read = min(max_position + 1, top * page_size if top else max_position + 1, window + most if window else max_position + 1)
+            splits = packed_splits(n * streams, read, sm_count() * (2 if cols == 8 and not f32 else 1))
+            part_o = part_ml = None
+            if splits > 1:
+                part_o = torch.empty((n * streams * splits * cols, hd), dtype=torch.float32, device=q.device)
+                part_ml = torch.empty((n * streams * splits * cols, 2), dtype=torch.float32, device=q.device)
+            _check(L.bg_packed_attention(_p(q), _dt(q), q.stride(0), _p(pool), block, pool.shape[0], page_size, _p(block_table), block_table.shape[1],
+                                         block_table.shape[0], _p(positions), None if plan is None else _p(plan.short), n, most, _p(pages), top, _p(part_o),
+                                         _p(part_ml), splits, nh, nkv, hd, window, float(scale), float(softcap), _p(sink_weight), 1 if sink else 0, _p(out),
+                                         out.stride(0), _p(status), _stream()), "packed_attention")
+            count_launches(1 if splits > 1 else 0)
+        if plan is not None and plan.n_long:
+            end = max_position + 1 if plan.long_end is None else min(plan.long_end, max_position + 1)
+            size = L.bg_packed_wide_page()
+            n_pages = max(1, -(-end // size))
+            wide = torch.empty((plan.n_long * n_pages, 2, nkv, size, hd), dtype=torch.bfloat16, device=q.device)
+            table = torch.empty((plan.n_long, n_pages), dtype=torch.int32, device=q.device)
+            _check(L.bg_packed_unpack(_p(pool), block, pool.shape[0], page_size, _p(positions), _p(block_table), block_table.shape[1],
+                                      block_table.shape[0], _p(plan.longs), plan.n_long, _p(wide), _p(table), n_pages, window, nkv, hd, _p(status), _stream()), "packed_unpack")
+            _attention(q, q.stride(0), wide, table, positions, plan.blocks, plan.n_blocks, end - 1, T, nh, nkv, hd, window, 256, plan.tile, plan.bq, scale, out,
+                       status, plan.kernel, sink=sink, sink_weight=sink_weight, softcap=softcap)
+
+
+def packed_select(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor, positions: torch.Tensor, nh: int, nkv: int, hd: int, page_size: int,
+                  max_position: int, out: torch.Tensor, status: Optional[torch.Tensor], first: int = 1, recent: int = 1) -> None:
+    """out int32 [T, nkv, n]: the n pages (by their index in the block table, ascending, -1 behind them) that row i, the one row of request i, reads for each kv
+    head.  All where a request has no more than n; else the `first` first ones, the `recent` last ones (the newest among them) and those of the others whose keys
+    can score highest, by their bounds (`packed_bounds`): the score of a page is the largest, over the query heads of the kv head, of
+    sum of max(q lo, q hi), summed in 64 bits and rounded to 32 (one that is no number is the largest); of equal ones the lower page."""
+    _here("packed_select", q, pool, block_table, positions, out, status)
+    block = _packed_pool("packed_select", pool, hd, page_size, nkv, bounds=True)
+    T = q.shape[0]
+    _packed_rows_of("packed_select", positions, None, block_table, T)
+    _i32(out, "packed_select: out")
+    if q.dim() != 2 or q.stride(1) != 1 or q.shape[1] < nh * hd or nkv <= 0 or nh % nkv:
+        raise KernelError("packed_select: q is [T, nh*hd] with unit inner stride, whole groups of query heads to a kv head")
+    if block_table.shape[0] < T or out.dim() != 3 or tuple(out.shape[:2]) != (T, nkv) or out.shape[2] < 1:
+        raise KernelError(f"packed_select: out [{T}, {nkv}, n], a block table for every row")
+    if first < 0 or recent < 1 or first + recent > out.shape[2]:
+        raise KernelError(f"packed_select: {first} first and {recent} last pages (the newest at least) of {out.shape[2]}")
+    n_pages = max_position // page_size + 1
+    if n_pages > lib().bg_packed_select_most():
+        raise KernelError(f"packed_select: {n_pages} pages, at most {lib().bg_packed_select_most()}")
+    if T == 0:
+        return
+    with phase("attn"):
+        _check(lib().bg_packed_select(_p(q), _dt(q), q.stride(0), _p(pool), block, pool.shape[0], page_size, _p(block_table), block_table.shape[1],
+                                      _p(positions), T, nh, nkv, hd, out.shape[2], first, recent, max(1, n_pages), _p(out), _p(status), _stream()),
+               "packed_select")
 
 # ------------------------------------------------------------------------------------------------
 # Attention of single tokens whose requests share their first positions

@@ -1,0 +1,401 @@
+// Writing and reading pages that hold keys and values in 4 bits (packed.cuh says how): the append of a step's rows with the rotation of queries and keys on
+// the way, rows read back, the smallest and largest values of a filled page's keys, and pages written out in bfloat16 for the prompt attention.
+//
+// A group of 64 features x becomes  lowest = bf16(min x),  step = bf16((max x - lowest) / 15),  u = clamp(round((x - lowest) / step), 0, 15).  The pair is
+// rounded before the codes are made, so that they are the nearest ones to what is read back: a value is off by half a step, and where rounding the pair cut
+// the range (by a part in 512) by that.  x is the rotated key in float, never rounded to bfloat16.  A group with a value that is not finite, or whose range is
+// not, is not a number throughout, as attention over it would be.  No result hangs on which thread wrote first: a position has one writer.
+#include "packed.cuh"
+
+namespace bg {
+
+// ------------------------------------------------------------------------------------------------ append
+struct PkAppend {
+    const void* src; long long src_stride, part_stride; int parts;
+    void* q_out; long long q_stride;
+    const float* cos_sin;
+    const int* positions; const int* row_req; const int* block_table;
+    unsigned char* pool; long long block_bytes;
+    int max_pages, num_pages, page_size, T, n_req, nh, nkv, rot, interleaved;
+    unsigned* status;
+};
+
+// Four neighbouring features of a row (summed over partial results).
+template <typename T>
+__device__ __forceinline__ void load4_parts(const T* p, int parts, long long stride, float (&v)[4]);
+template <>
+__device__ __forceinline__ void load4_parts<float>(const float* p, int parts, long long stride, float (&v)[4]) {
+    float4 a = *reinterpret_cast<const float4*>(p);
+    for (int i = 1; i < parts; ++i) {
+        const float4 b = *reinterpret_cast<const float4*>(p + i * stride);
+        a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
+    }
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+}
+template <>
+__device__ __forceinline__ void load4_parts<__nv_bfloat16>(const __nv_bfloat16* p, int parts, long long stride, float (&v)[4]) {
+    v[0] = v[1] = v[2] = v[3] = 0.0f;
+    for (int i = 0; i < parts; ++i) {
+        const uint2 r = *reinterpret_cast<const uint2*>(p + i * stride);
+        const float w[4] = {__uint_as_float(r.x << 16), __uint_as_float(r.x & 0xffff0000u), __uint_as_float(r.y << 16), __uint_as_float(r.y & 0xffff0000u)};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = i ? v[j] + w[j] : w[j];
+    }
+}
+__device__ __forceinline__ void store4(float* p, const float (&v)[4]) { *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]); }
+__device__ __forceinline__ void store4(__nv_bfloat16* p, const float (&v)[4]) {
+    uint2 r;
+    __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&r);
+    h[0] = __floats2bfloat162_rn(v[0], v[1]); h[1] = __floats2bfloat162_rn(v[2], v[3]);
+    *reinterpret_cast<uint2*>(p) = r;
+}
+
+// HD / 4 lanes take a head of a row, a lane four neighbouring features; a group's 16 lanes find its smallest and largest by shuffles, and two lanes' codes make
+// a word.  One row and a few heads a CTA: the rows of a decoding step are spread over the SMs.
+// The codes are those that 64 bits give: everything is done in 32 first, with a bound on how far off that may be, and where the bound reaches the border of
+// two codes, or of two roundings of the pair, the warp does its heads again in 64 (two or three warps of a thousand).
+constexpr int PK_THREADS = 256;
+template <typename TS, typename TQ, int HD>
+__global__ void __launch_bounds__(PK_THREADS) packed_append_kernel(const PkAppend p) {
+    constexpr int LANES = HD / 4, EACH = PK_THREADS / LANES;
+    pdl_launch();
+    const int head = blockIdx.y * EACH + threadIdx.x / LANES, l = threadIdx.x % LANES, f = l * 4;
+    const int heads = p.nh + 2 * p.nkv;
+    const bool idle = head >= heads;                   // (stays for the shuffles)
+    const int t = blockIdx.x, h = idle ? 0 : head;
+    const TS* row = reinterpret_cast<const TS*>(p.src) + (size_t)t * p.src_stride + (size_t)h * HD;
+    pdl_wait();
+    float x[4], far[4] = {}, cs[4], sn[4];             // far: |x cos| + |its partner sin|, where the feature is rotated
+    float y[4] = {};                                   // its partner
+    load4_parts<TS>(row + f, p.parts, p.part_stride, x);
+    const bool turned = h < p.nh + p.nkv && f < p.rot;
+    const int half = p.rot / 2;
+    if (turned) {
+        const float2* table = reinterpret_cast<const float2*>(p.cos_sin) + (size_t)t * half;
+        if (!p.interleaved) {
+            if (half % 4 == 0) {
+                load4_parts<TS>(row + (f < half ? f + half : f - half), p.parts, p.part_stride, y);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int at = f + j;
+                    y[j] = at < p.rot ? sum_parts(row + (at < half ? at + half : at - half), p.parts, (size_t)p.part_stride) : 0.0f;
+                }
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) y[j] = x[j ^ 1];
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int at = f + j;
+            if (at < p.rot) {
+                const float2 c = table[p.interleaved ? at / 2 : at < half ? at : at - half];
+                cs[j] = c.x;
+                sn[j] = (p.interleaved ? at % 2 == 0 : at < half) ? -c.y : c.y;      // (a cos - b sin, and b cos + a sin for the partner)
+            } else {
+                cs[j] = 1.0f; sn[j] = 0.0f;
+            }
+        }
+    }
+    float r[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        r[j] = turned && f + j < p.rot ? __fadd_rn(__fmul_rn(x[j], cs[j]), __fmul_rn(y[j], sn[j])) : x[j];
+        if (turned) far[j] = fabsf(x[j] * cs[j]) + fabsf(y[j] * sn[j]);
+    }
+    if (h < p.nh) {
+        if (!idle) store4(reinterpret_cast<TQ*>(p.q_out) + (size_t)t * p.q_stride + (size_t)h * HD + f, r);
+    }
+    if (__all_sync(0xffffffffu, idle || h < p.nh)) return;
+    float lo = fminf(fminf(r[0], r[1]), fminf(r[2], r[3])), hi = fmaxf(fmaxf(r[0], r[1]), fmaxf(r[2], r[3]));
+    float off = fmaxf(fmaxf(far[0], far[1]), fmaxf(far[2], far[3]));
+    const float nought = __fmul_rn(0.0f, r[0]) + __fmul_rn(0.0f, r[1]) + __fmul_rn(0.0f, r[2]) + __fmul_rn(0.0f, r[3]);
+    int sound = nought == 0.0f;                        // (nought times what is not finite is no number)
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) {
+        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        off = fmaxf(off, __shfl_xor_sync(0xffffffffu, off, o));
+        sound &= __shfl_xor_sync(0xffffffffu, sound, o);
+    }
+    off *= 1.5e-7f;                                    // a rotated feature's error: 2^-24 of each product and of their sum
+    __nv_bfloat16 lowest = __float2bfloat16_rn(lo);
+    float base = __bfloat162float(lowest);
+    const float span = __fmul_rn(__fsub_rn(hi, base), 1.0f / 15.0f), span_off = fmaf(3e-7f, fabsf(span), 0.1f * off);
+    sound &= fabsf(span) < INFINITY && fabsf(base) < INFINITY;
+    __nv_bfloat16 step = __float2bfloat16_rn(span);
+    float s = __bfloat162float(step);
+    float by = s > 0.0f ? s : 1.0f;                    // (a group of one value: every code 0)
+    int near = __bfloat16_as_ushort(__float2bfloat16_rn(lo - off)) != __bfloat16_as_ushort(__float2bfloat16_rn(lo + off))
+            || __bfloat16_as_ushort(__float2bfloat16_rn(span - span_off)) != __bfloat16_as_ushort(__float2bfloat16_rn(span + span_off));
+    float u[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float d = __fsub_rn(r[j], base), v = __fdiv_rn(d, by);
+        u[j] = rintf(v);
+        // bfloat16 as it came, and a difference without rounding: then the quotient is a border only if it is one in 64 bits too
+        const bool sure = sizeof(TS) == 2 && p.parts == 1 && !turned && __fadd_rn(d, base) == r[j] && __fsub_rn(r[j], d) == base;
+        near |= !sure && fabsf(fabsf(v - u[j]) - 0.5f) <= off / by + 3e-6f && v > -1.0f && v < 16.0f;
+    }
+    if (__any_sync(0xffffffffu, near && sound && !idle && h >= p.nh)) {
+        double w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = turned && f + j < p.rot ? (double)x[j] * cs[j] + (double)y[j] * sn[j] : (double)x[j];
+        double least64 = fmin(fmin(w[0], w[1]), fmin(w[2], w[3])), most64 = fmax(fmax(w[0], w[1]), fmax(w[2], w[3]));
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) {
+            least64 = fmin(least64, __shfl_xor_sync(0xffffffffu, least64, o));
+            most64 = fmax(most64, __shfl_xor_sync(0xffffffffu, most64, o));
+        }
+        lowest = __float2bfloat16_rn((float)least64);
+        base = __bfloat162float(lowest);
+        step = __float2bfloat16_rn((float)((most64 - (double)base) / 15.0));
+        s = __bfloat162float(step);
+        by = s > 0.0f ? s : 1.0f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) u[j] = (float)rint((w[j] - (double)base) / (double)by);
+    }
+    unsigned word = 0;
+    const bool key = h < p.nh + p.nkv;
+    const int odd = l & 1;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int e = odd * 4 + j;
+        word |= (unsigned)fminf(fmaxf(u[j], 0.0f), 15.0f) << (4 * (key ? e / 2 + 4 * (e % 2) : e));
+    }
+    if (!sound) {
+        lowest = step = __float2bfloat16_rn(__int_as_float(0x7fffffff));
+        word = 0;
+    }
+    word |= __shfl_xor_sync(0xffffffffu, word, 1);
+    if (idle || h < p.nh) return;
+    const int pos = p.positions[t], req = p.row_req[t], index = pos / p.page_size;
+    const int page = pos >= 0 && req >= 0 && req < p.n_req && index < p.max_pages ? p.block_table[(size_t)req * p.max_pages + index] : -1;
+    if (page < 0 || page >= p.num_pages) {
+        if (p.status && l == 0) atomicOr(p.status, BG_STATUS_BAD_PAGE);
+        return;
+    }
+    const int at = pos % p.page_size, slot = at % PK_TILE, kvh = (h - p.nh) % p.nkv;
+    unsigned char* tile = p.pool + ((size_t)page * p.nkv + kvh) * p.block_bytes + (size_t)(at / PK_TILE) * Packed<HD>::TILE;
+    if (!odd) *reinterpret_cast<unsigned*>(tile + (key ? Packed<HD>::key_word(slot, f) : Packed<HD>::value_word(slot, f))) = word;
+    if (l % 16 == 0) {
+        const unsigned pair = (unsigned)__bfloat16_as_ushort(step) | (unsigned)__bfloat16_as_ushort(lowest) << 16;
+        *reinterpret_cast<unsigned*>(tile + Packed<HD>::pair_word(slot, key ? 0 : 1, l / 16)) = pair;
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ rows read back
+struct PkRead {
+    const unsigned char* pool; long long block_bytes;
+    const int* positions; const int* row_req; const int* block_table;
+    void* out;
+    int max_pages, num_pages, page_size, n_req, nkv;
+    unsigned* status;
+};
+
+// out[t, keys and values, kv head, feature]: a thread reads a word of codes and writes its 8 values.
+template <typename TO, int HD>
+__global__ void __launch_bounds__(PK_THREADS) packed_rows_kernel(const PkRead p) {
+    constexpr int WORDS = HD / 8;
+    pdl_launch();
+    const int per_row = 2 * p.nkv * WORDS, i = blockIdx.y * PK_THREADS + threadIdx.x, t = blockIdx.x;
+    if (i >= per_row) return;
+    const int value = i / (p.nkv * WORDS), kvh = i / WORDS % p.nkv, f = i % WORDS * 8;
+    pdl_wait();
+    const int pos = p.positions[t], req = p.row_req[t], index = pos / p.page_size;
+    const int page = pos >= 0 && req >= 0 && req < p.n_req && index < p.max_pages ? p.block_table[(size_t)req * p.max_pages + index] : -1;
+    TO* out = reinterpret_cast<TO*>(p.out) + ((size_t)t * 2 * p.nkv + (size_t)value * p.nkv + kvh) * HD + f;
+    float v[8] = {};
+    if (page < 0 || page >= p.num_pages) {
+        if (p.status) atomicOr(p.status, BG_STATUS_BAD_PAGE);
+    } else {
+        const int at = pos % p.page_size, slot = at % PK_TILE;
+        const unsigned char* tile = p.pool + ((size_t)page * p.nkv + kvh) * p.block_bytes + (size_t)(at / PK_TILE) * Packed<HD>::TILE;
+        const unsigned pair = *reinterpret_cast<const unsigned*>(tile + Packed<HD>::pair_word(slot, value, f / PK_GROUP));
+        const unsigned word = *reinterpret_cast<const unsigned*>(tile + (value ? Packed<HD>::value_word(slot, f) : Packed<HD>::key_word(slot, f)));
+        if (value) packed_values<false>(word, pair, v);
+        else packed_values<true>(word, pair, v);
+    }
+    store8(out, v);
+}
+
+// ------------------------------------------------------------------------------------------------ bounds of filled pages
+struct PkBounds {
+    unsigned char* pool; long long block_bytes;
+    const int* positions; const int* row_req; const int* block_table;
+    int max_pages, num_pages, page_size, n_req, nkv;
+    unsigned* status;
+};
+
+// A row that fills its page (its position is the page's last) has the CTA of its (row, kv head) find the smallest and largest value of every feature of the
+// page's keys, as they are read back.  What a page's bounds are hangs on the page alone, whoever wrote it and in how many steps.  A thread takes a word of 8
+// features of every (PK_THREADS / words)-th position; a value that is no number stays one.
+__device__ __forceinline__ float least(float a, float b) { return a < b || a != a ? a : b; }
+__device__ __forceinline__ float most(float a, float b) { return a > b || a != a ? a : b; }
+template <int HD>
+__global__ void __launch_bounds__(PK_THREADS) packed_bounds_kernel(const PkBounds p) {
+    constexpr int WORDS = HD / 8, AT_ONCE = PK_THREADS / WORDS;
+    __shared__ float ends[2][AT_ONCE][HD + 1];
+    pdl_launch();
+    const int t = blockIdx.x, kvh = blockIdx.y;
+    pdl_wait();
+    const int pos = p.positions[t];
+    if (pos < 0 || pos % p.page_size != p.page_size - 1) return;
+    const int req = p.row_req[t], index = pos / p.page_size;
+    const int page = req >= 0 && req < p.n_req && index < p.max_pages ? p.block_table[(size_t)req * p.max_pages + index] : -1;
+    if (page < 0 || page >= p.num_pages) {
+        if (p.status && threadIdx.x == 0) atomicOr(p.status, BG_STATUS_BAD_PAGE);
+        return;
+    }
+    unsigned char* block = p.pool + ((size_t)page * p.nkv + kvh) * p.block_bytes;
+    const int w = threadIdx.x % WORDS, first = threadIdx.x / WORDS, f = w * 8;
+    float lo[8], hi[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) { lo[e] = INFINITY; hi[e] = -INFINITY; }
+    for (int at = first; at < p.page_size; at += AT_ONCE) {
+        const unsigned char* tile = block + (size_t)(at / PK_TILE) * Packed<HD>::TILE;
+        float v[8];
+        packed_values<true>(*reinterpret_cast<const unsigned*>(tile + Packed<HD>::key_word(at % PK_TILE, f)),
+                            *reinterpret_cast<const unsigned*>(tile + Packed<HD>::pair_word(at % PK_TILE, 0, f / PK_GROUP)), v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) { lo[e] = least(v[e], lo[e]); hi[e] = most(v[e], hi[e]); }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) { ends[0][first][f + e] = lo[e]; ends[1][first][f + e] = hi[e]; }
+    __syncthreads();
+    __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(block + (size_t)(p.page_size / PK_TILE) * Packed<HD>::TILE);
+    for (int i = threadIdx.x; i < 2 * HD; i += PK_THREADS) {
+        const int end = i / HD, feature = i % HD;
+        float v = ends[end][0][feature];
+        for (int j = 1; j < AT_ONCE; ++j) v = end ? most(ends[1][j][feature], v) : least(ends[0][j][feature], v);
+        out[i] = __float2bfloat16_rn(v);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ pages in bfloat16
+struct PkUnpack {
+    const unsigned char* pool; long long block_bytes;
+    const int* positions; const int* block_table;
+    const int* longs;                  // [n][3]: request, first row, rows
+    __nv_bfloat16* out;                // [n * pages, 2, nkv, PK_WIDE, HD]
+    int* table;                        // [n, pages]: their block table
+    int max_pages, num_pages, page_size, n_req, nkv, pages, window;
+    unsigned* status;
+};
+
+// The positions that a request's rows read, written out as the bfloat16 cache holds them, in pages of PK_WIDE whatever the packed ones hold: page i of the n-th
+// request at n * pages + i.  A CTA takes a tile of 16 positions of one kv head; bound by the bytes written (heads of 128: 144 bytes read and 512 written a
+// position and kv head).  Positions behind the request's last are written as noughts: nobody reads them, and no number from nowhere stands there.
+constexpr int PK_WIDE = 64;
+template <int HD>
+__global__ void __launch_bounds__(PK_THREADS) packed_unpack_kernel(const PkUnpack p) {
+    constexpr int WORDS = HD / 8, PER = 2 * PK_TILE * WORDS;
+    pdl_launch();
+    const int n = blockIdx.z, kvh = blockIdx.y, pos0 = blockIdx.x * PK_TILE, wide = pos0 / PK_WIDE;
+    pdl_wait();
+    if (pos0 % PK_WIDE == 0 && kvh == 0 && threadIdx.x == 0) p.table[(size_t)n * p.pages + wide] = n * p.pages + wide;
+    const int req = p.longs[3 * n], row0 = p.longs[3 * n + 1], rows = p.longs[3 * n + 2];
+    const int last = p.positions[row0 + rows - 1], lo = first_visible(p.positions[row0], p.window);
+    if (wide > last / PK_WIDE || wide < lo / PK_WIDE) return;
+    const int index = pos0 / p.page_size;
+    const bool read = pos0 <= last && pos0 + PK_TILE > lo;         // (what lies in front of a window may have been given back)
+    const int page = read && index < p.max_pages && req >= 0 && req < p.n_req ? p.block_table[(size_t)req * p.max_pages + index] : -1;
+    const bool bad = page < 0 || page >= p.num_pages;
+    if (read && bad && p.status && threadIdx.x == 0) atomicOr(p.status, BG_STATUS_BAD_PAGE);
+    const unsigned char* from = p.pool + ((size_t)(bad ? 0 : page) * p.nkv + kvh) * p.block_bytes + (size_t)(pos0 % p.page_size / PK_TILE) * Packed<HD>::TILE;
+    __nv_bfloat16* to = p.out + (((size_t)n * p.pages + wide) * 2 * p.nkv + kvh) * PK_WIDE * HD + (size_t)(pos0 % PK_WIDE) * HD;
+#pragma unroll
+    for (int i0 = 0; i0 < PER; i0 += PK_THREADS) {
+        const int i = i0 + threadIdx.x;
+        const int value = i / (PK_TILE * WORDS), slot = i / WORDS % PK_TILE, f = i % WORDS * 8;
+        float v[8] = {};
+        if (!bad && pos0 + slot <= last) {
+            const unsigned pair = *reinterpret_cast<const unsigned*>(from + Packed<HD>::pair_word(slot, value, f / PK_GROUP));
+            const unsigned word = *reinterpret_cast<const unsigned*>(from + (value ? Packed<HD>::value_word(slot, f) : Packed<HD>::key_word(slot, f)));
+            if (value) packed_values<false>(word, pair, v);
+            else packed_values<true>(word, pair, v);
+        }
+        store8(to + (size_t)value * p.nkv * PK_WIDE * HD + (size_t)slot * HD + f, v);
+    }
+}
+
+static int packed_shape(int hd, int page_size, int nkv, int num_pages, long long block_bytes, bool bounds) {
+    if (hd != 64 && hd != 128) return BG_ERR_UNSUPPORTED;
+    if (page_size <= 0 || page_size % PK_TILE || nkv <= 0 || nkv > 65535 || num_pages <= 0) return BG_ERR_SHAPE;
+    if (block_bytes % 16 || block_bytes < page_size / PK_TILE * packed_tile_bytes(hd) + (bounds ? 4 * hd : 0)) return BG_ERR_SHAPE;
+    return BG_OK;
+}
+
+template <typename TS, typename TQ, int HD>
+static int append_launch(const PkAppend& p, cudaStream_t stream) {
+    const int each = PK_THREADS / (HD / 4), heads = p.nh + 2 * p.nkv;
+    cudaError_t e = launch(packed_append_kernel<TS, TQ, HD>, dim3(p.T, (heads + each - 1) / each), dim3(PK_THREADS), 0, stream, p);
+    return e == cudaSuccess ? BG_OK : (int)e;
+}
+
+}  // namespace bg
+
+using namespace bg;
+
+// Bytes of a tile of 16 positions of one kv head, or a negative code.
+extern "C" int bg_packed_tile_bytes(int hd) { return hd == 64 || hd == 128 ? (int)packed_tile_bytes(hd) : BG_ERR_UNSUPPORTED; }
+
+extern "C" int bg_packed_append(const void* src, int src_dtype, long long src_stride, int parts, long long part_stride, void* q_out, int q_dtype,
+                                long long q_stride, const float* cos_sin, const int* positions, const int* row_req, const int* block_table, int max_pages,
+                                int n_req, unsigned char* pool, long long block_bytes, int num_pages, int page_size, int T, int nh, int nkv, int hd, int rot,
+                                int interleaved, unsigned* status, cudaStream_t stream) {
+    if (int e = packed_shape(hd, page_size, nkv, num_pages, block_bytes, false)) return e;
+    if (T <= 0) return BG_OK;
+    if (parts < 1 || nh <= 0 || rot < 0 || rot > hd || rot % 2 || max_pages <= 0 || (rot && !cos_sin)) return BG_ERR_SHAPE;
+    const long long fine = src_dtype == BG_DTYPE_F32 ? 15 : 7, fine_q = q_dtype == BG_DTYPE_F32 ? 15 : 7;
+    const long long size = src_dtype == BG_DTYPE_F32 ? 4 : 2, size_q = q_dtype == BG_DTYPE_F32 ? 4 : 2;
+    if (((long long)(uintptr_t)src | src_stride * size | (parts > 1 ? part_stride * size : 0)) & fine || ((long long)(uintptr_t)q_out | q_stride * size_q) & fine_q
+        || (uintptr_t)pool % 16 || (uintptr_t)cos_sin % 8) return BG_ERR_ALIGN;
+    const PkAppend p = {src, src_stride, part_stride, parts, q_out, q_stride, cos_sin, positions, row_req, block_table, pool, block_bytes,
+                        max_pages, num_pages, page_size, T, n_req, nh, nkv, rot, interleaved, status};
+    BG_DISPATCH_DTYPE(src_dtype, TS, BG_DISPATCH_DTYPE(q_dtype, TQ, return hd == 64 ? (append_launch<TS, TQ, 64>(p, stream)) : (append_launch<TS, TQ, 128>(p, stream))));
+}
+
+extern "C" int bg_packed_rows(const unsigned char* pool, long long block_bytes, int num_pages, int page_size, const int* positions, const int* row_req,
+                              const int* block_table, int max_pages, int n_req, void* out, int out_dtype, int T, int nkv, int hd, unsigned* status,
+                              cudaStream_t stream) {
+    if (int e = packed_shape(hd, page_size, nkv, num_pages, block_bytes, false)) return e;
+    if (T <= 0) return BG_OK;
+    if ((uintptr_t)pool % 16 || (uintptr_t)out % 16) return BG_ERR_ALIGN;
+    const PkRead p = {pool, block_bytes, positions, row_req, block_table, out, max_pages, num_pages, page_size, n_req, nkv, status};
+    const dim3 grid(T, (2 * nkv * hd / 8 + PK_THREADS - 1) / PK_THREADS);
+    cudaError_t e = cudaSuccess;
+    BG_DISPATCH_DTYPE(out_dtype, TO, e = hd == 64 ? launch(packed_rows_kernel<TO, 64>, grid, dim3(PK_THREADS), 0, stream, p)
+                                                  : launch(packed_rows_kernel<TO, 128>, grid, dim3(PK_THREADS), 0, stream, p));
+    return e == cudaSuccess ? BG_OK : (int)e;
+}
+
+extern "C" int bg_packed_bounds(unsigned char* pool, long long block_bytes, int num_pages, int page_size, const int* positions, const int* row_req,
+                                const int* block_table, int max_pages, int n_req, int T, int nkv, int hd, unsigned* status, cudaStream_t stream) {
+    if (int e = packed_shape(hd, page_size, nkv, num_pages, block_bytes, true)) return e;
+    if (T <= 0) return BG_OK;
+    if ((uintptr_t)pool % 16) return BG_ERR_ALIGN;
+    const PkBounds p = {pool, block_bytes, positions, row_req, block_table, max_pages, num_pages, page_size, n_req, nkv, status};
+    cudaError_t e = hd == 64 ? launch(packed_bounds_kernel<64>, dim3(T, nkv), dim3(PK_THREADS), 0, stream, p)
+                             : launch(packed_bounds_kernel<128>, dim3(T, nkv), dim3(PK_THREADS), 0, stream, p);
+    return e == cudaSuccess ? BG_OK : (int)e;
+}
+
+// Positions of a page that bg_packed_unpack writes.
+extern "C" int bg_packed_wide_page() { return PK_WIDE; }
+
+extern "C" int bg_packed_unpack(const unsigned char* pool, long long block_bytes, int num_pages, int page_size, const int* positions, const int* block_table,
+                                int max_pages, int n_req, const int* longs, int n, void* out, int* table, int pages, int window, int nkv, int hd,
+                                unsigned* status, cudaStream_t stream) {
+    if (int e = packed_shape(hd, page_size, nkv, num_pages, block_bytes, false)) return e;
+    if (n <= 0 || pages <= 0) return BG_OK;
+    if (n > 65535 || (long long)n * pages > 0x7fffffffLL || pages > 0x7fffffff / PK_WIDE) return BG_ERR_SHAPE;
+    if ((uintptr_t)pool % 16 || (uintptr_t)out % 16) return BG_ERR_ALIGN;
+    const PkUnpack p = {pool, block_bytes, positions, block_table, longs, (__nv_bfloat16*)out, table, max_pages, num_pages, page_size, n_req, nkv, pages,
+                        window, status};
+    const dim3 grid(pages * (PK_WIDE / PK_TILE), nkv, n);
+    cudaError_t e = hd == 64 ? launch(packed_unpack_kernel<64>, grid, dim3(PK_THREADS), 0, stream, p)
+                             : launch(packed_unpack_kernel<128>, grid, dim3(PK_THREADS), 0, stream, p);
+    return e == cudaSuccess ? BG_OK : (int)e;
+}

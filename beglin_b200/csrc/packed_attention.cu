@@ -1,0 +1,624 @@
+// Attention over pages that hold keys and values in 4 bits (packed.cuh), for single tokens and short runs of rows: softmax(q K^T scale) V with
+// K = lowest + step u, never written out.
+//
+// Both products run as mma.sync m16n8k16 with the CODES as the left operand: a code u becomes the bfloat16 128 + u by two bit operations (0x4300 | u), which
+// is exact, and (step, lowest) are applied in float outside the product:
+//     q . k   = sum over groups of  step (sum q (128 + u)) + (lowest - 128 step) (sum q)
+//     p V     = sum over positions of  (p step) (128 + u) - 128 (p step) + p lowest
+// so that the only rounding of the cache's side is that of p step to bfloat16 (-128 (p step) is a product with a constant left operand, of the same rounded
+// numbers).  Keys: 16 positions by 16 features times features by 8 columns; values: 16 features by 16 positions times positions by columns.  A column is one
+// (row, query head): the queries of a kv head are the narrow side, so 8 heads waste nothing of the product and a code is unpacked once for all of them.  The
+// weights reach the second product's layout through movmatrix.  With float queries the codes are made exact (u), and queries and weights go in three bfloat16 parts.
+//
+// Why this shape: at the bandwidth of HBM a position of a kv head (144 bytes for heads of 128) has to be done in some 6 cycles of an SM, 25 warp instructions.  The
+// left operand by codes takes about 15 for 8 columns; with the queries on the left (16 rows, half of them empty) it took the tensor cores twice the products
+// and the softmax twice the numbers.  A warp has a ring of its own (STAGES chunks of 16 or 32 positions, one bulk copy each) and its own running maximum, sum
+// and result, so that nothing in the loop waits for another warp; the warps' results meet at the end, those of a long request's ranges in packed_merge_kernel.
+#include <type_traits>
+
+#include "packed.cuh"
+
+namespace bg {
+
+constexpr int PA_WARPS = 8, PA_THREADS = PA_WARPS * 32, PA_STAGES = 3;
+constexpr float PA_LOG2E = 1.4426950408889634f;
+
+struct PaParams {
+    const void* q; long long q_stride;
+    const unsigned char* pool; long long block_bytes;
+    const int* table; const int* positions;
+    const int* blocks;                 // [n][3]: request, first row, rows; null: block i is row i of request i
+    const int* list;                   // [rows][nkv][top] page indexes to read (less than 0: none), or null: all
+    int num_pages, page_size, max_pages, top, n_req;
+    int nkv, group, head_blocks, heads_each;       // query heads of a kv head, the blocks that they are cut into, heads of a block
+    int window, splits;
+    float scale_log2, cap_log2, scale_over_cap;
+    float* part_o; float* part_ml;     // [block][kv head and head block][split][column][HD], [..][2]; null: finished rows go to `out`
+    void* out; long long out_stride;
+    const float* sink_w; int sink;
+    unsigned* status;
+};
+
+__device__ __forceinline__ void pa_mma(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ unsigned pa_transposed(unsigned a) {
+    unsigned d;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(d) : "r"(a));
+    return d;
+}
+__device__ __forceinline__ unsigned pa_pack(float a, float b) {
+    __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<unsigned*>(&h);
+}
+// The pair of codes at bits 4 i of both halves as bfloat16: 128 + u, or with EXACT u itself.
+template <bool EXACT>
+__device__ __forceinline__ unsigned pa_codes(unsigned w, int i) {
+    const unsigned v = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+    if constexpr (!EXACT) return v;
+    const __nv_bfloat162 k = __halves2bfloat162(__ushort_as_bfloat16(0x4300), __ushort_as_bfloat16(0x4300));
+    __nv_bfloat162 h = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), k);
+    return *reinterpret_cast<unsigned*>(&h);
+}
+__device__ __forceinline__ void pa_bulk_load(void* dst, const void* src, unsigned bytes, unsigned long long* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n"
+                 ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ float pa_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+    return y;
+}
+// A score as the exponent of two that the softmax takes.
+template <bool EXACT>
+__device__ __forceinline__ float pa_score(float s, const PaParams& p) {
+    if (!(p.cap_log2 > 0.0f)) return s * p.scale_log2;
+    if constexpr (EXACT) return p.cap_log2 * tanhf(s * p.scale_over_cap);
+    float r;                                           // tanh x = 1 - 2 / (1 + e^(2 x))
+    asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(1.0f + pa_exp2(s * p.scale_over_cap * (2.0f * PA_LOG2E))));
+    return p.cap_log2 * fmaf(-2.0f, r, 1.0f);
+}
+
+template <int HD, int NT, bool F32>
+struct PaShape {
+    static constexpr int PARTS = F32 ? 3 : 1, COLS = 8 * NT, ROW = HD + 2;      // ROW: floats of a column's result in shared memory
+    static constexpr int JOIN = PA_WARPS * COLS * (ROW + 2) * 4;
+};
+
+template <int HD, int NT, bool F32, int CT>
+__global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_attention_kernel(const PaParams p) {
+    using S = PaShape<HD, NT, F32>;
+    using L = Packed<HD>;
+    using TQ = typename std::conditional<F32, float, __nv_bfloat16>::type;
+    constexpr int GROUPS = L::GROUPS, PARTS = S::PARTS, COLS = S::COLS, KEYS = CT * PK_TILE, BYTES = CT * L::TILE;
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ unsigned long long bars[PA_WARPS][PA_STAGES];
+    __shared__ int where[PA_WARPS][PA_STAGES];         // a stage's first position, or -1: nothing to read
+    __shared__ int gave_up;
+    pdl_launch();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    if (threadIdx.x < PA_WARPS * PA_STAGES) mbar_init(&bars[threadIdx.x / PA_STAGES][threadIdx.x % PA_STAGES], 1);
+    if (threadIdx.x == 0) gave_up = 0;
+    mbar_init_fence();
+    __syncthreads();
+    const int block = blockIdx.x / p.splits, split = blockIdx.x % p.splits, kvh = blockIdx.y / p.head_blocks, head0 = blockIdx.y % p.head_blocks * p.heads_each;
+    const int heads = min(p.heads_each, p.group - head0);
+    pdl_wait();
+    int req = block, row0 = block, rows = 1;
+    if (p.blocks) { req = p.blocks[3 * block]; row0 = p.blocks[3 * block + 1]; rows = p.blocks[3 * block + 2]; }
+    const int cols = min(rows * heads, COLS), pos_first = p.positions[row0], pos_last = p.positions[row0 + rows - 1];
+    const int lo = p.window > 0 ? max(0, pos_first - p.window + 1) : 0;
+    const int per_page = p.page_size / KEYS;
+    const int* list = p.list ? p.list + ((size_t)row0 * p.nkv + kvh) * p.top : nullptr;
+    const int chunk0 = list ? 0 : lo / KEYS;
+    const int chunks = pos_last < 0 ? 0 : list ? min(p.top, pos_last / p.page_size + 1) * per_page : pos_last / KEYS + 1 - chunk0;
+    const int per = ((chunks + p.splits - 1) / p.splits + PA_WARPS - 1) / PA_WARPS * PA_WARPS;
+    const int begin = split * per + warp, end = min(chunks, (split + 1) * per);
+    const int turns = begin < end ? (end - begin + PA_WARPS - 1) / PA_WARPS : 0;
+    const size_t slot = (((size_t)block * gridDim.y + blockIdx.y) * p.splits + split) * COLS;
+    if (p.part_o && split * per >= chunks) {           // no range of this request is left for this CTA
+        if (threadIdx.x < COLS) reinterpret_cast<float2*>(p.part_ml)[slot + threadIdx.x] = make_float2(-INFINITY, 0.0f);
+        return;
+    }
+
+    // ---- copies: a lane looks up the page of one of the warp's next 32 turns
+    unsigned char* ring = smem + (size_t)warp * PA_STAGES * BYTES;
+    int page = -1, base = 0;
+    auto issue = [&](int turn) {
+        if (turn >= turns) return;
+        if ((turn & 31) == 0) {
+            const int c = begin + (turn + lane) * PA_WARPS;
+            page = -1;
+            if (c < end) {
+                int index;
+                if (list) {
+                    index = list[c / per_page];
+                    base = index * p.page_size + c % per_page * KEYS;
+                } else {
+                    base = (chunk0 + c) * KEYS;
+                    index = base / p.page_size;
+                }
+                if (index >= 0 && base <= pos_last) {
+                    page = index < p.max_pages && req >= 0 && req < p.n_req ? p.table[(size_t)req * p.max_pages + index] : -1;
+                    if (page < 0 || page >= p.num_pages) {
+                        page = -1;
+                        if (p.status) atomicOr(p.status, BG_STATUS_BAD_PAGE);
+                    }
+                }
+            }
+        }
+        const int from = __shfl_sync(0xffffffffu, page, turn & 31), at = __shfl_sync(0xffffffffu, base, turn & 31);
+        if (lane == 0) {
+            const int stage = turn % PA_STAGES;
+            where[warp][stage] = from < 0 ? -1 : at;
+            if (from < 0) {
+                mbar_arrive(&bars[warp][stage]);
+            } else {
+                mbar_expect_tx(&bars[warp][stage], BYTES);
+                pa_bulk_load(ring + stage * BYTES, p.pool + ((size_t)from * p.nkv + kvh) * p.block_bytes + (size_t)(at % p.page_size / PK_TILE) * L::TILE, BYTES,
+                             &bars[warp][stage]);
+            }
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < PA_STAGES; ++i) issue(i);
+
+    // ---- queries: column g of every block of 8, features 64 group + 16 t .. + 15 as four steps of a product
+    unsigned qf[PARTS][NT][GROUPS][8];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const int col = nt * 8 + g;
+        const bool have = col < cols;
+        const int r = have ? col / heads : 0, h = head0 + (have ? col - r * heads : 0);
+        const TQ* q = reinterpret_cast<const TQ*>(p.q) + (size_t)(row0 + r) * p.q_stride + (size_t)(kvh * p.group + h) * HD + 16 * t;
+#pragma unroll
+        for (int gr = 0; gr < GROUPS; ++gr) {
+            if constexpr (F32) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    float2 v = have ? *reinterpret_cast<const float2*>(q + gr * PK_GROUP + 2 * i) : make_float2(0.0f, 0.0f);
+#pragma unroll
+                    for (int part = 0; part < PARTS; ++part) {
+                        const __nv_bfloat16 a = __float2bfloat16_rn(v.x), b = __float2bfloat16_rn(v.y);
+                        qf[part][nt][gr][i] = (unsigned)__bfloat16_as_ushort(a) | (unsigned)__bfloat16_as_ushort(b) << 16;
+                        v.x -= __bfloat162float(a); v.y -= __bfloat162float(b);
+                    }
+                }
+            } else {
+                const uint4 a = have ? *reinterpret_cast<const uint4*>(q + gr * PK_GROUP) : make_uint4(0, 0, 0, 0);
+                const uint4 b = have ? *reinterpret_cast<const uint4*>(q + gr * PK_GROUP + 8) : make_uint4(0, 0, 0, 0);
+                qf[0][nt][gr][0] = a.x; qf[0][nt][gr][1] = a.y; qf[0][nt][gr][2] = a.z; qf[0][nt][gr][3] = a.w;
+                qf[0][nt][gr][4] = b.x; qf[0][nt][gr][5] = b.y; qf[0][nt][gr][6] = b.z; qf[0][nt][gr][7] = b.w;
+            }
+        }
+    }
+    float qsum[NT][GROUPS][2];                         // of columns 2t, 2t + 1 of every block
+    int seen[NT][2];                                   // the positions of their rows
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int gr = 0; gr < GROUPS; ++gr) {
+            float c[4] = {};
+#pragma unroll
+            for (int part = 0; part < PARTS; ++part)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) pa_mma(c, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u, qf[part][nt][gr][2 * k], qf[part][nt][gr][2 * k + 1]);
+            qsum[nt][gr][0] = c[0]; qsum[nt][gr][1] = c[1];
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int col = nt * 8 + 2 * t + j;
+            seen[nt][j] = col < cols ? p.positions[row0 + col / heads] : pos_last;
+        }
+    }
+
+    float o[GROUPS * 4][NT][4] = {}, minus[GROUPS][NT][4] = {}, low[NT][GROUPS][2] = {}, m[NT][2], l[NT][2] = {};
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) m[nt][0] = m[nt][1] = -INFINITY;
+
+    auto chunk = [&](const unsigned char* stage, int at, auto edge_) {
+        constexpr bool EDGE = decltype(edge_)::value;
+        float x[CT][NT][4];
+        unsigned hidden = 0;                           // EDGE: the numbers of x that their column does not see
+#pragma unroll
+        for (int i = 0; i < CT; ++i) {
+            const unsigned char* tile = stage + i * L::TILE;
+            unsigned kw[2][GROUPS * 2], kp[2][GROUPS];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const unsigned char* row = tile + (g + 8 * half) * (HD / 2) + t * GROUPS * 8;
+                const unsigned char* pair = tile + L::PAIRS + (g + 8 * half) * (2 * GROUPS * 4);
+                if constexpr (GROUPS == 2) {
+                    const uint4 w = *reinterpret_cast<const uint4*>(row);
+                    kw[half][0] = w.x; kw[half][1] = w.y; kw[half][2] = w.z; kw[half][3] = w.w;
+                    const uint2 v = *reinterpret_cast<const uint2*>(pair);
+                    kp[half][0] = v.x; kp[half][1] = v.y;
+                } else {
+                    const uint2 w = *reinterpret_cast<const uint2*>(row);
+                    kw[half][0] = w.x; kw[half][1] = w.y;
+                    kp[half][0] = *reinterpret_cast<const unsigned*>(pair);
+                }
+            }
+            float s[NT][4] = {};
+#pragma unroll
+            for (int gr = 0; gr < GROUPS; ++gr) {
+                float c[NT][4] = {};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const unsigned w0 = kw[0][gr * 2 + k / 2], w1 = kw[1][gr * 2 + k / 2];
+                    const int n = k % 2 * 2;
+                    const unsigned a0 = pa_codes<F32>(w0, n), a1 = pa_codes<F32>(w1, n), a2 = pa_codes<F32>(w0, n + 1), a3 = pa_codes<F32>(w1, n + 1);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int part = PARTS - 1; part >= 0; --part) pa_mma(c[nt], a0, a1, a2, a3, qf[part][nt][gr][2 * k], qf[part][nt][gr][2 * k + 1]);
+                }
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const float step = pair_step(kp[half][gr]);
+                    const float lowest = F32 ? pair_lowest(kp[half][gr]) : fmaf(-128.0f, step, pair_lowest(kp[half][gr]));
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) s[nt][2 * half + j] += fmaf(step, c[nt][2 * half + j], lowest * qsum[nt][gr][j]);
+                }
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    x[i][nt][e] = pa_score<F32>(s[nt][e], p);
+                    if constexpr (EDGE) {
+                        const int pos = at + i * PK_TILE + g + (e & 2) * 4, last = seen[nt][e & 1];
+                        if (pos > last || (p.window > 0 && pos <= last - p.window)) {
+                            x[i][nt][e] = -INFINITY;
+                            hidden |= 1u << ((i * NT + nt) * 4 + e);
+                        }
+                    }
+                }
+        }
+        // the running maximum, and what it does to what there is
+        float top[NT][2];
+        bool grew = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                float v = x[0][nt][j];
+#pragma unroll
+                for (int i = 0; i < CT; ++i) v = fmaxf(v, fmaxf(x[i][nt][j], x[i][nt][j + 2]));
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
+                top[nt][j] = fmaxf(m[nt][j], v);
+                grew |= top[nt][j] > m[nt][j];
+            }
+        if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const float keep = top[nt][j] == m[nt][j] ? 1.0f : F32 ? exp2f(m[nt][j] - top[nt][j]) : pa_exp2(m[nt][j] - top[nt][j]);
+                    m[nt][j] = top[nt][j];
+                    l[nt][j] *= keep;
+#pragma unroll
+                    for (int gr = 0; gr < GROUPS; ++gr) { low[nt][gr][j] *= keep; minus[gr][nt][j] *= keep; }
+#pragma unroll
+                    for (int i = 0; i < GROUPS * 4; ++i) { o[i][nt][j] *= keep; o[i][nt][j + 2] *= keep; }
+                }
+        }
+#pragma unroll
+        for (int i = 0; i < CT; ++i) {
+            const unsigned char* tile = stage + i * L::TILE;
+            float w[NT][4];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float from = m[nt][e & 1] == -INFINITY ? 0.0f : m[nt][e & 1];
+                    w[nt][e] = F32 ? exp2f(x[i][nt][e] - from) : pa_exp2(x[i][nt][e] - from);
+                    l[nt][e & 1] += w[nt][e];
+                }
+            unsigned vw[GROUPS][4], vp[2][GROUPS];     // words of positions 2t, 2t + 1, 2t + 8, 2t + 9; pairs of positions g, g + 8
+            if constexpr (GROUPS == 2) {
+                const uint4 a = *reinterpret_cast<const uint4*>(tile + L::CODES + lane * 16), b = *reinterpret_cast<const uint4*>(tile + L::CODES + 512 + lane * 16);
+                vw[0][0] = a.x; vw[1][0] = a.y; vw[0][1] = a.z; vw[1][1] = a.w;
+                vw[0][2] = b.x; vw[1][2] = b.y; vw[0][3] = b.z; vw[1][3] = b.w;
+            } else {
+                const uint4 a = *reinterpret_cast<const uint4*>(tile + L::CODES + lane * 16);
+                vw[0][0] = a.x; vw[0][1] = a.y; vw[0][2] = a.z; vw[0][3] = a.w;
+            }
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int gr = 0; gr < GROUPS; ++gr)
+                    vp[half][gr] = *reinterpret_cast<const unsigned*>(tile + L::PAIRS + (g + 8 * half) * (2 * GROUPS * 4) + (GROUPS + gr) * 4);
+#pragma unroll
+            for (int gr = 0; gr < GROUPS; ++gr) {
+                unsigned b[PARTS][NT][2];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        const float step = pair_step(vp[half][gr]), lowest = pair_lowest(vp[half][gr]);
+                        float e[2];
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            const float weight = w[nt][2 * half + j];
+                            e[j] = weight * step;
+                            float add = weight * lowest;
+                            if constexpr (EDGE) {      // (what lies in a place that is not seen may be no number)
+                                if (hidden >> ((i * NT + nt) * 4 + 2 * half + j) & 1) e[j] = add = 0.0f;
+                            }
+                            low[nt][gr][j] += add;
+                        }
+                        if constexpr (F32) {
+#pragma unroll
+                            for (int part = 0; part < PARTS; ++part) {
+                                const __nv_bfloat16 a = __float2bfloat16_rn(e[0]), c = __float2bfloat16_rn(e[1]);
+                                b[part][nt][half] = pa_transposed((unsigned)__bfloat16_as_ushort(a) | (unsigned)__bfloat16_as_ushort(c) << 16);
+                                e[0] -= __bfloat162float(a); e[1] -= __bfloat162float(c);
+                            }
+                        } else {
+                            b[0][nt][half] = pa_transposed(pa_pack(e[0], e[1]));
+                        }
+                    }
+                if constexpr (!F32) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) pa_mma(minus[gr][nt], 0xc300c300u, 0xc300c300u, 0xc300c300u, 0xc300c300u, b[0][nt][0], b[0][nt][1]);
+                }
+                const unsigned ab[2] = {__byte_perm(vw[gr][0], vw[gr][1], 0x5410), __byte_perm(vw[gr][0], vw[gr][1], 0x7632)};
+                const unsigned cd[2] = {__byte_perm(vw[gr][2], vw[gr][3], 0x5410), __byte_perm(vw[gr][2], vw[gr][3], 0x7632)};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {          // features 8 g + 2 k (rows g of the product) and 8 g + 2 k + 1 (rows g + 8)
+                    const int n = k % 2 * 2;
+                    const unsigned a0 = pa_codes<F32>(ab[k / 2], n), a1 = pa_codes<F32>(ab[k / 2], n + 1);
+                    const unsigned a2 = pa_codes<F32>(cd[k / 2], n), a3 = pa_codes<F32>(cd[k / 2], n + 1);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int part = PARTS - 1; part >= 0; --part) pa_mma(o[gr * 4 + k][nt], a0, a1, a2, a3, b[part][nt][0], b[part][nt][1]);
+                }
+            }
+        }
+    };
+
+    bool fine = true;
+    int turn = 0;
+    for (; turn < turns; ++turn) {
+        const int stage = turn % PA_STAGES;
+        fine = __all_sync(0xffffffffu, mbar_wait(&bars[warp][stage], (turn / PA_STAGES) & 1, &gave_up));
+        if (!fine) break;
+        const int at = where[warp][stage];
+        if (at >= 0) {
+            if (at + KEYS - 1 > pos_first || (p.window > 0 && at <= pos_last - p.window)) chunk(ring + stage * BYTES, at, std::true_type{});
+            else chunk(ring + stage * BYTES, at, std::false_type{});
+        }
+        __syncwarp();
+        issue(turn + PA_STAGES);
+    }
+    if (!fine) {                                       // a copy did not come: the others of this warp are waited for, and the status says so
+        if (lane == 0 && p.status) atomicOr(p.status, BG_STATUS_TIMEOUT);
+        for (int i = turn; i < min(turns, turn + PA_STAGES); ++i) mbar_wait(&bars[warp][i % PA_STAGES], (i / PA_STAGES) & 1);
+    }
+
+    // ---- the warps' results meet
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) {
+                l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], d);
+#pragma unroll
+                for (int gr = 0; gr < GROUPS; ++gr) low[nt][gr][j] += __shfl_xor_sync(0xffffffffu, low[nt][gr][j], d);
+            }
+    __syncthreads();                                   // (the rings are read out)
+    float* res = reinterpret_cast<float*>(smem);
+    float2* ml = reinterpret_cast<float2*>(res + PA_WARPS * COLS * S::ROW);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int col = nt * 8 + 2 * t + j;
+            if (g == 0) ml[warp * COLS + col] = make_float2(m[nt][j], l[nt][j]);
+#pragma unroll
+            for (int gr = 0; gr < GROUPS; ++gr) {
+                const float add = minus[gr][nt][j] + low[nt][gr][j];
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    *reinterpret_cast<float2*>(res + (size_t)(warp * COLS + col) * S::ROW + gr * PK_GROUP + 8 * g + 2 * k) =
+                        make_float2(o[gr * 4 + k][nt][j] + add, o[gr * 4 + k][nt][j + 2] + add);
+            }
+        }
+    __syncthreads();
+    for (int i = threadIdx.x; i < cols * (HD / 2); i += PA_THREADS) {
+        const int col = i / (HD / 2), f = i % (HD / 2) * 2;
+        float2 each[PA_WARPS];
+        float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < PA_WARPS; ++w) { each[w] = ml[w * COLS + col]; top = fmaxf(top, each[w].x); }
+        const float from = top == -INFINITY ? 0.0f : top;
+        float2 v = make_float2(0.0f, 0.0f);
+#pragma unroll
+        for (int w = 0; w < PA_WARPS; ++w) {
+            const float by = exp2f(each[w].x - from);  // (nothing seen: 0)
+            const float2 a = *reinterpret_cast<const float2*>(res + (size_t)(w * COLS + col) * S::ROW + f);
+            // (scores that are no numbers have no maximum: they show by their sum)
+            sum = fmaf(each[w].y, each[w].x == -INFINITY ? 1.0f : by, sum);
+            v.x = fmaf(a.x, by, v.x); v.y = fmaf(a.y, by, v.y);
+        }
+        if (p.part_o) {
+            reinterpret_cast<float2*>(p.part_o + (slot + col) * HD)[i % (HD / 2)] = v;
+            if (f == 0) reinterpret_cast<float2*>(p.part_ml)[slot + col] = make_float2(top, sum);
+            continue;
+        }
+        const int r = col / heads, h = kvh * p.group + head0 + col - r * heads;
+        float by = 1.0f;
+        if (p.sink) {
+            const float at = (p.sink_w ? p.sink_w[h] : 0.0f) * PA_LOG2E, most = fmaxf(top, at);
+            by = top == -INFINITY ? (sum == 0.0f ? 0.0f : 1.0f) : exp2f(top - most);
+            sum = fmaf(sum, by, exp2f(at - most));
+        }
+        by = sum == 0.0f ? 0.0f : by / sum;            // (a row that sees nothing is nought)
+        TQ* out = reinterpret_cast<TQ*>(p.out) + (size_t)(row0 + r) * p.out_stride + (size_t)h * HD + f;
+        if constexpr (F32) *reinterpret_cast<float2*>(out) = make_float2(v.x * by, v.y * by);
+        else *reinterpret_cast<__nv_bfloat162*>(out) = __floats2bfloat162_rn(v.x * by, v.y * by);
+    }
+}
+
+// out = sum_i o_i 2^(m_i - m) / sum_i l_i 2^(m_i - m) over the ranges of a column; EACH warps take every EACH-th range and join in their order.
+constexpr int PM_WARPS = 8;
+template <int HD, bool F32, int EACH>
+__global__ void __launch_bounds__(PM_WARPS * 32) packed_merge_kernel(const PaParams p, int cols_most) {
+    constexpr int PER = HD / 32, AT_ONCE = 8;
+    using TQ = typename std::conditional<F32, float, __nv_bfloat16>::type;
+    __shared__ float acc_s[PM_WARPS][HD];
+    __shared__ float2 ml_s[PM_WARPS];
+    pdl_launch();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp % EACH;
+    const int block = blockIdx.x, kvh = blockIdx.y / p.head_blocks, head0 = blockIdx.y % p.head_blocks * p.heads_each, heads = min(p.heads_each, p.group - head0);
+    const int col = blockIdx.z * (PM_WARPS / EACH) + warp / EACH;
+    pdl_wait();
+    int row0 = block, rows = 1;
+    if (p.blocks) { row0 = p.blocks[3 * block + 1]; rows = p.blocks[3 * block + 2]; }
+    const bool idle = col >= rows * heads || col >= cols_most;
+    const size_t base = ((size_t)block * gridDim.y + blockIdx.y) * p.splits * cols_most + (idle ? 0 : col);
+    float m = -INFINITY, l = 0.0f, acc[PER] = {};
+    for (int i0 = part; !idle && i0 < p.splits; i0 += AT_ONCE * EACH) {
+        float2 ml[AT_ONCE];
+        float v[AT_ONCE][PER];
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; ++j) {
+            const int i = i0 + j * EACH;
+            ml[j] = i < p.splits ? reinterpret_cast<const float2*>(p.part_ml)[base + (size_t)i * cols_most] : make_float2(-INFINITY, 0.0f);
+        }
+        float top = m;
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; ++j) {
+            const int i = i0 + j * EACH;
+            const bool have = ml[j].x != -INFINITY || ml[j].y != 0.0f;         // (a range without positions has written no more than that)
+            const float* from = p.part_o + (base + (size_t)i * cols_most) * HD + lane * PER;
+            if constexpr (PER == 4) {
+                const float4 a = have ? *reinterpret_cast<const float4*>(from) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                v[j][0] = a.x; v[j][1] = a.y; v[j][2] = a.z; v[j][3] = a.w;
+            } else {
+                const float2 a = have ? *reinterpret_cast<const float2*>(from) : make_float2(0.0f, 0.0f);
+                v[j][0] = a.x; v[j][1] = a.y;
+            }
+            top = fmaxf(top, ml[j].x);
+        }
+        const float from = top == -INFINITY ? 0.0f : top, keep = m == -INFINITY ? 1.0f : exp2f(m - from);
+        l *= keep;
+#pragma unroll
+        for (int e = 0; e < PER; ++e) acc[e] *= keep;
+        m = top;
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; ++j) {
+            const float by = ml[j].x == -INFINITY ? 1.0f : exp2f(ml[j].x - from);      // (scores that are no numbers have no maximum)
+            l = fmaf(ml[j].y, by, l);
+#pragma unroll
+            for (int e = 0; e < PER; ++e) acc[e] = fmaf(v[j][e], by, acc[e]);
+        }
+    }
+    if constexpr (EACH > 1) {
+#pragma unroll
+        for (int e = 0; e < PER; ++e) acc_s[warp][lane * PER + e] = acc[e];
+        if (lane == 0) ml_s[warp] = make_float2(m, l);
+        __syncthreads();
+        if (part) return;
+        float top = m;
+#pragma unroll
+        for (int j = 1; j < EACH; ++j) top = fmaxf(top, ml_s[warp + j].x);
+        const float from = top == -INFINITY ? 0.0f : top, keep = m == -INFINITY ? 1.0f : exp2f(m - from);
+        l *= keep;
+#pragma unroll
+        for (int e = 0; e < PER; ++e) acc[e] *= keep;
+        m = top;
+#pragma unroll
+        for (int j = 1; j < EACH; ++j) {
+            const float2 ml = ml_s[warp + j];
+            const float by = ml.x == -INFINITY ? 1.0f : exp2f(ml.x - from);
+            l = fmaf(ml.y, by, l);
+#pragma unroll
+            for (int e = 0; e < PER; ++e) acc[e] = fmaf(acc_s[warp + j][lane * PER + e], by, acc[e]);
+        }
+    }
+    if (idle) return;
+    const int r = col / heads, h = kvh * p.group + head0 + col - r * heads;
+    float by = 1.0f;
+    if (p.sink) {
+        const float at = (p.sink_w ? p.sink_w[h] : 0.0f) * PA_LOG2E, most = fmaxf(m, at);
+        by = m == -INFINITY ? (l == 0.0f ? 0.0f : 1.0f) : exp2f(m - most);
+        l = fmaf(l, by, exp2f(at - most));
+    }
+    by = l == 0.0f ? 0.0f : by / l;
+    TQ* out = reinterpret_cast<TQ*>(p.out) + (size_t)(row0 + r) * p.out_stride + (size_t)h * HD + lane * PER;
+#pragma unroll
+    for (int e = 0; e < PER; e += 2) {
+        if constexpr (F32) *reinterpret_cast<float2*>(out + e) = make_float2(acc[e] * by, acc[e + 1] * by);
+        else *reinterpret_cast<__nv_bfloat162*>(out + e) = __floats2bfloat162_rn(acc[e] * by, acc[e + 1] * by);
+    }
+}
+
+template <int HD, int NT, bool F32, int CT>
+static int pa_launch(const PaParams& p, int n, cudaStream_t stream) {
+    const size_t ring = (size_t)PA_WARPS * PA_STAGES * CT * Packed<HD>::TILE, join = PaShape<HD, NT, F32>::JOIN, smem = ring > join ? ring : join;
+    cudaError_t e = smem_limit(packed_attention_kernel<HD, NT, F32, CT>, smem);
+    if (e != cudaSuccess) return (int)e;
+    e = launch(packed_attention_kernel<HD, NT, F32, CT>, dim3((unsigned)((long long)n * p.splits), p.nkv * p.head_blocks), dim3(PA_THREADS), smem, stream, p);
+    if (e != cudaSuccess) return (int)e;
+    if (!p.part_o) return BG_OK;
+    constexpr int COLS = 8 * NT;
+    e = p.splits > 8 ? launch(packed_merge_kernel<HD, F32, PM_WARPS>, dim3(n, p.nkv * p.head_blocks, COLS), dim3(PM_WARPS * 32), 0, stream, p, COLS)
+                     : launch(packed_merge_kernel<HD, F32, 1>, dim3(n, p.nkv * p.head_blocks, NT), dim3(PM_WARPS * 32), 0, stream, p, COLS);
+    return e == cudaSuccess ? BG_OK : (int)e;
+}
+
+template <int HD, bool F32>
+static int pa_sized(const PaParams& p, int n, int nt, cudaStream_t stream) {
+    const bool wide = p.page_size % (2 * PK_TILE) == 0;
+    if (nt == 1) return wide ? pa_launch<HD, 1, F32, 2>(p, n, stream) : pa_launch<HD, 1, F32, 1>(p, n, stream);
+    if constexpr (F32) return BG_ERR_UNSUPPORTED;
+    else return wide ? pa_launch<HD, 2, F32, 2>(p, n, stream) : pa_launch<HD, 2, F32, 1>(p, n, stream);
+}
+
+}  // namespace bg
+
+using namespace bg;
+
+// Columns of a block of `rows` rows: blocks of 8 (row, head) pairs that one CTA takes (1 or 2; float queries, whose parts fill the registers, 1), and query
+// heads of a block.  heads_each * rows fits the columns.
+extern "C" int bg_packed_attention_columns(int group, int f32, int rows, int* heads_each) {
+    const int most = f32 ? 8 : 16;
+    if (group <= 0 || rows <= 0) return BG_ERR_SHAPE;
+    *heads_each = group <= most ? group : most;
+    if (*heads_each * rows > most) return BG_ERR_UNSUPPORTED;
+    return *heads_each * rows <= 8 ? 1 : 2;
+}
+
+// n blocks of rows; `rows` is the most rows of a block.  part_o / part_ml hold n * nkv * head_blocks * splits * columns results where splits > 1.
+extern "C" int bg_packed_attention(const void* q, int dtype, long long q_stride, const unsigned char* pool, long long block_bytes, int num_pages, int page_size,
+                                   const int* table, int max_pages, int n_req, const int* positions, const int* blocks, int n, int rows, const int* list,
+                                   int top, float* part_o, float* part_ml, int splits, int nh, int nkv, int hd, int window, float scale, float softcap,
+                                   const float* sink_w, int sink, void* out, long long out_stride, unsigned* status, cudaStream_t stream) {
+    if (hd != 64 && hd != 128) return BG_ERR_UNSUPPORTED;
+    if (n <= 0) return BG_OK;
+    if (page_size <= 0 || page_size % PK_TILE || nkv <= 0 || nh <= 0 || nh % nkv || splits <= 0 || num_pages <= 0 || max_pages <= 0 || window < 0) return BG_ERR_SHAPE;
+    if (block_bytes % 16 || block_bytes < page_size / PK_TILE * packed_tile_bytes(hd) || (long long)n * splits > 0x7fffffffLL || (list && (top <= 0 || rows != 1))) return BG_ERR_SHAPE;
+    if (dtype != BG_DTYPE_F32 && dtype != BG_DTYPE_BF16) return BG_ERR_DTYPE;
+    const bool f32 = dtype == BG_DTYPE_F32;
+    const long long size = f32 ? 4 : 2;
+    if ((uintptr_t)pool % 16 || ((long long)(uintptr_t)q | q_stride * size) % 16 || ((long long)(uintptr_t)out | out_stride * size) % (2 * size)) return BG_ERR_ALIGN;
+    if ((splits > 1) != (part_o != nullptr) || (part_o == nullptr) != (part_ml == nullptr) || (uintptr_t)part_o % 16 || (uintptr_t)part_ml % 8) return BG_ERR_SHAPE;
+    int each = 0;
+    const int nt = bg_packed_attention_columns(nh / nkv, f32, rows, &each);
+    if (nt < 0) return nt;
+    const int group = nh / nkv, head_blocks = (group + each - 1) / each;
+    if ((long long)nkv * head_blocks > 65535) return BG_ERR_SHAPE;
+    const PaParams p = {q, q_stride, pool, block_bytes, table, positions, blocks, list, num_pages, page_size, max_pages, top, n_req, nkv, group, head_blocks, each,
+                        window, splits, scale * PA_LOG2E, softcap > 0.0f ? softcap * PA_LOG2E : 0.0f, softcap > 0.0f ? scale / softcap : 0.0f,
+                        part_o, part_ml, out, out_stride, sink_w, sink, status};
+    if (hd == 64) return f32 ? pa_sized<64, true>(p, n, nt, stream) : pa_sized<64, false>(p, n, nt, stream);
+    return f32 ? pa_sized<128, true>(p, n, nt, stream) : pa_sized<128, false>(p, n, nt, stream);
+}
