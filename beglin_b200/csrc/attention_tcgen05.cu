@@ -31,6 +31,8 @@
 // Every wait on an mbarrier is bounded in time and records BG_STATUS_TIMEOUT.
 //
 // The result is the finished row, out[t, h, :] = O / l, as in attention_mma.cu's rows arrangement.
+#include <cuda_fp16.h>
+
 #include "float_pairs.cuh"
 #include "page_tma.cuh"
 
@@ -81,13 +83,21 @@ struct AttnTcSharedParams : AttnTcParams {
     float* part_ml;             // [rows][nh][slots][2] maximum (of scores as they are), sum
     int slots;
 };
+// What the HALF instances take besides.
+struct AttnTcHalfParams : AttnTcParams {
+    const int2* shifts;         // [n][nkv] of the requests that the query blocks name: the cache holds keys 2^-x and values 2^-y
+};
 template <bool V> struct AtSplit { static constexpr bool value = V; };
 // SHARED: of the pairs of exponentials every eighth is the float units' (256 rows of 28 heads over 32,768 positions, 140 CTAs: 113.5 us; none of them
 // 120.6, every fourth 125.7: the special function units and the instructions' issue are both near their limits).
 constexpr int AT_FLOAT_EVERY = 7;
-template <bool DIFF, bool SHARED> struct AtParams { using type = AttnTcParams; };
-template <> struct AtParams<true, false> { using type = AttnTcDiffParams; };
-template <> struct AtParams<false, true> { using type = AttnTcSharedParams; };
+template <bool DIFF, bool SHARED, bool HALF> struct AtParams { using type = AttnTcParams; };
+template <> struct AtParams<true, false, false> { using type = AttnTcDiffParams; };
+template <> struct AtParams<false, true, false> { using type = AttnTcSharedParams; };
+template <> struct AtParams<false, false, true> { using type = AttnTcHalfParams; };
+
+__device__ __forceinline__ int at_value_shift(const AttnTcParams&, int) { return 0; }
+__device__ __forceinline__ int at_value_shift(const AttnTcHalfParams& p, int i) { return p.shifts[i].y; }
 
 __device__ __forceinline__ float at_ex2(float x) {
     float y;
@@ -138,9 +148,15 @@ __device__ __forceinline__ float at_squash(float x, float cap_log2, float cap_k)
 // both (256 rows of 28 heads over 32,768 positions are bound by what the L2 delivers with 128 rows a CTA: 7.1 TB/s).
 // SHARED also has two warps to issue the scores' products (0 and 13) and two for the values' (6 and 15), each pair taking the turns in turns: a turn's
 // waits, eight MMAs and commits take one warp some 1,200 cycles, more than the tensor cores need for it.
-template <int HD, int AT_BK, bool SINK = false, bool EXT = false, bool DIFF = false, bool SHARED = false>
+// HALF: the operands are half precision (11 bits in place of bfloat16's 8): the cache is one that was written out of 4 bits for this step, its keys and values
+// scaled by a power of two for each kv head so that the largest lies below 2^15, and so is every row of queries on its way into shared memory; the scores
+// and the results get the powers back in float.  With keys rounded to bfloat16 the results over 16,000 positions were 0.0044 of their norm off, with halves
+// 0.0017, which is the rounding of the results themselves.  The weights go up to 2^15 (2^7 above the reference maximum), so that none above 2^-31 of it is lost.
+constexpr float AT_HALF_UP = 7.0f;
+template <int HD, int AT_BK, bool SINK = false, bool EXT = false, bool DIFF = false, bool SHARED = false, bool HALF = false>
 __global__ void __launch_bounds__(SHARED ? AT_SHARED_THREADS : AT_THREADS)
-attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename AtParams<DIFF, SHARED>::type p) {
+attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename AtParams<DIFF, SHARED, HALF>::type p) {
+    static_assert(!HALF || !(EXT || DIFF || SHARED), "halves: the plain softmax, and one with a sink");
     static_assert(!DIFF || (AT_BK == 64 && !SINK && !EXT), "the two maps take tiles of 64 keys in turns");
     static_assert(!SHARED || (AT_BK == 64 && !SINK && !EXT && !DIFF), "partial results of tiles of 64 keys");
     constexpr bool MAY_TWICE = DIFF || SHARED;           // a tile of keys may be taken twice, by one softmax group and then by the other
@@ -180,6 +196,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
     __shared__ int row_of[SHARED ? 2 * AT_BM : 1];
     __shared__ unsigned tmem_sh;
     __shared__ int failed;
+    __shared__ float unit_of[HALF ? AT_BM : 1];          // what a row's scores are multiplied with
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
     // the blocks with the most keys (the last ones of a prompt) are handed out first, for every kv head, so that
@@ -244,6 +261,24 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
             uint4 v = make_uint4(0, 0, 0, 0);
             if (r < n_rows)
                 v = *reinterpret_cast<const uint4*>(p.q + (size_t)(SHARED ? row_of[r] : batch_row(r)) * p.q_stride + (size_t)(kvh * group + head_of(r)) * HD + c * 8);
+            if constexpr (HALF) {                        // (the lanes of a row are neighbours)
+                const unsigned w[4] = {v.x, v.y, v.z, v.w};
+                float top = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) top = fmaxf(top, fmaxf(fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xffff0000u))));
+#pragma unroll
+                for (int o = HD / 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                const int e = max(-100, (int)(__float_as_uint(top) >> 23) - 127 - 14);       // (a row of noughts, or one that is no number: whatever)
+                const float down = __uint_as_float((unsigned)(127 - e) << 23);
+                unsigned h[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const __half2 x = __floats2half2_rn(__uint_as_float(w[i] << 16) * down, __uint_as_float(w[i] & 0xffff0000u) * down);
+                    h[i] = *reinterpret_cast<const unsigned*>(&x);
+                }
+                v = make_uint4(h[0], h[1], h[2], h[3]);
+                if (c == 0) unit_of[r] = exp2f((float)min(e + p.shifts[req * p.nkv + kvh].x, 120));
+            }
             const int cb = c >> 3, cc = c & 7;
             const int rr = SHARED ? r & (AT_BM - 1) : r;
             *reinterpret_cast<uint4*>(q_s + (SHARED ? (r / AT_BM) * QT_BYTES : 0) + cb * (AT_BM * 128) + rr * 128 + ((cc ^ (rr & 7)) << 4)) = v;
@@ -288,8 +323,9 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
         // uniform registers, which keeps the issue of one small MMA to a few cycles.  P, the left operand of the
         // second product, lies in tensor memory, so that MMA reads only its value tile from shared memory (with
         // both operands there, a 128 x 128 x 16 MMA asks for all of an SM's shared-memory bandwidth).
-        constexpr unsigned idesc_qk = instr_desc_bf16(AT_BM, AT_BK, 0);
-        constexpr unsigned idesc_pv = instr_desc_bf16(AT_BM, HD, 1);
+        constexpr unsigned bf16_bits = HALF ? (1u << 7) | (1u << 10) : 0u;
+        constexpr unsigned idesc_qk = instr_desc_bf16(AT_BM, AT_BK, 0) & ~bf16_bits;
+        constexpr unsigned idesc_pv = instr_desc_bf16(AT_BM, HD, 1) & ~bf16_bits;
         const unsigned q_addr = smem_u32(q_s);
         bool ok = true;
         auto wait_all = [&](unsigned long long* bar, unsigned parity) {
@@ -399,7 +435,9 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
         float m = -INFINITY, l = 0.0f;
         bool ok = true;
         const bool capped = p.cap_log2 > 0.0f;
-        const float sl2 = (capped || EXT) ? 1.0f : p.scale_log2;
+        const float unit_row = HALF ? unit_of[r] : 1.0f;
+        const float sl2 = (capped || EXT) ? 1.0f : HALF ? p.scale_log2 * unit_row : p.scale_log2;
+        const float cap_k = HALF ? p.cap_k * unit_row : p.cap_k;
         const float slope_l2 = (EXT && p.slopes && real) ? p.slopes[kvh * group + r % group] * AT_LOG2E : 0.0f;
         const int i_first = ALT ? grp : 0;                   // this group's first tile
         for (int i = i_first; i < n_turns && ok; i += (ALT ? 2 : 1)) {
@@ -414,7 +452,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
             else tc_ld32(tmem + lane_addr + s_col, s);
             if (capped) {                                // squashed scores come out as exponents of two
 #pragma unroll
-                for (int q = 0; q < GK; ++q) s[q] = at_squash(s[q], p.cap_log2, p.cap_k);
+                for (int q = 0; q < GK; ++q) s[q] = at_squash(s[q], p.cap_log2, cap_k);
             }
             if constexpr (EXT) {                         // exponents of two, less the head's slope times the distance
                 const float at0 = slope_l2 * (float)(key0 - pos), unit = capped ? 1.0f : p.scale_log2;
@@ -441,8 +479,9 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
             // exponentials keep the old reference and nothing that was accumulated needs touching.
             const bool grow = __any_sync(0xffffffffu, tmax > m + 8.0f) || (i == i_first);
             const float m_new = grow ? fmaxf(m, tmax) : m;
-            const float m_use = (m_new == -INFINITY) ? 0.0f : m_new;
-            const float corr = grow ? at_ex2(m - m_use) : 1.0f;
+            const float m_ref = (m_new == -INFINITY) ? 0.0f : m_new;
+            const float corr = grow ? at_ex2(m - m_ref) : 1.0f;
+            const float m_use = HALF ? m_ref - AT_HALF_UP : m_ref;
             float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
             float pk[GK / 2];                            // P: two keys a column
             if constexpr (SHARED) {
@@ -467,8 +506,13 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
             for (int c = 0; c < GK / 2; ++c) {
                 const float e0 = at_ex2(fmaf(s[2 * c], sl2, -m_use)), e1 = at_ex2(fmaf(s[2 * c + 1], sl2, -m_use));
                 sums[c & 3] += e0 + e1;
-                const __nv_bfloat162 h2 = __floats2bfloat162_rn(e0, e1);
-                pk[c] = __uint_as_float(*reinterpret_cast<const unsigned*>(&h2));
+                if constexpr (HALF) {
+                    const __half2 h2 = __floats2half2_rn(e0, e1);
+                    pk[c] = __uint_as_float(*reinterpret_cast<const unsigned*>(&h2));
+                } else {
+                    const __nv_bfloat162 h2 = __floats2bfloat162_rn(e0, e1);
+                    pk[c] = __uint_as_float(*reinterpret_cast<const unsigned*>(&h2));
+                }
             }
             const float sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
             l = l * corr + sum;
@@ -497,6 +541,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
         }
         if (ok && n_tiles > 0) ok = mbar_wait(&o_ready, 0);
         if (!ok) atomicExch(&failed, 1);
+        if constexpr (HALF) m -= AT_HALF_UP;             // (sums and accumulators are in its units)
         // the join of the two groups: the second hands its maximum and sum over, the first group's thread of the
         // same row (the same lanes of tensor memory) reads both accumulators
         if (grp == 1) ml_other[r] = make_float2(m, l);
@@ -597,7 +642,8 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
             const float a0 = at_ex2(m - m_ref), a1 = at_ex2(other.x - m_ref);
             const float l_all = l * a0 + other.y * a1 + (SINK ? at_ex2(sink_l2 - m_ref) : 0.0f);
             const float inv = (real && l_all > 0.0f) ? 1.0f / l_all : 0.0f;
-            const float w0 = a0 * inv, w1 = a1 * inv;
+            const float back = HALF ? exp2f((float)at_value_shift(p, req * p.nkv + kvh)) : 1.0f;
+            const float w0 = HALF ? a0 * inv * back : a0 * inv, w1 = HALF ? a1 * inv * back : a1 * inv;
             const bool has1 = !ALT || n_tiles > 1;       // with one tile the second group's accumulator was never written
             __nv_bfloat16* o = p.out + (size_t)(row0 + qi) * p.out_stride + (size_t)(kvh * group + g) * HD;
 #pragma unroll
@@ -744,6 +790,17 @@ static int at_launch_shared(const CUtensorMap& map, const AttnTcSharedParams& p,
     e = launch(kern, dim3(p.nkv, n_items), dim3(AT_SHARED_THREADS), smem, stream, map, p);
     if (e != cudaSuccess) return (int)e;
     return BG_OK;
+}
+
+// The same for a cache of halves.
+template <int HD, int BK, bool SINK>
+static int at_launch_half(const CUtensorMap& map, const AttnTcHalfParams& p, int n_qblk, cudaStream_t stream) {
+    auto kern = attention_tcgen05_kernel<HD, BK, SINK, false, false, false, true>;
+    const size_t smem = (size_t)(HD / 64) * AT_BM * 128 + (size_t)2 * 256 * (HD / 64) * 128 + 1024;
+    cudaError_t e = smem_limit(kern, smem);
+    if (e != cudaSuccess) return (int)e;
+    e = launch(kern, dim3(p.nkv, n_qblk), dim3(AT_THREADS), smem, stream, map, p);
+    return e == cudaSuccess ? BG_OK : (int)e;
 }
 
 // The same for differential attention (tiles of 64 keys).
@@ -901,4 +958,36 @@ extern "C" int bg_attention_tc_shared(const void* q, int q_stride, const void* k
     int rc = pt_pool_map(&map, kv_pool, num_pages, nkv, page_size, hd);
     if (rc != BG_OK) return rc;
     return hd == 128 ? at_launch_shared<128>(map, p, n_items, stream) : at_launch_shared<64>(map, p, n_items, stream);
+}
+
+// Rows over a cache of halves [num_pages, 2, nkv, page_size, hd] whose keys and values are scaled by 2^-shifts: see the kernel.  The queries and results are
+// bfloat16.  The cache is a step's own scratch, so its tensor map is made for this call.
+extern "C" int bg_attention_tc_half(const void* q, int q_stride, const void* kv_pool, int num_pages, int page_size, const int* block_table, int max_pages,
+                                    const int* positions, const int* qblk, int n_qblk, const void* shifts, void* out, int out_stride, int nh, int nkv, int hd,
+                                    int window, float scale, int max_position, int sink, const float* sink_weight, float softcap, unsigned* status,
+                                    cudaStream_t stream) {
+    if (n_qblk <= 0) return BG_OK;
+    if (nkv <= 0 || nh % nkv != 0 || (hd != 64 && hd != 128) || nh / nkv > 128 || !(scale > 0.0f) || softcap < 0.0f || (sink_weight && !sink)) return BG_ERR_UNSUPPORTED;
+    if (!pt_page_size_ok(page_size) || n_qblk > 65535 || !shifts) return BG_ERR_SHAPE;
+    if ((q_stride % 8) || (out_stride % 8) || ((uintptr_t)q % 16) || ((uintptr_t)kv_pool % 16) || ((uintptr_t)out % 16) || ((uintptr_t)shifts % 8)) return BG_ERR_ALIGN;
+    AttnTcHalfParams p;
+    memset(&p, 0, sizeof(p));
+    p.q = (const __nv_bfloat16*)q; p.q_stride = q_stride; p.kv_pool = (const __nv_bfloat16*)kv_pool;
+    p.num_pages = num_pages; p.page_size = page_size; p.page_shift = -1;
+    for (int sh = 0; sh < 30; ++sh) if ((1 << sh) == page_size) p.page_shift = sh;
+    p.block_table = block_table; p.max_pages = max_pages; p.positions = positions; p.qblk = qblk;
+    p.out = (__nv_bfloat16*)out; p.out_stride = out_stride; p.nh = nh; p.nkv = nkv; p.group = nh / nkv;
+    p.window = window; p.scale_log2 = scale * AT_LOG2E; p.status = status; p.sink_weight = sink_weight; p.shifts = (const int2*)shifts;
+    p.cap_log2 = softcap > 0.0f ? softcap * AT_LOG2E : 0.0f; p.cap_k = softcap > 0.0f ? 2.0f * AT_LOG2E * scale / softcap : 0.0f;
+    CUtensorMap map;
+    int rc = pt_pool_map_new(&map, kv_pool, num_pages, nkv, page_size, hd, CU_TENSOR_MAP_DATA_TYPE_FLOAT16);
+    if (rc != BG_OK) return rc;
+    const int reach = window != 0 ? abs(window) : max_position + 1;
+    const bool wide = (reach < max_position + 1 ? reach : max_position + 1) >= at_wide_from();
+    if (hd == 128) {
+        if (sink) return wide ? at_launch_half<128, 128, true>(map, p, n_qblk, stream) : at_launch_half<128, 64, true>(map, p, n_qblk, stream);
+        return wide ? at_launch_half<128, 128, false>(map, p, n_qblk, stream) : at_launch_half<128, 64, false>(map, p, n_qblk, stream);
+    }
+    if (sink) return wide ? at_launch_half<64, 128, true>(map, p, n_qblk, stream) : at_launch_half<64, 64, true>(map, p, n_qblk, stream);
+    return wide ? at_launch_half<64, 128, false>(map, p, n_qblk, stream) : at_launch_half<64, 64, false>(map, p, n_qblk, stream);
 }

@@ -215,8 +215,10 @@ _SIGNATURES = {
                        _c_void_p, _c_void_p],
     "bg_packed_bounds": [_c_void_p, _c_ll, _c_int, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_void_p, _c_void_p],
     "bg_packed_wide_page": [],
-    "bg_packed_unpack": [_c_void_p, _c_ll, _c_int, _c_int, _c_void_p, _c_void_p, _c_int, _c_int, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_int, _c_int,
-                         _c_int, _c_int, _c_void_p, _c_void_p],
+    "bg_packed_unpack": [_c_void_p, _c_ll, _c_int, _c_int, _c_void_p, _c_void_p, _c_int, _c_int, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_int,
+                         _c_int, _c_int, _c_int, _c_void_p, _c_void_p],
+    "bg_attention_tc_half": [_c_void_p, _c_int, _c_void_p, _c_int, _c_int, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_int,
+                             _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_void_p, _c_float, _c_void_p, _c_void_p],
     "bg_packed_attention_columns": [_c_int, _c_int, _c_int, ctypes.POINTER(_c_int)],
     "bg_packed_attention": [_c_void_p, _c_int, _c_ll, _c_void_p, _c_ll, _c_int, _c_int, _c_void_p, _c_int, _c_int, _c_void_p, _c_void_p, _c_int, _c_int,
                             _c_void_p, _c_int, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_float, _c_void_p, _c_int, _c_void_p,
@@ -958,7 +960,7 @@ def packed_rows(pool: torch.Tensor, positions: torch.Tensor, row_req: torch.Tens
                                 block_table.shape[0], _p(out), _dt(out), T, pool.shape[1], hd, _p(status), _stream()), "packed_rows")
 
 
-# Rows that a request brings from which its pages are written out in bfloat16 for the prompt attention.
+# Rows that a request brings from which its pages are written out in half precision for the prompt attention.
 PACKED_LONG_ROWS = 64
 
 
@@ -978,9 +980,10 @@ class PackedPlan:
         self.sizes, self.n_rows = (nh, nkv, hd, dtype, page_size), sum(lens)
         group, f32 = nh // nkv, dtype == torch.float32
         self.rows = max(1, (8 if f32 else 16) // group)        # rows of a block that the packed kernel takes
-        kernel, bq, tile = ("", 1, 0) if f32 else attention_plan(group, hd, torch.bfloat16, False, "auto", lib().bg_packed_wide_page())
-        self.kernel, self.tile, self.bq = kernel, tile, bq
-        long_from = PACKED_LONG_ROWS if kernel == "tc_rows" else 1 << 62
+        bq = _c_int(0)
+        wide = not f32 and lib().bg_attention_tc_plan(group, hd, lib().bg_packed_wide_page(), ctypes.byref(bq)) == 0
+        self.bq = bq = bq.value
+        long_from = PACKED_LONG_ROWS if wide else 1 << 62
         short, blocks, longs = [], [], []
         for i, (r0, n) in enumerate(zip(row_start, lens)):
             if n >= long_from:
@@ -1001,7 +1004,7 @@ class PackedPlan:
 def packed_plan(lens, nh: int, nkv: int, hd: int, dtype: torch.dtype, page_size: int, device, row_start=None, starts=None) -> PackedPlan:
     """The plan of `packed_attention` for a step whose request i brings lens[i] rows, from row row_start[i] on (default: one behind the other).  `starts`: the
     positions of their first rows, where the host knows them (less room is made then).  Requests of PACKED_LONG_ROWS rows and more (bfloat16) have their pages
-    written out in bfloat16 and run the prompt attention; the others' rows go in blocks of as many (row, query head) pairs as the kernel has columns."""
+    written out in half precision and run the prompt attention; the others' rows go in blocks of as many (row, query head) pairs as the kernel has columns."""
     lens = [int(n) for n in lens]
     if any(n < 0 for n in lens) or nh <= 0 or nkv <= 0 or nh % nkv:
         raise KernelError(f"packed_plan: rows {lens}, {nh} query heads for {nkv} kv heads")
@@ -1079,12 +1082,16 @@ def packed_attention(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Ten
             end = max_position + 1 if plan.long_end is None else min(plan.long_end, max_position + 1)
             size = L.bg_packed_wide_page()
             n_pages = max(1, -(-end // size))
-            wide = torch.empty((plan.n_long * n_pages, 2, nkv, size, hd), dtype=torch.bfloat16, device=q.device)
+            wide = torch.empty((plan.n_long * n_pages, 2, nkv, size, hd), dtype=torch.float16, device=q.device)
             table = torch.empty((plan.n_long, n_pages), dtype=torch.int32, device=q.device)
+            shifts = torch.empty((plan.n_long, nkv, 2), dtype=torch.int32, device=q.device)
             _check(L.bg_packed_unpack(_p(pool), block, pool.shape[0], page_size, _p(positions), _p(block_table), block_table.shape[1],
-                                      block_table.shape[0], _p(plan.longs), plan.n_long, _p(wide), _p(table), n_pages, window, nkv, hd, _p(status), _stream()), "packed_unpack")
-            _attention(q, q.stride(0), wide, table, positions, plan.blocks, plan.n_blocks, end - 1, T, nh, nkv, hd, window, 256, plan.tile, plan.bq, scale, out,
-                       status, plan.kernel, sink=sink, sink_weight=sink_weight, softcap=softcap)
+                                      block_table.shape[0], _p(plan.longs), plan.n_long, _p(wide), _p(table), _p(shifts), n_pages, window, nkv, hd,
+                                      _p(status), _stream()), "packed_unpack")
+            _check(L.bg_attention_tc_half(_p(q), q.stride(0), _p(wide), plan.n_long * n_pages, size, _p(table), n_pages, _p(positions), _p(plan.blocks),
+                                          plan.n_blocks, _p(shifts), _p(out), out.stride(0), nh, nkv, hd, window, float(scale), end - 1, 1 if sink else 0,
+                                          _p(sink_weight), float(softcap), _p(status), _stream()), "attention_tcgen05")
+            count_launches(1)
 
 
 def packed_select(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor, positions: torch.Tensor, nh: int, nkv: int, hd: int, page_size: int,

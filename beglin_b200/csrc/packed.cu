@@ -1,10 +1,13 @@
 // Writing and reading pages that hold keys and values in 4 bits (packed.cuh says how): the append of a step's rows with the rotation of queries and keys on
-// the way, rows read back, the smallest and largest values of a filled page's keys, and pages written out in bfloat16 for the prompt attention.
+// the way, rows read back, the smallest and largest values of a filled page's keys, and pages written out in half precision for the
+// prompt attention.
 //
 // A group of 64 features x becomes  lowest = bf16(min x),  step = bf16((max x - lowest) / 15),  u = clamp(round((x - lowest) / step), 0, 15).  The pair is
 // rounded before the codes are made, so that they are the nearest ones to what is read back: a value is off by half a step, and where rounding the pair cut
 // the range (by a part in 512) by that.  x is the rotated key in float, never rounded to bfloat16.  A group with a value that is not finite, or whose range is
 // not, is not a number throughout, as attention over it would be.  No result hangs on which thread wrote first: a position has one writer.
+#include <cuda_fp16.h>
+
 #include "packed.cuh"
 
 namespace bg {
@@ -273,20 +276,86 @@ __global__ void __launch_bounds__(PK_THREADS) packed_bounds_kernel(const PkBound
     }
 }
 
-// ------------------------------------------------------------------------------------------------ pages in bfloat16
+// ------------------------------------------------------------------------------------------------ pages in half precision
 struct PkUnpack {
     const unsigned char* pool; long long block_bytes;
     const int* positions; const int* block_table;
     const int* longs;                  // [n][3]: request, first row, rows
-    __nv_bfloat16* out;                // [n * pages, 2, nkv, PK_WIDE, HD]
+    __half* out;                       // [n * pages, 2, nkv, PK_WIDE, HD]
     int* table;                        // [n, pages]: their block table
+    int2* shifts;                      // [n][nkv]: keys are written times 2^-x, values times 2^-y
     int max_pages, num_pages, page_size, n_req, nkv, pages, window;
     unsigned* status;
 };
 
-// The positions that a request's rows read, written out as the bfloat16 cache holds them, in pages of PK_WIDE whatever the packed ones hold: page i of the n-th
-// request at n * pages + i.  A CTA takes a tile of 16 positions of one kv head; bound by the bytes written (heads of 128: 144 bytes read and 512 written a
-// position and kv head).  Positions behind the request's last are written as noughts: nobody reads them, and no number from nowhere stands there.
+// The page of a tile of 16 positions from `pos0` on that the n-th request's rows read, or -1 (and the status says where a page is not).
+__device__ __forceinline__ int unpack_page(const PkUnpack& p, int req, int pos0, int lo, int last, bool say) {
+    if (pos0 > last || pos0 + PK_TILE <= lo) return -1;            // (what lies in front of a window may have been given back)
+    const int index = pos0 / p.page_size;
+    const int page = index < p.max_pages && req >= 0 && req < p.n_req ? p.block_table[(size_t)req * p.max_pages + index] : -1;
+    if (page >= 0 && page < p.num_pages) return page;
+    if (say && p.status) atomicOr(p.status, BG_STATUS_BAD_PAGE);
+    return -1;
+}
+
+// How far the keys and the values of each (request, kv head) reach, from their (step, lowest) pairs alone: the power of two that brings the largest between
+// 2^14 and 2^15, so that half precision holds them whatever a model's scale is.  A cluster of CTAs takes a request's positions, a thread one at a time, several
+// on their way; the CTAs' maxima meet in the first one's shared memory.
+constexpr int PK_CLUSTER = 8;
+template <int HD>
+__global__ void __launch_bounds__(PK_THREADS) packed_reach_kernel(const PkUnpack p) {
+    constexpr int GROUPS = Packed<HD>::GROUPS, AT_ONCE = 4;
+    __shared__ float every[2][PK_CLUSTER];
+    __shared__ float scratch[32];
+    pdl_launch();
+    const int kvh = blockIdx.x, n = blockIdx.y, rank = blockIdx.z;
+    pdl_wait();
+    cluster_arrive_relaxed();                          // (the first CTA has begun before its memory is written)
+    cluster_wait();
+    const int req = p.longs[3 * n], row0 = p.longs[3 * n + 1], rows = p.longs[3 * n + 2];
+    const int last = p.positions[row0 + rows - 1], lo = first_visible(p.positions[row0], p.window);
+    float top[2] = {0.0f, 0.0f};
+    const int stride = PK_CLUSTER * PK_THREADS;
+    for (int pos0 = lo / PK_TILE * PK_TILE + rank * PK_THREADS + threadIdx.x; pos0 <= last; pos0 += AT_ONCE * stride) {
+        int page[AT_ONCE];
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) {
+            const int pos = pos0 + i * stride;
+            page[i] = pos <= last ? unpack_page(p, req, pos / PK_TILE * PK_TILE, lo, last, false) : -1;
+        }
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) {
+            if (page[i] < 0) continue;
+            const int at = (pos0 + i * stride) % p.page_size;
+            const unsigned* pair = reinterpret_cast<const unsigned*>(p.pool + ((size_t)page[i] * p.nkv + kvh) * p.block_bytes + (size_t)(at / PK_TILE) * Packed<HD>::TILE
+                                                                     + Packed<HD>::pair_word(at % PK_TILE, 0, 0));
+#pragma unroll
+            for (int e = 0; e < 2 * GROUPS; ++e) {
+                const float lowest = pair_lowest(pair[e]);
+                top[e / GROUPS] = fmaxf(top[e / GROUPS], fmaxf(fabsf(lowest), fabsf(fmaf(15.0f, pair_step(pair[e]), lowest))));
+            }
+        }
+    }
+#pragma unroll
+    for (int v = 0; v < 2; ++v) {
+        const float all = block_max(top[v], scratch);
+        if (threadIdx.x == 0) st_cluster(peer_addr(smem_u32(&every[v][rank]), 0), all);
+    }
+    cluster_sync_all();
+    if (rank || threadIdx.x) return;
+    int e[2];
+#pragma unroll
+    for (int v = 0; v < 2; ++v) {
+        float all = 0.0f;
+        for (int i = 0; i < PK_CLUSTER; ++i) all = fmaxf(all, every[v][i]);
+        e[v] = min(100, max(-100, (int)(__float_as_uint(all) >> 23) - 127 - 14));
+    }
+    p.shifts[(size_t)n * p.nkv + kvh] = make_int2(e[0], e[1]);
+}
+
+// The positions that a request's rows read, written out in half precision as the prompt attention takes them, in pages of PK_WIDE whatever the packed ones hold:
+// page i of the n-th request at n * pages + i.  A CTA takes a tile of 16 positions of one kv head; bound by the bytes written (heads of 128: 144 bytes read and
+// 512 written a position and kv head).  Positions behind the request's last are written as noughts: nobody reads them, and no number from nowhere stands there.
 constexpr int PK_WIDE = 64;
 template <int HD>
 __global__ void __launch_bounds__(PK_THREADS) packed_unpack_kernel(const PkUnpack p) {
@@ -298,25 +367,27 @@ __global__ void __launch_bounds__(PK_THREADS) packed_unpack_kernel(const PkUnpac
     const int req = p.longs[3 * n], row0 = p.longs[3 * n + 1], rows = p.longs[3 * n + 2];
     const int last = p.positions[row0 + rows - 1], lo = first_visible(p.positions[row0], p.window);
     if (wide > last / PK_WIDE || wide < lo / PK_WIDE) return;
-    const int index = pos0 / p.page_size;
-    const bool read = pos0 <= last && pos0 + PK_TILE > lo;         // (what lies in front of a window may have been given back)
-    const int page = read && index < p.max_pages && req >= 0 && req < p.n_req ? p.block_table[(size_t)req * p.max_pages + index] : -1;
-    const bool bad = page < 0 || page >= p.num_pages;
-    if (read && bad && p.status && threadIdx.x == 0) atomicOr(p.status, BG_STATUS_BAD_PAGE);
-    const unsigned char* from = p.pool + ((size_t)(bad ? 0 : page) * p.nkv + kvh) * p.block_bytes + (size_t)(pos0 % p.page_size / PK_TILE) * Packed<HD>::TILE;
-    __nv_bfloat16* to = p.out + (((size_t)n * p.pages + wide) * 2 * p.nkv + kvh) * PK_WIDE * HD + (size_t)(pos0 % PK_WIDE) * HD;
+    const int page = unpack_page(p, req, pos0, lo, last, threadIdx.x == 0);
+    const int2 shift = p.shifts[(size_t)n * p.nkv + kvh];
+    const unsigned char* from = p.pool + ((size_t)max(page, 0) * p.nkv + kvh) * p.block_bytes + (size_t)(pos0 % p.page_size / PK_TILE) * Packed<HD>::TILE;
+    __half* to = p.out + (((size_t)n * p.pages + wide) * 2 * p.nkv + kvh) * PK_WIDE * HD + (size_t)(pos0 % PK_WIDE) * HD;
 #pragma unroll
     for (int i0 = 0; i0 < PER; i0 += PK_THREADS) {
         const int i = i0 + threadIdx.x;
         const int value = i / (PK_TILE * WORDS), slot = i / WORDS % PK_TILE, f = i % WORDS * 8;
         float v[8] = {};
-        if (!bad && pos0 + slot <= last) {
+        if (page >= 0 && pos0 + slot <= last) {
             const unsigned pair = *reinterpret_cast<const unsigned*>(from + Packed<HD>::pair_word(slot, value, f / PK_GROUP));
             const unsigned word = *reinterpret_cast<const unsigned*>(from + (value ? Packed<HD>::value_word(slot, f) : Packed<HD>::key_word(slot, f)));
             if (value) packed_values<false>(word, pair, v);
             else packed_values<true>(word, pair, v);
         }
-        store8(to + (size_t)value * p.nkv * PK_WIDE * HD + (size_t)slot * HD + f, v);
+        const float down = __uint_as_float((unsigned)(127 - (value ? shift.y : shift.x)) << 23);
+        uint4 r;
+        __half2* h = reinterpret_cast<__half2*>(&r);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) h[e] = __floats2half2_rn(v[2 * e] * down, v[2 * e + 1] * down);
+        *reinterpret_cast<uint4*>(to + (size_t)value * p.nkv * PK_WIDE * HD + (size_t)slot * HD + f) = r;
     }
 }
 
@@ -386,16 +457,18 @@ extern "C" int bg_packed_bounds(unsigned char* pool, long long block_bytes, int 
 extern "C" int bg_packed_wide_page() { return PK_WIDE; }
 
 extern "C" int bg_packed_unpack(const unsigned char* pool, long long block_bytes, int num_pages, int page_size, const int* positions, const int* block_table,
-                                int max_pages, int n_req, const int* longs, int n, void* out, int* table, int pages, int window, int nkv, int hd,
+                                int max_pages, int n_req, const int* longs, int n, void* out, int* table, void* shifts, int pages, int window, int nkv, int hd,
                                 unsigned* status, cudaStream_t stream) {
     if (int e = packed_shape(hd, page_size, nkv, num_pages, block_bytes, false)) return e;
     if (n <= 0 || pages <= 0) return BG_OK;
     if (n > 65535 || (long long)n * pages > 0x7fffffffLL || pages > 0x7fffffff / PK_WIDE) return BG_ERR_SHAPE;
-    if ((uintptr_t)pool % 16 || (uintptr_t)out % 16) return BG_ERR_ALIGN;
-    const PkUnpack p = {pool, block_bytes, positions, block_table, longs, (__nv_bfloat16*)out, table, max_pages, num_pages, page_size, n_req, nkv, pages,
+    if ((uintptr_t)pool % 16 || (uintptr_t)out % 16 || (uintptr_t)shifts % 8) return BG_ERR_ALIGN;
+    const PkUnpack p = {pool, block_bytes, positions, block_table, longs, (__half*)out, table, (int2*)shifts, max_pages, num_pages, page_size, n_req, nkv, pages,
                         window, status};
-    const dim3 grid(pages * (PK_WIDE / PK_TILE), nkv, n);
-    cudaError_t e = hd == 64 ? launch(packed_unpack_kernel<64>, grid, dim3(PK_THREADS), 0, stream, p)
-                             : launch(packed_unpack_kernel<128>, grid, dim3(PK_THREADS), 0, stream, p);
+    const dim3 heads(nkv, n, PK_CLUSTER), tiles(pages * (PK_WIDE / PK_TILE), nkv, n);
+    cudaError_t e = hd == 64 ? launch_cluster(packed_reach_kernel<64>, heads, dim3(PK_THREADS), 0, stream, PK_CLUSTER, p)
+                             : launch_cluster(packed_reach_kernel<128>, heads, dim3(PK_THREADS), 0, stream, PK_CLUSTER, p);
+    if (e != cudaSuccess) return (int)e;
+    e = hd == 64 ? launch(packed_unpack_kernel<64>, tiles, dim3(PK_THREADS), 0, stream, p) : launch(packed_unpack_kernel<128>, tiles, dim3(PK_THREADS), 0, stream, p);
     return e == cudaSuccess ? BG_OK : (int)e;
 }

@@ -14,25 +14,30 @@ namespace bg {
 // Whether pages of this size can be copied as boxes into tiles of 64 keys.
 inline bool pt_page_size_ok(int page_size) { return page_size >= 1 && page_size <= 64 && 64 % page_size == 0; }
 
-// The tensor map of a pool, made once per (pointer, shape) and kept.
+// The tensor map of a pool of 16-bit values.
+inline int pt_pool_map_new(CUtensorMap* out, const void* pool, int num_pages, int nkv, int page_size, int hd, CUtensorMapDataType type) {
+    const EncodeTiledFn fn = encode_fn();
+    if (!fn || !pt_page_size_ok(page_size) || hd % 64 != 0) return BG_ERR_UNSUPPORTED;
+    cuuint64_t dims[2] = {(cuuint64_t)hd, (cuuint64_t)num_pages * 2 * nkv * page_size};
+    cuuint64_t strides[1] = {(cuuint64_t)hd * 2};
+    cuuint32_t box[2] = {64, (cuuint32_t)page_size};
+    cuuint32_t elem[2] = {1, 1};
+    const CUresult r = fn(out, type, 2, const_cast<void*>(pool), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? BG_OK : BG_ERR_SHAPE;
+}
+
+// The same in bfloat16, made once per (pointer, shape) and kept.
 inline int pt_pool_map(CUtensorMap* out, const void* pool, int num_pages, int nkv, int page_size, int hd) {
     static std::mutex mu;
     static std::map<std::tuple<const void*, int, int, int, int>, CUtensorMap> maps;
-    const EncodeTiledFn fn = encode_fn();
-    if (!fn || !pt_page_size_ok(page_size) || hd % 64 != 0) return BG_ERR_UNSUPPORTED;
     std::lock_guard<std::mutex> g(mu);
     const auto key = std::make_tuple(pool, num_pages, nkv, page_size, hd);
     auto it = maps.find(key);
     if (it == maps.end()) {
         CUtensorMap map;
-        cuuint64_t dims[2] = {(cuuint64_t)hd, (cuuint64_t)num_pages * 2 * nkv * page_size};
-        cuuint64_t strides[1] = {(cuuint64_t)hd * 2};
-        cuuint32_t box[2] = {64, (cuuint32_t)page_size};
-        cuuint32_t elem[2] = {1, 1};
-        CUresult r = fn(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(pool), dims, strides, box, elem,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-        if (r != CUDA_SUCCESS) return BG_ERR_SHAPE;
+        const int rc = pt_pool_map_new(&map, pool, num_pages, nkv, page_size, hd, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16);
+        if (rc != BG_OK) return rc;
         it = maps.emplace(key, map).first;
     }
     *out = it->second;

@@ -468,11 +468,31 @@ def test_attention_of_portions(parts, nh, nkv, hd, page, dtype, options):
         ops.raise_on_status(status)
         assert bool((out[len(rows):] == 7.0).all())                            # rows behind the last are left as they were
         got = out[:len(rows)].view(-1, nh, hd)
-        if plan.n_long:                                # (their keys and values are rounded to bfloat16: 2^-9 of up to 3.5 a value and, through the scores, a weight)
-            off = (got.double().cpu() - want).abs()
-            assert float(off.max()) < 0.05 and float(off.norm() / want.norm()) < 2.0 ** -7
-        else:
-            near(got, want, dtype)
+        # (those of many rows: keys, values and weights in halves, 2^-11 each, well inside what the weights' bfloat16 takes)
+        near(got, want, dtype)
+
+
+@GPU
+@pytest.mark.parametrize("key,value,query", [(1e-12, 1e-20, 1e9), (3e6, 1e7, 1e-6), (1e20, 1e30, 1e-20), (1.0, 1e-30, 1.0)])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_portions_over_keys_and_values_of_any_scale(key, value, query, hd):
+    """Half precision holds the written-out pages by a power of two for each kv head."""
+    nh, nkv, page, n = 4, 2, 32, 100
+    table, pages = make_table([n], page)
+    pool = make_pool(pages, nkv, hd, page, seed=3)
+    pairs = pool.unflatten(2, (page // 16, -1))[..., 16 * hd:].view(BF16).unflatten(3, (16, 2, hd // 64, 2))
+    pairs[..., 0, :, :] *= key
+    pairs[..., 1, :, :] *= value
+    pairs[:, 1] *= 0.01                                                        # the second kv head's scale is another
+    poison(pool, table, [n], hd, page)
+    q = (torch.randn((n, nh * hd), generator=torch.Generator().manual_seed(2)) * query / (key * query)).to(BF16)
+    out, status = torch.empty((n, nh * hd), dtype=BF16, device="cuda"), ops.new_status("cuda")
+    ops.packed_attention(q.cuda(), pool.cuda(), table.cuda(), torch.arange(n, dtype=torch.int32, device="cuda"), nh, nkv, hd, page, n - 1, 1 / math.sqrt(hd), out, status,
+                         plan=ops.packed_plan([n], nh, nkv, hd, BF16, page, "cuda"))
+    ops.raise_on_status(status)
+    want = plain_attention(q.view(n, nh, hd), pool, table, hd, page, [(0, i) for i in range(n)], 1 / math.sqrt(hd))
+    for heads, scale in ((slice(0, 2), value), (slice(2, 4), value * 0.01)):
+        near(out.view(n, nh, hd)[:, heads].double() / scale, want[:, heads] / scale, BF16)
 
 
 # ------------------------------------------------------------------------------------------------ the choice of pages
