@@ -199,7 +199,7 @@ class CacheManager:
     def allocate(self, device, dtype: torch.dtype) -> None:
         for g in self.kv_groups:
             g.device_pool = torch.empty((len(g.stages), self.num_pages + 1) + tuple(g.need.page_shape(self.page_size)),
-                                        dtype=dtype, device=device)
+                                        dtype=getattr(torch, g.need.dtype) if hasattr(g.need, "dtype") else dtype, device=device)
             g.device_pool[:, self.dump_page].zero_()
         for g in self.state_groups:
             g.slab = torch.zeros((len(g.stages), self.max_requests + 1) + tuple(g.need.shape),
@@ -305,7 +305,7 @@ class CacheManager:
             table = g.tables[rid]
             if rest and new_rids and g.device_pool is not None and table[whole] >= 0:
                 for part in g.need.page_parts(g.device_pool, self.page_size):
-                    ops().copy_pages(part, [table[whole]] * len(new_rids), [g.tables[new][whole] for new in new_rids], rest)
+                    ops().copy_pages(part, [table[whole]] * len(new_rids), [g.tables[new][whole] for new in new_rids], min(rest, part.shape[-2]))
         for g in self.state_groups:
             if g.slab is not None and new_rids:
                 flat = g.slab.view(g.slab.shape[0], g.slab.shape[1], 1, -1)

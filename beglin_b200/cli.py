@@ -20,7 +20,8 @@ comparison of the two orders, qwen_infer.c:20690), QWEN_HF_CONFIG (a config.json
 the model folder, :20121), QWEN_PROF (1: in `bench` and `greedy`, device time per kernel class from CUDA events,
 printed with the share of the total that the classes add up to, :1224-1235 and :20463-20486; the steps then
 run kernel by kernel, not as replayed graphs).
-Added: QWEN_DTYPE (bf16 | fp32, default bf16), QWEN_TEMPERATURE and QWEN_SEED (sampling),
+QWEN_KV_INT4 (1: keys and values in 4 bits).
+Added: QWEN_SPARSE_PAGES (n: single tokens read at most n pages of such a cache for each kv head), QWEN_DTYPE (bf16 | fp32, default bf16), QWEN_TEMPERATURE and QWEN_SEED (sampling),
 QWEN_PAGE_SIZE (default 64), QWEN_NUM_PAGES, QWEN_RANDOM (a seed: write random weights for
 <QWEN_BASE>/config.json first, if the folder has no model.safetensors), QWEN_DUMP_DIR.
 """
@@ -152,7 +153,8 @@ def main(argv: List[str]) -> int:
     num_pages = _env_int("QWEN_NUM_PAGES", live * -(-maxseq // page))
     try:
         eng = Engine.from_folder(base, config_path=config_path, dtype=dtype, max_tokens=num_pages * page, page_size=page,
-                                 max_requests=live, max_context=maxseq, use_graphs=not prof)
+                                 max_requests=live, max_context=maxseq, use_graphs=not prof,
+                                 cache_bits=4 if _env_int("QWEN_KV_INT4", 0) else 16, sparse_pages=_env_int("QWEN_SPARSE_PAGES", 0))
     except Exception as e:                                   # one line, as the reference's FATALs
         return _err(str(e))
     print(f"[engine] arch config ({config_path}): {describe(eng.spec)} MAXSEQ={maxseq} DTYPE={dtype}", file=sys.stderr)

@@ -108,6 +108,13 @@ class StepBatch:
             self.scratch[key] = plan if plan.shares else None
         return self.scratch[key]
 
+    def packed_plan(self, nh: int, nkv: int, hd: int, dtype, page_size: int):
+        """The plan of `ops.packed_attention` for this step's rows."""
+        key = ("packed", nh, nkv, hd, dtype, page_size)
+        if key not in self._qblk:
+            self._qblk[key] = ops.packed_plan(self.lens, nh, nkv, hd, dtype, page_size, self.device, row_start=self.row_start, starts=self.starts)
+        return self._qblk[key]
+
     def long_blocks(self, bq: int, min_rows: int):
         """`cut_long_requests` of this step on the device: (short, n, blocks, n, longs, n), one upload."""
         key = ("long", bq, min_rows)

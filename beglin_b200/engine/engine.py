@@ -17,6 +17,7 @@ import torch
 from ..cache.manager import CacheManager
 from ..config import load_config
 from ..csrc import ops
+from ..parts.cache_need import CompositeNeed, PagedPackedNeed
 from ..parts.context import BuildContext
 from ..sampling.rules import LogitRules
 from ..sampling.sampler import Sampler, uniform
@@ -54,17 +55,21 @@ class Engine:
     def __init__(self, spec, tensors, *, dtype="bfloat16", device="cuda:0", max_tokens: int = 8192,
                  page_size: int = 64, max_requests: int = 8, max_context: Optional[int] = None,
                  kv_split: int = 256, gemm: str = "auto", attention: str = "auto", fuse: bool = True,
-                 use_graphs: bool = True, portion_graph_rows: int = 256, config=None, origin: str = ""):
+                 use_graphs: bool = True, portion_graph_rows: int = 256, cache_bits: int = 16, sparse_pages: int = 0, config=None, origin: str = ""):
         """`tensors` is anything with names()/shape(name)/tensor(name): a Checkpoint or a TensorDict.
         `max_tokens` sizes the page pool: it holds that many positions (rounded up to whole pages).
         With `use_graphs`, decoding steps and portions of one request of at least `portion_graph_rows`
-        tokens whose shape comes again are replayed as CUDA graphs."""
+        tokens whose shape comes again are replayed as CUDA graphs.
+
+        `cache_bits` 4: the layers of plain grouped-query attention with heads of 64 or 128 features hold their keys and values in 4 bits (4.5 with what
+        goes with a group of 64 features), the others in the compute type; a model without such a layer is refused.  `sparse_pages` n: a single token
+        reads, in such a layer without a window and for each kv head, at most n pages of its request: the first, the last two and those whose keys can score highest."""
         self.device = require_gpu(device)
         self.dtype = parse_dtype(dtype)
         self.spec, self.config = spec, config
         bound = bind(spec, tensors, origin)
         self.ctx = BuildContext(device=self.device, compute_dtype=self.dtype, page_size=page_size,
-                                kv_split=kv_split, gemm=gemm, attention=attention, fuse=fuse)
+                                kv_split=kv_split, gemm=gemm, attention=attention, fuse=fuse, cache_bits=cache_bits, sparse_pages=sparse_pages)
         with torch.cuda.device(self.device):
             self.model = DecoderModel(spec, bound, self.ctx)
             del bound
@@ -72,7 +77,11 @@ class Engine:
             limit = max_context if max_context is not None else num_pages * page_size
             if spec.max_positions:
                 limit = min(limit, spec.max_positions)
-            self.cache = CacheManager(self.model.cache_needs(), page_size, num_pages, max_requests, limit)
+            needs = self.model.cache_needs()
+            if cache_bits == 4 and not any(isinstance(n, PagedPackedNeed) for need in needs for n in (need.needs if isinstance(need, CompositeNeed) else (need,))):
+                raise ValueError("cache_bits=4: no layer of this model holds keys and values that way (plain grouped-query attention, heads of 64 or 128 features, "
+                                 f"pages of a multiple of {ops.PACKED_TILE} positions)")
+            self.cache = CacheManager(needs, page_size, num_pages, max_requests, limit)
             self.cache.allocate(self.device, self.dtype)
         self.sampler = Sampler(self.device, self.ctx.status)
         self.vocab = spec.vocab

@@ -72,6 +72,12 @@ class _StaticPortion:
         return hit
 
 
+    def packed_plan(self, nh: int, nkv: int, hd: int, dtype, page_size: int):
+        key = ("packed", nh, nkv, hd, dtype, page_size)
+        if key not in self._qblk:              # (made by the warm-up: it stays for the capture)
+            self._qblk[key] = ops.packed_plan(self.lens, nh, nkv, hd, dtype, page_size, self.device)
+        return self._qblk[key]
+
     def long_blocks(self, bq: int, min_rows: int):
         key = ("long", bq, min_rows)
         hit = self._qblk.get(key)

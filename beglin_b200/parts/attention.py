@@ -16,6 +16,9 @@ product of the mixer's input, on the joined heads before the output product, fea
 one more block of rows of the one q/k/v product.  With any of the first two the kernel that norms, rotates and appends
 is `qk_norm_rope_append`.
 
+Where the build asks for a cache in 4 bits, the plain form's keys and values are held so (`ops.packed_append`, `ops.packed_attention`), and single tokens may
+read the pages that can score highest alone (`ops.packed_select`).  (The reference has caches of 8 and of 4 bits, qwen_infer.c:810-1209.)
+
 A step of single tokens whose requests hold their first positions in the same pages (requests that go on from one text) reads those once for all of
 them (`shared_attention`), where a query sees every position.
 """
@@ -28,7 +31,7 @@ import numpy as np
 import torch
 
 from ..csrc import ops
-from .cache_need import PagedKVNeed, PagedKVView
+from .cache_need import PagedKVNeed, PagedKVView, PagedPackedNeed
 from .context import BuildContext
 from .linear import Linear
 from .registry import register_mixer
@@ -84,14 +87,28 @@ class GQAAttention:
         return stored if max(hd, vd) <= 128 and stored <= hd + vd else None
 
     @staticmethod
-    def cache_need(spec: AttentionSpec, ctx: Optional[BuildContext] = None) -> Optional[PagedKVNeed]:
+    def packs(spec: AttentionSpec, ctx: Optional[BuildContext]) -> bool:
+        """Whether the layer holds its keys and values in 4 bits: where that is asked for and the layer is the plain form (windows, squashed scores and sinks
+        may be) with heads of 64 or 128 features and pages of whole tiles."""
+        return ctx is not None and ctx.cache_bits == 4 and spec.own_kv and spec.qk_norm is None and spec.value_dim == spec.head_dim and spec.gate is None \
+            and spec.slopes is None and spec.block is None and not spec.keep_first and spec.head_dim in (64, 128) and ctx.page_size % ops.PACKED_TILE == 0
+
+    @staticmethod
+    def cache_need(spec: AttentionSpec, ctx: Optional[BuildContext] = None):
         if not spec.own_kv:
             return None
+        if GQAAttention.packs(spec, ctx):
+            return PagedPackedNeed(spec.n_kv_heads, spec.head_dim, spec.window, GQAAttention.chooses(spec, ctx))
         stored = GQAAttention.stored_head(spec, ctx)
         if stored is not None:
             return PagedKVNeed(spec.n_kv_heads, stored, spec.window, None, spec.block, spec.keep_first)
         return PagedKVNeed(spec.n_kv_heads, spec.head_dim, spec.window,
                            None if spec.value_dim == spec.head_dim else spec.value_dim, spec.block, spec.keep_first)
+
+    @staticmethod
+    def chooses(spec: AttentionSpec, ctx: BuildContext) -> bool:
+        """Whether single tokens read the pages that score highest alone (a window is short already)."""
+        return ctx.sparse_pages > 0 and spec.window is None
 
     def __init__(self, spec: AttentionSpec, tensors: Dict[str, torch.Tensor], ctx: BuildContext):
         if spec.n_heads % spec.n_kv_heads:
@@ -157,21 +174,23 @@ class GQAAttention:
         # where only the decoding kernel takes the sizes on the tensor cores, it is ahead of the float units' sharing, whose blocks of one row share nothing
         self.shared_kernel = dict(page_size=ctx.page_size, vd=kvd_, prefer="generic" if ctx.attention == "generic" else "auto", query_dtype=ctx.compute_dtype)
         kernel, rows, _ = ops.shared_kernel(self.nh, self.nkv, khd, ctx.cache_dtype, **self.shared_kernel)
-        self.reads_shared = spec.window is None and spec.block is None and spec.slopes is None \
+        self.packed = self.packs(spec, ctx)
+        self.sparse_pages = ctx.sparse_pages if self.packed and self.chooses(spec, ctx) else 0
+        self.reads_shared = not self.packed and spec.window is None and spec.block is None and spec.slopes is None \
             and (kernel == "tc" or rows > 1 and self.plans[True][0] == "generic")
         ctx.reads_shared |= self.reads_shared
         # the fused q/k/v product can rotate and append itself: whole heads rotated in halves, a cache of its own
         # in bfloat16
         self.rope_in_product = (spec.own_kv and self.position.rotary_dim == self.hd and not self.position.interleaved
                                 and ctx.compute_dtype == torch.bfloat16 and ctx.cache_dtype == torch.bfloat16
-                                and not self.extended)
+                                and not self.extended and not self.packed)
 
         self._args = self._step_args()
 
     def _step_args(self):
         """The layer as the one-call float step takes it, for each of its two plans (portions, single tokens), or None: the plain form in float32."""
         s, ctx = self.spec, self.ctx
-        if ctx.compute_dtype != torch.float32 or ctx.cache_dtype != torch.float32 or self.extended or not s.own_kv or self.stored is not None \
+        if self.packed or ctx.compute_dtype != torch.float32 or ctx.cache_dtype != torch.float32 or self.extended or not s.own_kv or self.stored is not None \
                 or any(plan[0] != "generic" for plan in self.plans.values()):
             return None
         ptr = lambda t: None if t is None else t.data_ptr()
@@ -186,13 +205,25 @@ class GQAAttention:
             return None
         return batch.shared_plan(self.nh, self.nkv, self.stored or self.hd, self.ctx.cache_dtype, split=self.ctx.kv_split, **self.shared_kernel)
 
+    def _packed_attention(self, q, out, batch, cache: PagedKVView) -> None:
+        sizes, pages = (self.nh, self.nkv, self.hd), None
+        plan = None if batch.decode_only else batch.packed_plan(*sizes, self.ctx.compute_dtype, cache.page_size)
+        if plan is None and 0 < self.sparse_pages <= batch.max_position // cache.page_size:
+            pages = torch.empty((q.shape[0], self.nkv, self.sparse_pages), dtype=torch.int32, device=q.device)
+            ops.packed_select(q, cache.pool, cache.block_table, batch.positions, *sizes, cache.page_size, batch.max_position, pages, self.ctx.status, first=1, recent=2)
+        ops.packed_attention(q, cache.pool, cache.block_table, batch.positions, *sizes, cache.page_size, batch.max_position, self.scale, out, self.ctx.status, plan=plan,
+                             window=self.window, softcap=self.score_cap, sink=bool(self.spec.sink), sink_weight=self.sink_weight, pages=pages)
+
     takes_stream = True        # forward takes a NormedInput and may add its result to the stream itself
 
     def forward(self, h, batch, cache: PagedKVView, stream: Optional[ResidualStream] = None) -> Optional[torch.Tensor]:
         """h: the normed rows, or a NormedInput.  With `stream` the result is added to it (or left owed to
         it) and None is returned; without, the addend is returned."""
         T = batch.n_rows
-        shared = self._shared_plan(batch)
+        packed = cache.pool.dtype == torch.uint8       # its own pages, or those of the layer that it reads
+        if packed and (self.spec.block is not None or self.spec.keep_first or self.extended):
+            raise ValueError("a cache in 4 bits is read by plain attention, with a window or without")
+        shared = None if packed else self._shared_plan(batch)
         if self._args is not None and shared is None and not ops.profiling():
             rows = h if isinstance(h, torch.Tensor) else h.tensor()
             args = self._args[bool(getattr(batch, "decode_only", False))]
@@ -218,6 +249,13 @@ class GQAAttention:
                                     self.position.table(batch), batch.positions, batch.row_req, cache.block_table,
                                     cache.pool, cache.page_size, self.ctx.status, stored=self.stored,
                                     per_head=self.spec.qk_norm == "head")
+        elif self.packed:
+            qkv = self.qkv.of(h)
+            q = torch.empty((T, self.qd), dtype=self.ctx.compute_dtype, device=qkv.device)
+            ops.packed_append(qkv, q, self.nh, self.nkv, self.hd, self.position.rotary_dim, self.position.interleaved, self.position.table(batch),
+                              batch.positions, batch.row_req, cache.block_table, cache.pool, cache.page_size, self.ctx.status)
+            if self.sparse_pages:
+                ops.packed_bounds(cache.pool, batch.positions, batch.row_req, cache.block_table, self.hd, cache.page_size, self.ctx.status)
         elif self.rope_in_product and self.qkv.rope_fuses(T, self.hd):
             # a step of few tokens: rotation and cache append inside the q/k/v product
             q = torch.empty((T, self.qd), dtype=self.ctx.compute_dtype, device=self.ctx.device)
@@ -230,7 +268,9 @@ class GQAAttention:
                                self.position.table(batch), batch.positions, batch.row_req, cache.block_table,
                                cache.pool if self.spec.own_kv else None, cache.page_size, self.ctx.status)
         out = torch.empty((T, self.nh * kvd_), dtype=self.ctx.compute_dtype, device=q.device)
-        if shared is not None:
+        if packed:
+            self._packed_attention(q, out, batch, cache)
+        elif shared is not None:
             ops.shared_attention(q, cache.pool, cache.block_table, batch.positions, shared, batch.max_position, self.scale, out, self.ctx.status,
                                  sink=bool(self.spec.sink), sink_weight=self.sink_weight, softcap=self.score_cap)
         else:

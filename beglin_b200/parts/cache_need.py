@@ -45,6 +45,27 @@ class PagedKVNeed:
 
 
 @dataclass(frozen=True)
+class PagedPackedNeed:
+    """Keys and values of every position (or of the last `window`) in 4 bits, as `ops.packed_append` writes them: a page is bytes.  `bounds`: with the smallest
+    and largest value of every feature of a filled page's keys."""
+    n_kv_heads: int
+    head_dim: int
+    window: Optional[int] = None
+    bounds: bool = False
+    block = None               # (what the other needs have and this one does not)
+    keep_first = 0
+    dtype = "uint8"            # whatever the cache's type is
+
+    def page_shape(self, page_size: int) -> Tuple[int, ...]:
+        from ..csrc import ops
+        return (self.n_kv_heads, ops.packed_page_bytes(self.head_dim, page_size, self.bounds))
+
+    def page_parts(self, pool: torch.Tensor, page_size: int) -> List[torch.Tensor]:
+        """Positions of a page do not lie one behind the other: a page is copied as a whole."""
+        return [pool.flatten(2)[:, :, None, None]]
+
+
+@dataclass(frozen=True)
 class PagedLatentNeed:
     """ONE row of `width` features per position, shared by all heads (the latent of an attention that makes
     its keys and values from a low-rank projection, with whatever rides along, such as a rotated key part)."""
@@ -59,7 +80,7 @@ class PagedLatentNeed:
         return [pool]
 
 
-PAGED_NEEDS = (PagedKVNeed, PagedLatentNeed)
+PAGED_NEEDS = (PagedKVNeed, PagedPackedNeed, PagedLatentNeed)
 
 
 @dataclass(frozen=True)
@@ -80,7 +101,7 @@ class CompositeNeed:
 @dataclass
 class PagedKVView:
     """One stage's pages, [num_pages, 2, n_kv_heads, page_size, head_dim] (2 = keys, values) for keys and values
-    or [num_pages, page_size, width] for a latent, and the step's block table [requests, max_pages] (int32, -1
+    or [num_pages, page_size, width] for a latent (uint8 [num_pages, n_kv_heads, bytes] for keys and values in 4 bits), and the step's block table [requests, max_pages] (int32, -1
     where no page is held)."""
     pool: torch.Tensor
     block_table: torch.Tensor

@@ -23,6 +23,8 @@ class BuildContext:
     # few-token steps: norms, residual adds, SwiGLU, rotation and cache append inside the products.  True: where it was
     # measured to pay; "all": wherever the sizes allow it (tests of the fused kernels on tiny models); False: nowhere
     fuse: object = True
+    cache_bits: int = 16                    # 4: plain grouped-query layers hold keys and values in 4 bits (the others as they are)
+    sparse_pages: int = 0                   # pages that a single token reads for each kv head, where the cache is in 4 bits; 0: all
     status: Optional[torch.Tensor] = None   # device word in which kernels record bad ids and pages
     reads_shared: bool = False              # whether a layer reads positions that requests share once for all of them
     shared: Dict[object, object] = field(default_factory=dict)   # parts shared between layers, by spec
@@ -33,6 +35,10 @@ class BuildContext:
             raise ValueError(f"compute dtype must be float32 or bfloat16, got {self.compute_dtype}")
         if self.cache_dtype is None:
             self.cache_dtype = self.compute_dtype
+        if self.cache_bits not in (4, 16):
+            raise ValueError(f"cache_bits={self.cache_bits}: 4, or 16 for the compute type")
+        if self.sparse_pages and (self.sparse_pages < 4 or self.cache_bits != 4):
+            raise ValueError(f"sparse_pages={self.sparse_pages}: four pages at least (the first, the last two and chosen ones), of a cache in 4 bits")
         if self.kv_split % 64 != 0:
             raise ValueError("kv_split must be a multiple of 64")
 
