@@ -1043,8 +1043,8 @@ def packed_attention(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Ten
         raise KernelError(f"packed_attention: queries of {q.dtype} and results of {out.dtype}")
     if nkv <= 0 or nh % nkv:
         raise KernelError(f"packed_attention: {nh} query heads for {nkv} kv heads")
-    if window < 0 or softcap < 0.0:
-        raise KernelError("packed_attention: a sliding window or none, a positive bound of the scores or none")
+    if window < 0 or not softcap >= 0.0 or not scale > 0.0:
+        raise KernelError("packed_attention: a sliding window or none, a positive bound of the scores or none, a positive scale")
     if sink_weight is not None:
         sink = True
         if sink_weight.dtype != torch.float32 or sink_weight.numel() != nh or not sink_weight.is_contiguous():

@@ -1,14 +1,20 @@
 // Attention over pages that hold keys and values in 4 bits (packed.cuh), for single tokens and short runs of rows: softmax(q K^T scale) V with
 // K = lowest + step u, never written out.
 //
-// Both products run as mma.sync m16n8k16 with the CODES as the left operand: a code u becomes the bfloat16 128 + u by two bit operations (0x4300 | u), which
-// is exact, and (step, lowest) are applied in float outside the product:
-//     q . k   = sum over groups of  step (sum q (128 + u)) + (lowest - 128 step) (sum q)
-//     p V     = sum over positions of  (p step) (128 + u) - 128 (p step) + p lowest
-// so that the only rounding of the cache's side is that of p step to bfloat16 (-128 (p step) is a product with a constant left operand, of the same rounded
-// numbers).  Keys: 16 positions by 16 features times features by 8 columns; values: 16 features by 16 positions times positions by columns.  A column is one
-// (row, query head): the queries of a kv head are the narrow side, so 8 heads waste nothing of the product and a code is unpacked once for all of them.  The
-// weights reach the second product's layout through movmatrix.  With float queries the codes are made exact (u), and queries and weights go in three bfloat16 parts.
+// Both products run as mma.sync m16n8k16 with the CODES as the left operand.  The low byte of a bfloat16 whose upper byte is nought stands for itself times
+// 2^-133 (exponents 0 and 1 share a unit), so a code needs no conversion: masked out of its word at bits 0 or 4 it IS the number u 2^-133 or 16 u 2^-133, and
+// the right operand is scaled up by powers of two to meet it (two masks, a shift by 8, two masks: five operations for 8 codes; as 128 + u, 0x4300 | u, which
+// needs every code at bit 0, it took seven, a product more for the 128 and, over 131,072 positions, a third of the result's last digit).  (step, lowest)
+// are applied in float outside the product:
+//     q . k   = sum over groups of  step (sum q u) + lowest (sum q)
+//     p V     = sum over positions of  (p step) u + p lowest
+// so that the only rounding of the cache's side is that of p step to bfloat16.  Keys: 16 positions by 16 features times features by 8 columns; values: 16
+// features by 16 positions times positions by columns.  A column is one (row, query head): the queries of a kv head are the narrow side, so 8 heads waste
+// nothing of the product and a code is unpacked once for all of them.  The weights reach the second product's layout through movmatrix.  Float queries and
+// weights go in three bfloat16 parts.
+//
+// Ranges: a row of queries is scaled by the power of two that brings its largest to 2^100.  Weights carry 2^64, so values may have steps up to 2^63, and those
+// under 2^-50 lose digits.
 //
 // Why this shape: at the bandwidth of HBM a position of a kv head (144 bytes for heads of 128) has to be done in some 6 cycles of an SM, 25 warp instructions.  The
 // left operand by codes takes about 15 for 8 columns; with the queries on the left (16 rows, half of them empty) it took the tensor cores twice the products
@@ -52,15 +58,10 @@ __device__ __forceinline__ unsigned pa_pack(float a, float b) {
     __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<unsigned*>(&h);
 }
-// The pair of codes at bits 4 i of both halves as bfloat16: 128 + u, or with EXACT u itself.
-template <bool EXACT>
-__device__ __forceinline__ unsigned pa_codes(unsigned w, int i) {
-    const unsigned v = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
-    if constexpr (!EXACT) return v;
-    const __nv_bfloat162 k = __halves2bfloat162(__ushort_as_bfloat16(0x4300), __ushort_as_bfloat16(0x4300));
-    __nv_bfloat162 h = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), k);
-    return *reinterpret_cast<unsigned*>(&h);
-}
+constexpr float PA_UP = 64.0f;                         // weights are 2^(x - maximum + PA_UP)
+constexpr unsigned PA_ONE = 0x00010001u;               // the code 1 of two features, at bits 0
+// The pair of codes at bits 4 i of both halves of a word: u 2^-133 where i is even, 16 u 2^-133 where it is odd.
+__device__ __forceinline__ unsigned pa_codes(unsigned w, int i) { return (i < 2 ? w : w >> 8) & (i % 2 ? 0x00f000f0u : 0x000f000fu); }
 __device__ __forceinline__ void pa_bulk_load(void* dst, const void* src, unsigned bytes, unsigned long long* bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n"
                  ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
@@ -70,14 +71,13 @@ __device__ __forceinline__ float pa_exp2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
     return y;
 }
-// A score as the exponent of two that the softmax takes.
-template <bool EXACT>
-__device__ __forceinline__ float pa_score(float s, const PaParams& p) {
-    if (!(p.cap_log2 > 0.0f)) return s * p.scale_log2;
-    if constexpr (EXACT) return p.cap_log2 * tanhf(s * p.scale_over_cap);
+// c log2(e) tanh(x / c) of x / c.
+template <bool F32>
+__device__ __forceinline__ float pa_squashed(float x, float cap_log2) {
+    if constexpr (F32) return cap_log2 * tanhf(x);
     float r;                                           // tanh x = 1 - 2 / (1 + e^(2 x))
-    asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(1.0f + pa_exp2(s * p.scale_over_cap * (2.0f * PA_LOG2E))));
-    return p.cap_log2 * fmaf(-2.0f, r, 1.0f);
+    asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(1.0f + pa_exp2(x * (2.0f * PA_LOG2E))));
+    return cap_log2 * fmaf(-2.0f, r, 1.0f);
 }
 
 template <int HD, int NT, bool F32>
@@ -124,96 +124,105 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
 
     // ---- copies: a lane looks up the page of one of the warp's next 32 turns
     unsigned char* ring = smem + (size_t)warp * PA_STAGES * BYTES;
-    int page = -1, base = 0;
-    auto issue = [&](int turn) {
-        if (turn >= turns) return;
-        if ((turn & 31) == 0) {
-            const int c = begin + (turn + lane) * PA_WARPS;
-            page = -1;
-            if (c < end) {
-                int index;
-                if (list) {
-                    index = list[c / per_page];
-                    base = index * p.page_size + c % per_page * KEYS;
-                } else {
-                    base = (chunk0 + c) * KEYS;
-                    index = base / p.page_size;
-                }
-                if (index >= 0 && base <= pos_last) {
-                    page = index < p.max_pages && req >= 0 && req < p.n_req ? p.table[(size_t)req * p.max_pages + index] : -1;
-                    if (page < 0 || page >= p.num_pages) {
-                        page = -1;
-                        if (p.status) atomicOr(p.status, BG_STATUS_BAD_PAGE);
-                    }
-                }
-            }
+    const unsigned char* from = nullptr;
+    int base = 0;
+    auto look_up = [&](int turn) {                     // for turns turn .. turn + 31, a lane one
+        const int c = begin + (turn + lane) * PA_WARPS;
+        from = nullptr;
+        if (c >= end) return;
+        int index;
+        if (list) {
+            index = list[c / per_page];
+            base = index * p.page_size + c % per_page * KEYS;
+        } else {
+            base = (chunk0 + c) * KEYS;
+            index = base / p.page_size;
         }
-        const int from = __shfl_sync(0xffffffffu, page, turn & 31), at = __shfl_sync(0xffffffffu, base, turn & 31);
+        if (index < 0 || base > pos_last) return;
+        const int page = index < p.max_pages && req >= 0 && req < p.n_req ? p.table[(size_t)req * p.max_pages + index] : -1;
+        if (page < 0 || page >= p.num_pages) {
+            if (p.status) atomicOr(p.status, BG_STATUS_BAD_PAGE);
+            return;
+        }
+        from = p.pool + ((size_t)page * p.nkv + kvh) * p.block_bytes + (size_t)(base % p.page_size / PK_TILE) * L::TILE;
+    };
+    auto issue = [&](int turn, int stage) {
+        const unsigned long long src = __shfl_sync(0xffffffffu, (unsigned long long)from, turn & 31);
+        const int at = __shfl_sync(0xffffffffu, base, turn & 31);
         if (lane == 0) {
-            const int stage = turn % PA_STAGES;
-            where[warp][stage] = from < 0 ? -1 : at;
-            if (from < 0) {
-                mbar_arrive(&bars[warp][stage]);
-            } else {
+            where[warp][stage] = src ? at : -1;
+            if (src) {
                 mbar_expect_tx(&bars[warp][stage], BYTES);
-                pa_bulk_load(ring + stage * BYTES, p.pool + ((size_t)from * p.nkv + kvh) * p.block_bytes + (size_t)(at % p.page_size / PK_TILE) * L::TILE, BYTES,
-                             &bars[warp][stage]);
+                pa_bulk_load(ring + stage * BYTES, reinterpret_cast<const unsigned char*>(src), BYTES, &bars[warp][stage]);
+            } else {
+                mbar_arrive(&bars[warp][stage]);
             }
         }
     };
+    if (turns > 0) look_up(0);
 #pragma unroll
-    for (int i = 0; i < PA_STAGES; ++i) issue(i);
+    for (int i = 0; i < PA_STAGES; ++i)
+        if (i < turns) issue(i, i);
 
     // ---- queries: column g of every block of 8, features 64 group + 16 t .. + 15 as four steps of a product
+    // (those that meet codes at bits 4 are a 16th)
     unsigned qf[PARTS][NT][GROUPS][8];
+    float qsum[NT][GROUPS][2], unit[NT][2];            // of columns 2t, 2t + 1 of every block: the sum of a group, and what the column's scores are multiplied with
+    int seen[NT][2];                                   // the positions of their rows
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         const int col = nt * 8 + g;
         const bool have = col < cols;
         const int r = have ? col / heads : 0, h = head0 + (have ? col - r * heads : 0);
         const TQ* q = reinterpret_cast<const TQ*>(p.q) + (size_t)(row0 + r) * p.q_stride + (size_t)(kvh * p.group + h) * HD + 16 * t;
+        float v[GROUPS][16], top = 0.0f;
 #pragma unroll
-        for (int gr = 0; gr < GROUPS; ++gr) {
-            if constexpr (F32) {
+        for (int gr = 0; gr < GROUPS; ++gr)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    float2 v = have ? *reinterpret_cast<const float2*>(q + gr * PK_GROUP + 2 * i) : make_float2(0.0f, 0.0f);
+            for (int i = 0; i < 16; i += 8) {
+                float e[8] = {};
+                if (have) load8(q + gr * PK_GROUP + i, e);
 #pragma unroll
-                    for (int part = 0; part < PARTS; ++part) {
-                        const __nv_bfloat16 a = __float2bfloat16_rn(v.x), b = __float2bfloat16_rn(v.y);
-                        qf[part][nt][gr][i] = (unsigned)__bfloat16_as_ushort(a) | (unsigned)__bfloat16_as_ushort(b) << 16;
-                        v.x -= __bfloat162float(a); v.y -= __bfloat162float(b);
-                    }
-                }
-            } else {
-                const uint4 a = have ? *reinterpret_cast<const uint4*>(q + gr * PK_GROUP) : make_uint4(0, 0, 0, 0);
-                const uint4 b = have ? *reinterpret_cast<const uint4*>(q + gr * PK_GROUP + 8) : make_uint4(0, 0, 0, 0);
-                qf[0][nt][gr][0] = a.x; qf[0][nt][gr][1] = a.y; qf[0][nt][gr][2] = a.z; qf[0][nt][gr][3] = a.w;
-                qf[0][nt][gr][4] = b.x; qf[0][nt][gr][5] = b.y; qf[0][nt][gr][6] = b.z; qf[0][nt][gr][7] = b.w;
+                for (int j = 0; j < 8; ++j) { v[gr][i + j] = e[j]; top = fmaxf(top, fabsf(e[j])); }
             }
-        }
-    }
-    float qsum[NT][GROUPS][2];                         // of columns 2t, 2t + 1 of every block
-    int seen[NT][2];                                   // the positions of their rows
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int high = max(-20, (int)(__float_as_uint(top) >> 23) - 127);
+        const float up = __uint_as_float((unsigned)(227 - high) << 23);          // 2^(100 - high)
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
+        for (int gr = 0; gr < GROUPS; ++gr)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float by = i % 2 ? up * 0.0625f : up;
+                float a = v[gr][2 * i] * by, b = v[gr][2 * i + 1] * by;
+#pragma unroll
+                for (int part = 0; part < PARTS; ++part) {
+                    const __nv_bfloat16 x = __float2bfloat16_rn(a), y = __float2bfloat16_rn(b);
+                    qf[part][nt][gr][i] = (unsigned)__bfloat16_as_ushort(x) | (unsigned)__bfloat16_as_ushort(y) << 16;
+                    a -= __bfloat162float(x); b -= __bfloat162float(y);
+                }
+            }
 #pragma unroll
         for (int gr = 0; gr < GROUPS; ++gr) {
             float c[4] = {};
 #pragma unroll
             for (int part = 0; part < PARTS; ++part)
 #pragma unroll
-                for (int k = 0; k < 4; ++k) pa_mma(c, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u, qf[part][nt][gr][2 * k], qf[part][nt][gr][2 * k + 1]);
+                for (int k = 0; k < 4; ++k) pa_mma(c, PA_ONE, PA_ONE, PA_ONE << 4, PA_ONE << 4, qf[part][nt][gr][2 * k], qf[part][nt][gr][2 * k + 1]);
             qsum[nt][gr][0] = c[0]; qsum[nt][gr][1] = c[1];
         }
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            const int col = nt * 8 + 2 * t + j;
-            seen[nt][j] = col < cols ? p.positions[row0 + col / heads] : pos_last;
+            const int mine = nt * 8 + 2 * t + j;
+            seen[nt][j] = mine < cols ? p.positions[row0 + mine / heads] : pos_last;
+            // back from 2^(100 - high) and the codes' 2^-133 to q . k, times what makes it an exponent of two (or, squashed, a part of the bound)
+            const int back = min(33 + __shfl_sync(0xffffffffu, high, (2 * t + j) * 4), 127);
+            unit[nt][j] = __uint_as_float((unsigned)(127 + back) << 23) * (p.cap_log2 > 0.0f ? p.scale_over_cap : p.scale_log2);
         }
     }
 
-    float o[GROUPS * 4][NT][4] = {}, minus[GROUPS][NT][4] = {}, low[NT][GROUPS][2] = {}, m[NT][2], l[NT][2] = {};
+    const bool capped = p.cap_log2 > 0.0f;
+    float o[GROUPS * 4][NT][4] = {}, low[NT][GROUPS][2] = {}, m[NT][2], l[NT][2] = {};
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) m[nt][0] = m[nt][1] = -INFINITY;
 
@@ -248,7 +257,7 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
                 for (int k = 0; k < 4; ++k) {
                     const unsigned w0 = kw[0][gr * 2 + k / 2], w1 = kw[1][gr * 2 + k / 2];
                     const int n = k % 2 * 2;
-                    const unsigned a0 = pa_codes<F32>(w0, n), a1 = pa_codes<F32>(w1, n), a2 = pa_codes<F32>(w0, n + 1), a3 = pa_codes<F32>(w1, n + 1);
+                    const unsigned a0 = pa_codes(w0, n), a1 = pa_codes(w1, n), a2 = pa_codes(w0, n + 1), a3 = pa_codes(w1, n + 1);
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -256,19 +265,18 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
                 }
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
-                    const float step = pair_step(kp[half][gr]);
-                    const float lowest = F32 ? pair_lowest(kp[half][gr]) : fmaf(-128.0f, step, pair_lowest(kp[half][gr]));
+                    const float step = pair_step(kp[half][gr]), lowest = pair_lowest(kp[half][gr]);
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int j = 0; j < 2; ++j) s[nt][2 * half + j] += fmaf(step, c[nt][2 * half + j], lowest * qsum[nt][gr][j]);
+                        for (int j = 0; j < 2; ++j) s[nt][2 * half + j] = fmaf(step, c[nt][2 * half + j], fmaf(lowest, qsum[nt][gr][j], s[nt][2 * half + j]));
                 }
             }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    x[i][nt][e] = pa_score<F32>(s[nt][e], p);
+                    x[i][nt][e] = s[nt][e];
                     if constexpr (EDGE) {
                         const int pos = at + i * PK_TILE + g + (e & 2) * 4, last = seen[nt][e & 1];
                         if (pos > last || (p.window > 0 && pos <= last - p.window)) {
@@ -277,6 +285,15 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
                         }
                     }
                 }
+        }
+        if (capped) {
+#pragma unroll
+            for (int i = 0; i < CT; ++i)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (!(EDGE && (hidden >> ((i * NT + nt) * 4 + e) & 1))) x[i][nt][e] = pa_squashed<F32>(x[i][nt][e] * unit[nt][e & 1], p.cap_log2);
         }
         // the running maximum, and what it does to what there is
         float top[NT][2];
@@ -290,6 +307,7 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
                 for (int i = 0; i < CT; ++i) v = fmaxf(v, fmaxf(x[i][nt][j], x[i][nt][j + 2]));
 #pragma unroll
                 for (int d = 4; d < 32; d <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
+                if (!capped) v *= unit[nt][j];
                 top[nt][j] = fmaxf(m[nt][j], v);
                 grew |= top[nt][j] > m[nt][j];
             }
@@ -302,11 +320,16 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
                     m[nt][j] = top[nt][j];
                     l[nt][j] *= keep;
 #pragma unroll
-                    for (int gr = 0; gr < GROUPS; ++gr) { low[nt][gr][j] *= keep; minus[gr][nt][j] *= keep; }
+                    for (int gr = 0; gr < GROUPS; ++gr) low[nt][gr][j] *= keep;
 #pragma unroll
                     for (int i = 0; i < GROUPS * 4; ++i) { o[i][nt][j] *= keep; o[i][nt][j + 2] *= keep; }
                 }
         }
+        float less[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) less[nt][j] = PA_UP - (m[nt][j] == -INFINITY ? 0.0f : m[nt][j]);
 #pragma unroll
         for (int i = 0; i < CT; ++i) {
             const unsigned char* tile = stage + i * L::TILE;
@@ -315,8 +338,8 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float from = m[nt][e & 1] == -INFINITY ? 0.0f : m[nt][e & 1];
-                    w[nt][e] = F32 ? exp2f(x[i][nt][e] - from) : pa_exp2(x[i][nt][e] - from);
+                    const float z = fmaf(x[i][nt][e], capped ? 1.0f : unit[nt][e & 1], less[nt][e & 1]);
+                    w[nt][e] = F32 ? exp2f(z) : pa_exp2(z);
                     l[nt][e & 1] += w[nt][e];
                 }
             unsigned vw[GROUPS][4], vp[2][GROUPS];     // words of positions 2t, 2t + 1, 2t + 8, 2t + 9; pairs of positions g, g + 8
@@ -363,17 +386,13 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
                             b[0][nt][half] = pa_transposed(pa_pack(e[0], e[1]));
                         }
                     }
-                if constexpr (!F32) {
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) pa_mma(minus[gr][nt], 0xc300c300u, 0xc300c300u, 0xc300c300u, 0xc300c300u, b[0][nt][0], b[0][nt][1]);
-                }
                 const unsigned ab[2] = {__byte_perm(vw[gr][0], vw[gr][1], 0x5410), __byte_perm(vw[gr][0], vw[gr][1], 0x7632)};
                 const unsigned cd[2] = {__byte_perm(vw[gr][2], vw[gr][3], 0x5410), __byte_perm(vw[gr][2], vw[gr][3], 0x7632)};
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {          // features 8 g + 2 k (rows g of the product) and 8 g + 2 k + 1 (rows g + 8)
                     const int n = k % 2 * 2;
-                    const unsigned a0 = pa_codes<F32>(ab[k / 2], n), a1 = pa_codes<F32>(ab[k / 2], n + 1);
-                    const unsigned a2 = pa_codes<F32>(cd[k / 2], n), a3 = pa_codes<F32>(cd[k / 2], n + 1);
+                    const unsigned a0 = pa_codes(ab[k / 2], n), a1 = pa_codes(ab[k / 2], n + 1);
+                    const unsigned a2 = pa_codes(cd[k / 2], n), a3 = pa_codes(cd[k / 2], n + 1);
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -384,10 +403,10 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
     };
 
     bool fine = true;
-    int turn = 0;
+    int turn = 0, stage = 0;
+    unsigned phase = 0;
     for (; turn < turns; ++turn) {
-        const int stage = turn % PA_STAGES;
-        fine = __all_sync(0xffffffffu, mbar_wait(&bars[warp][stage], (turn / PA_STAGES) & 1, &gave_up));
+        fine = __all_sync(0xffffffffu, mbar_wait(&bars[warp][stage], phase, &gave_up));
         if (!fine) break;
         const int at = where[warp][stage];
         if (at >= 0) {
@@ -395,7 +414,12 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
             else chunk(ring + stage * BYTES, at, std::false_type{});
         }
         __syncwarp();
-        issue(turn + PA_STAGES);
+        const int next = turn + PA_STAGES;
+        if (next < turns) {
+            if ((next & 31) == 0) look_up(next);
+            issue(next, stage);
+        }
+        if (++stage == PA_STAGES) { stage = 0; phase ^= 1u; }
     }
     if (!fine) {                                       // a copy did not come: the others of this warp are waited for, and the status says so
         if (lane == 0 && p.status) atomicOr(p.status, BG_STATUS_TIMEOUT);
@@ -421,14 +445,14 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             const int col = nt * 8 + 2 * t + j;
-            if (g == 0) ml[warp * COLS + col] = make_float2(m[nt][j], l[nt][j]);
+            if (g == 0) ml[warp * COLS + col] = make_float2(m[nt][j] - PA_UP, l[nt][j]);
 #pragma unroll
             for (int gr = 0; gr < GROUPS; ++gr) {
-                const float add = minus[gr][nt][j] + low[nt][gr][j];
+                const float add = low[nt][gr][j], even = 0x1p100f, odd = 0x1p96f;        // (back from 2^-133, and from 16 times that)
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
                     *reinterpret_cast<float2*>(res + (size_t)(warp * COLS + col) * S::ROW + gr * PK_GROUP + 8 * g + 2 * k) =
-                        make_float2(o[gr * 4 + k][nt][j] + add, o[gr * 4 + k][nt][j + 2] + add);
+                        make_float2(fmaf(o[gr * 4 + k][nt][j] * even, 0x1p33f, add), fmaf(o[gr * 4 + k][nt][j + 2] * odd, 0x1p33f, add));
             }
         }
     __syncthreads();
@@ -604,7 +628,7 @@ extern "C" int bg_packed_attention(const void* q, int dtype, long long q_stride,
                                    const float* sink_w, int sink, void* out, long long out_stride, unsigned* status, cudaStream_t stream) {
     if (hd != 64 && hd != 128) return BG_ERR_UNSUPPORTED;
     if (n <= 0) return BG_OK;
-    if (page_size <= 0 || page_size % PK_TILE || nkv <= 0 || nh <= 0 || nh % nkv || splits <= 0 || num_pages <= 0 || max_pages <= 0 || window < 0) return BG_ERR_SHAPE;
+    if (page_size <= 0 || page_size % PK_TILE || nkv <= 0 || nh <= 0 || nh % nkv || splits <= 0 || num_pages <= 0 || max_pages <= 0 || window < 0 || !(scale > 0.0f)) return BG_ERR_SHAPE;
     if (block_bytes % 16 || block_bytes < page_size / PK_TILE * packed_tile_bytes(hd) || (long long)n * splits > 0x7fffffffLL || (list && (top <= 0 || rows != 1))) return BG_ERR_SHAPE;
     if (dtype != BG_DTYPE_F32 && dtype != BG_DTYPE_BF16) return BG_ERR_DTYPE;
     const bool f32 = dtype == BG_DTYPE_F32;
