@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import struct
 from array import array
 from typing import Optional, Tuple
 
@@ -209,23 +210,21 @@ _SIGNATURES = {
     "bg_copy_pages_most": [],
     "bg_copy_pages": [_c_void_p, _c_int, _c_ll, _c_int, _c_ll, _c_int, _c_int, _c_ll, _c_int, _c_void_p, _c_void_p, _c_int, _c_void_p],
     "bg_packed_tile_bytes": [_c_int],
-    "bg_packed_append": [_c_void_p, _c_int, _c_ll, _c_int, _c_ll, _c_void_p, _c_int, _c_ll, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int,
-                         _c_void_p, _c_ll, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_void_p, _c_void_p],
-    "bg_packed_rows": [_c_void_p, _c_ll, _c_int, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_void_p, _c_int, _c_int, _c_int, _c_int,
-                       _c_void_p, _c_void_p],
-    "bg_packed_bounds": [_c_void_p, _c_ll, _c_int, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_void_p, _c_void_p],
+    "bg_packed_call_bytes": [_c_int],
+    "bg_packed_append": [_c_void_p, _c_void_p],
+    "bg_packed_rows": [_c_void_p, _c_void_p],
+    "bg_packed_bounds": [_c_void_p, _c_void_p],
     "bg_packed_wide_page": [],
     "bg_packed_unpack": [_c_void_p, _c_ll, _c_int, _c_int, _c_void_p, _c_void_p, _c_int, _c_int, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_int,
                          _c_int, _c_int, _c_int, _c_void_p, _c_void_p],
     "bg_attention_tc_half": [_c_void_p, _c_int, _c_void_p, _c_int, _c_int, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_int,
                              _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_void_p, _c_float, _c_void_p, _c_void_p],
     "bg_packed_attention_columns": [_c_int, _c_int, _c_int, ctypes.POINTER(_c_int)],
-    "bg_packed_attention": [_c_void_p, _c_int, _c_ll, _c_void_p, _c_ll, _c_int, _c_int, _c_void_p, _c_int, _c_int, _c_void_p, _c_void_p, _c_int, _c_int,
-                            _c_void_p, _c_int, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_float, _c_void_p, _c_int, _c_void_p,
-                            _c_ll, _c_void_p, _c_void_p],
+    "bg_packed_attention_bytes": [],
+    "bg_packed_attention": [_c_void_p, _c_void_p],
     "bg_packed_select_most": [],
-    "bg_packed_select": [_c_void_p, _c_int, _c_ll, _c_void_p, _c_ll, _c_int, _c_int, _c_void_p, _c_int, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int,
-                         _c_int, _c_int, _c_int, _c_void_p, _c_void_p, _c_void_p],
+    "bg_packed_select_bytes": [],
+    "bg_packed_select": [_c_void_p, _c_void_p],
     "bg_sample": [_c_void_p, _c_int, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p],
     "bg_sample_feed": [_c_void_p, _c_int, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
                        _c_void_p],
@@ -258,6 +257,10 @@ def lib():
                                  (SharedAttnStep, "bg_shared_attention_bytes", (1,)), (LogitsArgs, "bg_logits_bytes", ())):
             if getattr(handle, name)(*which) != ctypes.sizeof(cls):
                 raise KernelError(f"the kernel library's {cls.__name__} has another size than its mirror here")
+        for fields, name, which in ((_PACKED_APPEND, "bg_packed_call_bytes", (0,)), (_PACKED_READ, "bg_packed_call_bytes", (1,)),
+                                    (_PACKED_ATTENTION, "bg_packed_attention_bytes", ()), (_PACKED_SELECT, "bg_packed_select_bytes", ())):
+            if getattr(handle, name)(*which) != fields.size:
+                raise KernelError(f"the kernel library's fields of '{name}' are others than here")
         _lib = handle
     return _lib
 
@@ -868,6 +871,20 @@ def _attention(q: torch.Tensor, q_stride: int, kv_pool: torch.Tensor, block_tabl
 # ------------------------------------------------------------------------------------------------
 # A cache in 4 bits
 PACKED_TILE = 16           # positions of a tile: pages hold whole tiles
+# The calls' fields in the order of the library's structures: one packed record costs the host a tenth of what as many arguments do, which is what a call
+# of a decoding step is bound by.
+_PACKED_APPEND, _PACKED_READ = struct.Struct("<12q14i"), struct.Struct("<7q8i")
+_PACKED_ATTENTION, _PACKED_SELECT = struct.Struct("<14q14i2f"), struct.Struct("<8q12i")
+
+
+def _at(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+@functools.lru_cache(maxsize=None)
+def _packed_sizes(hd: int, page_size: int) -> Tuple[int, int]:
+    """Bytes of a (page, kv head) without bounds and with them."""
+    return packed_page_bytes(hd, page_size), packed_page_bytes(hd, page_size, True)
 
 
 def packed_page_bytes(hd: int, page_size: int, bounds: bool = False) -> int:
@@ -882,13 +899,14 @@ def packed_page_bytes(hd: int, page_size: int, bounds: bool = False) -> int:
 
 def _packed_pool(what: str, pool: torch.Tensor, hd: int, page_size: int, nkv: Optional[int] = None, bounds: bool = False) -> int:
     """The pool's bytes of a (page, kv head), checked: uint8 [pages, nkv, bytes], with room for bounds or without."""
-    if pool.dtype != torch.uint8 or pool.dim() != 3 or not pool.is_contiguous() or (nkv is not None and pool.shape[1] != nkv):
-        raise KernelError(f"{what}: the pool is {tuple(pool.shape)} of {pool.dtype}, expected contiguous uint8 [pages, {'kv heads' if nkv is None else nkv}, bytes]")
-    plain, more = packed_page_bytes(hd, page_size), packed_page_bytes(hd, page_size, True)
-    if pool.shape[2] != more and (bounds or pool.shape[2] != plain):
+    shape = pool.shape
+    if pool.dtype != torch.uint8 or len(shape) != 3 or not pool.is_contiguous() or (nkv is not None and shape[1] != nkv):
+        raise KernelError(f"{what}: the pool is {tuple(shape)} of {pool.dtype}, expected contiguous uint8 [pages, {'kv heads' if nkv is None else nkv}, bytes]")
+    plain, more = _packed_sizes(hd, page_size)
+    if shape[2] != more and (bounds or shape[2] != plain):
         raise KernelError(f"{what}: a page of {page_size} positions holds {more if bounds else plain} bytes a kv head of {hd} features"
-                          + (" and their bounds" if bounds else f" ({more} with bounds)") + f", not {pool.shape[2]}")
-    return pool.shape[2]
+                          + (" and their bounds" if bounds else f" ({more} with bounds)") + f", not {shape[2]}")
+    return shape[2]
 
 
 def _packed_rows_of(what: str, positions: torch.Tensor, row_req: Optional[torch.Tensor], block_table: torch.Tensor, n_rows: int) -> None:
@@ -925,9 +943,10 @@ def packed_append(src: torch.Tensor, q_out: torch.Tensor, nh: int, nkv: int, hd:
     if T == 0:
         return
     with phase("rope+kv_write"):
-        _check(lib().bg_packed_append(_p(src), _dt(src), src.stride(-2), parts, stride, _p(q_out), _dt(q_out), q_out.stride(0), _p(cos_sin), _p(positions),
-                                      _p(row_req), _p(block_table), block_table.shape[1], block_table.shape[0], _p(pool), block, pool.shape[0], page_size, T,
-                                      nh, nkv, hd, rot, 1 if interleaved else 0, _p(status), _stream()), "packed_append")
+        fields = _PACKED_APPEND.pack(_at(src), src.stride(-2), stride, _at(q_out), q_out.stride(0), _at(cos_sin), _at(positions), _at(row_req), _at(block_table),
+                                     _at(pool), block, _at(status), _dt(src), _dt(q_out), parts, block_table.shape[1], pool.shape[0], page_size, T,
+                                     block_table.shape[0], nh, nkv, hd, rot, 1 if interleaved else 0, 0)
+        _check(lib().bg_packed_append(fields, _stream()), "packed_append")
 
 
 def packed_bounds(pool: torch.Tensor, positions: torch.Tensor, row_req: torch.Tensor, block_table: torch.Tensor, hd: int, page_size: int,
@@ -941,8 +960,12 @@ def packed_bounds(pool: torch.Tensor, positions: torch.Tensor, row_req: torch.Te
     if T == 0:
         return
     with phase("rope+kv_write"):
-        _check(lib().bg_packed_bounds(_p(pool), block, pool.shape[0], page_size, _p(positions), _p(row_req), _p(block_table), block_table.shape[1],
-                                      block_table.shape[0], T, pool.shape[1], hd, _p(status), _stream()), "packed_bounds")
+        _check(lib().bg_packed_bounds(_packed_read(pool, block, positions, row_req, block_table, None, 0, status, page_size, T, hd), _stream()), "packed_bounds")
+
+
+def _packed_read(pool, block, positions, row_req, block_table, out, out_type, status, page_size, T, hd) -> bytes:
+    return _PACKED_READ.pack(_at(pool), block, _at(positions), _at(row_req), _at(block_table), _at(out), _at(status), out_type, block_table.shape[1], pool.shape[0],
+                             page_size, block_table.shape[0], T, pool.shape[1], hd)
 
 
 def packed_rows(pool: torch.Tensor, positions: torch.Tensor, row_req: torch.Tensor, block_table: torch.Tensor, hd: int, page_size: int, out: torch.Tensor,
@@ -956,14 +979,14 @@ def packed_rows(pool: torch.Tensor, positions: torch.Tensor, row_req: torch.Tens
         raise KernelError(f"packed_rows: out is {tuple(out.shape)}, expected contiguous {(T, 2, pool.shape[1], hd)}")
     if T == 0:
         return
-    _check(lib().bg_packed_rows(_p(pool), block, pool.shape[0], page_size, _p(positions), _p(row_req), _p(block_table), block_table.shape[1],
-                                block_table.shape[0], _p(out), _dt(out), T, pool.shape[1], hd, _p(status), _stream()), "packed_rows")
+    _check(lib().bg_packed_rows(_packed_read(pool, block, positions, row_req, block_table, out, _dt(out), status, page_size, T, hd), _stream()), "packed_rows")
 
 
 # Rows that a request brings from which its pages are written out in half precision for the prompt attention.
 PACKED_LONG_ROWS = 64
 
 
+@functools.lru_cache(maxsize=None)
 def _packed_columns(group: int, f32: bool, rows: int) -> Tuple[int, int]:
     """(columns of a CTA's block, query heads of a block) of the packed attention kernel for blocks of `rows` rows."""
     each = _c_int(0)
@@ -1068,15 +1091,17 @@ def packed_attention(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Ten
             cols, each = _packed_columns(nh // nkv, f32, most)
             streams = nkv * -(-(nh // nkv) // each)
             read = min(max_position + 1, top * page_size if top else max_position + 1, window + most if window else max_position + 1)
-            splits = packed_splits(n * streams, read, sm_count() * (2 if cols == 8 and not f32 else 1))
-            part_o = part_ml = None
+            splits = packed_splits(n * streams, read, sm_count(q.device) * (2 if cols == 8 and not f32 else 1))
+            part_o = part_ml = 0
             if splits > 1:
-                part_o = torch.empty((n * streams * splits * cols, hd), dtype=torch.float32, device=q.device)
-                part_ml = torch.empty((n * streams * splits * cols, 2), dtype=torch.float32, device=q.device)
-            _check(L.bg_packed_attention(_p(q), _dt(q), q.stride(0), _p(pool), block, pool.shape[0], page_size, _p(block_table), block_table.shape[1],
-                                         block_table.shape[0], _p(positions), None if plan is None else _p(plan.short), n, most, _p(pages), top, _p(part_o),
-                                         _p(part_ml), splits, nh, nkv, hd, window, float(scale), float(softcap), _p(sink_weight), 1 if sink else 0, _p(out),
-                                         out.stride(0), _p(status), _stream()), "packed_attention")
+                results = n * streams * splits * cols
+                scratch = torch.empty((results * (hd + 2),), dtype=torch.float32, device=q.device)
+                part_o = scratch.data_ptr()
+                part_ml = part_o + 4 * hd * results
+            fields = _PACKED_ATTENTION.pack(_at(q), _at(pool), _at(block_table), _at(positions), 0 if plan is None else _at(plan.short), _at(pages), part_o, part_ml,
+                                            _at(out), _at(sink_weight), _at(status), q.stride(0), block, out.stride(0), _dt(q), pool.shape[0], page_size,
+                                            block_table.shape[1], block_table.shape[0], n, most, top, splits, nh, nkv, hd, window, 1 if sink else 0, scale, softcap)
+            _check(L.bg_packed_attention(fields, _stream()), "packed_attention")
             count_launches(1 if splits > 1 else 0)
         if plan is not None and plan.n_long:
             end = max_position + 1 if plan.long_end is None else min(plan.long_end, max_position + 1)
@@ -1117,9 +1142,10 @@ def packed_select(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor
     if T == 0:
         return
     with phase("attn"):
-        _check(lib().bg_packed_select(_p(q), _dt(q), q.stride(0), _p(pool), block, pool.shape[0], page_size, _p(block_table), block_table.shape[1],
-                                      _p(positions), T, nh, nkv, hd, out.shape[2], first, recent, max(1, n_pages), _p(out), _p(status), _stream()),
-               "packed_select")
+        fields = _PACKED_SELECT.pack(_at(q), q.stride(0), _at(pool), block, _at(block_table), _at(positions), _at(out), _at(status), _dt(q), pool.shape[0], page_size,
+                                     block_table.shape[1], T, nh, nkv, hd, out.shape[2], first, recent, max(1, n_pages))
+        _check(lib().bg_packed_select(fields, _stream()), "packed_select")
+
 
 # ------------------------------------------------------------------------------------------------
 # Attention of single tokens whose requests share their first positions

@@ -13,14 +13,15 @@
 namespace bg {
 
 // ------------------------------------------------------------------------------------------------ append
+// (the host side packs this and the other calls' fields in their order)
 struct PkAppend {
-    const void* src; long long src_stride, part_stride; int parts;
+    const void* src; long long src_stride, part_stride;
     void* q_out; long long q_stride;
     const float* cos_sin;
     const int* positions; const int* row_req; const int* block_table;
     unsigned char* pool; long long block_bytes;
-    int max_pages, num_pages, page_size, T, n_req, nh, nkv, rot, interleaved;
     unsigned* status;
+    int src_dtype, q_dtype, parts, max_pages, num_pages, page_size, T, n_req, nh, nkv, hd, rot, interleaved, pad;
 };
 
 // Four neighbouring features of a row (summed over partial results).
@@ -190,11 +191,11 @@ __global__ void __launch_bounds__(PK_THREADS) packed_append_kernel(const PkAppen
 
 // ------------------------------------------------------------------------------------------------ rows read back
 struct PkRead {
-    const unsigned char* pool; long long block_bytes;
+    unsigned char* pool; long long block_bytes;
     const int* positions; const int* row_req; const int* block_table;
     void* out;
-    int max_pages, num_pages, page_size, n_req, nkv;
     unsigned* status;
+    int out_dtype, max_pages, num_pages, page_size, n_req, T, nkv, hd;
 };
 
 // out[t, keys and values, kv head, feature]: a thread reads a word of codes and writes its 8 values.
@@ -224,20 +225,13 @@ __global__ void __launch_bounds__(PK_THREADS) packed_rows_kernel(const PkRead p)
 }
 
 // ------------------------------------------------------------------------------------------------ bounds of filled pages
-struct PkBounds {
-    unsigned char* pool; long long block_bytes;
-    const int* positions; const int* row_req; const int* block_table;
-    int max_pages, num_pages, page_size, n_req, nkv;
-    unsigned* status;
-};
-
 // A row that fills its page (its position is the page's last) has the CTA of its (row, kv head) find the smallest and largest value of every feature of the
 // page's keys, as they are read back.  What a page's bounds are hangs on the page alone, whoever wrote it and in how many steps.  A thread takes a word of 8
 // features of every (PK_THREADS / words)-th position; a value that is no number stays one.
 __device__ __forceinline__ float least(float a, float b) { return a < b || a != a ? a : b; }
 __device__ __forceinline__ float most(float a, float b) { return a > b || a != a ? a : b; }
 template <int HD>
-__global__ void __launch_bounds__(PK_THREADS) packed_bounds_kernel(const PkBounds p) {
+__global__ void __launch_bounds__(PK_THREADS) packed_bounds_kernel(const PkRead p) {
     constexpr int WORDS = HD / 8, AT_ONCE = PK_THREADS / WORDS;
     __shared__ float ends[2][AT_ONCE][HD + 1];
     pdl_launch();
@@ -412,44 +406,40 @@ using namespace bg;
 // Bytes of a tile of 16 positions of one kv head, or a negative code.
 extern "C" int bg_packed_tile_bytes(int hd) { return hd == 64 || hd == 128 ? (int)packed_tile_bytes(hd) : BG_ERR_UNSUPPORTED; }
 
-extern "C" int bg_packed_append(const void* src, int src_dtype, long long src_stride, int parts, long long part_stride, void* q_out, int q_dtype,
-                                long long q_stride, const float* cos_sin, const int* positions, const int* row_req, const int* block_table, int max_pages,
-                                int n_req, unsigned char* pool, long long block_bytes, int num_pages, int page_size, int T, int nh, int nkv, int hd, int rot,
-                                int interleaved, unsigned* status, cudaStream_t stream) {
-    if (int e = packed_shape(hd, page_size, nkv, num_pages, block_bytes, false)) return e;
-    if (T <= 0) return BG_OK;
-    if (parts < 1 || nh <= 0 || rot < 0 || rot > hd || rot % 2 || max_pages <= 0 || (rot && !cos_sin)) return BG_ERR_SHAPE;
-    const long long fine = src_dtype == BG_DTYPE_F32 ? 15 : 7, fine_q = q_dtype == BG_DTYPE_F32 ? 15 : 7;
-    const long long size = src_dtype == BG_DTYPE_F32 ? 4 : 2, size_q = q_dtype == BG_DTYPE_F32 ? 4 : 2;
-    if (((long long)(uintptr_t)src | src_stride * size | (parts > 1 ? part_stride * size : 0)) & fine || ((long long)(uintptr_t)q_out | q_stride * size_q) & fine_q
-        || (uintptr_t)pool % 16 || (uintptr_t)cos_sin % 8) return BG_ERR_ALIGN;
-    const PkAppend p = {src, src_stride, part_stride, parts, q_out, q_stride, cos_sin, positions, row_req, block_table, pool, block_bytes,
-                        max_pages, num_pages, page_size, T, n_req, nh, nkv, rot, interleaved, status};
-    BG_DISPATCH_DTYPE(src_dtype, TS, BG_DISPATCH_DTYPE(q_dtype, TQ, return hd == 64 ? (append_launch<TS, TQ, 64>(p, stream)) : (append_launch<TS, TQ, 128>(p, stream))));
+// Bytes of the calls' fields: 0 an append, 1 a reading call.
+extern "C" int bg_packed_call_bytes(int which) { return which == 0 ? (int)sizeof(PkAppend) : (int)sizeof(PkRead); }
+
+extern "C" int bg_packed_append(const void* call, cudaStream_t stream) {
+    const PkAppend& p = *(const PkAppend*)call;
+    if (int e = packed_shape(p.hd, p.page_size, p.nkv, p.num_pages, p.block_bytes, false)) return e;
+    if (p.T <= 0) return BG_OK;
+    if (p.parts < 1 || p.nh <= 0 || p.rot < 0 || p.rot > p.hd || p.rot % 2 || p.max_pages <= 0 || (p.rot && !p.cos_sin)) return BG_ERR_SHAPE;
+    const long long fine = p.src_dtype == BG_DTYPE_F32 ? 15 : 7, fine_q = p.q_dtype == BG_DTYPE_F32 ? 15 : 7;
+    const long long size = p.src_dtype == BG_DTYPE_F32 ? 4 : 2, size_q = p.q_dtype == BG_DTYPE_F32 ? 4 : 2;
+    if (((long long)(uintptr_t)p.src | p.src_stride * size | (p.parts > 1 ? p.part_stride * size : 0)) & fine
+        || ((long long)(uintptr_t)p.q_out | p.q_stride * size_q) & fine_q || (uintptr_t)p.pool % 16 || (uintptr_t)p.cos_sin % 8) return BG_ERR_ALIGN;
+    BG_DISPATCH_DTYPE(p.src_dtype, TS, BG_DISPATCH_DTYPE(p.q_dtype, TQ, return p.hd == 64 ? (append_launch<TS, TQ, 64>(p, stream)) : (append_launch<TS, TQ, 128>(p, stream))));
 }
 
-extern "C" int bg_packed_rows(const unsigned char* pool, long long block_bytes, int num_pages, int page_size, const int* positions, const int* row_req,
-                              const int* block_table, int max_pages, int n_req, void* out, int out_dtype, int T, int nkv, int hd, unsigned* status,
-                              cudaStream_t stream) {
-    if (int e = packed_shape(hd, page_size, nkv, num_pages, block_bytes, false)) return e;
-    if (T <= 0) return BG_OK;
-    if ((uintptr_t)pool % 16 || (uintptr_t)out % 16) return BG_ERR_ALIGN;
-    const PkRead p = {pool, block_bytes, positions, row_req, block_table, out, max_pages, num_pages, page_size, n_req, nkv, status};
-    const dim3 grid(T, (2 * nkv * hd / 8 + PK_THREADS - 1) / PK_THREADS);
+extern "C" int bg_packed_rows(const void* call, cudaStream_t stream) {
+    const PkRead& p = *(const PkRead*)call;
+    if (int e = packed_shape(p.hd, p.page_size, p.nkv, p.num_pages, p.block_bytes, false)) return e;
+    if (p.T <= 0) return BG_OK;
+    if ((uintptr_t)p.pool % 16 || (uintptr_t)p.out % 16) return BG_ERR_ALIGN;
+    const dim3 grid(p.T, (2 * p.nkv * p.hd / 8 + PK_THREADS - 1) / PK_THREADS);
     cudaError_t e = cudaSuccess;
-    BG_DISPATCH_DTYPE(out_dtype, TO, e = hd == 64 ? launch(packed_rows_kernel<TO, 64>, grid, dim3(PK_THREADS), 0, stream, p)
-                                                  : launch(packed_rows_kernel<TO, 128>, grid, dim3(PK_THREADS), 0, stream, p));
+    BG_DISPATCH_DTYPE(p.out_dtype, TO, e = p.hd == 64 ? launch(packed_rows_kernel<TO, 64>, grid, dim3(PK_THREADS), 0, stream, p)
+                                                      : launch(packed_rows_kernel<TO, 128>, grid, dim3(PK_THREADS), 0, stream, p));
     return e == cudaSuccess ? BG_OK : (int)e;
 }
 
-extern "C" int bg_packed_bounds(unsigned char* pool, long long block_bytes, int num_pages, int page_size, const int* positions, const int* row_req,
-                                const int* block_table, int max_pages, int n_req, int T, int nkv, int hd, unsigned* status, cudaStream_t stream) {
-    if (int e = packed_shape(hd, page_size, nkv, num_pages, block_bytes, true)) return e;
-    if (T <= 0) return BG_OK;
-    if ((uintptr_t)pool % 16) return BG_ERR_ALIGN;
-    const PkBounds p = {pool, block_bytes, positions, row_req, block_table, max_pages, num_pages, page_size, n_req, nkv, status};
-    cudaError_t e = hd == 64 ? launch(packed_bounds_kernel<64>, dim3(T, nkv), dim3(PK_THREADS), 0, stream, p)
-                             : launch(packed_bounds_kernel<128>, dim3(T, nkv), dim3(PK_THREADS), 0, stream, p);
+extern "C" int bg_packed_bounds(const void* call, cudaStream_t stream) {
+    const PkRead& p = *(const PkRead*)call;
+    if (int e = packed_shape(p.hd, p.page_size, p.nkv, p.num_pages, p.block_bytes, true)) return e;
+    if (p.T <= 0) return BG_OK;
+    if ((uintptr_t)p.pool % 16) return BG_ERR_ALIGN;
+    cudaError_t e = p.hd == 64 ? launch(packed_bounds_kernel<64>, dim3(p.T, p.nkv), dim3(PK_THREADS), 0, stream, p)
+                               : launch(packed_bounds_kernel<128>, dim3(p.T, p.nkv), dim3(PK_THREADS), 0, stream, p);
     return e == cudaSuccess ? BG_OK : (int)e;
 }
 

@@ -29,20 +29,23 @@ namespace bg {
 constexpr int PA_WARPS = 8, PA_THREADS = PA_WARPS * 32, PA_STAGES = 3;
 constexpr float PA_LOG2E = 1.4426950408889634f;
 
-struct PaParams {
-    const void* q; long long q_stride;
-    const unsigned char* pool; long long block_bytes;
+// What a call brings; the host side packs the fields in their order.
+struct PaCall {
+    const void* q; const unsigned char* pool;
     const int* table; const int* positions;
     const int* blocks;                 // [n][3]: request, first row, rows; null: block i is row i of request i
     const int* list;                   // [rows][nkv][top] page indexes to read (less than 0: none), or null: all
-    int num_pages, page_size, max_pages, top, n_req;
-    int nkv, group, head_blocks, heads_each;       // query heads of a kv head, the blocks that they are cut into, heads of a block
-    int window, splits;
-    float scale_log2, cap_log2, scale_over_cap;
     float* part_o; float* part_ml;     // [block][kv head and head block][split][column][HD], [..][2]; null: finished rows go to `out`
-    void* out; long long out_stride;
-    const float* sink_w; int sink;
-    unsigned* status;
+    void* out; const float* sink_w; unsigned* status;
+    long long q_stride, block_bytes, out_stride;
+    int dtype, num_pages, page_size, max_pages, n_req;
+    int n, rows;                       // blocks, and the most rows of one
+    int top, splits, nh, nkv, hd, window, sink;
+    float scale, softcap;
+};
+struct PaParams : PaCall {
+    int group, head_blocks, heads_each;            // query heads of a kv head, the blocks that they are cut into, heads of a block
+    float scale_log2, cap_log2, scale_over_cap;
 };
 
 __device__ __forceinline__ void pa_mma(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
@@ -621,28 +624,32 @@ extern "C" int bg_packed_attention_columns(int group, int f32, int rows, int* he
     return *heads_each * rows <= 8 ? 1 : 2;
 }
 
-// n blocks of rows; `rows` is the most rows of a block.  part_o / part_ml hold n * nkv * head_blocks * splits * columns results where splits > 1.
-extern "C" int bg_packed_attention(const void* q, int dtype, long long q_stride, const unsigned char* pool, long long block_bytes, int num_pages, int page_size,
-                                   const int* table, int max_pages, int n_req, const int* positions, const int* blocks, int n, int rows, const int* list,
-                                   int top, float* part_o, float* part_ml, int splits, int nh, int nkv, int hd, int window, float scale, float softcap,
-                                   const float* sink_w, int sink, void* out, long long out_stride, unsigned* status, cudaStream_t stream) {
-    if (hd != 64 && hd != 128) return BG_ERR_UNSUPPORTED;
-    if (n <= 0) return BG_OK;
-    if (page_size <= 0 || page_size % PK_TILE || nkv <= 0 || nh <= 0 || nh % nkv || splits <= 0 || num_pages <= 0 || max_pages <= 0 || window < 0 || !(scale > 0.0f)) return BG_ERR_SHAPE;
-    if (block_bytes % 16 || block_bytes < page_size / PK_TILE * packed_tile_bytes(hd) || (long long)n * splits > 0x7fffffffLL || (list && (top <= 0 || rows != 1))) return BG_ERR_SHAPE;
-    if (dtype != BG_DTYPE_F32 && dtype != BG_DTYPE_BF16) return BG_ERR_DTYPE;
-    const bool f32 = dtype == BG_DTYPE_F32;
+extern "C" int bg_packed_attention_bytes() { return (int)sizeof(PaCall); }
+
+// part_o / part_ml hold n * nkv * head_blocks * splits * columns results where splits > 1.
+extern "C" int bg_packed_attention(const void* call, cudaStream_t stream) {
+    const PaCall& c = *(const PaCall*)call;
+    if (c.hd != 64 && c.hd != 128) return BG_ERR_UNSUPPORTED;
+    if (c.n <= 0) return BG_OK;
+    if (c.page_size <= 0 || c.page_size % PK_TILE || c.nkv <= 0 || c.nh <= 0 || c.nh % c.nkv || c.splits <= 0 || c.num_pages <= 0 || c.max_pages <= 0
+        || c.window < 0 || !(c.scale > 0.0f)) return BG_ERR_SHAPE;
+    if (c.block_bytes % 16 || c.block_bytes < c.page_size / PK_TILE * packed_tile_bytes(c.hd) || (long long)c.n * c.splits > 0x7fffffffLL
+        || (c.list && (c.top <= 0 || c.rows != 1))) return BG_ERR_SHAPE;
+    if (c.dtype != BG_DTYPE_F32 && c.dtype != BG_DTYPE_BF16) return BG_ERR_DTYPE;
+    const bool f32 = c.dtype == BG_DTYPE_F32;
     const long long size = f32 ? 4 : 2;
-    if ((uintptr_t)pool % 16 || ((long long)(uintptr_t)q | q_stride * size) % 16 || ((long long)(uintptr_t)out | out_stride * size) % (2 * size)) return BG_ERR_ALIGN;
-    if ((splits > 1) != (part_o != nullptr) || (part_o == nullptr) != (part_ml == nullptr) || (uintptr_t)part_o % 16 || (uintptr_t)part_ml % 8) return BG_ERR_SHAPE;
-    int each = 0;
-    const int nt = bg_packed_attention_columns(nh / nkv, f32, rows, &each);
+    if ((uintptr_t)c.pool % 16 || ((long long)(uintptr_t)c.q | c.q_stride * size) % 16 || ((long long)(uintptr_t)c.out | c.out_stride * size) % (2 * size)) return BG_ERR_ALIGN;
+    if ((c.splits > 1) != (c.part_o != nullptr) || (c.part_o == nullptr) != (c.part_ml == nullptr) || (uintptr_t)c.part_o % 16 || (uintptr_t)c.part_ml % 8) return BG_ERR_SHAPE;
+    PaParams p;
+    static_cast<PaCall&>(p) = c;
+    const int nt = bg_packed_attention_columns(c.nh / c.nkv, f32, c.rows, &p.heads_each);
     if (nt < 0) return nt;
-    const int group = nh / nkv, head_blocks = (group + each - 1) / each;
-    if ((long long)nkv * head_blocks > 65535) return BG_ERR_SHAPE;
-    const PaParams p = {q, q_stride, pool, block_bytes, table, positions, blocks, list, num_pages, page_size, max_pages, top, n_req, nkv, group, head_blocks, each,
-                        window, splits, scale * PA_LOG2E, softcap > 0.0f ? softcap * PA_LOG2E : 0.0f, softcap > 0.0f ? scale / softcap : 0.0f,
-                        part_o, part_ml, out, out_stride, sink_w, sink, status};
-    if (hd == 64) return f32 ? pa_sized<64, true>(p, n, nt, stream) : pa_sized<64, false>(p, n, nt, stream);
-    return f32 ? pa_sized<128, true>(p, n, nt, stream) : pa_sized<128, false>(p, n, nt, stream);
+    p.group = c.nh / c.nkv;
+    p.head_blocks = (p.group + p.heads_each - 1) / p.heads_each;
+    if ((long long)c.nkv * p.head_blocks > 65535) return BG_ERR_SHAPE;
+    p.scale_log2 = c.scale * PA_LOG2E;
+    p.cap_log2 = c.softcap > 0.0f ? c.softcap * PA_LOG2E : 0.0f;
+    p.scale_over_cap = c.softcap > 0.0f ? c.scale / c.softcap : 0.0f;
+    if (c.hd == 64) return f32 ? pa_sized<64, true>(p, c.n, nt, stream) : pa_sized<64, false>(p, c.n, nt, stream);
+    return f32 ? pa_sized<128, true>(p, c.n, nt, stream) : pa_sized<128, false>(p, c.n, nt, stream);
 }

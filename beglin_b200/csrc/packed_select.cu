@@ -15,13 +15,14 @@ namespace bg {
 
 constexpr int PS_THREADS = 256, PS_CLUSTER = 8, PS_HEADS = 8, PS_FLOATS = 50000;       // PS_FLOATS: the most pages, whose scores are in shared memory
 
+// What a call brings; the host side packs the fields in their order.
 struct PsParams {
     const void* q; long long q_stride;
-    const unsigned char* pool; long long block_bytes, bounds_at;
+    const unsigned char* pool; long long block_bytes;
     const int* table; const int* positions;
-    int* out;
-    int num_pages, page_size, max_pages, nkv, group, top, first, recent, pages_most;
-    unsigned* status;
+    int* out; unsigned* status;
+    int dtype, num_pages, page_size, max_pages, T, nh, nkv, hd, top, first, recent;
+    int pages_most;                    // bounds the pages of every row
 };
 
 // Ordered as the scores are, as a whole number; both noughts are one.
@@ -40,6 +41,8 @@ __global__ void __launch_bounds__(PS_THREADS) packed_select_kernel(const PsParam
     const int row = blockIdx.x, kvh = blockIdx.y, rank = blockIdx.z, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     pdl_wait();
     const int pos = p.positions[row], pages = pos < 0 ? 0 : min(pos / p.page_size + 1, p.pages_most);
+    const int group = p.nh / p.nkv;
+    const long long bounds_at = (long long)(p.page_size / PK_TILE) * Packed<HD>::TILE;
     int* out = p.out + ((size_t)row * p.nkv + kvh) * p.top;
     if (pages <= p.top) {                              // (every CTA of the cluster: nobody waits for another)
         if (rank == 0)
@@ -50,23 +53,23 @@ __global__ void __launch_bounds__(PS_THREADS) packed_select_kernel(const PsParam
     cluster_wait();
     const int each = (pages + PS_CLUSTER - 1) / PS_CLUSTER, from = rank * each, to = min(pages, from + each);
     const unsigned there = peer_addr(smem_u32(scores), 0);
-    for (int h0 = 0; h0 < p.group; h0 += PS_HEADS) {
+    for (int h0 = 0; h0 < group; h0 += PS_HEADS) {
         __syncthreads();
         for (int i = tid; i < PS_HEADS * HD; i += PS_THREADS) {
             const int h = i / HD, f = i % HD;
-            const double v = h0 + h < p.group
-                ? (double)to_float(reinterpret_cast<const TQ*>(p.q)[(size_t)row * p.q_stride + (size_t)(kvh * p.group + h0 + h) * HD + f]) : 0.0;
+            const double v = h0 + h < group
+                ? (double)to_float(reinterpret_cast<const TQ*>(p.q)[(size_t)row * p.q_stride + (size_t)(kvh * group + h0 + h) * HD + f]) : 0.0;
             q_s[f / 8][f % 8 * PS_HEADS + h] = make_double2(v > 0.0 ? v : 0.0, v > 0.0 ? 0.0 : v);
         }
         __syncthreads();
-        const int heads = min(PS_HEADS, p.group - h0);
+        const int heads = min(PS_HEADS, group - h0);
         for (int i0 = from; i0 < to; i0 += PS_THREADS / 4) {
             const int index = i0 + tid / 4, quarter = tid & 3;
             const bool have = index < to;
             int page = have && index < p.max_pages ? p.table[(size_t)row * p.max_pages + index] : -1;
             const bool bad = have && (page < 0 || page >= p.num_pages);
             if (bad || !have) page = 0;
-            const uint4* ends = reinterpret_cast<const uint4*>(p.pool + ((size_t)page * p.nkv + kvh) * p.block_bytes + p.bounds_at);
+            const uint4* ends = reinterpret_cast<const uint4*>(p.pool + ((size_t)page * p.nkv + kvh) * p.block_bytes + bounds_at);
             uint4 lo4[MINE], hi4[MINE];
 #pragma unroll
             for (int c = 0; c < MINE; ++c) { lo4[c] = ends[quarter + 4 * c]; hi4[c] = ends[CHUNKS + quarter + 4 * c]; }
@@ -167,11 +170,11 @@ __global__ void __launch_bounds__(PS_THREADS) packed_select_kernel(const PsParam
 }
 
 template <typename TQ, int HD>
-static int ps_launch(const PsParams& p, int T, cudaStream_t stream) {
+static int ps_launch(const PsParams& p, cudaStream_t stream) {
     const size_t smem = (size_t)p.pages_most * 4;
     cudaError_t e = smem_limit(packed_select_kernel<TQ, HD>, smem);
     if (e != cudaSuccess) return (int)e;
-    e = launch_cluster(packed_select_kernel<TQ, HD>, dim3(T, p.nkv, PS_CLUSTER), dim3(PS_THREADS), smem, stream, PS_CLUSTER, p);
+    e = launch_cluster(packed_select_kernel<TQ, HD>, dim3(p.T, p.nkv, PS_CLUSTER), dim3(PS_THREADS), smem, stream, PS_CLUSTER, p);
     return e == cudaSuccess ? BG_OK : (int)e;
 }
 
@@ -181,18 +184,16 @@ using namespace bg;
 
 extern "C" int bg_packed_select_most() { return PS_FLOATS; }
 
-// out[row][kv head][top]: the pages that row `row` (of request `row`) reads, ascending, -1 behind them.  pages_most bounds the pages of every row.
-extern "C" int bg_packed_select(const void* q, int dtype, long long q_stride, const unsigned char* pool, long long block_bytes, int num_pages, int page_size,
-                                const int* table, int max_pages, const int* positions, int T, int nh, int nkv, int hd, int top, int first, int recent,
-                                int pages_most, int* out, unsigned* status, cudaStream_t stream) {
-    if (hd != 64 && hd != 128) return BG_ERR_UNSUPPORTED;
-    if (T <= 0) return BG_OK;
-    if (page_size <= 0 || page_size % PK_TILE || nkv <= 0 || nkv > 65535 || nh <= 0 || nh % nkv || num_pages <= 0 || max_pages <= 0) return BG_ERR_SHAPE;
-    const long long bounds_at = page_size / PK_TILE * packed_tile_bytes(hd);
-    if (block_bytes % 16 || block_bytes < bounds_at + 4 * hd || (uintptr_t)pool % 16) return BG_ERR_ALIGN;
-    if (top <= 0 || first < 0 || recent < 1 || first + recent > top || pages_most <= 0) return BG_ERR_SHAPE;
-    if (pages_most > PS_FLOATS) return BG_ERR_UNSUPPORTED;
-    const PsParams p = {q, q_stride, pool, block_bytes, bounds_at, table, positions, out, num_pages, page_size, max_pages, nkv, nh / nkv, top, first, recent,
-                        pages_most, status};
-    BG_DISPATCH_DTYPE(dtype, TQ, return hd == 64 ? (ps_launch<TQ, 64>(p, T, stream)) : (ps_launch<TQ, 128>(p, T, stream)));
+extern "C" int bg_packed_select_bytes() { return (int)sizeof(PsParams); }
+
+// out[row][kv head][top]: the pages that row `row` (of request `row`) reads, ascending, -1 behind them.
+extern "C" int bg_packed_select(const void* call, cudaStream_t stream) {
+    const PsParams& p = *(const PsParams*)call;
+    if (p.hd != 64 && p.hd != 128) return BG_ERR_UNSUPPORTED;
+    if (p.T <= 0) return BG_OK;
+    if (p.page_size <= 0 || p.page_size % PK_TILE || p.nkv <= 0 || p.nkv > 65535 || p.nh <= 0 || p.nh % p.nkv || p.num_pages <= 0 || p.max_pages <= 0) return BG_ERR_SHAPE;
+    if (p.block_bytes % 16 || p.block_bytes < p.page_size / PK_TILE * packed_tile_bytes(p.hd) + 4 * p.hd || (uintptr_t)p.pool % 16) return BG_ERR_ALIGN;
+    if (p.top <= 0 || p.first < 0 || p.recent < 1 || p.first + p.recent > p.top || p.pages_most <= 0) return BG_ERR_SHAPE;
+    if (p.pages_most > PS_FLOATS) return BG_ERR_UNSUPPORTED;
+    BG_DISPATCH_DTYPE(p.dtype, TQ, return p.hd == 64 ? (ps_launch<TQ, 64>(p, stream)) : (ps_launch<TQ, 128>(p, stream)));
 }
