@@ -24,100 +24,143 @@ struct PkAppend {
     int src_dtype, q_dtype, parts, max_pages, num_pages, page_size, T, n_req, nh, nkv, hd, rot, interleaved, pad;
 };
 
-// Four neighbouring features of a row (summed over partial results).
+// Eight neighbouring features of a row (summed over partial results).
 template <typename T>
-__device__ __forceinline__ void load4_parts(const T* p, int parts, long long stride, float (&v)[4]);
-template <>
-__device__ __forceinline__ void load4_parts<float>(const float* p, int parts, long long stride, float (&v)[4]) {
-    float4 a = *reinterpret_cast<const float4*>(p);
+__device__ __forceinline__ void load8_parts(const T* p, int parts, long long stride, float (&v)[8]) {
+    load8(p, v);
     for (int i = 1; i < parts; ++i) {
-        const float4 b = *reinterpret_cast<const float4*>(p + i * stride);
-        a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
-    }
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-}
-template <>
-__device__ __forceinline__ void load4_parts<__nv_bfloat16>(const __nv_bfloat16* p, int parts, long long stride, float (&v)[4]) {
-    v[0] = v[1] = v[2] = v[3] = 0.0f;
-    for (int i = 0; i < parts; ++i) {
-        const uint2 r = *reinterpret_cast<const uint2*>(p + i * stride);
-        const float w[4] = {__uint_as_float(r.x << 16), __uint_as_float(r.x & 0xffff0000u), __uint_as_float(r.y << 16), __uint_as_float(r.y & 0xffff0000u)};
+        float w[8];
+        load8(p + i * stride, w);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = i ? v[j] + w[j] : w[j];
+        for (int j = 0; j < 8; ++j) v[j] += w[j];
     }
 }
-__device__ __forceinline__ void store4(float* p, const float (&v)[4]) { *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]); }
-__device__ __forceinline__ void store4(__nv_bfloat16* p, const float (&v)[4]) {
-    uint2 r;
-    __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&r);
-    h[0] = __floats2bfloat162_rn(v[0], v[1]); h[1] = __floats2bfloat162_rn(v[2], v[3]);
-    *reinterpret_cast<uint2*>(p) = r;
+// The (cos, sin) of features f .. f + 7's rotation and their partners in the row (SPLIT: halves of whole pieces of 8; else anything, neighbours or halves).
+template <typename T, bool SPLIT>
+__device__ __forceinline__ void rotation8(const PkAppend& p, const T* head, const float2* table, int f, const float (&x)[8], float (&y)[8], float (&cs)[8], float (&sn)[8]) {
+    const int half = p.rot / 2;
+    if constexpr (SPLIT) {
+        const bool front = f < half;
+        load8_parts<T>(head + (front ? f + half : f - half), p.parts, p.part_stride, y);
+        const float4* from = reinterpret_cast<const float4*>(table + (front ? f : f - half));
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+            const float4 c = from[j / 2];
+            cs[j] = c.x; sn[j] = front ? -c.y : c.y; cs[j + 1] = c.z; sn[j + 1] = front ? -c.w : c.w;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int at = f + j;
+            cs[j] = 1.0f; sn[j] = 0.0f; y[j] = 0.0f;
+            if (at >= p.rot) continue;
+            const float2 c = table[p.interleaved ? at / 2 : at < half ? at : at - half];
+            cs[j] = c.x;
+            sn[j] = (p.interleaved ? at % 2 == 0 : at < half) ? -c.y : c.y;              // (a cos - b sin, and b cos + a sin for the partner)
+            y[j] = p.interleaved ? x[j ^ 1] : sum_parts(head + (at < half ? at + half : at - half), p.parts, (size_t)p.part_stride);
+        }
+    }
 }
 
-// HD / 4 lanes take a head of a row, a lane four neighbouring features; a group's 16 lanes find its smallest and largest by shuffles, and two lanes' codes make
-// a word.  One row and a few heads a CTA: the rows of a decoding step are spread over the SMs.
-// The codes are those that 64 bits give: everything is done in 32 first, with a bound on how far off that may be, and where the bound reaches the border of
-// two codes, or of two roundings of the pair, the warp does its heads again in 64 (two or three warps of a thousand).
+// Queries: HD / 16 lanes take a head of a row, a lane two pieces of 8 features: with SPLIT a piece and its partner, so that each is read once.
 constexpr int PK_THREADS = 256;
-template <typename TS, typename TQ, int HD>
-__global__ void __launch_bounds__(PK_THREADS) packed_append_kernel(const PkAppend p) {
-    constexpr int LANES = HD / 4, EACH = PK_THREADS / LANES;
+template <typename TS, typename TQ, int HD, bool SPLIT>
+__device__ __forceinline__ void append_query(const PkAppend& p, long long item, int l) {
+    const int t = (int)(item / p.nh), h = (int)(item - (long long)t * p.nh);
+    const TS* head = reinterpret_cast<const TS*>(p.src) + (size_t)t * p.src_stride + (size_t)h * HD;
+    const float2* table = reinterpret_cast<const float2*>(p.cos_sin) + (size_t)t * (p.rot / 2);
+    TQ* out = reinterpret_cast<TQ*>(p.q_out) + (size_t)t * p.q_stride + (size_t)h * HD;
+    float a[8], b[8];
+    if constexpr (SPLIT) {
+        const int half = p.rot / 2;
+        const bool turned = 8 * l < half;
+        const int f = turned ? 8 * l : p.rot + 2 * (8 * l - half), g = turned ? f + half : f + 8;
+        load8_parts<TS>(head + f, p.parts, p.part_stride, a);
+        load8_parts<TS>(head + g, p.parts, p.part_stride, b);
+        if (turned) {
+            const float4* from = reinterpret_cast<const float4*>(table + f);
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) {
+                const float4 c = from[j / 2];
+                const float a0 = a[j], a1 = a[j + 1];
+                a[j] = __fadd_rn(__fmul_rn(a0, c.x), -__fmul_rn(b[j], c.y));
+                b[j] = __fadd_rn(__fmul_rn(b[j], c.x), __fmul_rn(a0, c.y));
+                a[j + 1] = __fadd_rn(__fmul_rn(a1, c.z), -__fmul_rn(b[j + 1], c.w));
+                b[j + 1] = __fadd_rn(__fmul_rn(b[j + 1], c.z), __fmul_rn(a1, c.w));
+            }
+        }
+        store8(out + f, a);
+        store8(out + g, b);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int f = 16 * l + 8 * i;
+            float y[8], cs[8], sn[8];
+            load8_parts<TS>(head + f, p.parts, p.part_stride, a);
+            if (f < p.rot) {
+                rotation8<TS, false>(p, head, table, f, a, y, cs, sn);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) a[j] = __fadd_rn(__fmul_rn(a[j], cs[j]), __fmul_rn(y[j], sn[j]));
+            }
+            store8(out + f, a);
+        }
+    }
+}
+
+// Keys and values: HD / 8 lanes take a head of a row, a lane eight neighbouring features, which are a word of codes; a group's 8 lanes find its smallest and
+// largest by shuffles.  The codes are those that 64 bits give: everything is done in 32 first, with a bound on how far off that may be, and where the bound
+// reaches the border of two codes, or of two roundings of the pair, the warp does its heads again in 64 (two or three warps of a thousand).  The border itself,
+// (k + 1/2) step, has 13 bits and is exact, so a difference x - lowest that is exact (bfloat16 that was not rotated) needs no more than a comparison; no
+// division is made in 32 bits.
+// The first CTAs take the queries' heads, the others the keys' and values', both row after row: bound by the latency of a CTA (its loads, one behind the
+// other), so every lane has work and as many CTAs as can be are under way.  4,917 rows of 36 heads: 90 us with a CTA for some heads of one row, four
+// features a lane and every head on the keys' path.
+template <typename TS, typename TQ, int HD, bool SPLIT>
+__global__ void __launch_bounds__(PK_THREADS, 4) packed_append_kernel(const PkAppend p, int query_ctas) {
+    constexpr int LANES = HD / 8;
     pdl_launch();
-    const int head = blockIdx.y * EACH + threadIdx.x / LANES, l = threadIdx.x % LANES, f = l * 4;
-    const int heads = p.nh + 2 * p.nkv;
-    const bool idle = head >= heads;                   // (stays for the shuffles)
-    const int t = blockIdx.x, h = idle ? 0 : head;
-    const TS* row = reinterpret_cast<const TS*>(p.src) + (size_t)t * p.src_stride + (size_t)h * HD;
     pdl_wait();
-    float x[4], far[4] = {}, cs[4], sn[4];             // far: |x cos| + |its partner sin|, where the feature is rotated
-    float y[4] = {};                                   // its partner
-    load4_parts<TS>(row + f, p.parts, p.part_stride, x);
-    const bool turned = h < p.nh + p.nkv && f < p.rot;
-    const int half = p.rot / 2;
+    if ((int)blockIdx.x < query_ctas) {
+        const long long item = (long long)blockIdx.x * (PK_THREADS / (HD / 16)) + threadIdx.x / (HD / 16);
+        if (item < (long long)p.T * p.nh) append_query<TS, TQ, HD, SPLIT>(p, item, threadIdx.x % (HD / 16));
+        return;
+    }
+    const long long item = (long long)((int)blockIdx.x - query_ctas) * (PK_THREADS / LANES) + threadIdx.x / LANES;
+    const int l = threadIdx.x % LANES, f = l * 8;
+    const bool idle = item >= (long long)p.T * 2 * p.nkv;              // (stays for the shuffles)
+    const int t = idle ? 0 : (int)(item / (2 * p.nkv)), h = p.nh + (idle ? 0 : (int)(item - (long long)t * 2 * p.nkv));
+    const TS* row = reinterpret_cast<const TS*>(p.src) + (size_t)t * p.src_stride + (size_t)h * HD;
+    const bool key = h < p.nh + p.nkv;
+    // (where the row goes is looked up while its features are on their way)
+    const int pos = p.positions[t], req = p.row_req[t];
+    float x[8], y[8] = {}, cs[8], sn[8];               // y: a feature's partner
+    load8_parts<TS>(row + f, p.parts, p.part_stride, x);
+    int page = -1, at = 0;
+    if (pos >= 0 && req >= 0 && req < p.n_req) {
+        const int index = pos / p.page_size;
+        at = pos - index * p.page_size;
+        if (index < p.max_pages) page = p.block_table[(size_t)req * p.max_pages + index];
+    }
+    const bool turned = key && f < p.rot;
+    float r[8], off = 0.0f;                            // off: the largest |x cos| + |partner sin|
     if (turned) {
-        const float2* table = reinterpret_cast<const float2*>(p.cos_sin) + (size_t)t * half;
-        if (!p.interleaved) {
-            if (half % 4 == 0) {
-                load4_parts<TS>(row + (f < half ? f + half : f - half), p.parts, p.part_stride, y);
-            } else {
+        rotation8<TS, SPLIT>(p, row, reinterpret_cast<const float2*>(p.cos_sin) + (size_t)t * (p.rot / 2), f, x, y, cs, sn);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int at = f + j;
-                    y[j] = at < p.rot ? sum_parts(row + (at < half ? at + half : at - half), p.parts, (size_t)p.part_stride) : 0.0f;
-                }
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) y[j] = x[j ^ 1];
+        for (int j = 0; j < 8; ++j) {
+            const float a = __fmul_rn(x[j], cs[j]), b = __fmul_rn(y[j], sn[j]);
+            r[j] = __fadd_rn(a, b);
+            off = fmaxf(off, fabsf(a) + fabsf(b));
         }
+    } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int at = f + j;
-            if (at < p.rot) {
-                const float2 c = table[p.interleaved ? at / 2 : at < half ? at : at - half];
-                cs[j] = c.x;
-                sn[j] = (p.interleaved ? at % 2 == 0 : at < half) ? -c.y : c.y;      // (a cos - b sin, and b cos + a sin for the partner)
-            } else {
-                cs[j] = 1.0f; sn[j] = 0.0f;
-            }
-        }
+        for (int j = 0; j < 8; ++j) r[j] = x[j];
     }
-    float r[4];
+    float lo = r[0], hi = r[0], nought = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        r[j] = turned && f + j < p.rot ? __fadd_rn(__fmul_rn(x[j], cs[j]), __fmul_rn(y[j], sn[j])) : x[j];
-        if (turned) far[j] = fabsf(x[j] * cs[j]) + fabsf(y[j] * sn[j]);
-    }
-    if (h < p.nh) {
-        if (!idle) store4(reinterpret_cast<TQ*>(p.q_out) + (size_t)t * p.q_stride + (size_t)h * HD + f, r);
-    }
-    if (__all_sync(0xffffffffu, idle || h < p.nh)) return;
-    float lo = fminf(fminf(r[0], r[1]), fminf(r[2], r[3])), hi = fmaxf(fmaxf(r[0], r[1]), fmaxf(r[2], r[3]));
-    float off = fmaxf(fmaxf(far[0], far[1]), fmaxf(far[2], far[3]));
-    const float nought = __fmul_rn(0.0f, r[0]) + __fmul_rn(0.0f, r[1]) + __fmul_rn(0.0f, r[2]) + __fmul_rn(0.0f, r[3]);
+    for (int j = 0; j < 8; ++j) { lo = fminf(lo, r[j]); hi = fmaxf(hi, r[j]); nought = fmaf(0.0f, r[j], nought); }
     int sound = nought == 0.0f;                        // (nought times what is not finite is no number)
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) {
+    for (int o = 4; o > 0; o >>= 1) {
         lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
         hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
         off = fmaxf(off, __shfl_xor_sync(0xffffffffu, off, o));
@@ -133,22 +176,27 @@ __global__ void __launch_bounds__(PK_THREADS) packed_append_kernel(const PkAppen
     float by = s > 0.0f ? s : 1.0f;                    // (a group of one value: every code 0)
     int near = __bfloat16_as_ushort(__float2bfloat16_rn(lo - off)) != __bfloat16_as_ushort(__float2bfloat16_rn(lo + off))
             || __bfloat16_as_ushort(__float2bfloat16_rn(span - span_off)) != __bfloat16_as_ushort(__float2bfloat16_rn(span + span_off));
-    float u[4];
+    const float inv = __frcp_rn(by);
+    float u[8];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const float d = __fsub_rn(r[j], base), v = __fdiv_rn(d, by);
-        u[j] = rintf(v);
-        // bfloat16 as it came, and a difference without rounding: then the quotient is a border only if it is one in 64 bits too
+    for (int j = 0; j < 8; ++j) {
+        const float d = __fsub_rn(r[j], base), k = floorf(d * inv), border = __fmul_rn(k + 0.5f, by), over = __fsub_rn(d, border);
+        u[j] = over > 0.0f || (over == 0.0f && ((int)k & 1)) ? k + 1.0f : k;
+        // (the two errors of the difference x - lowest: both nought where it is exact)
         const bool sure = sizeof(TS) == 2 && p.parts == 1 && !turned && __fadd_rn(d, base) == r[j] && __fsub_rn(r[j], d) == base;
-        near |= !sure && fabsf(fabsf(v - u[j]) - 0.5f) <= off / by + 3e-6f && v > -1.0f && v < 16.0f;
+        near |= !sure && fabsf(over) <= off + 2.5e-7f * (fabsf(d) + fabsf(border));
     }
-    if (__any_sync(0xffffffffu, near && sound && !idle && h >= p.nh)) {
-        double w[4];
+    if (!(by >= 1e-36f)) near = 1;                     // (a step whose reciprocal or borders leave the normal range)
+    if (__any_sync(0xffffffffu, near && sound && !idle)) {
+        double w[8], least64, most64;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = turned && f + j < p.rot ? (double)x[j] * cs[j] + (double)y[j] * sn[j] : (double)x[j];
-        double least64 = fmin(fmin(w[0], w[1]), fmin(w[2], w[3])), most64 = fmax(fmax(w[0], w[1]), fmax(w[2], w[3]));
+        for (int j = 0; j < 8; ++j) {
+            w[j] = turned ? (double)x[j] * cs[j] + (double)y[j] * sn[j] : (double)x[j];
+            least64 = j ? fmin(least64, w[j]) : w[j];
+            most64 = j ? fmax(most64, w[j]) : w[j];
+        }
 #pragma unroll
-        for (int o = 8; o > 0; o >>= 1) {
+        for (int o = 4; o > 0; o >>= 1) {
             least64 = fmin(least64, __shfl_xor_sync(0xffffffffu, least64, o));
             most64 = fmax(most64, __shfl_xor_sync(0xffffffffu, most64, o));
         }
@@ -158,34 +206,29 @@ __global__ void __launch_bounds__(PK_THREADS) packed_append_kernel(const PkAppen
         s = __bfloat162float(step);
         by = s > 0.0f ? s : 1.0f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) u[j] = (float)rint((w[j] - (double)base) / (double)by);
+        for (int j = 0; j < 8; ++j) u[j] = (float)rint((w[j] - (double)base) / (double)by);
     }
+    if (idle) return;
     unsigned word = 0;
-    const bool key = h < p.nh + p.nkv;
-    const int odd = l & 1;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const int e = odd * 4 + j;
-        word |= (unsigned)fminf(fmaxf(u[j], 0.0f), 15.0f) << (4 * (key ? e / 2 + 4 * (e % 2) : e));
+    for (int e = 0; e < 8; ++e) {
+        const unsigned code = (unsigned)fminf(fmaxf(u[e], 0.0f), 15.0f);
+        word |= key ? code << (4 * (e / 2 + 4 * (e % 2))) : code << (4 * e);
     }
     if (!sound) {
         lowest = step = __float2bfloat16_rn(__int_as_float(0x7fffffff));
         word = 0;
     }
-    word |= __shfl_xor_sync(0xffffffffu, word, 1);
-    if (idle || h < p.nh) return;
-    const int pos = p.positions[t], req = p.row_req[t], index = pos / p.page_size;
-    const int page = pos >= 0 && req >= 0 && req < p.n_req && index < p.max_pages ? p.block_table[(size_t)req * p.max_pages + index] : -1;
     if (page < 0 || page >= p.num_pages) {
         if (p.status && l == 0) atomicOr(p.status, BG_STATUS_BAD_PAGE);
         return;
     }
-    const int at = pos % p.page_size, slot = at % PK_TILE, kvh = (h - p.nh) % p.nkv;
+    const int slot = at % PK_TILE, kvh = h - p.nh - (key ? 0 : p.nkv);
     unsigned char* tile = p.pool + ((size_t)page * p.nkv + kvh) * p.block_bytes + (size_t)(at / PK_TILE) * Packed<HD>::TILE;
-    if (!odd) *reinterpret_cast<unsigned*>(tile + (key ? Packed<HD>::key_word(slot, f) : Packed<HD>::value_word(slot, f))) = word;
-    if (l % 16 == 0) {
+    *reinterpret_cast<unsigned*>(tile + (key ? Packed<HD>::key_word(slot, f) : Packed<HD>::value_word(slot, f))) = word;
+    if (l % 8 == 0) {
         const unsigned pair = (unsigned)__bfloat16_as_ushort(step) | (unsigned)__bfloat16_as_ushort(lowest) << 16;
-        *reinterpret_cast<unsigned*>(tile + Packed<HD>::pair_word(slot, key ? 0 : 1, l / 16)) = pair;
+        *reinterpret_cast<unsigned*>(tile + Packed<HD>::pair_word(slot, key ? 0 : 1, l / 8)) = pair;
     }
 }
 
@@ -225,9 +268,11 @@ __global__ void __launch_bounds__(PK_THREADS) packed_rows_kernel(const PkRead p)
 }
 
 // ------------------------------------------------------------------------------------------------ bounds of filled pages
-// A row that fills its page (its position is the page's last) has the CTA of its (row, kv head) find the smallest and largest value of every feature of the
-// page's keys, as they are read back.  What a page's bounds are hangs on the page alone, whoever wrote it and in how many steps.  A thread takes a word of 8
-// features of every (PK_THREADS / words)-th position; a value that is no number stays one.
+// A row that fills its page (its position is the page's last) has the CTA of its rows find the smallest and largest value of every feature of the page's keys, as
+// they are read back.  What a page's bounds are hangs on the page alone, whoever wrote it and in how many steps.  A CTA looks at PK_ROWS rows of one kv head; for
+// one that fills its page a thread takes a word of 8 features of every (PK_THREADS / words)-th position; a value that is no number stays one.  (A CTA for every
+// row: 26 us for 4,917 rows, of CTAs that had nothing to do; a warp for every row: 19 us for the page that one row fills.)
+constexpr int PK_ROWS = 8;
 __device__ __forceinline__ float least(float a, float b) { return a < b || a != a ? a : b; }
 __device__ __forceinline__ float most(float a, float b) { return a > b || a != a ? a : b; }
 template <int HD>
@@ -235,38 +280,42 @@ __global__ void __launch_bounds__(PK_THREADS) packed_bounds_kernel(const PkRead 
     constexpr int WORDS = HD / 8, AT_ONCE = PK_THREADS / WORDS;
     __shared__ float ends[2][AT_ONCE][HD + 1];
     pdl_launch();
-    const int t = blockIdx.x, kvh = blockIdx.y;
+    const int kvh = blockIdx.y, row0 = blockIdx.x * PK_ROWS, lane = threadIdx.x % 32;
     pdl_wait();
-    const int pos = p.positions[t];
-    if (pos < 0 || pos % p.page_size != p.page_size - 1) return;
-    const int req = p.row_req[t], index = pos / p.page_size;
-    const int page = req >= 0 && req < p.n_req && index < p.max_pages ? p.block_table[(size_t)req * p.max_pages + index] : -1;
-    if (page < 0 || page >= p.num_pages) {
-        if (p.status && threadIdx.x == 0) atomicOr(p.status, BG_STATUS_BAD_PAGE);
-        return;
-    }
-    unsigned char* block = p.pool + ((size_t)page * p.nkv + kvh) * p.block_bytes;
+    const int mine = lane < PK_ROWS && row0 + lane < p.T ? p.positions[row0 + lane] : -1;
+    unsigned full = __ballot_sync(0xffffffffu, mine >= 0 && mine % p.page_size == p.page_size - 1);          // (the same in every warp)
     const int w = threadIdx.x % WORDS, first = threadIdx.x / WORDS, f = w * 8;
-    float lo[8], hi[8];
+    for (; full; full &= full - 1) {
+        const int t = row0 + __ffs(full) - 1, req = p.row_req[t], index = p.positions[t] / p.page_size;
+        const int page = req >= 0 && req < p.n_req && index < p.max_pages ? p.block_table[(size_t)req * p.max_pages + index] : -1;
+        if (page < 0 || page >= p.num_pages) {
+            if (p.status && threadIdx.x == 0) atomicOr(p.status, BG_STATUS_BAD_PAGE);
+            continue;
+        }
+        unsigned char* block = p.pool + ((size_t)page * p.nkv + kvh) * p.block_bytes;
+        float lo[8], hi[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) { lo[e] = INFINITY; hi[e] = -INFINITY; }
-    for (int at = first; at < p.page_size; at += AT_ONCE) {
-        const unsigned char* tile = block + (size_t)(at / PK_TILE) * Packed<HD>::TILE;
-        float v[8];
-        packed_values<true>(*reinterpret_cast<const unsigned*>(tile + Packed<HD>::key_word(at % PK_TILE, f)),
-                            *reinterpret_cast<const unsigned*>(tile + Packed<HD>::pair_word(at % PK_TILE, 0, f / PK_GROUP)), v);
+        for (int e = 0; e < 8; ++e) { lo[e] = INFINITY; hi[e] = -INFINITY; }
+#pragma unroll 4
+        for (int at = first; at < p.page_size; at += AT_ONCE) {
+            const unsigned char* tile = block + (size_t)(at / PK_TILE) * Packed<HD>::TILE;
+            float v[8];
+            packed_values<true>(*reinterpret_cast<const unsigned*>(tile + Packed<HD>::key_word(at % PK_TILE, f)),
+                                *reinterpret_cast<const unsigned*>(tile + Packed<HD>::pair_word(at % PK_TILE, 0, f / PK_GROUP)), v);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) { lo[e] = least(v[e], lo[e]); hi[e] = most(v[e], hi[e]); }
-    }
+            for (int e = 0; e < 8; ++e) { lo[e] = least(v[e], lo[e]); hi[e] = most(v[e], hi[e]); }
+        }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) { ends[0][first][f + e] = lo[e]; ends[1][first][f + e] = hi[e]; }
-    __syncthreads();
-    __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(block + (size_t)(p.page_size / PK_TILE) * Packed<HD>::TILE);
-    for (int i = threadIdx.x; i < 2 * HD; i += PK_THREADS) {
-        const int end = i / HD, feature = i % HD;
-        float v = ends[end][0][feature];
-        for (int j = 1; j < AT_ONCE; ++j) v = end ? most(ends[1][j][feature], v) : least(ends[0][j][feature], v);
-        out[i] = __float2bfloat16_rn(v);
+        for (int e = 0; e < 8; ++e) { ends[0][first][f + e] = lo[e]; ends[1][first][f + e] = hi[e]; }
+        __syncthreads();
+        __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(block + (size_t)(p.page_size / PK_TILE) * Packed<HD>::TILE);
+        for (int i = threadIdx.x; i < 2 * HD; i += PK_THREADS) {
+            const int end = i / HD, feature = i % HD;
+            float v = ends[end][0][feature];
+            for (int j = 1; j < AT_ONCE; ++j) v = end ? most(ends[1][j][feature], v) : least(ends[0][j][feature], v);
+            out[i] = __float2bfloat16_rn(v);
+        }
+        __syncthreads();
     }
 }
 
@@ -394,8 +443,14 @@ static int packed_shape(int hd, int page_size, int nkv, int num_pages, long long
 
 template <typename TS, typename TQ, int HD>
 static int append_launch(const PkAppend& p, cudaStream_t stream) {
-    const int each = PK_THREADS / (HD / 4), heads = p.nh + 2 * p.nkv;
-    cudaError_t e = launch(packed_append_kernel<TS, TQ, HD>, dim3(p.T, (heads + each - 1) / each), dim3(PK_THREADS), 0, stream, p);
+    const long long each_q = PK_THREADS / (HD / 16), each = PK_THREADS / (HD / 8);
+    const long long queries = ((long long)p.T * p.nh + each_q - 1) / each_q, others = ((long long)p.T * 2 * p.nkv + each - 1) / each;
+    if (queries + others > 0x7fffffffLL) return BG_ERR_SHAPE;
+    const dim3 grid((unsigned)(queries + others));
+    // (halves of whole pieces of 8 features, whose table rows are whole float4s)
+    const bool split = !p.interleaved && p.rot % 16 == 0 && (uintptr_t)p.cos_sin % 16 == 0;
+    cudaError_t e = split ? launch(packed_append_kernel<TS, TQ, HD, true>, grid, dim3(PK_THREADS), 0, stream, p, (int)queries)
+                          : launch(packed_append_kernel<TS, TQ, HD, false>, grid, dim3(PK_THREADS), 0, stream, p, (int)queries);
     return e == cudaSuccess ? BG_OK : (int)e;
 }
 
@@ -414,10 +469,9 @@ extern "C" int bg_packed_append(const void* call, cudaStream_t stream) {
     if (int e = packed_shape(p.hd, p.page_size, p.nkv, p.num_pages, p.block_bytes, false)) return e;
     if (p.T <= 0) return BG_OK;
     if (p.parts < 1 || p.nh <= 0 || p.rot < 0 || p.rot > p.hd || p.rot % 2 || p.max_pages <= 0 || (p.rot && !p.cos_sin)) return BG_ERR_SHAPE;
-    const long long fine = p.src_dtype == BG_DTYPE_F32 ? 15 : 7, fine_q = p.q_dtype == BG_DTYPE_F32 ? 15 : 7;
     const long long size = p.src_dtype == BG_DTYPE_F32 ? 4 : 2, size_q = p.q_dtype == BG_DTYPE_F32 ? 4 : 2;
-    if (((long long)(uintptr_t)p.src | p.src_stride * size | (p.parts > 1 ? p.part_stride * size : 0)) & fine
-        || ((long long)(uintptr_t)p.q_out | p.q_stride * size_q) & fine_q || (uintptr_t)p.pool % 16 || (uintptr_t)p.cos_sin % 8) return BG_ERR_ALIGN;
+    if (((long long)(uintptr_t)p.src | p.src_stride * size | (p.parts > 1 ? p.part_stride * size : 0)) & 15
+        || ((long long)(uintptr_t)p.q_out | p.q_stride * size_q) & 15 || (uintptr_t)p.pool % 16 || (uintptr_t)p.cos_sin % 8) return BG_ERR_ALIGN;
     BG_DISPATCH_DTYPE(p.src_dtype, TS, BG_DISPATCH_DTYPE(p.q_dtype, TQ, return p.hd == 64 ? (append_launch<TS, TQ, 64>(p, stream)) : (append_launch<TS, TQ, 128>(p, stream))));
 }
 
@@ -438,8 +492,9 @@ extern "C" int bg_packed_bounds(const void* call, cudaStream_t stream) {
     if (int e = packed_shape(p.hd, p.page_size, p.nkv, p.num_pages, p.block_bytes, true)) return e;
     if (p.T <= 0) return BG_OK;
     if ((uintptr_t)p.pool % 16) return BG_ERR_ALIGN;
-    cudaError_t e = p.hd == 64 ? launch(packed_bounds_kernel<64>, dim3(p.T, p.nkv), dim3(PK_THREADS), 0, stream, p)
-                               : launch(packed_bounds_kernel<128>, dim3(p.T, p.nkv), dim3(PK_THREADS), 0, stream, p);
+    const dim3 grid((p.T + PK_ROWS - 1) / PK_ROWS, p.nkv);
+    cudaError_t e = p.hd == 64 ? launch(packed_bounds_kernel<64>, grid, dim3(PK_THREADS), 0, stream, p)
+                               : launch(packed_bounds_kernel<128>, grid, dim3(PK_THREADS), 0, stream, p);
     return e == cudaSuccess ? BG_OK : (int)e;
 }
 
