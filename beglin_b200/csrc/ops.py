@@ -221,6 +221,7 @@ _SIGNATURES = {
                              _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_void_p, _c_float, _c_void_p, _c_void_p],
     "bg_packed_attention_columns": [_c_int, _c_int, _c_int, ctypes.POINTER(_c_int)],
     "bg_packed_attention_bytes": [],
+    "bg_packed_attention_blocks": [],
     "bg_packed_attention": [_c_void_p, _c_void_p],
     "bg_packed_select_most": [],
     "bg_packed_select_bytes": [],
@@ -1041,12 +1042,14 @@ def packed_plan(lens, nh: int, nkv: int, hd: int, dtype: torch.dtype, page_size:
     return PackedPlan(lens, [int(r) for r in row_start], nh, nkv, hd, dtype, page_size, device, starts)
 
 
-def packed_splits(n_streams: int, positions: int, at_once: int) -> int:
-    """How many CTAs share the positions of one (block of rows, kv head): those that make one wave of the `at_once` CTAs that run side by side, three waves where a
-    wave holds less than two of a stream (lengths differ), and none with fewer than 256 positions of the longest stream."""
-    most = -(-positions // 256)
-    want = at_once // n_streams if 2 * n_streams <= at_once else 3 * at_once // n_streams
-    return max(1, min(most, want))
+def packed_ctas(streams: int, blocks: int, positions: int, at_once: int) -> int:
+    """How many CTAs share the positions of all streams (a kv head of a block of rows) evenly: the `at_once` that run side by side, or as many as have 256 positions
+    of streams of `positions`.  0: a CTA a stream, where no stream is longer than that, or where there are so many that they even out (or that a CTA does not
+    sum up their lengths)."""
+    units = -(-positions // 256)
+    if units <= 1 or streams >= 16 * at_once or blocks > lib().bg_packed_attention_blocks():
+        return 0
+    return min(at_once, streams * units)
 
 
 def packed_attention(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor, positions: torch.Tensor, nh: int, nkv: int, hd: int, page_size: int,
@@ -1091,18 +1094,18 @@ def packed_attention(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Ten
             cols, each = _packed_columns(nh // nkv, f32, most)
             streams = nkv * -(-(nh // nkv) // each)
             read = min(max_position + 1, top * page_size if top else max_position + 1, window + most if window else max_position + 1)
-            splits = packed_splits(n * streams, read, sm_count(q.device) * (2 if cols == 8 and not f32 else 1))
+            ctas = packed_ctas(n * streams, n, read, sm_count(q.device) * (2 if cols == 8 and not f32 else 1))
             part_o = part_ml = 0
-            if splits > 1:
-                results = n * streams * splits * cols
+            if ctas:
+                results = 2 * ctas * cols
                 scratch = torch.empty((results * (hd + 2),), dtype=torch.float32, device=q.device)
                 part_o = scratch.data_ptr()
                 part_ml = part_o + 4 * hd * results
             fields = _PACKED_ATTENTION.pack(_at(q), _at(pool), _at(block_table), _at(positions), 0 if plan is None else _at(plan.short), _at(pages), part_o, part_ml,
                                             _at(out), _at(sink_weight), _at(status), q.stride(0), block, out.stride(0), _dt(q), pool.shape[0], page_size,
-                                            block_table.shape[1], block_table.shape[0], n, most, top, splits, nh, nkv, hd, window, 1 if sink else 0, scale, softcap)
+                                            block_table.shape[1], block_table.shape[0], n, most, top, ctas, nh, nkv, hd, window, 1 if sink else 0, scale, softcap)
             _check(L.bg_packed_attention(fields, _stream()), "packed_attention")
-            count_launches(1 if splits > 1 else 0)
+            count_launches(1 if ctas else 0)
         if plan is not None and plan.n_long:
             end = max_position + 1 if plan.long_end is None else min(plan.long_end, max_position + 1)
             size = L.bg_packed_wide_page()

@@ -27,6 +27,7 @@
 namespace bg {
 
 constexpr int PA_WARPS = 8, PA_THREADS = PA_WARPS * 32, PA_STAGES = 3;
+constexpr int PA_BLOCKS = 1024;            // blocks of rows whose units a CTA sums up
 constexpr float PA_LOG2E = 1.4426950408889634f;
 
 // What a call brings; the host side packs the fields in their order.
@@ -35,18 +36,36 @@ struct PaCall {
     const int* table; const int* positions;
     const int* blocks;                 // [n][3]: request, first row, rows; null: block i is row i of request i
     const int* list;                   // [rows][nkv][top] page indexes to read (less than 0: none), or null: all
-    float* part_o; float* part_ml;     // [block][kv head and head block][split][column][HD], [..][2]; null: finished rows go to `out`
+    float* part_o; float* part_ml;     // [CTA][2][column][HD], [..][2]: what a CTA has of a stream that it shares with others
     void* out; const float* sink_w; unsigned* status;
     long long q_stride, block_bytes, out_stride;
     int dtype, num_pages, page_size, max_pages, n_req;
     int n, rows;                       // blocks, and the most rows of one
-    int top, splits, nh, nkv, hd, window, sink;
+    int top;
+    int ctas;                          // CTAs that share all streams' positions evenly; 0: a CTA a stream
+    int nh, nkv, hd, window, sink;
     float scale, softcap;
 };
 struct PaParams : PaCall {
     int group, head_blocks, heads_each;            // query heads of a kv head, the blocks that they are cut into, heads of a block
+    int heads_all;                                 // kv heads times head blocks: a stream is one of them of one block of rows
     float scale_log2, cap_log2, scale_over_cap;
 };
+
+// The chunks of KEYS positions that a block of rows reads: the first one, and how many (of a list, from its first entry on).
+struct PaChunks { int first, count; };
+__device__ __forceinline__ PaChunks pa_chunks(const PaParams& p, int keys, int row0, int rows) {
+    const int pos_first = p.positions[row0], pos_last = p.positions[row0 + rows - 1];
+    if (pos_last < 0) return {0, 0};
+    if (p.list) return {0, min(p.top, pos_last / p.page_size + 1) * (p.page_size / keys)};
+    const int first = (p.window > 0 ? max(0, pos_first - p.window + 1) : 0) / keys;
+    return {first, pos_last / keys + 1 - first};
+}
+// ... in units of a chunk for each warp, one at least (a block without positions has results too).
+__device__ __forceinline__ int pa_units(const PaParams& p, int keys, int block) {
+    const int row0 = p.blocks ? p.blocks[3 * block + 1] : block, rows = p.blocks ? p.blocks[3 * block + 2] : 1;
+    return max(1, (pa_chunks(p, keys, row0, rows).count + PA_WARPS - 1) / PA_WARPS);
+}
 
 __device__ __forceinline__ void pa_mma(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
@@ -98,6 +117,7 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ unsigned long long bars[PA_WARPS][PA_STAGES];
     __shared__ int where[PA_WARPS][PA_STAGES];         // a stage's first position, or -1: nothing to read
+    __shared__ int before[PA_BLOCKS + PA_WARPS];       // units of a head's blocks in front of each block
     __shared__ int gave_up;
     pdl_launch();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -105,25 +125,79 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
     if (threadIdx.x == 0) gave_up = 0;
     mbar_init_fence();
     __syncthreads();
-    const int block = blockIdx.x / p.splits, split = blockIdx.x % p.splits, kvh = blockIdx.y / p.head_blocks, head0 = blockIdx.y % p.head_blocks * p.heads_each;
-    const int heads = min(p.heads_each, p.group - head0);
     pdl_wait();
+    // ---- what this CTA reads.  The streams (a kv head, or a block of its query heads, of a block of rows; the blocks of one head one behind the other) are cut
+    // in units of PA_WARPS chunks, and the CTAs share the units evenly, whatever the lengths: a CTA's run of units begins and ends inside streams, whose results
+    // packed_merge_kernel joins, and those that lie inside the run are finished here.  (A fixed number of CTAs for every stream left 64 rows of 2,048 to 8,192
+    // positions, 2 kv heads, at 40 us for the longest ones; shared evenly: see below.)
+    long long unit = 0, stop = 1;
+    int per_head = 1;
+    if (p.ctas) {
+        int mine[PA_BLOCKS / PA_THREADS], sum = 0;
+#pragma unroll
+        for (int i = 0; i < PA_BLOCKS / PA_THREADS; ++i) {
+            const int b = threadIdx.x * (PA_BLOCKS / PA_THREADS) + i;
+            mine[i] = b < p.n ? pa_units(p, KEYS, b) : 0;
+            sum += mine[i];
+        }
+        int upto = sum;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, upto, d);
+            if (lane >= d) upto += v;
+        }
+        if (lane == 31) before[PA_BLOCKS + warp] = upto;
+        __syncthreads();
+        for (int w = 0; w < PA_WARPS; ++w) {
+            if (w < warp) upto += before[PA_BLOCKS + w];
+            per_head = w ? per_head + before[PA_BLOCKS + w] : before[PA_BLOCKS];
+        }
+        upto -= sum;
+#pragma unroll
+        for (int i = 0; i < PA_BLOCKS / PA_THREADS; ++i) {
+            before[threadIdx.x * (PA_BLOCKS / PA_THREADS) + i] = upto;
+            upto += mine[i];
+        }
+        __syncthreads();
+        const long long units = (long long)per_head * p.heads_all;
+        const long long share = min((long long)p.ctas, units);          // (none without a unit: the merge counts on it)
+        unit = blockIdx.x < share ? blockIdx.x * units / share : 0;
+        stop = blockIdx.x < share ? (blockIdx.x + 1) * units / share : 0;
+    }
+    int stage = 0;
+    unsigned phase = 0;
+    while (unit < stop) {
+    int block, hy, u0 = 0, u1 = 0x7fffffff / PA_WARPS, u_all = u1;
+    if (p.ctas) {
+        hy = (int)(unit / per_head);
+        const int r = (int)(unit - (long long)hy * per_head);
+        int low = 0, high = p.n - 1;                   // the last block that begins at or before r
+        while (low < high) {
+            const int mid = (low + high + 1) / 2;
+            if (before[mid] <= r) low = mid;
+            else high = mid - 1;
+        }
+        block = low;
+        u_all = (block + 1 < p.n ? before[block + 1] : per_head) - before[block];
+        u0 = r - before[block];
+        u1 = (int)min((long long)u_all, u0 + stop - unit);
+        unit += u1 - u0;
+    } else {
+        block = blockIdx.x; hy = blockIdx.y;
+        ++unit;
+    }
+    const bool finished = u0 == 0 && u1 == u_all;
+    const int kvh = hy / p.head_blocks, head0 = hy % p.head_blocks * p.heads_each;
+    const int heads = min(p.heads_each, p.group - head0);
     int req = block, row0 = block, rows = 1;
     if (p.blocks) { req = p.blocks[3 * block]; row0 = p.blocks[3 * block + 1]; rows = p.blocks[3 * block + 2]; }
     const int cols = min(rows * heads, COLS), pos_first = p.positions[row0], pos_last = p.positions[row0 + rows - 1];
-    const int lo = p.window > 0 ? max(0, pos_first - p.window + 1) : 0;
     const int per_page = p.page_size / KEYS;
     const int* list = p.list ? p.list + ((size_t)row0 * p.nkv + kvh) * p.top : nullptr;
-    const int chunk0 = list ? 0 : lo / KEYS;
-    const int chunks = pos_last < 0 ? 0 : list ? min(p.top, pos_last / p.page_size + 1) * per_page : pos_last / KEYS + 1 - chunk0;
-    const int per = ((chunks + p.splits - 1) / p.splits + PA_WARPS - 1) / PA_WARPS * PA_WARPS;
-    const int begin = split * per + warp, end = min(chunks, (split + 1) * per);
+    const PaChunks all = pa_chunks(p, KEYS, row0, rows);
+    const int chunk0 = all.first, begin = u0 * PA_WARPS + warp, end = min(all.count, u1 * PA_WARPS);
     const int turns = begin < end ? (end - begin + PA_WARPS - 1) / PA_WARPS : 0;
-    const size_t slot = (((size_t)block * gridDim.y + blockIdx.y) * p.splits + split) * COLS;
-    if (p.part_o && split * per >= chunks) {           // no range of this request is left for this CTA
-        if (threadIdx.x < COLS) reinterpret_cast<float2*>(p.part_ml)[slot + threadIdx.x] = make_float2(-INFINITY, 0.0f);
-        return;
-    }
+    const size_t slot = ((size_t)blockIdx.x * 2 + (u0 == 0)) * COLS;     // (a run's first stream may have begun before it, its last one may go on behind it)
 
     // ---- copies: a lane looks up the page of one of the warp's next 32 turns
     unsigned char* ring = smem + (size_t)warp * PA_STAGES * BYTES;
@@ -165,12 +239,12 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
     if (turns > 0) look_up(0);
 #pragma unroll
     for (int i = 0; i < PA_STAGES; ++i)
-        if (i < turns) issue(i, i);
+        if (i < turns) issue(i, stage + i < PA_STAGES ? stage + i : stage + i - PA_STAGES);
 
     // ---- queries: column g of every block of 8, features 64 group + 16 t .. + 15 as four steps of a product
     // (those that meet codes at bits 4 are a 16th)
     unsigned qf[PARTS][NT][GROUPS][8];
-    float qsum[NT][GROUPS][2], unit[NT][2];            // of columns 2t, 2t + 1 of every block: the sum of a group, and what the column's scores are multiplied with
+    float qsum[NT][GROUPS][2], mult[NT][2];            // of columns 2t, 2t + 1 of every block: the sum of a group, and what the column's scores are multiplied with
     int seen[NT][2];                                   // the positions of their rows
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -220,7 +294,7 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
             seen[nt][j] = mine < cols ? p.positions[row0 + mine / heads] : pos_last;
             // back from 2^(100 - high) and the codes' 2^-133 to q . k, times what makes it an exponent of two (or, squashed, a part of the bound)
             const int back = min(33 + __shfl_sync(0xffffffffu, high, (2 * t + j) * 4), 127);
-            unit[nt][j] = __uint_as_float((unsigned)(127 + back) << 23) * (p.cap_log2 > 0.0f ? p.scale_over_cap : p.scale_log2);
+            mult[nt][j] = __uint_as_float((unsigned)(127 + back) << 23) * (p.cap_log2 > 0.0f ? p.scale_over_cap : p.scale_log2);
         }
     }
 
@@ -296,7 +370,7 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        if (!(EDGE && (hidden >> ((i * NT + nt) * 4 + e) & 1))) x[i][nt][e] = pa_squashed<F32>(x[i][nt][e] * unit[nt][e & 1], p.cap_log2);
+                        if (!(EDGE && (hidden >> ((i * NT + nt) * 4 + e) & 1))) x[i][nt][e] = pa_squashed<F32>(x[i][nt][e] * mult[nt][e & 1], p.cap_log2);
         }
         // the running maximum, and what it does to what there is
         float top[NT][2];
@@ -310,7 +384,7 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
                 for (int i = 0; i < CT; ++i) v = fmaxf(v, fmaxf(x[i][nt][j], x[i][nt][j + 2]));
 #pragma unroll
                 for (int d = 4; d < 32; d <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
-                if (!capped) v *= unit[nt][j];
+                if (!capped) v *= mult[nt][j];
                 top[nt][j] = fmaxf(m[nt][j], v);
                 grew |= top[nt][j] > m[nt][j];
             }
@@ -341,7 +415,7 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float z = fmaf(x[i][nt][e], capped ? 1.0f : unit[nt][e & 1], less[nt][e & 1]);
+                    const float z = fmaf(x[i][nt][e], capped ? 1.0f : mult[nt][e & 1], less[nt][e & 1]);
                     w[nt][e] = F32 ? exp2f(z) : pa_exp2(z);
                     l[nt][e & 1] += w[nt][e];
                 }
@@ -406,8 +480,7 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
     };
 
     bool fine = true;
-    int turn = 0, stage = 0;
-    unsigned phase = 0;
+    int turn = 0;
     for (; turn < turns; ++turn) {
         fine = __all_sync(0xffffffffu, mbar_wait(&bars[warp][stage], phase, &gave_up));
         if (!fine) break;
@@ -426,7 +499,10 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
     }
     if (!fine) {                                       // a copy did not come: the others of this warp are waited for, and the status says so
         if (lane == 0 && p.status) atomicOr(p.status, BG_STATUS_TIMEOUT);
-        for (int i = turn; i < min(turns, turn + PA_STAGES); ++i) mbar_wait(&bars[warp][i % PA_STAGES], (i / PA_STAGES) & 1);
+        for (int i = turn; i < min(turns, turn + PA_STAGES); ++i) {
+            mbar_wait(&bars[warp][stage], phase);
+            if (++stage == PA_STAGES) { stage = 0; phase ^= 1u; }
+        }
     }
 
     // ---- the warps' results meet
@@ -475,7 +551,7 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
             sum = fmaf(each[w].y, each[w].x == -INFINITY ? 1.0f : by, sum);
             v.x = fmaf(a.x, by, v.x); v.y = fmaf(a.y, by, v.y);
         }
-        if (p.part_o) {
+        if (!finished) {
             reinterpret_cast<float2*>(p.part_o + (slot + col) * HD)[i % (HD / 2)] = v;
             if (f == 0) reinterpret_cast<float2*>(p.part_ml)[slot + col] = make_float2(top, sum);
             continue;
@@ -492,49 +568,71 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
         if constexpr (F32) *reinterpret_cast<float2*>(out) = make_float2(v.x * by, v.y * by);
         else *reinterpret_cast<__nv_bfloat162*>(out) = __floats2bfloat162_rn(v.x * by, v.y * by);
     }
+    if (unit >= stop) break;
+    fence_proxy_async();                               // (copies come to where the results stood)
+    __syncthreads();
+    if (gave_up) break;
+    }
 }
 
-// out = sum_i o_i 2^(m_i - m) / sum_i l_i 2^(m_i - m) over the ranges of a column; EACH warps take every EACH-th range and join in their order.
+// out = sum_i o_i 2^(m_i - m) / sum_i l_i 2^(m_i - m) over the CTAs that share a stream (a stream that one CTA had is done); EACH warps take every EACH-th of
+// them and join in their order.
 constexpr int PM_WARPS = 8;
 template <int HD, bool F32, int EACH>
-__global__ void __launch_bounds__(PM_WARPS * 32) packed_merge_kernel(const PaParams p, int cols_most) {
+__global__ void __launch_bounds__(PM_WARPS * 32) packed_merge_kernel(const PaParams p, int cols_most, int keys) {
     constexpr int PER = HD / 32, AT_ONCE = 8;
     using TQ = typename std::conditional<F32, float, __nv_bfloat16>::type;
     __shared__ float acc_s[PM_WARPS][HD];
     __shared__ float2 ml_s[PM_WARPS];
+    __shared__ int sums[2][PM_WARPS];
     pdl_launch();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp % EACH;
-    const int block = blockIdx.x, kvh = blockIdx.y / p.head_blocks, head0 = blockIdx.y % p.head_blocks * p.heads_each, heads = min(p.heads_each, p.group - head0);
+    const int block = blockIdx.x, hy = blockIdx.y, kvh = hy / p.head_blocks, head0 = hy % p.head_blocks * p.heads_each, heads = min(p.heads_each, p.group - head0);
     const int col = blockIdx.z * (PM_WARPS / EACH) + warp / EACH;
     pdl_wait();
+    int ahead = 0, per_head = 0;
+    for (int b = threadIdx.x; b < p.n; b += PM_WARPS * 32) {
+        const int u = pa_units(p, keys, b);
+        per_head += u;
+        if (b < block) ahead += u;
+    }
+    ahead = __reduce_add_sync(0xffffffffu, ahead);
+    per_head = __reduce_add_sync(0xffffffffu, per_head);
+    if (lane == 0) { sums[0][warp] = ahead; sums[1][warp] = per_head; }
+    __syncthreads();
+    ahead = per_head = 0;
+#pragma unroll
+    for (int w = 0; w < PM_WARPS; ++w) { ahead += sums[0][w]; per_head += sums[1][w]; }
+    const long long units = (long long)per_head * p.heads_all, at = (long long)hy * per_head + ahead;
+    const long long share = min((long long)p.ctas, units);
+    const int first = (int)(((at + 1) * share - 1) / units), last = (int)(((at + pa_units(p, keys, block)) * share - 1) / units), parts = last - first + 1;
+    if (parts == 1) return;
     int row0 = block, rows = 1;
     if (p.blocks) { row0 = p.blocks[3 * block + 1]; rows = p.blocks[3 * block + 2]; }
     const bool idle = col >= rows * heads || col >= cols_most;
-    const size_t base = ((size_t)block * gridDim.y + blockIdx.y) * p.splits * cols_most + (idle ? 0 : col);
+    // the first CTA has its part in its second place, the others theirs in their first
+    auto place = [&](int i) { return ((size_t)(first + i) * 2 + (i == 0)) * cols_most + (idle ? 0 : col); };
     float m = -INFINITY, l = 0.0f, acc[PER] = {};
-    for (int i0 = part; !idle && i0 < p.splits; i0 += AT_ONCE * EACH) {
+    for (int i0 = part; !idle && i0 < parts; i0 += AT_ONCE * EACH) {
         float2 ml[AT_ONCE];
         float v[AT_ONCE][PER];
-#pragma unroll
-        for (int j = 0; j < AT_ONCE; ++j) {
-            const int i = i0 + j * EACH;
-            ml[j] = i < p.splits ? reinterpret_cast<const float2*>(p.part_ml)[base + (size_t)i * cols_most] : make_float2(-INFINITY, 0.0f);
-        }
         float top = m;
 #pragma unroll
         for (int j = 0; j < AT_ONCE; ++j) {
             const int i = i0 + j * EACH;
-            const bool have = ml[j].x != -INFINITY || ml[j].y != 0.0f;         // (a range without positions has written no more than that)
-            const float* from = p.part_o + (base + (size_t)i * cols_most) * HD + lane * PER;
+            const bool have = i < parts;
+            const size_t from = place(have ? i : 0);
+            ml[j] = have ? reinterpret_cast<const float2*>(p.part_ml)[from] : make_float2(-INFINITY, 0.0f);
             if constexpr (PER == 4) {
-                const float4 a = have ? *reinterpret_cast<const float4*>(from) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                const float4 a = have ? *reinterpret_cast<const float4*>(p.part_o + from * HD + lane * PER) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                 v[j][0] = a.x; v[j][1] = a.y; v[j][2] = a.z; v[j][3] = a.w;
             } else {
-                const float2 a = have ? *reinterpret_cast<const float2*>(from) : make_float2(0.0f, 0.0f);
+                const float2 a = have ? *reinterpret_cast<const float2*>(p.part_o + from * HD + lane * PER) : make_float2(0.0f, 0.0f);
                 v[j][0] = a.x; v[j][1] = a.y;
             }
-            top = fmaxf(top, ml[j].x);
         }
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; ++j) top = fmaxf(top, ml[j].x);
         const float from = top == -INFINITY ? 0.0f : top, keep = m == -INFINITY ? 1.0f : exp2f(m - from);
         l *= keep;
 #pragma unroll
@@ -593,12 +691,14 @@ static int pa_launch(const PaParams& p, int n, cudaStream_t stream) {
     const size_t ring = (size_t)PA_WARPS * PA_STAGES * CT * Packed<HD>::TILE, join = PaShape<HD, NT, F32>::JOIN, smem = ring > join ? ring : join;
     cudaError_t e = smem_limit(packed_attention_kernel<HD, NT, F32, CT>, smem);
     if (e != cudaSuccess) return (int)e;
-    e = launch(packed_attention_kernel<HD, NT, F32, CT>, dim3((unsigned)((long long)n * p.splits), p.nkv * p.head_blocks), dim3(PA_THREADS), smem, stream, p);
+    const dim3 grid = p.ctas ? dim3(p.ctas) : dim3(n, p.heads_all);
+    e = launch(packed_attention_kernel<HD, NT, F32, CT>, grid, dim3(PA_THREADS), smem, stream, p);
     if (e != cudaSuccess) return (int)e;
-    if (!p.part_o) return BG_OK;
-    constexpr int COLS = 8 * NT;
-    e = p.splits > 8 ? launch(packed_merge_kernel<HD, F32, PM_WARPS>, dim3(n, p.nkv * p.head_blocks, COLS), dim3(PM_WARPS * 32), 0, stream, p, COLS)
-                     : launch(packed_merge_kernel<HD, F32, 1>, dim3(n, p.nkv * p.head_blocks, NT), dim3(PM_WARPS * 32), 0, stream, p, COLS);
+    if (!p.ctas) return BG_OK;
+    constexpr int COLS = 8 * NT, KEYS = CT * PK_TILE;
+    // (many CTAs a stream: a CTA joins one column, not a warp)
+    e = p.ctas > 8 * n * p.heads_all ? launch(packed_merge_kernel<HD, F32, PM_WARPS>, dim3(n, p.heads_all, COLS), dim3(PM_WARPS * 32), 0, stream, p, COLS, KEYS)
+                                     : launch(packed_merge_kernel<HD, F32, 1>, dim3(n, p.heads_all, NT), dim3(PM_WARPS * 32), 0, stream, p, COLS, KEYS);
     return e == cudaSuccess ? BG_OK : (int)e;
 }
 
@@ -624,22 +724,25 @@ extern "C" int bg_packed_attention_columns(int group, int f32, int rows, int* he
     return *heads_each * rows <= 8 ? 1 : 2;
 }
 
+// The most blocks whose positions CTAs share.
+extern "C" int bg_packed_attention_blocks() { return PA_BLOCKS; }
+
 extern "C" int bg_packed_attention_bytes() { return (int)sizeof(PaCall); }
 
-// part_o / part_ml hold n * nkv * head_blocks * splits * columns results where splits > 1.
+// part_o / part_ml hold 2 * ctas * columns results.
 extern "C" int bg_packed_attention(const void* call, cudaStream_t stream) {
     const PaCall& c = *(const PaCall*)call;
     if (c.hd != 64 && c.hd != 128) return BG_ERR_UNSUPPORTED;
     if (c.n <= 0) return BG_OK;
-    if (c.page_size <= 0 || c.page_size % PK_TILE || c.nkv <= 0 || c.nh <= 0 || c.nh % c.nkv || c.splits <= 0 || c.num_pages <= 0 || c.max_pages <= 0
+    if (c.page_size <= 0 || c.page_size % PK_TILE || c.nkv <= 0 || c.nh <= 0 || c.nh % c.nkv || c.ctas < 0 || c.num_pages <= 0 || c.max_pages <= 0
         || c.window < 0 || !(c.scale > 0.0f)) return BG_ERR_SHAPE;
-    if (c.block_bytes % 16 || c.block_bytes < c.page_size / PK_TILE * packed_tile_bytes(c.hd) || (long long)c.n * c.splits > 0x7fffffffLL
+    if (c.block_bytes % 16 || c.block_bytes < c.page_size / PK_TILE * packed_tile_bytes(c.hd) || (c.ctas && c.n > PA_BLOCKS)
         || (c.list && (c.top <= 0 || c.rows != 1))) return BG_ERR_SHAPE;
     if (c.dtype != BG_DTYPE_F32 && c.dtype != BG_DTYPE_BF16) return BG_ERR_DTYPE;
     const bool f32 = c.dtype == BG_DTYPE_F32;
     const long long size = f32 ? 4 : 2;
     if ((uintptr_t)c.pool % 16 || ((long long)(uintptr_t)c.q | c.q_stride * size) % 16 || ((long long)(uintptr_t)c.out | c.out_stride * size) % (2 * size)) return BG_ERR_ALIGN;
-    if ((c.splits > 1) != (c.part_o != nullptr) || (c.part_o == nullptr) != (c.part_ml == nullptr) || (uintptr_t)c.part_o % 16 || (uintptr_t)c.part_ml % 8) return BG_ERR_SHAPE;
+    if ((c.ctas > 0) != (c.part_o != nullptr) || (c.part_o == nullptr) != (c.part_ml == nullptr) || (uintptr_t)c.part_o % 16 || (uintptr_t)c.part_ml % 8) return BG_ERR_SHAPE;
     PaParams p;
     static_cast<PaCall&>(p) = c;
     const int nt = bg_packed_attention_columns(c.nh / c.nkv, f32, c.rows, &p.heads_each);
@@ -647,6 +750,7 @@ extern "C" int bg_packed_attention(const void* call, cudaStream_t stream) {
     p.group = c.nh / c.nkv;
     p.head_blocks = (p.group + p.heads_each - 1) / p.heads_each;
     if ((long long)c.nkv * p.head_blocks > 65535) return BG_ERR_SHAPE;
+    p.heads_all = c.nkv * p.head_blocks;
     p.scale_log2 = c.scale * PA_LOG2E;
     p.cap_log2 = c.softcap > 0.0f ? c.softcap * PA_LOG2E : 0.0f;
     p.scale_over_cap = c.softcap > 0.0f ? c.scale / c.softcap : 0.0f;

@@ -178,10 +178,11 @@ def test_plans_refuse_what_does_not_fit():
         ops.packed_plan([1, 2], 4, 2, 64, BF16, 64, device="cpu", starts=[0])
 
 
-@pytest.mark.parametrize("streams,positions,at_once", [(1, 1, 296), (2, 4096, 296), (128, 8192, 296), (16, 131072, 148), (5000, 100, 296), (149, 100000, 296)])
-def test_ranges_of_a_stream_have_work(streams, positions, at_once):
-    n = ops.packed_splits(streams, positions, at_once)
-    assert 1 <= n <= max(1, -(-positions // 256)) and (n == 1 or n * streams <= 3 * at_once)
+@pytest.mark.parametrize("streams,positions,at_once", [(1, 1, 296), (2, 4096, 296), (128, 8192, 296), (16, 131072, 148), (900, 100, 296), (149, 100000, 296), (5000, 9999, 296)])
+def test_ctas_that_share_streams_have_work(streams, positions, at_once):
+    n = ops.packed_ctas(streams, min(streams, 64), positions, at_once)
+    assert n <= at_once and n <= streams * -(-positions // 256) and (n > 0) == (positions > 256 and streams < 16 * at_once)
+    assert ops.packed_ctas(2, 1025, 100000, 296) == 0
 
 
 # ------------------------------------------------------------------------------------------------ append
