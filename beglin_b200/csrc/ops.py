@@ -1098,7 +1098,7 @@ def packed_attention(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Ten
             part_o = part_ml = 0
             if ctas:
                 results = 2 * ctas * cols
-                scratch = torch.empty((results * (hd + 2),), dtype=torch.float32, device=q.device)
+                scratch = torch.empty((results * (hd + 2) + 2 * n * streams,), dtype=torch.float32, device=q.device)
                 part_o = scratch.data_ptr()
                 part_ml = part_o + 4 * hd * results
             fields = _PACKED_ATTENTION.pack(_at(q), _at(pool), _at(block_table), _at(positions), 0 if plan is None else _at(plan.short), _at(pages), part_o, part_ml,

@@ -26,7 +26,7 @@
 
 namespace bg {
 
-constexpr int PA_WARPS = 8, PA_THREADS = PA_WARPS * 32, PA_STAGES = 3;
+constexpr int PA_WARPS = 8, PA_THREADS = PA_WARPS * 32, PA_STAGES = 2;
 constexpr int PA_BLOCKS = 1024;            // blocks of rows whose units a CTA sums up
 constexpr float PA_LOG2E = 1.4426950408889634f;
 
@@ -36,7 +36,7 @@ struct PaCall {
     const int* table; const int* positions;
     const int* blocks;                 // [n][3]: request, first row, rows; null: block i is row i of request i
     const int* list;                   // [rows][nkv][top] page indexes to read (less than 0: none), or null: all
-    float* part_o; float* part_ml;     // [CTA][2][column][HD], [..][2]: what a CTA has of a stream that it shares with others
+    float* part_o; float* part_ml;     // (with ctas) [CTA][2][column][HD], [..][2]: what a CTA has of a stream that it shares with others
     void* out; const float* sink_w; unsigned* status;
     long long q_stride, block_bytes, out_stride;
     int dtype, num_pages, page_size, max_pages, n_req;
@@ -48,6 +48,7 @@ struct PaCall {
 };
 struct PaParams : PaCall {
     int group, head_blocks, heads_each;            // query heads of a kv head, the blocks that they are cut into, heads of a block
+    int2* shared_by;                               // [block][heads_all]: the first CTA that has a part of a stream, and how many have
     int heads_all;                                 // kv heads times head blocks: a stream is one of them of one block of rows
     float scale_log2, cap_log2, scale_over_cap;
 };
@@ -164,10 +165,14 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
         unit = blockIdx.x < share ? blockIdx.x * units / share : 0;
         stop = blockIdx.x < share ? (blockIdx.x + 1) * units / share : 0;
     }
-    int stage = 0;
-    unsigned phase = 0;
-    while (unit < stop) {
-    int block, hy, u0 = 0, u1 = 0x7fffffff / PA_WARPS, u_all = u1;
+    // What is left of the stream that holds `unit`, as far as this CTA's run goes: where its copies come from, and which of them this warp waits for.
+    int block, hy, u0, turns, begin, end, chunk0, req, pos_last;
+    bool finished;
+    const int* list;
+    const int per_page = p.page_size / KEYS;
+    auto next_stream = [&]() {
+    block = blockIdx.x; hy = blockIdx.y; u0 = 0;
+    int u1 = 0x7fffffff / PA_WARPS, u_all = u1;
     if (p.ctas) {
         hy = (int)(unit / per_head);
         const int r = (int)(unit - (long long)hy * per_head);
@@ -182,22 +187,24 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
         u0 = r - before[block];
         u1 = (int)min((long long)u_all, u0 + stop - unit);
         unit += u1 - u0;
+        // (the CTA with a stream's first unit says where its parts are, for the merge)
+        if (u0 == 0 && threadIdx.x == 0) {
+            const long long units = (long long)per_head * p.heads_all, share = min((long long)p.ctas, units), at = (long long)hy * per_head + r;
+            p.shared_by[(size_t)block * p.heads_all + hy] = make_int2(blockIdx.x, (int)(((at + u_all) * share - 1) / units) - (int)blockIdx.x + 1);
+        }
     } else {
-        block = blockIdx.x; hy = blockIdx.y;
         ++unit;
     }
-    const bool finished = u0 == 0 && u1 == u_all;
-    const int kvh = hy / p.head_blocks, head0 = hy % p.head_blocks * p.heads_each;
-    const int heads = min(p.heads_each, p.group - head0);
-    int req = block, row0 = block, rows = 1;
+    finished = u0 == 0 && u1 == u_all;
+    req = block;
+    int row0 = block, rows = 1;
     if (p.blocks) { req = p.blocks[3 * block]; row0 = p.blocks[3 * block + 1]; rows = p.blocks[3 * block + 2]; }
-    const int cols = min(rows * heads, COLS), pos_first = p.positions[row0], pos_last = p.positions[row0 + rows - 1];
-    const int per_page = p.page_size / KEYS;
-    const int* list = p.list ? p.list + ((size_t)row0 * p.nkv + kvh) * p.top : nullptr;
+    pos_last = p.positions[row0 + rows - 1];
+    list = p.list ? p.list + ((size_t)row0 * p.nkv + hy / p.head_blocks) * p.top : nullptr;
     const PaChunks all = pa_chunks(p, KEYS, row0, rows);
-    const int chunk0 = all.first, begin = u0 * PA_WARPS + warp, end = min(all.count, u1 * PA_WARPS);
-    const int turns = begin < end ? (end - begin + PA_WARPS - 1) / PA_WARPS : 0;
-    const size_t slot = ((size_t)blockIdx.x * 2 + (u0 == 0)) * COLS;     // (a run's first stream may have begun before it, its last one may go on behind it)
+    chunk0 = all.first; begin = u0 * PA_WARPS + warp; end = min(all.count, u1 * PA_WARPS);
+    turns = begin < end ? (end - begin + PA_WARPS - 1) / PA_WARPS : 0;
+    };
 
     // ---- copies: a lane looks up the page of one of the warp's next 32 turns
     unsigned char* ring = smem + (size_t)warp * PA_STAGES * BYTES;
@@ -221,7 +228,7 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
             if (p.status) atomicOr(p.status, BG_STATUS_BAD_PAGE);
             return;
         }
-        from = p.pool + ((size_t)page * p.nkv + kvh) * p.block_bytes + (size_t)(base % p.page_size / PK_TILE) * L::TILE;
+        from = p.pool + ((size_t)page * p.nkv + hy / p.head_blocks) * p.block_bytes + (size_t)(base % p.page_size / PK_TILE) * L::TILE;
     };
     auto issue = [&](int turn, int stage) {
         const unsigned long long src = __shfl_sync(0xffffffffu, (unsigned long long)from, turn & 31);
@@ -236,10 +243,23 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
             }
         }
     };
-    if (turns > 0) look_up(0);
+    int stage = 0;
+    unsigned phase = 0;
+    bool fine = true;                                  // no wait of this warp has run out
+    auto first_copies = [&]() {
+        if (turns > 0) look_up(0);
 #pragma unroll
-    for (int i = 0; i < PA_STAGES; ++i)
-        if (i < turns) issue(i, stage + i < PA_STAGES ? stage + i : stage + i - PA_STAGES);
+        for (int i = 0; i < PA_STAGES; ++i)
+            if (i < turns) issue(i, stage + i < PA_STAGES ? stage + i : stage + i - PA_STAGES);
+    };
+    if (unit >= stop) return;
+    next_stream();
+    first_copies();
+    for (;;) {
+    const int kvh = hy / p.head_blocks, head0 = hy % p.head_blocks * p.heads_each, heads = min(p.heads_each, p.group - head0);
+    const int row0 = p.blocks ? p.blocks[3 * block + 1] : block, cols = min((p.blocks ? p.blocks[3 * block + 2] : 1) * heads, COLS), pos_first = p.positions[row0];
+    const bool whole = finished;
+    const size_t slot = ((size_t)blockIdx.x * 2 + (u0 == 0)) * COLS;     // (a run's first stream may have begun before it, its last one may go on behind it)
 
     // ---- queries: column g of every block of 8, features 64 group + 16 t .. + 15 as four steps of a product
     // (those that meet codes at bits 4 are a 16th)
@@ -479,11 +499,10 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
         }
     };
 
-    bool fine = true;
     int turn = 0;
-    for (; turn < turns; ++turn) {
+    for (; fine && turn < turns; ++turn) {
         fine = __all_sync(0xffffffffu, mbar_wait(&bars[warp][stage], phase, &gave_up));
-        if (!fine) break;
+        if (!fine) break;                              // (turn stays)
         const int at = where[warp][stage];
         if (at >= 0) {
             if (at + KEYS - 1 > pos_first || (p.window > 0 && at <= pos_last - p.window)) chunk(ring + stage * BYTES, at, std::true_type{});
@@ -497,12 +516,22 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
         }
         if (++stage == PA_STAGES) { stage = 0; phase ^= 1u; }
     }
-    if (!fine) {                                       // a copy did not come: the others of this warp are waited for, and the status says so
+    if (!fine && turn < turns) {
+        // a copy did not come: those of this warp that are on their way are waited for, and the status says so; the warp asks for no more (its results
+        // still meet the others', so that nobody waits for it)
         if (lane == 0 && p.status) atomicOr(p.status, BG_STATUS_TIMEOUT);
         for (int i = turn; i < min(turns, turn + PA_STAGES); ++i) {
             mbar_wait(&bars[warp][stage], phase);
             if (++stage == PA_STAGES) { stage = 0; phase ^= 1u; }
         }
+    }
+
+    // ---- the next stream's copies come while this one's results meet
+    const bool more = unit < stop;
+    if (more) {
+        next_stream();
+        if (fine) first_copies();
+        else turns = 0;
     }
 
     // ---- the warps' results meet
@@ -516,8 +545,8 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
 #pragma unroll
                 for (int gr = 0; gr < GROUPS; ++gr) low[nt][gr][j] += __shfl_xor_sync(0xffffffffu, low[nt][gr][j], d);
             }
-    __syncthreads();                                   // (the rings are read out)
-    float* res = reinterpret_cast<float*>(smem);
+    __syncthreads();                                   // (the stream before this one is read out)
+    float* res = reinterpret_cast<float*>(smem + (size_t)PA_WARPS * PA_STAGES * BYTES);
     float2* ml = reinterpret_cast<float2*>(res + PA_WARPS * COLS * S::ROW);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -551,7 +580,7 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
             sum = fmaf(each[w].y, each[w].x == -INFINITY ? 1.0f : by, sum);
             v.x = fmaf(a.x, by, v.x); v.y = fmaf(a.y, by, v.y);
         }
-        if (!finished) {
+        if (!whole) {
             reinterpret_cast<float2*>(p.part_o + (slot + col) * HD)[i % (HD / 2)] = v;
             if (f == 0) reinterpret_cast<float2*>(p.part_ml)[slot + col] = make_float2(top, sum);
             continue;
@@ -568,10 +597,7 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
         if constexpr (F32) *reinterpret_cast<float2*>(out) = make_float2(v.x * by, v.y * by);
         else *reinterpret_cast<__nv_bfloat162*>(out) = __floats2bfloat162_rn(v.x * by, v.y * by);
     }
-    if (unit >= stop) break;
-    fence_proxy_async();                               // (copies come to where the results stood)
-    __syncthreads();
-    if (gave_up) break;
+    if (!more) break;
     }
 }
 
@@ -579,33 +605,18 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
 // them and join in their order.
 constexpr int PM_WARPS = 8;
 template <int HD, bool F32, int EACH>
-__global__ void __launch_bounds__(PM_WARPS * 32) packed_merge_kernel(const PaParams p, int cols_most, int keys) {
+__global__ void __launch_bounds__(PM_WARPS * 32) packed_merge_kernel(const PaParams p, int cols_most) {
     constexpr int PER = HD / 32, AT_ONCE = 8;
     using TQ = typename std::conditional<F32, float, __nv_bfloat16>::type;
     __shared__ float acc_s[PM_WARPS][HD];
     __shared__ float2 ml_s[PM_WARPS];
-    __shared__ int sums[2][PM_WARPS];
     pdl_launch();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp % EACH;
     const int block = blockIdx.x, hy = blockIdx.y, kvh = hy / p.head_blocks, head0 = hy % p.head_blocks * p.heads_each, heads = min(p.heads_each, p.group - head0);
     const int col = blockIdx.z * (PM_WARPS / EACH) + warp / EACH;
     pdl_wait();
-    int ahead = 0, per_head = 0;
-    for (int b = threadIdx.x; b < p.n; b += PM_WARPS * 32) {
-        const int u = pa_units(p, keys, b);
-        per_head += u;
-        if (b < block) ahead += u;
-    }
-    ahead = __reduce_add_sync(0xffffffffu, ahead);
-    per_head = __reduce_add_sync(0xffffffffu, per_head);
-    if (lane == 0) { sums[0][warp] = ahead; sums[1][warp] = per_head; }
-    __syncthreads();
-    ahead = per_head = 0;
-#pragma unroll
-    for (int w = 0; w < PM_WARPS; ++w) { ahead += sums[0][w]; per_head += sums[1][w]; }
-    const long long units = (long long)per_head * p.heads_all, at = (long long)hy * per_head + ahead;
-    const long long share = min((long long)p.ctas, units);
-    const int first = (int)(((at + 1) * share - 1) / units), last = (int)(((at + pa_units(p, keys, block)) * share - 1) / units), parts = last - first + 1;
+    const int2 by_ = p.shared_by[(size_t)block * p.heads_all + hy];
+    const int first = by_.x, parts = by_.y;
     if (parts == 1) return;
     int row0 = block, rows = 1;
     if (p.blocks) { row0 = p.blocks[3 * block + 1]; rows = p.blocks[3 * block + 2]; }
@@ -688,17 +699,17 @@ __global__ void __launch_bounds__(PM_WARPS * 32) packed_merge_kernel(const PaPar
 
 template <int HD, int NT, bool F32, int CT>
 static int pa_launch(const PaParams& p, int n, cudaStream_t stream) {
-    const size_t ring = (size_t)PA_WARPS * PA_STAGES * CT * Packed<HD>::TILE, join = PaShape<HD, NT, F32>::JOIN, smem = ring > join ? ring : join;
+    const size_t smem = (size_t)PA_WARPS * PA_STAGES * CT * Packed<HD>::TILE + PaShape<HD, NT, F32>::JOIN;      // the rings, and where results meet
     cudaError_t e = smem_limit(packed_attention_kernel<HD, NT, F32, CT>, smem);
     if (e != cudaSuccess) return (int)e;
     const dim3 grid = p.ctas ? dim3(p.ctas) : dim3(n, p.heads_all);
     e = launch(packed_attention_kernel<HD, NT, F32, CT>, grid, dim3(PA_THREADS), smem, stream, p);
     if (e != cudaSuccess) return (int)e;
     if (!p.ctas) return BG_OK;
-    constexpr int COLS = 8 * NT, KEYS = CT * PK_TILE;
+    constexpr int COLS = 8 * NT;
     // (many CTAs a stream: a CTA joins one column, not a warp)
-    e = p.ctas > 8 * n * p.heads_all ? launch(packed_merge_kernel<HD, F32, PM_WARPS>, dim3(n, p.heads_all, COLS), dim3(PM_WARPS * 32), 0, stream, p, COLS, KEYS)
-                                     : launch(packed_merge_kernel<HD, F32, 1>, dim3(n, p.heads_all, NT), dim3(PM_WARPS * 32), 0, stream, p, COLS, KEYS);
+    e = p.ctas > 8 * n * p.heads_all ? launch(packed_merge_kernel<HD, F32, PM_WARPS>, dim3(n, p.heads_all, COLS), dim3(PM_WARPS * 32), 0, stream, p, COLS)
+                                     : launch(packed_merge_kernel<HD, F32, 1>, dim3(n, p.heads_all, NT), dim3(PM_WARPS * 32), 0, stream, p, COLS);
     return e == cudaSuccess ? BG_OK : (int)e;
 }
 
@@ -729,7 +740,7 @@ extern "C" int bg_packed_attention_blocks() { return PA_BLOCKS; }
 
 extern "C" int bg_packed_attention_bytes() { return (int)sizeof(PaCall); }
 
-// part_o / part_ml hold 2 * ctas * columns results.
+// part_o holds 2 * ctas * columns results, part_ml their maxima and sums and, behind them, two whole numbers for every stream.
 extern "C" int bg_packed_attention(const void* call, cudaStream_t stream) {
     const PaCall& c = *(const PaCall*)call;
     if (c.hd != 64 && c.hd != 128) return BG_ERR_UNSUPPORTED;
@@ -751,6 +762,7 @@ extern "C" int bg_packed_attention(const void* call, cudaStream_t stream) {
     p.head_blocks = (p.group + p.heads_each - 1) / p.heads_each;
     if ((long long)c.nkv * p.head_blocks > 65535) return BG_ERR_SHAPE;
     p.heads_all = c.nkv * p.head_blocks;
+    p.shared_by = reinterpret_cast<int2*>(c.part_ml + (size_t)4 * c.ctas * 8 * nt);
     p.scale_log2 = c.scale * PA_LOG2E;
     p.cap_log2 = c.softcap > 0.0f ? c.softcap * PA_LOG2E : 0.0f;
     p.scale_over_cap = c.softcap > 0.0f ? c.scale / c.softcap : 0.0f;
