@@ -875,7 +875,7 @@ PACKED_TILE = 16           # positions of a tile: pages hold whole tiles
 # The calls' fields in the order of the library's structures: one packed record costs the host a tenth of what as many arguments do, which is what a call
 # of a decoding step is bound by.
 _PACKED_APPEND, _PACKED_READ = struct.Struct("<12q14i"), struct.Struct("<7q8i")
-_PACKED_ATTENTION, _PACKED_SELECT = struct.Struct("<14q14i2f"), struct.Struct("<8q12i")
+_PACKED_ATTENTION, _PACKED_SELECT = struct.Struct("<14q16i2f"), struct.Struct("<8q12i")
 
 
 def _at(t: Optional[torch.Tensor]) -> int:
@@ -1042,14 +1042,21 @@ def packed_plan(lens, nh: int, nkv: int, hd: int, dtype: torch.dtype, page_size:
     return PackedPlan(lens, [int(r) for r in row_start], nh, nkv, hd, dtype, page_size, device, starts)
 
 
-def packed_ctas(streams: int, blocks: int, positions: int, at_once: int) -> int:
-    """How many CTAs share the positions of all streams (a kv head of a block of rows) evenly: the `at_once` that run side by side, or as many as have 256 positions
-    of streams of `positions`.  0: a CTA a stream, where no stream is longer than that, or where there are so many that they even out (or that a CTA does not
-    sum up their lengths)."""
+PACKED_TURNS = 6           # units of 256 positions that a CTA of a cluster takes, at most
+
+
+def packed_ctas(streams: int, blocks: int, positions: int, at_once: int) -> Tuple[int, int]:
+    """(CTAs that share the positions of all streams evenly or 0, CTAs of a cluster that share a stream) for streams (a kv head of a block of rows) of up to
+    `positions`, `at_once` CTAs side by side.  Where a cluster of up to 8 CTAs a stream leaves each of them little to do, that: the results meet inside it.  A CTA
+    a stream where streams are so many that they even out (or more than a CTA sums up the lengths of).  Else as many CTAs as run side by side, of which a
+    second kernel joins what they have of a stream."""
     units = -(-positions // 256)
-    if units <= 1 or streams >= 16 * at_once or blocks > lib().bg_packed_attention_blocks():
-        return 0
-    return min(at_once, streams * units)
+    cluster = 1
+    while cluster < 8 and 2 * cluster * streams <= at_once and cluster < units:
+        cluster *= 2
+    if units <= PACKED_TURNS * cluster or streams >= 16 * at_once or blocks > lib().bg_packed_attention_blocks():
+        return 0, cluster
+    return min(at_once, streams * units), 1
 
 
 def packed_attention(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor, positions: torch.Tensor, nh: int, nkv: int, hd: int, page_size: int,
@@ -1094,7 +1101,7 @@ def packed_attention(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Ten
             cols, each = _packed_columns(nh // nkv, f32, most)
             streams = nkv * -(-(nh // nkv) // each)
             read = min(max_position + 1, top * page_size if top else max_position + 1, window + most if window else max_position + 1)
-            ctas = packed_ctas(n * streams, n, read, sm_count(q.device) * (2 if cols == 8 and not f32 else 1))
+            ctas, cluster = packed_ctas(n * streams, n, read, sm_count(q.device) * (2 if cols == 8 and not f32 else 1))
             part_o = part_ml = 0
             if ctas:
                 results = 2 * ctas * cols
@@ -1103,7 +1110,7 @@ def packed_attention(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Ten
                 part_ml = part_o + 4 * hd * results
             fields = _PACKED_ATTENTION.pack(_at(q), _at(pool), _at(block_table), _at(positions), 0 if plan is None else _at(plan.short), _at(pages), part_o, part_ml,
                                             _at(out), _at(sink_weight), _at(status), q.stride(0), block, out.stride(0), _dt(q), pool.shape[0], page_size,
-                                            block_table.shape[1], block_table.shape[0], n, most, top, ctas, nh, nkv, hd, window, 1 if sink else 0, scale, softcap)
+                                            block_table.shape[1], block_table.shape[0], n, most, top, ctas, cluster, nh, nkv, hd, window, 1 if sink else 0, 0, scale, softcap)
             _check(L.bg_packed_attention(fields, _stream()), "packed_attention")
             count_launches(1 if ctas else 0)
         if plan is not None and plan.n_long:

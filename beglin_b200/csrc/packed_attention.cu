@@ -42,8 +42,9 @@ struct PaCall {
     int dtype, num_pages, page_size, max_pages, n_req;
     int n, rows;                       // blocks, and the most rows of one
     int top;
-    int ctas;                          // CTAs that share all streams' positions evenly; 0: a CTA a stream
-    int nh, nkv, hd, window, sink;
+    int ctas;                          // CTAs that share all streams' positions evenly; 0: none is shared so
+    int cluster;                       // (without ctas) CTAs of a cluster that share a stream's positions
+    int nh, nkv, hd, window, sink, pad;
     float scale, softcap;
 };
 struct PaParams : PaCall {
@@ -118,19 +119,25 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ unsigned long long bars[PA_WARPS][PA_STAGES];
     __shared__ int where[PA_WARPS][PA_STAGES];         // a stage's first position, or -1: nothing to read
-    __shared__ int before[PA_BLOCKS + PA_WARPS];       // units of a head's blocks in front of each block
+    // units of a head's blocks in front of each block; or what a cluster's CTAs have of this one's columns
+    constexpr int MEET = COLS * (HD + 2) > PA_BLOCKS + PA_WARPS ? COLS * (HD + 2) : PA_BLOCKS + PA_WARPS;
+    __shared__ __align__(16) int before[MEET];
     __shared__ int gave_up;
     pdl_launch();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     if (threadIdx.x < PA_WARPS * PA_STAGES) mbar_init(&bars[threadIdx.x / PA_STAGES][threadIdx.x % PA_STAGES], 1);
     if (threadIdx.x == 0) gave_up = 0;
     mbar_init_fence();
+    const int ranks = gridDim.z, rank = blockIdx.z;
+    if (ranks > 1) cluster_arrive_relaxed();           // (the others have begun before their memory is written)
     __syncthreads();
+    if (ranks > 1) cluster_wait();
     pdl_wait();
     // ---- what this CTA reads.  The streams (a kv head, or a block of its query heads, of a block of rows; the blocks of one head one behind the other) are cut
     // in units of PA_WARPS chunks, and the CTAs share the units evenly, whatever the lengths: a CTA's run of units begins and ends inside streams, whose results
     // packed_merge_kernel joins, and those that lie inside the run are finished here.  (A fixed number of CTAs for every stream left 64 rows of 2,048 to 8,192
-    // positions, 2 kv heads, at 40 us for the longest ones; shared evenly: see below.)
+        // positions, 2 kv heads, at 40 us for the longest ones.)  Few and short streams have a cluster each instead, whose CTAs take even parts and join them in shared
+    // memory: no second kernel, no scratch.
     long long unit = 0, stop = 1;
     int per_head = 1;
     if (p.ctas) {
@@ -171,8 +178,8 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
     const int* list;
     const int per_page = p.page_size / KEYS;
     auto next_stream = [&]() {
-    block = blockIdx.x; hy = blockIdx.y; u0 = 0;
-    int u1 = 0x7fffffff / PA_WARPS, u_all = u1;
+    block = blockIdx.x; hy = blockIdx.y;
+    int u1, u_all;
     if (p.ctas) {
         hy = (int)(unit / per_head);
         const int r = (int)(unit - (long long)hy * per_head);
@@ -194,6 +201,10 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
         }
     } else {
         ++unit;
+        u_all = pa_units(p, KEYS, block);
+        const int each = (u_all + ranks - 1) / ranks;
+        u0 = rank * each;
+        u1 = min(u_all, u0 + each);
     }
     finished = u0 == 0 && u1 == u_all;
     req = block;
@@ -564,6 +575,19 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
             }
         }
     __syncthreads();
+    auto write = [&](int col, int f, float2 v, float top, float sum) {         // a finished pair of features
+        const int r = col / heads, h = kvh * p.group + head0 + col - r * heads;
+        float by = 1.0f;
+        if (p.sink) {
+            const float at = (p.sink_w ? p.sink_w[h] : 0.0f) * PA_LOG2E, most = fmaxf(top, at);
+            by = top == -INFINITY ? (sum == 0.0f ? 0.0f : 1.0f) : exp2f(top - most);
+            sum = fmaf(sum, by, exp2f(at - most));
+        }
+        by = sum == 0.0f ? 0.0f : by / sum;            // (a row that sees nothing is nought)
+        TQ* out = reinterpret_cast<TQ*>(p.out) + (size_t)(row0 + r) * p.out_stride + (size_t)h * HD + f;
+        if constexpr (F32) *reinterpret_cast<float2*>(out) = make_float2(v.x * by, v.y * by);
+        else *reinterpret_cast<__nv_bfloat162*>(out) = __floats2bfloat162_rn(v.x * by, v.y * by);
+    };
     for (int i = threadIdx.x; i < cols * (HD / 2); i += PA_THREADS) {
         const int col = i / (HD / 2), f = i % (HD / 2) * 2;
         float2 each[PA_WARPS];
@@ -580,22 +604,37 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
             sum = fmaf(each[w].y, each[w].x == -INFINITY ? 1.0f : by, sum);
             v.x = fmaf(a.x, by, v.x); v.y = fmaf(a.y, by, v.y);
         }
+        if (ranks > 1) {                               // to the CTA that joins this column
+            const unsigned at = peer_addr(smem_u32(before), (unsigned)(col % ranks)) + 4u * (unsigned)((rank * ((COLS + ranks - 1) / ranks) + col / ranks) * (HD + 2));
+            st_cluster(at + 4 * f, v.x); st_cluster(at + 4 * f + 4, v.y);
+            if (f == 0) { st_cluster(at + 4 * HD, top); st_cluster(at + 4 * HD + 4, sum); }
+            continue;
+        }
         if (!whole) {
             reinterpret_cast<float2*>(p.part_o + (slot + col) * HD)[i % (HD / 2)] = v;
             if (f == 0) reinterpret_cast<float2*>(p.part_ml)[slot + col] = make_float2(top, sum);
             continue;
         }
-        const int r = col / heads, h = kvh * p.group + head0 + col - r * heads;
-        float by = 1.0f;
-        if (p.sink) {
-            const float at = (p.sink_w ? p.sink_w[h] : 0.0f) * PA_LOG2E, most = fmaxf(top, at);
-            by = top == -INFINITY ? (sum == 0.0f ? 0.0f : 1.0f) : exp2f(top - most);
-            sum = fmaf(sum, by, exp2f(at - most));
+        write(col, f, v, top, sum);
+    }
+    if (ranks > 1) {
+        cluster_sync_all();
+        const int mine = rank < cols ? (cols - rank + ranks - 1) / ranks : 0, apart = (COLS + ranks - 1) / ranks * (HD + 2);
+        for (int i = threadIdx.x; i < mine * (HD / 2); i += PA_THREADS) {
+            const int f = i % (HD / 2) * 2;
+            const float* at = reinterpret_cast<const float*>(before) + i / (HD / 2) * (HD + 2);
+            float top = -INFINITY, sum = 0.0f;
+            for (int c = 0; c < ranks; ++c) top = fmaxf(top, at[c * apart + HD]);
+            const float from = top == -INFINITY ? 0.0f : top;
+            float2 v = make_float2(0.0f, 0.0f);
+            for (int c = 0; c < ranks; ++c) {
+                const float m_c = at[c * apart + HD], by = exp2f(m_c - from);
+                const float2 a = *reinterpret_cast<const float2*>(at + c * apart + f);
+                sum = fmaf(at[c * apart + HD + 1], m_c == -INFINITY ? 1.0f : by, sum);
+                v.x = fmaf(a.x, by, v.x); v.y = fmaf(a.y, by, v.y);
+            }
+            write(rank + i / (HD / 2) * ranks, f, v, top, sum);
         }
-        by = sum == 0.0f ? 0.0f : by / sum;            // (a row that sees nothing is nought)
-        TQ* out = reinterpret_cast<TQ*>(p.out) + (size_t)(row0 + r) * p.out_stride + (size_t)h * HD + f;
-        if constexpr (F32) *reinterpret_cast<float2*>(out) = make_float2(v.x * by, v.y * by);
-        else *reinterpret_cast<__nv_bfloat162*>(out) = __floats2bfloat162_rn(v.x * by, v.y * by);
     }
     if (!more) break;
     }
@@ -702,8 +741,8 @@ static int pa_launch(const PaParams& p, int n, cudaStream_t stream) {
     const size_t smem = (size_t)PA_WARPS * PA_STAGES * CT * Packed<HD>::TILE + PaShape<HD, NT, F32>::JOIN;      // the rings, and where results meet
     cudaError_t e = smem_limit(packed_attention_kernel<HD, NT, F32, CT>, smem);
     if (e != cudaSuccess) return (int)e;
-    const dim3 grid = p.ctas ? dim3(p.ctas) : dim3(n, p.heads_all);
-    e = launch(packed_attention_kernel<HD, NT, F32, CT>, grid, dim3(PA_THREADS), smem, stream, p);
+    const dim3 grid = p.ctas ? dim3(p.ctas) : dim3(n, p.heads_all, p.cluster);
+    e = launch_cluster(packed_attention_kernel<HD, NT, F32, CT>, grid, dim3(PA_THREADS), smem, stream, p.ctas ? 1 : p.cluster, p);
     if (e != cudaSuccess) return (int)e;
     if (!p.ctas) return BG_OK;
     constexpr int COLS = 8 * NT;
@@ -745,7 +784,7 @@ extern "C" int bg_packed_attention(const void* call, cudaStream_t stream) {
     const PaCall& c = *(const PaCall*)call;
     if (c.hd != 64 && c.hd != 128) return BG_ERR_UNSUPPORTED;
     if (c.n <= 0) return BG_OK;
-    if (c.page_size <= 0 || c.page_size % PK_TILE || c.nkv <= 0 || c.nh <= 0 || c.nh % c.nkv || c.ctas < 0 || c.num_pages <= 0 || c.max_pages <= 0
+    if (c.page_size <= 0 || c.page_size % PK_TILE || c.nkv <= 0 || c.nh <= 0 || c.nh % c.nkv || c.ctas < 0 || c.cluster < 1 || c.cluster > 8 || c.num_pages <= 0 || c.max_pages <= 0
         || c.window < 0 || !(c.scale > 0.0f)) return BG_ERR_SHAPE;
     if (c.block_bytes % 16 || c.block_bytes < c.page_size / PK_TILE * packed_tile_bytes(c.hd) || (c.ctas && c.n > PA_BLOCKS)
         || (c.list && (c.top <= 0 || c.rows != 1))) return BG_ERR_SHAPE;

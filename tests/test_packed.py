@@ -180,9 +180,11 @@ def test_plans_refuse_what_does_not_fit():
 
 @pytest.mark.parametrize("streams,positions,at_once", [(1, 1, 296), (2, 4096, 296), (128, 8192, 296), (16, 131072, 148), (900, 100, 296), (149, 100000, 296), (5000, 9999, 296)])
 def test_ctas_that_share_streams_have_work(streams, positions, at_once):
-    n = ops.packed_ctas(streams, min(streams, 64), positions, at_once)
-    assert n <= at_once and n <= streams * -(-positions // 256) and (n > 0) == (positions > 256 and streams < 16 * at_once)
-    assert ops.packed_ctas(2, 1025, 100000, 296) == 0
+    n, cluster = ops.packed_ctas(streams, min(streams, 64), positions, at_once)
+    units = -(-positions // 256)
+    assert n <= at_once and n <= streams * units and cluster in (1, 2, 4, 8) and cluster < 2 * units and (cluster == 1 or cluster * streams <= at_once)
+    assert not n or (cluster == 1 and streams < 16 * at_once and units > ops.PACKED_TURNS)
+    assert ops.packed_ctas(2, 1025, 100000, 296) == (0, 8)
 
 
 # ------------------------------------------------------------------------------------------------ append
