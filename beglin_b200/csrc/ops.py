@@ -1045,14 +1045,14 @@ def packed_plan(lens, nh: int, nkv: int, hd: int, dtype: torch.dtype, page_size:
 PACKED_TURNS = 6           # units of 256 positions that a CTA of a cluster takes, at most
 
 
-def packed_ctas(streams: int, blocks: int, positions: int, at_once: int) -> Tuple[int, int]:
+def packed_ctas(streams: int, blocks: int, positions: int, at_once: int, beside: int = 2) -> Tuple[int, int]:
     """(CTAs that share the positions of all streams evenly or 0, CTAs of a cluster that share a stream) for streams (a kv head of a block of rows) of up to
-    `positions`, `at_once` CTAs side by side.  Where a cluster of up to 8 CTAs a stream leaves each of them little to do, that: the results meet inside it.  A CTA
+    `positions`, `at_once` CTAs side by side, `beside` of them on an SM.  Where a cluster of up to 8 CTAs a stream leaves each of them little to do, that: the results meet inside it.  A CTA
     a stream where streams are so many that they even out (or more than a CTA sums up the lengths of).  Else as many CTAs as run side by side, of which a
     second kernel joins what they have of a stream."""
     units = -(-positions // 256)
-    cluster = 1
-    while cluster < 8 and 2 * cluster * streams <= at_once and cluster < units:
+    cluster, room = 1, at_once if beside > 1 else at_once * 3 // 4         # (CTAs alone on their SMs leave some SMs of a part of the GPU without a cluster)
+    while cluster < 8 and 2 * cluster * streams <= room and cluster < units:
         cluster *= 2
     if units <= PACKED_TURNS * cluster or streams >= 16 * at_once or blocks > lib().bg_packed_attention_blocks():
         return 0, cluster
@@ -1099,9 +1099,10 @@ def packed_attention(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Ten
         n, most = (T, 1) if plan is None else (plan.n_short, plan.most)
         if n:
             cols, each = _packed_columns(nh // nkv, f32, most)
+            beside = 2 if cols == 8 and not f32 else 1           # (what their registers and shared memory allow)
             streams = nkv * -(-(nh // nkv) // each)
             read = min(max_position + 1, top * page_size if top else max_position + 1, window + most if window else max_position + 1)
-            ctas, cluster = packed_ctas(n * streams, n, read, sm_count(q.device) * (2 if cols == 8 and not f32 else 1))
+            ctas, cluster = packed_ctas(n * streams, n, read, sm_count(q.device) * beside, beside)
             part_o = part_ml = 0
             if ctas:
                 results = 2 * ctas * cols

@@ -3,22 +3,24 @@
 // the kv head:
 //     score = max over heads of  sum over features of  max(q lo, q hi)  =  sum of  max(q, 0) hi + min(q, 0) lo.
 //
-// The sums run in 64 bits and are rounded to 32 once: of products of bfloat16 they are exact but for the last few bits of 64, so the scores, and with them the
-// order, do not hang on the order of the sum; equal scores go to the lower page.  A score that is no number counts as the largest one.
+// The choice is that of sums in 64 bits, rounded to 32 once: of products of bfloat16 they are exact but for the last few bits of 64, so the order does not hang
+// on the order of the sum; equal scores go to the lower page.  A score that is no number counts as the largest one.  But 64 bits are only needed next to the
+// border: every page gets its score in 32 bits with a bound E on how far off that may be (2^-17 of the sum of magnitudes; 66 additions make 2^-18), and
+// with A the `top`-th largest of these scores and M the largest bound, a page over A + M + E is in, one under A - M - E is out, and those between, a handful, get
+// their sums in 64 bits.  (All of them in 64 bits: 50 us for 16 rows and heads of 2,000 pages, whose 64-bit multiply-adds alone take 7 and whose reads of
+// the queries from shared memory as much again.)
 //
-// A cluster of CTAs takes one (row, kv head), a CTA a part of the pages, four lanes a page (a quarter of the features each) and as many
-// pages at once as lanes allow, because the 64-bit chain of a page is long (2,000 pages in CTAs of 256 threads, two pages a lane: 41 us); the scores go to the first CTA's shared memory, which finds the border by halving: how many scores
-// reach a threshold, bit by bit from the first that differs, until exactly as many do as are wanted or no bit is left.  (Counting 8 bits at a time with
-// shared-memory atomics put nearly every score of a row into one counter, one after the other: 49 us for 16 rows and heads of 2,000 pages, of which the
-// scores took some 15.)  Bound by latency where there are few rows, else by the 64-bit units (two multiply-adds a feature and head).
-#include <type_traits>
-
+// A cluster of CTAs takes one (row, kv head), a CTA a part of the pages, four lanes two pages at a time (a quarter of the features each); the scores go to the
+// first CTA's shared memory, which finds a border by quartering: how many scores reach a threshold, two bits a round from the first that differs, until exactly as many
+// do as are wanted or no bit is left.  (Counting 8 bits at a time with shared-memory atomics put nearly every score into one counter, one after the other.)
+// Bound by latency: three meetings of the cluster and two searches for a border.
 #include "packed.cuh"
 
 namespace bg {
 
-constexpr int PS_THREADS = 512, PS_CLUSTER = 8, PS_HEADS = 8;      // (the most CTAs of a cluster; query heads at a time)
-constexpr int PS_FLOATS = 50000;           // the most pages: their scores are in shared memory
+constexpr int PS_THREADS = 256, PS_WARPS = PS_THREADS / 32, PS_CLUSTER = 8, PS_HEADS = 8;       // (the most CTAs of a cluster; query heads at a time)
+constexpr int PS_MOST = 36000;             // the most pages: their scores are in shared memory
+constexpr float PS_LARGEST = 3.4028234e38f;
 
 // What a call brings; the host side packs the fields in their order.
 struct PsParams {
@@ -35,16 +37,73 @@ __device__ __forceinline__ unsigned ps_key(float s) {
     const unsigned b = __float_as_uint(s + 0.0f);
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
+__device__ __forceinline__ float ps_score(unsigned key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
+__device__ __forceinline__ void ps_store(unsigned addr, unsigned v) { asm volatile("st.shared::cluster.u32 [%0], %1;\n" ::"r"(addr), "r"(v) : "memory"); }
+
+// The largest threshold that at least `top` of the keys reach, or one that exactly `top` of them reach (then `exactly`), two bits a round.  All threads; a
+// thread has up to PS_KEYS keys in registers (more are read again from shared memory: one read behind the other was most of a round).  `room` holds
+// 2 * PS_WARPS + 32 numbers.
+constexpr int PS_KEYS = 8;
+struct PsBorder { unsigned at; bool exactly; };
+__device__ __forceinline__ PsBorder ps_border(const unsigned* keys, int n, int top, unsigned* room) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const bool few = n <= PS_KEYS * PS_THREADS;
+    unsigned k[PS_KEYS], all = 0xffffffffu, any = 0;
+#pragma unroll
+    for (int j = 0; j < PS_KEYS; ++j) {
+        const int i = tid + j * PS_THREADS;
+        k[j] = i < n ? keys[i] : 0u;                   // (no threshold is nought)
+        if (i < n) { all &= k[j]; any |= k[j]; }
+    }
+    for (int i = tid + PS_KEYS * PS_THREADS; i < n; i += PS_THREADS) { all &= keys[i]; any |= keys[i]; }
+    all = __reduce_and_sync(0xffffffffu, all);
+    any = __reduce_or_sync(0xffffffffu, any);
+    __syncthreads();                                   // (the room's last use)
+    if (lane == 0) { room[warp] = all; room[PS_WARPS + warp] = any; }
+    if (tid < 32) room[2 * PS_WARPS + tid] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < PS_WARPS; ++w) { all &= room[w]; any |= room[PS_WARPS + w]; }
+    const int bits = (32 - __clz(all ^ any) + 1) / 2 * 2;              // the bits that are not the same in all of them, in pairs
+    unsigned border = bits >= 32 ? 0u : all >> bits << bits;
+    int reached = n;
+    for (int bit = bits - 2; bit >= 0 && reached != top; bit -= 2) {
+        unsigned low = 0, high = 0;                    // how many reach the border with 1 (low half) and 2, and with 3, in these two bits
+        const unsigned t1 = border | 1u << bit, t2 = border | 2u << bit, t3 = border | 3u << bit;
+#pragma unroll
+        for (int j = 0; j < PS_KEYS; ++j) {
+            low += (k[j] >= t1 ? 1u : 0u) + (k[j] >= t2 ? 0x10000u : 0u);
+            high += k[j] >= t3 ? 1u : 0u;
+        }
+        if (!few)
+            for (int i = tid + PS_KEYS * PS_THREADS; i < n; i += PS_THREADS) {
+                const unsigned v = keys[i];
+                low += (v >= t1 ? 1u : 0u) + (v >= t2 ? 0x10000u : 0u);
+                high += v >= t3 ? 1u : 0u;
+            }
+        low = __reduce_add_sync(0xffffffffu, low);     // (fewer than 65,536 keys)
+        high = __reduce_add_sync(0xffffffffu, high);
+        if (lane < 2) atomicAdd(&room[2 * PS_WARPS + bit + lane], lane ? high : low);
+        __syncthreads();
+        low = room[2 * PS_WARPS + bit]; high = room[2 * PS_WARPS + bit + 1];
+        const int c1 = (int)(low & 0xffffu), c2 = (int)(low >> 16), c3 = (int)high;
+        if (c3 >= top) { border = t3; reached = c3; }
+        else if (c2 >= top) { border = t2; reached = c2; }
+        else if (c1 >= top) { border = t1; reached = c1; }
+    }
+    return {border, reached == top};
+}
 
 template <typename TQ, int HD>
 __global__ void __launch_bounds__(PS_THREADS) packed_select_kernel(const PsParams p) {
     constexpr int CHUNKS = HD / 8, MINE = CHUNKS / 4;  // pieces of 8 features of a page's bounds, and those of a lane
-    extern __shared__ __align__(16) float scores[];
-    __shared__ double2 q_s[CHUNKS][PS_HEADS * 8 + 1];  // (max(q, 0), min(q, 0)); the odd piece keeps four lanes' reads apart
-    __shared__ unsigned ends_s[2][PS_THREADS / 32];
-    __shared__ int counts[32];                         // of every bit
+    extern __shared__ __align__(16) unsigned keys[];   // the first CTA's: of every page; then this CTA's own (score, bound)
+    __shared__ float2 q_s[CHUNKS][PS_HEADS * 8 + 1];   // (max(q, 0), min(q, 0)); the odd piece keeps four lanes' reads apart
+    __shared__ unsigned room[2 * PS_WARPS + 32];
+    __shared__ float far_of[PS_CLUSTER], cut[2], scratch[32];
+    __shared__ int unsure[PS_THREADS], n_unsure;
     pdl_launch();
-    const int row = blockIdx.x, kvh = blockIdx.y, rank = blockIdx.z, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int row = blockIdx.x, kvh = blockIdx.y, rank = blockIdx.z, ranks = gridDim.z, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     pdl_wait();
     const int pos = p.positions[row], pages = pos < 0 ? 0 : min(pos / p.page_size + 1, p.pages_most);
     const int group = p.nh / p.nkv;
@@ -55,111 +114,176 @@ __global__ void __launch_bounds__(PS_THREADS) packed_select_kernel(const PsParam
             for (int i = tid; i < p.top; i += PS_THREADS) out[i] = i < pages ? i : -1;
         return;
     }
-    cluster_arrive_relaxed();                          // (the first CTA has begun before its memory is written)
+    cluster_arrive_relaxed();                          // (the others have begun before their memory is written)
     cluster_wait();
-    const int each = (pages + (int)gridDim.z - 1) / (int)gridDim.z, from = rank * each, to = min(pages, from + each);
-    const unsigned there = peer_addr(smem_u32(scores), 0);
+    const int each = (pages + ranks - 1) / ranks, from = rank * each, to = min(pages, from + each);
+    float2* mine = reinterpret_cast<float2*>(keys + (p.pages_most + 1) / 2 * 2);       // [each]: a page's score in 32 bits, and how far off it may be
+    const unsigned there = peer_addr(smem_u32(keys), 0);
+    const TQ* q = reinterpret_cast<const TQ*>(p.q) + (size_t)row * p.q_stride + (size_t)kvh * group * HD;
+    // the bounds of a page, or null where the table names none
+    auto bounds_of = [&](int index) -> const unsigned char* {
+        const int page = index < p.max_pages ? p.table[(size_t)row * p.max_pages + index] : -1;
+        return page >= 0 && page < p.num_pages ? p.pool + ((size_t)page * p.nkv + kvh) * p.block_bytes + bounds_at : nullptr;
+    };
+
+    // ---- every page's score in 32 bits
+    float far = 0.0f;                                  // the largest bound
     for (int h0 = 0; h0 < group; h0 += PS_HEADS) {
         __syncthreads();
         for (int i = tid; i < PS_HEADS * HD; i += PS_THREADS) {
             const int h = i / HD, f = i % HD;
-            const double v = h0 + h < group
-                ? (double)to_float(reinterpret_cast<const TQ*>(p.q)[(size_t)row * p.q_stride + (size_t)(kvh * group + h0 + h) * HD + f]) : 0.0;
-            q_s[f / 8][f % 8 * PS_HEADS + h] = make_double2(v > 0.0 ? v : 0.0, v > 0.0 ? 0.0 : v);
+            const float v = h0 + h < group ? to_float(q[(size_t)(h0 + h) * HD + f]) : 0.0f;
+            q_s[f / 8][f % 8 * PS_HEADS + h] = make_float2(fmaxf(v, 0.0f), v > 0.0f ? 0.0f : v);      // (what is no number stays so in the second)
         }
         __syncthreads();
         const int heads = min(PS_HEADS, group - h0), quarter = tid & 3;
-        auto score = [&](auto heads_) {                // (the 64-bit units are what this waits for: heads that are not there cost nothing)
-        constexpr int HEADS = decltype(heads_)::value;
-        for (int i0 = from; i0 + tid / 32 * 8 < to; i0 += PS_THREADS / 4) {        // (a warp without a page is done)
-            const int index = i0 + tid / 4;
-            const int page = index < to && index < p.max_pages ? p.table[(size_t)row * p.max_pages + index] : -1;
-            const bool bad = page < 0 || page >= p.num_pages;
-            const uint4* ends = reinterpret_cast<const uint4*>(p.pool + ((size_t)(bad ? 0 : page) * p.nkv + kvh) * p.block_bytes + bounds_at);
-            double acc[HEADS] = {};
+        for (int i0 = from; i0 + tid / 32 * 8 < to; i0 += PS_THREADS / 2) {      // (a warp without a page is done)
+            const uint4* ends[2];
+            int index[2];
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                index[n] = i0 + n * (PS_THREADS / 4) + tid / 4;
+                ends[n] = reinterpret_cast<const uint4*>(index[n] < to ? bounds_of(index[n]) : nullptr);
+            }
+            float s[2][PS_HEADS] = {}, size[2][PS_HEADS] = {};
 #pragma unroll
             for (int c = 0; c < MINE; ++c) {
-                const uint4 lo4 = ends[quarter + 4 * c], hi4 = ends[CHUNKS + quarter + 4 * c];
+                uint4 lo4[2], hi4[2];
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    lo4[n] = ends[n] ? ends[n][quarter + 4 * c] : make_uint4(0, 0, 0, 0);
+                    hi4[n] = ends[n] ? ends[n][CHUNKS + quarter + 4 * c] : make_uint4(0, 0, 0, 0);
+                }
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const unsigned a = e < 2 ? lo4.x : e < 4 ? lo4.y : e < 6 ? lo4.z : lo4.w;
-                    const unsigned b = e < 2 ? hi4.x : e < 4 ? hi4.y : e < 6 ? hi4.z : hi4.w;
-                    const double lo = (double)__uint_as_float(e & 1 ? a & 0xffff0000u : a << 16);
-                    const double hi = (double)__uint_as_float(e & 1 ? b & 0xffff0000u : b << 16);
+                    float lo[2], hi[2], most[2];
 #pragma unroll
-                    for (int h = 0; h < HEADS; ++h) {
-                        const double2 w = q_s[quarter + 4 * c][e * PS_HEADS + h];
-                        acc[h] = fma(w.x, hi, fma(w.y, lo, acc[h]));
+                    for (int n = 0; n < 2; ++n) {
+                        const unsigned a = e < 2 ? lo4[n].x : e < 4 ? lo4[n].y : e < 6 ? lo4[n].z : lo4[n].w;
+                        const unsigned b = e < 2 ? hi4[n].x : e < 4 ? hi4[n].y : e < 6 ? hi4[n].z : hi4[n].w;
+                        lo[n] = __uint_as_float(e & 1 ? a & 0xffff0000u : a << 16);
+                        hi[n] = __uint_as_float(e & 1 ? b & 0xffff0000u : b << 16);
+                        most[n] = fmaxf(fabsf(lo[n]), fabsf(hi[n]));
+                    }
+#pragma unroll
+                    for (int h = 0; h < PS_HEADS; ++h) {
+                        const float2 w = q_s[quarter + 4 * c][e * PS_HEADS + h];
+                        const float magnitude = w.x - w.y;
+#pragma unroll
+                        for (int n = 0; n < 2; ++n) {
+                            s[n][h] = fmaf(w.x, hi[n], fmaf(w.y, lo[n], s[n][h]));
+                            size[n][h] = fmaf(magnitude, most[n], size[n][h]);
+                        }
                     }
                 }
             }
-            float best = -INFINITY;
 #pragma unroll
-            for (int h = 0; h < HEADS; ++h) {
-                acc[h] += __shfl_xor_sync(0xffffffffu, acc[h], 1);
-                acc[h] += __shfl_xor_sync(0xffffffffu, acc[h], 2);
-                float s = (float)acc[h];
-                if (!(s <= 3.4028234e38f)) s = 3.4028234e38f;
-                if (h < heads) best = fmaxf(best, s);
+            for (int n = 0; n < 2; ++n) {
+                float best = -INFINITY, bound = 0.0f;
+#pragma unroll
+                for (int h = 0; h < PS_HEADS; ++h) {
+                    float a = s[n][h], b = size[n][h];
+                    a += __shfl_xor_sync(0xffffffffu, a, 1); b += __shfl_xor_sync(0xffffffffu, b, 1);
+                    a += __shfl_xor_sync(0xffffffffu, a, 2); b += __shfl_xor_sync(0xffffffffu, b, 2);
+                    if (h >= heads) continue;
+                    if (!(b < 1e37f) || a != a) { a = 0.0f; b = INFINITY; }      // (beyond what 32 bits hold, or no number)
+                    best = fmaxf(best, a); bound = fmaxf(bound, 7.7e-6f * b);
+                }
+                if (index[n] >= to || quarter) continue;
+                if (!ends[n]) {
+                    best = -INFINITY; bound = 0.0f;
+                    if (p.status) atomicOr(p.status, BG_STATUS_BAD_PAGE);
+                }
+                float2& have = mine[index[n] - from];
+                if (h0) { best = fmaxf(best, have.x); bound = fmaxf(bound, have.y); }
+                have = make_float2(best, bound);
+                const bool always = index[n] < p.first || index[n] >= pages - p.recent;
+                if (!always) far = fmaxf(far, bound);
+                if (h0 + PS_HEADS >= group) ps_store(there + 4u * (unsigned)index[n], ps_key(always ? INFINITY : best));
             }
-            if (index >= to || quarter) continue;
-            if (bad) {
-                best = -INFINITY;
-                if (p.status) atomicOr(p.status, BG_STATUS_BAD_PAGE);
-            }
-            if (index < p.first || index >= pages - p.recent) best = INFINITY;
-            const unsigned at = there + (unsigned)index * 4u;
-            if (h0) {                                  // the best of the heads before: this thread's own store
-                float old;
-                asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(old) : "r"(at) : "memory");
-                best = fmaxf(best, old);
-            }
-            st_cluster(at, best);
         }
-        };
-        if (heads <= 2) score(std::integral_constant<int, 2>{});
-        else if (heads <= 4) score(std::integral_constant<int, 4>{});
-        else if (heads <= 6) score(std::integral_constant<int, 6>{});
-        else score(std::integral_constant<int, 8>{});
+    }
+    far = block_max(far, scratch);
+    if (tid == 0) {
+        n_unsure = 0;
+        st_cluster(peer_addr(smem_u32(&far_of[rank]), 0), far);
+    }
+    cluster_sync_all();
+
+    // ---- the `top`-th largest of them, and the largest bound, for all CTAs
+    if (rank == 0) {
+        const PsBorder b = ps_border(keys, pages, p.top, room);
+        unsigned least = 0xffffffffu;                  // (where exactly `top` scores reach the border, it is the least of those)
+        for (int i = tid; i < pages; i += PS_THREADS)
+            if (keys[i] >= b.at) least = min(least, keys[i]);
+        least = __reduce_min_sync(0xffffffffu, least);
+        __syncthreads();
+        if (lane == 0) room[warp] = least;
+        __syncthreads();
+        if (tid < ranks) {
+            for (int w = 0; w < PS_WARPS; ++w) least = min(least, room[w]);
+            float most = 0.0f;
+            for (int r = 0; r < ranks; ++r) most = fmaxf(most, far_of[r]);
+            st_cluster(peer_addr(smem_u32(&cut[0]), (unsigned)tid), ps_score(least));
+            st_cluster(peer_addr(smem_u32(&cut[1]), (unsigned)tid), most);
+        }
+    }
+    cluster_sync_all();
+
+    // ---- what is in, what is out, and the sums in 64 bits of what is between
+    const float middle = cut[0], most = cut[1];
+    for (int i0 = from; i0 < to; i0 += PS_THREADS) {
+        const int index = i0 + tid;
+        if (index < to) {
+            const float2 have = mine[index - from];
+            const bool always = index < p.first || index >= pages - p.recent;
+            if (always || have.x - have.y > middle + most) ps_store(there + 4u * (unsigned)index, 0xffffffffu);
+            else if (have.x + have.y < middle - most) ps_store(there + 4u * (unsigned)index, 0u);
+            else unsure[atomicAdd(&n_unsure, 1)] = index;            // (their order is nobody's business)
+        }
+        __syncthreads();
+        const int n = n_unsure;
+        for (int i = warp; i < n; i += PS_WARPS) {
+            constexpr int PER = HD / 32;               // features of a lane
+            const unsigned char* ends = bounds_of(unsure[i]);
+            float best = -INFINITY;
+            if (ends) {
+                double lo[PER], hi[PER];
+#pragma unroll
+                for (int e = 0; e < PER; ++e) {
+                    lo[e] = (double)__bfloat162float(reinterpret_cast<const __nv_bfloat16*>(ends)[lane * PER + e]);
+                    hi[e] = (double)__bfloat162float(reinterpret_cast<const __nv_bfloat16*>(ends)[HD + lane * PER + e]);
+                }
+                for (int h = 0; h < group; ++h) {
+                    double a = 0.0;
+#pragma unroll
+                    for (int e = 0; e < PER; ++e) {
+                        const double v = (double)to_float(q[(size_t)h * HD + lane * PER + e]);
+                        a = fma(v > 0.0 ? v : 0.0, hi[e], fma(v > 0.0 ? 0.0 : v, lo[e], a));
+                    }
+#pragma unroll
+                    for (int o = 16; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+                    float s = (float)a;
+                    if (!(s <= PS_LARGEST)) s = PS_LARGEST;
+                    best = fmaxf(best, s);
+                }
+            }
+            if (lane == 0) ps_store(there + 4u * (unsigned)unsure[i], ps_key(best));     // (between nought and the largest number)
+        }
+        __syncthreads();
+        if (tid == 0) n_unsure = 0;
+        __syncthreads();
     }
     cluster_sync_all();
     if (rank) return;
 
-    // ---- the border: the largest threshold that at least `top` of the ordered scores reach
-    unsigned* keys = reinterpret_cast<unsigned*>(scores);
-    unsigned all = 0xffffffffu, any = 0;
-    for (int i = tid; i < pages; i += PS_THREADS) {
-        const unsigned k = ps_key(scores[i]);
-        keys[i] = k;
-        all &= k; any |= k;
-    }
-    all = __reduce_and_sync(0xffffffffu, all);
-    any = __reduce_or_sync(0xffffffffu, any);
-    if (lane == 0) { ends_s[0][warp] = all; ends_s[1][warp] = any; }
-    if (tid < 32) counts[tid] = 0;
-    __syncthreads();
-    for (int w = 0; w < PS_THREADS / 32; ++w) { all &= ends_s[0][w]; any |= ends_s[1][w]; }
-    const int bits = 32 - __clz(all ^ any);            // the bits that are not the same in all of them
-    unsigned border = bits >= 32 ? 0u : all >> bits << bits;
-    int reached = pages;                               // how many scores reach the border
-    for (int bit = bits - 1; bit >= 0 && reached != p.top; --bit) {
-        const unsigned next = border | 1u << bit;
-        int n = 0;
-        for (int i = tid; i < pages; i += PS_THREADS) n += keys[i] >= next;
-        n = __reduce_add_sync(0xffffffffu, n);
-        if (lane == 0 && n) atomicAdd(&counts[bit], n);
-        __syncthreads();
-        n = counts[bit];
-        if (n >= p.top) { border = next; reached = n; }
-    }
-    // Where exactly `top` scores reach it, all of them are taken.  Else every bit is settled and the border is a score itself: of its equals the first ones.
-    // ---- the list: every page above the border and the first `want` at it, in order; a thread takes a run of pages
-    const bool whole = reached == p.top;
+    // ---- the list: every page above the border and the first ones at it, in order; a thread takes a run of pages
+    const PsBorder b = ps_border(keys, pages, p.top, room);
     const int run = (pages + PS_THREADS - 1) / PS_THREADS, i0 = min(pages, tid * run), i1 = min(pages, i0 + run);
     unsigned above = 0, at = 0;
     for (int i = i0; i < i1; ++i) {
-        above += whole ? keys[i] >= border : keys[i] > border;
-        at += !whole && keys[i] == border;
+        above += b.exactly ? keys[i] >= b.at : keys[i] > b.at;
+        at += !b.exactly && keys[i] == b.at;
     }
     const unsigned both = above << 16 | at;            // (fewer than 65,536 pages)
     unsigned upto = both;
@@ -168,19 +292,20 @@ __global__ void __launch_bounds__(PS_THREADS) packed_select_kernel(const PsParam
         const unsigned v = __shfl_up_sync(0xffffffffu, upto, d);
         if (lane >= d) upto += v;
     }
-    if (lane == 31) ends_s[0][warp] = upto;
+    __syncthreads();
+    if (lane == 31) room[warp] = upto;
     __syncthreads();
     unsigned total = 0;
 #pragma unroll
-    for (int w = 0; w < PS_THREADS / 32; ++w) {
-        if (w < warp) upto += ends_s[0][w];
-        total += ends_s[0][w];
+    for (int w = 0; w < PS_WARPS; ++w) {
+        if (w < warp) upto += room[w];
+        total += room[w];
     }
     upto -= both;
     const unsigned want = p.top - (total >> 16);       // of those at the border
     unsigned n_above = upto >> 16, n_at = upto & 0xffffu;
     for (int i = i0; i < i1; ++i) {
-        const bool over = whole ? keys[i] >= border : keys[i] > border, equal = !whole && keys[i] == border;
+        const bool over = b.exactly ? keys[i] >= b.at : keys[i] > b.at, equal = !b.exactly && keys[i] == b.at;
         if (over || (equal && n_at < want)) out[n_above + min(n_at, want)] = i;
         n_above += over; n_at += equal;
     }
@@ -188,12 +313,13 @@ __global__ void __launch_bounds__(PS_THREADS) packed_select_kernel(const PsParam
 
 template <typename TQ, int HD>
 static int ps_launch(const PsParams& p, cudaStream_t stream) {
-    const size_t smem = (size_t)p.pages_most * 4;
+    // as many CTAs a (row, kv head) as two an SM give all of them at once, and at least as many as hold the scores of the pages
+    auto bytes = [&](int ctas) { return (size_t)(p.pages_most + 1) / 2 * 8 + (size_t)((p.pages_most + ctas - 1) / ctas) * 8; };
+    int ctas = PS_CLUSTER;
+    while (ctas > 1 && (long long)p.T * p.nkv * ctas > 2LL * sm_count() && bytes(ctas / 2) <= 100 * 1024) ctas /= 2;
+    const size_t smem = bytes(ctas);
     cudaError_t e = smem_limit(packed_select_kernel<TQ, HD>, smem);
     if (e != cudaSuccess) return (int)e;
-    // as many CTAs a (row, kv head) as one an SM gives all of them at once
-    int ctas = PS_CLUSTER;
-    while (ctas > 1 && (long long)p.T * p.nkv * ctas > sm_count()) ctas /= 2;
     e = launch_cluster(packed_select_kernel<TQ, HD>, dim3(p.T, p.nkv, ctas), dim3(PS_THREADS), smem, stream, ctas, p);
     return e == cudaSuccess ? BG_OK : (int)e;
 }
@@ -202,7 +328,7 @@ static int ps_launch(const PsParams& p, cudaStream_t stream) {
 
 using namespace bg;
 
-extern "C" int bg_packed_select_most() { return PS_FLOATS; }
+extern "C" int bg_packed_select_most() { return PS_MOST; }
 
 extern "C" int bg_packed_select_bytes() { return (int)sizeof(PsParams); }
 
@@ -214,6 +340,6 @@ extern "C" int bg_packed_select(const void* call, cudaStream_t stream) {
     if (p.page_size <= 0 || p.page_size % PK_TILE || p.nkv <= 0 || p.nkv > 65535 || p.nh <= 0 || p.nh % p.nkv || p.num_pages <= 0 || p.max_pages <= 0) return BG_ERR_SHAPE;
     if (p.block_bytes % 16 || p.block_bytes < p.page_size / PK_TILE * packed_tile_bytes(p.hd) + 4 * p.hd || (uintptr_t)p.pool % 16) return BG_ERR_ALIGN;
     if (p.top <= 0 || p.first < 0 || p.recent < 1 || p.first + p.recent > p.top || p.pages_most <= 0) return BG_ERR_SHAPE;
-    if (p.pages_most > PS_FLOATS) return BG_ERR_UNSUPPORTED;
+    if (p.pages_most > PS_MOST) return BG_ERR_UNSUPPORTED;
     BG_DISPATCH_DTYPE(p.dtype, TQ, return p.hd == 64 ? (ps_launch<TQ, 64>(p, stream)) : (ps_launch<TQ, 128>(p, stream)));
 }

@@ -547,7 +547,28 @@ def test_the_pages_that_score_highest(nh, nkv, hd, page, dtype, top, first, rece
 def test_many_pages_and_a_bound_far_above():
     got, want, *_ = selection([16 * 9000 + 3, 16 * 2100], 3, 1, 64, 16, BF16, 200, 1, 2)
     assert torch.equal(got, want)
-    got, want, *_ = selection([700, 16 * 60], 3, 1, 64, 16, BF16, 8, 1, 2, most=16 * 50000 - 1)
+    got, want, *_ = selection([700, 16 * 60], 3, 1, 64, 16, BF16, 8, 1, 2, most=16 * 36000 - 1)
+    assert torch.equal(got, want)
+
+
+@GPU
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("heads", [1, 9])
+def test_scores_that_32_bits_do_not_tell_apart(dtype, heads):
+    """Pages whose bounds differ by a unit in one feature, and pages that are equal: the choice is that of 64 bits."""
+    def change(q, pool, table, n):
+        data = pool[:, :, n:].contiguous().view(BF16)
+        one = data[table[0, 3].long()].clone()
+        g = torch.Generator().manual_seed(1)
+        for i in range(2, 700):
+            near = one.clone()
+            f = int(torch.randint(0, 256, (1,), generator=g))
+            if i % 3:
+                near[:, f] = torch.nextafter(near[:, f].float(), torch.tensor(math.inf)).to(BF16) if i % 2 else (near[:, f].float() * (1 + 2.0 ** -7)).to(BF16)
+            data[table[0, i].long()] = near
+        pool[:, :, n:] = data.view(torch.uint8)
+        q.copy_((q.float() * torch.logspace(-3, 3, q.shape[1])).to(q.dtype))
+    got, want, *_ = selection([800 * 16], heads, 1, 128, 16, dtype, 150, 1, 2, change=change)
     assert torch.equal(got, want)
 
 
@@ -792,7 +813,7 @@ def test_what_does_not_fit_is_refused():
              ((attend,), dict(given=good["pages"][:2])), ((attend,), dict(given=good["pages"].long())), ((attend,), dict(given=good["pages"], window=3)),
              ((attend,), dict(given=good["pages"], plan=ops.packed_plan([1, 1, 1], nh, nkv, hd, BF16, page, "cuda"))),
              ((select,), dict(recent=0)), ((select,), dict(first=2)), ((select,), dict(first=-1)), ((select,), dict(pages=good["pages"].long())),
-             ((select,), dict(pages=good["pages"][:2])), ((select,), dict(most=16 * 50000)), ((select,), dict(q=good["q"].half()))]
+             ((select,), dict(pages=good["pages"][:2])), ((select,), dict(most=16 * 36000)), ((select,), dict(q=good["q"].half()))]
     for calls, change in wrong:
         for call in calls:
             with pytest.raises(ops.KernelError):
