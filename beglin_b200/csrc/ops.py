@@ -1054,7 +1054,7 @@ def packed_ctas(streams: int, blocks: int, positions: int, at_once: int, beside:
     cluster, room = 1, at_once if beside > 1 else at_once * 3 // 4         # (CTAs alone on their SMs leave some SMs of a part of the GPU without a cluster)
     while cluster < 8 and 2 * cluster * streams <= room and cluster < units:
         cluster *= 2
-    if units <= PACKED_TURNS * cluster or streams >= 16 * at_once or blocks > lib().bg_packed_attention_blocks():
+    if units <= PACKED_TURNS * cluster or streams >= 16 * at_once or blocks > lib().bg_packed_attention_blocks() or streams * units >= 1 << 30:
         return 0, cluster
     return min(at_once, streams * units), 1
 

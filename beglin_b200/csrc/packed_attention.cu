@@ -110,7 +110,8 @@ struct PaShape {
     static constexpr int JOIN = PA_WARPS * COLS * (ROW + 2) * 4;
 };
 
-template <int HD, int NT, bool F32, int CT>
+// SHARE: the CTAs share all streams evenly; else a stream has a CTA, or a cluster of them.  (Both in one kernel cost the first 5 % by the registers of the second.)
+template <int HD, int NT, bool F32, int CT, bool SHARE>
 __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_attention_kernel(const PaParams p) {
     using S = PaShape<HD, NT, F32>;
     using L = Packed<HD>;
@@ -120,7 +121,7 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
     __shared__ unsigned long long bars[PA_WARPS][PA_STAGES];
     __shared__ int where[PA_WARPS][PA_STAGES];         // a stage's first position, or -1: nothing to read
     // units of a head's blocks in front of each block; or what a cluster's CTAs have of this one's columns
-    constexpr int MEET = COLS * (HD + 2) > PA_BLOCKS + PA_WARPS ? COLS * (HD + 2) : PA_BLOCKS + PA_WARPS;
+    constexpr int MEET = SHARE ? PA_BLOCKS + 1 + PA_WARPS : COLS * (HD + 2);
     __shared__ __align__(16) int before[MEET];
     __shared__ int gave_up;
     pdl_launch();
@@ -128,7 +129,7 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
     if (threadIdx.x < PA_WARPS * PA_STAGES) mbar_init(&bars[threadIdx.x / PA_STAGES][threadIdx.x % PA_STAGES], 1);
     if (threadIdx.x == 0) gave_up = 0;
     mbar_init_fence();
-    const int ranks = gridDim.z, rank = blockIdx.z;
+    const int ranks = SHARE ? 1 : gridDim.z, rank = SHARE ? 0 : blockIdx.z;
     if (ranks > 1) cluster_arrive_relaxed();           // (the others have begun before their memory is written)
     __syncthreads();
     if (ranks > 1) cluster_wait();
@@ -138,9 +139,8 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
     // packed_merge_kernel joins, and those that lie inside the run are finished here.  (A fixed number of CTAs for every stream left 64 rows of 2,048 to 8,192
         // positions, 2 kv heads, at 40 us for the longest ones.)  Few and short streams have a cluster each instead, whose CTAs take even parts and join them in shared
     // memory: no second kernel, no scratch.
-    long long unit = 0, stop = 1;
-    int per_head = 1;
-    if (p.ctas) {
+    int unit = 0, stop = 1;                            // (the host sees to it that they fit)
+    if constexpr (SHARE) {
         int mine[PA_BLOCKS / PA_THREADS], sum = 0;
 #pragma unroll
         for (int i = 0; i < PA_BLOCKS / PA_THREADS; ++i) {
@@ -154,13 +154,15 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
             const int v = __shfl_up_sync(0xffffffffu, upto, d);
             if (lane >= d) upto += v;
         }
-        if (lane == 31) before[PA_BLOCKS + warp] = upto;
+        if (lane == 31) before[PA_BLOCKS + 1 + warp] = upto;
         __syncthreads();
+        int per_head = 0;
         for (int w = 0; w < PA_WARPS; ++w) {
-            if (w < warp) upto += before[PA_BLOCKS + w];
-            per_head = w ? per_head + before[PA_BLOCKS + w] : before[PA_BLOCKS];
+            if (w < warp) upto += before[PA_BLOCKS + 1 + w];
+            per_head += before[PA_BLOCKS + 1 + w];
         }
         upto -= sum;
+        if (threadIdx.x == 0) before[PA_BLOCKS] = per_head;
 #pragma unroll
         for (int i = 0; i < PA_BLOCKS / PA_THREADS; ++i) {
             before[threadIdx.x * (PA_BLOCKS / PA_THREADS) + i] = upto;
@@ -169,8 +171,8 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
         __syncthreads();
         const long long units = (long long)per_head * p.heads_all;
         const long long share = min((long long)p.ctas, units);          // (none without a unit: the merge counts on it)
-        unit = blockIdx.x < share ? blockIdx.x * units / share : 0;
-        stop = blockIdx.x < share ? (blockIdx.x + 1) * units / share : 0;
+        unit = blockIdx.x < share ? (int)(blockIdx.x * units / share) : 0;
+        stop = blockIdx.x < share ? (int)((blockIdx.x + 1) * units / share) : 0;
     }
     // What is left of the stream that holds `unit`, as far as this CTA's run goes: where its copies come from, and which of them this warp waits for.
     int block, hy, u0, turns, begin, end, chunk0, req, pos_last;
@@ -180,9 +182,10 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
     auto next_stream = [&]() {
     block = blockIdx.x; hy = blockIdx.y;
     int u1, u_all;
-    if (p.ctas) {
-        hy = (int)(unit / per_head);
-        const int r = (int)(unit - (long long)hy * per_head);
+    if constexpr (SHARE) {
+        const int per_head = before[PA_BLOCKS];
+        hy = unit / per_head;
+        const int r = unit - hy * per_head;
         int low = 0, high = p.n - 1;                   // the last block that begins at or before r
         while (low < high) {
             const int mid = (low + high + 1) / 2;
@@ -192,7 +195,7 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
         block = low;
         u_all = (block + 1 < p.n ? before[block + 1] : per_head) - before[block];
         u0 = r - before[block];
-        u1 = (int)min((long long)u_all, u0 + stop - unit);
+        u1 = min(u_all, u0 + stop - unit);
         unit += u1 - u0;
         // (the CTA with a stream's first unit says where its parts are, for the merge)
         if (u0 == 0 && threadIdx.x == 0) {
@@ -538,7 +541,7 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
     }
 
     // ---- the next stream's copies come while this one's results meet
-    const bool more = unit < stop;
+    const bool more = SHARE && unit < stop;
     if (more) {
         next_stream();
         if (fine) first_copies();
@@ -610,7 +613,7 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
             if (f == 0) { st_cluster(at + 4 * HD, top); st_cluster(at + 4 * HD + 4, sum); }
             continue;
         }
-        if (!whole) {
+        if (SHARE && !whole) {
             reinterpret_cast<float2*>(p.part_o + (slot + col) * HD)[i % (HD / 2)] = v;
             if (f == 0) reinterpret_cast<float2*>(p.part_ml)[slot + col] = make_float2(top, sum);
             continue;
@@ -739,12 +742,16 @@ __global__ void __launch_bounds__(PM_WARPS * 32) packed_merge_kernel(const PaPar
 template <int HD, int NT, bool F32, int CT>
 static int pa_launch(const PaParams& p, int n, cudaStream_t stream) {
     const size_t smem = (size_t)PA_WARPS * PA_STAGES * CT * Packed<HD>::TILE + PaShape<HD, NT, F32>::JOIN;      // the rings, and where results meet
-    cudaError_t e = smem_limit(packed_attention_kernel<HD, NT, F32, CT>, smem);
+    if (!p.ctas) {
+        cudaError_t e = smem_limit(packed_attention_kernel<HD, NT, F32, CT, false>, smem);
+        if (e != cudaSuccess) return (int)e;
+        e = launch_cluster(packed_attention_kernel<HD, NT, F32, CT, false>, dim3(n, p.heads_all, p.cluster), dim3(PA_THREADS), smem, stream, p.cluster, p);
+        return e == cudaSuccess ? BG_OK : (int)e;
+    }
+    cudaError_t e = smem_limit(packed_attention_kernel<HD, NT, F32, CT, true>, smem);
     if (e != cudaSuccess) return (int)e;
-    const dim3 grid = p.ctas ? dim3(p.ctas) : dim3(n, p.heads_all, p.cluster);
-    e = launch_cluster(packed_attention_kernel<HD, NT, F32, CT>, grid, dim3(PA_THREADS), smem, stream, p.ctas ? 1 : p.cluster, p);
+    e = launch(packed_attention_kernel<HD, NT, F32, CT, true>, dim3(p.ctas), dim3(PA_THREADS), smem, stream, p);
     if (e != cudaSuccess) return (int)e;
-    if (!p.ctas) return BG_OK;
     constexpr int COLS = 8 * NT;
     // (many CTAs a stream: a CTA joins one column, not a warp)
     e = p.ctas > 8 * n * p.heads_all ? launch(packed_merge_kernel<HD, F32, PM_WARPS>, dim3(n, p.heads_all, COLS), dim3(PM_WARPS * 32), 0, stream, p, COLS)
