@@ -1096,6 +1096,20 @@ def packed_attention(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Ten
         return
     L, f32 = lib(), q.dtype == torch.float32
     with phase("attn"):
+        if plan is not None and plan.n_long:
+            end = max_position + 1 if plan.long_end is None else min(plan.long_end, max_position + 1)
+            size = L.bg_packed_wide_page()
+            n_pages = max(1, -(-end // size))
+            wide = torch.empty((plan.n_long * n_pages, 2, nkv, size, hd), dtype=torch.float16, device=q.device)
+            table = torch.empty((plan.n_long, n_pages), dtype=torch.int32, device=q.device)
+            shifts = torch.empty((plan.n_long, nkv, 2), dtype=torch.int32, device=q.device)
+            _check(L.bg_packed_unpack(_p(pool), block, pool.shape[0], page_size, _p(positions), _p(block_table), block_table.shape[1],
+                                      block_table.shape[0], _p(plan.longs), plan.n_long, _p(wide), _p(table), _p(shifts), n_pages, window, nkv, hd,
+                                      _p(status), _stream()), "packed_unpack")
+            _check(L.bg_attention_tc_half(_p(q), q.stride(0), _p(wide), plan.n_long * n_pages, size, _p(table), n_pages, _p(positions), _p(plan.blocks),
+                                          plan.n_blocks, _p(shifts), _p(out), out.stride(0), nh, nkv, hd, window, float(scale), end - 1, 1 if sink else 0,
+                                          _p(sink_weight), float(softcap), _p(status), _stream()), "attention_tcgen05")
+            count_launches(1)
         n, most = (T, 1) if plan is None else (plan.n_short, plan.most)
         if n:
             cols, each = _packed_columns(nh // nkv, f32, most)
@@ -1114,20 +1128,6 @@ def packed_attention(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Ten
                                             block_table.shape[1], block_table.shape[0], n, most, top, ctas, cluster, nh, nkv, hd, window, 1 if sink else 0, 0, scale, softcap)
             _check(L.bg_packed_attention(fields, _stream()), "packed_attention")
             count_launches(1 if ctas else 0)
-        if plan is not None and plan.n_long:
-            end = max_position + 1 if plan.long_end is None else min(plan.long_end, max_position + 1)
-            size = L.bg_packed_wide_page()
-            n_pages = max(1, -(-end // size))
-            wide = torch.empty((plan.n_long * n_pages, 2, nkv, size, hd), dtype=torch.float16, device=q.device)
-            table = torch.empty((plan.n_long, n_pages), dtype=torch.int32, device=q.device)
-            shifts = torch.empty((plan.n_long, nkv, 2), dtype=torch.int32, device=q.device)
-            _check(L.bg_packed_unpack(_p(pool), block, pool.shape[0], page_size, _p(positions), _p(block_table), block_table.shape[1],
-                                      block_table.shape[0], _p(plan.longs), plan.n_long, _p(wide), _p(table), _p(shifts), n_pages, window, nkv, hd,
-                                      _p(status), _stream()), "packed_unpack")
-            _check(L.bg_attention_tc_half(_p(q), q.stride(0), _p(wide), plan.n_long * n_pages, size, _p(table), n_pages, _p(positions), _p(plan.blocks),
-                                          plan.n_blocks, _p(shifts), _p(out), out.stride(0), nh, nkv, hd, window, float(scale), end - 1, 1 if sink else 0,
-                                          _p(sink_weight), float(softcap), _p(status), _stream()), "attention_tcgen05")
-            count_launches(1)
 
 
 def packed_select(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor, positions: torch.Tensor, nh: int, nkv: int, hd: int, page_size: int,

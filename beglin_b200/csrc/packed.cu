@@ -347,7 +347,7 @@ __device__ __forceinline__ int unpack_page(const PkUnpack& p, int req, int pos0,
 constexpr int PK_CLUSTER = 8;
 template <int HD>
 __global__ void __launch_bounds__(PK_THREADS) packed_reach_kernel(const PkUnpack p) {
-    constexpr int GROUPS = Packed<HD>::GROUPS, AT_ONCE = 4;
+    constexpr int GROUPS = Packed<HD>::GROUPS, AT_ONCE = 8;
     __shared__ float every[2][PK_CLUSTER];
     __shared__ float scratch[32];
     pdl_launch();
@@ -397,40 +397,55 @@ __global__ void __launch_bounds__(PK_THREADS) packed_reach_kernel(const PkUnpack
 }
 
 // The positions that a request's rows read, written out in half precision as the prompt attention takes them, in pages of PK_WIDE whatever the packed ones hold:
-// page i of the n-th request at n * pages + i.  A CTA takes a tile of 16 positions of one kv head; bound by the bytes written (heads of 128: 144 bytes read and
-// 512 written a position and kv head).  Positions behind the request's last are written as noughts: nobody reads them, and no number from nowhere stands there.
+// page i of the n-th request at n * pages + i.  A CTA takes one of those pages of one kv head, a thread a word of 8 codes at a time, all its loads on their way
+// together (a CTA for every 16 positions waited for its loads: 16 us for 16,000 positions of 4 kv heads); bound by the bytes written (heads of 128: 144 bytes
+// read and 512 written a position and kv head).  Positions behind the request's last are written as noughts: nobody reads them, and no number from nowhere
+// stands there.
 constexpr int PK_WIDE = 64;
 template <int HD>
 __global__ void __launch_bounds__(PK_THREADS) packed_unpack_kernel(const PkUnpack p) {
-    constexpr int WORDS = HD / 8, PER = 2 * PK_TILE * WORDS;
+    constexpr int WORDS = HD / 8, EACH = 2 * PK_WIDE * WORDS / PK_THREADS;
     pdl_launch();
-    const int n = blockIdx.z, kvh = blockIdx.y, pos0 = blockIdx.x * PK_TILE, wide = pos0 / PK_WIDE;
+    const int n = blockIdx.z, kvh = blockIdx.y, wide = blockIdx.x;
     pdl_wait();
-    if (pos0 % PK_WIDE == 0 && kvh == 0 && threadIdx.x == 0) p.table[(size_t)n * p.pages + wide] = n * p.pages + wide;
+    if (kvh == 0 && threadIdx.x == 0) p.table[(size_t)n * p.pages + wide] = n * p.pages + wide;
     const int req = p.longs[3 * n], row0 = p.longs[3 * n + 1], rows = p.longs[3 * n + 2];
     const int last = p.positions[row0 + rows - 1], lo = first_visible(p.positions[row0], p.window);
     if (wide > last / PK_WIDE || wide < lo / PK_WIDE) return;
-    const int page = unpack_page(p, req, pos0, lo, last, threadIdx.x == 0);
     const int2 shift = p.shifts[(size_t)n * p.nkv + kvh];
-    const unsigned char* from = p.pool + ((size_t)max(page, 0) * p.nkv + kvh) * p.block_bytes + (size_t)(pos0 % p.page_size / PK_TILE) * Packed<HD>::TILE;
-    __half* to = p.out + (((size_t)n * p.pages + wide) * 2 * p.nkv + kvh) * PK_WIDE * HD + (size_t)(pos0 % PK_WIDE) * HD;
+    __shared__ const unsigned char* tiles[PK_WIDE / PK_TILE];
+    if (threadIdx.x < PK_WIDE / PK_TILE) {
+        const int pos0 = wide * PK_WIDE + threadIdx.x * PK_TILE, page = unpack_page(p, req, pos0, lo, last, true);
+        tiles[threadIdx.x] = page < 0 ? nullptr
+            : p.pool + ((size_t)page * p.nkv + kvh) * p.block_bytes + (size_t)(pos0 % p.page_size / PK_TILE) * Packed<HD>::TILE;
+    }
+    __syncthreads();
+    unsigned pair[EACH], word[EACH];
+    unsigned have = 0;
 #pragma unroll
-    for (int i0 = 0; i0 < PER; i0 += PK_THREADS) {
-        const int i = i0 + threadIdx.x;
-        const int value = i / (PK_TILE * WORDS), slot = i / WORDS % PK_TILE, f = i % WORDS * 8;
+    for (int j = 0; j < EACH; ++j) {                   // (first the keys of all positions, then their values)
+        const int i = j * PK_THREADS + threadIdx.x, value = i / (PK_WIDE * WORDS), slot = i / WORDS % PK_WIDE, f = i % WORDS * 8;
+        const unsigned char* from = tiles[slot / PK_TILE];
+        pair[j] = word[j] = 0;
+        if (!from || wide * PK_WIDE + slot > last) continue;
+        pair[j] = *reinterpret_cast<const unsigned*>(from + Packed<HD>::pair_word(slot % PK_TILE, value, f / PK_GROUP));
+        word[j] = *reinterpret_cast<const unsigned*>(from + (value ? Packed<HD>::value_word(slot % PK_TILE, f) : Packed<HD>::key_word(slot % PK_TILE, f)));
+        have |= 1u << j;
+    }
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) {
+        const int i = j * PK_THREADS + threadIdx.x, value = i / (PK_WIDE * WORDS), slot = i / WORDS % PK_WIDE, f = i % WORDS * 8;
         float v[8] = {};
-        if (page >= 0 && pos0 + slot <= last) {
-            const unsigned pair = *reinterpret_cast<const unsigned*>(from + Packed<HD>::pair_word(slot, value, f / PK_GROUP));
-            const unsigned word = *reinterpret_cast<const unsigned*>(from + (value ? Packed<HD>::value_word(slot, f) : Packed<HD>::key_word(slot, f)));
-            if (value) packed_values<false>(word, pair, v);
-            else packed_values<true>(word, pair, v);
+        if (have >> j & 1) {
+            if (value) packed_values<false>(word[j], pair[j], v);
+            else packed_values<true>(word[j], pair[j], v);
         }
         const float down = __uint_as_float((unsigned)(127 - (value ? shift.y : shift.x)) << 23);
         uint4 r;
         __half2* h = reinterpret_cast<__half2*>(&r);
 #pragma unroll
         for (int e = 0; e < 4; ++e) h[e] = __floats2half2_rn(v[2 * e] * down, v[2 * e + 1] * down);
-        *reinterpret_cast<uint4*>(to + (size_t)value * p.nkv * PK_WIDE * HD + (size_t)slot * HD + f) = r;
+        *reinterpret_cast<uint4*>(p.out + ((((size_t)n * p.pages + wide) * 2 + value) * p.nkv + kvh) * PK_WIDE * HD + (size_t)slot * HD + f) = r;
     }
 }
 
@@ -510,10 +525,10 @@ extern "C" int bg_packed_unpack(const unsigned char* pool, long long block_bytes
     if ((uintptr_t)pool % 16 || (uintptr_t)out % 16 || (uintptr_t)shifts % 8) return BG_ERR_ALIGN;
     const PkUnpack p = {pool, block_bytes, positions, block_table, longs, (__half*)out, table, (int2*)shifts, max_pages, num_pages, page_size, n_req, nkv, pages,
                         window, status};
-    const dim3 heads(nkv, n, PK_CLUSTER), tiles(pages * (PK_WIDE / PK_TILE), nkv, n);
+    const dim3 heads(nkv, n, PK_CLUSTER), whole(pages, nkv, n);
     cudaError_t e = hd == 64 ? launch_cluster(packed_reach_kernel<64>, heads, dim3(PK_THREADS), 0, stream, PK_CLUSTER, p)
                              : launch_cluster(packed_reach_kernel<128>, heads, dim3(PK_THREADS), 0, stream, PK_CLUSTER, p);
     if (e != cudaSuccess) return (int)e;
-    e = hd == 64 ? launch(packed_unpack_kernel<64>, tiles, dim3(PK_THREADS), 0, stream, p) : launch(packed_unpack_kernel<128>, tiles, dim3(PK_THREADS), 0, stream, p);
+    e = hd == 64 ? launch(packed_unpack_kernel<64>, whole, dim3(PK_THREADS), 0, stream, p) : launch(packed_unpack_kernel<128>, whole, dim3(PK_THREADS), 0, stream, p);
     return e == cudaSuccess ? BG_OK : (int)e;
 }
