@@ -82,7 +82,7 @@ __device__ __forceinline__ unsigned pa_pack(float a, float b) {
     __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<unsigned*>(&h);
 }
-constexpr float PA_UP = 64.0f;                         // weights are 2^(x - maximum + PA_UP)
+constexpr float PA_UP = 64.0f;                         // weights, and sums of them, are 2^(x - maximum) times 2^PA_UP
 constexpr unsigned PA_ONE = 0x00010001u;               // the code 1 of two features, at bits 0
 // The pair of codes at bits 4 i of both halves of a word: u 2^-133 where i is even, 16 u 2^-133 where it is odd.
 __device__ __forceinline__ unsigned pa_codes(unsigned w, int i) { return (i < 2 ? w : w >> 8) & (i % 2 ? 0x00f000f0u : 0x000f000fu); }
@@ -440,7 +440,7 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int j = 0; j < 2; ++j) less[nt][j] = PA_UP - (m[nt][j] == -INFINITY ? 0.0f : m[nt][j]);
+            for (int j = 0; j < 2; ++j) less[nt][j] = (F32 ? 0.0f : PA_UP) - (m[nt][j] == -INFINITY ? 0.0f : m[nt][j]);
 #pragma unroll
         for (int i = 0; i < CT; ++i) {
             const unsigned char* tile = stage + i * L::TILE;
@@ -450,7 +450,7 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const float z = fmaf(x[i][nt][e], capped ? 1.0f : mult[nt][e & 1], less[nt][e & 1]);
-                    w[nt][e] = F32 ? exp2f(z) : pa_exp2(z);
+                    w[nt][e] = F32 ? exp2f(z) * 0x1p64f : pa_exp2(z);    // (a float next to PA_UP has 6 bits fewer behind its point)
                     l[nt][e & 1] += w[nt][e];
                 }
             unsigned vw[GROUPS][4], vp[2][GROUPS];     // words of positions 2t, 2t + 1, 2t + 8, 2t + 9; pairs of positions g, g + 8
@@ -505,9 +505,17 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
                     const unsigned a0 = pa_codes(ab[k / 2], n), a1 = pa_codes(ab[k / 2], n + 1);
                     const unsigned a2 = pa_codes(cd[k / 2], n), a3 = pa_codes(cd[k / 2], n + 1);
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
+                    for (int nt = 0; nt < NT; ++nt) {
+                        if constexpr (F32) {           // (the tensor cores' sums are cut off, not rounded: over many positions that shows, so only a tile's are theirs)
+                            float sum[4] = {};
 #pragma unroll
-                        for (int part = PARTS - 1; part >= 0; --part) pa_mma(o[gr * 4 + k][nt], a0, a1, a2, a3, b[part][nt][0], b[part][nt][1]);
+                            for (int part = PARTS - 1; part >= 0; --part) pa_mma(sum, a0, a1, a2, a3, b[part][nt][0], b[part][nt][1]);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) o[gr * 4 + k][nt][e] += sum[e];
+                        } else {
+                            pa_mma(o[gr * 4 + k][nt], a0, a1, a2, a3, b[0][nt][0], b[0][nt][1]);
+                        }
+                    }
                 }
             }
         }
@@ -567,7 +575,7 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             const int col = nt * 8 + 2 * t + j;
-            if (g == 0) ml[warp * COLS + col] = make_float2(m[nt][j] - PA_UP, l[nt][j]);
+            if (g == 0) ml[warp * COLS + col] = make_float2(m[nt][j], l[nt][j]);
 #pragma unroll
             for (int gr = 0; gr < GROUPS; ++gr) {
                 const float add = low[nt][gr][j], even = 0x1p100f, odd = 0x1p96f;        // (back from 2^-133, and from 16 times that)
@@ -584,7 +592,7 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
         if (p.sink) {
             const float at = (p.sink_w ? p.sink_w[h] : 0.0f) * PA_LOG2E, most = fmaxf(top, at);
             by = top == -INFINITY ? (sum == 0.0f ? 0.0f : 1.0f) : exp2f(top - most);
-            sum = fmaf(sum, by, exp2f(at - most));
+            sum = fmaf(sum, by, exp2f(at - most) * 0x1p64f);         // (as the weights)
         }
         by = sum == 0.0f ? 0.0f : by / sum;            // (a row that sees nothing is nought)
         TQ* out = reinterpret_cast<TQ*>(p.out) + (size_t)(row0 + r) * p.out_stride + (size_t)h * HD + f;
@@ -728,7 +736,7 @@ __global__ void __launch_bounds__(PM_WARPS * 32) packed_merge_kernel(const PaPar
     if (p.sink) {
         const float at = (p.sink_w ? p.sink_w[h] : 0.0f) * PA_LOG2E, most = fmaxf(m, at);
         by = m == -INFINITY ? (l == 0.0f ? 0.0f : 1.0f) : exp2f(m - most);
-        l = fmaf(l, by, exp2f(at - most));
+        l = fmaf(l, by, exp2f(at - most) * 0x1p64f);
     }
     by = l == 0.0f ? 0.0f : by / l;
     TQ* out = reinterpret_cast<TQ*>(p.out) + (size_t)(row0 + r) * p.out_stride + (size_t)h * HD + lane * PER;
