@@ -83,6 +83,7 @@ __device__ __forceinline__ unsigned pa_pack(float a, float b) {
     return *reinterpret_cast<unsigned*>(&h);
 }
 constexpr float PA_UP = 64.0f;                         // weights, and sums of them, are 2^(x - maximum) times 2^PA_UP
+constexpr float PA_SLACK = 8.0f;
 constexpr unsigned PA_ONE = 0x00010001u;               // the code 1 of two features, at bits 0
 // The pair of codes at bits 4 i of both halves of a word: u 2^-133 where i is even, 16 u 2^-133 where it is odd.
 __device__ __forceinline__ unsigned pa_codes(unsigned w, int i) { return (i < 2 ? w : w >> 8) & (i % 2 ? 0x00f000f0u : 0x000f000fu); }
@@ -278,7 +279,8 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
     // ---- queries: column g of every block of 8, features 64 group + 16 t .. + 15 as four steps of a product
     // (those that meet codes at bits 4 are a 16th)
     unsigned qf[PARTS][NT][GROUPS][8];
-    float qsum[NT][GROUPS][2], mult[NT][2];            // of columns 2t, 2t + 1 of every block: the sum of a group, and what the column's scores are multiplied with
+    unsigned qsum[NT];                                 // of column g of every block: the sums of its groups, the t-th of three parts
+    float mult[NT][2];                                 // of columns 2t, 2t + 1: what their scores are multiplied with
     int seen[NT][2];                                   // the positions of their rows
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -313,6 +315,9 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
                     a -= __bfloat162float(x); b -= __bfloat162float(y);
                 }
             }
+        // the sums as the codes 1 give them, in units of 2^-133 (a column's sum is with the lanes 4 x + column / 2); they go back as the right operand of a
+        // product with the pairs' lowest values, k = 2t, 2t + 1 the t-th parts of both groups
+        float sums[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int gr = 0; gr < GROUPS; ++gr) {
             float c[4] = {};
@@ -320,7 +325,15 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
             for (int part = 0; part < PARTS; ++part)
 #pragma unroll
                 for (int k = 0; k < 4; ++k) pa_mma(c, PA_ONE, PA_ONE, PA_ONE << 4, PA_ONE << 4, qf[part][nt][gr][2 * k], qf[part][nt][gr][2 * k + 1]);
-            qsum[nt][gr][0] = c[0]; qsum[nt][gr][1] = c[1];
+            const float even = __shfl_sync(0xffffffffu, c[0], g / 2), odd = __shfl_sync(0xffffffffu, c[1], g / 2);
+            sums[gr] = g % 2 ? odd : even;
+        }
+        qsum[nt] = 0;
+#pragma unroll
+        for (int part = 0; part < 3; ++part) {
+            const __nv_bfloat16 x = __float2bfloat16_rn(sums[0]), y = __float2bfloat16_rn(sums[1]);
+            if (part == t) qsum[nt] = (unsigned)__bfloat16_as_ushort(x) | (unsigned)__bfloat16_as_ushort(y) << 16;
+            sums[0] -= __bfloat162float(x); sums[1] -= __bfloat162float(y);
         }
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
@@ -360,7 +373,11 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
                     kp[half][0] = *reinterpret_cast<const unsigned*>(pair);
                 }
             }
+            // lowest (sum q) of both groups at once
             float s[NT][4] = {};
+            const unsigned low0 = __byte_perm(kp[0][0], kp[0][GROUPS - 1], 0x7632), low1 = __byte_perm(kp[1][0], kp[1][GROUPS - 1], 0x7632);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) pa_mma(s[nt], low0, low1, 0u, 0u, qsum[nt], 0u);
 #pragma unroll
             for (int gr = 0; gr < GROUPS; ++gr) {
                 float c[NT][4] = {};
@@ -376,11 +393,11 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
                 }
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
-                    const float step = pair_step(kp[half][gr]), lowest = pair_lowest(kp[half][gr]);
+                    const float step = pair_step(kp[half][gr]);
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int j = 0; j < 2; ++j) s[nt][2 * half + j] = fmaf(step, c[nt][2 * half + j], fmaf(lowest, qsum[nt][gr][j], s[nt][2 * half + j]));
+                        for (int j = 0; j < 2; ++j) s[nt][2 * half + j] = fmaf(step, c[nt][2 * half + j], s[nt][2 * half + j]);
                 }
             }
 #pragma unroll
@@ -406,7 +423,8 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
                     for (int e = 0; e < 4; ++e)
                         if (!(EDGE && (hidden >> ((i * NT + nt) * 4 + e) & 1))) x[i][nt][e] = pa_squashed<F32>(x[i][nt][e] * mult[nt][e & 1], p.cap_log2);
         }
-        // the running maximum, and what it does to what there is
+        // The reference maximum of a column moves when some lane has a score 2^8 above it (all lanes of a column have to have the same one, and finding the
+        // largest costs three exchanges): until then weights up to 2^8 are as good as those up to 1.
         float top[NT][2];
         bool grew = false;
 #pragma unroll
@@ -416,19 +434,20 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
                 float v = x[0][nt][j];
 #pragma unroll
                 for (int i = 0; i < CT; ++i) v = fmaxf(v, fmaxf(x[i][nt][j], x[i][nt][j + 2]));
-#pragma unroll
-                for (int d = 4; d < 32; d <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
-                if (!capped) v *= mult[nt][j];
-                top[nt][j] = fmaxf(m[nt][j], v);
-                grew |= top[nt][j] > m[nt][j];
+                top[nt][j] = capped ? v : v * mult[nt][j];
+                grew |= top[nt][j] > m[nt][j] + PA_SLACK;
             }
         if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    const float keep = top[nt][j] == m[nt][j] ? 1.0f : F32 ? exp2f(m[nt][j] - top[nt][j]) : pa_exp2(m[nt][j] - top[nt][j]);
-                    m[nt][j] = top[nt][j];
+                    float v = top[nt][j];
+#pragma unroll
+                    for (int d = 4; d < 32; d <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
+                    v = fmaxf(m[nt][j], v);
+                    const float keep = v == m[nt][j] ? 1.0f : F32 ? exp2f(m[nt][j] - v) : pa_exp2(m[nt][j] - v);
+                    m[nt][j] = v;
                     l[nt][j] *= keep;
 #pragma unroll
                     for (int gr = 0; gr < GROUPS; ++gr) low[nt][gr][j] *= keep;
