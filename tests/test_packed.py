@@ -716,6 +716,72 @@ def test_on_another_stream():
 
 
 @GPU
+def test_two_streams_at_once():
+    steps, sides, got = [Step([1500, 3, 31], 1), Step([700, 701], 2)], [torch.cuda.Stream(), torch.cuda.Stream()], [None, None]
+    for side in sides:
+        side.wait_stream(torch.cuda.current_stream())
+    for _ in range(5):
+        for i, (step, side) in enumerate(zip(steps, sides)):
+            with torch.cuda.stream(side):
+                got[i] = step()
+    for i, (step, side) in enumerate(zip(steps, sides)):
+        side.synchronize()
+        step.check(*got[i])
+
+
+@GPU
+def test_rows_apart_in_memory():
+    """Queries, results and portions' rows as parts of wider rows."""
+    nh, nkv, hd, page, lens = 6, 2, 64, 32, [70, 1, 9]
+    lengths = [200, 300, 9]
+    table, pages = make_table(lengths, page)
+    pool = make_pool(pages, nkv, hd, page, seed=2)
+    rows = [(i, p) for i, (n, length) in enumerate(zip(lens, lengths)) for p in range(length - n, length)]
+    wide = torch.randn((80, nh * hd + 64), generator=torch.Generator().manual_seed(4)).to(BF16).cuda()
+    q, positions, status = wide[:, 64:], torch.tensor([p for _, p in rows], dtype=torch.int32).cuda(), ops.new_status("cuda")
+    room = torch.full((80, nh * hd + 16), 7.0, dtype=BF16, device="cuda")
+    ops.packed_attention(q, pool.cuda(), table.cuda(), positions, nh, nkv, hd, page, 299, 0.125, room[:, 8:-8], status,
+                         plan=ops.packed_plan(lens, nh, nkv, hd, BF16, page, "cuda"))
+    ops.raise_on_status(status)
+    near(room[:, 8:-8].reshape(80, nh, hd), plain_attention(q.cpu().view(80, nh, hd), pool, table, hd, page, rows, 0.125), BF16)
+    assert bool((room[:, :8] == 7.0).all()) and bool((room[:, -8:] == 7.0).all())
+    with pytest.raises(ops.KernelError, match="misaligned"):
+        ops.packed_attention(wide[:, 1:1 + nh * hd], pool.cuda(), table.cuda(), positions, nh, nkv, hd, page, 299, 0.125, room[:, 8:-8], status,
+                             plan=ops.packed_plan(lens, nh, nkv, hd, BF16, page, "cuda"))
+
+
+@GPU
+def test_pages_beyond_four_gigabytes():
+    """A pool of 5 GB whose last pages are used: every call finds them."""
+    nh, nkv, hd, page, length = 8, 4, 128, 64, 150
+    few = make_pool(3, nkv, hd, page, bounds=True, seed=1)
+    pages = 5_000_000_000 // few[0].numel()
+    pool = torch.empty((pages, nkv, few.shape[2]), dtype=torch.uint8, device="cuda")
+    pool[-3:] = few.cuda()
+    small, table = torch.tensor([[2, 0, 1]], dtype=torch.int32), torch.tensor([[pages - 1, pages - 3, pages - 2]], dtype=torch.int32, device="cuda")
+    status, g = ops.new_status("cuda"), torch.Generator().manual_seed(5)
+    at, req = torch.tensor([length - 1], dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    src = torch.randn((1, (nh + 2 * nkv) * hd), generator=g).to(BF16)
+    q, values = torch.empty((1, nh * hd), dtype=BF16, device="cuda"), torch.empty((1, 2, nkv, hd), device="cuda")
+    ops.packed_append(src.cuda(), q, nh, nkv, hd, 0, False, None, at, req, table, pool, page, status)
+    ops.packed_rows(pool, at, req, table, hd, page, values, status)
+    for k, (u, step, lowest) in enumerate(map(quantised, (src.view(-1, hd)[nh:nh + nkv].double(), src.view(-1, hd)[nh + nkv:].double()))):
+        assert torch.equal(values[0, k].cpu(), (lowest + step * u).float())
+    ops.packed_bounds(pool, torch.tensor([63, 127], dtype=torch.int32, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda"), table, hd, page, status)
+    near_pool, pick = pool[-3:].cpu(), torch.empty((1, nkv, 2), dtype=torch.int32, device="cuda")
+    ops.packed_select(q, pool, table, at, nh, nkv, hd, page, length - 1, pick, status, first=0, recent=1)
+    assert torch.equal(pick.cpu(), chosen(q.cpu(), near_pool, small, [length], nh, nkv, hd, page, 2, 0, 1))
+    for n in (1, 70):                                                          # single tokens, and a portion by way of pages written out
+        rows = q.expand(n, -1).contiguous()
+        positions = torch.arange(length - n, length, dtype=torch.int32, device="cuda")
+        out = torch.empty_like(rows)
+        ops.packed_attention(rows, pool, table, positions, nh, nkv, hd, page, length - 1, 0.1, out, status,
+                             plan=ops.packed_plan([n], nh, nkv, hd, BF16, page, "cuda"))
+        near(out.view(n, nh, hd), plain_attention(rows.cpu().view(n, nh, hd), near_pool, small, hd, page, [(0, int(p)) for p in positions], 0.1), BF16, steps=0.6)
+    ops.raise_on_status(status)
+
+
+@GPU
 def test_the_same_call_twice_is_the_same():
     step = Step([1500, 3, 310])
     one, two = step(), step()
