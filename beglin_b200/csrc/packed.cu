@@ -116,16 +116,16 @@ __device__ __forceinline__ void append_query(const PkAppend& p, long long item, 
 // other), so every lane has work and as many CTAs as can be are under way.  4,917 rows of 36 heads: 90 us with a CTA for some heads of one row, four
 // features a lane and every head on the keys' path.
 template <typename TS, typename TQ, int HD, bool SPLIT>
-__global__ void __launch_bounds__(PK_THREADS, 4) packed_append_kernel(const PkAppend p, int query_ctas) {
+__global__ void __launch_bounds__(PK_THREADS, 4) packed_append_kernel(const PkAppend p, int other_ctas) {
     constexpr int LANES = HD / 8;
     pdl_launch();
     pdl_wait();
-    if ((int)blockIdx.x < query_ctas) {
-        const long long item = (long long)blockIdx.x * (PK_THREADS / (HD / 16)) + threadIdx.x / (HD / 16);
+    if ((int)blockIdx.x >= other_ctas) {
+        const long long item = (long long)((int)blockIdx.x - other_ctas) * (PK_THREADS / (HD / 16)) + threadIdx.x / (HD / 16);
         if (item < (long long)p.T * p.nh) append_query<TS, TQ, HD, SPLIT>(p, item, threadIdx.x % (HD / 16));
         return;
     }
-    const long long item = (long long)((int)blockIdx.x - query_ctas) * (PK_THREADS / LANES) + threadIdx.x / LANES;
+    const long long item = (long long)blockIdx.x * (PK_THREADS / LANES) + threadIdx.x / LANES;
     const int l = threadIdx.x % LANES, f = l * 8;
     const bool idle = item >= (long long)p.T * 2 * p.nkv;              // (stays for the shuffles)
     const int t = idle ? 0 : (int)(item / (2 * p.nkv)), h = p.nh + (idle ? 0 : (int)(item - (long long)t * 2 * p.nkv));
@@ -464,8 +464,8 @@ static int append_launch(const PkAppend& p, cudaStream_t stream) {
     const dim3 grid((unsigned)(queries + others));
     // (halves of whole pieces of 8 features, whose table rows are whole float4s)
     const bool split = !p.interleaved && p.rot % 16 == 0 && (uintptr_t)p.cos_sin % 16 == 0;
-    cudaError_t e = split ? launch(packed_append_kernel<TS, TQ, HD, true>, grid, dim3(PK_THREADS), 0, stream, p, (int)queries)
-                          : launch(packed_append_kernel<TS, TQ, HD, false>, grid, dim3(PK_THREADS), 0, stream, p, (int)queries);
+    cudaError_t e = split ? launch(packed_append_kernel<TS, TQ, HD, true>, grid, dim3(PK_THREADS), 0, stream, p, (int)others)
+                          : launch(packed_append_kernel<TS, TQ, HD, false>, grid, dim3(PK_THREADS), 0, stream, p, (int)others);
     return e == cudaSuccess ? BG_OK : (int)e;
 }
 
