@@ -5,20 +5,22 @@
 //
 // The choice is that of sums in 64 bits, rounded to 32 once: of products of bfloat16 they are exact but for the last few bits of 64, so the order does not hang
 // on the order of the sum; equal scores go to the lower page.  A score that is no number counts as the largest one.  But 64 bits are only needed next to the
-// border: every page gets its score in 32 bits with a bound E on how far off that may be (2^-17 of the sum of magnitudes; 66 additions make 2^-18), and
+// border: every page gets its score in 32 bits with a bound E on how far off that may be, and
 // with A the `top`-th largest of these scores and M the largest bound, a page over A + M + E is in, one under A - M - E is out, and those between, a handful, get
 // their sums in 64 bits.  (All of them in 64 bits: 50 us for 16 rows and heads of 2,000 pages, whose 64-bit multiply-adds alone take 7 and whose reads of
-// the queries from shared memory as much again.)
+// the queries from shared memory as much again.)  The sums in 32 bits are products of the tensor cores, mma.sync m16n8k16 with 16 pages' bounds as they lie as the
+// left operand and 8 heads' max(q, 0) and min(q, 0) as the right one; the same with the larger magnitude of both bounds and |q| gives the sum of magnitudes.
+// 16 additions to an accumulator that is cut off make 2^-18 of that, E is 2^-16; queries in float are rounded to bfloat16 for this, E is then 2^-8.  (By float
+// units, four lanes a page: 10 us for 256 pages of a CTA, of instructions.)
 //
-// A cluster of CTAs takes one (row, kv head), a CTA a part of the pages, four lanes two pages at a time (a quarter of the features each); the scores go to the
-// first CTA's shared memory, which finds a border by quartering: how many scores reach a threshold, two bits a round from the first that differs, until exactly as many
+// A cluster of CTAs takes one (row, kv head), a CTA a part of the pages, a warp 16 of them at a time; the scores go to the first CTA's shared memory, which finds a border by quartering: how many scores reach a threshold, two bits a round from the first that differs, until exactly as many
 // do as are wanted or no bit is left.  (Counting 8 bits at a time with shared-memory atomics put nearly every score into one counter, one after the other.)
 // Bound by latency: three meetings of the cluster and two searches for a border.
 #include "packed.cuh"
 
 namespace bg {
 
-constexpr int PS_THREADS = 256, PS_WARPS = PS_THREADS / 32, PS_CLUSTER = 8, PS_HEADS = 8;       // (the most CTAs of a cluster; query heads at a time)
+constexpr int PS_THREADS = 256, PS_WARPS = PS_THREADS / 32, PS_CLUSTER = 8, PS_HEADS = 8, PS_PAGES = 16;       // (the most CTAs of a cluster; heads and pages of a product)
 constexpr int PS_MOST = 36000;             // the most pages: their scores are in shared memory
 constexpr float PS_LARGEST = 3.4028234e38f;
 
@@ -38,6 +40,10 @@ __device__ __forceinline__ unsigned ps_key(float s) {
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float ps_score(unsigned key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
+__device__ __forceinline__ void ps_mma(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
 __device__ __forceinline__ void ps_store(unsigned addr, unsigned v) { asm volatile("st.shared::cluster.u32 [%0], %1;\n" ::"r"(addr), "r"(v) : "memory"); }
 
 // The largest threshold that at least `top` of the keys reach, or one that exactly `top` of them reach (then `exactly`), two bits a round.  All threads; a
@@ -95,10 +101,10 @@ __device__ __forceinline__ PsBorder ps_border(const unsigned* keys, int n, int t
 }
 
 template <typename TQ, int HD>
-__global__ void __launch_bounds__(PS_THREADS) packed_select_kernel(const PsParams p) {
-    constexpr int CHUNKS = HD / 8, MINE = CHUNKS / 4;  // pieces of 8 features of a page's bounds, and those of a lane
+__global__ void __launch_bounds__(PS_THREADS, 2) packed_select_kernel(const PsParams p) {
+    constexpr int CHUNKS = HD / 32;                    // runs of 32 features, a lane 8 of each: two steps of a product
+    constexpr bool F32 = sizeof(TQ) == 4;
     extern __shared__ __align__(16) unsigned keys[];   // the first CTA's: of every page; then this CTA's own (score, bound)
-    __shared__ float2 q_s[CHUNKS][PS_HEADS * 8 + 1];   // (max(q, 0), min(q, 0)); the odd piece keeps four lanes' reads apart
     __shared__ unsigned room[2 * PS_WARPS + 32];
     __shared__ float far_of[PS_CLUSTER], cut[2], scratch[32];
     __shared__ int unsure[PS_THREADS], n_unsure;
@@ -128,68 +134,71 @@ __global__ void __launch_bounds__(PS_THREADS) packed_select_kernel(const PsParam
 
     // ---- every page's score in 32 bits
     float far = 0.0f;                                  // the largest bound
+    const int g = lane >> 2, t = lane & 3;
     for (int h0 = 0; h0 < group; h0 += PS_HEADS) {
-        __syncthreads();
-        for (int i = tid; i < PS_HEADS * HD; i += PS_THREADS) {
-            const int h = i / HD, f = i % HD;
-            const float v = h0 + h < group ? to_float(q[(size_t)(h0 + h) * HD + f]) : 0.0f;
-            q_s[f / 8][f % 8 * PS_HEADS + h] = make_float2(fmaxf(v, 0.0f), v > 0.0f ? 0.0f : v);      // (what is no number stays so in the second)
+        const int heads = min(PS_HEADS, group - h0);
+        unsigned above[CHUNKS][4], below[CHUNKS][4], size[CHUNKS][4];           // max(q, 0), min(q, 0), |q| of head g
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) {
+            float v[8] = {};
+            if (g < heads) load8(q + (size_t)(h0 + g) * HD + 32 * c + 8 * t, v);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const __nv_bfloat162 x = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+                const unsigned bits = *reinterpret_cast<const unsigned*>(&x);
+                const unsigned negative = ((bits >> 15) & 0x00010001u) * 0xffffu;
+                above[c][i] = bits & ~negative; below[c][i] = bits & negative; size[c][i] = bits & 0x7fff7fffu;
+            }
         }
-        __syncthreads();
-        const int heads = min(PS_HEADS, group - h0), quarter = tid & 3;
-        for (int i0 = from; i0 + tid / 32 * 8 < to; i0 += PS_THREADS / 2) {      // (a warp without a page is done)
-            const uint4* ends[2];
+        for (int i0 = from + warp * PS_PAGES; i0 < to; i0 += PS_WARPS * PS_PAGES) {
             int index[2];
+            const unsigned char* ends[2];              // pages g and g + 8
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
-                index[n] = i0 + n * (PS_THREADS / 4) + tid / 4;
-                ends[n] = reinterpret_cast<const uint4*>(index[n] < to ? bounds_of(index[n]) : nullptr);
+                index[n] = i0 + 8 * n + g;
+                ends[n] = index[n] < to ? bounds_of(index[n]) : nullptr;
             }
-            float s[2][PS_HEADS] = {}, size[2][PS_HEADS] = {};
+            uint4 lo[CHUNKS][2], hi[CHUNKS][2];
 #pragma unroll
-            for (int c = 0; c < MINE; ++c) {
-                uint4 lo4[2], hi4[2];
+            for (int c = 0; c < CHUNKS; ++c)
 #pragma unroll
                 for (int n = 0; n < 2; ++n) {
-                    lo4[n] = ends[n] ? ends[n][quarter + 4 * c] : make_uint4(0, 0, 0, 0);
-                    hi4[n] = ends[n] ? ends[n][CHUNKS + quarter + 4 * c] : make_uint4(0, 0, 0, 0);
+                    const uint4* at = reinterpret_cast<const uint4*>(ends[n] ? ends[n] : p.pool + bounds_at) + 4 * c + t;
+                    lo[c][n] = at[0]; hi[c][n] = at[HD / 8];
                 }
+            float s[4] = {}, sum[4] = {};              // (page g, heads 2t and 2t + 1; page g + 8)
+            auto most = [](unsigned a, unsigned b) {   // the larger magnitude of two pairs
+                const unsigned x = a & 0x7fff7fffu, y = b & 0x7fff7fffu;
+                return __vmaxu2(x, y);                 // (magnitudes are ordered as whole numbers)
+            };
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    float lo[2], hi[2], most[2];
+            for (int c = 0; c < CHUNKS; ++c) {
+                const unsigned l[2][4] = {{lo[c][0].x, lo[c][0].y, lo[c][0].z, lo[c][0].w}, {lo[c][1].x, lo[c][1].y, lo[c][1].z, lo[c][1].w}};
+                const unsigned u[2][4] = {{hi[c][0].x, hi[c][0].y, hi[c][0].z, hi[c][0].w}, {hi[c][1].x, hi[c][1].y, hi[c][1].z, hi[c][1].w}};
 #pragma unroll
-                    for (int n = 0; n < 2; ++n) {
-                        const unsigned a = e < 2 ? lo4[n].x : e < 4 ? lo4[n].y : e < 6 ? lo4[n].z : lo4[n].w;
-                        const unsigned b = e < 2 ? hi4[n].x : e < 4 ? hi4[n].y : e < 6 ? hi4[n].z : hi4[n].w;
-                        lo[n] = __uint_as_float(e & 1 ? a & 0xffff0000u : a << 16);
-                        hi[n] = __uint_as_float(e & 1 ? b & 0xffff0000u : b << 16);
-                        most[n] = fmaxf(fabsf(lo[n]), fabsf(hi[n]));
-                    }
-#pragma unroll
-                    for (int h = 0; h < PS_HEADS; ++h) {
-                        const float2 w = q_s[quarter + 4 * c][e * PS_HEADS + h];
-                        const float magnitude = w.x - w.y;
-#pragma unroll
-                        for (int n = 0; n < 2; ++n) {
-                            s[n][h] = fmaf(w.x, hi[n], fmaf(w.y, lo[n], s[n][h]));
-                            size[n][h] = fmaf(magnitude, most[n], size[n][h]);
-                        }
-                    }
+                for (int k = 0; k < 4; k += 2) {
+                    ps_mma(s, u[0][k], u[1][k], u[0][k + 1], u[1][k + 1], above[c][k], above[c][k + 1]);
+                    ps_mma(s, l[0][k], l[1][k], l[0][k + 1], l[1][k + 1], below[c][k], below[c][k + 1]);
+                    ps_mma(sum, most(l[0][k], u[0][k]), most(l[1][k], u[1][k]), most(l[0][k + 1], u[0][k + 1]), most(l[1][k + 1], u[1][k + 1]),
+                           size[c][k], size[c][k + 1]);
                 }
             }
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
                 float best = -INFINITY, bound = 0.0f;
 #pragma unroll
-                for (int h = 0; h < PS_HEADS; ++h) {
-                    float a = s[n][h], b = size[n][h];
-                    a += __shfl_xor_sync(0xffffffffu, a, 1); b += __shfl_xor_sync(0xffffffffu, b, 1);
-                    a += __shfl_xor_sync(0xffffffffu, a, 2); b += __shfl_xor_sync(0xffffffffu, b, 2);
-                    if (h >= heads) continue;
+                for (int j = 0; j < 2; ++j) {
+                    float a = s[2 * n + j], b = sum[2 * n + j];
+                    if (2 * t + j >= heads) continue;
                     if (!(b < 1e37f) || a != a) { a = 0.0f; b = INFINITY; }      // (beyond what 32 bits hold, or no number)
-                    best = fmaxf(best, a); bound = fmaxf(bound, 7.7e-6f * b);
+                    best = fmaxf(best, a); bound = fmaxf(bound, (F32 ? 0x1p-8f : 0x1p-16f) * b);
                 }
-                if (index[n] >= to || quarter) continue;
+#pragma unroll
+                for (int d = 1; d < 4; d <<= 1) {
+                    best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, d));
+                    bound = fmaxf(bound, __shfl_xor_sync(0xffffffffu, bound, d));
+                }
+                if (index[n] >= to || t) continue;
                 if (!ends[n]) {
                     best = -INFINITY; bound = 0.0f;
                     if (p.status) atomicOr(p.status, BG_STATUS_BAD_PAGE);
@@ -338,7 +347,8 @@ extern "C" int bg_packed_select(const void* call, cudaStream_t stream) {
     if (p.hd != 64 && p.hd != 128) return BG_ERR_UNSUPPORTED;
     if (p.T <= 0) return BG_OK;
     if (p.page_size <= 0 || p.page_size % PK_TILE || p.nkv <= 0 || p.nkv > 65535 || p.nh <= 0 || p.nh % p.nkv || p.num_pages <= 0 || p.max_pages <= 0) return BG_ERR_SHAPE;
-    if (p.block_bytes % 16 || p.block_bytes < p.page_size / PK_TILE * packed_tile_bytes(p.hd) + 4 * p.hd || (uintptr_t)p.pool % 16) return BG_ERR_ALIGN;
+    if (p.block_bytes % 16 || p.block_bytes < p.page_size / PK_TILE * packed_tile_bytes(p.hd) + 4 * p.hd || (uintptr_t)p.pool % 16
+        || ((long long)(uintptr_t)p.q | p.q_stride * (p.dtype == BG_DTYPE_F32 ? 4 : 2)) % 16) return BG_ERR_ALIGN;
     if (p.top <= 0 || p.first < 0 || p.recent < 1 || p.first + p.recent > p.top || p.pages_most <= 0) return BG_ERR_SHAPE;
     if (p.pages_most > PS_MOST) return BG_ERR_UNSUPPORTED;
     BG_DISPATCH_DTYPE(p.dtype, TQ, return p.hd == 64 ? (ps_launch<TQ, 64>(p, stream)) : (ps_launch<TQ, 128>(p, stream)));
