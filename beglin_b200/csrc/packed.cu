@@ -109,9 +109,9 @@ __device__ __forceinline__ void append_query(const PkAppend& p, long long item, 
 
 // Keys and values: HD / 8 lanes take a head of a row, a lane eight neighbouring features, which are a word of codes; a group's 8 lanes find its smallest and
 // largest by shuffles.  The codes are those that 64 bits give: everything is done in 32 first, with a bound on how far off that may be, and where the bound
-// reaches the border of two codes, or of two roundings of the pair, the warp does its heads again in 64 (two or three warps of a thousand).  The border itself,
-// (k + 1/2) step, has 13 bits and is exact, so a difference x - lowest that is exact (bfloat16 that was not rotated) needs no more than a comparison; no
-// division is made in 32 bits.
+// reaches the border of two codes, or of two roundings of the pair, the warp does its heads again in 64 (two or three warps of a thousand).  What
+// is left of x - lowest beside the nearest whole number of steps is one fused multiply-add, exact where that difference is (bfloat16 that was not rotated): a
+// comparison with half a step then decides as 64 bits do, without a division.
 // The first CTAs take the queries' heads, the others the keys' and values', both row after row: bound by the latency of a CTA (its loads, one behind the
 // other), so every lane has work and as many CTAs as can be are under way.  4,917 rows of 36 heads: 90 us with a CTA for some heads of one row, four
 // features a lane and every head on the keys' path.
@@ -176,15 +176,17 @@ __global__ void __launch_bounds__(PK_THREADS, 4) packed_append_kernel(const PkAp
     float by = s > 0.0f ? s : 1.0f;                    // (a group of one value: every code 0)
     int near = __bfloat16_as_ushort(__float2bfloat16_rn(lo - off)) != __bfloat16_as_ushort(__float2bfloat16_rn(lo + off))
             || __bfloat16_as_ushort(__float2bfloat16_rn(span - span_off)) != __bfloat16_as_ushort(__float2bfloat16_rn(span + span_off));
-    const float inv = __frcp_rn(by);
+    const float inv = __frcp_rn(by), half_step = 0.5f * by;
     float u[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        const float d = __fsub_rn(r[j], base), k = floorf(d * inv), border = __fmul_rn(k + 0.5f, by), over = __fsub_rn(d, border);
-        u[j] = over > 0.0f || (over == 0.0f && ((int)k & 1)) ? k + 1.0f : k;
+        // the whole number next to d / by, by adding 1.5 2^23 (whose last bit is then its parity), and what is left of d, which is exact up to one rounding
+        const float d = __fsub_rn(r[j], base), t = fmaf(d, inv, 12582912.0f), k = __fsub_rn(t, 12582912.0f), left = fmaf(-k, by, d);
+        const float over = __fsub_rn(fabsf(left), half_step);
+        u[j] = over > 0.0f || (over == 0.0f && (__float_as_uint(t) & 1u)) ? k + copysignf(1.0f, left) : k;
         // (the two errors of the difference x - lowest: both nought where it is exact)
         const bool sure = sizeof(TS) == 2 && p.parts == 1 && !turned && __fadd_rn(d, base) == r[j] && __fsub_rn(r[j], d) == base;
-        near |= !sure && fabsf(over) <= off + 2.5e-7f * (fabsf(d) + fabsf(border));
+        near |= !sure && fabsf(over) <= fmaf(2.5e-7f, fabsf(d) + by, off);
     }
     if (!(by >= 1e-36f)) near = 1;                     // (a step whose reciprocal or borders leave the normal range)
     if (__any_sync(0xffffffffu, near && sound && !idle)) {
@@ -209,12 +211,12 @@ __global__ void __launch_bounds__(PK_THREADS, 4) packed_append_kernel(const PkAp
         for (int j = 0; j < 8; ++j) u[j] = (float)rint((w[j] - (double)base) / (double)by);
     }
     if (idle) return;
-    unsigned word = 0;
+    // four codes to a whole number below 2^16, whose bits 2^23 lays bare (conversions are for units of a quarter of the width)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const unsigned code = (unsigned)fminf(fmaxf(u[e], 0.0f), 15.0f);
-        word |= key ? code << (4 * (e / 2 + 4 * (e % 2))) : code << (4 * e);
-    }
+    for (int e = 0; e < 8; ++e) u[e] = fminf(fmaxf(u[e], 0.0f), 15.0f);
+    auto four = [](float a, float b, float c, float d) { return __float_as_uint(fmaf(4096.0f, d, fmaf(256.0f, c, fmaf(16.0f, b, a))) + 8388608.0f); };
+    unsigned word = key ? __byte_perm(four(u[0], u[2], u[4], u[6]), four(u[1], u[3], u[5], u[7]), 0x5410)
+                        : __byte_perm(four(u[0], u[1], u[2], u[3]), four(u[4], u[5], u[6], u[7]), 0x5410);
     if (!sound) {
         lowest = step = __float2bfloat16_rn(__int_as_float(0x7fffffff));
         word = 0;
