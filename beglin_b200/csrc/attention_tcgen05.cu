@@ -225,7 +225,11 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&tmem_sh)), "r"(TMEM_COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
     };
-    if constexpr (!SHARED) {
+    if constexpr (HALF) {
+        // (behind the wait: the kernels ahead are small ones that let this one begin while a product in front of them may still want its columns)
+        pdl_wait();
+        if (warp == 0) allocate();
+    } else if constexpr (!SHARED) {
         if (warp == 0) allocate();
         pdl_wait();
     }

@@ -249,9 +249,9 @@ __global__ void __launch_bounds__(PK_THREADS) packed_rows_kernel(const PkRead p)
     constexpr int WORDS = HD / 8;
     pdl_launch();
     const int per_row = 2 * p.nkv * WORDS, i = blockIdx.y * PK_THREADS + threadIdx.x, t = blockIdx.x;
-    if (i >= per_row) return;
     const int value = i / (p.nkv * WORDS), kvh = i / WORDS % p.nkv, f = i % WORDS * 8;
-    pdl_wait();
+    pdl_wait();                                        // (all warps of a CTA, those without work too)
+    if (i >= per_row) return;
     const int pos = p.positions[t], req = p.row_req[t], index = pos / p.page_size;
     const int page = pos >= 0 && req >= 0 && req < p.n_req && index < p.max_pages ? p.block_table[(size_t)req * p.max_pages + index] : -1;
     TO* out = reinterpret_cast<TO*>(p.out) + ((size_t)t * 2 * p.nkv + (size_t)value * p.nkv + kvh) * HD + f;
