@@ -983,8 +983,11 @@ def packed_rows(pool: torch.Tensor, positions: torch.Tensor, row_req: torch.Tens
     _check(lib().bg_packed_rows(_packed_read(pool, block, positions, row_req, block_table, out, _dt(out), status, page_size, T, hd), _stream()), "packed_rows")
 
 
-# Rows that a request brings from which its pages are written out in half precision for the prompt attention.
-PACKED_LONG_ROWS = 64
+# Streams (kv heads of blocks of rows) that a request brings above which its pages are written out in half precision for the prompt attention: the packed kernel's
+# CTAs, two an SM, then go over the pages more than once, which is about what writing them out costs.  28 heads, 4 kv heads, behind 1,000 positions: 64 rows (128
+# streams) 14.7 us by the packed kernel and 24.6 written out, 128 rows (256) 28.3 and 25.4, 256 rows 55 and 28; behind 16,000: 99 and 173, 185 and 174, 361 and 176.  32 heads
+# with keys of their own, 128 rows (256 streams) behind 4,000: 67 and 73; 256 rows 123 and 78.
+PACKED_LONG_STREAMS = 240
 
 
 @functools.lru_cache(maxsize=None)
@@ -1007,10 +1010,10 @@ class PackedPlan:
         bq = _c_int(0)
         wide = not f32 and lib().bg_attention_tc_plan(group, hd, lib().bg_packed_wide_page(), ctypes.byref(bq)) == 0
         self.bq = bq = bq.value
-        long_from = PACKED_LONG_ROWS if wide else 1 << 62
+        streams = nkv * -(-group // (8 if f32 else 16))        # of a block of rows
         short, blocks, longs = [], [], []
         for i, (r0, n) in enumerate(zip(row_start, lens)):
-            if n >= long_from:
+            if wide and n > self.rows and -(-n // self.rows) * streams > PACKED_LONG_STREAMS:
                 blocks += [(len(longs), r0 + f, min(bq, n - f)) for f in range(0, n, bq)]
                 longs.append((i, r0, n))
             else:
@@ -1027,8 +1030,8 @@ class PackedPlan:
 
 def packed_plan(lens, nh: int, nkv: int, hd: int, dtype: torch.dtype, page_size: int, device, row_start=None, starts=None) -> PackedPlan:
     """The plan of `packed_attention` for a step whose request i brings lens[i] rows, from row row_start[i] on (default: one behind the other).  `starts`: the
-    positions of their first rows, where the host knows them (less room is made then).  Requests of PACKED_LONG_ROWS rows and more (bfloat16) have their pages
-    written out in half precision and run the prompt attention; the others' rows go in blocks of as many (row, query head) pairs as the kernel has columns."""
+    positions of their first rows, where the host knows them (less room is made then).  Rows go in blocks of as many (row, query head) pairs as the packed kernel has
+    columns; requests of more than PACKED_LONG_STREAMS kv heads of such blocks (bfloat16) have their pages written out in half precision and run the prompt attention."""
     lens = [int(n) for n in lens]
     if any(n < 0 for n in lens) or nh <= 0 or nkv <= 0 or nh % nkv:
         raise KernelError(f"packed_plan: rows {lens}, {nh} query heads for {nkv} kv heads")
@@ -1042,19 +1045,23 @@ def packed_plan(lens, nh: int, nkv: int, hd: int, dtype: torch.dtype, page_size:
     return PackedPlan(lens, [int(r) for r in row_start], nh, nkv, hd, dtype, page_size, device, starts)
 
 
-PACKED_TURNS = 6           # units of 256 positions that a CTA of a cluster takes, at most
-
-
 def packed_ctas(streams: int, blocks: int, positions: int, at_once: int, beside: int = 2) -> Tuple[int, int]:
     """(CTAs that share the positions of all streams evenly or 0, CTAs of a cluster that share a stream) for streams (a kv head of a block of rows) of up to
-    `positions`, `at_once` CTAs side by side, `beside` of them on an SM.  Where a cluster of up to 8 CTAs a stream leaves each of them little to do, that: the results meet inside it.  A CTA
-    a stream where streams are so many that they even out (or more than a CTA sums up the lengths of).  Else as many CTAs as run side by side, of which a
-    second kernel joins what they have of a stream."""
+    `positions`, `at_once` CTAs side by side, `beside` of them on an SM.
+
+    A cluster of up to 8 CTAs a stream meets inside it, but its CTAs wait for the longest stream; as many CTAs as run side by side that share all positions evenly
+    need partial results and a second kernel.  So clusters, while a CTA's units of 256 positions of the longest stream are few, the more the
+    fuller clusters have the device anyway.  4 kv heads, us by clusters and shared: 1 row of 4,000 positions 8.3 and 11.0, of 16,000 15.5 and 12.3; 33 rows of 4,000
+    23.0 and 30.9, of 1,000 to 8,000 35.8 and 31.8; 64 rows of 300 to 2,400 23.1 and 26.3, of 1,000 to 8,000 63.6 and 53.2.  Where streams outnumber the CTAs one
+    CTA takes a stream, and the more streams there are the better they even out: 150 rows of 300 to 2,400 43.1 and 50.9, of 8,000 158 and 147; 400 rows of 8,000 337 and
+    371.  Float queries have one CTA on an SM, of half the speed: 1 row of 8,000 14.9 and 11.8, 33 rows of 300 to 2,400 25.7 and 29.8."""
     units = -(-positions // 256)
-    cluster, room = 1, at_once if beside > 1 else at_once * 3 // 4         # (CTAs alone on their SMs leave some SMs of a part of the GPU without a cluster)
+    cluster, room = 1, at_once if beside > 1 else at_once * 3 // 4         # (with all SMs, some of a part of the GPU are left without a cluster: 18.5 us for 14.8)
     while cluster < 8 and 2 * cluster * streams <= room and cluster < units:
         cluster *= 2
-    if units <= PACKED_TURNS * cluster or streams >= 16 * at_once or blocks > lib().bg_packed_attention_blocks() or streams * units >= 1 << 30:
+    full = streams * cluster / at_once
+    few = (3 if beside > 1 else 1) + 11 * full if full <= 1 else 10 + 0.15 * units * full
+    if -(-units // cluster) <= few or blocks > lib().bg_packed_attention_blocks() or streams * units >= 1 << 30:
         return 0, cluster
     return min(at_once, streams * units), 1
 

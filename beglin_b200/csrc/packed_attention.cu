@@ -16,9 +16,11 @@
 // Ranges: a row of queries is scaled by the power of two that brings its largest to 2^100.  Weights carry 2^64, so values may have steps up to 2^63, and those
 // under 2^-50 lose digits.
 //
-// Why this shape: at the bandwidth of HBM a position of a kv head (144 bytes for heads of 128) has to be done in some 6 cycles of an SM, 25 warp instructions.  The
-// left operand by codes takes about 15 for 8 columns; with the queries on the left (16 rows, half of them empty) it took the tensor cores twice the products
-// and the softmax twice the numbers.  A warp has a ring of its own (STAGES chunks of 16 or 32 positions, one bulk copy each) and its own running maximum, sum
+// Why this shape: at the bandwidth of HBM a position of a kv head (144 bytes for heads of 128) has to be done in some 6 cycles of an SM, 25 warp instructions at
+// best.  It takes 17 for 8 columns, half of them on the units of integers and logic, which take one every two cycles; with the queries on the left (16 rows, half
+// of them empty) it took the tensor cores twice the products and the softmax twice the numbers.  4 rows of 131,072 positions, 4 kv heads: 68 us, 65 % of the bandwidth of
+// a copy (83 % but for what does not grow with the length: a start, two kernels, where results meet); 64 rows of 2,048 to 8,192, 2 kv heads: 34 us, 42 %.  Bound
+// by these instructions: with all pages in the L2 it takes 95 % of the time.  A warp has a ring of its own (STAGES chunks of 16 or 32 positions, one bulk copy each) and its own running maximum, sum
 // and result, so that nothing in the loop waits for another warp; the warps' results meet at the end, those of a long request's ranges in packed_merge_kernel.
 #include <type_traits>
 
@@ -138,7 +140,7 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
     // ---- what this CTA reads.  The streams (a kv head, or a block of its query heads, of a block of rows; the blocks of one head one behind the other) are cut
     // in units of PA_WARPS chunks, and the CTAs share the units evenly, whatever the lengths: a CTA's run of units begins and ends inside streams, whose results
     // packed_merge_kernel joins, and those that lie inside the run are finished here.  (A fixed number of CTAs for every stream left 64 rows of 2,048 to 8,192
-        // positions, 2 kv heads, at 40 us for the longest ones.)  Few and short streams have a cluster each instead, whose CTAs take even parts and join them in shared
+    // positions, 2 kv heads, at 40 us for the longest ones.)  Few and short streams have a cluster each instead, whose CTAs take even parts and join them in shared
     // memory: no second kernel, no scratch.
     int unit = 0, stop = 1;                            // (the host sees to it that they fit)
     if constexpr (SHARE) {
@@ -780,7 +782,8 @@ static int pa_launch(const PaParams& p, int n, cudaStream_t stream) {
     e = launch(packed_attention_kernel<HD, NT, F32, CT, true>, dim3(p.ctas), dim3(PA_THREADS), smem, stream, p);
     if (e != cudaSuccess) return (int)e;
     constexpr int COLS = 8 * NT;
-    // (many CTAs a stream: a CTA joins one column, not a warp)
+    // (many CTAs a stream: a CTA joins one column, not a warp: 1 row of 131,072 positions, 4 kv heads, 25.5 us with attention, by warps 32.4; 4 rows 68.5 and 70.2; but 16
+    // rows of 8,000 28.9 and 27.9, 64 rows 76.4 and 72.2)
     e = p.ctas > 8 * n * p.heads_all ? launch(packed_merge_kernel<HD, F32, PM_WARPS>, dim3(n, p.heads_all, COLS), dim3(PM_WARPS * 32), 0, stream, p, COLS)
                                      : launch(packed_merge_kernel<HD, F32, 1>, dim3(n, p.heads_all, NT), dim3(PM_WARPS * 32), 0, stream, p, COLS);
     return e == cudaSuccess ? BG_OK : (int)e;

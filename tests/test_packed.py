@@ -164,7 +164,8 @@ def test_a_plan_takes_every_row_once(lens, nh, nkv, hd, dtype):
         assert 1 <= n <= plan.bq
         taken += [(longs[i][0], r) for r in range(r0, r0 + n)]
     assert sorted(taken, key=lambda x: x[1]) == [(i, sum(lens[:i]) + j) for i, n in enumerate(lens) for j in range(n)]
-    assert all(n >= ops.PACKED_LONG_ROWS for _, _, n in longs) and (dtype == BF16 or not longs)
+    streams = lambda n: -(-n // max(1, 16 // (nh // nkv))) * nkv * -(-nh // nkv // 16)
+    assert [i for i, _, _ in longs] == [i for i, n in enumerate(lens) if dtype == BF16 and n > 1 and streams(n) > ops.PACKED_LONG_STREAMS]
 
 
 def test_plans_refuse_what_does_not_fit():
@@ -183,7 +184,7 @@ def test_ctas_that_share_streams_have_work(streams, positions, at_once):
     n, cluster = ops.packed_ctas(streams, min(streams, 64), positions, at_once)
     units = -(-positions // 256)
     assert n <= at_once and n <= streams * units and cluster in (1, 2, 4, 8) and cluster < 2 * units and (cluster == 1 or cluster * streams <= at_once)
-    assert not n or (cluster == 1 and streams < 16 * at_once and units > ops.PACKED_TURNS)
+    assert not n or (cluster == 1 and units > 3)
     assert ops.packed_ctas(2, 1025, 100000, 296) == (0, 8)
 
 
@@ -452,7 +453,11 @@ def test_a_held_group_that_is_no_number_shows_where_it_is_seen(dtype, what):
 @pytest.mark.parametrize("nh,nkv,hd,page,dtype", [(12, 2, 128, 64, BF16), (14, 2, 64, 16, BF16), (20, 1, 128, 48, BF16), (4, 4, 64, 128, BF16), (12, 2, 128, 64, F32),
                                                    (9, 1, 64, 16, F32)])
 @pytest.mark.parametrize("options", [dict(), dict(window=50), dict(softcap=9.0, sink=True)], ids=["plain", "window", "squashed"])
-def test_attention_of_portions(parts, nh, nkv, hd, page, dtype, options):
+@pytest.mark.parametrize("many", [0, 1 << 30], ids=["written out", "packed"])
+def test_attention_of_portions(parts, nh, nkv, hd, page, dtype, options, many, monkeypatch):
+    if dtype == F32 and not many:
+        pytest.skip("float queries have no pages written out")
+    monkeypatch.setattr(ops, "PACKED_LONG_STREAMS", many)
     parts = [tuple(int(v) for v in p.split(":")) for p in parts.split(",")]
     lens, starts = [n for n, _ in parts], [s for _, s in parts]
     lengths = [n + s for n, s in parts]
@@ -478,8 +483,9 @@ def test_attention_of_portions(parts, nh, nkv, hd, page, dtype, options):
 @GPU
 @pytest.mark.parametrize("key,value,query", [(1e-12, 1e-20, 1e9), (3e6, 1e7, 1e-6), (1e20, 1e30, 1e-20), (1.0, 1e-30, 1.0)])
 @pytest.mark.parametrize("hd", [64, 128])
-def test_portions_over_keys_and_values_of_any_scale(key, value, query, hd):
+def test_portions_over_keys_and_values_of_any_scale(key, value, query, hd, monkeypatch):
     """Half precision holds the written-out pages by a power of two for each kv head."""
+    monkeypatch.setattr(ops, "PACKED_LONG_STREAMS", 0)
     nh, nkv, page, n = 4, 2, 32, 100
     table, pages = make_table([n], page)
     pool = make_pool(pages, nkv, hd, page, seed=3)
@@ -730,8 +736,9 @@ def test_two_streams_at_once():
 
 
 @GPU
-def test_rows_apart_in_memory():
+def test_rows_apart_in_memory(monkeypatch):
     """Queries, results and portions' rows as parts of wider rows."""
+    monkeypatch.setattr(ops, "PACKED_LONG_STREAMS", 20)                        # (the first request's pages are written out)
     nh, nkv, hd, page, lens = 6, 2, 64, 32, [70, 1, 9]
     lengths = [200, 300, 9]
     table, pages = make_table(lengths, page)
@@ -751,8 +758,9 @@ def test_rows_apart_in_memory():
 
 
 @GPU
-def test_pages_beyond_four_gigabytes():
+def test_pages_beyond_four_gigabytes(monkeypatch):
     """A pool of 5 GB whose last pages are used: every call finds them."""
+    monkeypatch.setattr(ops, "PACKED_LONG_STREAMS", 30)                        # (the portion's pages are written out)
     nh, nkv, hd, page, length = 8, 4, 128, 64, 150
     few = make_pool(3, nkv, hd, page, bounds=True, seed=1)
     pages = 5_000_000_000 // few[0].numel()
@@ -807,7 +815,8 @@ def test_calls_without_rows():
 # ------------------------------------------------------------------------------------------------ refusals
 @GPU
 @pytest.mark.parametrize("entry,request_", [(-1, 0), (9, 0), (-5, 0), (0, 3)])
-def test_bad_pages_are_recorded(entry, request_):
+def test_bad_pages_are_recorded(entry, request_, monkeypatch):
+    monkeypatch.setattr(ops, "PACKED_LONG_STREAMS", 0)                         # (the many rows' pages are written out)
     """A table's entry outside the pool, or a request without a table: nothing outside is touched, and the status says so."""
     hd, page = 64, 16
     pool = make_pool(3, 1, hd, page, bounds=True).cuda()

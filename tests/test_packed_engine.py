@@ -71,11 +71,13 @@ def engine(folder, dtype, **kw):
 @GPU
 @pytest.mark.parametrize("name,config", [("D", TINY_D), ("W", WIDE)])
 @pytest.mark.parametrize("dtype,tol", [("float32", 2e-3), ("bfloat16", 8e-2)])
-def test_logits_are_those_of_keys_and_values_in_4_bits(model_root, name, config, dtype, tol):
+@pytest.mark.parametrize("many", [20, 240])
+def test_logits_are_those_of_keys_and_values_in_4_bits(model_root, name, config, dtype, tol, many, monkeypatch):
     """float32: a key or value may lie so near the border of two codes that the layer's own rounding takes the other (a step of one feature of one position).
     bfloat16: many do.  A number that is off by d before it is rounded to steps of s crosses a border with probability d / s, and is then off by s: by sqrt(d s) in
     the mean of squares.  Of 64 normal numbers the largest and smallest lie 4.7 deviations apart, so s = 4.7 / 15 = 0.31 of one; d is what bfloat16 is allowed
     without such rounding, 2e-2: sqrt(2e-2 * 0.31) = 7.9e-2."""
+    monkeypatch.setattr(ops, "PACKED_LONG_STREAMS", many)                      # (portions by either way)
     folder = make_model(model_root, "packed" + name, config=config, std=0.05, bias_std=0.05)
     ids, other = seeded_ids(170, config["vocab_size"], 5), seeded_ids(90, config["vocab_size"], 6)
     want, want_other = oracle(folder, ids), oracle(folder, other)
