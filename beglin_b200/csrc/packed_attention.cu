@@ -8,18 +8,20 @@
 // are applied in float outside the product:
 //     q . k   = sum over groups of  step (sum q u) + lowest (sum q)
 //     p V     = sum over positions of  (p step) u + p lowest
-// so that the only rounding of the cache's side is that of p step to bfloat16.  Keys: 16 positions by 16 features times features by 8 columns; values: 16
+//             = sum over positions of  r u - 8 r + p (lowest + 8 step),  r = p step rounded to bfloat16 (but for float queries),
+// so that the only rounding of the cache's side is that of r, and it counts for u - 8 alone: 4.6 in the root of the mean of
+// squares, where u are 8 (results 0.0021 of their norm off, with u alone 0.0029; rounding them to bfloat16 is 0.0017).  The sum of r is a product with -1; 2 us of 70.  Keys: 16 positions by 16 features times features by 8 columns; values: 16
 // features by 16 positions times positions by columns.  A column is one (row, query head): the queries of a kv head are the narrow side, so 8 heads waste
 // nothing of the product and a code is unpacked once for all of them.  The weights reach the second product's layout through movmatrix.  Float queries and
 // weights go in three bfloat16 parts.
 //
-// Ranges: a row of queries is scaled by the power of two that brings its largest to 2^100.  Weights carry 2^64, so values may have steps up to 2^63, and those
-// under 2^-50 lose digits.
+// Ranges: a row of queries is scaled by the power of two that brings its largest to 2^100.  Weights carry 2^64, and 2^8 where the maximum has not moved, so values
+// may have steps up to 2^36 (32,768 positions of such weights), and those under 2^-50 lose digits.
 //
 // Why this shape: at the bandwidth of HBM a position of a kv head (144 bytes for heads of 128) has to be done in some 6 cycles of an SM, 25 warp instructions at
-// best.  It takes 17 for 8 columns, half of them on the units of integers and logic, which take one every two cycles; with the queries on the left (16 rows, half
-// of them empty) it took the tensor cores twice the products and the softmax twice the numbers.  4 rows of 131,072 positions, 4 kv heads: 68 us, 65 % of the bandwidth of
-// a copy (83 % but for what does not grow with the length: a start, two kernels, where results meet); 64 rows of 2,048 to 8,192, 2 kv heads: 34 us, 42 %.  Bound
+// best.  It takes 18 for 8 columns, half of them on the units of integers and logic, which take one every two cycles; with the queries on the left (16 rows, half
+// of them empty) it took the tensor cores twice the products and the softmax twice the numbers.  4 rows of 131,072 positions, 4 kv heads: 70 us, 63 % of the bandwidth of
+// a copy (some 80 % but for what does not grow with the length: a start, two kernels, where results meet); 64 rows of 2,048 to 8,192, 2 kv heads: 35 us, 41 %.  Bound
 // by these instructions: with all pages in the L2 it takes 95 % of the time.  A warp has a ring of its own (STAGES chunks of 16 or 32 positions, one bulk copy each) and its own running maximum, sum
 // and result, so that nothing in the loop waits for another warp; the warps' results meet at the end, those of a long request's ranges in packed_merge_kernel.
 #include <type_traits>
@@ -87,6 +89,7 @@ __device__ __forceinline__ unsigned pa_pack(float a, float b) {
 constexpr float PA_UP = 64.0f;                         // weights, and sums of them, are 2^(x - maximum) times 2^PA_UP
 constexpr float PA_SLACK = 8.0f;
 constexpr unsigned PA_ONE = 0x00010001u;               // the code 1 of two features, at bits 0
+constexpr unsigned PA_MINUS = 0xbf80bf80u;             // -1 twice
 // The pair of codes at bits 4 i of both halves of a word: u 2^-133 where i is even, 16 u 2^-133 where it is odd.
 __device__ __forceinline__ unsigned pa_codes(unsigned w, int i) { return (i < 2 ? w : w >> 8) & (i % 2 ? 0x00f000f0u : 0x000f000fu); }
 __device__ __forceinline__ void pa_bulk_load(void* dst, const void* src, unsigned bytes, unsigned long long* bar) {
@@ -495,7 +498,7 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
-                        const float step = pair_step(vp[half][gr]), lowest = pair_lowest(vp[half][gr]);
+                        const float step = pair_step(vp[half][gr]), lowest = F32 ? pair_lowest(vp[half][gr]) : fmaf(8.0f, step, pair_lowest(vp[half][gr]));
                         float e[2];
 #pragma unroll
                         for (int j = 0; j < 2; ++j) {
@@ -518,6 +521,14 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
                             b[0][nt][half] = pa_transposed(pa_pack(e[0], e[1]));
                         }
                     }
+                if constexpr (!F32) {                  // less 8 (p step) as it was rounded; an eighth of it in each of the 8 lanes whose sums meet
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        float sum[4] = {low[nt][gr][0], low[nt][gr][1], 0.0f, 0.0f};
+                        pa_mma(sum, PA_MINUS, PA_MINUS, PA_MINUS, PA_MINUS, b[0][nt][0], b[0][nt][1]);
+                        low[nt][gr][0] = sum[0]; low[nt][gr][1] = sum[1];
+                    }
+                }
                 const unsigned ab[2] = {__byte_perm(vw[gr][0], vw[gr][1], 0x5410), __byte_perm(vw[gr][0], vw[gr][1], 0x7632)};
                 const unsigned cd[2] = {__byte_perm(vw[gr][2], vw[gr][3], 0x5410), __byte_perm(vw[gr][2], vw[gr][3], 0x7632)};
 #pragma unroll

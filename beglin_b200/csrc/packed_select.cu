@@ -13,9 +13,10 @@
 // 16 additions to an accumulator that is cut off make 2^-18 of that, E is 2^-16; queries in float are rounded to bfloat16 for this, E is then 2^-8.  (By float
 // units, four lanes a page: 10 us for 256 pages of a CTA, of instructions.)
 //
-// A cluster of CTAs takes one (row, kv head), a CTA a part of the pages, a warp 16 of them at a time; the scores go to the first CTA's shared memory, which finds a border by quartering: how many scores reach a threshold, two bits a round from the first that differs, until exactly as many
-// do as are wanted or no bit is left.  (Counting 8 bits at a time with shared-memory atomics put nearly every score into one counter, one after the other.)
-// Bound by latency: three meetings of the cluster and two searches for a border.
+// A cluster of CTAs takes one (row, kv head), a CTA a part of the pages, a warp 16 of them at a time; the scores go to the first CTA's shared
+// memory, which finds a border by quartering: how many scores reach a threshold, two bits a round from the first that differs, until exactly as many do as are
+// wanted or no bit is left.  (Counting 8 bits at a time with shared-memory atomics put nearly every score into one counter, one after the other.)
+// Bound by latency: three meetings of the cluster and two searches for a border.  4 rows of 131,072 positions, 4 kv heads, pages of 64: 20 us, an eighth of them its reads.
 #include "packed.cuh"
 
 namespace bg {
@@ -322,7 +323,8 @@ __global__ void __launch_bounds__(PS_THREADS, 2) packed_select_kernel(const PsPa
 
 template <typename TQ, int HD>
 static int ps_launch(const PsParams& p, cudaStream_t stream) {
-    // as many CTAs a (row, kv head) as two an SM give all of them at once, and at least as many as hold the scores of the pages
+    // as many CTAs a (row, kv head) as two an SM give all of them at once, and at least as many as hold the scores of the pages (4 kv heads, us by this rule, always 8, and as
+    // few as hold them: 4 rows of 131,072 positions 20.9, 21.2, 42.4; 16 rows of 32,000 19.1, 35.5, 24.7; 64 rows of 8,000 16.5, 93.6, 16.5)
     auto bytes = [&](int ctas) { return (size_t)(p.pages_most + 1) / 2 * 8 + (size_t)((p.pages_most + ctas - 1) / ctas) * 8; };
     int ctas = PS_CLUSTER;
     while (ctas > 1 && (long long)p.T * p.nkv * ctas > 2LL * sm_count() && bytes(ctas / 2) <= 100 * 1024) ctas /= 2;
