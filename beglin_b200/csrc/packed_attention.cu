@@ -9,21 +9,22 @@
 //     q . k   = sum over groups of  step (sum q u) + lowest (sum q)
 //     p V     = sum over positions of  (p step) u + p lowest
 //             = sum over positions of  r u - 8 r + p (lowest + 8 step),  r = p step rounded to bfloat16 (but for float queries),
-// so that the only rounding of the cache's side is that of r, and it counts for u - 8 alone: 4.6 in the root of the mean of
-// squares, where u are 8 (results 0.0021 of their norm off, with u alone 0.0029; rounding them to bfloat16 is 0.0017).  The sum of r is a product with -1; 2 us of 70.  Keys: 16 positions by 16 features times features by 8 columns; values: 16
-// features by 16 positions times positions by columns.  A column is one (row, query head): the queries of a kv head are the narrow side, so 8 heads waste
-// nothing of the product and a code is unpacked once for all of them.  The weights reach the second product's layout through movmatrix.  Float queries and
-// weights go in three bfloat16 parts.
+// so that the only rounding of the cache's side is that of r, and it counts for u - 8 alone: 4.6 in the root of the mean of squares, where u are 8.8 (results
+// 0.0021 of their norm off, with u alone 0.0029; rounding them to bfloat16 is 0.0017).  The sum of r is a product with -1; 2 us of 70.  Keys: 16 positions
+// by 16 features times features by 8 columns; values: 16 features by 16 positions times positions by columns.  A column is one (row, query head): the
+// queries of a kv head are the narrow side, so 8 heads waste nothing of the product and a code is unpacked once for all of them.  The weights reach the
+// second product's layout through movmatrix.  Float queries and weights go in three bfloat16 parts.
 //
 // Ranges: a row of queries is scaled by the power of two that brings its largest to 2^100.  Weights carry 2^64, and 2^8 where the maximum has not moved, so values
 // may have steps up to 2^36 (32,768 positions of such weights), and those under 2^-50 lose digits.
 //
-// Why this shape: at the bandwidth of HBM a position of a kv head (144 bytes for heads of 128) has to be done in some 6 cycles of an SM, 25 warp instructions at
-// best.  It takes 18 for 8 columns, half of them on the units of integers and logic, which take one every two cycles; with the queries on the left (16 rows, half
-// of them empty) it took the tensor cores twice the products and the softmax twice the numbers.  4 rows of 131,072 positions, 4 kv heads: 70 us, 63 % of the bandwidth of
-// a copy (some 80 % but for what does not grow with the length: a start, two kernels, where results meet); 64 rows of 2,048 to 8,192, 2 kv heads: 35 us, 41 %.  Bound
-// by these instructions: with all pages in the L2 it takes 95 % of the time.  A warp has a ring of its own (STAGES chunks of 16 or 32 positions, one bulk copy each) and its own running maximum, sum
-// and result, so that nothing in the loop waits for another warp; the warps' results meet at the end, those of a long request's ranges in packed_merge_kernel.
+// Why this shape: at the bandwidth of HBM a position of a kv head (144 bytes for heads of 128) has to be done in some 6 cycles of an SM, 25 warp
+// instructions at best.  It takes 18 for 8 columns, half of them on the units of integers and logic, which take one every two cycles; with the queries on
+// the left (16 rows, half of them empty) it took the tensor cores twice the products and the softmax twice the numbers.  4 rows of 131,072 positions, 4 kv
+// heads: 70 us, 63 % of the bandwidth of a copy (some 80 % but for what does not grow with the length: a start, two kernels, where results meet); 64 rows
+// of 2,048 to 8,192, 2 kv heads: 35 us, 41 %.  Bound by these instructions: with all pages in the L2 it takes 95 % of the time.  A warp has a ring of its
+// own (STAGES chunks of 16 or 32 positions, one bulk copy each) and its own running maximum, sum and result, so that nothing in the loop waits for another
+// warp; the warps' results meet at the end, those of a long request's ranges in packed_merge_kernel.
 #include <type_traits>
 
 #include "packed.cuh"
@@ -793,8 +794,8 @@ static int pa_launch(const PaParams& p, int n, cudaStream_t stream) {
     e = launch(packed_attention_kernel<HD, NT, F32, CT, true>, dim3(p.ctas), dim3(PA_THREADS), smem, stream, p);
     if (e != cudaSuccess) return (int)e;
     constexpr int COLS = 8 * NT;
-    // (many CTAs a stream: a CTA joins one column, not a warp: 1 row of 131,072 positions, 4 kv heads, 25.5 us with attention, by warps 32.4; 4 rows 68.5 and 70.2; but 16
-    // rows of 8,000 28.9 and 27.9, 64 rows 76.4 and 72.2)
+    // (many CTAs a stream: a CTA joins one column, not a warp: 1 row of 131,072 positions, 4 kv heads, 25.5 us with attention, by warps 32.4; 4 rows 68.5 and
+    // 70.2; but 16 rows of 8,000 28.9 and 27.9, 64 rows 76.4 and 72.2)
     e = p.ctas > 8 * n * p.heads_all ? launch(packed_merge_kernel<HD, F32, PM_WARPS>, dim3(n, p.heads_all, COLS), dim3(PM_WARPS * 32), 0, stream, p, COLS)
                                      : launch(packed_merge_kernel<HD, F32, 1>, dim3(n, p.heads_all, NT), dim3(PM_WARPS * 32), 0, stream, p, COLS);
     return e == cudaSuccess ? BG_OK : (int)e;

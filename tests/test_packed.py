@@ -424,6 +424,19 @@ def test_large_scores_and_a_row_that_is_no_number(dtype):
 
 
 @GPU
+@pytest.mark.parametrize("lengths", [[4096, 3000], [2000] * 70], ids=["few", "many"])
+def test_weights_are_rounded_beside_the_middle_of_the_codes(lengths):
+    """Weights next to equal, so that every one of them is rounded.  A rounding to bfloat16 is off by at most 2^-8, by 2^-8 / sqrt(3) in the root of the mean of
+    squares; one such is that of the results, one that of weight and step together, which counts for step (u - 8): as large as the values are, in the root of the
+    mean of squares (codes in 0 .. 15 are 4.6 from 8, values are 7.5 steps lower and half a unit beside): 2^-8 sqrt(2 / 3) = 0.0032.  Against u itself, 8.8 in the
+    root of the mean of squares, the second would be 1.9 times that."""
+    nh, nkv, hd, page = 12, 2, 128, 64
+    q = torch.randn((len(lengths), nh * hd), generator=torch.Generator().manual_seed(1)) * 0.05
+    got, want = single(lengths, nh, nkv, hd, page, BF16, q=q)
+    assert float((got.double() - want).norm() / want.norm()) < 0.0032
+
+
+@GPU
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("what", ["key", "value"])
 def test_a_held_group_that_is_no_number_shows_where_it_is_seen(dtype, what):
