@@ -1029,8 +1029,8 @@ class PackedPlan:
 
 
 def packed_plan(lens, nh: int, nkv: int, hd: int, dtype: torch.dtype, page_size: int, device, row_start=None, starts=None) -> PackedPlan:
-    """The plan of `packed_attention` for a step whose request i brings lens[i] rows, from row row_start[i] on (default: one behind the other).  `starts`: the
-    positions of their first rows, where the host knows them (less room is made then).  Rows go in blocks of as many (row, query head) pairs as the packed kernel has
+    """The plan of `packed_attention` for a step whose request i brings lens[i] rows, from row row_start[i] on (default: one behind the other; together they are the
+    step's rows, each once), at consecutive positions.  `starts`: the positions of their first rows, where the host knows them (less room is made then).  Rows go in blocks of as many (row, query head) pairs as the packed kernel has
     columns; requests of more than PACKED_LONG_STREAMS kv heads of such blocks (bfloat16) have their pages written out in half precision and run the prompt attention."""
     lens = [int(n) for n in lens]
     if any(n < 0 for n in lens) or nh <= 0 or nkv <= 0 or nh % nkv:
@@ -1042,6 +1042,11 @@ def packed_plan(lens, nh: int, nkv: int, hd: int, dtype: torch.dtype, page_size:
         row_start = [sum(lens[:i]) for i in range(len(lens))] if len(lens) < 64 else np.concatenate([[0], np.cumsum(lens)[:-1]]).tolist()
     if len(row_start) != len(lens) or (starts is not None and len(starts) != len(lens)):
         raise KernelError("packed_plan: a first row and a first position for every request")
+    at = 0
+    for first, n in sorted((r, n) for r, n in zip(row_start, lens) if n):
+        if first != at:
+            raise KernelError(f"packed_plan: first rows {row_start} of requests of {lens} rows: every row from nought on belongs to one request")
+        at += n
     return PackedPlan(lens, [int(r) for r in row_start], nh, nkv, hd, dtype, page_size, device, starts)
 
 
