@@ -910,14 +910,16 @@ def _packed_pool(what: str, pool: torch.Tensor, hd: int, page_size: int, nkv: Op
     return shape[2]
 
 
-def _packed_rows_of(what: str, positions: torch.Tensor, row_req: Optional[torch.Tensor], block_table: torch.Tensor, n_rows: int) -> None:
+def _packed_rows_of(what: str, positions: torch.Tensor, block_table: torch.Tensor, n_rows: int) -> None:
     _i32(positions, f"{what}: positions"); _i32(block_table, f"{what}: block_table")
     if block_table.dim() != 2 or positions.dim() != 1 or positions.numel() < n_rows:
         raise KernelError(f"{what}: a position for every row, block tables [requests, pages]")
-    if row_req is not None:
-        _i32(row_req, f"{what}: row_req")
-        if row_req.dim() != 1 or row_req.numel() < n_rows:
-            raise KernelError(f"{what}: a request for every row")
+
+
+def _packed_requests_of(what: str, row_req: torch.Tensor, n_rows: int) -> None:
+    if row_req is None or row_req.dim() != 1 or row_req.numel() < n_rows:
+        raise KernelError(f"{what}: a request for every row")
+    _i32(row_req, f"{what}: row_req")
 
 
 def packed_append(src: torch.Tensor, q_out: torch.Tensor, nh: int, nkv: int, hd: int, rot: int, interleaved: bool, cos_sin: Optional[torch.Tensor],
@@ -931,7 +933,8 @@ def packed_append(src: torch.Tensor, q_out: torch.Tensor, nh: int, nkv: int, hd:
     parts, stride = _parts(src, "packed_append: src")
     T, width = src.shape[-2], src.shape[-1]
     block = _packed_pool("packed_append", pool, hd, page_size, nkv)
-    _packed_rows_of("packed_append", positions, row_req, block_table, T)
+    _packed_rows_of("packed_append", positions, block_table, T)
+    _packed_requests_of("packed_append", row_req, T)
     if src.stride(-1) != 1 or width < (nh + 2 * nkv) * hd:
         raise KernelError(f"packed_append: rows of {width} features cannot hold q, k, v ({(nh + 2 * nkv) * hd})")
     if q_out.dim() != 2 or q_out.stride(1) != 1 or q_out.shape[1] < nh * hd or q_out.shape[0] < T or (T and q_out.data_ptr() == src.data_ptr()):
@@ -957,7 +960,8 @@ def packed_bounds(pool: torch.Tensor, positions: torch.Tensor, row_req: torch.Te
     _here("packed_bounds", pool, positions, row_req, block_table, status)
     block = _packed_pool("packed_bounds", pool, hd, page_size, bounds=True)
     T = positions.numel()
-    _packed_rows_of("packed_bounds", positions, row_req, block_table, T)
+    _packed_rows_of("packed_bounds", positions, block_table, T)
+    _packed_requests_of("packed_bounds", row_req, T)
     if T == 0:
         return
     with phase("rope+kv_write"):
@@ -975,7 +979,8 @@ def packed_rows(pool: torch.Tensor, positions: torch.Tensor, row_req: torch.Tens
     _here("packed_rows", pool, positions, row_req, block_table, out, status)
     block = _packed_pool("packed_rows", pool, hd, page_size)
     T = positions.numel()
-    _packed_rows_of("packed_rows", positions, row_req, block_table, T)
+    _packed_rows_of("packed_rows", positions, block_table, T)
+    _packed_requests_of("packed_rows", row_req, T)
     if tuple(out.shape) != (T, 2, pool.shape[1], hd) or not out.is_contiguous():
         raise KernelError(f"packed_rows: out is {tuple(out.shape)}, expected contiguous {(T, 2, pool.shape[1], hd)}")
     if T == 0:
@@ -1081,7 +1086,7 @@ def packed_attention(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Ten
     _here("packed_attention", q, pool, block_table, positions, out, status, sink_weight, pages, None if plan is None else plan.short)
     block = _packed_pool("packed_attention", pool, hd, page_size, nkv)
     T = q.shape[0]
-    _packed_rows_of("packed_attention", positions, None, block_table, T)
+    _packed_rows_of("packed_attention", positions, block_table, T)
     if q.dim() != 2 or q.stride(1) != 1 or q.shape[1] < nh * hd or out.dim() != 2 or out.stride(1) != 1 or out.shape[1] < nh * hd or out.shape[0] < T:
         raise KernelError("packed_attention: q and out are [T, nh*hd] with unit inner stride")
     if q.dtype != out.dtype or _dt(q) < 0:
@@ -1151,7 +1156,7 @@ def packed_select(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor
     _here("packed_select", q, pool, block_table, positions, out, status)
     block = _packed_pool("packed_select", pool, hd, page_size, nkv, bounds=True)
     T = q.shape[0]
-    _packed_rows_of("packed_select", positions, None, block_table, T)
+    _packed_rows_of("packed_select", positions, block_table, T)
     _i32(out, "packed_select: out")
     if q.dim() != 2 or q.stride(1) != 1 or q.shape[1] < nh * hd or nkv <= 0 or nh % nkv:
         raise KernelError("packed_select: q is [T, nh*hd] with unit inner stride, whole groups of query heads to a kv head")

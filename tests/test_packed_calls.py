@@ -22,3 +22,17 @@ def test_a_plan_refuses_rows_that_the_step_does_not_have(lens, row_start):
 def test_a_plan_takes_rows_in_any_order():
     plan = ops.packed_plan([1, 0, 2, 1], 4, 2, 64, BF16, 64, device="cpu", row_start=[3, -7, 0, 2])
     assert plan.short.view(-1, 3).tolist() == [[0, 3, 1], [2, 0, 2], [3, 2, 1]]
+
+
+# ------------------------------------------------------------------------------------------------ calls without what they need
+def test_rows_need_their_requests(monkeypatch):
+    """Only attention knows whose a row is without a list of requests."""
+    monkeypatch.setattr(ops, "_here", lambda *a: None)                         # (nothing is launched)
+    hd, page, T = 64, 16, 3
+    pool, table, positions = make_pool(2, 1, hd, page, True), torch.zeros((T, 1), dtype=torch.int32), torch.zeros(T, dtype=torch.int32)
+    src, q = torch.zeros((T, 3 * hd), dtype=BF16), torch.zeros((T, hd), dtype=BF16)
+    for call in (lambda: ops.packed_append(src, q, 1, 1, hd, 0, False, None, positions, None, table, pool, page, None),
+                 lambda: ops.packed_bounds(pool, positions, None, table, hd, page, None),
+                 lambda: ops.packed_rows(pool, positions, None, table, hd, page, torch.empty((T, 2, 1, hd)), None)):
+        with pytest.raises(ops.KernelError, match="a request for every row"):
+            call()
