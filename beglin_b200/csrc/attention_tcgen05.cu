@@ -196,7 +196,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
     __shared__ int row_of[SHARED ? 2 * AT_BM : 1];
     __shared__ unsigned tmem_sh;
     __shared__ int failed;
-    __shared__ float unit_of[HALF ? AT_BM : 1];          // what a row's scores are multiplied with
+    __shared__ int shift_of[HALF ? AT_BM : 1];           // the power of two that a row's scores lack
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
     // the blocks with the most keys (the last ones of a prompt) are handed out first, for every kv head, so that
@@ -281,7 +281,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
                     h[i] = *reinterpret_cast<const unsigned*>(&x);
                 }
                 v = make_uint4(h[0], h[1], h[2], h[3]);
-                if (c == 0) unit_of[r] = exp2f((float)min(e + p.shifts[req * p.nkv + kvh].x, 120));
+                if (c == 0) shift_of[r] = e + p.shifts[req * p.nkv + kvh].x;
             }
             const int cb = c >> 3, cc = c & 7;
             const int rr = SHARED ? r & (AT_BM - 1) : r;
@@ -439,9 +439,13 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
         float m = -INFINITY, l = 0.0f;
         bool ok = true;
         const bool capped = p.cap_log2 > 0.0f;
-        const float unit_row = HALF ? unit_of[r] : 1.0f;
-        const float sl2 = (capped || EXT) ? 1.0f : HALF ? p.scale_log2 * unit_row : p.scale_log2;
-        const float cap_k = HALF ? p.cap_k * unit_row : p.cap_k;
+        // (HALF: never nought, which times the score of a hidden key, minus infinity, is no number, and never beyond float. Scores lie below 2^37: at 2^-100 they
+        // are noughts as they should be, at 2^90 the largest takes all)
+        auto scaled = [&](float by) {
+            if constexpr (HALF) return fminf(fmaxf(ldexpf(by, shift_of[r]), 0x1p-100f), 0x1p90f);
+            else return by;
+        };
+        const float sl2 = (capped || EXT) ? 1.0f : scaled(p.scale_log2), cap_k = scaled(p.cap_k);
         const float slope_l2 = (EXT && p.slopes && real) ? p.slopes[kvh * group + r % group] * AT_LOG2E : 0.0f;
         const int i_first = ALT ? grp : 0;                   // this group's first tile
         for (int i = i_first; i < n_turns && ok; i += (ALT ? 2 : 1)) {

@@ -36,3 +36,60 @@ def test_rows_need_their_requests(monkeypatch):
                  lambda: ops.packed_rows(pool, positions, None, table, hd, page, torch.empty((T, 2, 1, hd)), None)):
         with pytest.raises(ops.KernelError, match="a request for every row"):
             call()
+
+
+# ------------------------------------------------------------------------------------------------ portions whose pages are written out
+def portion(n, start, nh, nkv, hd, page, monkeypatch, change=None, scale=None, window=0, softcap=0.0, sink=False, dtype=BF16, many=0, most=None, given=True):
+    """`n` rows of one request behind `start` positions: (results [n, nh, hd], what 64 bits say).  `change` takes the queries [n, nh, hd] and the pairs (step,
+    lowest) of all pages [pages, kv heads, tiles, positions, keys and values, groups, 2]."""
+    monkeypatch.setattr(ops, "PACKED_LONG_STREAMS", many)
+    table, pages = make_table([start + n], page)
+    pool = make_pool(pages, nkv, hd, page, seed=3)
+    poison(pool, table, [start + n], hd, page)
+    q = torch.randn((n, nh, hd), generator=torch.Generator().manual_seed(2))
+    if change:
+        change(q, pool.unflatten(2, (page // 16, -1))[..., 16 * hd:].view(BF16).unflatten(3, (16, 2, hd // 64, 2)))
+    q, scale = q.flatten(1).to(dtype), 1 / math.sqrt(hd) if scale is None else scale
+    out, status = torch.full((n, nh * hd), 7.0, dtype=dtype, device="cuda"), ops.new_status("cuda")
+    ops.packed_attention(q.cuda(), pool.cuda(), table.cuda(), torch.arange(start, start + n, dtype=torch.int32, device="cuda"), nh, nkv, hd, page,
+                         most or start + n - 1, scale, out, status, window=window, softcap=softcap, sink=sink,
+                         plan=ops.packed_plan([n], nh, nkv, hd, dtype, page, "cuda", starts=[start] if given else None))
+    ops.raise_on_status(status)
+    want = plain_attention(q.view(n, nh, hd), pool, table, hd, page, [(0, start + i) for i in range(n)], scale, window, softcap, torch.zeros(nh) if sink else None)
+    return out.cpu().view(n, nh, hd), want
+
+
+@GPU
+@pytest.mark.parametrize("options", [dict(), dict(window=50), dict(softcap=9.0, sink=True)], ids=["plain", "window", "squashed"])
+@pytest.mark.parametrize("what", ["queries", "a row", "keys", "both", "values too", "tiny"])
+@pytest.mark.parametrize("nh,nkv,hd,page,n,start", [(4, 2, 128, 32, 100, 0), (6, 2, 64, 16, 70, 200)])
+def test_rows_and_heads_of_noughts_in_a_portion(nh, nkv, hd, page, n, start, what, options, monkeypatch):
+    """A row whose scores are all nought is the mean of the values that it sees: padded heads have such queries and keys."""
+    def change(q, pairs):
+        if what in ("queries", "both", "values too"):
+            q[:, :nh // nkv + 1] = 0.0
+        if what == "a row":
+            q[n // 2] = 0.0
+        if what in ("keys", "both", "values too"):
+            pairs[:, 0, :, :, 0] = 0.0
+        if what == "values too":
+            pairs[:, 0, :, :, 1] = 0.0
+        if what == "tiny":
+            q *= 1e-22
+            pairs[..., 0, :, :] *= 1e-22
+    near(*portion(n, start, nh, nkv, hd, page, monkeypatch, change, **options), BF16)
+
+
+@GPU
+@pytest.mark.parametrize("key,value,query", [(1e-12, 1e-20, 1e9), (3e6, 1e7, 1e-6), (1e20, 1e30, 1e-20), (1.0, 1e-30, 1.0), (1e-15, 1.0, 1e-15), (1e15, 1.0, 1e15), (1e-30, 1.0, 1.0)])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_queries_keys_and_values_of_any_scale_in_a_portion(key, value, query, hd, monkeypatch):
+    """Queries, keys and values each of a scale of their own, the scores made ordinary by `scale` alone."""
+    def change(q, pairs):
+        q *= query
+        pairs[..., 0, :, :] *= key
+        pairs[..., 1, :, :] *= value
+        pairs[:, 1] *= 0.01                                                    # the second kv head's scale is another
+    got, want = portion(100, 0, 4, 2, hd, 32, monkeypatch, change, scale=1 / (key * query * math.sqrt(hd)))
+    for heads, scale in ((slice(0, 2), value), (slice(2, 4), value * 0.01)):
+        near(got[:, heads].double() / scale, want[:, heads] / scale, BF16)
