@@ -34,6 +34,7 @@
 #include <cuda_fp16.h>
 
 #include "float_pairs.cuh"
+#include "packed.cuh"
 #include "page_tma.cuh"
 
 namespace bg {
@@ -272,7 +273,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
                 for (int i = 0; i < 4; ++i) top = fmaxf(top, fmaxf(fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xffff0000u))));
 #pragma unroll
                 for (int o = HD / 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                const int e = max(-100, (int)(__float_as_uint(top) >> 23) - 127 - 14);       // (a row of noughts, or one that is no number: whatever)
+                const int e = half_shift(top);           // (a row of noughts, or one that is no number: whatever)
                 const float down = __uint_as_float((unsigned)(127 - e) << 23);
                 unsigned h[4];
 #pragma unroll
@@ -651,7 +652,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
             const float l_all = l * a0 + other.y * a1 + (SINK ? at_ex2(sink_l2 - m_ref) : 0.0f);
             const float inv = (real && l_all > 0.0f) ? 1.0f / l_all : 0.0f;
             const float back = HALF ? exp2f((float)at_value_shift(p, req * p.nkv + kvh)) : 1.0f;
-            const float w0 = HALF ? a0 * inv * back : a0 * inv, w1 = HALF ? a1 * inv * back : a1 * inv;
+            const float w0 = a0 * inv, w1 = a1 * inv;
             const bool has1 = !ALT || n_tiles > 1;       // with one tile the second group's accumulator was never written
             __nv_bfloat16* o = p.out + (size_t)(row0 + qi) * p.out_stride + (size_t)(kvh * group + g) * HD;
 #pragma unroll
@@ -665,7 +666,10 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
                     for (int q = 0; q < 32; q += 8) {
                         float v8[8];
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) v8[k] = t[q + k] * w0 + (has1 ? u[q + k] * w1 : 0.0f);
+                        for (int k = 0; k < 8; ++k) {
+                            v8[k] = t[q + k] * w0 + (has1 ? u[q + k] * w1 : 0.0f);
+                            if constexpr (HALF) v8[k] *= back;       // (at the end: at the ends of its range the product with a weight is no normal number)
+                        }
                         store8(o + c0 + q, v8);
                     }
                 }

@@ -393,7 +393,7 @@ __global__ void __launch_bounds__(PK_THREADS) packed_reach_kernel(const PkUnpack
     for (int v = 0; v < 2; ++v) {
         float all = 0.0f;
         for (int i = 0; i < PK_CLUSTER; ++i) all = fmaxf(all, every[v][i]);
-        e[v] = min(100, max(-100, (int)(__float_as_uint(all) >> 23) - 127 - 14));
+        e[v] = half_shift(all);
     }
     p.shifts[(size_t)n * p.nkv + kvh] = make_int2(e[0], e[1]);
 }

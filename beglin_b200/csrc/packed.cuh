@@ -41,6 +41,10 @@ __host__ __device__ inline long long packed_tile_bytes(int hd) { return hd == 64
 __device__ __forceinline__ float pair_step(unsigned pair) { return __uint_as_float(pair << 16); }
 __device__ __forceinline__ float pair_lowest(unsigned pair) { return __uint_as_float(pair & 0xffff0000u); }
 
+// The power of two (times 2^14) of the largest of some numbers: less that, they lie below 2^15, where half precision holds them whatever their scale is. 2^-this
+// is a normal number too.
+__device__ __forceinline__ int half_shift(float largest) { return min(113, max(-126, (int)(__float_as_uint(largest) >> 23) - 127 - 14)); }
+
 // The 8 values of a word of codes (KEY: a key's order of nibbles).
 template <bool KEY>
 __device__ __forceinline__ void packed_values(unsigned word, unsigned pair, float (&v)[8]) {

@@ -93,3 +93,14 @@ def test_queries_keys_and_values_of_any_scale_in_a_portion(key, value, query, hd
     got, want = portion(100, 0, 4, 2, hd, 32, monkeypatch, change, scale=1 / (key * query * math.sqrt(hd)))
     for heads, scale in ((slice(0, 2), value), (slice(2, 4), value * 0.01)):
         near(got[:, heads].double() / scale, want[:, heads] / scale, BF16)
+
+
+@GPU
+@pytest.mark.parametrize("key,value,query", [(1e36, 1e36, 1e-36), (1e-36, 1e-34, 1e36)])
+def test_numbers_next_to_the_ends_of_their_range_in_a_portion(key, value, query, monkeypatch):
+    def change(q, pairs):
+        q *= query
+        pairs[..., 0, :, :] *= key
+        pairs[..., 1, :, :] *= value
+    got, want = portion(100, 0, 4, 2, 128, 32, monkeypatch, change)
+    near(got.double() / value, want / value, BF16)
