@@ -86,7 +86,8 @@ struct AttnTcSharedParams : AttnTcParams {
 };
 // What the HALF instances take besides.
 struct AttnTcHalfParams : AttnTcParams {
-    const int2* shifts;         // [n][nkv] of the requests that the query blocks name: the cache holds keys 2^-x and values 2^-y
+    const PkWritten* written;   // [n][nkv] of the requests that the query blocks name: how the cache holds its keys and values
+    const unsigned long long* marks;            // [num_pages][nkv][features / 64]: positions whose values are no numbers, written as noughts
 };
 template <bool V> struct AtSplit { static constexpr bool value = V; };
 // SHARED: of the pairs of exponentials every eighth is the float units' (256 rows of 28 heads over 32,768 positions, 140 CTAs: 113.5 us; none of them
@@ -97,8 +98,22 @@ template <> struct AtParams<true, false, false> { using type = AttnTcDiffParams;
 template <> struct AtParams<false, true, false> { using type = AttnTcSharedParams; };
 template <> struct AtParams<false, false, true> { using type = AttnTcHalfParams; };
 
-__device__ __forceinline__ int at_value_shift(const AttnTcParams&, int) { return 0; }
-__device__ __forceinline__ int at_value_shift(const AttnTcHalfParams& p, int i) { return p.shifts[i].y; }
+// The groups of 64 features (a bit each) in which a row that sees the positions lo .. pos is no number, because one of those values is none.
+template <int HD>
+__device__ __forceinline__ unsigned at_no_numbers(const AttnTcHalfParams& p, int req, int kvh, int lo, int pos) {
+    unsigned groups = 0;
+    for (int page = lo / PK_WIDE; page <= pos / PK_WIDE && page < p.max_pages; ++page) {
+        const int at = p.block_table[(size_t)req * p.max_pages + page];
+        if (at < 0 || at >= p.num_pages) continue;
+        unsigned long long seen = ~0ull;
+        if (page == lo / PK_WIDE) seen &= ~0ull << (lo % PK_WIDE);
+        if (page == pos / PK_WIDE) seen &= ~0ull >> (PK_WIDE - 1 - pos % PK_WIDE);
+#pragma unroll
+        for (int g = 0; g < HD / 64; ++g)
+            if (p.marks[((size_t)at * p.nkv + kvh) * (HD / 64) + g] & seen) groups |= 1u << g;
+    }
+    return groups;
+}
 
 __device__ __forceinline__ float at_ex2(float x) {
     float y;
@@ -152,7 +167,8 @@ __device__ __forceinline__ float at_squash(float x, float cap_log2, float cap_k)
 // HALF: the operands are half precision (11 bits in place of bfloat16's 8): the cache is one that was written out of 4 bits for this step, its keys and values
 // scaled by a power of two for each kv head so that the largest lies below 2^15, and so is every row of queries on its way into shared memory; the scores
 // and the results get the powers back in float.  With keys rounded to bfloat16 the results over 16,000 positions were 0.0044 of their norm off, with halves
-// 0.0017, which is the rounding of the results themselves.  The weights go up to 2^15 (2^7 above the reference maximum), so that none above 2^-31 of it is lost.
+// 0.0017, which is the rounding of the results themselves.  The weights go up to 2^15 (2^7 above the reference maximum), so that none above 2^-31 of it is lost
+// (those under 2^-21 of it lose digits: halves below 2^-14 have fewer).  A value that is no number was written as nought and marked: the rows that see it are told so at the end.
 constexpr float AT_HALF_UP = 7.0f;
 template <int HD, int AT_BK, bool SINK = false, bool EXT = false, bool DIFF = false, bool SHARED = false, bool HALF = false>
 __global__ void __launch_bounds__(SHARED ? AT_SHARED_THREADS : AT_THREADS)
@@ -282,7 +298,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
                     h[i] = *reinterpret_cast<const unsigned*>(&x);
                 }
                 v = make_uint4(h[0], h[1], h[2], h[3]);
-                if (c == 0) shift_of[r] = e + p.shifts[req * p.nkv + kvh].x;
+                if (c == 0) shift_of[r] = e + p.written[req * p.nkv + kvh].keys;
             }
             const int cb = c >> 3, cc = c & 7;
             const int rr = SHARED ? r & (AT_BM - 1) : r;
@@ -651,7 +667,13 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
             const float a0 = at_ex2(m - m_ref), a1 = at_ex2(other.x - m_ref);
             const float l_all = l * a0 + other.y * a1 + (SINK ? at_ex2(sink_l2 - m_ref) : 0.0f);
             const float inv = (real && l_all > 0.0f) ? 1.0f / l_all : 0.0f;
-            const float back = HALF ? exp2f((float)at_value_shift(p, req * p.nkv + kvh)) : 1.0f;
+            float back = 1.0f;
+            unsigned no_numbers = 0;
+            if constexpr (HALF) {
+                const PkWritten as = p.written[req * p.nkv + kvh];
+                back = exp2f((float)as.values);
+                if (as.marked && real) no_numbers = at_no_numbers<HD>(p, req, kvh, lo, pos);
+            }
             const float w0 = a0 * inv, w1 = a1 * inv;
             const bool has1 = !ALT || n_tiles > 1;       // with one tile the second group's accumulator was never written
             __nv_bfloat16* o = p.out + (size_t)(row0 + qi) * p.out_stride + (size_t)(kvh * group + g) * HD;
@@ -668,7 +690,8 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, typename At
 #pragma unroll
                         for (int k = 0; k < 8; ++k) {
                             v8[k] = t[q + k] * w0 + (has1 ? u[q + k] * w1 : 0.0f);
-                            if constexpr (HALF) v8[k] *= back;       // (at the end: at the ends of its range the product with a weight is no normal number)
+                            if constexpr (HALF)        // (at the end: at the ends of its range the product with a weight is no normal number)
+                                v8[k] = no_numbers >> (c0 / 64) & 1u ? NAN : v8[k] * back;
                         }
                         store8(o + c0 + q, v8);
                     }
@@ -972,16 +995,16 @@ extern "C" int bg_attention_tc_shared(const void* q, int q_stride, const void* k
     return hd == 128 ? at_launch_shared<128>(map, p, n_items, stream) : at_launch_shared<64>(map, p, n_items, stream);
 }
 
-// Rows over a cache of halves [num_pages, 2, nkv, page_size, hd] whose keys and values are scaled by 2^-shifts: see the kernel.  The queries and results are
+// Rows over a cache of halves [num_pages, 2, nkv, page_size, hd] whose keys and values are scaled as `written` says: see the kernel.  The queries and results are
 // bfloat16.  The cache is a step's own scratch, so its tensor map is made for this call.
 extern "C" int bg_attention_tc_half(const void* q, int q_stride, const void* kv_pool, int num_pages, int page_size, const int* block_table, int max_pages,
-                                    const int* positions, const int* qblk, int n_qblk, const void* shifts, void* out, int out_stride, int nh, int nkv, int hd,
-                                    int window, float scale, int max_position, int sink, const float* sink_weight, float softcap, unsigned* status,
+                                    const int* positions, const int* qblk, int n_qblk, const void* written, const void* marks, void* out, int out_stride, int nh,
+                                    int nkv, int hd, int window, float scale, int max_position, int sink, const float* sink_weight, float softcap, unsigned* status,
                                     cudaStream_t stream) {
     if (n_qblk <= 0) return BG_OK;
     if (nkv <= 0 || nh % nkv != 0 || (hd != 64 && hd != 128) || nh / nkv > 128 || !(scale > 0.0f) || softcap < 0.0f || (sink_weight && !sink)) return BG_ERR_UNSUPPORTED;
-    if (!pt_page_size_ok(page_size) || n_qblk > 65535 || !shifts) return BG_ERR_SHAPE;
-    if ((q_stride % 8) || (out_stride % 8) || ((uintptr_t)q % 16) || ((uintptr_t)kv_pool % 16) || ((uintptr_t)out % 16) || ((uintptr_t)shifts % 8)) return BG_ERR_ALIGN;
+    if (page_size != PK_WIDE || !pt_page_size_ok(page_size) || n_qblk > 65535 || !written || !marks) return BG_ERR_SHAPE;
+    if ((q_stride % 8) || (out_stride % 8) || ((uintptr_t)q % 16) || ((uintptr_t)kv_pool % 16) || ((uintptr_t)out % 16) || ((uintptr_t)written % 16) || ((uintptr_t)marks % 8)) return BG_ERR_ALIGN;
     AttnTcHalfParams p;
     memset(&p, 0, sizeof(p));
     p.q = (const __nv_bfloat16*)q; p.q_stride = q_stride; p.kv_pool = (const __nv_bfloat16*)kv_pool;
@@ -989,7 +1012,8 @@ extern "C" int bg_attention_tc_half(const void* q, int q_stride, const void* kv_
     for (int sh = 0; sh < 30; ++sh) if ((1 << sh) == page_size) p.page_shift = sh;
     p.block_table = block_table; p.max_pages = max_pages; p.positions = positions; p.qblk = qblk;
     p.out = (__nv_bfloat16*)out; p.out_stride = out_stride; p.nh = nh; p.nkv = nkv; p.group = nh / nkv;
-    p.window = window; p.scale_log2 = scale * AT_LOG2E; p.status = status; p.sink_weight = sink_weight; p.shifts = (const int2*)shifts;
+    p.window = window; p.scale_log2 = scale * AT_LOG2E; p.status = status; p.sink_weight = sink_weight; p.written = (const PkWritten*)written;
+    p.marks = (const unsigned long long*)marks;
     p.cap_log2 = softcap > 0.0f ? softcap * AT_LOG2E : 0.0f; p.cap_k = softcap > 0.0f ? 2.0f * AT_LOG2E * scale / softcap : 0.0f;
     CUtensorMap map;
     int rc = pt_pool_map_new(&map, kv_pool, num_pages, nkv, page_size, hd, CU_TENSOR_MAP_DATA_TYPE_FLOAT16);

@@ -215,9 +215,9 @@ _SIGNATURES = {
     "bg_packed_rows": [_c_void_p, _c_void_p],
     "bg_packed_bounds": [_c_void_p, _c_void_p],
     "bg_packed_wide_page": [],
-    "bg_packed_unpack": [_c_void_p, _c_ll, _c_int, _c_int, _c_void_p, _c_void_p, _c_int, _c_int, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_int,
-                         _c_int, _c_int, _c_int, _c_void_p, _c_void_p],
-    "bg_attention_tc_half": [_c_void_p, _c_int, _c_void_p, _c_int, _c_int, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_int,
+    "bg_packed_unpack": [_c_void_p, _c_ll, _c_int, _c_int, _c_void_p, _c_void_p, _c_int, _c_int, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
+                         _c_int, _c_int, _c_int, _c_int, _c_void_p, _c_void_p],
+    "bg_attention_tc_half": [_c_void_p, _c_int, _c_void_p, _c_int, _c_int, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_int,
                              _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_void_p, _c_float, _c_void_p, _c_void_p],
     "bg_packed_attention_columns": [_c_int, _c_int, _c_int, ctypes.POINTER(_c_int)],
     "bg_packed_attention_bytes": [],
@@ -1119,13 +1119,14 @@ def packed_attention(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Ten
             n_pages = max(1, -(-end // size))
             wide = torch.empty((plan.n_long * n_pages, 2, nkv, size, hd), dtype=torch.float16, device=q.device)
             table = torch.empty((plan.n_long, n_pages), dtype=torch.int32, device=q.device)
-            shifts = torch.empty((plan.n_long, nkv, 2), dtype=torch.int32, device=q.device)
+            written = torch.empty((plan.n_long, nkv, 4), dtype=torch.int32, device=q.device)
+            marks = torch.empty((plan.n_long * n_pages, nkv, hd // 64), dtype=torch.int64, device=q.device)
             _check(L.bg_packed_unpack(_p(pool), block, pool.shape[0], page_size, _p(positions), _p(block_table), block_table.shape[1],
-                                      block_table.shape[0], _p(plan.longs), plan.n_long, _p(wide), _p(table), _p(shifts), n_pages, window, nkv, hd,
-                                      _p(status), _stream()), "packed_unpack")
+                                      block_table.shape[0], _p(plan.longs), plan.n_long, _p(wide), _p(table), _p(written), _p(marks), n_pages, window,
+                                      nkv, hd, _p(status), _stream()), "packed_unpack")
             _check(L.bg_attention_tc_half(_p(q), q.stride(0), _p(wide), plan.n_long * n_pages, size, _p(table), n_pages, _p(positions), _p(plan.blocks),
-                                          plan.n_blocks, _p(shifts), _p(out), out.stride(0), nh, nkv, hd, window, float(scale), end - 1, 1 if sink else 0,
-                                          _p(sink_weight), float(softcap), _p(status), _stream()), "attention_tcgen05")
+                                          plan.n_blocks, _p(written), _p(marks), _p(out), out.stride(0), nh, nkv, hd, window, float(scale), end - 1,
+                                          1 if sink else 0, _p(sink_weight), float(softcap), _p(status), _stream()), "attention_tcgen05")
             count_launches(1)
         n, most = (T, 1) if plan is None else (plan.n_short, plan.most)
         if n:

@@ -328,7 +328,8 @@ struct PkUnpack {
     const int* longs;                  // [n][3]: request, first row, rows
     __half* out;                       // [n * pages, 2, nkv, PK_WIDE, HD]
     int* table;                        // [n, pages]: their block table
-    int2* shifts;                      // [n][nkv]: keys are written times 2^-x, values times 2^-y
+    PkWritten* written;                // [n][nkv]
+    unsigned long long* marks;         // [n * pages][nkv][groups]: the page's positions whose values are no numbers, where `written` says that there are some
     int max_pages, num_pages, page_size, n_req, nkv, pages, window;
     unsigned* status;
 };
@@ -350,7 +351,7 @@ constexpr int PK_CLUSTER = 8;
 template <int HD>
 __global__ void __launch_bounds__(PK_THREADS) packed_reach_kernel(const PkUnpack p) {
     constexpr int GROUPS = Packed<HD>::GROUPS, AT_ONCE = 8;
-    __shared__ float every[2][PK_CLUSTER];
+    __shared__ float every[3][PK_CLUSTER];
     __shared__ float scratch[32];
     pdl_launch();
     const int kvh = blockIdx.x, n = blockIdx.y, rank = blockIdx.z;
@@ -360,6 +361,7 @@ __global__ void __launch_bounds__(PK_THREADS) packed_reach_kernel(const PkUnpack
     const int req = p.longs[3 * n], row0 = p.longs[3 * n + 1], rows = p.longs[3 * n + 2];
     const int last = p.positions[row0 + rows - 1], lo = first_visible(p.positions[row0], p.window);
     float top[2] = {0.0f, 0.0f};
+    int marked = 0;
     const int stride = PK_CLUSTER * PK_THREADS;
     for (int pos0 = lo / PK_TILE * PK_TILE + rank * PK_THREADS + threadIdx.x; pos0 <= last; pos0 += AT_ONCE * stride) {
         int page[AT_ONCE];
@@ -377,6 +379,10 @@ __global__ void __launch_bounds__(PK_THREADS) packed_reach_kernel(const PkUnpack
 #pragma unroll
             for (int e = 0; e < 2 * GROUPS; ++e) {
                 const float lowest = pair_lowest(pair[e]);
+                if (!pair_finite(pair[e])) {           // (says nothing of how far the others reach)
+                    if (e >= GROUPS) marked |= 1 << (e - GROUPS);
+                    continue;
+                }
                 top[e / GROUPS] = fmaxf(top[e / GROUPS], fmaxf(fabsf(lowest), fabsf(fmaf(15.0f, pair_step(pair[e]), lowest))));
             }
         }
@@ -386,6 +392,8 @@ __global__ void __launch_bounds__(PK_THREADS) packed_reach_kernel(const PkUnpack
         const float all = block_max(top[v], scratch);
         if (threadIdx.x == 0) st_cluster(peer_addr(smem_u32(&every[v][rank]), 0), all);
     }
+    const int first = __syncthreads_or(marked & 1), second = __syncthreads_or(marked & 2);
+    if (threadIdx.x == 0) st_cluster(peer_addr(smem_u32(&every[2][rank]), 0), (float)((first ? 1 : 0) + (second ? 2 : 0)));
     cluster_sync_all();
     if (rank || threadIdx.x) return;
     int e[2];
@@ -395,7 +403,9 @@ __global__ void __launch_bounds__(PK_THREADS) packed_reach_kernel(const PkUnpack
         for (int i = 0; i < PK_CLUSTER; ++i) all = fmaxf(all, every[v][i]);
         e[v] = half_shift(all);
     }
-    p.shifts[(size_t)n * p.nkv + kvh] = make_int2(e[0], e[1]);
+    marked = 0;
+    for (int i = 0; i < PK_CLUSTER; ++i) marked |= (int)every[2][i];
+    p.written[(size_t)n * p.nkv + kvh] = {e[0], e[1], marked, 0};
 }
 
 // The positions that a request's rows read, written out in half precision as the prompt attention takes them, in pages of PK_WIDE whatever the packed ones hold:
@@ -403,7 +413,6 @@ __global__ void __launch_bounds__(PK_THREADS) packed_reach_kernel(const PkUnpack
 // together (a CTA for every 16 positions waited for its loads: 16 us for 16,000 positions of 4 kv heads); bound by the bytes written (heads of 128: 144 bytes
 // read and 512 written a position and kv head).  Positions behind the request's last are written as noughts: nobody reads them, and no number from nowhere
 // stands there.
-constexpr int PK_WIDE = 64;
 template <int HD>
 __global__ void __launch_bounds__(PK_THREADS) packed_unpack_kernel(const PkUnpack p) {
     constexpr int WORDS = HD / 8, EACH = 2 * PK_WIDE * WORDS / PK_THREADS;
@@ -414,8 +423,10 @@ __global__ void __launch_bounds__(PK_THREADS) packed_unpack_kernel(const PkUnpac
     const int req = p.longs[3 * n], row0 = p.longs[3 * n + 1], rows = p.longs[3 * n + 2];
     const int last = p.positions[row0 + rows - 1], lo = first_visible(p.positions[row0], p.window);
     if (wide > last / PK_WIDE || wide < lo / PK_WIDE) return;
-    const int2 shift = p.shifts[(size_t)n * p.nkv + kvh];
+    const PkWritten as = p.written[(size_t)n * p.nkv + kvh];
     __shared__ const unsigned char* tiles[PK_WIDE / PK_TILE];
+    __shared__ unsigned marks[Packed<HD>::GROUPS][PK_WIDE / 32];
+    if (threadIdx.x < Packed<HD>::GROUPS * PK_WIDE / 32) marks[threadIdx.x / (PK_WIDE / 32)][threadIdx.x % (PK_WIDE / 32)] = 0;
     if (threadIdx.x < PK_WIDE / PK_TILE) {
         const int pos0 = wide * PK_WIDE + threadIdx.x * PK_TILE, page = unpack_page(p, req, pos0, lo, last, true);
         tiles[threadIdx.x] = page < 0 ? nullptr
@@ -439,16 +450,22 @@ __global__ void __launch_bounds__(PK_THREADS) packed_unpack_kernel(const PkUnpac
         const int i = j * PK_THREADS + threadIdx.x, value = i / (PK_WIDE * WORDS), slot = i / WORDS % PK_WIDE, f = i % WORDS * 8;
         float v[8] = {};
         if (have >> j & 1) {
-            if (value) packed_values<false>(word[j], pair[j], v);
-            else packed_values<true>(word[j], pair[j], v);
+            if (!value) packed_values<true>(word[j], pair[j], v);
+            else if (!as.marked || pair_finite(pair[j])) packed_values<false>(word[j], pair[j], v);
+            else atomicOr(&marks[f / PK_GROUP][slot / 32], 1u << (slot % 32));
         }
-        const float down = __uint_as_float((unsigned)(127 - (value ? shift.y : shift.x)) << 23);
+        const float down = __uint_as_float((unsigned)(127 - (value ? as.values : as.keys)) << 23);
         uint4 r;
         __half2* h = reinterpret_cast<__half2*>(&r);
 #pragma unroll
         for (int e = 0; e < 4; ++e) h[e] = __floats2half2_rn(v[2 * e] * down, v[2 * e + 1] * down);
         *reinterpret_cast<uint4*>(p.out + ((((size_t)n * p.pages + wide) * 2 + value) * p.nkv + kvh) * PK_WIDE * HD + (size_t)slot * HD + f) = r;
     }
+    if (!as.marked) return;
+    __syncthreads();
+    if (threadIdx.x < Packed<HD>::GROUPS)
+        p.marks[(((size_t)n * p.pages + wide) * p.nkv + kvh) * Packed<HD>::GROUPS + threadIdx.x] =
+            (unsigned long long)marks[threadIdx.x][1] << 32 | marks[threadIdx.x][0];
 }
 
 static int packed_shape(int hd, int page_size, int nkv, int num_pages, long long block_bytes, bool bounds) {
@@ -519,14 +536,14 @@ extern "C" int bg_packed_bounds(const void* call, cudaStream_t stream) {
 extern "C" int bg_packed_wide_page() { return PK_WIDE; }
 
 extern "C" int bg_packed_unpack(const unsigned char* pool, long long block_bytes, int num_pages, int page_size, const int* positions, const int* block_table,
-                                int max_pages, int n_req, const int* longs, int n, void* out, int* table, void* shifts, int pages, int window, int nkv, int hd,
-                                unsigned* status, cudaStream_t stream) {
+                                int max_pages, int n_req, const int* longs, int n, void* out, int* table, void* written, void* marks, int pages, int window,
+                                int nkv, int hd, unsigned* status, cudaStream_t stream) {
     if (int e = packed_shape(hd, page_size, nkv, num_pages, block_bytes, false)) return e;
     if (n <= 0 || pages <= 0) return BG_OK;
     if (n > 65535 || (long long)n * pages > 0x7fffffffLL || pages > 0x7fffffff / PK_WIDE) return BG_ERR_SHAPE;
-    if ((uintptr_t)pool % 16 || (uintptr_t)out % 16 || (uintptr_t)shifts % 8) return BG_ERR_ALIGN;
-    const PkUnpack p = {pool, block_bytes, positions, block_table, longs, (__half*)out, table, (int2*)shifts, max_pages, num_pages, page_size, n_req, nkv, pages,
-                        window, status};
+    if ((uintptr_t)pool % 16 || (uintptr_t)out % 16 || (uintptr_t)written % 16 || (uintptr_t)marks % 8) return BG_ERR_ALIGN;
+    const PkUnpack p = {pool, block_bytes, positions, block_table, longs, (__half*)out, table, (PkWritten*)written, (unsigned long long*)marks, max_pages, num_pages,
+                        page_size, n_req, nkv, pages, window, status};
     const dim3 heads(nkv, n, PK_CLUSTER), whole(pages, nkv, n);
     cudaError_t e = hd == 64 ? launch_cluster(packed_reach_kernel<64>, heads, dim3(PK_THREADS), 0, stream, PK_CLUSTER, p)
                              : launch_cluster(packed_reach_kernel<128>, heads, dim3(PK_THREADS), 0, stream, PK_CLUSTER, p);

@@ -17,6 +17,12 @@
 namespace bg {
 
 constexpr int PK_TILE = 16, PK_GROUP = 64;
+constexpr int PK_WIDE = 64;                // positions of a page written out in half precision
+
+// What is written out with the pages of a kv head of a request: its keys are written times 2^-keys and its values times 2^-values; bit g of `marked`: some of its
+// values' g-th groups are no numbers. Those are written as noughts and marked, a bit a position of a page: a product would carry them to the rows
+// that do not see them, whose weight for them is nought.
+struct __align__(16) PkWritten { int keys, values, marked, pad; };
 
 template <int HD>
 struct Packed {
@@ -40,6 +46,7 @@ __host__ __device__ inline long long packed_tile_bytes(int hd) { return hd == 64
 
 __device__ __forceinline__ float pair_step(unsigned pair) { return __uint_as_float(pair << 16); }
 __device__ __forceinline__ float pair_lowest(unsigned pair) { return __uint_as_float(pair & 0xffff0000u); }
+__device__ __forceinline__ bool pair_finite(unsigned pair) { return fabsf(fmaf(15.0f, pair_step(pair), pair_lowest(pair))) < INFINITY; }
 
 // The power of two (times 2^14) of the largest of some numbers: less that, they lie below 2^15, where half precision holds them whatever their scale is. 2^-this
 // is a normal number too.

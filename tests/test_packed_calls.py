@@ -104,3 +104,23 @@ def test_numbers_next_to_the_ends_of_their_range_in_a_portion(key, value, query,
         pairs[..., 1, :, :] *= value
     got, want = portion(100, 0, 4, 2, 128, 32, monkeypatch, change)
     near(got.double() / value, want / value, BF16)
+
+
+@GPU
+@pytest.mark.parametrize("options", [dict(), dict(window=40), dict(softcap=9.0, sink=True)], ids=["plain", "window", "squashed"])
+@pytest.mark.parametrize("what,places_", [("value", [50]), ("value", [0, 95, 129]), ("key", [50]), ("both", [20, 64, 127])])
+@pytest.mark.parametrize("nh,nkv,hd,page,n,start", [(4, 2, 128, 32, 130, 20), (6, 2, 64, 16, 150, 0)])
+@pytest.mark.parametrize("many", [0, 1 << 30], ids=["written out", "packed"])
+def test_a_group_that_is_no_number_in_a_portion(nh, nkv, hd, page, n, start, what, places_, options, many, monkeypatch):
+    """It shows in the rows that see it, in its own features, and in no other: not in those in front of it, nor in those whose window is past it."""
+    table, _ = make_table([start + n], page)
+    def change(q, pairs):
+        for i, pos in enumerate(places_):
+            at = int(table[0, pos // page]), 1, pos % page // 16, pos % 16
+            if what != "value":
+                pairs[at + (0,)][-1] = math.nan
+            if what != "key":
+                pairs[at + (1,)][-1 if i % 2 else 0] = math.nan
+    got, want = portion(n, start, nh, nkv, hd, page, monkeypatch, change, many=many, **options)
+    near(got, want, BF16)
+    assert bool(torch.isnan(got).any()) and (places_[0] <= start or not bool(torch.isnan(got[0]).any()))
