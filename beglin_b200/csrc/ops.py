@@ -215,8 +215,9 @@ _SIGNATURES = {
     "bg_packed_rows": [_c_void_p, _c_void_p],
     "bg_packed_bounds": [_c_void_p, _c_void_p],
     "bg_packed_wide_page": [],
-    "bg_packed_unpack": [_c_void_p, _c_ll, _c_int, _c_int, _c_void_p, _c_void_p, _c_int, _c_int, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
-                         _c_int, _c_int, _c_int, _c_int, _c_void_p, _c_void_p],
+    "bg_packed_room": [_c_int, _c_int, _c_int],
+    "bg_packed_unpack": [_c_void_p, _c_ll, _c_int, _c_int, _c_void_p, _c_void_p, _c_int, _c_int, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
+                         _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_void_p, _c_void_p],
     "bg_attention_tc_half": [_c_void_p, _c_int, _c_void_p, _c_int, _c_int, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_int,
                              _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_void_p, _c_float, _c_void_p, _c_void_p],
     "bg_packed_attention_columns": [_c_int, _c_int, _c_int, ctypes.POINTER(_c_int)],
@@ -1025,12 +1026,26 @@ class PackedPlan:
                 short += [(i, r0 + f, min(self.rows, n - f)) for f in range(0, n, self.rows)]
         self.most = max((s[2] for s in short), default=1)
         self.n_short, self.n_blocks, self.n_long = len(short), len(blocks), len(longs)
-        self.long_end = None if starts is None else max((starts[i] + n for i, _, n in longs), default=0)
-        flat = torch.tensor([v for rows in (short, blocks, longs) for r in rows for v in r] or [0], dtype=torch.int32)
+        # (rows, a bound of their positions or 0) of the requests whose pages are written out
+        self.long_rows = [(n, 0 if starts is None else int(starts[i]) + n) for i, _, n in longs]
+        flat = torch.tensor([v for rows in (short, blocks, longs) for r in rows for v in r] + [end for _, end in self.long_rows] or [0], dtype=torch.int32)
         device = torch.device(device)
         flat = flat.pin_memory().to(device, non_blocking=True) if device.type == "cuda" else flat
         a, b = 3 * len(short), 3 * (len(short) + len(blocks))
-        self.short, self.blocks, self.longs = flat[:a], flat[a:b], flat[b:b + 3 * len(longs)]
+        c = b + 3 * len(longs)
+        self.short, self.blocks, self.longs, self.ends = flat[:a], flat[a:b], flat[b:c], flat[c:c + len(longs)]
+        self._rooms = {}
+
+    def rooms(self, max_position: int, window: int = 0) -> Tuple[Tuple[int, ...], int]:
+        """(Pages of 64 positions that are written out for each such request, a bound of their positions): for what its rows read, its window in front of them or all.
+        A page takes 4 * 64 * kv heads * head size bytes while the call lasts."""
+        hit = self._rooms.get((max_position, window))
+        if hit is None:
+            most = max(max_position + 1, 1)
+            ends = [min(end or most, most) for _, end in self.long_rows]
+            hit = self._rooms[max_position, window] = (tuple(lib().bg_packed_room(n, end, window) for (n, _), end in zip(self.long_rows, ends)),
+                                                       max(ends + [1]))
+        return hit
 
 
 def packed_plan(lens, nh: int, nkv: int, hd: int, dtype: torch.dtype, page_size: int, device, row_start=None, starts=None) -> PackedPlan:
@@ -1045,7 +1060,7 @@ def packed_plan(lens, nh: int, nkv: int, hd: int, dtype: torch.dtype, page_size:
     packed_page_bytes(hd, page_size)
     if row_start is None:
         row_start = [sum(lens[:i]) for i in range(len(lens))] if len(lens) < 64 else np.concatenate([[0], np.cumsum(lens)[:-1]]).tolist()
-    if len(row_start) != len(lens) or (starts is not None and len(starts) != len(lens)):
+    if len(row_start) != len(lens) or (starts is not None and (len(starts) != len(lens) or min(starts, default=0) < 0)):
         raise KernelError("packed_plan: a first row and a first position for every request")
     at = 0
     for first, n in sorted((r, n) for r, n in zip(row_start, lens) if n):
@@ -1114,18 +1129,20 @@ def packed_attention(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Ten
     L, f32 = lib(), q.dtype == torch.float32
     with phase("attn"):
         if plan is not None and plan.n_long:
-            end = max_position + 1 if plan.long_end is None else min(plan.long_end, max_position + 1)
-            size = L.bg_packed_wide_page()
-            n_pages = max(1, -(-end // size))
-            wide = torch.empty((plan.n_long * n_pages, 2, nkv, size, hd), dtype=torch.float16, device=q.device)
-            table = torch.empty((plan.n_long, n_pages), dtype=torch.int32, device=q.device)
-            written = torch.empty((plan.n_long, nkv, 4), dtype=torch.int32, device=q.device)
-            marks = torch.empty((plan.n_long * n_pages, nkv, hd // 64), dtype=torch.int64, device=q.device)
+            rooms, end = plan.rooms(max_position, window)
+            size, room = L.bg_packed_wide_page(), sum(rooms)
+            n_pages = -(-end // size)
+            wide = torch.empty((room, 2, nkv, size, hd), dtype=torch.float16, device=q.device)
+            # how each request's kv heads are written (4 numbers), which values are no numbers (2 for each group of a page), and the block table
+            n_written, n_marks = 4 * plan.n_long * nkv, 2 * room * nkv * (hd // 64)
+            written = torch.empty(n_written + n_marks + plan.n_long * n_pages, dtype=torch.int32, device=q.device)
+            marks = written.data_ptr() + 4 * n_written
+            table = marks + 4 * n_marks
             _check(L.bg_packed_unpack(_p(pool), block, pool.shape[0], page_size, _p(positions), _p(block_table), block_table.shape[1],
-                                      block_table.shape[0], _p(plan.longs), plan.n_long, _p(wide), _p(table), _p(written), _p(marks), n_pages, window,
-                                      nkv, hd, _p(status), _stream()), "packed_unpack")
-            _check(L.bg_attention_tc_half(_p(q), q.stride(0), _p(wide), plan.n_long * n_pages, size, _p(table), n_pages, _p(positions), _p(plan.blocks),
-                                          plan.n_blocks, _p(written), _p(marks), _p(out), out.stride(0), nh, nkv, hd, window, float(scale), end - 1,
+                                      block_table.shape[0], _p(plan.longs), _p(plan.ends), plan.n_long, _p(wide), table, _p(written), marks,
+                                      max(rooms), n_pages, room, max(max_position + 1, 1), window, nkv, hd, _p(status), _stream()), "packed_unpack")
+            _check(L.bg_attention_tc_half(_p(q), q.stride(0), _p(wide), room, size, table, n_pages, _p(positions), _p(plan.blocks),
+                                          plan.n_blocks, _p(written), marks, _p(out), out.stride(0), nh, nkv, hd, window, float(scale), end - 1,
                                           1 if sink else 0, _p(sink_weight), float(softcap), _p(status), _stream()), "attention_tcgen05")
             count_launches(1)
         n, most = (T, 1) if plan is None else (plan.n_short, plan.most)

@@ -326,13 +326,18 @@ struct PkUnpack {
     const unsigned char* pool; long long block_bytes;
     const int* positions; const int* block_table;
     const int* longs;                  // [n][3]: request, first row, rows
-    __half* out;                       // [n * pages, 2, nkv, PK_WIDE, HD]
-    int* table;                        // [n, pages]: their block table
+    const int* ends;                   // [n]: a bound of their positions, or 0: `end` is
+    __half* out;                       // [room, 2, nkv, PK_WIDE, HD]
+    int* table;                        // [n, table_pages]: their block table
     PkWritten* written;                // [n][nkv]
-    unsigned long long* marks;         // [n * pages][nkv][groups]: the page's positions whose values are no numbers, where `written` says that there are some
-    int max_pages, num_pages, page_size, n_req, nkv, pages, window;
+    unsigned long long* marks;         // [room][nkv][groups]: the page's positions whose values are no numbers, where `written` says that there are some
+    int max_pages, num_pages, page_size, n_req, nkv, table_pages, room, end, window;
     unsigned* status;
 };
+__device__ __forceinline__ int unpack_room(const PkUnpack& p, int n) {
+    const int end = p.ends[n];
+    return packed_room(p.longs[3 * n + 2], end > 0 ? min(end, p.end) : p.end, p.window);
+}
 
 // The page of a tile of 16 positions from `pos0` on that the n-th request's rows read, or -1 (and the status says where a page is not).
 __device__ __forceinline__ int unpack_page(const PkUnpack& p, int req, int pos0, int lo, int last, bool say) {
@@ -395,7 +400,11 @@ __global__ void __launch_bounds__(PK_THREADS) packed_reach_kernel(const PkUnpack
     const int first = __syncthreads_or(marked & 1), second = __syncthreads_or(marked & 2);
     if (threadIdx.x == 0) st_cluster(peer_addr(smem_u32(&every[2][rank]), 0), (float)((first ? 1 : 0) + (second ? 2 : 0)));
     cluster_sync_all();
-    if (rank || threadIdx.x) return;
+    if (rank || threadIdx.x >= 32) return;
+    int ahead = 0;                                     // pages of the requests in front of this one
+    for (int i = threadIdx.x; i < n; i += 32) ahead += unpack_room(p, i);
+    ahead = __reduce_add_sync(0xffffffffu, ahead);
+    if (threadIdx.x) return;
     int e[2];
 #pragma unroll
     for (int v = 0; v < 2; ++v) {
@@ -405,11 +414,11 @@ __global__ void __launch_bounds__(PK_THREADS) packed_reach_kernel(const PkUnpack
     }
     marked = 0;
     for (int i = 0; i < PK_CLUSTER; ++i) marked |= (int)every[2][i];
-    p.written[(size_t)n * p.nkv + kvh] = {e[0], e[1], marked, 0};
+    p.written[(size_t)n * p.nkv + kvh] = {e[0], e[1], marked, ahead - lo / PK_WIDE};
 }
 
 // The positions that a request's rows read, written out in half precision as the prompt attention takes them, in pages of PK_WIDE whatever the packed ones hold:
-// page i of the n-th request at n * pages + i.  A CTA takes one of those pages of one kv head, a thread a word of 8 codes at a time, all its loads on their way
+// page i of a request where `written` says.  A CTA takes one of those pages of one kv head, a thread a word of 8 codes at a time, all its loads on their way
 // together (a CTA for every 16 positions waited for its loads: 16 us for 16,000 positions of 4 kv heads); bound by the bytes written (heads of 128: 144 bytes
 // read and 512 written a position and kv head).  Positions behind the request's last are written as noughts: nobody reads them, and no number from nowhere
 // stands there.
@@ -417,13 +426,19 @@ template <int HD>
 __global__ void __launch_bounds__(PK_THREADS) packed_unpack_kernel(const PkUnpack p) {
     constexpr int WORDS = HD / 8, EACH = 2 * PK_WIDE * WORDS / PK_THREADS;
     pdl_launch();
-    const int n = blockIdx.z, kvh = blockIdx.y, wide = blockIdx.x;
+    const int n = blockIdx.z, kvh = blockIdx.y;
     pdl_wait();
-    if (kvh == 0 && threadIdx.x == 0) p.table[(size_t)n * p.pages + wide] = n * p.pages + wide;
     const int req = p.longs[3 * n], row0 = p.longs[3 * n + 1], rows = p.longs[3 * n + 2];
-    const int last = p.positions[row0 + rows - 1], lo = first_visible(p.positions[row0], p.window);
-    if (wide > last / PK_WIDE || wide < lo / PK_WIDE) return;
+    const int last = p.positions[row0 + rows - 1], lo = first_visible(p.positions[row0], p.window), wide = lo / PK_WIDE + blockIdx.x;
     const PkWritten as = p.written[(size_t)n * p.nkv + kvh];
+    const int room = unpack_room(p, n), place = as.base + wide;
+    if (blockIdx.x == 0 && kvh == 0 && (last / PK_WIDE - lo / PK_WIDE >= room || last / PK_WIDE >= p.table_pages)) {
+        // (positions beyond what the plan or the call's bound says: what there is no room for is not there)
+        if (p.status && threadIdx.x == 0) atomicOr(p.status, BG_STATUS_BAD_PAGE);
+        for (int i = lo / PK_WIDE + room + threadIdx.x; i < p.table_pages; i += PK_THREADS) p.table[(size_t)n * p.table_pages + i] = -1;
+    }
+    if (wide > last / PK_WIDE || wide >= p.table_pages || (int)blockIdx.x >= room || place < 0 || place >= p.room) return;
+    if (kvh == 0 && threadIdx.x == 0) p.table[(size_t)n * p.table_pages + wide] = place;
     __shared__ const unsigned char* tiles[PK_WIDE / PK_TILE];
     __shared__ unsigned marks[Packed<HD>::GROUPS][PK_WIDE / 32];
     if (threadIdx.x < Packed<HD>::GROUPS * PK_WIDE / 32) marks[threadIdx.x / (PK_WIDE / 32)][threadIdx.x % (PK_WIDE / 32)] = 0;
@@ -459,13 +474,12 @@ __global__ void __launch_bounds__(PK_THREADS) packed_unpack_kernel(const PkUnpac
         __half2* h = reinterpret_cast<__half2*>(&r);
 #pragma unroll
         for (int e = 0; e < 4; ++e) h[e] = __floats2half2_rn(v[2 * e] * down, v[2 * e + 1] * down);
-        *reinterpret_cast<uint4*>(p.out + ((((size_t)n * p.pages + wide) * 2 + value) * p.nkv + kvh) * PK_WIDE * HD + (size_t)slot * HD + f) = r;
+        *reinterpret_cast<uint4*>(p.out + (((size_t)place * 2 + value) * p.nkv + kvh) * PK_WIDE * HD + (size_t)slot * HD + f) = r;
     }
     if (!as.marked) return;
     __syncthreads();
     if (threadIdx.x < Packed<HD>::GROUPS)
-        p.marks[(((size_t)n * p.pages + wide) * p.nkv + kvh) * Packed<HD>::GROUPS + threadIdx.x] =
-            (unsigned long long)marks[threadIdx.x][1] << 32 | marks[threadIdx.x][0];
+        p.marks[((size_t)place * p.nkv + kvh) * Packed<HD>::GROUPS + threadIdx.x] = (unsigned long long)marks[threadIdx.x][1] << 32 | marks[threadIdx.x][0];
 }
 
 static int packed_shape(int hd, int page_size, int nkv, int num_pages, long long block_bytes, bool bounds) {
@@ -535,16 +549,22 @@ extern "C" int bg_packed_bounds(const void* call, cudaStream_t stream) {
 // Positions of a page that bg_packed_unpack writes.
 extern "C" int bg_packed_wide_page() { return PK_WIDE; }
 
+// Pages of them that `rows` rows need whose positions lie below `end`.
+extern "C" int bg_packed_room(int rows, int end, int window) { return packed_room(rows, end, window); }
+
+// Pages in half precision for the prompt attention.  out [room, ..] holds the requests' pages one behind the other, bg_packed_room() of each (most_pages the most
+// of one); table [n][table_pages] their numbers.  `ends` or `end` bound the positions; a request that goes on beyond them has the status say so.
+
 extern "C" int bg_packed_unpack(const unsigned char* pool, long long block_bytes, int num_pages, int page_size, const int* positions, const int* block_table,
-                                int max_pages, int n_req, const int* longs, int n, void* out, int* table, void* written, void* marks, int pages, int window,
-                                int nkv, int hd, unsigned* status, cudaStream_t stream) {
+                                int max_pages, int n_req, const int* longs, const int* ends, int n, void* out, int* table, void* written, void* marks,
+                                int most_pages, int table_pages, int room, int end, int window, int nkv, int hd, unsigned* status, cudaStream_t stream) {
     if (int e = packed_shape(hd, page_size, nkv, num_pages, block_bytes, false)) return e;
-    if (n <= 0 || pages <= 0) return BG_OK;
-    if (n > 65535 || (long long)n * pages > 0x7fffffffLL || pages > 0x7fffffff / PK_WIDE) return BG_ERR_SHAPE;
+    if (n <= 0) return BG_OK;
+    if (n > 65535 || most_pages <= 0 || table_pages < most_pages || room < most_pages || table_pages > 0x7fffffff / PK_WIDE || end <= 0) return BG_ERR_SHAPE;
     if ((uintptr_t)pool % 16 || (uintptr_t)out % 16 || (uintptr_t)written % 16 || (uintptr_t)marks % 8) return BG_ERR_ALIGN;
-    const PkUnpack p = {pool, block_bytes, positions, block_table, longs, (__half*)out, table, (PkWritten*)written, (unsigned long long*)marks, max_pages, num_pages,
-                        page_size, n_req, nkv, pages, window, status};
-    const dim3 heads(nkv, n, PK_CLUSTER), whole(pages, nkv, n);
+    const PkUnpack p = {pool, block_bytes, positions, block_table, longs, ends, (__half*)out, table, (PkWritten*)written, (unsigned long long*)marks, max_pages,
+                        num_pages, page_size, n_req, nkv, table_pages, room, end, window, status};
+    const dim3 heads(nkv, n, PK_CLUSTER), whole(most_pages, nkv, n);
     cudaError_t e = hd == 64 ? launch_cluster(packed_reach_kernel<64>, heads, dim3(PK_THREADS), 0, stream, PK_CLUSTER, p)
                              : launch_cluster(packed_reach_kernel<128>, heads, dim3(PK_THREADS), 0, stream, PK_CLUSTER, p);
     if (e != cudaSuccess) return (int)e;

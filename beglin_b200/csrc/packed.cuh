@@ -22,7 +22,16 @@ constexpr int PK_WIDE = 64;                // positions of a page written out in
 // What is written out with the pages of a kv head of a request: its keys are written times 2^-keys and its values times 2^-values; bit g of `marked`: some of its
 // values' g-th groups are no numbers. Those are written as noughts and marked, a bit a position of a page: a product would carry them to the rows
 // that do not see them, whose weight for them is nought.
-struct __align__(16) PkWritten { int keys, values, marked, pad; };
+// `base`: its page i (of PK_WIDE positions) is page base + i of what is written out.
+struct __align__(16) PkWritten { int keys, values, marked, base; };
+
+// Pages that `rows` rows need whose last position lies below `end`: the requests' lie one behind the other, each with room for what it reads, not for the longest.
+__host__ __device__ inline int packed_room(int rows, int end, int window) {
+    const int whole = end > 0 ? (end - 1) / PK_WIDE + 1 : 1;
+    if (window <= 0) return whole;
+    const long long span = ((long long)rows + window - 2 + PK_WIDE - 1) / PK_WIDE + 1;          // (rows + window - 1 positions, wherever they begin in a page)
+    return span < whole ? (int)span : whole;
+}
 
 template <int HD>
 struct Packed {

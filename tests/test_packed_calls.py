@@ -124,3 +124,66 @@ def test_a_group_that_is_no_number_in_a_portion(nh, nkv, hd, page, n, start, wha
     got, want = portion(n, start, nh, nkv, hd, page, monkeypatch, change, many=many, **options)
     near(got, want, BF16)
     assert bool(torch.isnan(got).any()) and (places_[0] <= start or not bool(torch.isnan(got[0]).any()))
+
+
+# ------------------------------------------------------------------------------------------------ the room of pages written out
+def test_every_portion_has_room_for_what_it_reads():
+    starts, lens = [131072 - 300] + [0] * 7, [300] * 8
+    plan = ops.packed_plan(lens, 32, 4, 128, BF16, 64, "cpu", starts=starts)
+    assert plan.n_long == 8 and plan.rooms(131071)[0] == (2048,) + (5,) * 7 and plan.rooms(131071)[1] == 131072
+    assert plan.rooms(131071, 1000)[0] == (22,) + (5,) * 7                     # 1,299 positions that begin anywhere in a page
+    assert plan.rooms(131071, 1)[0] == (6,) + (5,) * 7 and plan.rooms(131071, 1 << 30)[0] == (2048,) + (5,) * 7
+    assert plan.rooms(999)[0] == (16,) + (5,) * 7                              # (the call's bound holds too)
+    unknown = ops.packed_plan(lens[:2], 32, 4, 128, BF16, 64, "cpu")
+    assert unknown.rooms(8191)[0] == (128, 128) and unknown.rooms(8191, 100)[0] == (8, 8)
+    for start in range(64):                                                    # as many as are touched at the worst
+        assert (start + 299 + 1000 - 1) // 64 + 1 <= 22
+    with pytest.raises(ops.KernelError, match="first position"):
+        ops.packed_plan([300], 8, 4, 128, BF16, 64, "cpu", starts=[-1])
+
+
+@GPU
+@pytest.mark.parametrize("window", [0, 70])
+def test_long_and_short_portions_lie_one_behind_the_other(window, monkeypatch):
+    monkeypatch.setattr(ops, "PACKED_LONG_STREAMS", 0)
+    nh, nkv, hd, page, lens, starts = 4, 2, 64, 16, [70, 90, 1, 3, 65], [5, 4000, 6, 0, 64]
+    lengths = [n + s for n, s in zip(lens, starts)]
+    table, pages = make_table(lengths, page)
+    pool = make_pool(pages, nkv, hd, page, seed=8)
+    poison(pool, table, lengths, hd, page)
+    rows = [(i, p) for i, (n, s) in enumerate(zip(lens, starts)) for p in range(s, s + n)]
+    q = torch.randn((len(rows), nh * hd), generator=torch.Generator().manual_seed(2)).to(BF16)
+    want = plain_attention(q.view(-1, nh, hd), pool, table, hd, page, rows, 0.125, window)
+    positions, dev = torch.tensor([p for _, p in rows], dtype=torch.int32).cuda(), (q.cuda(), pool.cuda(), table.cuda())
+    out, status = torch.empty_like(dev[0]), ops.new_status("cuda")
+    peaks, rooms = [], []
+    for given in (starts, None):
+        plan = ops.packed_plan(lens, nh, nkv, hd, BF16, page, "cuda", starts=given)
+        rooms.append(sum(plan.rooms(max(lengths) - 1, window)[0]))
+        out.fill_(7.0)
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        ops.packed_attention(*dev, positions, nh, nkv, hd, page, max(lengths) - 1, 0.125, out, status, plan=plan, window=window)
+        peaks.append(torch.cuda.max_memory_allocated() - before)
+        ops.raise_on_status(status)
+        near(out.view(-1, nh, hd), want, BF16)
+    assert rooms == ([2 + 64 + 3, 3 * 64] if not window else [2 + 4 + 3, 3 * 4])          # (the requests of 70, 90 and 65 rows)
+    assert peaks[1] - peaks[0] >= (rooms[1] - rooms[0]) * 4 * 64 * nkv * hd * 0.9
+
+
+@GPU
+@pytest.mark.parametrize("window", [0, 70])
+@pytest.mark.parametrize("starts,most", [([0, 0], 699), ([600, 0], 699), (None, 99), ([600, 600], 99)], ids=str)
+def test_rows_beyond_their_bounds_are_recorded(starts, most, window, monkeypatch):
+    """First positions or a bound below the rows' own: what has no room is not written, and the status says so."""
+    monkeypatch.setattr(ops, "PACKED_LONG_STREAMS", 0)
+    nh, nkv, hd, page = 4, 2, 64, 16
+    table, pages = make_table([700, 700], page)
+    q = torch.randn((200, nh * hd), generator=torch.Generator().manual_seed(2)).to(BF16).cuda()
+    positions = torch.arange(600, 700, dtype=torch.int32).repeat(2).cuda()
+    status = ops.new_status("cuda")
+    ops.packed_attention(q, make_pool(pages, nkv, hd, page).cuda(), table.cuda(), positions, nh, nkv, hd, page, most, 0.125, torch.empty_like(q), status, window=window,
+                         plan=ops.packed_plan([100, 100], nh, nkv, hd, BF16, page, "cuda", starts=starts))
+    with pytest.raises(ops.KernelError, match="block-table"):
+        ops.raise_on_status(status)
