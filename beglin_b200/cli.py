@@ -21,7 +21,7 @@ the model folder, :20121), QWEN_PROF (1: in `bench` and `greedy`, device time pe
 printed with the share of the total that the classes add up to, :1224-1235 and :20463-20486; the steps then
 run kernel by kernel, not as replayed graphs).
 QWEN_KV_INT4 (1: keys and values in 4 bits).
-Added: QWEN_SPARSE_PAGES (n: single tokens read at most n pages of such a cache for each kv head), QWEN_DTYPE (bf16 | fp32, default bf16), QWEN_TEMPERATURE and QWEN_SEED (sampling),
+Added: QWEN_SPARSE_PAGES (n: tokens that are decoded read at most n pages of such a cache for each kv head), QWEN_DTYPE (bf16 | fp32, default bf16), QWEN_TEMPERATURE and QWEN_SEED (sampling),
 QWEN_PAGE_SIZE (default 64), QWEN_NUM_PAGES, QWEN_RANDOM (a seed: write random weights for
 <QWEN_BASE>/config.json first, if the folder has no model.safetensors), QWEN_DUMP_DIR.
 """

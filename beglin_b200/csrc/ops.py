@@ -876,7 +876,7 @@ PACKED_TILE = 16           # positions of a tile: pages hold whole tiles
 # The calls' fields in the order of the library's structures: one packed record costs the host a tenth of what as many arguments do, which is what a call
 # of a decoding step is bound by.
 _PACKED_APPEND, _PACKED_READ = struct.Struct("<12q14i"), struct.Struct("<7q8i")
-_PACKED_ATTENTION, _PACKED_SELECT = struct.Struct("<14q16i2f"), struct.Struct("<8q12i")
+_PACKED_ATTENTION, _PACKED_SELECT = struct.Struct("<14q16i2f"), struct.Struct("<9q14i")
 
 
 def _at(t: Optional[torch.Tensor]) -> int:
@@ -1009,7 +1009,7 @@ def _packed_columns(group: int, f32: bool, rows: int) -> Tuple[int, int]:
 class PackedPlan:
     """How attention over pages in 4 bits goes over a step's rows: made by `packed_plan`."""
 
-    def __init__(self, lens, row_start, nh, nkv, hd, dtype, page_size, device, starts):
+    def __init__(self, lens, row_start, nh, nkv, hd, dtype, page_size, device, starts, chosen):
         self.sizes, self.n_rows = (nh, nkv, hd, dtype, page_size), sum(lens)
         group, f32 = nh // nkv, dtype == torch.float32
         self.rows = max(1, (8 if f32 else 16) // group)        # rows of a block that the packed kernel takes
@@ -1017,23 +1017,25 @@ class PackedPlan:
         wide = not f32 and lib().bg_attention_tc_plan(group, hd, lib().bg_packed_wide_page(), ctypes.byref(bq)) == 0
         self.bq = bq = bq.value
         streams = nkv * -(-group // (8 if f32 else 16))        # of a block of rows
-        short, blocks, longs = [], [], []
+        short, picks, blocks, longs = [], [], [], []
         for i, (r0, n) in enumerate(zip(row_start, lens)):
-            if wide and n > self.rows and -(-n // self.rows) * streams > PACKED_LONG_STREAMS:
+            if chosen[i]:
+                picks.append((i, r0, 1))
+            elif wide and n > self.rows and -(-n // self.rows) * streams > PACKED_LONG_STREAMS:
                 blocks += [(len(longs), r0 + f, min(bq, n - f)) for f in range(0, n, bq)]
                 longs.append((i, r0, n))
             else:
                 short += [(i, r0 + f, min(self.rows, n - f)) for f in range(0, n, self.rows)]
         self.most = max((s[2] for s in short), default=1)
-        self.n_short, self.n_blocks, self.n_long = len(short), len(blocks), len(longs)
+        self.n_short, self.n_chosen, self.n_blocks, self.n_long = len(short), len(picks), len(blocks), len(longs)
         # (rows, a bound of their positions or 0) of the requests whose pages are written out
         self.long_rows = [(n, 0 if starts is None else int(starts[i]) + n) for i, _, n in longs]
-        flat = torch.tensor([v for rows in (short, blocks, longs) for r in rows for v in r] + [end for _, end in self.long_rows] or [0], dtype=torch.int32)
+        flat = torch.tensor([v for rows in (short, picks, blocks, longs) for r in rows for v in r] + [end for _, end in self.long_rows] or [0], dtype=torch.int32)
         device = torch.device(device)
         flat = flat.pin_memory().to(device, non_blocking=True) if device.type == "cuda" else flat
-        a, b = 3 * len(short), 3 * (len(short) + len(blocks))
-        c = b + 3 * len(longs)
-        self.short, self.blocks, self.longs, self.ends = flat[:a], flat[a:b], flat[b:c], flat[c:c + len(longs)]
+        ends = np.cumsum([3 * len(short), 3 * len(picks), 3 * len(blocks), 3 * len(longs), len(longs)]).tolist()
+        self.short, self.chosen, self.blocks, self.longs, self.ends = (flat[a:b] for a, b in zip([0] + ends, ends))
+        self.upto_chosen = flat[:ends[1]]                      # the short blocks and the chosen ones behind them
         self._rooms = {}
 
     def rooms(self, max_position: int, window: int = 0) -> Tuple[Tuple[int, ...], int]:
@@ -1048,10 +1050,11 @@ class PackedPlan:
         return hit
 
 
-def packed_plan(lens, nh: int, nkv: int, hd: int, dtype: torch.dtype, page_size: int, device, row_start=None, starts=None) -> PackedPlan:
+def packed_plan(lens, nh: int, nkv: int, hd: int, dtype: torch.dtype, page_size: int, device, row_start=None, starts=None, chosen=None) -> PackedPlan:
     """The plan of `packed_attention` for a step whose request i brings lens[i] rows, from row row_start[i] on (default: one behind the other; together they are the
     step's rows, each once), at consecutive positions.  `starts`: the positions of their first rows, where the host knows them (less room is made then).  Rows go in blocks of as many (row, query head) pairs as the packed kernel has
-    columns; requests of more than PACKED_LONG_STREAMS kv heads of such blocks (bfloat16) have their pages written out in half precision and run the prompt attention."""
+    columns; requests of more than PACKED_LONG_STREAMS kv heads of such blocks (bfloat16) have their pages written out in half precision and run the prompt attention.
+    `chosen`: for every request whether its one row reads chosen pages (`packed_select` with the plan lists them, `pages` of `packed_attention` takes them) or all."""
     lens = [int(n) for n in lens]
     if any(n < 0 for n in lens) or nh <= 0 or nkv <= 0 or nh % nkv:
         raise KernelError(f"packed_plan: rows {lens}, {nh} query heads for {nkv} kv heads")
@@ -1067,7 +1070,10 @@ def packed_plan(lens, nh: int, nkv: int, hd: int, dtype: torch.dtype, page_size:
         if first != at:
             raise KernelError(f"packed_plan: first rows {row_start} of requests of {lens} rows: every row from nought on belongs to one request")
         at += n
-    return PackedPlan(lens, [int(r) for r in row_start], nh, nkv, hd, dtype, page_size, device, starts)
+    chosen = [False] * len(lens) if chosen is None else [bool(c) for c in chosen]
+    if len(chosen) != len(lens) or any(c and n != 1 for c, n in zip(chosen, lens)):
+        raise KernelError(f"packed_plan: pages are chosen for requests of one row, of {lens} for {chosen}")
+    return PackedPlan(lens, [int(r) for r in row_start], nh, nkv, hd, dtype, page_size, device, starts, chosen)
 
 
 def packed_ctas(streams: int, blocks: int, positions: int, at_once: int, beside: int = 2) -> Tuple[int, int]:
@@ -1097,7 +1103,8 @@ def packed_attention(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Ten
     """Grouped-query attention of rows q [T, nh*hd] over pages in 4 bits; out [T, nh*hd].  Without a plan row i is the one row of request i; with one
     (`packed_plan`) the requests bring what it was made for.  `max_position` bounds the rows' positions.  `window` w > 0: a query sees itself and the w - 1
     positions before it.  `softcap`, `sink` and `sink_weight` as `attention` has them.  `pages` int32 [T, nkv, n] (single tokens): the pages, by their index in
-    the row's block table, that a row reads for a kv head, each once, -1 behind them (`packed_select` makes such lists)."""
+    the row's block table, that a row reads for a kv head, each once, -1 behind them (`packed_select` makes such lists); with a plan, [plan.n_chosen, nkv, n] for the
+    rows that it has as chosen, which read all their pages without."""
     _here("packed_attention", q, pool, block_table, positions, out, status, sink_weight, pages, None if plan is None else plan.short)
     block = _packed_pool("packed_attention", pool, hd, page_size, nkv)
     T = q.shape[0]
@@ -1118,12 +1125,11 @@ def packed_attention(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Ten
         raise KernelError("packed_attention: the plan is for other sizes")
     if plan is None and block_table.shape[0] < T:
         raise KernelError(f"packed_attention: {T} rows without a plan need a block table each, there are {block_table.shape[0]}")
-    top = 0
     if pages is not None:
         _i32(pages, "packed_attention: pages")
-        if plan is not None or window or pages.dim() != 3 or tuple(pages.shape[:2]) != (T, nkv) or pages.shape[2] < 1:
-            raise KernelError(f"packed_attention: pages [{T}, {nkv}, n] for single tokens without a window")
-        top = pages.shape[2]
+        n = T if plan is None else plan.n_chosen
+        if (plan is not None and not n) or window or pages.dim() != 3 or tuple(pages.shape[:2]) != (n, nkv) or pages.shape[2] < 1:
+            raise KernelError(f"packed_attention: pages [{n}, {nkv}, n] for single tokens without a window")
     if T == 0:
         return
     L, f32 = lib(), q.dtype == torch.float32
@@ -1145,8 +1151,17 @@ def packed_attention(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Ten
                                           plan.n_blocks, _p(written), marks, _p(out), out.stride(0), nh, nkv, hd, window, float(scale), end - 1,
                                           1 if sink else 0, _p(sink_weight), float(softcap), _p(status), _stream()), "attention_tcgen05")
             count_launches(1)
-        n, most = (T, 1) if plan is None else (plan.n_short, plan.most)
-        if n:
+        # (blocks of rows, how many, the most rows of one, their lists)
+        if plan is None:
+            runs = ((None, T, 1, pages),)
+        elif pages is None:
+            runs = ((plan.upto_chosen, plan.n_short + plan.n_chosen, plan.most, None),)
+        else:
+            runs = ((plan.short, plan.n_short, plan.most, None), (plan.chosen, plan.n_chosen, 1, pages))
+        for blocks, n, most, lists in runs:
+            if not n:
+                continue
+            top = 0 if lists is None else lists.shape[2]
             cols, each = _packed_columns(nh // nkv, f32, most)
             beside = 2 if cols == 8 and not f32 else 1           # (what their registers and shared memory allow)
             streams = nkv * -(-(nh // nkv) // each)
@@ -1158,7 +1173,7 @@ def packed_attention(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Ten
                 scratch = torch.empty((results * (hd + 2) + 2 * n * streams,), dtype=torch.float32, device=q.device)
                 part_o = scratch.data_ptr()
                 part_ml = part_o + 4 * hd * results
-            fields = _PACKED_ATTENTION.pack(_at(q), _at(pool), _at(block_table), _at(positions), 0 if plan is None else _at(plan.short), _at(pages), part_o, part_ml,
+            fields = _PACKED_ATTENTION.pack(_at(q), _at(pool), _at(block_table), _at(positions), _at(blocks), _at(lists), part_o, part_ml,
                                             _at(out), _at(sink_weight), _at(status), q.stride(0), block, out.stride(0), _dt(q), pool.shape[0], page_size,
                                             block_table.shape[1], block_table.shape[0], n, most, top, ctas, cluster, nh, nkv, hd, window, 1 if sink else 0, 0, scale, softcap)
             _check(L.bg_packed_attention(fields, _stream()), "packed_attention")
@@ -1166,30 +1181,33 @@ def packed_attention(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Ten
 
 
 def packed_select(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor, positions: torch.Tensor, nh: int, nkv: int, hd: int, page_size: int,
-                  max_position: int, out: torch.Tensor, status: Optional[torch.Tensor], first: int = 1, recent: int = 1) -> None:
+                  max_position: int, out: torch.Tensor, status: Optional[torch.Tensor], first: int = 1, recent: int = 1, plan: Optional[PackedPlan] = None) -> None:
     """out int32 [T, nkv, n]: the n pages (by their index in the block table, ascending, -1 behind them) that row i, the one row of request i, reads for each kv
-    head.  All where a request has no more than n; else the `first` first ones, the `recent` last ones (the newest among them) and those of the others whose keys
+    head; with a plan, [plan.n_chosen, nkv, n] for the rows that it has as chosen.  All where a request has no more than n; else the `first` first ones, the `recent` last ones (the newest among them) and those of the others whose keys
     can score highest, by their bounds (`packed_bounds`): the score of a page is the largest, over the query heads of the kv head, of
     sum of max(q lo, q hi), summed in 64 bits and rounded to 32 (one that is no number is the largest); of equal ones the lower page."""
-    _here("packed_select", q, pool, block_table, positions, out, status)
+    _here("packed_select", q, pool, block_table, positions, out, status, None if plan is None else plan.short)
     block = _packed_pool("packed_select", pool, hd, page_size, nkv, bounds=True)
     T = q.shape[0]
     _packed_rows_of("packed_select", positions, block_table, T)
     _i32(out, "packed_select: out")
     if q.dim() != 2 or q.stride(1) != 1 or q.shape[1] < nh * hd or nkv <= 0 or nh % nkv:
         raise KernelError("packed_select: q is [T, nh*hd] with unit inner stride, whole groups of query heads to a kv head")
-    if block_table.shape[0] < T or out.dim() != 3 or tuple(out.shape[:2]) != (T, nkv) or out.shape[2] < 1:
-        raise KernelError(f"packed_select: out [{T}, {nkv}, n], a block table for every row")
+    if plan is not None and (plan.sizes != (nh, nkv, hd, q.dtype, page_size) or plan.n_rows != T):
+        raise KernelError("packed_select: the plan is for other sizes")
+    n = T if plan is None else plan.n_chosen
+    if (plan is None and block_table.shape[0] < T) or out.dim() != 3 or tuple(out.shape[:2]) != (n, nkv) or out.shape[2] < 1:
+        raise KernelError(f"packed_select: out [{n}, {nkv}, n], a block table for every row")
     if first < 0 or recent < 1 or first + recent > out.shape[2]:
         raise KernelError(f"packed_select: {first} first and {recent} last pages (the newest at least) of {out.shape[2]}")
     n_pages = max_position // page_size + 1
     if n_pages > lib().bg_packed_select_most():
         raise KernelError(f"packed_select: {n_pages} pages, at most {lib().bg_packed_select_most()}")
-    if T == 0:
+    if n == 0:
         return
     with phase("attn"):
-        fields = _PACKED_SELECT.pack(_at(q), q.stride(0), _at(pool), block, _at(block_table), _at(positions), _at(out), _at(status), _dt(q), pool.shape[0], page_size,
-                                     block_table.shape[1], T, nh, nkv, hd, out.shape[2], first, recent, max(1, n_pages))
+        fields = _PACKED_SELECT.pack(_at(q), q.stride(0), _at(pool), block, _at(block_table), _at(positions), 0 if plan is None else _at(plan.chosen), _at(out), _at(status),
+                                     _dt(q), pool.shape[0], page_size, block_table.shape[1], block_table.shape[0], n, nh, nkv, hd, out.shape[2], first, recent, max(1, n_pages), 0)
         _check(lib().bg_packed_select(fields, _stream()), "packed_select")
 
 

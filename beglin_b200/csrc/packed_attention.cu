@@ -40,7 +40,7 @@ struct PaCall {
     const void* q; const unsigned char* pool;
     const int* table; const int* positions;
     const int* blocks;                 // [n][3]: request, first row, rows; null: block i is row i of request i
-    const int* list;                   // [rows][nkv][top] page indexes to read (less than 0: none), or null: all
+    const int* list;                   // [blocks][nkv][top] page indexes to read (less than 0: none), or null: all
     float* part_o; float* part_ml;     // (with ctas) [CTA][2][column][HD], [..][2]: what a CTA has of a stream that it shares with others
     void* out; const float* sink_w; unsigned* status;
     long long q_stride, block_bytes, out_stride;
@@ -221,7 +221,7 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 && !F32 ? 2 : 1) packed_at
     int row0 = block, rows = 1;
     if (p.blocks) { req = p.blocks[3 * block]; row0 = p.blocks[3 * block + 1]; rows = p.blocks[3 * block + 2]; }
     pos_last = p.positions[row0 + rows - 1];
-    list = p.list ? p.list + ((size_t)row0 * p.nkv + hy / p.head_blocks) * p.top : nullptr;
+    list = p.list ? p.list + ((size_t)block * p.nkv + hy / p.head_blocks) * p.top : nullptr;
     const PaChunks all = pa_chunks(p, KEYS, row0, rows);
     chunk0 = all.first; begin = u0 * PA_WARPS + warp; end = min(all.count, u1 * PA_WARPS);
     turns = begin < end ? (end - begin + PA_WARPS - 1) / PA_WARPS : 0;

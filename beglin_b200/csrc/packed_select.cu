@@ -30,9 +30,11 @@ struct PsParams {
     const void* q; long long q_stride;
     const unsigned char* pool; long long block_bytes;
     const int* table; const int* positions;
+    const int* blocks;                 // [T][3]: request, row (, 1); null: i and i
     int* out; unsigned* status;
-    int dtype, num_pages, page_size, max_pages, T, nh, nkv, hd, top, first, recent;
+    int dtype, num_pages, page_size, max_pages, n_req, T, nh, nkv, hd, top, first, recent;
     int pages_most;                    // bounds the pages of every row
+    int pad;
 };
 
 // Ordered as the scores are, as a whole number; both noughts are one.
@@ -110,12 +112,13 @@ __global__ void __launch_bounds__(PS_THREADS, 2) packed_select_kernel(const PsPa
     __shared__ float far_of[PS_CLUSTER], cut[2], scratch[32];
     __shared__ int unsure[PS_THREADS], n_unsure;
     pdl_launch();
-    const int row = blockIdx.x, kvh = blockIdx.y, rank = blockIdx.z, ranks = gridDim.z, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int item = blockIdx.x, kvh = blockIdx.y, rank = blockIdx.z, ranks = gridDim.z, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     pdl_wait();
+    const int req = p.blocks ? p.blocks[3 * item] : item, row = p.blocks ? p.blocks[3 * item + 1] : item;
     const int pos = p.positions[row], pages = pos < 0 ? 0 : min(pos / p.page_size + 1, p.pages_most);
     const int group = p.nh / p.nkv;
     const long long bounds_at = (long long)(p.page_size / PK_TILE) * Packed<HD>::TILE;
-    int* out = p.out + ((size_t)row * p.nkv + kvh) * p.top;
+    int* out = p.out + ((size_t)item * p.nkv + kvh) * p.top;
     if (pages <= p.top) {                              // (every CTA of the cluster: nobody waits for another)
         if (rank == 0)
             for (int i = tid; i < p.top; i += PS_THREADS) out[i] = i < pages ? i : -1;
@@ -129,7 +132,7 @@ __global__ void __launch_bounds__(PS_THREADS, 2) packed_select_kernel(const PsPa
     const TQ* q = reinterpret_cast<const TQ*>(p.q) + (size_t)row * p.q_stride + (size_t)kvh * group * HD;
     // the bounds of a page, or null where the table names none
     auto bounds_of = [&](int index) -> const unsigned char* {
-        const int page = index < p.max_pages ? p.table[(size_t)row * p.max_pages + index] : -1;
+        const int page = index < p.max_pages && req >= 0 && req < p.n_req ? p.table[(size_t)req * p.max_pages + index] : -1;
         return page >= 0 && page < p.num_pages ? p.pool + ((size_t)page * p.nkv + kvh) * p.block_bytes + bounds_at : nullptr;
     };
 
@@ -343,7 +346,7 @@ extern "C" int bg_packed_select_most() { return PS_MOST; }
 
 extern "C" int bg_packed_select_bytes() { return (int)sizeof(PsParams); }
 
-// out[row][kv head][top]: the pages that row `row` (of request `row`) reads, ascending, -1 behind them.
+// out[i][kv head][top]: the pages that the i-th row of `blocks` (or row i, of request i) reads, ascending, -1 behind them.
 extern "C" int bg_packed_select(const void* call, cudaStream_t stream) {
     const PsParams& p = *(const PsParams*)call;
     if (p.hd != 64 && p.hd != 128) return BG_ERR_UNSUPPORTED;

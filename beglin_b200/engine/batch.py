@@ -18,10 +18,12 @@ from ..csrc import ops
 @dataclass
 class Entry:
     """A request's part of a step: its next tokens and the places among them whose logits are
-    wanted."""
+    wanted.  `prompt`: they are a portion of its prompt (several tokens are in any case): a single token that is not may
+    read chosen pages alone."""
     rid: Hashable
     tokens: Sequence[int]
     want: Sequence[int] = ()
+    prompt: bool = False
 
     def ids(self) -> np.ndarray:
         """The tokens as an int64 array, converted once."""
@@ -78,6 +80,7 @@ class StepBatch:
         self.n_rows = n_rows
         self.max_position = max((s + n - 1 for s, n in zip(self.starts, self.lens) if n > 0), default=0)
         self.decode_only = all(n == 1 for n in self.lens)      # every request brings a single token
+        self.decoding = [n == 1 and not e.prompt for e, n in zip(self.entries, self.lens)]         # ... that is not the rest of its prompt
         self.n_logit_rows = len(rows)
         arrays = {"token_ids": cat(ids_parts), "positions": cat(pos_parts), "row_req": cat(req_parts)}
         if rows:
@@ -108,11 +111,12 @@ class StepBatch:
             self.scratch[key] = plan if plan.shares else None
         return self.scratch[key]
 
-    def packed_plan(self, nh: int, nkv: int, hd: int, dtype, page_size: int):
-        """The plan of `ops.packed_attention` for this step's rows."""
-        key = ("packed", nh, nkv, hd, dtype, page_size)
+    def packed_plan(self, nh: int, nkv: int, hd: int, dtype, page_size: int, choose: bool = False):
+        """The plan of `ops.packed_attention` for this step's rows; with `choose` the requests that decode read chosen pages."""
+        key = ("packed", nh, nkv, hd, dtype, page_size, choose)
         if key not in self._qblk:
-            self._qblk[key] = ops.packed_plan(self.lens, nh, nkv, hd, dtype, page_size, self.device, row_start=self.row_start, starts=self.starts)
+            self._qblk[key] = ops.packed_plan(self.lens, nh, nkv, hd, dtype, page_size, self.device, row_start=self.row_start, starts=self.starts,
+                                              chosen=self.decoding if choose else None)
         return self._qblk[key]
 
     def long_blocks(self, bq: int, min_rows: int):

@@ -61,6 +61,7 @@ class _StaticBatch:
         self.entries = []
         self.n_logit_rows = n
         self.decode_only = True
+        self.decoding = [True] * n
         self.implicit_blocks = True
         self.max_position = cache.max_context - 1
         i32 = dict(dtype=torch.int32, device=device)

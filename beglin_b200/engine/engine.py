@@ -62,8 +62,10 @@ class Engine:
         tokens whose shape comes again are replayed as CUDA graphs.
 
         `cache_bits` 4: the layers of plain grouped-query attention with heads of 64 or 128 features hold their keys and values in 4 bits (4.5 with what
-        goes with a group of 64 features), the others in the compute type; a model without such a layer is refused.  `sparse_pages` n: a single token
-        reads, in such a layer without a window and for each kv head, at most n pages of its request: the first, the last two and those whose keys can score highest."""
+        goes with a group of 64 features), the others in the compute type; a model without such a layer is refused.  `sparse_pages` n: a token that is
+        decoded reads, in such a layer without a window and for each kv head, at most n pages of its request: the first, the last two and those whose keys can score
+        highest.  Tokens of a prompt read all of it, however it is cut into portions and whoever shares their step (so does what is computed again after a
+        preemption); a single token given to `step` is one that is decoded, unless its `Entry` says `prompt`."""
         self.device = require_gpu(device)
         self.dtype = parse_dtype(dtype)
         self.spec, self.config = spec, config
@@ -186,7 +188,7 @@ class Engine:
         if isinstance(e, Entry):
             return e
         if isinstance(e, dict):
-            return Entry(e["id"], list(e["tokens"]), list(e.get("want", ())))
+            return Entry(e["id"], list(e["tokens"]), list(e.get("want", ())), bool(e.get("prompt", False)))
         rid, tokens, *rest = e
         return Entry(rid, list(tokens), list(rest[0]) if rest else [])
 

@@ -37,6 +37,7 @@ class _StaticPortion:
         self.row_start, self.lens = [0], [rows]
         self.starts = None                     # differs between replays: nothing on the host may depend on it
         self.decode_only = False
+        self.decoding = [False]
         self.implicit_blocks = False
         self.n_logit_rows = wanted
         self.max_position = bound
@@ -72,7 +73,7 @@ class _StaticPortion:
         return hit
 
 
-    def packed_plan(self, nh: int, nkv: int, hd: int, dtype, page_size: int):
+    def packed_plan(self, nh: int, nkv: int, hd: int, dtype, page_size: int, choose: bool = False):
         key = ("packed", nh, nkv, hd, dtype, page_size)
         if key not in self._qblk:              # (made by the warm-up: it stays for the capture)
             self._qblk[key] = ops.packed_plan(self.lens, nh, nkv, hd, dtype, page_size, self.device)
@@ -175,6 +176,8 @@ class PortionGraphs:
             return None
         rows, wanted = len(ents[0].tokens), len(ents[0].want)
         if rows < self.min_rows or wanted > self.max_wanted:
+            return None
+        if rows == 1 and self.engine.ctx.sparse_pages:         # (a single token may read chosen pages, which a portion does not)
             return None
         limit = self.engine.cache.max_context - 1
         bound = min(limit, -(-(starts[0] + rows) // self.BOUND_STEP) * self.BOUND_STEP - 1)

@@ -236,7 +236,7 @@ class Scheduler:
             entries = [Entry(r.rid, [r.output[-1]], [0]) for r in decode]
             for r, take, last in prefill:
                 toks = r.tokens_in[r.done_prompt:r.done_prompt + take]
-                entries.append(Entry(r.rid, toks, [take - 1] if last else []))
+                entries.append(Entry(r.rid, toks, [take - 1] if last else [], prompt=True))
             lengths = plan
             c = self.counters
             c.steps += 1

@@ -207,10 +207,15 @@ class GQAAttention:
 
     def _packed_attention(self, q, out, batch, cache: PagedKVView) -> None:
         sizes, pages = (self.nh, self.nkv, self.hd), None
-        plan = None if batch.decode_only else batch.packed_plan(*sizes, self.ctx.compute_dtype, cache.page_size)
-        if plan is None and 0 < self.sparse_pages <= batch.max_position // cache.page_size:
-            pages = torch.empty((q.shape[0], self.nkv, self.sparse_pages), dtype=torch.int32, device=q.device)
-            ops.packed_select(q, cache.pool, cache.block_table, batch.positions, *sizes, cache.page_size, batch.max_position, pages, self.ctx.status, first=1, recent=2)
+        choose = 0 < self.sparse_pages <= batch.max_position // cache.page_size and any(batch.decoding)
+        plan = None
+        if not batch.decode_only or (choose and not all(batch.decoding)):
+            plan = batch.packed_plan(*sizes, self.ctx.compute_dtype, cache.page_size, choose)
+        if choose:
+            n = q.shape[0] if plan is None else plan.n_chosen
+            pages = torch.empty((n, self.nkv, self.sparse_pages), dtype=torch.int32, device=q.device)
+            ops.packed_select(q, cache.pool, cache.block_table, batch.positions, *sizes, cache.page_size, batch.max_position, pages, self.ctx.status, first=1, recent=2,
+                              plan=plan)
         ops.packed_attention(q, cache.pool, cache.block_table, batch.positions, *sizes, cache.page_size, batch.max_position, self.scale, out, self.ctx.status, plan=plan,
                              window=self.window, softcap=self.score_cap, sink=bool(self.spec.sink), sink_weight=self.sink_weight, pages=pages)
 

@@ -187,3 +187,61 @@ def test_rows_beyond_their_bounds_are_recorded(starts, most, window, monkeypatch
                          plan=ops.packed_plan([100, 100], nh, nkv, hd, BF16, page, "cuda", starts=starts))
     with pytest.raises(ops.KernelError, match="block-table"):
         ops.raise_on_status(status)
+
+
+# ------------------------------------------------------------------------------------------------ rows over chosen pages beside others
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_a_plan_has_rows_over_chosen_pages(dtype):
+    plan = ops.packed_plan([1, 70, 1, 3, 1], 12, 2, 128, dtype, 64, "cpu", chosen=[True, False, False, False, True])
+    assert plan.n_chosen == 2 and plan.chosen.tolist() == [0, 0, 1, 4, 75, 1]
+    assert plan.upto_chosen.tolist() == plan.short.tolist() + plan.chosen.tolist() and [2, 71, 1] in plan.short.view(-1, 3).tolist()
+    assert sum(plan.short.view(-1, 3)[:, 2].tolist()) + 2 + sum(plan.blocks.view(-1, 3)[:, 2].tolist()) == 76
+    for wrong in ([True], [False, True, False, False, False], [False] * 6):
+        with pytest.raises(ops.KernelError, match="one row"):
+            ops.packed_plan([1, 70, 1, 3, 1], 12, 2, 128, dtype, 64, "cpu", chosen=wrong)
+    with pytest.raises(ops.KernelError, match="one row"):
+        ops.packed_plan([0], 12, 2, 128, dtype, 64, "cpu", chosen=[True])
+
+
+@GPU
+@pytest.mark.parametrize("nh,nkv,hd,page,dtype", [(12, 2, 128, 64, BF16), (14, 2, 64, 16, BF16), (40, 2, 64, 16, BF16), (6, 2, 128, 32, F32)])
+@pytest.mark.parametrize("many", [0, 1 << 30], ids=["written out", "packed"])
+def test_chosen_pages_beside_portions(nh, nkv, hd, page, dtype, many, monkeypatch):
+    """Single tokens over chosen pages, one over all of its pages, a long and a short portion, the requests' rows in another order than the requests."""
+    monkeypatch.setattr(ops, "PACKED_LONG_STREAMS", many)
+    lens, row_start = [1, 70, 1, 3, 1, 1], [72, 0, 70, 73, 71, 76]
+    lengths = [30 * page - 5, 200, 12 * page, 9, 50 * page + 1, page + 3]
+    pick, top = [True, False, True, False, True, False], 7
+    table, count = make_table(lengths, page)
+    pool = make_pool(count, nkv, hd, page, bounds=True, seed=4)
+    ends = torch.randn((count, nkv, 2, hd), generator=torch.Generator().manual_seed(3)).sort(2).values.to(BF16)
+    pool[:, :, tiles_bytes(hd, page):] = ends.flatten(2).view(torch.uint8)
+    poison(pool, table, lengths, hd, page)
+    rows = [None] * 77
+    for i, (n, r0, length) in enumerate(zip(lens, row_start, lengths)):
+        rows[r0:r0 + n] = [(i, p) for p in range(length - n, length)]
+    q = torch.randn((77, nh * hd), generator=torch.Generator().manual_seed(7)).to(dtype)
+    positions, status = torch.tensor([p for _, p in rows], dtype=torch.int32).cuda(), ops.new_status("cuda")
+    plan = ops.packed_plan(lens, nh, nkv, hd, dtype, page, "cuda", row_start=row_start, starts=[n - k for n, k in zip(lengths, lens)], chosen=pick)
+    pages, out = torch.full((3, nkv, top), 99, dtype=torch.int32, device="cuda"), torch.empty((77, nh * hd), dtype=dtype, device="cuda")
+    call = (q.cuda(), pool.cuda(), table.cuda(), positions, nh, nkv, hd, page, max(lengths) - 1)
+    ops.packed_select(*call, pages, status, first=1, recent=2, plan=plan)
+    mine = [i for i, p in enumerate(pick) if p]
+    at = [row_start[i] for i in mine]
+    assert torch.equal(pages.cpu(), chosen(q[at], pool, table[mine], [lengths[i] for i in mine], nh, nkv, hd, page, top, 1, 2))
+    every = torch.arange(table.shape[1], dtype=torch.int32)[None, None].expand(77, nkv, -1)
+    for given in (pages, None):
+        which = every.clone()
+        if given is not None:
+            which[at] = -1
+            which[at, :, :top] = pages.cpu()
+        out.fill_(7.0)
+        ops.packed_attention(*call, 0.1, out, status, plan=plan, pages=given)
+        near(out.view(77, nh, hd), plain_attention(q.view(77, nh, hd), pool, table, hd, page, rows, 0.1, pages=which), dtype)
+    ops.raise_on_status(status)
+    for wrong in (dict(pages=pages[:2]), dict(pages=pages, window=9), dict(pages=pages, plan=ops.packed_plan([77], nh, nkv, hd, dtype, page, "cuda"))):
+        with pytest.raises(ops.KernelError):
+            ops.packed_attention(*call, 0.1, out, status, **{"plan": plan, **wrong})
+    for wrong in (dict(plan=ops.packed_plan([77], nh, nkv, hd, dtype, page, "cuda")), dict(plan=ops.packed_plan([1] * 3, nh, nkv, hd, dtype, page, "cuda", chosen=[True] * 3))):
+        with pytest.raises(ops.KernelError):
+            ops.packed_select(*call, pages, status, first=1, recent=2, **wrong)
