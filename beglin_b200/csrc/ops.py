@@ -1180,6 +1180,11 @@ def packed_attention(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Ten
             count_launches(1 if ctas else 0)
 
 
+def packed_select_most() -> int:
+    """Of how many pages `packed_select` can choose at most."""
+    return lib().bg_packed_select_most()
+
+
 def packed_select(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor, positions: torch.Tensor, nh: int, nkv: int, hd: int, page_size: int,
                   max_position: int, out: torch.Tensor, status: Optional[torch.Tensor], first: int = 1, recent: int = 1, plan: Optional[PackedPlan] = None) -> None:
     """out int32 [T, nkv, n]: the n pages (by their index in the block table, ascending, -1 behind them) that row i, the one row of request i, reads for each kv
@@ -1201,8 +1206,8 @@ def packed_select(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor
     if first < 0 or recent < 1 or first + recent > out.shape[2]:
         raise KernelError(f"packed_select: {first} first and {recent} last pages (the newest at least) of {out.shape[2]}")
     n_pages = max_position // page_size + 1
-    if n_pages > lib().bg_packed_select_most():
-        raise KernelError(f"packed_select: {n_pages} pages, at most {lib().bg_packed_select_most()}")
+    if n_pages > packed_select_most():
+        raise KernelError(f"packed_select: {n_pages} pages, at most {packed_select_most()}")
     if n == 0:
         return
     with phase("attn"):

@@ -51,6 +51,18 @@ def require_gpu(device) -> torch.device:
     return device
 
 
+def check_packed(needs, ctx: BuildContext, max_context: int) -> None:
+    """Whether the layers' cache needs go with what the build asks for of a cache in 4 bits."""
+    packed = [n for need in needs for n in (need.needs if isinstance(need, CompositeNeed) else (need,)) if isinstance(n, PagedPackedNeed)]
+    if ctx.cache_bits == 4 and not packed:
+        raise ValueError("cache_bits=4: no layer of this model holds keys and values that way (plain grouped-query attention, heads of 64 or 128 features, "
+                         f"pages of a multiple of {ops.PACKED_TILE} positions)")
+    pages = -(-max_context // ctx.page_size)
+    if any(n.bounds for n in packed) and ctx.sparse_pages < pages and pages > ops.packed_select_most():
+        raise ValueError(f"sparse_pages={ctx.sparse_pages}: requests of up to {max_context} positions have {pages} pages of {ctx.page_size}, pages can be chosen of at most "
+                         f"{ops.packed_select_most()}")
+
+
 class Engine:
     def __init__(self, spec, tensors, *, dtype="bfloat16", device="cuda:0", max_tokens: int = 8192,
                  page_size: int = 64, max_requests: int = 8, max_context: Optional[int] = None,
@@ -80,9 +92,7 @@ class Engine:
             if spec.max_positions:
                 limit = min(limit, spec.max_positions)
             needs = self.model.cache_needs()
-            if cache_bits == 4 and not any(isinstance(n, PagedPackedNeed) for need in needs for n in (need.needs if isinstance(need, CompositeNeed) else (need,))):
-                raise ValueError("cache_bits=4: no layer of this model holds keys and values that way (plain grouped-query attention, heads of 64 or 128 features, "
-                                 f"pages of a multiple of {ops.PACKED_TILE} positions)")
+            check_packed(needs, self.ctx, limit)
             self.cache = CacheManager(needs, page_size, num_pages, max_requests, limit)
             self.cache.allocate(self.device, self.dtype)
         self.sampler = Sampler(self.device, self.ctx.status)

@@ -7,9 +7,12 @@ from helpers import make_model, rel_err, seeded_ids
 from test_packed_engine import GPU, WIDE, engine
 
 from beglin_b200.cache import CacheManager
+from beglin_b200.csrc import ops
 from beglin_b200.engine.batch import Entry, StepBatch
+from beglin_b200.engine.engine import check_packed
 from beglin_b200.engine.scheduler import Request, Scheduler
-from beglin_b200.parts.cache_need import PagedPackedNeed
+from beglin_b200.parts.cache_need import CompositeNeed, PagedPackedNeed
+from beglin_b200.parts.context import BuildContext
 
 
 def test_entries_say_whether_they_are_of_a_prompt():
@@ -72,3 +75,23 @@ def test_both_orders_of_prompts_give_the_same_tokens(model_root):
                 eng = engine(folder, "float32", sparse_pages=4, use_graphs=graphs)
                 made.append(eng.generate(prompts, max_new_tokens=24, temperature=1.0, seed=5, stop_ids=(), mixed=mixed, max_step_tokens=budget))
     assert all(m == made[0] for m in made)
+
+
+# ------------------------------------------------------------------------------------------------ more pages than can be chosen of
+def test_a_context_of_more_pages_than_can_be_chosen_of_is_refused():
+    most, ctx = ops.packed_select_most(), lambda **kw: BuildContext(torch.device("cpu"), torch.bfloat16, page_size=16, cache_bits=4, **kw)
+    bounded, plain = CompositeNeed((PagedPackedNeed(2, 64, None, True),)), PagedPackedNeed(2, 64)
+    check_packed([plain, bounded], ctx(sparse_pages=8), 16 * most)
+    check_packed([plain], ctx(sparse_pages=8), 16 * most + 1)                  # (a layer with a window has all of it read)
+    check_packed([bounded], ctx(sparse_pages=most + 1), 16 * most + 1)         # (never are pages chosen)
+    with pytest.raises(ValueError, match=f"sparse_pages=8.*{16 * most + 1}.*{most}"):
+        check_packed([plain, bounded], ctx(sparse_pages=8), 16 * most + 1)
+
+
+@GPU
+def test_an_engine_of_such_a_context_is_not_built(model_root):
+    folder = make_model(model_root, "packedFar", config=dict(WIDE, max_position_embeddings=1 << 20), std=0.05, bias_std=0.05)
+    with pytest.raises(ValueError, match="sparse_pages=6"):
+        engine(folder, "bfloat16", sparse_pages=6, max_context=16 * 36000 + 1)
+    eng = engine(folder, "bfloat16", sparse_pages=6, max_context=16 * 36000)
+    assert len(eng.generate([seeded_ids(200, 200, 1)], max_new_tokens=4, stop_ids=())[0]) == 4
