@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import math
 import struct
 from array import array
 from typing import Optional, Tuple
@@ -1115,7 +1116,7 @@ def packed_attention(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Ten
         raise KernelError(f"packed_attention: queries of {q.dtype} and results of {out.dtype}")
     if nkv <= 0 or nh % nkv:
         raise KernelError(f"packed_attention: {nh} query heads for {nkv} kv heads")
-    if window < 0 or not softcap >= 0.0 or not scale > 0.0:
+    if window < 0 or not 0.0 <= softcap < math.inf or not 0.0 < scale < math.inf:
         raise KernelError("packed_attention: a sliding window or none, a positive bound of the scores or none, a positive scale")
     if sink_weight is not None:
         sink = True

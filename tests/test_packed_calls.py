@@ -245,3 +245,14 @@ def test_chosen_pages_beside_portions(nh, nkv, hd, page, dtype, many, monkeypatc
     for wrong in (dict(plan=ops.packed_plan([77], nh, nkv, hd, dtype, page, "cuda")), dict(plan=ops.packed_plan([1] * 3, nh, nkv, hd, dtype, page, "cuda", chosen=[True] * 3))):
         with pytest.raises(ops.KernelError):
             ops.packed_select(*call, pages, status, first=1, recent=2, **wrong)
+
+
+# ------------------------------------------------------------------------------------------------ refusals
+@pytest.mark.parametrize("options", [dict(scale=math.inf), dict(scale=math.nan), dict(scale=0.0), dict(softcap=math.inf), dict(softcap=math.nan), dict(softcap=-1.0)], ids=str)
+def test_scales_and_bounds_of_scores_are_finite(options, monkeypatch):
+    monkeypatch.setattr(ops, "_here", lambda *a: None)                         # (nothing is launched)
+    hd, page = 64, 16
+    q, table, positions = torch.zeros((1, hd), dtype=BF16), torch.zeros((1, 1), dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    options = dict(options)
+    with pytest.raises(ops.KernelError, match="scale"):
+        ops.packed_attention(q, make_pool(2, 1, hd, page), table, positions, 1, 1, hd, page, 0, options.pop("scale", 1.0), torch.zeros_like(q), None, **options)
