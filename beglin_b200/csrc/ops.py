@@ -929,7 +929,8 @@ def packed_append(src: torch.Tensor, q_out: torch.Tensor, nh: int, nkv: int, hd:
                   status: Optional[torch.Tensor]) -> None:
     """Rows [q | k | v] of `src` ([T, W], or partial sums [parts, T, W]): rotate q into q_out [T, nh*hd], rotate k, and store k and v in 4 bits in the pages of
     `pool` uint8 [pages, nkv, packed_page_bytes] through the block table [requests, max_pages].  A group of 64 features x is held as lowest = bf16(min x),
-    step = bf16((max x - lowest) / 15) and codes clamp(round((x - lowest) / step), 0, 15), as 64 bits give them; one that holds what is not finite is not a
+    step = bf16((max x - lowest) / 15) and codes clamp(round((x - lowest) / step), 0, 15) (0 where the step is not positive), as 64 bits give them; a group whose range is
+    small beside its values loses by the rounding of lowest, 2^-8 of it; one that holds what is not finite is not a
     number throughout.  A (request, position) comes once a call."""
     _here("packed_append", src, q_out, cos_sin, positions, row_req, block_table, pool, status)
     parts, stride = _parts(src, "packed_append: src")
@@ -957,8 +958,8 @@ def packed_append(src: torch.Tensor, q_out: torch.Tensor, nh: int, nkv: int, hd:
 
 def packed_bounds(pool: torch.Tensor, positions: torch.Tensor, row_req: torch.Tensor, block_table: torch.Tensor, hd: int, page_size: int,
                   status: Optional[torch.Tensor]) -> None:
-    """For every row whose position is the last of its page: the smallest and largest value that the page holds of every feature of its keys, written behind
-    the page's codes.  Behind `packed_append` of the same rows; a page that is not full has no bounds."""
+    """For every row whose position is the last of its page: the smallest and largest value that the page holds of every feature of its keys, to the nearest
+    bfloat16 number, written behind the page's codes.  Behind `packed_append` of the same rows; a page that is not full has no bounds."""
     _here("packed_bounds", pool, positions, row_req, block_table, status)
     block = _packed_pool("packed_bounds", pool, hd, page_size, bounds=True)
     T = positions.numel()

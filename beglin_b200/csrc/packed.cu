@@ -2,9 +2,11 @@
 // the way, rows read back, the smallest and largest values of a filled page's keys, and pages written out in half precision for the
 // prompt attention.
 //
-// A group of 64 features x becomes  lowest = bf16(min x),  step = bf16((max x - lowest) / 15),  u = clamp(round((x - lowest) / step), 0, 15).  The pair is
-// rounded before the codes are made, so that they are the nearest ones to what is read back: a value is off by half a step, and where rounding the pair cut
-// the range (by a part in 512) by that.  x is the rotated key in float, never rounded to bfloat16.  A group with a value that is not finite, or whose range is
+// A group of 64 features x becomes  lowest = bf16(min x),  step = bf16((max x - lowest) / 15),  u = clamp(round((x - lowest) / step), 0, 15), nought where the step
+// is not positive.  The pair is rounded before the codes are made, so that they are the nearest ones to what is read back: a value is off by half a step, or by
+// as much as rounding moved the end of the range that it lies beyond, which is up to 2^-8 of lowest below and 2^-8 of 15 steps above.  So a group needs a range that is
+// not small beside its values: one of 100.30 .. 100.45 has lowest 100.5, a step below nought and every code 0, 0.2 off.  x is the rotated key in float, never
+// rounded to bfloat16.  A group with a value that is not finite, or whose range is
 // not, is not a number throughout, as attention over it would be.  No result hangs on which thread wrote first: a position has one writer.
 #include <cuda_fp16.h>
 
@@ -271,7 +273,7 @@ __global__ void __launch_bounds__(PK_THREADS) packed_rows_kernel(const PkRead p)
 
 // ------------------------------------------------------------------------------------------------ bounds of filled pages
 // A row that fills its page (its position is the page's last) has the CTA of its rows find the smallest and largest value of every feature of the page's keys, as
-// they are read back.  What a page's bounds are hangs on the page alone, whoever wrote it and in how many steps.  A CTA looks at PK_ROWS rows of one kv head; for
+// they are read back, rounded to the nearest bfloat16 number: a feature may lie beyond its bound by up to 2^-8 of itself.  What a page's bounds are hangs on the page alone, whoever wrote it and in how many steps.  A CTA looks at PK_ROWS rows of one kv head; for
 // one that fills its page a thread takes a word of 8 features of every (PK_THREADS / words)-th position; a value that is no number stays one.  (A CTA for every
 // row: 26 us for 4,917 rows, of CTAs that had nothing to do; a warp for every row: 19 us for the page that one row fills.)
 constexpr int PK_ROWS = 8;

@@ -10,7 +10,9 @@
 //     p V     = sum over positions of  (p step) u + p lowest
 //             = sum over positions of  r u - 8 r + p (lowest + 8 step),  r = p step rounded to bfloat16 (but for float queries),
 // so that the only rounding of the cache's side is that of r, and it counts for u - 8 alone: 4.6 in the root of the mean of squares, where u are 8.8 (results
-// 0.0021 of their norm off, with u alone 0.0029; rounding them to bfloat16 is 0.0017).  The sum of r is a product with -1; 2 us of 70.  Keys: 16 positions
+// 0.0021 of their norm off, with u alone 0.0029; rounding them to bfloat16 is 0.0017).  The sum of r is a product with -1; 2 us of 70.  Sums over a warp's whole range
+// of positions stay in the tensor cores' accumulators, 32 bits that are cut off rather than rounded (float queries take a tile's sums out: next to what r loses that
+// does not show, in float it does); 2^x and tanh are the approximate instructions, good to 22 bits, and float's own for float queries.  Keys: 16 positions
 // by 16 features times features by 8 columns; values: 16 features by 16 positions times positions by columns.  A column is one (row, query head): the
 // queries of a kv head are the narrow side, so 8 heads waste nothing of the product and a code is unpacked once for all of them.  The weights reach the
 // second product's layout through movmatrix.  Float queries and weights go in three bfloat16 parts.

@@ -1,6 +1,6 @@
 // Which pages of its request a decoding row reads, for each kv head: the `first` first and the `recent` last ones, and of those between them the ones whose keys
 // can score highest.  A page's score is the most that q . k can be for any key inside the page's bounds (packed.cu), for the best of the query heads that share
-// the kv head:
+// the kv head (the bounds are rounded to the nearest, so that a key may lie outside by up to 2^-8 of a feature: the score orders pages, it proves nothing):
 //     score = max over heads of  sum over features of  max(q lo, q hi)  =  sum of  max(q, 0) hi + min(q, 0) lo.
 //
 // The choice is that of sums in 64 bits, rounded to 32 once: of products of bfloat16 they are exact but for the last few bits of 64, so the order does not hang

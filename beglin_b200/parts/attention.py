@@ -16,7 +16,7 @@ product of the mixer's input, on the joined heads before the output product, fea
 one more block of rows of the one q/k/v product.  With any of the first two the kernel that norms, rotates and appends
 is `qk_norm_rope_append`.
 
-Where the build asks for a cache in 4 bits, the plain form's keys and values are held so (`ops.packed_append`, `ops.packed_attention`), and single tokens may
+Where the build asks for a cache in 4 bits, the plain form's keys and values are held so (`ops.packed_append`, `ops.packed_attention`), and tokens that are decoded may
 read the pages that can score highest alone (`ops.packed_select`).  (The reference has caches of 8 and of 4 bits, qwen_infer.c:810-1209.)
 
 A step of single tokens whose requests hold their first positions in the same pages (requests that go on from one text) reads those once for all of
@@ -107,7 +107,7 @@ class GQAAttention:
 
     @staticmethod
     def chooses(spec: AttentionSpec, ctx: BuildContext) -> bool:
-        """Whether single tokens read the pages that score highest alone (a window is short already)."""
+        """Whether tokens that are decoded read the pages that score highest alone (a window is short already)."""
         return ctx.sparse_pages > 0 and spec.window is None
 
     def __init__(self, spec: AttentionSpec, tensors: Dict[str, torch.Tensor], ctx: BuildContext):

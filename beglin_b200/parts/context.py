@@ -24,7 +24,7 @@ class BuildContext:
     # measured to pay; "all": wherever the sizes allow it (tests of the fused kernels on tiny models); False: nowhere
     fuse: object = True
     cache_bits: int = 16                    # 4: plain grouped-query layers hold keys and values in 4 bits (the others as they are)
-    sparse_pages: int = 0                   # pages that a single token reads for each kv head, where the cache is in 4 bits; 0: all
+    sparse_pages: int = 0                   # pages that a decoded token reads for each kv head, where the cache is in 4 bits; 0: all
     status: Optional[torch.Tensor] = None   # device word in which kernels record bad ids and pages
     reads_shared: bool = False              # whether a layer reads positions that requests share once for all of them
     shared: Dict[object, object] = field(default_factory=dict)   # parts shared between layers, by spec
