@@ -1045,6 +1045,8 @@ class PackedPlan:
         A page takes 4 * 64 * kv heads * head size bytes while the call lasts."""
         hit = self._rooms.get((max_position, window))
         if hit is None:
+            if len(self._rooms) == 64:
+                self._rooms.clear()
             most = max(max_position + 1, 1)
             ends = [min(end or most, most) for _, end in self.long_rows]
             hit = self._rooms[max_position, window] = (tuple(lib().bg_packed_room(n, end, window) for (n, _), end in zip(self.long_rows, ends)),
@@ -1054,8 +1056,8 @@ class PackedPlan:
 
 def packed_plan(lens, nh: int, nkv: int, hd: int, dtype: torch.dtype, page_size: int, device, row_start=None, starts=None, chosen=None) -> PackedPlan:
     """The plan of `packed_attention` for a step whose request i brings lens[i] rows, from row row_start[i] on (default: one behind the other; together they are the
-    step's rows, each once), at consecutive positions.  `starts`: the positions of their first rows, where the host knows them (less room is made then).  Rows go in blocks of as many (row, query head) pairs as the packed kernel has
-    columns; requests of more than PACKED_LONG_STREAMS kv heads of such blocks (bfloat16) have their pages written out in half precision and run the prompt attention.
+    step's rows, each once), at consecutive positions.  `starts`: the positions of their first rows, where the host knows them (less room is made then).  Rows go in
+    blocks of as many (row, query head) pairs as the packed kernel has columns; requests of more than PACKED_LONG_STREAMS kv heads of such blocks (bfloat16) have their pages written out in half precision and run the prompt attention.
     `chosen`: for every request whether its one row reads chosen pages (`packed_select` with the plan lists them, `pages` of `packed_attention` takes them) or all."""
     lens = [int(n) for n in lens]
     if any(n < 0 for n in lens) or nh <= 0 or nkv <= 0 or nh % nkv:
