@@ -929,9 +929,9 @@ def packed_append(src: torch.Tensor, q_out: torch.Tensor, nh: int, nkv: int, hd:
                   status: Optional[torch.Tensor]) -> None:
     """Rows [q | k | v] of `src` ([T, W], or partial sums [parts, T, W]): rotate q into q_out [T, nh*hd], rotate k, and store k and v in 4 bits in the pages of
     `pool` uint8 [pages, nkv, packed_page_bytes] through the block table [requests, max_pages].  A group of 64 features x is held as lowest = bf16(min x),
-    step = bf16((max x - lowest) / 15) and codes clamp(round((x - lowest) / step), 0, 15) (0 where the step is not positive), as 64 bits give them; a group whose range is
-    small beside its values loses by the rounding of lowest, 2^-8 of it; one that holds what is not finite is not a
-    number throughout.  A (request, position) comes once a call."""
+    step = bf16((max x - lowest) / 15) and codes clamp(round((x - lowest) / step), 0, 15) (0 where the step is not positive), as 64 bits give them; a group whose
+    range is small beside its values loses by the rounding of lowest, 2^-8 of it; one that holds what is not finite is not a number throughout.  A (request, position)
+    comes once a call."""
     _here("packed_append", src, q_out, cos_sin, positions, row_req, block_table, pool, status)
     parts, stride = _parts(src, "packed_append: src")
     T, width = src.shape[-2], src.shape[-1]
@@ -1057,8 +1057,9 @@ class PackedPlan:
 def packed_plan(lens, nh: int, nkv: int, hd: int, dtype: torch.dtype, page_size: int, device, row_start=None, starts=None, chosen=None) -> PackedPlan:
     """The plan of `packed_attention` for a step whose request i brings lens[i] rows, from row row_start[i] on (default: one behind the other; together they are the
     step's rows, each once), at consecutive positions.  `starts`: the positions of their first rows, where the host knows them (less room is made then).  Rows go in
-    blocks of as many (row, query head) pairs as the packed kernel has columns; requests of more than PACKED_LONG_STREAMS kv heads of such blocks (bfloat16) have their pages written out in half precision and run the prompt attention.
-    `chosen`: for every request whether its one row reads chosen pages (`packed_select` with the plan lists them, `pages` of `packed_attention` takes them) or all."""
+    blocks of as many (row, query head) pairs as the packed kernel has columns; requests of more than PACKED_LONG_STREAMS kv heads of such blocks
+    (bfloat16) have their pages written out in half precision and run the prompt attention.  `chosen`: for every request whether its one row reads chosen pages (`packed_select` with the plan
+    lists them, `pages` of `packed_attention` takes them) or all."""
     lens = [int(n) for n in lens]
     if any(n < 0 for n in lens) or nh <= 0 or nkv <= 0 or nh % nkv:
         raise KernelError(f"packed_plan: rows {lens}, {nh} query heads for {nkv} kv heads")
